@@ -549,6 +549,33 @@ int b200moe_quant_mxfp8_ex(const void* x, b200moe_dtype dtype, void* q, void* s,
                            int64_t rows, int cols, int terms, int block_sums,
                            int gated, b200moe_stream stream);
 
+/* Root-mean-square norm of rows, with the residual's addition ahead of it and 8-bit
+ * rows with dynamic scales behind it (no counterpart op of this form in the reference,
+ * which has the norm and the quantisation as separate steps):
+ *   s = T(input + residual), written back to `residual`   (s = input if it is NULL)
+ *   y = s / sqrt(mean(s^2) + eps) * weight                (fp32; weight NULL: 1)
+ *   out = T(y);  q = e4m3(y / scale), per group of a row
+ *   scale = max(amax|y| / 448, 1 / (448*512)), with scale_ue8m0 rounded up to a power
+ *   of two; NaN if the group holds a NaN or an infinity.
+ * `out` may be the input (same pointer and stride); no other buffers may overlap. */
+typedef struct {
+  const void* input;      /* [rows, hidden] dtype, row stride in elements            */
+  void* residual;         /* [rows, hidden] dtype, updated; or NULL                  */
+  const void* weight;     /* [hidden] weight_dtype, or NULL                          */
+  void* out;              /* [rows, hidden] dtype, or NULL                           */
+  void* q;                /* [rows, hidden] e4m3, or NULL (one of out, q is needed)  */
+  float* scales;          /* with q: element strides s_stride_row, s_stride_group    */
+  int64_t rows, input_stride, residual_stride, out_stride, q_stride;
+  int64_t s_stride_row, s_stride_group;
+  int hidden;
+  int group_size;         /* values per scale (divides hidden); 0: one scale a row   */
+  float eps;
+  int scale_ue8m0;
+  b200moe_dtype dtype;    /* F32, F16 or BF16                                        */
+  b200moe_dtype weight_dtype; /* dtype or F32                                        */
+} b200moe_rms_norm_args;
+int b200moe_add_rms_norm(const b200moe_rms_norm_args* args, b200moe_stream stream);
+
 /* Replaces `moe_gather` (csrc/moe/moe_gather.cpp:161-204; schema
  * csrc/moe/torch_bindings.cpp:78-82).
  * out[t,:] = sum_k w[t,k] * moe_out[row_map[t,k],:] (fp32), skipping -1. */

@@ -238,6 +238,119 @@ void silu_and_mul_quant(at::Tensor& out, at::Tensor& input, at::Tensor& scale) {
                                           scale.data_ptr<float>(), rows, (int)d, current_stream()));
 }
 
+// Rows [..., hidden] whose last dimension is dense and whose rows are evenly spaced: the row stride in elements.
+int64_t row_stride(const at::Tensor& t, const char* name) {
+  const int64_t hidden = t.size(-1);
+  if (t.numel() == 0) return hidden;
+  TORCH_CHECK(hidden == 1 || t.stride(-1) == 1, "b200_add_rms_norm: the last dimension of ", name, " must be contiguous");
+  if (t.dim() == 1) return hidden;
+  int64_t at = t.dim() - 2;
+  while (at > 0 && t.size(at) == 1) --at;       // (the stride of a single row says nothing)
+  const int64_t stride = t.size(at) == 1 ? hidden : t.stride(at);
+  int64_t next = stride * t.size(at);
+  for (int64_t d = at - 1; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    TORCH_CHECK(t.stride(d) == next, "b200_add_rms_norm: the rows of ", name, " must be evenly spaced");
+    next *= t.size(d);
+  }
+  return stride;
+}
+
+// Whether the memory that the rows of a and b span overlaps.
+bool rows_overlap(const at::Tensor& a, const at::Tensor& b) {
+  auto span = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    const char* p = (const char*)t.data_ptr();
+    return std::make_pair(p, p + (last + 1) * t.element_size());
+  };
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto x = span(a), y = span(b);
+  return x.first < y.second && y.first < x.second;
+}
+
+// residual += input, norm, weight; the result in the input's dtype (out) and as e4m3 rows with scales (out_q, scales).
+void b200_add_rms_norm(const at::Tensor& input, const std::optional<at::Tensor>& residual,
+                       const std::optional<at::Tensor>& weight, double epsilon, const std::optional<at::Tensor>& out,
+                       const std::optional<at::Tensor>& out_q, const std::optional<at::Tensor>& scales, int64_t group_size,
+                       bool scale_ue8m0) {
+  check_cuda(input, "input");
+  TORCH_CHECK(input.dim() >= 1, "b200_add_rms_norm: input must be [..., hidden_size]");
+  TORCH_CHECK(out.has_value() || out_q.has_value(), "b200_add_rms_norm: out or out_q is needed");
+  TORCH_CHECK(out_q.has_value() == scales.has_value(), "b200_add_rms_norm: out_q and scales go together");
+  const int64_t hidden = input.size(-1), rows = hidden ? input.numel() / hidden : 0;
+  TORCH_CHECK(hidden <= 0x7fffffff && rows <= 0x7fffffff, "b200_add_rms_norm: input is too large");
+  b200moe_rms_norm_args a = {};
+  a.dtype = float_dtype(input, "b200_add_rms_norm");
+  const std::pair<const std::optional<at::Tensor>*, const char*> others[] = {
+      {&residual, "residual"}, {&weight, "weight"}, {&out, "out"}, {&out_q, "out_q"}, {&scales, "scales"}};
+  for (const auto& [t, name] : others)
+    TORCH_CHECK(!t->has_value() || (*t)->device() == input.device(), "b200_add_rms_norm: ", name, " must be on the input's device");
+  for (const auto& [t, name] : {others[0], others[2], others[3]}) {
+    if (!t->has_value()) continue;
+    TORCH_CHECK((*t)->sizes() == input.sizes(), "b200_add_rms_norm: ", name, " must have the input's shape");
+    TORCH_CHECK((*t)->scalar_type() == (t == &out_q ? at::kFloat8_e4m3fn : input.scalar_type()), "b200_add_rms_norm: ", name,
+                t == &out_q ? " must be float8_e4m3fn" : " must have the input's dtype");
+  }
+  a.rows = rows;
+  a.hidden = (int)hidden;
+  a.eps = (float)epsilon;
+  a.input = input.data_ptr();
+  a.input_stride = row_stride(input, "input");
+  if (residual.has_value()) {
+    a.residual = residual->data_ptr();
+    a.residual_stride = row_stride(*residual, "residual");
+    TORCH_CHECK(rows <= 1 || a.residual_stride >= hidden, "b200_add_rms_norm: the rows of residual must not overlap");
+    TORCH_CHECK(!rows_overlap(input, *residual), "b200_add_rms_norm: residual must not overlap the input");
+  }
+  if (weight.has_value()) {
+    TORCH_CHECK(weight->dim() == 1 && weight->size(0) == hidden && weight->is_contiguous(),
+                "b200_add_rms_norm: weight must be contiguous [hidden_size]");
+    TORCH_CHECK(weight->scalar_type() == at::kFloat || weight->scalar_type() == input.scalar_type(),
+                "b200_add_rms_norm: weight must be float32 or have the input's dtype");
+    a.weight = weight->data_ptr();
+    a.weight_dtype = float_dtype(*weight, "b200_add_rms_norm");
+  }
+  if (out.has_value()) {
+    a.out = out->data_ptr();
+    a.out_stride = row_stride(*out, "out");
+    TORCH_CHECK(rows <= 1 || a.out_stride >= hidden, "b200_add_rms_norm: the rows of out must not overlap");
+    TORCH_CHECK(!rows_overlap(*out, input) || (a.out == a.input && (rows <= 1 || a.out_stride == a.input_stride)),
+                "b200_add_rms_norm: out must be the input or not overlap it");
+  }
+  if (out_q.has_value()) {
+    TORCH_CHECK(group_size >= 0 && (group_size == 0 || hidden % group_size == 0),
+                "b200_add_rms_norm: hidden_size must be divisible by group_size");
+    const int64_t groups = group_size ? hidden / group_size : 1;
+    TORCH_CHECK(scales->scalar_type() == at::kFloat && scales->dim() == 2 && scales->size(0) == rows &&
+                    (hidden == 0 || scales->size(1) == groups),
+                "b200_add_rms_norm: scales must be float32 [rows, hidden_size / group_size]");
+    TORCH_CHECK((rows <= 1 || scales->stride(0) != 0) && (groups <= 1 || scales->stride(1) != 0),
+                "b200_add_rms_norm: scales must not be expanded");
+    a.q = out_q->data_ptr();
+    a.q_stride = row_stride(*out_q, "out_q");
+    TORCH_CHECK(rows <= 1 || a.q_stride >= hidden, "b200_add_rms_norm: the rows of out_q must not overlap");
+    a.scales = scales->data_ptr<float>();
+    a.s_stride_row = scales->stride(0);
+    a.s_stride_group = scales->stride(1);
+    a.group_size = (int)group_size;
+    a.scale_ue8m0 = scale_ue8m0;
+  }
+  const at::Tensor* written[] = {residual.has_value() ? &*residual : nullptr, out.has_value() ? &*out : nullptr,
+                                 out_q.has_value() ? &*out_q : nullptr, scales.has_value() ? &*scales : nullptr};
+  for (int i = 0; i < 4; ++i) {
+    if (written[i] == nullptr) continue;
+    for (int j = 0; j < i; ++j)
+      TORCH_CHECK(written[j] == nullptr || !rows_overlap(*written[i], *written[j]),
+                  "b200_add_rms_norm: the tensors that are written must not overlap");
+    TORCH_CHECK(i == 1 || !rows_overlap(*written[i], input), "b200_add_rms_norm: only out may be the input");
+    TORCH_CHECK(!weight.has_value() || !rows_overlap(*written[i], *weight), "b200_add_rms_norm: weight must not be written");
+  }
+  if (rows == 0 || hidden == 0) return;
+  const c10::cuda::CUDAGuard guard(input.device());
+  check_status(b200moe_add_rms_norm(&a, current_stream()));
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(_C, m) {
@@ -265,6 +378,9 @@ TORCH_LIBRARY_FRAGMENT(_C, m) {
   m.def(
       "per_token_group_quant_mxfp4(Tensor input, Tensor! output_q, Tensor! "
       "output_s, int group_size, float eps) -> ()");
+  m.def(
+      "b200_add_rms_norm(Tensor input, Tensor(a!)? residual, Tensor? weight, float epsilon, Tensor(b!)? out=None, "
+      "Tensor(c!)? out_q=None, Tensor(d!)? scales=None, int group_size=0, bool scale_ue8m0=False) -> ()");
   m.def("b200_quant_mxfp8(Tensor input, Tensor! output_q, Tensor! output_s) -> ()");
   m.def("silu_and_mul(Tensor! result, Tensor input) -> ()");
   m.def("swigluoai_and_mul(Tensor! out, Tensor input, float alpha=1.702, float limit=7.0) -> ()");
@@ -280,6 +396,7 @@ TORCH_LIBRARY_IMPL(_C, CUDA, m) {
   m.impl("silu_and_mul", &silu_and_mul);
   m.impl("swigluoai_and_mul", &swigluoai_and_mul);
   m.impl("per_token_group_fp8_quant", &per_token_group_fp8_quant);
+  m.impl("b200_add_rms_norm", &b200_add_rms_norm);
   m.impl("b200_quant_mxfp8", &b200_quant_mxfp8);
   m.impl("gelu_and_mul", &gelu_and_mul);
   m.impl("gelu_tanh_and_mul", &gelu_tanh_and_mul);

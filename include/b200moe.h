@@ -594,6 +594,52 @@ int b200moe_moe_sum(void* out, const void* in, b200moe_dtype dtype,
                     const int32_t* expert_map, b200moe_stream stream);
 
 /* ------------------------------------------------------------------------- */
+/* A whole layer for a few tokens                                             */
+/* ------------------------------------------------------------------------- */
+
+typedef enum {
+  B200MOE_ACT_SILU = 0,       /* silu(gate) * up, gate = features [0, I), up = [I, 2I)  */
+  B200MOE_ACT_GELU = 1,       /* gelu(gate) * up, erf form                              */
+  B200MOE_ACT_GELU_TANH = 2,  /* the same, tanh form                                    */
+  B200MOE_ACT_SWIGLUOAI = 3,  /* gate = even, up = odd features; act_alpha, act_limit   */
+  B200MOE_ACT_SWIGLUSTEP = 4  /* min(silu(gate), act_limit) * clamp(up, +-act_limit)    */
+} b200moe_activation;
+
+/* out[t] = sum_k w[t,k] * (W2[e] act(W13[e] x[t] + b13[e]) + b2[e]), e the local expert
+ * of topk_ids[t,k] (slots without one add nothing), in two kernels and for up to
+ * B200MOE_FEW_TOKENS tokens.  What the stages of a layer call compute (permutation, two
+ * grouped GEMMs, activation, top-k reduction), with fewer roundings: activations are not
+ * quantised, and only those that the tensor cores multiply are rounded, to 16 bits.
+ * No counterpart op in the reference.  Begin with an all-zero struct. */
+#define B200MOE_FEW_TOKENS 16
+typedef struct {
+  const void* x;              /* [num_tokens, hidden] dtype                           */
+  const void* topk_ids;       /* [num_tokens, topk] i32 / i64                         */
+  const float* topk_weights;  /* [num_tokens, topk]                                   */
+  const int32_t* expert_map;  /* [total_experts] local expert or -1; NULL: ids are local */
+  void* out;                  /* [num_tokens, hidden] dtype                           */
+  /* weights [num_experts, ...]: 16-bit [E,K,N] (of dtype), block-scaled fp8 (either
+     layout), MXFP4 or int4, as b200moe_grouped_gemm takes them; biases [E,N] of dtype or
+     NULL; N x K of w13 is 2*inter x hidden, of w2 hidden x inter                       */
+  const void *w13, *w13_scale, *w13_bias;
+  const void *w2, *w2_scale, *w2_bias;
+  void* workspace;            /* b200moe_few_tokens_workspace_bytes, 16-byte aligned; its
+                                 contents need not outlive the call, nor be cleared     */
+  size_t workspace_bytes;
+  b200moe_weight_format w13_format, w2_format;
+  int w13_group, w2_group;    /* int4: values per scale                               */
+  int num_tokens, hidden, inter, topk, num_experts, total_experts;
+  b200moe_dtype dtype;        /* BF16 or F16                                          */
+  b200moe_dtype ids_dtype;
+  b200moe_activation activation;
+  float act_alpha, act_limit;
+  float clamp_limit;          /* >0: gate = min(gate, L), up = clamp(up, +-L) first    */
+  int max_ctas;               /* >0: at most this many CTAs; 0: one per SM            */
+} b200moe_few_tokens_args;
+size_t b200moe_few_tokens_workspace_bytes(int num_tokens, int topk, int inter);
+int b200moe_few_tokens_layer(const b200moe_few_tokens_args* args, b200moe_stream stream);
+
+/* ------------------------------------------------------------------------- */
 /* Expert parallelism over peer memory                                        */
 /* ------------------------------------------------------------------------- */
 

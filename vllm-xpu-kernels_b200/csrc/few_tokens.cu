@@ -1,0 +1,160 @@
+// A whole Mixture-of-Experts layer for a few tokens in two kernels:
+//
+//   up:    h[s] = act(W13[e] x[t] + b13[e])              for every slot s = (t, k) with a local expert e
+//   down:  out[t] = sum_k w[t,k] (W2[e] h[s] + b2[e])
+//
+// Weights are taken as they are stored; activations stay in 16 bits or more, sums in fp32.
+#include "common.cuh"
+#include "few_tokens.cuh"
+
+namespace b200moe {
+namespace {
+
+// One weight, W_e[n, k], in fp32.
+template <typename T>
+__device__ __forceinline__ float weight_at(const FewMatrix& w, int64_t e, int n, int k) {
+  const int64_t N = w.n, K = w.k;
+  const uint8_t* b = reinterpret_cast<const uint8_t*>(w.w);
+  switch (w.format) {
+    case B200MOE_W_BF16_KN: return to_f32<T>(reinterpret_cast<const T*>(w.w)[(e * K + k) * N + n]);
+    case B200MOE_W_FP8_BLOCK_NK:
+    case B200MOE_W_FP8_BLOCK_KN: {
+      const uint8_t q = w.format == B200MOE_W_FP8_BLOCK_NK ? b[(e * N + n) * K + k] : b[(e * K + k) * N + n];
+      return e4m3_to_f32(q) * reinterpret_cast<const float*>(w.scale)[(e * (N / 128) + n / 128) * (K / 128) + k / 128];
+    }
+    case B200MOE_W_INT4_NK: {
+      const uint8_t q = b[(e * N + n) * (K / 2) + k / 2];
+      const int v = (int)(((k & 1) ? (q >> 4) : (q & 15)) ^ 8) - 8;
+      return (float)v * to_f32<T>(reinterpret_cast<const T*>(w.scale)[(e * N + n) * (K / w.group) + k / w.group]);
+    }
+    default: {
+      const uint8_t q = b[(e * N + n) * (K / 2) + k / 2];
+      return e2m1_to_f32((k & 1) ? (q >> 4) : (q & 15)) *
+             e8m0_to_f32(reinterpret_cast<const uint8_t*>(w.scale)[(e * N + n) * (K / 32) + k / 32]);
+    }
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// A warp per feature of h and slot.
+template <typename T>
+__global__ void __launch_bounds__(256) few_up_simple_kernel(FewParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int f = blockIdx.x * 8 + (threadIdx.x >> 5), slot = blockIdx.y, lane = threadIdx.x & 31;
+  const int e = local_expert(p, slot);
+  if (e < 0 || f >= p.inter) return;
+  const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;   // gate and up of a feature side by side
+  const int ng = pairs ? 2 * f : f, nu = pairs ? 2 * f + 1 : p.inter + f;
+  const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)(slot / p.topk) * p.hidden;
+  float g = 0.f, u = 0.f;
+  for (int k = lane; k < p.hidden; k += 32) {
+    const float v = to_f32<T>(x[k]);
+    g = fmaf(v, weight_at<T>(p.w13, e, ng, k), g);
+    u = fmaf(v, weight_at<T>(p.w13, e, nu, k), u);
+  }
+  g = warp_sum(g);
+  u = warp_sum(u);
+  if (lane == 0) {
+    const T* b = reinterpret_cast<const T*>(p.w13.bias);
+    if (b) {
+      g += to_f32<T>(b[(int64_t)e * p.w13.n + ng]);
+      u += to_f32<T>(b[(int64_t)e * p.w13.n + nu]);
+    }
+    p.h[(int64_t)slot * p.inter + f] = gated(p, g, u);
+  }
+}
+
+// A warp per output feature and token.
+template <typename T>
+__global__ void __launch_bounds__(256) few_down_simple_kernel(FewParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int n = blockIdx.x * 8 + (threadIdx.x >> 5), t = blockIdx.y, lane = threadIdx.x & 31;
+  if (n >= p.hidden) return;
+  const T* b = reinterpret_cast<const T*>(p.w2.bias);
+  float sum = 0.f;
+  for (int k = 0; k < p.topk; ++k) {
+    const int slot = t * p.topk + k, e = local_expert(p, slot);
+    if (e < 0) continue;
+    const float* h = p.h + (int64_t)slot * p.inter;
+    float y = 0.f;
+    for (int i = lane; i < p.inter; i += 32) y = fmaf(h[i], weight_at<T>(p.w2, e, n, i), y);
+    y = warp_sum(y);
+    if (b) y += to_f32<T>(b[(int64_t)e * p.hidden + n]);
+    sum = fmaf(p.weights[slot], y, sum);
+  }
+  if (lane == 0) reinterpret_cast<T*>(p.out)[(int64_t)t * p.hidden + n] = from_f32<T>(sum);
+}
+
+template <typename T>
+int launch_simple(const FewParams& p, cudaStream_t st) {
+  B200_LAUNCHED("few_up_simple_kernel", launch_pdl(true, few_up_simple_kernel<T>, dim3((p.inter + 7) / 8, p.tokens * p.topk), dim3(256), 0, st, p));
+  B200_LAUNCHED("few_down_simple_kernel", launch_pdl(true, few_down_simple_kernel<T>, dim3((p.hidden + 7) / 8, p.tokens), dim3(256), 0, st, p));
+  return B200MOE_OK;
+}
+
+bool known_format(int f) {
+  return f == B200MOE_W_BF16_KN || f == B200MOE_W_FP8_BLOCK_NK || f == B200MOE_W_FP8_BLOCK_KN || f == B200MOE_W_MXFP4_NK ||
+         f == B200MOE_W_INT4_NK;
+}
+
+// What the sizes of a matrix have to be for its format.
+int check_matrix(const b200moe_few_tokens_args* a, b200moe_weight_format f, const void* w, const void* scale, int group, int n, int k,
+                 const char* name) {
+  if (!known_format(f))
+    return fail(B200MOE_E_UNSUPPORTED, "few_tokens_layer: 16-bit [E,K,N], block-scaled fp8, MXFP4 and int4 weights only");
+  B200_CHECK_ARG(w != nullptr && (f == B200MOE_W_BF16_KN || scale != nullptr), "few_tokens_layer: %s or its scales are missing", name);
+  if (f == B200MOE_W_FP8_BLOCK_NK || f == B200MOE_W_FP8_BLOCK_KN)
+    B200_CHECK_ARG(n % 128 == 0 && k % 128 == 0, "few_tokens_layer: block-scaled %s needs sizes divisible by 128", name);
+  if (f == B200MOE_W_MXFP4_NK) B200_CHECK_ARG(k % 32 == 0, "few_tokens_layer: MXFP4 %s needs rows of a multiple of 32", name);
+  if (f == B200MOE_W_INT4_NK)
+    B200_CHECK_ARG((group == 32 || group == 64 || group == 128 || group == 256) && k % group == 0,
+                   "few_tokens_layer: int4 %s needs groups of 32, 64, 128 or 256 that divide its rows", name);
+  (void)a;
+  return B200MOE_OK;
+}
+
+}  // namespace
+}  // namespace b200moe
+
+using namespace b200moe;
+
+extern "C" size_t b200moe_few_tokens_workspace_bytes(int num_tokens, int topk, int inter) {
+  if (num_tokens <= 0 || topk <= 0 || inter <= 0) return 0;
+  return (size_t)num_tokens * topk * inter * sizeof(float);
+}
+
+extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200moe_stream stream) {
+  B200_CHECK_ARG(a != nullptr, "few_tokens_layer: null arguments");
+  B200_CHECK_ARG(a->dtype == B200MOE_BF16 || a->dtype == B200MOE_F16, "few_tokens_layer: hidden states must be bfloat16 or float16");
+  B200_CHECK_ARG(a->num_tokens >= 0 && a->num_tokens <= B200MOE_FEW_TOKENS, "few_tokens_layer: at most %d tokens", B200MOE_FEW_TOKENS);
+  B200_CHECK_ARG(a->hidden >= 1 && a->inter >= 1 && a->inter <= (1 << 29), "few_tokens_layer: sizes must be positive");
+  B200_CHECK_ARG(a->topk >= 1 && a->topk <= kFewMaxTopk, "few_tokens_layer: topk must be in [1, %d]", kFewMaxTopk);
+  B200_CHECK_ARG(a->num_experts >= 1 && a->num_experts <= kFewMaxExperts, "few_tokens_layer: num_experts must be in [1, %d]", kFewMaxExperts);
+  B200_CHECK_ARG(a->ids_dtype == B200MOE_I32 || a->ids_dtype == B200MOE_I64, "few_tokens_layer: topk_ids must be int32 or int64");
+  B200_CHECK_ARG(a->activation >= B200MOE_ACT_SILU && a->activation <= B200MOE_ACT_SWIGLUSTEP, "few_tokens_layer: unknown activation");
+  int rc = check_matrix(a, a->w13_format, a->w13, a->w13_scale, a->w13_group, 2 * a->inter, a->hidden, "w13");
+  if (rc == B200MOE_OK) rc = check_matrix(a, a->w2_format, a->w2, a->w2_scale, a->w2_group, a->hidden, a->inter, "w2");
+  if (rc != B200MOE_OK) return rc;
+  B200_CHECK_ARG(a->w13_format == a->w2_format, "few_tokens_layer: w13 and w2 must have the same format");
+  if (a->num_tokens == 0) return B200MOE_OK;
+  B200_CHECK_ARG(a->x && a->topk_ids && a->topk_weights && a->out, "few_tokens_layer: null pointer");
+  const size_t need = b200moe_few_tokens_workspace_bytes(a->num_tokens, a->topk, a->inter);
+  if (a->workspace == nullptr || a->workspace_bytes < need || ((uintptr_t)a->workspace & 15) != 0)
+    return fail(B200MOE_E_WORKSPACE, "few_tokens_layer: needs %zu bytes of 16-byte aligned workspace", need);
+  FewParams p = {};
+  p.x = a->x; p.ids = a->topk_ids; p.ids64 = a->ids_dtype == B200MOE_I64; p.weights = a->topk_weights;
+  p.expert_map = a->expert_map; p.out = a->out; p.h = (float*)a->workspace;
+  p.tokens = a->num_tokens; p.hidden = a->hidden; p.inter = a->inter; p.topk = a->topk;
+  p.experts = a->num_experts; p.id_limit = a->expert_map ? a->total_experts : a->num_experts;
+  p.act = a->activation; p.alpha = a->act_alpha; p.limit = a->act_limit; p.clamp = a->clamp_limit;
+  p.w13 = {a->w13, a->w13_scale, a->w13_bias, a->w13_format, a->w13_group, 2 * a->inter, a->hidden};
+  p.w2 = {a->w2, a->w2_scale, a->w2_bias, a->w2_format, a->w2_group, a->hidden, a->inter};
+  return a->dtype == B200MOE_BF16 ? launch_simple<__nv_bfloat16>(p, as_stream(stream)) : launch_simple<__half>(p, as_stream(stream));
+}

@@ -1,0 +1,74 @@
+// What the kernels of the layer for a few tokens share.
+#pragma once
+
+#include "common.cuh"
+
+namespace b200moe {
+namespace {
+
+constexpr int kFewMaxTopk = 32, kFewMaxExperts = 1024;
+
+struct FewMatrix {
+  const void* w;
+  const void* scale;
+  const void* bias;      // [E, n] in the activation type, or NULL
+  int format, group;     // b200moe_weight_format; int4: values per scale
+  int n, k;
+};
+
+struct FewParams {
+  const void* x;               // [tokens, hidden]
+  const void* ids;             // [tokens, topk]
+  const float* weights;        // [tokens, topk]
+  const int32_t* expert_map;   // [id_limit], or NULL
+  void* out;                   // [tokens, hidden]
+  float* h;                    // [tokens * topk, inter]
+  int tokens, hidden, inter, topk, experts, id_limit;
+  int act;
+  float alpha, limit, clamp;
+  bool ids64;
+  FewMatrix w13, w2;
+};
+
+// The slot's expert among the local ones, -1 if it has none here.
+__device__ __forceinline__ int local_expert(const FewParams& p, int slot) {
+  const int64_t id = p.ids64 ? reinterpret_cast<const int64_t*>(p.ids)[slot] : (int64_t)reinterpret_cast<const int32_t*>(p.ids)[slot];
+  if (id < 0 || id >= p.id_limit) return -1;
+  const int e = p.expert_map ? p.expert_map[id] : (int)id;
+  return e >= 0 && e < p.experts ? e : -1;
+}
+
+// Minimum and maximum that keep a NaN.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float clamp_nan(float v, float limit) { return max_nan(min_nan(v, limit), -limit); }
+
+// The gated activation in fp32, unrounded.
+__device__ __forceinline__ float gated(const FewParams& p, float g, float u) {
+  if (p.clamp > 0.f) {
+    g = min_nan(g, p.clamp);
+    u = clamp_nan(u, p.clamp);
+  }
+  switch (p.act) {
+    case B200MOE_ACT_SILU: return g / (1.0f + expf(-g)) * u;
+    case B200MOE_ACT_GELU: return 0.5f * g * (1.0f + erff(g * 0.70710678118654752440f)) * u;
+    case B200MOE_ACT_GELU_TANH:
+      return 0.5f * g * (1.0f + tanhf(0.79788456080286535588f * (g + 0.044715f * (g * g * g)))) * u;
+    case B200MOE_ACT_SWIGLUOAI:
+      g = min_nan(g, p.limit);
+      u = clamp_nan(u, p.limit);
+      return (u + 1.0f) * (g / (1.0f + expf(-g * p.alpha)));
+    default: return min_nan(g / (1.0f + expf(-g)), p.limit) * clamp_nan(u, p.limit);
+  }
+}
+
+}  // namespace
+}  // namespace b200moe

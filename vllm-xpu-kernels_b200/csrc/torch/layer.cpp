@@ -564,6 +564,70 @@ PyObject* layer_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// layer_few(plan, output, hidden, topk_weights, topk_ids, expert_map | None, max_ctas, persistent): the whole layer in
+// two kernels, for up to B200MOE_FEW_TOKENS tokens.
+PyObject* layer_few(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 8, "layer_few takes 8 arguments");
+  const Plan& p = *plan_arg(a[0]);
+  const at::Tensor &y = tensor_arg(a[1], "output"), &x = tensor_arg(a[2], "hidden_states"), &w = tensor_arg(a[3], "topk_weights"),
+                   &ids = tensor_arg(a[4], "topk_ids");
+  const std::optional<at::Tensor> map = optional_arg(a[5], "expert_map");
+  need_cuda(x, "hidden_states");
+  TORCH_CHECK(x.dim() == 2, "hidden_states must be [num_rows, hidden_size]");
+  const int64_t T = x.size(0), H = x.size(1), K = p.topk, M = T * K;
+  TORCH_CHECK(T <= B200MOE_FEW_TOKENS, "the layer for a few tokens takes at most ", B200MOE_FEW_TOKENS, " of them");
+  const b200moe_dtype dt = dtype16(y.scalar_type(), "ptr_D");
+  TORCH_CHECK(x.scalar_type() == y.scalar_type(), "ptr_A and ptr_D must have the same dtype");
+  TORCH_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, "topk_ids must be int64 or int32");
+  TORCH_CHECK(ids.dim() == 2 && ids.size(0) == T && ids.size(1) == K, "topk_ids must be [num_rows, TopK]");
+  TORCH_CHECK(w.scalar_type() == at::kFloat, "topk_weights must be float32");
+  TORCH_CHECK(y.dim() == 2 && y.size(0) == T && y.size(1) == H && w.numel() == M,
+              "output must be [num_rows, hidden_size], topk_weights [num_rows, TopK]");
+  TORCH_CHECK(x.is_contiguous() && ids.is_contiguous() && w.is_contiguous() && y.is_contiguous(),
+              "the layer for a few tokens expects contiguous tensors");
+  if (map.has_value()) {
+    TORCH_CHECK(map->scalar_type() == at::kInt && map->is_contiguous(), "expert_map must be int32");
+    TORCH_CHECK(map->size(0) == p.total_experts, "expert_map must be [total_experts_num]");
+  }
+  for (const at::Tensor* t : {&y, &w, &ids, map.has_value() ? &*map : &x, &p.w13, &p.w2})
+    TORCH_CHECK(t->device() == x.device(), "all tensors of a layer call must be on the device of hidden_states");
+  const int64_t k2 = p.inter * p.inter_scale;
+  TORCH_CHECK_NOT_IMPLEMENTED(p.inter_scale == 1, "the layer for a few tokens has no relu2_no_mul");
+  Plan q = p;   // (weights are read as they are: no quantised activations to go with them)
+  q.block_fp8 = q.mx = false;
+  const Weights weights = describe(q, H, y.scalar_type());
+  if (T == 0) Py_RETURN_NONE;
+  static const b200moe_activation acts[] = {B200MOE_ACT_SILU, B200MOE_ACT_GELU, B200MOE_ACT_GELU_TANH, B200MOE_ACT_SWIGLUOAI,
+                                            B200MOE_ACT_SILU, B200MOE_ACT_SWIGLUSTEP};
+  b200moe_few_tokens_args g = {};
+  g.x = x.data_ptr(); g.out = y.data_ptr(); g.dtype = dt;
+  g.topk_ids = ids.data_ptr(); g.ids_dtype = index_dtype(ids); g.topk_weights = w.data_ptr<float>();
+  g.expert_map = map.has_value() ? map->data_ptr<int32_t>() : nullptr;
+  g.w13 = p.w13.data_ptr(); g.w13_format = weights.d13.format; g.w13_group = weights.d13.group;
+  g.w2 = p.w2.data_ptr(); g.w2_format = weights.d2.format; g.w2_group = weights.d2.group;
+  g.w13_scale = p.s13.has_value() ? p.s13->data_ptr() : nullptr;
+  g.w2_scale = p.s2.has_value() ? p.s2->data_ptr() : nullptr;
+  g.w13_bias = p.b13.has_value() ? p.b13->data_ptr() : nullptr;
+  g.w2_bias = p.b2.has_value() ? p.b2->data_ptr() : nullptr;
+  g.num_tokens = (int)T; g.hidden = (int)H; g.inter = (int)k2; g.topk = (int)K;
+  g.num_experts = (int)p.experts; g.total_experts = (int)p.total_experts;
+  g.activation = acts[p.act]; g.act_alpha = 1.702f; g.act_limit = 7.0f; g.clamp_limit = (float)p.clamp;
+  g.max_ctas = (int)int_arg(a[6]);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  WithoutGil gil;
+  {
+    g.workspace_bytes = b200moe_few_tokens_workspace_bytes((int)T, (int)K, (int)k2);
+    const Workspace workspace(stream, g.workspace_bytes, a[7] == Py_True);
+    g.workspace = workspace.mem.data_ptr();
+    check_status(b200moe_few_tokens_layer(&g, (b200moe_stream)stream.stream()));
+  }
+  gil.end();
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* workspace_clear(PyObject*, PyObject*) {
   HANDLE_TH_ERRORS
   clear_slabs();
@@ -577,6 +641,7 @@ PyMethodDef* layer_methods() {
   static PyMethodDef methods[] = {
       {"layer_plan", (PyCFunction)(void (*)(void))layer_plan, METH_FASTCALL, nullptr},
       {"layer_run", (PyCFunction)(void (*)(void))layer_run, METH_FASTCALL, nullptr},
+      {"layer_few", (PyCFunction)(void (*)(void))layer_few, METH_FASTCALL, nullptr},
       {"layer_experts", (PyCFunction)(void (*)(void))layer_experts, METH_FASTCALL, nullptr},
       {"workspace_clear", workspace_clear, METH_NOARGS, nullptr},
       {nullptr, nullptr, 0, nullptr}};

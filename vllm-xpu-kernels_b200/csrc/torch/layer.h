@@ -20,7 +20,7 @@ struct WeightDesc {
 WeightDesc describe_weights(const at::Tensor& w, const std::optional<at::Tensor>& scale, int64_t N, int64_t K,
                             int64_t num_experts, int64_t layout, at::ScalarType activation_dtype);
 
-// Functions of the extension module: layer_plan, layer_run, layer_experts, workspace_clear.
+// Functions of the extension module: layer_plan, layer_run, layer_few, layer_experts, workspace_clear.
 PyMethodDef* layer_methods();
 
 }  // namespace b200shim

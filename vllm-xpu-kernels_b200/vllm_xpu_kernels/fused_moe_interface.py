@@ -34,6 +34,7 @@ except ImportError as e:  # native libraries not built
 REF_FUSED_MOE_ENV = "VLLM_XPU_FUSED_MOE_USE_REF"
 USE_MXFP4_FP8_ENV = "VLLM_XPU_FUSED_MOE_USE_MXFP4_FP8"
 FP8_BLOCK_SIZE = 128
+FEW_TOKENS = 16          # tokens up to which few_tokens=True takes the form of two kernels
 FP8_FUSED_MIN_ROWS = 12   # routed rows per expert from which fuse_activation=True takes the fused form of fp8 layers
 
 
@@ -212,7 +213,19 @@ class XpuFusedMoe:
     selects it); ``"bf16"`` keeps 16-bit activations exactly as the reference's
     device kernel does (w4a16) and dequantises the weights on the way into the
     tensor cores.
+
+    ``few_tokens`` (not in the reference; keyword only, default False): calls of
+    ``apply`` with up to ``FEW_TOKENS`` tokens run as two kernels instead of a chain of five or
+    more: one that multiplies with ``w13`` and applies the activation, one that
+    multiplies with ``w2`` and adds the experts up.  Weights are used as they are stored,
+    activations are not quantised (``mxfp4_activations`` and the fp8 activations of
+    block-scaled layers concern the other calls), so results differ from the other form's in
+    rounding and are the more accurate.  For 16-bit, block-scaled fp8, MXFP4 and int4
+    weights and every activation but ``relu2_no_mul``; calls with ``a1q_scale`` and larger
+    ones run as without it.
     """
+
+    few_tokens = False       # (also of layers that were saved before there was a choice)
 
     def __init__(
         self,
@@ -233,6 +246,7 @@ class XpuFusedMoe:
         fuse_activation: Optional[bool] = None,
         mxfp4_activations: Optional[str] = None,
         persistent_workspace: bool = True,
+        few_tokens: bool = False,
     ):
         assert w13.is_contiguous() and w2.is_contiguous()
         _require_native()
@@ -336,6 +350,11 @@ class XpuFusedMoe:
             raise ValueError("the block-scaled MXFP4 GEMM has no fused SiLU epilogue")
         if fuse_activation and self._act_kind not in ("silu", "swigluoai"):
             raise ValueError(f"no fused epilogue for the {self._act_kind} activation")
+        if few_tokens and (is_fp8 or is_mxfp8):
+            raise NotImplementedError("few_tokens: 16-bit, block-scaled fp8, MXFP4 and int4 weights only")
+        if few_tokens and self._act_kind == "relu2_no_mul":
+            raise NotImplementedError("few_tokens: no kernel for the relu2_no_mul activation")
+        self.few_tokens = few_tokens
         self._native_plan = None
 
         self.expert_map = expert_map
@@ -389,8 +408,21 @@ class XpuFusedMoe:
 
     def apply(self, output, hidden_states, topk_weights, topk_ids,
               expert_map=None, a1q_scale=None):
+        if self.few_tokens and a1q_scale is None and hidden_states.shape[0] <= FEW_TOKENS:
+            self._apply_few_tokens(output, hidden_states, topk_weights, topk_ids, expert_map)
+            return
         self._apply_kernel(output, hidden_states, topk_weights, topk_ids,
                            expert_map, a1q_scale)
+
+    def _apply_few_tokens(self, output, hidden_states, topk_weights, topk_ids, expert_map):
+        if expert_map is None and self.ep_size > 1:
+            expert_map = self.expert_map
+        if self.stage_hook is not None:
+            self.stage_hook("routing")
+        _xpu_C.layer_few(self._native_plan or self._plan(), output, hidden_states, topk_weights, topk_ids, expert_map,
+                         self.gemm_max_ctas, self.persistent_workspace)
+        if self.stage_hook is not None:
+            self.stage_hook("experts")
 
     # The stages are the reference's eight steps (:328-419), launched from native code; what
     # differs is inside the kernels and, for block fp8, that activations really are quantised

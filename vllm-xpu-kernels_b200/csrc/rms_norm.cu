@@ -120,8 +120,189 @@ __global__ void __launch_bounds__(256) rms_norm_scalar_kernel(RmsParams p) {
   }
 }
 
+// A thread's piece of a row: N values, moved with one access of up to 32 bytes.
+template <typename T, int N> struct alignas(N * sizeof(T)) Piece { T e[N]; };
+template <typename T, int N>
+__device__ __forceinline__ void ld_piece(Piece<T, N>& d, const T* p) {
+  if constexpr (sizeof(T) * N == 32) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&d);
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+  } else if constexpr (sizeof(T) * N == 64) {   // (fp32 weights of a 16-bit piece)
+    ld_piece<T, N / 2>(reinterpret_cast<Piece<T, N / 2>*>(&d)[0], p);
+    ld_piece<T, N / 2>(reinterpret_cast<Piece<T, N / 2>*>(&d)[1], p + N / 2);
+  } else {
+    d = *reinterpret_cast<const Piece<T, N>*>(p);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void st_piece(T* p, const Piece<T, N>& s) {
+  if constexpr (sizeof(T) * N == 32) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&s);
+    asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+                 :: "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "l"(p) : "memory");
+  } else {
+    *reinterpret_cast<Piece<T, N>*>(p) = s;
+  }
+}
+
+enum ScaleMode { kNoScales, kRowScale, kGroupScales };
+
+// Rows are read once and stay in registers between their sums and the result.  blockDim = (threads of a row, rows of a
+// block); a thread has V pieces of N values, blockDim.x pieces apart.  A resident block takes row after row and asks for
+// the next one before it waits for its sums.
+template <typename T, typename W, int N, int V, int kMode>
+__global__ void __launch_bounds__(1024) rms_norm_kernel(RmsParams p) {
+  __shared__ float2 red[2][32];
+  pdl_trigger();
+  pdl_wait();
+  const int tx = threadIdx.x, lane = tx & 31, warps = blockDim.x >> 5, warp = threadIdx.y * warps + (tx >> 5);
+  const int pieces = p.hidden / N;
+  const T* const input = reinterpret_cast<const T*>(p.input);
+  T* const residual = reinterpret_cast<T*>(p.residual);
+  const W* const w = reinterpret_cast<const W*>(p.weight);
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  Piece<T, N> x[V], b[V];
+  auto ask = [&](int64_t r) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int j = tx + i * blockDim.x;
+      if (r < p.rows && j < pieces) {
+        ld_piece<T, N>(x[i], input + r * p.input_stride + (int64_t)j * N);
+        if (residual) ld_piece<T, N>(b[i], residual + r * p.residual_stride + (int64_t)j * N);
+      }
+    }
+  };
+  int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  ask(r);
+  // (the rows of a block run through the same number of turns, so that its barrier is met by all)
+  for (int64_t first = (int64_t)blockIdx.x * blockDim.y, turn = 0; first < p.rows; first += step, r += step, ++turn) {
+    Piece<T, N> v[V];
+    Piece<W, N> wv[V];
+    float sum = 0.f, top = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int j = tx + i * blockDim.x;
+      if (r < p.rows && j < pieces) {
+        if (w) ld_piece<W, N>(wv[i], w + (int64_t)j * N);
+        v[i] = x[i];
+        if (residual) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) v[i].e[k] = from_f32<T>(to_f32<T>(x[i].e[k]) + to_f32<T>(b[i].e[k]));
+          st_piece<T, N>(residual + r * p.residual_stride + (int64_t)j * N, v[i]);
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const float s = to_f32<T>(v[i].e[k]);
+          sum = fmaf(s, s, sum);
+          if (kMode == kRowScale) top = max_nan(top, fabsf(w ? s * to_f32<W>(wv[i].e[k]) : s));
+        }
+      }
+    }
+    ask(r + step);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (kMode == kRowScale) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+    }
+    if (warps > 1) {   // two buffers in turn: one barrier a row
+      if (lane == 0) red[turn & 1][warp] = make_float2(sum, top);
+      __syncthreads();
+      sum = 0.f;
+      for (int i = 0; i < warps; ++i) {
+        const float2 o = red[turn & 1][threadIdx.y * warps + i];
+        sum += o.x;
+        if (kMode == kRowScale) top = max_nan(top, o.y);
+      }
+    }
+    const float rs = rsqrtf(sum / (float)p.hidden + p.eps);
+    float scale = 0.f, inv = 0.f;
+    if (kMode == kRowScale) {
+      scale = scale_of(top * rs, p.ue8m0);
+      inv = __fdiv_rn(1.0f, scale);
+      if (tx == 0 && r < p.rows) p.scales[r * p.s_stride_row] = scale;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int j = tx + i * blockDim.x;
+      const bool mine = r < p.rows && j < pieces;
+      float y[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float n = to_f32<T>(v[i].e[k]) * rs;
+        y[k] = w ? n * to_f32<W>(wv[i].e[k]) : n;
+      }
+      if (p.out && mine) {
+        Piece<T, N> o;
+#pragma unroll
+        for (int k = 0; k < N; ++k) o.e[k] = from_f32<T>(y[k]);
+        st_piece<T, N>(reinterpret_cast<T*>(p.out) + r * p.out_stride + (int64_t)j * N, o);
+      }
+      if (kMode == kGroupScales) {
+        const int lanes = p.group / N;   // of a group: a power of two
+        float m = 0.f;
+        if (mine) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) m = max_nan(m, fabsf(y[k]));
+        }
+        for (int d = 1; d < lanes; d <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+        scale = scale_of(m, p.ue8m0);
+        inv = __fdiv_rn(1.0f, scale);
+        if (mine && (j & (lanes - 1)) == 0)
+          p.scales[r * p.s_stride_row + (int64_t)(j / lanes) * p.s_stride_group] = scale;
+      }
+      if (kMode != kNoScales && mine) {
+        uint8_t* q = p.q + r * p.q_stride + (int64_t)j * N;
+        if constexpr (N == 1) {
+          *q = f32_to_e4m3(y[0] * inv);
+        } else {
+          Piece<uint32_t, N / 4> o;
+#pragma unroll
+          for (int k = 0; k < N / 4; ++k)
+            o.e[k] = f32x2_to_e4m3x2(y[4 * k] * inv, y[4 * k + 1] * inv) | (f32x2_to_e4m3x2(y[4 * k + 2] * inv, y[4 * k + 3] * inv) << 16);
+          *reinterpret_cast<Piece<uint32_t, N / 4>*>(q) = o;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, typename W, int N, int V, int kMode>
+int launch_rows(const RmsParams& p, cudaStream_t st) {
+  const int threads = ((p.hidden / N + V - 1) / V + 31) / 32 * 32;
+  int rows = 1;   // of a block: at least 128 threads where there are rows for every SM
+  while (rows * threads < 128 && p.rows > (int64_t)rows * sm_count()) rows *= 2;
+  const int64_t blocks = (p.rows + rows - 1) / rows, resident = (int64_t)sm_count() * (1024 / (rows * threads));
+  B200_LAUNCHED("rms_norm_kernel", launch_pdl(p.rows <= kEarlyLaunchRows, rms_norm_kernel<T, W, N, V, kMode>,
+                                              dim3((unsigned)(blocks < resident ? blocks : resident)), dim3(threads, rows), 0, st, p));
+  return B200MOE_OK;
+}
+template <typename T, typename W, int N, int V>
+int launch_mode(const RmsParams& p, cudaStream_t st) {
+  if (p.q == nullptr) return launch_rows<T, W, N, V, kNoScales>(p, st);
+  if (p.group == 0) return launch_rows<T, W, N, V, kRowScale>(p, st);
+  if constexpr (N > 1) return launch_rows<T, W, N, V, kGroupScales>(p, st);
+  return fail(B200MOE_E_BADARG, "add_rms_norm: no such variant");   // (not reached: see pieces_fit)
+}
+
+// Whether rows are made of pieces of n values that can be moved as such.
+bool pieces_fit(const RmsParams& p, int n, int size, int weight_size) {
+  auto fits = [](const void* b, int64_t stride, int bytes, int align) {
+    return ((uintptr_t)b % align) == 0 && (stride * bytes) % align == 0;
+  };
+  const int align = n * size, lanes = p.group / n;
+  return p.hidden % n == 0 && p.hidden / n <= 1024 && fits(p.input, p.input_stride, size, align) &&
+         fits(p.residual, p.residual_stride, size, align) && fits(p.out, p.out_stride, size, align) &&
+         fits(p.weight, 0, 1, n * weight_size < 32 ? n * weight_size : 32) && fits(p.q, p.q_stride, 1, n) &&
+         (p.q == nullptr || p.group == 0 || (p.group % n == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0));
+}
+
 template <typename T, typename W>
 int launch_rms_norm(const RmsParams& p, cudaStream_t st) {
+  constexpr int N = 32 / sizeof(T), kSingles = 8;
+  if (pieces_fit(p, N, sizeof(T), sizeof(W))) return launch_mode<T, W, N, 1>(p, st);
+  if (pieces_fit(p, N / 2, sizeof(T), sizeof(W))) return launch_mode<T, W, N / 2, 1>(p, st);
+  if (p.hidden <= 1024 * kSingles && (p.q == nullptr || p.group == 0)) return launch_mode<T, W, 1, kSingles>(p, st);
   B200_LAUNCHED("rms_norm_scalar_kernel",
                 launch_pdl(p.rows <= kEarlyLaunchRows, rms_norm_scalar_kernel<T, W>, dim3((unsigned)p.rows), dim3(256), 0, st, p));
   return B200MOE_OK;

@@ -6,6 +6,7 @@
 // Weights are taken as they are stored; activations stay in 16 bits or more, sums in fp32.
 #include "common.cuh"
 #include "few_tokens.cuh"
+#include "few_tokens_nk.cuh"
 
 namespace b200moe {
 namespace {
@@ -99,6 +100,58 @@ int launch_simple(const FewParams& p, cudaStream_t st) {
   return B200MOE_OK;
 }
 
+// ---- weights by output feature ---------------------------------------------------------
+constexpr int kMaxSmem = 232448;   // of a block
+
+// The attribute is set once per kernel and device, and always to the most that a block may have, so that calls with
+// different needs do not get into each other's way.
+template <void (*Kern)(FewParams, FewLaunch)>
+int launch_block_per_sm(const char* name, int grid, int smem, cudaStream_t st, const FewParams& p, const FewLaunch& l) {
+  static std::atomic<bool> done[kMaxDevices];
+  const int dev = current_device();
+  if (!done[dev].load(std::memory_order_acquire)) {
+    B200_CUDA_OK(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    done[dev].store(true, std::memory_order_release);
+  }
+  B200_LAUNCHED(name, launch_pdl(true, Kern, dim3(grid), dim3(kThreads), smem, st, p, l));
+  return B200MOE_OK;
+}
+
+template <int F, int NT>
+int launch_nk(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
+  constexpr int MT = F == kFewFp8 ? 2 : 4;
+  constexpr int up_fixed = UpShape<F, MT, NT>::kFixed;
+  const int up_row = (p.hidden + 127) / 128 * 256, down_row = (p.inter + 127) / 128 * 256;
+  l.panel_bytes = min(p.tokens * up_row, (kMaxSmem - up_fixed) / up_row * up_row);
+  int rc = launch_block_per_sm<few_up_kernel<F, MT, NT>>("few_up_kernel", ctas, up_fixed + l.panel_bytes, st, p, l);
+  if (rc != B200MOE_OK) return rc;
+  const int rows = (p.hidden + ctas - 1) / ctas;
+  auto down = [&](auto tiles) {
+    constexpr int M2 = decltype(tiles)::value;
+    constexpr int fixed = DownShape<F, M2, NT>::kFixed;
+    const int64_t want = (int64_t)p.tokens * p.topk * down_row;
+    l.panel_bytes = (int)(want < kMaxSmem - fixed ? want : (kMaxSmem - fixed) / 256 * 256);
+    return launch_block_per_sm<few_down_kernel<F, M2, NT>>("few_down_kernel", ctas, fixed + l.panel_bytes, st, p, l);
+  };
+  if (rows <= 16) return down(std::integral_constant<int, 1>());
+  if (rows <= 32) return down(std::integral_constant<int, 2>());
+  return down(std::integral_constant<int, 4>());
+}
+
+template <int F>
+int launch_nk(const FewParams& p, const FewLaunch& l, int ctas, cudaStream_t st) {
+  return p.tokens <= 8 ? launch_nk<F, 1>(p, l, ctas, st) : launch_nk<F, 2>(p, l, ctas, st);
+}
+
+// Sizes and addresses that these kernels can take; one row of tokens has to fit a block's shared memory.
+bool takes_nk(const FewParams& p) {
+  const int f = p.w13.format;
+  if (f != B200MOE_W_FP8_BLOCK_NK && f != B200MOE_W_MXFP4_NK && f != B200MOE_W_INT4_NK) return false;
+  for (const void* a : {p.x, p.w13.w, p.w13.scale, p.w2.w, p.w2.scale})
+    if (((uintptr_t)a & 15) != 0) return false;
+  return p.hidden % 32 == 0 && p.inter % 32 == 0 && p.hidden <= 16384;
+}
+
 bool known_format(int f) {
   return f == B200MOE_W_BF16_KN || f == B200MOE_W_FP8_BLOCK_NK || f == B200MOE_W_FP8_BLOCK_KN || f == B200MOE_W_MXFP4_NK ||
          f == B200MOE_W_INT4_NK;
@@ -134,7 +187,8 @@ extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200mo
   B200_CHECK_ARG(a != nullptr, "few_tokens_layer: null arguments");
   B200_CHECK_ARG(a->dtype == B200MOE_BF16 || a->dtype == B200MOE_F16, "few_tokens_layer: hidden states must be bfloat16 or float16");
   B200_CHECK_ARG(a->num_tokens >= 0 && a->num_tokens <= B200MOE_FEW_TOKENS, "few_tokens_layer: at most %d tokens", B200MOE_FEW_TOKENS);
-  B200_CHECK_ARG(a->hidden >= 1 && a->inter >= 1 && a->inter <= (1 << 29), "few_tokens_layer: sizes must be positive");
+  B200_CHECK_ARG(a->hidden >= 1 && a->inter >= 1 && a->hidden <= (1 << 20) && a->inter <= (1 << 20),
+                 "few_tokens_layer: sizes must be between 1 and 2^20");
   B200_CHECK_ARG(a->topk >= 1 && a->topk <= kFewMaxTopk, "few_tokens_layer: topk must be in [1, %d]", kFewMaxTopk);
   B200_CHECK_ARG(a->num_experts >= 1 && a->num_experts <= kFewMaxExperts, "few_tokens_layer: num_experts must be in [1, %d]", kFewMaxExperts);
   B200_CHECK_ARG(a->ids_dtype == B200MOE_I32 || a->ids_dtype == B200MOE_I64, "few_tokens_layer: topk_ids must be int32 or int64");
@@ -156,5 +210,14 @@ extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200mo
   p.act = a->activation; p.alpha = a->act_alpha; p.limit = a->act_limit; p.clamp = a->clamp_limit;
   p.w13 = {a->w13, a->w13_scale, a->w13_bias, a->w13_format, a->w13_group, 2 * a->inter, a->hidden};
   p.w2 = {a->w2, a->w2_scale, a->w2_bias, a->w2_format, a->w2_group, a->hidden, a->inter};
+  const int ctas = a->max_ctas > 0 && a->max_ctas < sm_count() ? a->max_ctas : sm_count();
+  if (takes_nk(p)) {
+    FewLaunch l = {};
+    l.f16 = a->dtype == B200MOE_F16;
+    if (p.w13.format == B200MOE_W_FP8_BLOCK_NK) return launch_nk<kFewFp8>(p, l, ctas, as_stream(stream));
+    if (p.w13.format == B200MOE_W_MXFP4_NK) return launch_nk<kFewFp4>(p, l, ctas, as_stream(stream));
+    const bool fine = p.w13.group < 128 || p.w2.group < 128;
+    return fine ? launch_nk<kFewInt4Fine>(p, l, ctas, as_stream(stream)) : launch_nk<kFewInt4>(p, l, ctas, as_stream(stream));
+  }
   return a->dtype == B200MOE_BF16 ? launch_simple<__nv_bfloat16>(p, as_stream(stream)) : launch_simple<__half>(p, as_stream(stream));
 }

@@ -119,23 +119,15 @@ int launch_block_per_sm(const char* name, int grid, int smem, cudaStream_t st, c
 
 template <int F, int NT>
 int launch_nk(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
-  constexpr int MT = F == kFewFp8 ? 2 : 4;
-  constexpr int up_fixed = UpShape<F, MT, NT>::kFixed;
-  const int up_row = (p.hidden + 127) / 128 * 256, down_row = (p.inter + 127) / 128 * 256;
-  l.panel_bytes = min(p.tokens * up_row, (kMaxSmem - up_fixed) / up_row * up_row);
-  int rc = launch_block_per_sm<few_up_kernel<F, MT, NT>>("few_up_kernel", ctas, up_fixed + l.panel_bytes, st, p, l);
+  constexpr int k = FewShape<F>::kK, up_room = kMaxSmem - UpShape<F, NT>::kFixed, down_room = kMaxSmem - DownShape<F>::kFixed;
+  const int up_row = (p.hidden + k - 1) / k * k * 2, down_row = (p.inter + k - 1) / k * k * 2;
+  l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
+  int rc = launch_block_per_sm<few_up_kernel<F, NT>>("few_up_kernel", ctas, UpShape<F, NT>::kFixed + l.panel_bytes, st, p, l);
   if (rc != B200MOE_OK) return rc;
-  const int rows = (p.hidden + ctas - 1) / ctas;
-  auto down = [&](auto tiles) {
-    constexpr int M2 = decltype(tiles)::value;
-    constexpr int fixed = DownShape<F, M2, NT>::kFixed;
-    const int64_t want = (int64_t)p.tokens * p.topk * down_row;
-    l.panel_bytes = (int)(want < kMaxSmem - fixed ? want : (kMaxSmem - fixed) / 256 * 256);
-    return launch_block_per_sm<few_down_kernel<F, M2, NT>>("few_down_kernel", ctas, fixed + l.panel_bytes, st, p, l);
-  };
-  if (rows <= 16) return down(std::integral_constant<int, 1>());
-  if (rows <= 32) return down(std::integral_constant<int, 2>());
-  return down(std::integral_constant<int, 4>());
+  const int64_t want = (int64_t)p.tokens * p.topk * down_row;
+  l.panel_bytes = (int)(want < down_room ? want : down_room / 256 * 256);
+  if (l.panel_bytes < RedShape<NT>::kBytes) l.panel_bytes = RedShape<NT>::kBytes;
+  return launch_block_per_sm<few_down_kernel<F, NT>>("few_down_kernel", ctas, DownShape<F>::kFixed + l.panel_bytes, st, p, l);
 }
 
 template <int F>

@@ -21,15 +21,22 @@
 namespace b200moe {
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kWarps = 16, kThreads = 32 * kWarps;
+constexpr int kTiles = 2;        // tiles of 16 rows that a warp takes at once
+constexpr int kRows = 16 * kTiles;
 constexpr int kMaxSlots = kFewMaxTopk * B200MOE_FEW_TOKENS;   // routed slots of a call
 
 enum FewFormat { kFewFp8, kFewFp4, kFewInt4Fine, kFewInt4 };   // Fine: groups of 32 or 64
 
+// A step of a warp is 64 bytes of its 32 rows.
 template <int F> struct FewShape {
-  static constexpr int kChunks = F == kFewFp8 ? 2 : 1;          // 16-byte pieces of a row per lane and step of 128 k
-  static constexpr int kStepBytes = F == kFewFp8 ? 128 : 64;    // of a row
-  static constexpr int kScaleWords = F == kFewFp8 || F == kFewInt4 ? 1 : F == kFewFp4 ? 2 : 3;   // of a row and step
+  static constexpr int kK = F == kFewFp8 ? 64 : 128;             // values of a row
+  static constexpr int kBlocks = kK / 32;                        // of the panel: a lane's eight values, two instructions
+  static constexpr int kScaleWords = F == kFewFp8 || F == kFewInt4 ? 1 : F == kFewFp4 ? 2 : 3;   // that hold a row's scales of a step
+  static constexpr int kScales = F == kFewFp8 || F == kFewInt4 ? 1 : 4;                          // of a row and step, in fp32
+  static constexpr int kSlot = kRows * (64 + 4 * kScaleWords);
+  static constexpr int kDepth = 3;
+  static constexpr int kRing = kDepth * kSlot + kRows * kScales * 4;
 };
 
 // ---- which experts a call uses ------------------------------------------------------
@@ -120,25 +127,17 @@ __device__ __forceinline__ void build_table(FewTable& t, const FewParams& p) {
 
 // ---- loads ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// `bytes` of the 16 or 4 come from memory, the rest are zeros.
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+// `bytes` of the four come from memory, the rest are zeros.
 __device__ __forceinline__ void copy4(uint32_t to, const void* from, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds4(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
+// Barrier of some of the block's warps.
+__device__ __forceinline__ void group_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // ---- conversions and products ------------------------------------------------------------
 __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t v) {
@@ -169,20 +168,19 @@ __device__ __forceinline__ void s4x8_to_h2(uint32_t w, uint32_t (&o)[4]) {
   }
 }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // ---- tokens and activations as float16 -------------------------------------------------
-// A panel holds rows of values in the order in which the lanes want them: per step of 128 k four blocks, a block
-// [row][4 lanes][8 values].  Where k sits: fp8 lanes hold 16 bytes of a row, 16 values; 4-bit formats hand a group of 32
-// values out to the four lanes, eight each.
+// A panel holds rows of values in the order in which the lanes want them: per step blocks of [row][4 lanes][8 values].
+// Where k sits: fp8 lanes hold 16 bytes of a row, 16 values; 4-bit formats hand a group of 32 values out to the four lanes,
+// eight each.
 template <int F>
 __device__ __forceinline__ uint32_t panel_at(int k8, int row, int rows) {   // k8: k / 8
-  const int s = k8 >> 4;
-  const int block = F == kFewFp8 ? ((k8 >> 2) & 2) | (k8 & 1) : (k8 >> 2) & 3;
+  const int block = F == kFewFp8 ? (k8 >> 3) * 2 + (k8 & 1) : k8 >> 2;
   const int t = F == kFewFp8 ? (k8 >> 1) & 3 : k8 & 3;
-  return (uint32_t)((((s * 4 + block) * rows + row) * 4 + t) * 16);
+  return (uint32_t)(((block * rows + row) * 4 + t) * 16);
 }
 
 enum FewSource { kFromBf16, kFromF16, kFromF32 };
@@ -253,177 +251,160 @@ __device__ __forceinline__ float row_top(const void* src, int source, int k, int
   return top;
 }
 // Warps of a row where a panel has `rows` of them.
-__device__ __forceinline__ int warps_per_row(int rows) { return rows == 1 ? 8 : rows == 2 ? 4 : rows <= 4 ? 2 : 1; }
+__device__ __forceinline__ int warps_per_row(int rows) { return rows == 1 ? 16 : rows == 2 ? 8 : rows <= 4 ? 4 : rows <= 8 ? 2 : 1; }
 
 // ---- weights: a warp's ring ------------------------------------------------------------
-// A step is 128 k of MT tiles of 16 rows.  fp8: a lane finds its own bytes again; 4 bits: a lane fetches 16 bytes of a row
-// (a group of 32) and reads a word of each of the row's four groups, whose places are swapped so that the eight rows of a
-// read fall on different banks.
-template <int F, int MT> struct FewRing {
-  static constexpr int kData = MT * 16 * FewShape<F>::kStepBytes;
-  static constexpr int kScales = MT * 16 * FewShape<F>::kScaleWords * 4;
-  static constexpr int kSlot = kData + kScales;
-};
+// fp8: a lane reads the bytes that it fetched.  4 bits: a lane fetches 16 bytes of a row, which is a group of 32 values, and
+// reads a word of each of the row's four groups; the groups' places are swapped so that the eight rows of a read fall on
+// different banks.  The scales of a row are fetched and made fp32 by one lane per row.
 
-// Where the rows of a tile lie, for one matrix of one expert.
+// The lane's part of 32 rows of one expert's matrix.
 struct FewRows {
-  const uint8_t* w;       // the expert's weights and scales
-  const uint8_t* s;
-  int64_t row_bytes, scale_bytes;   // of a row (fp8: of a row of blocks)
+  const uint8_t* w;          // its 16 bytes of step 0 in the first row that it fetches (row g of the first tile)
+  int64_t to[4];             // from there to rows g (0) and g + 8 of the first tile, g and g + 8 of the second
+  const uint8_t* s;          // first byte of the scales of the row that it looks after (row `lane` of the 32)
+  int tiles;                 // that there are
 };
-
+// The matrix as a whole.
+struct FewLayout {
+  int row_bytes, scale_bytes, group;
+  bool f16;
+  __device__ __forceinline__ FewLayout(const FewMatrix& m, int f, bool half) {
+    row_bytes = f == kFewFp8 ? m.k : m.k / 2;
+    scale_bytes = f == kFewFp8 ? m.k / 128 * 4 : f == kFewFp4 ? m.k / 32 : m.k / m.group * 2;
+    group = m.group;
+    f16 = half;
+  }
+};
+// Byte of a row's scales where those of step s begin.
 template <int F>
-__device__ __forceinline__ FewRows rows_of(const FewMatrix& m, int e) {
-  FewRows r;
-  const int64_t n = m.n, k = m.k;
-  r.row_bytes = F == kFewFp8 ? k : k / 2;
-  r.scale_bytes = F == kFewFp8 ? k / 128 * 4 : F == kFewFp4 ? k / 32 : k / m.group * 2;
-  r.w = reinterpret_cast<const uint8_t*>(m.w) + e * n * r.row_bytes;
-  r.s = reinterpret_cast<const uint8_t*>(m.scale) + e * (F == kFewFp8 ? n / 128 : n) * r.scale_bytes;
-  return r;
-}
-// First byte of the scales of step s within a row.
-template <int F>
-__device__ __forceinline__ int scale_offset(const FewMatrix& m, int s) {
-  return F == kFewFp8 ? 4 * s : F == kFewFp4 ? 4 * s : 128 * s / m.group * 2;
+__device__ __forceinline__ int scale_offset(const FewLayout& l, int s) {
+  return F == kFewFp8 ? s >> 1 << 2 : F == kFewFp4 ? 4 * s : (s * 128) / l.group * 2;
 }
 
-// Copies step s of the tiles into a slot.  row(i) gives row i of the 16 * MT, or -1 where there is none.
-template <int F, int MT, typename Row>
-__device__ __forceinline__ void copy_step(uint32_t slot, const FewRows& r, const FewMatrix& m, int s, Row row) {
+// Fetches step s into a slot.
+template <int F>
+__device__ __forceinline__ void copy_step(uint32_t slot, const FewRows& r, const FewLayout& l, int s) {
   using S = FewShape<F>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint8_t* w = r.w + s * 64;
+  // What is beyond a row of 4-bit codes stays what it was: any code is finite, and its tokens' values are zeros.
+  if (F == kFewFp8 || s * 64 + t * 16 < l.row_bytes) {
+    const uint32_t to = slot + (F == kFewFp8 ? lane * 16 : g * 64 + ((t ^ (g >> 1)) << 4));
 #pragma unroll
-  for (int i = 0; i < 2 * MT; ++i) {
-    const int n = row(i * 8 + g);
-#pragma unroll
-    for (int c = 0; c < S::kChunks; ++c) {
-      const int at = s * S::kStepBytes + (c * 4 + t) * 16;
-      const bool there = n >= 0 && at < r.row_bytes;
-      const uint32_t to = F == kFewFp8 ? slot + (i * 2 + c) * 512 + lane * 16 : slot + i * 512 + g * 64 + ((t ^ (g >> 1)) << 4);
-      copy16(to, there ? r.w + n * r.row_bytes + at : r.w, there ? 16 : 0);
-    }
-  }
-  const uint32_t sc = slot + FewRing<F, MT>::kData;
-  const int off = scale_offset<F>(m, s);
-#pragma unroll
-  for (int i = 0; i < (MT + 1) / 2; ++i) {
-    const int local = i * 32 + lane;
-    if (local < 16 * MT) {
-      const int n = row(local);
-      // words that hold the step's scales (they need not begin at one), as far as the row goes
-      const int64_t first = n < 0 ? 0 : (F == kFewFp8 ? n / 128 : n) * r.scale_bytes;
-      const int64_t begin = (first + off) & ~(int64_t)3;
-#pragma unroll
-      for (int w = 0; w < S::kScaleWords; ++w) {
-        const int64_t left = n < 0 ? 0 : first + r.scale_bytes - (begin + 4 * w);
-        copy4(sc + (local * S::kScaleWords + w) * 4, left > 0 ? r.s + begin + 4 * w : r.s, left >= 4 ? 4 : left > 0 ? (int)left : 0);
+    for (int i = 0; i < kTiles; ++i) {
+      if (i < r.tiles) {
+        copy16(to + i * 1024, w + r.to[2 * i]);
+        copy16(to + i * 1024 + 512, w + r.to[2 * i + 1]);
       }
     }
   }
-}
-
-// The step's scale of each group of 32 values (fp8, int4 with long groups: one for all) of local row i, which is row n.
-template <int F, int MT>
-__device__ __forceinline__ void step_scales(float (&o)[4], uint32_t slot, const FewRows& r, const FewMatrix& m, int s, int i, int n, bool f16) {
-  const uint32_t at = slot + FewRing<F, MT>::kData + i * FewShape<F>::kScaleWords * 4;
-  if (F == kFewFp8) { o[0] = __uint_as_float(lds4(at)); return; }
-  const int shift = (int)((n < 0 ? 0 : n * r.scale_bytes + scale_offset<F>(m, s)) & 3) * 8;
-  if (F == kFewFp4) {
-    // 2^(byte - 127): the byte is the exponent (0 gives zero for 2^-127, 255 infinity for NaN)
-    const uint32_t v = __funnelshift_r(lds4(at), lds4(at + 4), shift);
+  // the words that hold the step's scales (they need not begin at one), as far as the row goes
+  const int off = scale_offset<F>(l, s), skip = (int)((uintptr_t)r.s + off) & 3;
+  const uint8_t* from = r.s + off - skip;
+  const int left = l.scale_bytes - off + skip;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) o[q] = __uint_as_float(((v >> (8 * q)) & 255u) << 23);
-    return;
-  }
-  auto value = [&](uint32_t h) { return f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16); };
-  if (F == kFewInt4) { o[0] = value((lds4(at) >> shift) & 0xffffu); return; }
-  const uint32_t w0 = lds4(at), w1 = lds4(at + 4), w2 = lds4(at + 8);
-  const uint32_t lo = __funnelshift_r(w0, w1, shift), hi = __funnelshift_r(w1, w2, shift);
-  const bool fine = m.group == 32;
-  o[0] = value(lo & 0xffffu);
-  o[1] = fine ? value(lo >> 16) : o[0];
-  o[2] = value(fine ? hi & 0xffffu : lo >> 16);
-  o[3] = fine ? value(hi >> 16) : o[2];
+  for (int i = 0; i < S::kScaleWords; ++i)
+    copy4(slot + kRows * 64 + (lane * S::kScaleWords + i) * 4, left > 4 * i ? from + 4 * i : from, max(0, min(4, left - 4 * i)));
 }
 
-// acc += W x of one step.  b[j]: where this lane finds its token's values in the panel's first block of the step (0: no such
-// token); block: bytes from one block to the next.
-template <int F, int MT, int NT, typename Row>
-__device__ __forceinline__ void multiply_step(float (&acc)[MT][NT][4], uint32_t slot, const FewRows& r, const FewMatrix& m, int s, bool f16,
-                                              const uint32_t (&b)[NT], uint32_t block, Row row) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+// The scales of the step in the slot, of the lane's own row, as fp32.
+template <int F>
+__device__ __forceinline__ void spread_scales(float* to, const uint8_t* slot, const FewRows& r, const FewLayout& l, int s) {
+  using S = FewShape<F>;
+  const int lane = threadIdx.x & 31;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(slot + kRows * 64) + lane * S::kScaleWords;
   if constexpr (F == kFewFp8) {
-    float d[MT][NT][4] = {};
+    to[lane] = __uint_as_float(w[0]);
+  } else {
+    const int shift = ((int)((uintptr_t)r.s + scale_offset<F>(l, s)) & 3) * 8;
+    auto value = [&](uint32_t h) { return l.f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16); };
+    if constexpr (F == kFewFp4) {
+      // 2^(byte - 127): the byte is the exponent (0 gives zero for 2^-127, 255 infinity for NaN)
+      const uint32_t v = __funnelshift_r(w[0], w[1], shift);
+      reinterpret_cast<float4*>(to)[lane] = make_float4(__uint_as_float((v & 255u) << 23), __uint_as_float((v << 15) & 0x7f800000u),
+                                                        __uint_as_float((v << 7) & 0x7f800000u), __uint_as_float((v >> 1) & 0x7f800000u));
+    } else if constexpr (F == kFewInt4) {
+      to[lane] = value((w[0] >> shift) & 0xffffu);
+    } else {
+      const uint32_t lo = __funnelshift_r(w[0], w[1], shift), hi = __funnelshift_r(w[1], w[2], shift);
+      const float a = value(lo & 0xffffu), b = value(lo >> 16);
+      const bool fine = l.group == 32;
+      reinterpret_cast<float4*>(to)[lane] = make_float4(a, fine ? b : a, fine ? value(hi & 0xffffu) : b, fine ? value(hi >> 16) : b);
+    }
+  }
+}
+
+// Where a lane finds the values of its columns' tokens in the panel: the step's first block and the way to the next one.
+// Without a token: zeros, and no way.
+struct FewTokens {
+  const uint8_t* at;
+  uint32_t block;
+};
+
+// acc += W x of the step in the slot.
+template <int F, int NT>
+__device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const uint8_t* slot, const float* scales, int tiles,
+                                              const FewTokens (&x)[NT], int s) {
+  using S = FewShape<F>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint4 v[S::kBlocks][NT];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      uint4 x[2][NT];
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+    for (int q = 0; q < S::kBlocks; ++q) v[q][n] = *reinterpret_cast<const uint4*>(x[n].at + (s * S::kBlocks + q) * x[n].block);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) x[j][n] = b[n] ? lds16(b[n] + (2 * c + j) * block) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < kTiles; ++i) {
+    if (i >= tiles) break;
+    float d[NT][4] = {};
+    if constexpr (F == kFewFp8) {
+      const uint4 lo = *reinterpret_cast<const uint4*>(slot + i * 1024 + lane * 16), hi = *reinterpret_cast<const uint4*>(slot + i * 1024 + 512 + lane * 16);
+      const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const uint4 lo = lds16(slot + (4 * i + c) * 512 + lane * 16), hi = lds16(slot + (4 * i + 2 + c) * 512 + lane * 16);
-        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t a0 = e4m3x2_to_h2(wl[w] & 0xffffu), a2 = e4m3x2_to_h2(wl[w] >> 16);
+        const uint32_t a1 = e4m3x2_to_h2(wh[w] & 0xffffu), a3 = e4m3x2_to_h2(wh[w] >> 16);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t a0 = e4m3x2_to_h2(wl[w] & 0xffffu), a2 = e4m3x2_to_h2(wl[w] >> 16);
-          const uint32_t a1 = e4m3x2_to_h2(wh[w] & 0xffffu), a3 = e4m3x2_to_h2(wh[w] >> 16);
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            mma(d[i][n], a0, a1, a2, a3, w & 1 ? x[w >> 1][n].z : x[w >> 1][n].x, w & 1 ? x[w >> 1][n].w : x[w >> 1][n].y);
-        }
+        for (int n = 0; n < NT; ++n)
+          mma(d[n], a0, a1, a2, a3, w & 1 ? v[w >> 1][n].z : v[w >> 1][n].x, w & 1 ? v[w >> 1][n].w : v[w >> 1][n].y);
       }
     }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      float lo[4], hi[4];
-      step_scales<F, MT>(lo, slot, r, m, s, 16 * i + g, 0, f16);
-      step_scales<F, MT>(hi, slot, r, m, s, 16 * i + 8 + g, 0, f16);
+    float4 lo = {}, hi = {};
+    if constexpr (S::kScales == 4) {
+      lo = reinterpret_cast<const float4*>(scales)[16 * i + g];
+      hi = reinterpret_cast<const float4*>(scales)[16 * i + 8 + g];
+    } else {
+      lo.w = scales[16 * i + g];
+      hi.w = scales[16 * i + 8 + g];
+    }
+    auto add = [&](float a, float b) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        acc[i][n][0] = fmaf(lo[0], d[i][n][0], acc[i][n][0]);
-        acc[i][n][1] = fmaf(lo[0], d[i][n][1], acc[i][n][1]);
-        acc[i][n][2] = fmaf(hi[0], d[i][n][2], acc[i][n][2]);
-        acc[i][n][3] = fmaf(hi[0], d[i][n][3], acc[i][n][3]);
+        acc[i][n][0] = fmaf(a, d[n][0], acc[i][n][0]);
+        acc[i][n][1] = fmaf(a, d[n][1], acc[i][n][1]);
+        acc[i][n][2] = fmaf(b, d[n][2], acc[i][n][2]);
+        acc[i][n][3] = fmaf(b, d[n][3], acc[i][n][3]);
+        d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
       }
-    }
-  } else {
-    constexpr bool kOneScale = F == kFewInt4;
-    uint4 x[4][NT];
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) x[q][n] = b[n] ? lds16(b[n] + q * block) : make_uint4(0, 0, 0, 0);
-    const uint32_t at = slot + g * 64 + t * 4;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      float lo[4], hi[4];
-      step_scales<F, MT>(lo, slot, r, m, s, 16 * i + g, row(16 * i + g), f16);
-      step_scales<F, MT>(hi, slot, r, m, s, 16 * i + 8 + g, row(16 * i + 8 + g), f16);
-      float d[NT][4] = {};
+    };
+    if constexpr (F != kFewFp8) {
+      const uint8_t* w = slot + i * 1024 + g * 64 + t * 4;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
+        const int at = (q ^ (g >> 1)) << 4;
+        const uint32_t wl = *reinterpret_cast<const uint32_t*>(w + at), wh = *reinterpret_cast<const uint32_t*>(w + 512 + at);
         uint32_t al[4], ah[4];
-        const uint32_t wl = lds4(at + 2 * i * 512 + ((q ^ (g >> 1)) << 4)), wh = lds4(at + (2 * i + 1) * 512 + ((q ^ (g >> 1)) << 4));
         if constexpr (F == kFewFp4) { e2m1x8_to_h2(wl, al); e2m1x8_to_h2(wh, ah); }
         else { s4x8_to_h2(wl, al); s4x8_to_h2(wh, ah); }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma(d[n], al[0], ah[0], al[1], ah[1], x[q][n].x, x[q][n].y);
-          mma(d[n], al[2], ah[2], al[3], ah[3], x[q][n].z, x[q][n].w);
-          if (!kOneScale || q == 3) {
-            const int k = kOneScale ? 0 : q;
-            acc[i][n][0] = fmaf(lo[k], d[n][0], acc[i][n][0]);
-            acc[i][n][1] = fmaf(lo[k], d[n][1], acc[i][n][1]);
-            acc[i][n][2] = fmaf(hi[k], d[n][2], acc[i][n][2]);
-            acc[i][n][3] = fmaf(hi[k], d[n][3], acc[i][n][3]);
-            d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
-          }
+          mma(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
+          mma(d[n], al[2], ah[2], al[3], ah[3], v[q][n].z, v[q][n].w);
         }
+        if (S::kScales == 4 && q < 3) add(q == 0 ? lo.x : q == 1 ? lo.y : lo.z, q == 0 ? hi.x : q == 1 ? hi.y : hi.z);
       }
     }
+    add(lo.w, hi.w);
   }
 }
 
@@ -437,35 +418,43 @@ struct FewLaunch {
   bool f16;
 };
 
-template <int F, int MT, int NT> struct UpShape {
-  static constexpr int kDepth = 3;
-  static constexpr int kRed = kWarps * MT * NT * 4 * 32 * 4;
-  static constexpr int kFixed = (sizeof(FewTable) + 127) / 128 * 128 + 2 * kRed + 512 + kWarps * kDepth * FewRing<F, MT>::kSlot;
+constexpr int kTableBytes = (sizeof(FewTable) + 127) / 128 * 128;
+// Sums of the warps, for their owner to add up.
+template <int NT> struct RedShape { static constexpr int kWarpFloats = kTiles * NT * 4 * 32, kBytes = kWarps * kWarpFloats * 4; };
+template <int F, int NT> struct UpShape {
+  static constexpr int kFixed = kTableBytes + 512 + RedShape<NT>::kBytes + kWarps * FewShape<F>::kRing;
+};
+template <int F> struct DownShape {
+  static constexpr int kFixed = kTableBytes + 128 + kMaxSlots * 4 + kWarps * FewShape<F>::kRing;
 };
 
 // h[row] = act(W13 x + b13).  The features of all active experts, in pieces of eight (a tile's rows: eight gates and their
-// eight ups), are dealt out evenly to the blocks; the warps of a block take the steps of its tiles in turn and add their sums up
-// in shared memory.
-template <int F, int MT, int NT>
-__global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLaunch l) {
-  using S = UpShape<F, MT, NT>;
+// eight ups), are dealt out evenly to the blocks, and within a block to groups of warps; the warps of a group take the
+// steps of its tiles in turn and add their sums up in shared memory.
+template <int F, int NT>
+__global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLaunch launch) {
+  using S = FewShape<F>;
   extern __shared__ __align__(128) uint8_t smem[];
   FewTable& table = *reinterpret_cast<FewTable*>(smem);
-  float* const red = reinterpret_cast<float*>(smem + (sizeof(FewTable) + 127) / 128 * 128);
-  float* const inverse = red + 2 * S::kRed / 4;       // of the panel's rows' scales
-  float* const tops = inverse + 64;                    // (per warp)
+  float* const inverse = reinterpret_cast<float*>(smem + kTableBytes);   // of the panel's rows' scales
+  float* const tops = inverse + 32;                                       // (per warp)
+  uint8_t* const zeros = smem + kTableBytes + 256;                        // a token's values where there is no token
+  float* const red = reinterpret_cast<float*>(smem + kTableBytes + 512);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_at(red) + 2 * S::kRed + 512 + warp * S::kDepth * FewRing<F, MT>::kSlot;
-  uint8_t* const panel = smem + S::kFixed;
+  uint8_t* const ring = smem + kTableBytes + 512 + RedShape<NT>::kBytes + warp * S::kRing;
+  float* const scales = reinterpret_cast<float*>(ring + S::kDepth * S::kSlot);
+  uint8_t* const panel = smem + UpShape<F, NT>::kFixed;
   pdl_wait();
   pdl_trigger();
+  if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0;
   build_table<false>(table, p);
   const FewMatrix& m = p.w13;
-  const int steps = (p.hidden + 127) / 128, per_expert = p.inter / 8;
+  const FewLayout layout(m, F, launch.f16);
+  const int steps = (p.hidden + S::kK - 1) / S::kK, per_expert = p.inter / 8;
   const int64_t all = (int64_t)table.active * per_expert;
   const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
   const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
-  const int most = l.panel_bytes / (steps * 256);      // rows that the panel holds
+  const int most = launch.panel_bytes / (steps * S::kK * 2);      // rows that the panel holds
 
   for (int from = begin; from < end;) {
     // as many experts as have their tokens in the panel at once; one with more tokens than that goes through its
@@ -479,169 +468,220 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         to = min(end, (a + 1) * per_expert);
       }
     }
+    // Warps of a group: few where there are many tiles, as every tile's sums cost a barrier of the group; many where there
+    // are few, so that all have work.
+    int group = kWarps;
+    {
+      int least = 1 << 30;
+#pragma unroll
+      for (int w = 1; w <= kWarps; w *= 2) {
+        const int pieces = ((to - from) * w + kWarps - 1) / kWarps;
+        const int cost = (pieces + kTiles - 1) / kTiles * (4 * ((steps + w - 1) / w) + (w > 1 ? 4 : 1));
+        if (cost < least) { least = cost; group = w; }
+      }
+    }
+    const int groups = kWarps / group, mine_of = warp / group, member = warp % group;
+    const int my_from = from + (to - from) * mine_of / groups, my_to = from + (to - from) * (mine_of + 1) / groups;
+
     for (uint32_t rest = tokens; rest;) {
       uint32_t now = rest;
       while (__popc(now) > most) now &= ~(1u << (31 - __clz(now)));
       rest &= ~now;
       const int rows = __popc(now);
 
+      auto tile_rows = [&](int first) {       // of the tiles that begin with piece `first`
+        FewRows r;
+        const int a = first / per_expert, f = (first - a * per_expert) * 8;
+        const int64_t e = table.expert[a], rb = layout.row_bytes;
+        r.tiles = min(kTiles, min(per_expert - f / 8, my_to - first));
+        r.to[0] = 0;
+        r.to[1] = pairs ? rb : p.inter * rb;
+        r.to[2] = (pairs ? 16 : 8) * rb;
+        r.to[3] = r.to[1] + r.to[2];
+        r.w = reinterpret_cast<const uint8_t*>(m.w) + (e * m.n + (pairs ? 2 * (f + g) : f + g)) * rb + t * 16;
+        // (rows of a tile that is not there: any)
+        const int fs = f + (lane < 16 * r.tiles ? lane >> 4 : 0) * 8 + (lane & 7), up = (lane >> 3) & 1;
+        const int64_t n = pairs ? 2 * fs + up : fs + up * p.inter;
+        r.s = reinterpret_cast<const uint8_t*>(m.scale) + (F == kFewFp8 ? e * (m.n / 128) + n / 128 : e * m.n + n) * layout.scale_bytes;
+        return r;
+      };
       // the ring begins to fill
-      int tile = from, left = 0, s = warp;     // of the step that is copied next: its tile, the tile's pieces
-      FewRows where = {};
-      auto locate = [&]() {
-        const int e = table.expert[tile / per_expert];
-        where = rows_of<F>(m, e);
-        left = min(MT, min(per_expert - tile % per_expert, to - tile));
-      };
-      auto feature_row = [&](int first, int count, int i) {   // row i of a tile whose first piece is `first`
-        const int piece = i >> 4, f = (first + piece) * 8 + (i & 7);
-        return piece >= count ? -1 : pairs ? 2 * f + ((i >> 3) & 1) : f + ((i >> 3) & 1) * p.inter;
-      };
+      int next = my_from, s = member;     // of the step that is fetched next: its first piece
+      FewRows fetch = {};
+      if (next < my_to) fetch = tile_rows(next);
       auto settle = [&]() {
-        while (s >= steps && tile < to) {
+        while (s >= steps && next < my_to) {
           s -= steps;
-          tile += left;
-          if (tile < to) locate();
+          next += fetch.tiles;
+          if (next < my_to) fetch = tile_rows(next);
         }
       };
       auto copy_next = [&](int slot) {
-        if (tile < to) {
-          copy_step<F, MT>(ring + slot * FewRing<F, MT>::kSlot, where, m, s, [&](int i) { return feature_row(tile % per_expert, left, i); });
-          s += kWarps;
+        if (next < my_to) {
+          copy_step<F>(smem_at(ring) + slot * S::kSlot, fetch, layout, s);
+          s += group;
           settle();
         }
         copies_end();
       };
-      locate();
       settle();
 #pragma unroll
       for (int i = 0; i < S::kDepth; ++i) copy_next(i);
 
       // the panel
       {
-        const int parts = warps_per_row(rows), row = warp / parts, part = warp % parts;
-        const int source = l.f16 ? kFromF16 : kFromBf16, k8 = steps * 16;
-        for (int r0 = 0; r0 < rows; r0 += kWarps / parts) {
-          const int r = r0 + row;
-          uint32_t left_tokens = now;
-          for (int i = 0; i < r && i < 32; ++i) left_tokens &= left_tokens - 1;
-          const uint8_t* x = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)(r < rows ? __ffs(left_tokens) - 1 : 0) * p.hidden * 2;
-          float top = r < rows ? row_top(x, source, p.hidden, 0, k8, part, parts) : 0.f;
-          if (parts > 1) {
-            if (lane == 0) tops[warp] = top;
-            __syncthreads();
-            for (int i = 0; i < parts; ++i) top = max_nan(top, tops[row * parts + i]);
-          }
-          if (r < rows) {
-            float inv;
-            const float scale = row_scale(top, inv);
-            if (lane == 0 && part == 0) inverse[r] = inv;
-            convert_row<F>(panel, r, rows, x, source, p.hidden, 0, k8, scale, part, parts);
-          }
+        const int parts = warps_per_row(rows), row = warp / parts, part = warp % parts;   // (a round of the rows is all of them)
+        const int source = launch.f16 ? kFromF16 : kFromBf16, k8 = steps * (S::kK / 8);
+        uint32_t left_tokens = now;
+        for (int i = 0; i < row; ++i) left_tokens &= left_tokens - 1;
+        const bool there = row < rows;
+        const uint8_t* x = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)(there ? __ffs(left_tokens) - 1 : 0) * p.hidden * 2;
+        float top = there ? row_top(x, source, p.hidden, 0, k8, part, parts) : 0.f;
+        if (parts > 1) {
+          if (lane == 0) tops[warp] = top;
+          __syncthreads();
+          for (int i = 0; i < parts; ++i) top = max_nan(top, tops[row * parts + i]);
+        }
+        if (there) {
+          float inv;
+          const float scale = row_scale(top, inv);
+          if (lane == 0 && part == 0) inverse[row] = inv;
+          convert_row<F>(panel, row, rows, x, source, p.hidden, 0, k8, scale, part, parts);
         }
         __syncthreads();
       }
 
-      int slot = 0, turn = 0, cs = warp, count = 0;
-      for (int first = from; first < to; first += count, ++turn) {
+      int slot = 0, cs = member;
+      for (int first = my_from; first < my_to;) {
+        const FewRows r = tile_rows(first);
         const int a = first / per_expert;
-        const FewRows rows_here = rows_of<F>(m, table.expert[a]);
-        count = min(MT, min(per_expert - first % per_expert, to - first));
         const uint32_t mine = table.tokens[a] & now;
-        const uint32_t block = rows * 64;
-        uint32_t b[NT];
+        FewTokens x[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          b[n] = (mine >> (8 * n + g)) & 1 ? smem_at(panel) + rank_below(now, 8 * n + g) * 64 + t * 16 : 0;
-        float acc[MT][NT][4] = {};
-        for (; cs < steps; cs += kWarps) {
+        for (int n = 0; n < NT; ++n) {
+          const bool used = (mine >> (8 * n + g)) & 1;
+          x[n].at = used ? panel + rank_below(now, 8 * n + g) * 64 + t * 16 : zeros;
+          x[n].block = used ? rows * 64 : 0;
+        }
+        float acc[kTiles][NT][4] = {};
+        for (; cs < steps; cs += group) {
           copies_wait<S::kDepth - 1>();
+          spread_scales<F>(scales, ring + slot * S::kSlot, r, layout, cs);
           __syncwarp();
-          uint32_t bs[NT];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) bs[n] = b[n] ? b[n] + cs * 4 * block : 0;
-          multiply_step<F, MT, NT>(acc, ring + slot * FewRing<F, MT>::kSlot, rows_here, m, cs, l.f16, bs, block,
-                                   [&](int i) { return feature_row(first % per_expert, count, i); });
+          multiply_step<F, NT>(acc, ring + slot * S::kSlot, scales, r.tiles, x, cs);
           __syncwarp();
           copy_next(slot);
           slot = slot + 1 == S::kDepth ? 0 : slot + 1;
         }
         cs -= steps;
-        float* const to_red = red + (turn & 1) * (S::kRed / 4);
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) to_red[((warp * MT + i) * NT + n) * 128 + c * 32 + lane] = acc[i][n][c];
-        __syncthreads();   // (two buffers: what the tile after next writes is read before the next one's barrier)
-        for (int j = tid; j < MT * NT * 64; j += kThreads) {
-          const int l2 = j & 31, c = (j >> 5) & 1, n = (j >> 6) % NT, i = (j >> 6) / NT;
-          const int token = 8 * n + 2 * (l2 & 3) + c;
-          if (i >= count || !((mine >> token) & 1)) continue;
-          float gate = 0.f, up = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            gate += to_red[((w * MT + i) * NT + n) * 128 + c * 32 + l2];
-            up += to_red[((w * MT + i) * NT + n) * 128 + (c + 2) * 32 + l2];
-          }
-          const float inv = inverse[rank_below(now, token)];
-          const int f = (first % per_expert + i) * 8 + (l2 >> 2);
+        auto finish = [&](int i, int col, int f_in_tile, float gate, float up) {
+          if (i >= r.tiles || !((mine >> col) & 1)) return;
+          const float inv = inverse[rank_below(now, col)];
+          const int f = (first - a * per_expert + i) * 8 + f_in_tile;
           gate *= inv;
           up *= inv;
           if (m.bias) {
             const int64_t at = (int64_t)table.expert[a] * m.n;
-            gate += load16(m.bias, at + (pairs ? 2 * f : f), l.f16);
-            up += load16(m.bias, at + (pairs ? 2 * f + 1 : p.inter + f), l.f16);
+            gate += load16(m.bias, at + (pairs ? 2 * f : f), launch.f16);
+            up += load16(m.bias, at + (pairs ? 2 * f + 1 : p.inter + f), launch.f16);
           }
-          p.h[(int64_t)(table.first_row[a] + rank_below(table.tokens[a], token)) * p.inter + f] = gated(p, gate, up);
+          p.h[(int64_t)(table.first_row[a] + rank_below(table.tokens[a], col)) * p.inter + f] = gated(p, gate, up);
+        };
+        if (group == 1) {
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) finish(i, 8 * n + 2 * t + c, g, acc[i][n][c], acc[i][n][c + 2]);
+        } else {
+          constexpr int kWarpFloats = RedShape<NT>::kWarpFloats;
+          float* const to_red = red + warp * kWarpFloats + lane;
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) to_red[((i * NT + n) * 4 + c) * 32] = acc[i][n][c];
+          group_sync(1 + mine_of, group * 32);
+          for (int j = member * 32 + lane; j < kTiles * NT * 64; j += group * 32) {
+            const int l2 = j & 31, c = (j >> 5) & 1, n = (j >> 6) % NT, i = (j >> 6) / NT;
+            float gate = 0.f, up = 0.f;
+            const float* from_red = red + (warp - member) * kWarpFloats + ((i * NT + n) * 4 + c) * 32 + l2;
+            for (int w = 0; w < group; ++w) {
+              gate += from_red[w * kWarpFloats];
+              up += from_red[w * kWarpFloats + 64];
+            }
+            finish(i, 8 * n + 2 * (l2 & 3) + c, l2 >> 2, gate, up);
+          }
+          group_sync(1 + mine_of, group * 32);   // the sums' place is free again
         }
+        first += r.tiles;
       }
       copies_wait<0>();
-      __syncthreads();   // panel, ring and sums are free again
+      __syncthreads();   // the panel is free again
     }
     from = to;
   }
 }
 
-template <int F, int MT, int NT> struct DownShape {
-  static constexpr int kDepth = MT > 2 ? 2 : 3;
-  static constexpr int kRed = kWarps * MT * NT * 4 * 32 * 4;
-  static constexpr int kFixed = (sizeof(FewTable) + 127) / 128 * 128 + kRed + kMaxSlots * 4 + 128 + kWarps * kDepth * FewRing<F, MT>::kSlot;
-};
-
-// out = sum over experts of weight * (W2 h + b2).  A block has up to 16 * MT rows of W2 and goes through all active experts
-// with them; its warps take the steps in turn.
-template <int F, int MT, int NT>
-__global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewLaunch l) {
-  using S = DownShape<F, MT, NT>;
+// out = sum over experts of weight * (W2 h + b2).  A block has some rows of W2 and goes through all active experts with them;
+// its warps take the steps in turn, in two halves with half of the rows each where there are more than 32.
+template <int F, int NT>
+__global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewLaunch launch) {
+  using S = FewShape<F>;
   extern __shared__ __align__(128) uint8_t smem[];
   FewTable& table = *reinterpret_cast<FewTable*>(smem);
-  float* const red = reinterpret_cast<float*>(smem + (sizeof(FewTable) + 127) / 128 * 128);
-  float* const coef = red + S::kRed / 4;               // of the panel's rows: routing weight and the inverse of the scale
-  float* const tops = coef + kMaxSlots;                // (per warp)
+  float* const tops = reinterpret_cast<float*>(smem + kTableBytes);       // (per warp)
+  uint8_t* const zeros = smem + kTableBytes + 64;
+  float* const coef = reinterpret_cast<float*>(smem + kTableBytes + 128);   // of the panel's rows: routing weight and the inverse of the scale
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_at(red) + S::kRed + kMaxSlots * 4 + 128 + warp * S::kDepth * FewRing<F, MT>::kSlot;
-  uint8_t* const panel = smem + S::kFixed;
+  uint8_t* const ring = smem + kTableBytes + 128 + kMaxSlots * 4 + warp * S::kRing;
+  float* const scales = reinterpret_cast<float*>(ring + S::kDepth * S::kSlot);
+  uint8_t* const panel = smem + DownShape<F>::kFixed;
+  float* const red = reinterpret_cast<float*>(panel);                     // (after the last panel)
   // What routed the tokens was complete before the kernel ahead of this one let it start.
+  if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0;
   build_table<true>(table, p);
   const FewMatrix& m = p.w2;
-  const int steps = (p.inter + 127) / 128, total = table.active * steps;
+  const FewLayout layout(m, F, launch.f16);
+  const int steps = (p.inter + S::kK - 1) / S::kK;
   const int row_begin = (int)((int64_t)p.hidden * blockIdx.x / gridDim.x), row_end = (int)((int64_t)p.hidden * (blockIdx.x + 1) / gridDim.x);
-  const int room = l.panel_bytes / 256;                // rows times steps that the panel holds
+  const int room = launch.panel_bytes / (S::kK * 2);                      // rows times steps that the panel holds
   bool waited = false;
 
-  for (int r0 = row_begin; r0 < row_end || !waited; r0 += 16 * MT) {
-    auto matrix_row = [&](int i) { return r0 + i < row_end ? r0 + i : -1; };
-    int at = warp;                 // the step that is copied next, counted over all experts
+  for (int r0 = row_begin; r0 < row_end || !waited; r0 += 2 * kRows) {
+    const int block_rows = max(0, min(2 * kRows, row_end - r0));
+    const int halves = block_rows > kRows ? 2 : 1, group = kWarps / halves, half = warp / group, member = warp % group;
+    const int my_r0 = r0 + block_rows * half / halves, my_rows = block_rows * (half + 1) / halves - block_rows * half / halves;
+    auto expert_rows = [&](int a) {
+      FewRows r;
+      const int64_t e = table.expert[a], rb = layout.row_bytes;
+      r.tiles = (my_rows + 15) / 16;
+      r.w = reinterpret_cast<const uint8_t*>(m.w) + (e * m.n + my_r0) * rb + t * 16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.to[i] = min(8 * i + g, my_rows - 1) * rb;   // (what a tile has not got is the last row again)
+      const int64_t n = my_r0 + min(lane, my_rows - 1);
+      r.s = reinterpret_cast<const uint8_t*>(m.scale) + (F == kFewFp8 ? e * (m.n / 128) + n / 128 : e * m.n + n) * layout.scale_bytes;
+      return r;
+    };
+    int fetch_a = 0, s = member;     // of the step that is fetched next
+    FewRows fetch = {};
+    auto settle = [&]() {
+      bool moved = false;
+      while (s >= steps && fetch_a < table.active) { s -= steps; ++fetch_a; moved = true; }
+      if (moved && fetch_a < table.active) fetch = expert_rows(fetch_a);
+    };
     auto copy_next = [&](int slot) {
-      if (at < total) {
-        const int a = at / steps;
-        copy_step<F, MT>(ring + slot * FewRing<F, MT>::kSlot, rows_of<F>(m, table.expert[a]), m, at - a * steps, matrix_row);
-        at += kWarps;
+      if (fetch_a < table.active && my_rows > 0) {
+        copy_step<F>(smem_at(ring) + slot * S::kSlot, fetch, layout, s);
+        s += group;
+        settle();
       }
       copies_end();
     };
+    if (table.active > 0 && my_rows > 0) fetch = expert_rows(0);
+    settle();
 #pragma unroll
     for (int i = 0; i < S::kDepth; ++i) copy_next(i);
     if (!waited) {
@@ -649,8 +689,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       pdl_trigger();
       waited = true;
     }
-    float out[MT][NT][4] = {};
-    int slot = 0, pos = warp;
+    float out[kTiles][NT][4] = {};
+    int slot = 0, pos = member;
     for (int a0 = 0, s0 = 0; a0 < table.active;) {
       // how far the panel reaches: whole experts, then as many steps of the next one as there is room for (at least one)
       int a1 = a0, s1 = s0, free = room;
@@ -667,11 +707,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       const int row0 = table.first_row[a0], rows = table.first_row[last + 1] - row0;
       {
         const int parts = warps_per_row(rows), row = warp / parts, part = warp % parts;
-        for (int q0 = 0; q0 < rows; q0 += kWarps / parts) {
+        for (int q0 = 0; q0 < rows; q0 += kWarps / parts) {   // (once where a row has several warps)
           const int r = row0 + q0 + row;
           const bool there = q0 + row < rows;
           const int a = there ? table.row_expert[r] : a0;
-          const int k8_0 = a == a0 ? s0 * 16 : 0, k8_1 = (a == a1 ? s1 : steps) * 16;
+          const int k8_0 = (a == a0 ? s0 : 0) * (S::kK / 8), k8_1 = (a == a1 ? s1 : steps) * (S::kK / 8);
           const float* h = p.h + (int64_t)(there ? r : 0) * p.inter;
           float top = there ? row_top(h, kFromF32, p.inter, k8_0, k8_1, part, parts) : 0.f;
           if (parts > 1) {
@@ -685,77 +725,81 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
             if (lane == 0 && part == 0) coef[q0 + row] = table.weight[r] * inv;
             // rows of earlier experts in the panel: the first one's with the steps that it has there
             const int before = a == a0 ? 0 : (table.first_row[a0 + 1] - row0) * (steps - s0) + (table.first_row[a] - table.first_row[a0 + 1]) * steps;
-            convert_row<F>(panel + (int64_t)before * 256, r - table.first_row[a], table.first_row[a + 1] - table.first_row[a], h, kFromF32, p.inter,
-                           k8_0, k8_1, scale, part, parts);
+            convert_row<F>(panel + (int64_t)before * (S::kK * 2), r - table.first_row[a], table.first_row[a + 1] - table.first_row[a], h,
+                           kFromF32, p.inter, k8_0, k8_1, scale, part, parts);
           }
         }
         __syncthreads();
       }
-      uint32_t base = smem_at(panel);
+      const uint8_t* base = panel;
       for (int a = a0; a <= last; ++a) {
         const int first = a == a0 ? s0 : 0, stop = a == a1 ? s1 : steps, n_rows = table.first_row[a + 1] - table.first_row[a];
-        const uint32_t mine = table.tokens[a], block = n_rows * 64;
-        const FewRows where = rows_of<F>(m, table.expert[a]);
-        uint32_t b[NT];
+        const uint32_t mine = table.tokens[a];
+        if (pos < a * steps + stop && my_rows > 0) {
+          const FewRows r = expert_rows(a);
+          FewTokens x[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) b[n] = (mine >> (8 * n + g)) & 1 ? base + rank_below(mine, 8 * n + g) * 64 + t * 16 : 0;
-        float acc[MT][NT][4] = {};
-        for (; pos < a * steps + stop; pos += kWarps) {
-          copies_wait<S::kDepth - 1>();
-          __syncwarp();
-          const int s = pos - a * steps;
-          uint32_t bs[NT];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) bs[n] = b[n] ? b[n] + (s - first) * 4 * block : 0;
-          multiply_step<F, MT, NT>(acc, ring + slot * FewRing<F, MT>::kSlot, where, m, s, l.f16, bs, block, matrix_row);
-          __syncwarp();
-          copy_next(slot);
-          slot = slot + 1 == S::kDepth ? 0 : slot + 1;
-        }
-        base += (stop - first) * 4 * block;
-        // (columns of tokens without this expert are left out: a weight that is not finite would get into them)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int token = 8 * n + 2 * t + c;
-            if (!((mine >> token) & 1)) continue;
-            const float w = coef[table.first_row[a] - row0 + rank_below(mine, token)];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              out[i][n][c] = fmaf(w, acc[i][n][c], out[i][n][c]);
-              out[i][n][c + 2] = fmaf(w, acc[i][n][c + 2], out[i][n][c + 2]);
-            }
+          for (int n = 0; n < NT; ++n) {
+            const bool used = (mine >> (8 * n + g)) & 1;
+            x[n].at = used ? base + rank_below(mine, 8 * n + g) * 64 + t * 16 : zeros;
+            x[n].block = used ? n_rows * 64 : 0;
           }
+          float acc[kTiles][NT][4] = {};
+          for (; pos < a * steps + stop; pos += group) {
+            copies_wait<S::kDepth - 1>();
+            spread_scales<F>(scales, ring + slot * S::kSlot, r, layout, pos - a * steps);
+            __syncwarp();
+            multiply_step<F, NT>(acc, ring + slot * S::kSlot, scales, r.tiles, x, pos - a * steps - first);
+            __syncwarp();
+            copy_next(slot);
+            slot = slot + 1 == S::kDepth ? 0 : slot + 1;
+          }
+          // (columns of tokens without this expert are left out: a weight that is not finite would get into them)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int token = 8 * n + 2 * t + c;
+              if (!((mine >> token) & 1)) continue;
+              const float w = coef[table.first_row[a] - row0 + rank_below(mine, token)];
+#pragma unroll
+              for (int i = 0; i < kTiles; ++i) {
+                out[i][n][c] = fmaf(w, acc[i][n][c], out[i][n][c]);
+                out[i][n][c + 2] = fmaf(w, acc[i][n][c + 2], out[i][n][c + 2]);
+              }
+            }
+        }
+        base += (stop - first) * n_rows * (S::kK * 2);
       }
       a0 = a1;
       s0 = s1;
       __syncthreads();   // the panel is free again
     }
+    constexpr int kWarpFloats = RedShape<NT>::kWarpFloats;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < kTiles; ++i)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) red[((warp * MT + i) * NT + n) * 128 + c * 32 + lane] = out[i][n][c];
+        for (int c = 0; c < 4; ++c) red[warp * kWarpFloats + ((i * NT + n) * 4 + c) * 32 + lane] = out[i][n][c];
     copies_wait<0>();
     __syncthreads();
-    for (int j = tid; j < 16 * MT * 8 * NT; j += kThreads) {
+    for (int j = tid; j < 2 * kRows * p.tokens; j += kThreads) {
       // consecutive threads, consecutive features of a token
-      const int row = j % (16 * MT), token = j / (16 * MT);
-      if (r0 + row >= row_end || token >= p.tokens) continue;
-      const int at_red = (((row >> 4) * NT) + (token >> 3)) * 128 + (((row >> 3) & 1) * 2 + (token & 1)) * 32 + (row & 7) * 4 + ((token & 7) >> 1);
+      const int row = j % (2 * kRows), token = j / (2 * kRows);
+      if (row >= block_rows) continue;
+      const int h = halves == 2 && row >= block_rows / 2, i = row - (h ? block_rows / 2 : 0);   // of that half
+      const int at = (((i >> 4) * NT + (token >> 3)) * 4 + ((i >> 3) & 1) * 2 + (token & 1)) * 32 + (i & 7) * 4 + ((token & 7) >> 1);
       float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += red[w * MT * NT * 128 + at_red];
+      for (int w = 0; w < group; ++w) v += red[(h * group + w) * kWarpFloats + at];
       if (m.bias) {
         for (int k = 0; k < p.topk; ++k) {
           const int a = table.slot_expert[token * p.topk + k];
-          if (a >= 0) v = fmaf(p.weights[token * p.topk + k], load16(m.bias, (int64_t)table.expert[a] * m.n + r0 + row, l.f16), v);
+          if (a >= 0) v = fmaf(p.weights[token * p.topk + k], load16(m.bias, (int64_t)table.expert[a] * m.n + r0 + row, launch.f16), v);
         }
       }
       const int64_t to = (int64_t)token * p.hidden + r0 + row;
-      if (l.f16) reinterpret_cast<__half*>(p.out)[to] = __float2half_rn(v);
+      if (launch.f16) reinterpret_cast<__half*>(p.out)[to] = __float2half_rn(v);
       else reinterpret_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(v);
     }
     __syncthreads();

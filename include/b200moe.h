@@ -636,7 +636,7 @@ typedef struct {
   float clamp_limit;          /* >0: gate = min(gate, L), up = clamp(up, +-L) first    */
   int max_ctas;               /* >0: at most this many CTAs; 0: one per SM            */
 } b200moe_few_tokens_args;
-size_t b200moe_few_tokens_workspace_bytes(int num_tokens, int topk, int inter);
+size_t b200moe_few_tokens_workspace_bytes(int num_tokens, int topk, int hidden, int inter);
 int b200moe_few_tokens_layer(const b200moe_few_tokens_args* args, b200moe_stream stream);
 
 /* ------------------------------------------------------------------------- */

@@ -117,17 +117,36 @@ int launch_block_per_sm(const char* name, int grid, int smem, cudaStream_t st, c
   return B200MOE_OK;
 }
 
+// Where things are in the workspace: h, then what the blocks of the two kernels tell one another.
+struct FewWorkspace {
+  size_t top, arrived, part, bytes;
+  FewWorkspace(int64_t tokens, int64_t topk, int64_t hidden, int64_t inter) {
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    top = up(tokens * topk * inter * sizeof(float));
+    arrived = top + up((size_t)kFewMaxBlocks * tokens * topk * sizeof(float));
+    part = arrived + kFewMaxColumns * sizeof(uint32_t);
+    bytes = part + up((size_t)splits(hidden, kFewMaxBlocks) * tokens * hidden * sizeof(float));
+  }
+  // Shares of the second kernel's steps: as many as make `ctas` blocks with up to 64 rows each.
+  static int splits(int64_t hidden, int ctas) {
+    const int64_t n = (int64_t)ctas * kRows / hidden;
+    return n < 1 ? 1 : n > ctas ? ctas : (int)n;
+  }
+};
+
 template <int F, int NT>
 int launch_nk(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   constexpr int k = FewShape<F>::kK, up_room = kMaxSmem - UpShape<F, NT>::kFixed, down_room = kMaxSmem - DownShape<F>::kFixed;
   const int up_row = (p.hidden + k - 1) / k * k * 2, down_row = (p.inter + k - 1) / k * k * 2;
   l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
+  l.up_blocks = ctas;
+  l.splits = FewWorkspace::splits(p.hidden, ctas);
   int rc = launch_block_per_sm<few_up_kernel<F, NT>>("few_up_kernel", ctas, UpShape<F, NT>::kFixed + l.panel_bytes, st, p, l);
   if (rc != B200MOE_OK) return rc;
   const int64_t want = (int64_t)p.tokens * p.topk * down_row;
   l.panel_bytes = (int)(want < down_room ? want : down_room / 256 * 256);
   if (l.panel_bytes < RedShape<NT>::kBytes) l.panel_bytes = RedShape<NT>::kBytes;
-  return launch_block_per_sm<few_down_kernel<F, NT>>("few_down_kernel", ctas, DownShape<F>::kFixed + l.panel_bytes, st, p, l);
+  return launch_block_per_sm<few_down_kernel<F, NT>>("few_down_kernel", ctas / l.splits * l.splits, DownShape<F>::kFixed + l.panel_bytes, st, p, l);
 }
 
 template <int F>
@@ -170,9 +189,9 @@ int check_matrix(const b200moe_few_tokens_args* a, b200moe_weight_format f, cons
 
 using namespace b200moe;
 
-extern "C" size_t b200moe_few_tokens_workspace_bytes(int num_tokens, int topk, int inter) {
-  if (num_tokens <= 0 || topk <= 0 || inter <= 0) return 0;
-  return (size_t)num_tokens * topk * inter * sizeof(float);
+extern "C" size_t b200moe_few_tokens_workspace_bytes(int num_tokens, int topk, int hidden, int inter) {
+  if (num_tokens <= 0 || topk <= 0 || hidden <= 0 || inter <= 0) return 0;
+  return FewWorkspace(num_tokens, topk, hidden, inter).bytes;
 }
 
 extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200moe_stream stream) {
@@ -191,7 +210,7 @@ extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200mo
   B200_CHECK_ARG(a->w13_format == a->w2_format, "few_tokens_layer: w13 and w2 must have the same format");
   if (a->num_tokens == 0) return B200MOE_OK;
   B200_CHECK_ARG(a->x && a->topk_ids && a->topk_weights && a->out, "few_tokens_layer: null pointer");
-  const size_t need = b200moe_few_tokens_workspace_bytes(a->num_tokens, a->topk, a->inter);
+  const size_t need = b200moe_few_tokens_workspace_bytes(a->num_tokens, a->topk, a->hidden, a->inter);
   if (a->workspace == nullptr || a->workspace_bytes < need || ((uintptr_t)a->workspace & 15) != 0)
     return fail(B200MOE_E_WORKSPACE, "few_tokens_layer: needs %zu bytes of 16-byte aligned workspace", need);
   FewParams p = {};
@@ -202,10 +221,15 @@ extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200mo
   p.act = a->activation; p.alpha = a->act_alpha; p.limit = a->act_limit; p.clamp = a->clamp_limit;
   p.w13 = {a->w13, a->w13_scale, a->w13_bias, a->w13_format, a->w13_group, 2 * a->inter, a->hidden};
   p.w2 = {a->w2, a->w2_scale, a->w2_bias, a->w2_format, a->w2_group, a->hidden, a->inter};
-  const int ctas = a->max_ctas > 0 && a->max_ctas < sm_count() ? a->max_ctas : sm_count();
+  int ctas = a->max_ctas > 0 && a->max_ctas < sm_count() ? a->max_ctas : sm_count();
+  if (ctas > kFewMaxBlocks) ctas = kFewMaxBlocks;
   if (takes_nk(p)) {
     FewLaunch l = {};
     l.f16 = a->dtype == B200MOE_F16;
+    const FewWorkspace ws(p.tokens, p.topk, p.hidden, p.inter);
+    l.top = (float*)((char*)a->workspace + ws.top);
+    l.arrived = (uint32_t*)((char*)a->workspace + ws.arrived);
+    l.part = (float*)((char*)a->workspace + ws.part);
     if (p.w13.format == B200MOE_W_FP8_BLOCK_NK) return launch_nk<kFewFp8>(p, l, ctas, as_stream(stream));
     if (p.w13.format == B200MOE_W_MXFP4_NK) return launch_nk<kFewFp4>(p, l, ctas, as_stream(stream));
     const bool fine = p.w13.group < 128 || p.w2.group < 128;

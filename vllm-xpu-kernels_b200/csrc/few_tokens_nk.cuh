@@ -21,19 +21,21 @@
 namespace b200moe {
 namespace {
 
-constexpr int kWarps = 16, kThreads = 32 * kWarps;
-constexpr int kTiles = 2;        // tiles of 16 rows that a warp takes at once
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kTiles = 4;        // tiles of 16 rows that a warp takes at once
 constexpr int kRows = 16 * kTiles;
+constexpr int kFewMaxBlocks = 160;      // of a kernel (one per SM)
+constexpr int kFewMaxColumns = kFewMaxBlocks;
 constexpr int kMaxSlots = kFewMaxTopk * B200MOE_FEW_TOKENS;   // routed slots of a call
 
 enum FewFormat { kFewFp8, kFewFp4, kFewInt4Fine, kFewInt4 };   // Fine: groups of 32 or 64
 
-// A step of a warp is 64 bytes of its 32 rows.
+// A step of a warp is 64 bytes of its 64 rows.
 template <int F> struct FewShape {
   static constexpr int kK = F == kFewFp8 ? 64 : 128;             // values of a row
   static constexpr int kBlocks = kK / 32;                        // of the panel: a lane's eight values, two instructions
   static constexpr int kScaleWords = F == kFewFp8 || F == kFewInt4 ? 1 : F == kFewFp4 ? 2 : 3;   // that hold a row's scales of a step
-  static constexpr int kScales = F == kFewFp8 || F == kFewInt4 ? 1 : 4;                          // of a row and step, in fp32
+  static constexpr int kScales = F == kFewFp8 ? 0 : F == kFewInt4 ? 1 : 4;                       // of a row and step, made fp32 (fp8: are so)
   static constexpr int kSlot = kRows * (64 + 4 * kScaleWords);
   static constexpr int kDepth = 3;
   static constexpr int kRing = kDepth * kSlot + kRows * kScales * 4;
@@ -140,9 +142,11 @@ template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("c
 __device__ __forceinline__ void group_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // ---- conversions and products ------------------------------------------------------------
-__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t v) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)v, __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// Four e4m3 codes of a word -> float16 pairs (0,1) (2,3).  (One instruction each; through the header's function, which takes
+// and returns halves of registers, seven for the two.)
+__device__ __forceinline__ void e4m3x4_to_h2(uint32_t w, uint32_t& a, uint32_t& b) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(a), "=r"(b) : "r"(w));
 }
 // Eight e2m1 codes of a word -> float16 pairs (0,1) (2,3) (4,5) (6,7).
 __device__ __forceinline__ void e2m1x8_to_h2(uint32_t w, uint32_t (&o)[4]) {
@@ -170,6 +174,12 @@ __device__ __forceinline__ void s4x8_to_h2(uint32_t w, uint32_t (&o)[4]) {
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The first product of a sum.
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // ---- tokens and activations as float16 -------------------------------------------------
@@ -251,19 +261,19 @@ __device__ __forceinline__ float row_top(const void* src, int source, int k, int
   return top;
 }
 // Warps of a row where a panel has `rows` of them.
-__device__ __forceinline__ int warps_per_row(int rows) { return rows == 1 ? 16 : rows == 2 ? 8 : rows <= 4 ? 4 : rows <= 8 ? 2 : 1; }
+__device__ __forceinline__ int warps_per_row(int rows) { return rows == 1 ? 8 : rows == 2 ? 4 : rows <= 4 ? 2 : 1; }
 
 // ---- weights: a warp's ring ------------------------------------------------------------
 // fp8: a lane reads the bytes that it fetched.  4 bits: a lane fetches 16 bytes of a row, which is a group of 32 values, and
 // reads a word of each of the row's four groups; the groups' places are swapped so that the eight rows of a read fall on
 // different banks.  The scales of a row are fetched and made fp32 by one lane per row.
 
-// The lane's part of 32 rows of one expert's matrix.
+// The lane's part of 64 rows of one expert's matrix.
 struct FewRows {
-  const uint8_t* w;          // its 16 bytes of step 0 in the first row that it fetches (row g of the first tile)
-  int64_t to[4];             // from there to rows g (0) and g + 8 of the first tile, g and g + 8 of the second
-  const uint8_t* s;          // first byte of the scales of the row that it looks after (row `lane` of the 32)
-  int tiles;                 // that there are
+  const uint8_t* w;              // its 16 bytes of step 0 in row g (lane = 4 g + t)
+  int64_t to[2 * kTiles];        // from there to rows g + 8 i
+  const uint8_t* s[kTiles / 2];  // first byte of the scales of the rows that it looks after, lane + 32 i
+  int tiles;                     // that there are
 };
 // The matrix as a whole.
 struct FewLayout {
@@ -293,44 +303,48 @@ __device__ __forceinline__ void copy_step(uint32_t slot, const FewRows& r, const
     const uint32_t to = slot + (F == kFewFp8 ? lane * 16 : g * 64 + ((t ^ (g >> 1)) << 4));
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
-      if (i < r.tiles) {
-        copy16(to + i * 1024, w + r.to[2 * i]);
-        copy16(to + i * 1024 + 512, w + r.to[2 * i + 1]);
-      }
+      if (i >= r.tiles) break;
+      copy16(to + i * 1024, w + r.to[2 * i]);
+      copy16(to + i * 1024 + 512, w + r.to[2 * i + 1]);
     }
   }
   // the words that hold the step's scales (they need not begin at one), as far as the row goes
-  const int off = scale_offset<F>(l, s), skip = (int)((uintptr_t)r.s + off) & 3;
-  const uint8_t* from = r.s + off - skip;
-  const int left = l.scale_bytes - off + skip;
+  const int off = scale_offset<F>(l, s);
 #pragma unroll
-  for (int i = 0; i < S::kScaleWords; ++i)
-    copy4(slot + kRows * 64 + (lane * S::kScaleWords + i) * 4, left > 4 * i ? from + 4 * i : from, max(0, min(4, left - 4 * i)));
+  for (int j = 0; j < kTiles / 2; ++j) {
+    if (2 * j >= r.tiles) break;
+    const int skip = F == kFewFp8 ? 0 : (int)((uintptr_t)r.s[j] + off) & 3;
+    const uint8_t* from = r.s[j] + off - skip;
+    const int left = l.scale_bytes - off + skip;
+#pragma unroll
+    for (int i = 0; i < S::kScaleWords; ++i)
+      copy4(slot + kRows * 64 + ((j * 32 + lane) * S::kScaleWords + i) * 4, i == 0 || left > 4 * i ? from + 4 * i : from, max(0, min(4, left - 4 * i)));
+  }
 }
 
-// The scales of the step in the slot, of the lane's own row, as fp32.
+// The scales of the step in the slot, of the rows that the lane looks after, as fp32.  low: the two lowest bits of their addresses.
 template <int F>
-__device__ __forceinline__ void spread_scales(float* to, const uint8_t* slot, const FewRows& r, const FewLayout& l, int s) {
+__device__ __forceinline__ void spread_scales(float* to, const uint8_t* slot, const int (&low)[kTiles / 2], int tiles, const FewLayout& l, int s) {
   using S = FewShape<F>;
-  const int lane = threadIdx.x & 31;
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(slot + kRows * 64) + lane * S::kScaleWords;
-  if constexpr (F == kFewFp8) {
-    to[lane] = __uint_as_float(w[0]);
-  } else {
-    const int shift = ((int)((uintptr_t)r.s + scale_offset<F>(l, s)) & 3) * 8;
+#pragma unroll
+  for (int j = 0; j < kTiles / 2; ++j) {
+    if (2 * j >= tiles) break;
+    const int row = j * 32 + (threadIdx.x & 31);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(slot + kRows * 64) + row * S::kScaleWords;
+    const int shift = F == kFewFp4 ? low[j] * 8 : ((low[j] + scale_offset<F>(l, s)) & 3) * 8;
     auto value = [&](uint32_t h) { return l.f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16); };
     if constexpr (F == kFewFp4) {
       // 2^(byte - 127): the byte is the exponent (0 gives zero for 2^-127, 255 infinity for NaN)
       const uint32_t v = __funnelshift_r(w[0], w[1], shift);
-      reinterpret_cast<float4*>(to)[lane] = make_float4(__uint_as_float((v & 255u) << 23), __uint_as_float((v << 15) & 0x7f800000u),
-                                                        __uint_as_float((v << 7) & 0x7f800000u), __uint_as_float((v >> 1) & 0x7f800000u));
+      reinterpret_cast<float4*>(to)[row] = make_float4(__uint_as_float((v & 255u) << 23), __uint_as_float((v << 15) & 0x7f800000u),
+                                                       __uint_as_float((v << 7) & 0x7f800000u), __uint_as_float((v >> 1) & 0x7f800000u));
     } else if constexpr (F == kFewInt4) {
-      to[lane] = value((w[0] >> shift) & 0xffffu);
-    } else {
+      to[row] = value((w[0] >> shift) & 0xffffu);
+    } else if constexpr (F == kFewInt4Fine) {
       const uint32_t lo = __funnelshift_r(w[0], w[1], shift), hi = __funnelshift_r(w[1], w[2], shift);
       const float a = value(lo & 0xffffu), b = value(lo >> 16);
       const bool fine = l.group == 32;
-      reinterpret_cast<float4*>(to)[lane] = make_float4(a, fine ? b : a, fine ? value(hi & 0xffffu) : b, fine ? value(hi >> 16) : b);
+      reinterpret_cast<float4*>(to)[row] = make_float4(a, fine ? b : a, fine ? value(hi & 0xffffu) : b, fine ? value(hi >> 16) : b);
     }
   }
 }
@@ -342,9 +356,10 @@ struct FewTokens {
   uint32_t block;
 };
 
-// acc += W x of the step in the slot.
-template <int F, int NT>
-__device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const uint8_t* slot, const float* scales, int tiles,
+// acc += W x of the step in the slot, for the first `Tiles` tiles (what one of them has not got is something finite or not, in
+// rows that nobody reads).
+template <int F, int NT, int Tiles>
+__device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const uint8_t* slot, const float* scales,
                                               const FewTokens (&x)[NT], int s) {
   using S = FewShape<F>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -354,29 +369,8 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const
 #pragma unroll
     for (int q = 0; q < S::kBlocks; ++q) v[q][n] = *reinterpret_cast<const uint4*>(x[n].at + (s * S::kBlocks + q) * x[n].block);
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i) {
-    if (i >= tiles) break;
-    float d[NT][4] = {};
-    if constexpr (F == kFewFp8) {
-      const uint4 lo = *reinterpret_cast<const uint4*>(slot + i * 1024 + lane * 16), hi = *reinterpret_cast<const uint4*>(slot + i * 1024 + 512 + lane * 16);
-      const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t a0 = e4m3x2_to_h2(wl[w] & 0xffffu), a2 = e4m3x2_to_h2(wl[w] >> 16);
-        const uint32_t a1 = e4m3x2_to_h2(wh[w] & 0xffffu), a3 = e4m3x2_to_h2(wh[w] >> 16);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          mma(d[n], a0, a1, a2, a3, w & 1 ? v[w >> 1][n].z : v[w >> 1][n].x, w & 1 ? v[w >> 1][n].w : v[w >> 1][n].y);
-      }
-    }
-    float4 lo = {}, hi = {};
-    if constexpr (S::kScales == 4) {
-      lo = reinterpret_cast<const float4*>(scales)[16 * i + g];
-      hi = reinterpret_cast<const float4*>(scales)[16 * i + 8 + g];
-    } else {
-      lo.w = scales[16 * i + g];
-      hi.w = scales[16 * i + 8 + g];
-    }
+  for (int i = 0; i < Tiles; ++i) {
+    float d[NT][4];
     auto add = [&](float a, float b) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -384,10 +378,34 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const
         acc[i][n][1] = fmaf(a, d[n][1], acc[i][n][1]);
         acc[i][n][2] = fmaf(b, d[n][2], acc[i][n][2]);
         acc[i][n][3] = fmaf(b, d[n][3], acc[i][n][3]);
-        d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
       }
     };
-    if constexpr (F != kFewFp8) {
+    if constexpr (F == kFewFp8) {
+      const uint4 lo = *reinterpret_cast<const uint4*>(slot + i * 1024 + lane * 16), hi = *reinterpret_cast<const uint4*>(slot + i * 1024 + 512 + lane * 16);
+      const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t a0, a1, a2, a3;
+        e4m3x4_to_h2(wl[w], a0, a2);
+        e4m3x4_to_h2(wh[w], a1, a3);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4 b = v[w >> 1][n];
+          if (w == 0) mma_first(d[n], a0, a1, a2, a3, b.x, b.y);
+          else mma(d[n], a0, a1, a2, a3, w & 1 ? b.z : b.x, w & 1 ? b.w : b.y);
+        }
+      }
+      const float* sc = reinterpret_cast<const float*>(slot + kRows * 64) + 16 * i + g;
+      add(sc[0], sc[8]);
+    } else {
+      float4 lo, hi;
+      if constexpr (S::kScales == 4) {
+        lo = reinterpret_cast<const float4*>(scales)[16 * i + g];
+        hi = reinterpret_cast<const float4*>(scales)[16 * i + 8 + g];
+      } else {
+        lo.w = scales[16 * i + g];
+        hi.w = scales[16 * i + 8 + g];
+      }
       const uint8_t* w = slot + i * 1024 + g * 64 + t * 4;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -398,14 +416,31 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const
         else { s4x8_to_h2(wl, al); s4x8_to_h2(wh, ah); }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
+          if (S::kScales == 4 || q == 0) mma_first(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
+          else mma(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
           mma(d[n], al[2], ah[2], al[3], ah[3], v[q][n].z, v[q][n].w);
         }
-        if (S::kScales == 4 && q < 3) add(q == 0 ? lo.x : q == 1 ? lo.y : lo.z, q == 0 ? hi.x : q == 1 ? hi.y : hi.z);
+        if (S::kScales == 4 || q == 3) add(q == 0 ? lo.x : q == 1 ? lo.y : q == 2 ? lo.z : lo.w, q == 0 ? hi.x : q == 1 ? hi.y : q == 2 ? hi.z : hi.w);
       }
     }
-    add(lo.w, hi.w);
   }
+}
+
+// Takes the step in the slot and fetches the next one into it.
+template <int F, int NT, typename Next>
+__device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], uint8_t* ring, int& slot, const int (&low)[kTiles / 2], int tiles,
+                                          const FewLayout& l, const FewTokens (&x)[NT], int s, int panel_step, Next next) {
+  using S = FewShape<F>;
+  float* const scales = reinterpret_cast<float*>(ring + S::kDepth * S::kSlot);
+  uint8_t* const at = ring + slot * S::kSlot;
+  copies_wait<S::kDepth - 1>();
+  if (F != kFewFp8) spread_scales<F>(scales, at, low, tiles, l, s);
+  __syncwarp();
+  if (tiles > kTiles / 2) multiply_step<F, NT, kTiles>(acc, at, scales, x, panel_step);
+  else multiply_step<F, NT, kTiles / 2>(acc, at, scales, x, panel_step);
+  __syncwarp();
+  next(slot);
+  slot = slot + 1 == S::kDepth ? 0 : slot + 1;
 }
 
 __device__ __forceinline__ float load16(const void* p, int64_t i, bool f16) {
@@ -416,13 +451,18 @@ __device__ __forceinline__ float load16(const void* p, int64_t i, bool f16) {
 struct FewLaunch {
   int panel_bytes;       // of shared memory for the panel
   bool f16;
+  int up_blocks;         // of the first kernel
+  int splits;            // of the second kernel's steps: it has hidden / splits columns of blocks
+  float* top;            // [up_blocks][tokens * topk]: largest |h| that a block of the first kernel has found, per row of h
+  uint32_t* arrived;     // per column of blocks of the second kernel
+  float* part;           // [splits][tokens][hidden]: partial sums, with more than one split
 };
 
 constexpr int kTableBytes = (sizeof(FewTable) + 127) / 128 * 128;
 // Sums of the warps, for their owner to add up.
 template <int NT> struct RedShape { static constexpr int kWarpFloats = kTiles * NT * 4 * 32, kBytes = kWarps * kWarpFloats * 4; };
 template <int F, int NT> struct UpShape {
-  static constexpr int kFixed = kTableBytes + 512 + RedShape<NT>::kBytes + kWarps * FewShape<F>::kRing;
+  static constexpr int kFixed = kTableBytes + 512 + kMaxSlots * 4 + RedShape<NT>::kBytes + kWarps * FewShape<F>::kRing;
 };
 template <int F> struct DownShape {
   static constexpr int kFixed = kTableBytes + 128 + kMaxSlots * 4 + kWarps * FewShape<F>::kRing;
@@ -439,14 +479,17 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
   float* const inverse = reinterpret_cast<float*>(smem + kTableBytes);   // of the panel's rows' scales
   float* const tops = inverse + 32;                                       // (per warp)
   uint8_t* const zeros = smem + kTableBytes + 256;                        // a token's values where there is no token
-  float* const red = reinterpret_cast<float*>(smem + kTableBytes + 512);
+  uint32_t* const h_top = reinterpret_cast<uint32_t*>(smem + kTableBytes + 512);   // largest |h| per row (bits: NaN counts as largest)
+  float* const red = reinterpret_cast<float*>(smem + kTableBytes + 512 + kMaxSlots * 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* const ring = smem + kTableBytes + 512 + RedShape<NT>::kBytes + warp * S::kRing;
-  float* const scales = reinterpret_cast<float*>(ring + S::kDepth * S::kSlot);
+  uint8_t* const ring = smem + kTableBytes + 512 + kMaxSlots * 4 + RedShape<NT>::kBytes + warp * S::kRing;
   uint8_t* const panel = smem + UpShape<F, NT>::kFixed;
   pdl_wait();
   pdl_trigger();
   if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0;
+  for (int i = tid; i < p.tokens * p.topk; i += kThreads) h_top[i] = 0;
+  if (blockIdx.x == 0)   // (the second kernel counts from there)
+    for (int i = tid; i < kFewMaxColumns; i += kThreads) launch.arrived[i] = 0;
   build_table<false>(table, p);
   const FewMatrix& m = p.w13;
   const FewLayout layout(m, F, launch.f16);
@@ -475,8 +518,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       int least = 1 << 30;
 #pragma unroll
       for (int w = 1; w <= kWarps; w *= 2) {
-        const int pieces = ((to - from) * w + kWarps - 1) / kWarps;
-        const int cost = (pieces + kTiles - 1) / kTiles * (4 * ((steps + w - 1) / w) + (w > 1 ? 4 : 1));
+        const int pieces = ((to - from) * w + kWarps - 1) / kWarps, tiles = (pieces + kTiles - 1) / kTiles;
+        const int cost = (steps + w - 1) / w * (pieces + tiles) + tiles * (w > 1 ? 8 : 4);
         if (cost < least) { least = cost; group = w; }
       }
     }
@@ -489,31 +532,35 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       rest &= ~now;
       const int rows = __popc(now);
 
-      auto tile_rows = [&](int first) {       // of the tiles that begin with piece `first`
-        FewRows r;
-        const int a = first / per_expert, f = (first - a * per_expert) * 8;
-        const int64_t e = table.expert[a], rb = layout.row_bytes;
-        r.tiles = min(kTiles, min(per_expert - f / 8, my_to - first));
-        r.to[0] = 0;
-        r.to[1] = pairs ? rb : p.inter * rb;
-        r.to[2] = (pairs ? 16 : 8) * rb;
-        r.to[3] = r.to[1] + r.to[2];
-        r.w = reinterpret_cast<const uint8_t*>(m.w) + (e * m.n + (pairs ? 2 * (f + g) : f + g)) * rb + t * 16;
-        // (rows of a tile that is not there: any)
-        const int fs = f + (lane < 16 * r.tiles ? lane >> 4 : 0) * 8 + (lane & 7), up = (lane >> 3) & 1;
+      // scales of the rows that the lane looks after, where features [f, f + 8 tiles) begin
+      auto scale_row = [&](int64_t e, int f, int tiles, int j) {
+        const int row = j * 32 + lane, piece = row < 16 * tiles ? row >> 4 : 0, fs = f + piece * 8 + (row & 7), up = (row >> 3) & 1;
         const int64_t n = pairs ? 2 * fs + up : fs + up * p.inter;
-        r.s = reinterpret_cast<const uint8_t*>(m.scale) + (F == kFewFp8 ? e * (m.n / 128) + n / 128 : e * m.n + n) * layout.scale_bytes;
-        return r;
+        return reinterpret_cast<const uint8_t*>(m.scale) + (F == kFewFp8 ? e * (m.n / 128) + n / 128 : e * m.n + n) * layout.scale_bytes;
+      };
+      auto tile_rows = [&](FewRows& r, int a, int f, int last) {       // of the tiles that begin with feature f
+        const int64_t e = table.expert[a], rb = layout.row_bytes;
+        r.tiles = min(kTiles, last);
+        r.w = reinterpret_cast<const uint8_t*>(m.w) + (e * m.n + (pairs ? 2 * (f + g) : f + g)) * rb + t * 16;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          r.to[2 * i] = (pairs ? 16 : 8) * i * rb;
+          r.to[2 * i + 1] = r.to[2 * i] + (pairs ? rb : p.inter * rb);
+        }
+#pragma unroll
+        for (int j = 0; j < kTiles / 2; ++j) r.s[j] = scale_row(e, f, r.tiles, j);
       };
       // the ring begins to fill
-      int next = my_from, s = member;     // of the step that is fetched next: its first piece
-      FewRows fetch = {};
-      if (next < my_to) fetch = tile_rows(next);
+      // of the step that is fetched next: its tiles' first piece (of all, and within its expert), the expert
+      int next = my_from, next_a = my_from / per_expert, next_u = my_from - next_a * per_expert, s = member;
+      FewRows fetch;
       auto settle = [&]() {
         while (s >= steps && next < my_to) {
           s -= steps;
           next += fetch.tiles;
-          if (next < my_to) fetch = tile_rows(next);
+          next_u += fetch.tiles;
+          if (next_u == per_expert) { next_u = 0; ++next_a; }
+          if (next < my_to) tile_rows(fetch, next_a, next_u * 8, min(per_expert - next_u, my_to - next));
         }
       };
       auto copy_next = [&](int slot) {
@@ -524,38 +571,43 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         }
         copies_end();
       };
+      if (next < my_to) tile_rows(fetch, next_a, next_u * 8, min(per_expert - next_u, my_to - next));
       settle();
 #pragma unroll
       for (int i = 0; i < S::kDepth; ++i) copy_next(i);
 
       // the panel
       {
-        const int parts = warps_per_row(rows), row = warp / parts, part = warp % parts;   // (a round of the rows is all of them)
+        const int parts = warps_per_row(rows), part = warp % parts;
         const int source = launch.f16 ? kFromF16 : kFromBf16, k8 = steps * (S::kK / 8);
-        uint32_t left_tokens = now;
-        for (int i = 0; i < row; ++i) left_tokens &= left_tokens - 1;
-        const bool there = row < rows;
-        const uint8_t* x = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)(there ? __ffs(left_tokens) - 1 : 0) * p.hidden * 2;
-        float top = there ? row_top(x, source, p.hidden, 0, k8, part, parts) : 0.f;
-        if (parts > 1) {
-          if (lane == 0) tops[warp] = top;
-          __syncthreads();
-          for (int i = 0; i < parts; ++i) top = max_nan(top, tops[row * parts + i]);
-        }
-        if (there) {
-          float inv;
-          const float scale = row_scale(top, inv);
-          if (lane == 0 && part == 0) inverse[row] = inv;
-          convert_row<F>(panel, row, rows, x, source, p.hidden, 0, k8, scale, part, parts);
+        for (int row = warp / parts, q0 = 0; q0 < rows; q0 += kWarps / parts, row += kWarps / parts) {   // (once where a row has several warps)
+          uint32_t left_tokens = now;
+          for (int i = 0; i < row; ++i) left_tokens &= left_tokens - 1;
+          const bool there = row < rows;
+          const uint8_t* x = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)(there ? __ffs(left_tokens) - 1 : 0) * p.hidden * 2;
+          float top = there ? row_top(x, source, p.hidden, 0, k8, part, parts) : 0.f;
+          if (parts > 1) {
+            if (lane == 0) tops[warp] = top;
+            __syncthreads();
+            for (int i = 0; i < parts; ++i) top = max_nan(top, tops[row * parts + i]);
+          }
+          if (there) {
+            float inv;
+            const float scale = row_scale(top, inv);
+            if (lane == 0 && part == 0) inverse[row] = inv;
+            convert_row<F>(panel, row, rows, x, source, p.hidden, 0, k8, scale, part, parts);
+          }
         }
         __syncthreads();
       }
 
-      int slot = 0, cs = member;
+      int slot = 0, cs = member, a = my_from / per_expert, u = my_from - a * per_expert;
       for (int first = my_from; first < my_to;) {
-        const FewRows r = tile_rows(first);
-        const int a = first / per_expert;
+        const int tiles = min(kTiles, min(per_expert - u, my_to - first));
         const uint32_t mine = table.tokens[a] & now;
+        int low[kTiles / 2];
+#pragma unroll
+        for (int j = 0; j < kTiles / 2; ++j) low[j] = F == kFewFp8 ? 0 : (int)((uintptr_t)scale_row(table.expert[a], u * 8, tiles, j) & 3);
         FewTokens x[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -564,20 +616,12 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
           x[n].block = used ? rows * 64 : 0;
         }
         float acc[kTiles][NT][4] = {};
-        for (; cs < steps; cs += group) {
-          copies_wait<S::kDepth - 1>();
-          spread_scales<F>(scales, ring + slot * S::kSlot, r, layout, cs);
-          __syncwarp();
-          multiply_step<F, NT>(acc, ring + slot * S::kSlot, scales, r.tiles, x, cs);
-          __syncwarp();
-          copy_next(slot);
-          slot = slot + 1 == S::kDepth ? 0 : slot + 1;
-        }
+        for (; cs < steps; cs += group) take_step<F, NT>(acc, ring, slot, low, tiles, layout, x, cs, cs, copy_next);
         cs -= steps;
         auto finish = [&](int i, int col, int f_in_tile, float gate, float up) {
-          if (i >= r.tiles || !((mine >> col) & 1)) return;
+          if (i >= tiles || !((mine >> col) & 1)) return;
           const float inv = inverse[rank_below(now, col)];
-          const int f = (first - a * per_expert + i) * 8 + f_in_tile;
+          const int f = (u + i) * 8 + f_in_tile;
           gate *= inv;
           up *= inv;
           if (m.bias) {
@@ -585,7 +629,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
             gate += load16(m.bias, at + (pairs ? 2 * f : f), launch.f16);
             up += load16(m.bias, at + (pairs ? 2 * f + 1 : p.inter + f), launch.f16);
           }
-          p.h[(int64_t)(table.first_row[a] + rank_below(table.tokens[a], col)) * p.inter + f] = gated(p, gate, up);
+          const int row = table.first_row[a] + rank_below(table.tokens[a], col);
+          const float h = gated(p, gate, up);
+          p.h[(int64_t)row * p.inter + f] = h;
+          atomicMax(&h_top[row], __float_as_uint(h) & 0x7fffffffu);
         };
         if (group == 1) {
 #pragma unroll
@@ -616,28 +663,35 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
           }
           group_sync(1 + mine_of, group * 32);   // the sums' place is free again
         }
-        first += r.tiles;
+        first += tiles;
+        u += tiles;
+        if (u == per_expert) { u = 0; ++a; }
       }
       copies_wait<0>();
       __syncthreads();   // the panel is free again
     }
     from = to;
   }
+  if (begin < end) {
+    const int r0 = table.first_row[begin / per_expert], r1 = table.first_row[(end - 1) / per_expert + 1];
+    for (int r = r0 + tid; r < r1; r += kThreads) launch.top[(int64_t)blockIdx.x * (p.tokens * p.topk) + r] = __uint_as_float(h_top[r]);
+  }
 }
 
-// out = sum over experts of weight * (W2 h + b2).  A block has some rows of W2 and goes through all active experts with them;
-// its warps take the steps in turn, in two halves with half of the rows each where there are more than 32.
+// out = sum over experts of weight * (W2 h + b2).  A block has some rows of W2 and a share of the steps over all active
+// experts: of rows up to 64, so that few blocks need the same values of h, and of steps what makes as many blocks as there are
+// SMs.  It goes through its steps with as many of h's values at a time as its panel holds, each warp with a stretch of them.
+// Of the blocks with the same rows the last one to be done adds the partial sums up, in their order.
 template <int F, int NT>
 __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewLaunch launch) {
   using S = FewShape<F>;
   extern __shared__ __align__(128) uint8_t smem[];
   FewTable& table = *reinterpret_cast<FewTable*>(smem);
-  float* const tops = reinterpret_cast<float*>(smem + kTableBytes);       // (per warp)
+  int& last_one = *reinterpret_cast<int*>(smem + kTableBytes);
   uint8_t* const zeros = smem + kTableBytes + 64;
   float* const coef = reinterpret_cast<float*>(smem + kTableBytes + 128);   // of the panel's rows: routing weight and the inverse of the scale
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* const ring = smem + kTableBytes + 128 + kMaxSlots * 4 + warp * S::kRing;
-  float* const scales = reinterpret_cast<float*>(ring + S::kDepth * S::kSlot);
   uint8_t* const panel = smem + DownShape<F>::kFixed;
   float* const red = reinterpret_cast<float*>(panel);                     // (after the last panel)
   // What routed the tokens was complete before the kernel ahead of this one let it start.
@@ -646,42 +700,86 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   const FewMatrix& m = p.w2;
   const FewLayout layout(m, F, launch.f16);
   const int steps = (p.inter + S::kK - 1) / S::kK;
-  const int row_begin = (int)((int64_t)p.hidden * blockIdx.x / gridDim.x), row_end = (int)((int64_t)p.hidden * (blockIdx.x + 1) / gridDim.x);
+  const int columns = gridDim.x / launch.splits, column = blockIdx.x % columns, split = blockIdx.x / columns;
+  const int row_begin = (int)((int64_t)p.hidden * column / columns), row_end = (int)((int64_t)p.hidden * (column + 1) / columns);
+  const int64_t total = (int64_t)table.active * steps;
+  const int step_begin = (int)(total * split / launch.splits), step_end = (int)(total * (split + 1) / launch.splits);
+  const int per_expert = p.inter / 8;                                     // (as the first kernel deals its features out)
   const int room = launch.panel_bytes / (S::kK * 2);                      // rows times steps that the panel holds
   bool waited = false;
 
-  for (int r0 = row_begin; r0 < row_end || !waited; r0 += 2 * kRows) {
-    const int block_rows = max(0, min(2 * kRows, row_end - r0));
-    const int halves = block_rows > kRows ? 2 : 1, group = kWarps / halves, half = warp / group, member = warp % group;
-    const int my_r0 = r0 + block_rows * half / halves, my_rows = block_rows * (half + 1) / halves - block_rows * half / halves;
-    auto expert_rows = [&](int a) {
-      FewRows r;
-      const int64_t e = table.expert[a], rb = layout.row_bytes;
-      r.tiles = (my_rows + 15) / 16;
-      r.w = reinterpret_cast<const uint8_t*>(m.w) + (e * m.n + my_r0) * rb + t * 16;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r.to[i] = min(8 * i + g, my_rows - 1) * rb;   // (what a tile has not got is the last row again)
-      const int64_t n = my_r0 + min(lane, my_rows - 1);
-      r.s = reinterpret_cast<const uint8_t*>(m.scale) + (F == kFewFp8 ? e * (m.n / 128) + n / 128 : e * m.n + n) * layout.scale_bytes;
-      return r;
+  // How far a panel reaches that begins with step s0 of expert a0: whole experts, then as many steps of the next one as
+  // there is room for (at least one).
+  auto panel_end = [&](int a0, int s0, int& a1, int& s1) {
+    int free = room;
+    a1 = a0;
+    s1 = s0;
+    while (a1 * steps + s1 < step_end) {
+      const int n = table.first_row[a1 + 1] - table.first_row[a1], fit = min(min(steps - s1, step_end - a1 * steps - s1), free / n);
+      if (fit == 0) break;
+      free -= fit * n;
+      s1 += fit;
+      if (s1 < steps) break;
+      s1 = 0;
+      ++a1;
+    }
+  };
+  auto finish = [&](float v, int token, int n) {
+    if (m.bias) {
+      for (int k = 0; k < p.topk; ++k) {
+        const int a = table.slot_expert[token * p.topk + k];
+        if (a >= 0) v = fmaf(p.weights[token * p.topk + k], load16(m.bias, (int64_t)table.expert[a] * m.n + n, launch.f16), v);
+      }
+    }
+    const int64_t to = (int64_t)token * p.hidden + n;
+    if (launch.f16) reinterpret_cast<__half*>(p.out)[to] = __float2half_rn(v);
+    else reinterpret_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(v);
+  };
+  for (int r0 = row_begin; r0 < row_end || !waited; r0 += kRows) {
+    const int rows_here = max(0, min(kRows, row_end - r0)), tiles = (rows_here + 15) / 16;
+    auto scale_row = [&](int a, int j) {
+      const int64_t n = r0 + min(j * 32 + lane, rows_here - 1), e = table.expert[a];
+      return reinterpret_cast<const uint8_t*>(m.scale) + (F == kFewFp8 ? e * (m.n / 128) + n / 128 : e * m.n + n) * layout.scale_bytes;
     };
-    int fetch_a = 0, s = member;     // of the step that is fetched next
-    FewRows fetch = {};
-    auto settle = [&]() {
-      bool moved = false;
-      while (s >= steps && fetch_a < table.active) { s -= steps; ++fetch_a; moved = true; }
-      if (moved && fetch_a < table.active) fetch = expert_rows(fetch_a);
+    FewRows fetch;
+    fetch.tiles = tiles;
+#pragma unroll
+    for (int i = 0; i < 2 * kTiles; ++i)
+      fetch.to[i] = (int64_t)max(0, min(8 * i + g, rows_here - 1)) * layout.row_bytes;   // (what a tile has not got is the last row again)
+    auto expert_rows = [&](int a) {
+      fetch.w = reinterpret_cast<const uint8_t*>(m.w) + ((int64_t)table.expert[a] * m.n + r0) * layout.row_bytes + t * 16;
+#pragma unroll
+      for (int j = 0; j < kTiles / 2; ++j) fetch.s[j] = scale_row(a, j);
+    };
+    // The step that is fetched next, the end of this warp's stretch, and where the panel after that begins.
+    int fetch_a = 0, fetch_s = 0, left = 0, panel_a = step_begin / steps, panel_s = step_begin - panel_a * steps;
+    auto next_stretch = [&]() {
+      while (left == 0 && panel_a * steps + panel_s < step_end) {
+        int a1, s1;
+        panel_end(panel_a, panel_s, a1, s1);
+        const int from = panel_a * steps + panel_s, all = a1 * steps + s1 - from, mine = all * warp / kWarps;
+        left = all * (warp + 1) / kWarps - mine;
+        fetch_a = (from + mine) / steps;
+        fetch_s = from + mine - fetch_a * steps;
+        panel_a = a1;
+        panel_s = s1;
+        if (left > 0) expert_rows(fetch_a);
+      }
     };
     auto copy_next = [&](int slot) {
-      if (fetch_a < table.active && my_rows > 0) {
-        copy_step<F>(smem_at(ring) + slot * S::kSlot, fetch, layout, s);
-        s += group;
-        settle();
+      if (left > 0) {
+        copy_step<F>(smem_at(ring) + slot * S::kSlot, fetch, layout, fetch_s);
+        ++fetch_s;
+        if (--left == 0) {
+          next_stretch();
+        } else if (fetch_s == steps) {
+          fetch_s = 0;
+          expert_rows(++fetch_a);
+        }
       }
       copies_end();
     };
-    if (table.active > 0 && my_rows > 0) fetch = expert_rows(0);
-    settle();
+    if (rows_here > 0) next_stretch();
 #pragma unroll
     for (int i = 0; i < S::kDepth; ++i) copy_next(i);
     if (!waited) {
@@ -690,19 +788,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       waited = true;
     }
     float out[kTiles][NT][4] = {};
-    int slot = 0, pos = member;
-    for (int a0 = 0, s0 = 0; a0 < table.active;) {
-      // how far the panel reaches: whole experts, then as many steps of the next one as there is room for (at least one)
-      int a1 = a0, s1 = s0, free = room;
-      while (a1 < table.active) {
-        const int n = table.first_row[a1 + 1] - table.first_row[a1], fit = min(steps - s1, free / n);
-        if (fit == 0) break;
-        free -= fit * n;
-        s1 += fit;
-        if (s1 < steps) break;
-        s1 = 0;
-        ++a1;
-      }
+    int slot = 0;
+    for (int a0 = step_begin / steps, s0 = step_begin - a0 * steps; a0 * steps + s0 < step_end;) {
+      int a1, s1;
+      panel_end(a0, s0, a1, s1);
       const int last = s1 > 0 ? a1 : a1 - 1;           // the last expert with steps in the panel
       const int row0 = table.first_row[a0], rows = table.first_row[last + 1] - row0;
       {
@@ -712,14 +801,16 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
           const bool there = q0 + row < rows;
           const int a = there ? table.row_expert[r] : a0;
           const int k8_0 = (a == a0 ? s0 : 0) * (S::kK / 8), k8_1 = (a == a1 ? s1 : steps) * (S::kK / 8);
-          const float* h = p.h + (int64_t)(there ? r : 0) * p.inter;
-          float top = there ? row_top(h, kFromF32, p.inter, k8_0, k8_1, part, parts) : 0.f;
-          if (parts > 1) {
-            if (lane == 0) tops[warp] = top;
-            __syncthreads();
-            for (int i = 0; i < parts; ++i) top = max_nan(top, tops[row * parts + i]);
-          }
           if (there) {
+            // the largest |h| of the row, over the blocks of the first kernel that had features of its expert
+            const int64_t all = (int64_t)table.active * per_expert, g1 = launch.up_blocks;
+            const int c0 = (int)((((int64_t)a * per_expert + 1) * g1 - 1) / all), c1 = (int)(((int64_t)(a + 1) * per_expert * g1 - 1) / all);
+            float top = 0.f;
+            for (int c = c0 + lane; c <= c1; c += 32)   // (with less than a piece a block, some have none)
+              if (all * c / g1 < all * (c + 1) / g1) top = max_nan(top, launch.top[(int64_t)c * (p.tokens * p.topk) + r]);
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float* h = p.h + (int64_t)r * p.inter;
             float inv;
             const float scale = row_scale(top, inv);
             if (lane == 0 && part == 0) coef[q0 + row] = table.weight[r] * inv;
@@ -731,12 +822,19 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
         }
         __syncthreads();
       }
-      const uint8_t* base = panel;
-      for (int a = a0; a <= last; ++a) {
-        const int first = a == a0 ? s0 : 0, stop = a == a1 ? s1 : steps, n_rows = table.first_row[a + 1] - table.first_row[a];
-        const uint32_t mine = table.tokens[a];
-        if (pos < a * steps + stop && my_rows > 0) {
-          const FewRows r = expert_rows(a);
+      {
+        const int from = a0 * steps + s0, all = a1 * steps + s1 - from;
+        int pos = from + all * warp / kWarps;
+        const int stop = rows_here > 0 ? from + all * (warp + 1) / kWarps : 0;
+        for (int a = pos / steps; pos < stop; ++a) {
+          const int row = table.first_row[a], n_rows = table.first_row[a + 1] - row, end = min(stop, (a + 1) * steps);
+          // rows of earlier experts in the panel, as above
+          const int before = a == a0 ? 0 : (table.first_row[a0 + 1] - row0) * (steps - s0) + (row - table.first_row[a0 + 1]) * steps;
+          const uint8_t* base = panel + (before - (a == a0 ? s0 : 0) * n_rows) * (S::kK * 2);
+          const uint32_t mine = table.tokens[a];
+          int low[kTiles / 2];
+#pragma unroll
+          for (int j = 0; j < kTiles / 2; ++j) low[j] = F == kFewFp8 ? 0 : (int)((uintptr_t)scale_row(a, j) & 3);
           FewTokens x[NT];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -745,15 +843,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
             x[n].block = used ? n_rows * 64 : 0;
           }
           float acc[kTiles][NT][4] = {};
-          for (; pos < a * steps + stop; pos += group) {
-            copies_wait<S::kDepth - 1>();
-            spread_scales<F>(scales, ring + slot * S::kSlot, r, layout, pos - a * steps);
-            __syncwarp();
-            multiply_step<F, NT>(acc, ring + slot * S::kSlot, scales, r.tiles, x, pos - a * steps - first);
-            __syncwarp();
-            copy_next(slot);
-            slot = slot + 1 == S::kDepth ? 0 : slot + 1;
-          }
+          for (; pos < end; ++pos) take_step<F, NT>(acc, ring, slot, low, tiles, layout, x, pos - a * steps, pos - a * steps, copy_next);
           // (columns of tokens without this expert are left out: a weight that is not finite would get into them)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
@@ -761,7 +851,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
             for (int c = 0; c < 2; ++c) {
               const int token = 8 * n + 2 * t + c;
               if (!((mine >> token) & 1)) continue;
-              const float w = coef[table.first_row[a] - row0 + rank_below(mine, token)];
+              const float w = coef[row - row0 + rank_below(mine, token)];
 #pragma unroll
               for (int i = 0; i < kTiles; ++i) {
                 out[i][n][c] = fmaf(w, acc[i][n][c], out[i][n][c]);
@@ -769,7 +859,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
               }
             }
         }
-        base += (stop - first) * n_rows * (S::kK * 2);
       }
       a0 = a1;
       s0 = s1;
@@ -784,25 +873,33 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
         for (int c = 0; c < 4; ++c) red[warp * kWarpFloats + ((i * NT + n) * 4 + c) * 32 + lane] = out[i][n][c];
     copies_wait<0>();
     __syncthreads();
-    for (int j = tid; j < 2 * kRows * p.tokens; j += kThreads) {
+    for (int j = tid; j < kRows * p.tokens; j += kThreads) {
       // consecutive threads, consecutive features of a token
-      const int row = j % (2 * kRows), token = j / (2 * kRows);
-      if (row >= block_rows) continue;
-      const int h = halves == 2 && row >= block_rows / 2, i = row - (h ? block_rows / 2 : 0);   // of that half
-      const int at = (((i >> 4) * NT + (token >> 3)) * 4 + ((i >> 3) & 1) * 2 + (token & 1)) * 32 + (i & 7) * 4 + ((token & 7) >> 1);
+      const int row = j % kRows, token = j / kRows;
+      if (row >= rows_here) continue;
+      const int at = (((row >> 4) * NT + (token >> 3)) * 4 + ((row >> 3) & 1) * 2 + (token & 1)) * 32 + (row & 7) * 4 + ((token & 7) >> 1);
       float v = 0.f;
-      for (int w = 0; w < group; ++w) v += red[(h * group + w) * kWarpFloats + at];
-      if (m.bias) {
-        for (int k = 0; k < p.topk; ++k) {
-          const int a = table.slot_expert[token * p.topk + k];
-          if (a >= 0) v = fmaf(p.weights[token * p.topk + k], load16(m.bias, (int64_t)table.expert[a] * m.n + r0 + row, launch.f16), v);
-        }
-      }
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) v += red[w * kWarpFloats + at];
       const int64_t to = (int64_t)token * p.hidden + r0 + row;
-      if (launch.f16) reinterpret_cast<__half*>(p.out)[to] = __float2half_rn(v);
-      else reinterpret_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(v);
+      if (launch.splits == 1) finish(v, token, r0 + row);
+      else launch.part[(int64_t)split * p.tokens * p.hidden + to] = v;
     }
     __syncthreads();
+  }
+  if (launch.splits == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last_one = atomicAdd(&launch.arrived[column], 1u) == (uint32_t)launch.splits - 1;
+  __syncthreads();
+  if (!last_one) return;
+  __threadfence();
+  const int width = row_end - row_begin;
+  for (int j = tid; j < width * p.tokens; j += kThreads) {
+    const int row = row_begin + j % width, token = j / width;
+    float v = 0.f;
+    for (int i = 0; i < launch.splits; ++i) v += __ldcg(launch.part + ((int64_t)i * p.tokens + token) * p.hidden + row);
+    finish(v, token, row);
   }
 }
 

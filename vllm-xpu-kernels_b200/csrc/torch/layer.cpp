@@ -618,7 +618,7 @@ PyObject* layer_few(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const auto stream = at::cuda::getCurrentCUDAStream();
   WithoutGil gil;
   {
-    g.workspace_bytes = b200moe_few_tokens_workspace_bytes((int)T, (int)K, (int)k2);
+    g.workspace_bytes = b200moe_few_tokens_workspace_bytes((int)T, (int)K, (int)H, (int)k2);
     const Workspace workspace(stream, g.workspace_bytes, a[7] == Py_True);
     g.workspace = workspace.mem.data_ptr();
     check_status(b200moe_few_tokens_layer(&g, (b200moe_stream)stream.stream()));

@@ -138,6 +138,23 @@ __device__ __forceinline__ void copy4(uint32_t to, const void* from, int bytes) 
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// (volatile: they stay behind the waits and barriers ahead of them)
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float ldsf(uint32_t a) { return __uint_as_float(lds4(a)); }
+__device__ __forceinline__ void sts16(uint32_t a, float x, float y, float z, float w) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+}
+__device__ __forceinline__ void sts4(uint32_t a, float x) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(x) : "memory"); }
+
 // Barrier of some of the block's warps.
 __device__ __forceinline__ void group_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
@@ -324,27 +341,27 @@ __device__ __forceinline__ void copy_step(uint32_t slot, const FewRows& r, const
 
 // The scales of the step in the slot, of the rows that the lane looks after, as fp32.  low: the two lowest bits of their addresses.
 template <int F>
-__device__ __forceinline__ void spread_scales(float* to, const uint8_t* slot, const int (&low)[kTiles / 2], int tiles, const FewLayout& l, int s) {
+__device__ __forceinline__ void spread_scales(uint32_t to, uint32_t slot, const int (&low)[kTiles / 2], int tiles, const FewLayout& l, int s) {
   using S = FewShape<F>;
 #pragma unroll
   for (int j = 0; j < kTiles / 2; ++j) {
     if (2 * j >= tiles) break;
     const int row = j * 32 + (threadIdx.x & 31);
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(slot + kRows * 64) + row * S::kScaleWords;
+    const uint32_t w = slot + kRows * 64 + row * S::kScaleWords * 4;
     const int shift = F == kFewFp4 ? low[j] * 8 : ((low[j] + scale_offset<F>(l, s)) & 3) * 8;
     auto value = [&](uint32_t h) { return l.f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16); };
     if constexpr (F == kFewFp4) {
       // 2^(byte - 127): the byte is the exponent (0 gives zero for 2^-127, 255 infinity for NaN)
-      const uint32_t v = __funnelshift_r(w[0], w[1], shift);
-      reinterpret_cast<float4*>(to)[row] = make_float4(__uint_as_float((v & 255u) << 23), __uint_as_float((v << 15) & 0x7f800000u),
-                                                       __uint_as_float((v << 7) & 0x7f800000u), __uint_as_float((v >> 1) & 0x7f800000u));
+      const uint32_t v = __funnelshift_r(lds4(w), lds4(w + 4), shift);
+      sts16(to + row * 16, __uint_as_float((v & 255u) << 23), __uint_as_float((v << 15) & 0x7f800000u),
+            __uint_as_float((v << 7) & 0x7f800000u), __uint_as_float((v >> 1) & 0x7f800000u));
     } else if constexpr (F == kFewInt4) {
-      to[row] = value((w[0] >> shift) & 0xffffu);
+      sts4(to + row * 4, value((lds4(w) >> shift) & 0xffffu));
     } else if constexpr (F == kFewInt4Fine) {
-      const uint32_t lo = __funnelshift_r(w[0], w[1], shift), hi = __funnelshift_r(w[1], w[2], shift);
+      const uint32_t mid = lds4(w + 4), lo = __funnelshift_r(lds4(w), mid, shift), hi = __funnelshift_r(mid, lds4(w + 8), shift);
       const float a = value(lo & 0xffffu), b = value(lo >> 16);
       const bool fine = l.group == 32;
-      reinterpret_cast<float4*>(to)[row] = make_float4(a, fine ? b : a, fine ? value(hi & 0xffffu) : b, fine ? value(hi >> 16) : b);
+      sts16(to + row * 16, a, fine ? b : a, fine ? value(hi & 0xffffu) : b, fine ? value(hi >> 16) : b);
     }
   }
 }
@@ -352,14 +369,13 @@ __device__ __forceinline__ void spread_scales(float* to, const uint8_t* slot, co
 // Where a lane finds the values of its columns' tokens in the panel: the step's first block and the way to the next one.
 // Without a token: zeros, and no way.
 struct FewTokens {
-  const uint8_t* at;
-  uint32_t block;
+  uint32_t at, block;
 };
 
 // acc += W x of the step in the slot, for the first `Tiles` tiles (what one of them has not got is something finite or not, in
 // rows that nobody reads).
 template <int F, int NT, int Tiles>
-__device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const uint8_t* slot, const float* scales,
+__device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint32_t slot, uint32_t scales,
                                               const FewTokens (&x)[NT], int s) {
   using S = FewShape<F>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -367,7 +383,7 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int q = 0; q < S::kBlocks; ++q) v[q][n] = *reinterpret_cast<const uint4*>(x[n].at + (s * S::kBlocks + q) * x[n].block);
+    for (int q = 0; q < S::kBlocks; ++q) v[q][n] = lds16(x[n].at + (s * S::kBlocks + q) * x[n].block);
 #pragma unroll
   for (int i = 0; i < Tiles; ++i) {
     float d[NT][4];
@@ -381,7 +397,7 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const
       }
     };
     if constexpr (F == kFewFp8) {
-      const uint4 lo = *reinterpret_cast<const uint4*>(slot + i * 1024 + lane * 16), hi = *reinterpret_cast<const uint4*>(slot + i * 1024 + 512 + lane * 16);
+      const uint4 lo = lds16(slot + i * 1024 + lane * 16), hi = lds16(slot + i * 1024 + 512 + lane * 16);
       const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -395,22 +411,22 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const
           else mma(d[n], a0, a1, a2, a3, w & 1 ? b.z : b.x, w & 1 ? b.w : b.y);
         }
       }
-      const float* sc = reinterpret_cast<const float*>(slot + kRows * 64) + 16 * i + g;
-      add(sc[0], sc[8]);
+      const uint32_t sc = slot + kRows * 64 + (16 * i + g) * 4;
+      add(ldsf(sc), ldsf(sc + 32));
     } else {
-      float4 lo, hi;
+      uint4 lo, hi;
       if constexpr (S::kScales == 4) {
-        lo = reinterpret_cast<const float4*>(scales)[16 * i + g];
-        hi = reinterpret_cast<const float4*>(scales)[16 * i + 8 + g];
+        lo = lds16(scales + (16 * i + g) * 16);
+        hi = lds16(scales + (16 * i + 8 + g) * 16);
       } else {
-        lo.w = scales[16 * i + g];
-        hi.w = scales[16 * i + 8 + g];
+        lo.w = lds4(scales + (16 * i + g) * 4);
+        hi.w = lds4(scales + (16 * i + 8 + g) * 4);
       }
-      const uint8_t* w = slot + i * 1024 + g * 64 + t * 4;
+      const uint32_t w = slot + i * 1024 + g * 64 + t * 4;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int at = (q ^ (g >> 1)) << 4;
-        const uint32_t wl = *reinterpret_cast<const uint32_t*>(w + at), wh = *reinterpret_cast<const uint32_t*>(w + 512 + at);
+        const uint32_t wl = lds4(w + at), wh = lds4(w + at + 512);
         uint32_t al[4], ah[4];
         if constexpr (F == kFewFp4) { e2m1x8_to_h2(wl, al); e2m1x8_to_h2(wh, ah); }
         else { s4x8_to_h2(wl, al); s4x8_to_h2(wh, ah); }
@@ -420,7 +436,8 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const
           else mma(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
           mma(d[n], al[2], ah[2], al[3], ah[3], v[q][n].z, v[q][n].w);
         }
-        if (S::kScales == 4 || q == 3) add(q == 0 ? lo.x : q == 1 ? lo.y : q == 2 ? lo.z : lo.w, q == 0 ? hi.x : q == 1 ? hi.y : q == 2 ? hi.z : hi.w);
+        if (S::kScales == 4 || q == 3) add(__uint_as_float(q == 0 ? lo.x : q == 1 ? lo.y : q == 2 ? lo.z : lo.w),
+                                             __uint_as_float(q == 0 ? hi.x : q == 1 ? hi.y : q == 2 ? hi.z : hi.w));
       }
     }
   }
@@ -428,11 +445,10 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], const
 
 // Takes the step in the slot and fetches the next one into it.
 template <int F, int NT, typename Next>
-__device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], uint8_t* ring, int& slot, const int (&low)[kTiles / 2], int tiles,
+__device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], uint32_t ring, int& slot, const int (&low)[kTiles / 2], int tiles,
                                           const FewLayout& l, const FewTokens (&x)[NT], int s, int panel_step, Next next) {
   using S = FewShape<F>;
-  float* const scales = reinterpret_cast<float*>(ring + S::kDepth * S::kSlot);
-  uint8_t* const at = ring + slot * S::kSlot;
+  const uint32_t scales = ring + S::kDepth * S::kSlot, at = ring + slot * S::kSlot;
   copies_wait<S::kDepth - 1>();
   if (F != kFewFp8) spread_scales<F>(scales, at, low, tiles, l, s);
   __syncwarp();
@@ -482,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
   uint32_t* const h_top = reinterpret_cast<uint32_t*>(smem + kTableBytes + 512);   // largest |h| per row (bits: NaN counts as largest)
   float* const red = reinterpret_cast<float*>(smem + kTableBytes + 512 + kMaxSlots * 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* const ring = smem + kTableBytes + 512 + kMaxSlots * 4 + RedShape<NT>::kBytes + warp * S::kRing;
+  const uint32_t ring = smem_at(smem) + kTableBytes + 512 + kMaxSlots * 4 + RedShape<NT>::kBytes + warp * S::kRing;
   uint8_t* const panel = smem + UpShape<F, NT>::kFixed;
   pdl_wait();
   pdl_trigger();
@@ -565,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       };
       auto copy_next = [&](int slot) {
         if (next < my_to) {
-          copy_step<F>(smem_at(ring) + slot * S::kSlot, fetch, layout, s);
+          copy_step<F>(ring + slot * S::kSlot, fetch, layout, s);
           s += group;
           settle();
         }
@@ -573,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       };
       if (next < my_to) tile_rows(fetch, next_a, next_u * 8, min(per_expert - next_u, my_to - next));
       settle();
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < S::kDepth; ++i) copy_next(i);
 
       // the panel
@@ -612,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const bool used = (mine >> (8 * n + g)) & 1;
-          x[n].at = used ? panel + rank_below(now, 8 * n + g) * 64 + t * 16 : zeros;
+          x[n].at = used ? smem_at(panel) + rank_below(now, 8 * n + g) * 64 + t * 16 : smem_at(zeros);
           x[n].block = used ? rows * 64 : 0;
         }
         float acc[kTiles][NT][4] = {};
@@ -691,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   uint8_t* const zeros = smem + kTableBytes + 64;
   float* const coef = reinterpret_cast<float*>(smem + kTableBytes + 128);   // of the panel's rows: routing weight and the inverse of the scale
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* const ring = smem + kTableBytes + 128 + kMaxSlots * 4 + warp * S::kRing;
+  const uint32_t ring = smem_at(smem) + kTableBytes + 128 + kMaxSlots * 4 + warp * S::kRing;
   uint8_t* const panel = smem + DownShape<F>::kFixed;
   float* const red = reinterpret_cast<float*>(panel);                     // (after the last panel)
   // What routed the tokens was complete before the kernel ahead of this one let it start.
@@ -768,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
     };
     auto copy_next = [&](int slot) {
       if (left > 0) {
-        copy_step<F>(smem_at(ring) + slot * S::kSlot, fetch, layout, fetch_s);
+        copy_step<F>(ring + slot * S::kSlot, fetch, layout, fetch_s);
         ++fetch_s;
         if (--left == 0) {
           next_stretch();
@@ -780,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       copies_end();
     };
     if (rows_here > 0) next_stretch();
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < S::kDepth; ++i) copy_next(i);
     if (!waited) {
       pdl_wait();
@@ -830,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
           const int row = table.first_row[a], n_rows = table.first_row[a + 1] - row, end = min(stop, (a + 1) * steps);
           // rows of earlier experts in the panel, as above
           const int before = a == a0 ? 0 : (table.first_row[a0 + 1] - row0) * (steps - s0) + (row - table.first_row[a0 + 1]) * steps;
-          const uint8_t* base = panel + (before - (a == a0 ? s0 : 0) * n_rows) * (S::kK * 2);
+          const uint32_t base = smem_at(panel) + (before - (a == a0 ? s0 : 0) * n_rows) * (S::kK * 2);
           const uint32_t mine = table.tokens[a];
           int low[kTiles / 2];
 #pragma unroll
@@ -839,7 +855,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const bool used = (mine >> (8 * n + g)) & 1;
-            x[n].at = used ? base + rank_below(mine, 8 * n + g) * 64 + t * 16 : zeros;
+            x[n].at = used ? base + rank_below(mine, 8 * n + g) * 64 + t * 16 : smem_at(zeros);
             x[n].block = used ? n_rows * 64 : 0;
           }
           float acc[kTiles][NT][4] = {};

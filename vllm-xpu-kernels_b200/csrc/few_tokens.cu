@@ -26,12 +26,13 @@ __device__ __forceinline__ float weight_at(const FewMatrix& w, int64_t e, int n,
     case B200MOE_W_INT4_NK: {
       const uint8_t q = b[(e * N + n) * (K / 2) + k / 2];
       const int v = (int)(((k & 1) ? (q >> 4) : (q & 15)) ^ 8) - 8;
-      return (float)v * to_f32<T>(reinterpret_cast<const T*>(w.scale)[(e * N + n) * (K / w.group) + k / w.group]);
+      const int i = k / (w.group < 128 ? w.group : 128);   // of the row's 16-bit scales, two a word
+      return (float)v * to_f32<T>(reinterpret_cast<const T*>(w.scale)[((e * few_scale_words(w.format, w.group, w.k) + i / 2) * N + n) * 2 + i % 2]);
     }
     default: {
       const uint8_t q = b[(e * N + n) * (K / 2) + k / 2];
       return e2m1_to_f32((k & 1) ? (q >> 4) : (q & 15)) *
-             e8m0_to_f32(reinterpret_cast<const uint8_t*>(w.scale)[(e * N + n) * (K / 32) + k / 32]);
+             e8m0_to_f32(reinterpret_cast<const uint8_t*>(w.scale)[((e * few_scale_words(w.format, 0, w.k) + k / 128) * N + n) * 4 + k / 32 % 4]);
     }
   }
 }
@@ -160,7 +161,7 @@ bool takes_nk(const FewParams& p) {
   if (f != B200MOE_W_FP8_BLOCK_NK && f != B200MOE_W_MXFP4_NK && f != B200MOE_W_INT4_NK) return false;
   for (const void* a : {p.x, p.w13.w, p.w13.scale, p.w2.w, p.w2.scale})
     if (((uintptr_t)a & 15) != 0) return false;
-  return p.hidden % 32 == 0 && p.inter % 32 == 0 && p.hidden <= 16384;
+  return p.hidden % 32 == 0 && p.inter % 32 == 0 && p.hidden <= 16384 && p.inter <= 65536;
 }
 
 bool known_format(int f) {
@@ -188,6 +189,11 @@ int check_matrix(const b200moe_few_tokens_args* a, b200moe_weight_format f, cons
 }  // namespace b200moe
 
 using namespace b200moe;
+
+extern "C" int b200moe_few_tokens_scale_words(b200moe_weight_format format, int group_size, int k) {
+  if (k <= 0 || (format != B200MOE_W_MXFP4_NK && format != B200MOE_W_INT4_NK)) return 0;
+  return few_scale_words(format, group_size, k);
+}
 
 extern "C" size_t b200moe_few_tokens_workspace_bytes(int num_tokens, int topk, int hidden, int inter) {
   if (num_tokens <= 0 || topk <= 0 || hidden <= 0 || inter <= 0) return 0;

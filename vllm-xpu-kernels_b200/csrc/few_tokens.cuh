@@ -30,6 +30,13 @@ struct FewParams {
   FewMatrix w13, w2;
 };
 
+// Words of four bytes that hold a row's scales of a 4-bit matrix, in the order of k: one e8m0 byte per 32 values, or one
+// 16-bit scale per group (per 128 values where groups are longer), as many as whole steps of 128 values take.
+__host__ __device__ __forceinline__ int few_scale_words(int format, int group, int k) {
+  const int steps = (k + 127) / 128;
+  return format == B200MOE_W_MXFP4_NK || group == 64 ? steps : group == 32 ? 2 * steps : (steps + 1) / 2;
+}
+
 // The slot's expert among the local ones, -1 if it has none here.
 __device__ __forceinline__ int local_expert(const FewParams& p, int slot) {
   const int64_t id = p.ids64 ? reinterpret_cast<const int64_t*>(p.ids)[slot] : (int64_t)reinterpret_cast<const int32_t*>(p.ids)[slot];

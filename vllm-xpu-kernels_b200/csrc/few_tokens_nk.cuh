@@ -34,7 +34,7 @@ enum FewFormat { kFewFp8, kFewFp4, kFewInt4Fine, kFewInt4 };   // Fine: groups o
 template <int F> struct FewShape {
   static constexpr int kK = F == kFewFp8 ? 64 : 128;             // values of a row
   static constexpr int kBlocks = kK / 32;                        // of the panel: a lane's eight values, two instructions
-  static constexpr int kScaleWords = F == kFewFp8 || F == kFewInt4 ? 1 : F == kFewFp4 ? 2 : 3;   // that hold a row's scales of a step
+  static constexpr int kScaleWords = F == kFewInt4Fine ? 2 : 1;  // that hold a row's scales of a step
   static constexpr int kScales = F == kFewFp8 ? 0 : F == kFewInt4 ? 1 : 4;                       // of a row and step, made fp32 (fp8: are so)
   static constexpr int kSlot = kRows * (64 + 4 * kScaleWords);
   static constexpr int kDepth = 3;
@@ -53,25 +53,26 @@ struct FewTable {
   int first_row[kMaxSlots + 1];
   int slot_expert[kMaxSlots];      // the slot's expert, as an index of the active ones (-1: none)
   uint16_t row_expert[kMaxSlots];
-  uint16_t row_token[kMaxSlots];
   float weight[kMaxSlots];         // of a row: the sum over the slots that name its expert
 };
 
 __device__ __forceinline__ int rank_below(uint32_t mask, int bit) { return __popc(mask & ((1u << bit) - 1u)); }
 
+// By one warp; the others meet it at the block's next barrier.
 template <bool kWeights>
 __device__ __forceinline__ void build_table(FewTable& t, const FewParams& p) {
-  const int slots = p.tokens * p.topk, tid = threadIdx.x, lane = tid & 31;
-  if (tid < 32) t.bits[tid] = 0;
-  for (int i = tid; i < slots; i += kThreads) t.tokens[i] = 0;
-  __syncthreads();
-  for (int i = tid; i < slots; i += kThreads) {
+  const int slots = p.tokens * p.topk, lane = threadIdx.x & 31;
+  t.bits[lane] = 0;
+  for (int i = lane; i < slots; i += 32) t.tokens[i] = 0;
+  __syncwarp();
+#pragma unroll 1
+  for (int i = lane; i < slots; i += 32) {
     const int e = local_expert(p, i);
     t.slot_expert[i] = e;
     if (e >= 0) atomicOr(&t.bits[e >> 5], 1u << (e & 31));
   }
-  __syncthreads();
-  if (tid < 32) {
+  __syncwarp();
+  {
     const int n = __popc(t.bits[lane]);
     int sum = n;
 #pragma unroll
@@ -82,48 +83,51 @@ __device__ __forceinline__ void build_table(FewTable& t, const FewParams& p) {
     t.before[lane] = sum - n;
     if (lane == 31) t.active = sum;
   }
-  __syncthreads();
-  for (int i = tid; i < slots; i += kThreads) {
-    const int e = t.slot_expert[i];
+  __syncwarp();
+  bool again = false;      // a token that names an expert twice
+#pragma unroll 1
+  for (int i = lane; i < slots; i += 32) {
+    const int e = t.slot_expert[i], tok = i / p.topk;
     if (e < 0) continue;
     const int a = t.before[e >> 5] + rank_below(t.bits[e >> 5], e & 31);
     t.slot_expert[i] = a;
     t.expert[a] = e;
-    atomicOr(&t.tokens[a], 1u << (i / p.topk));
+    again |= (atomicOr(&t.tokens[a], 1u << tok) >> tok) & 1;
   }
-  __syncthreads();
-  if (tid < 32) {
-    int base = 0;
-    for (int a0 = 0; a0 < t.active; a0 += 32) {
-      const int a = a0 + lane, n = a < t.active ? __popc(t.tokens[a]) : 0;
-      int sum = n;
+  again = __any_sync(0xffffffffu, again);
+  __syncwarp();
+  int base = 0;
+#pragma unroll 1
+  for (int a0 = 0; a0 < t.active; a0 += 32) {
+    const int a = a0 + lane, n = a < t.active ? __popc(t.tokens[a]) : 0;
+    int sum = n;
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, sum, d);
-        if (lane >= d) sum += o;
-      }
-      if (a < t.active) t.first_row[a] = base + sum - n;
-      base += __shfl_sync(0xffffffffu, sum, 31);
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
     }
-    if (lane == 0) { t.first_row[t.active] = base; t.rows = base; }
+    if (a < t.active) t.first_row[a] = base + sum - n;
+    base += __shfl_sync(0xffffffffu, sum, 31);
   }
-  __syncthreads();
+  if (lane == 0) { t.first_row[t.active] = base; t.rows = base; }
+  __syncwarp();
   if (kWeights) {
-    for (int i = tid; i < slots; i += kThreads) {
-      const int a = t.slot_expert[i], tok = i / p.topk, k0 = tok * p.topk;
+#pragma unroll 1
+    for (int i = lane; i < slots; i += 32) {
+      const int a = t.slot_expert[i], tok = i / p.topk;
       if (a < 0) continue;
-      bool again = false;
-      for (int j = k0; j < i; ++j) again |= t.slot_expert[j] == a;
-      if (again) continue;
-      float w = 0.f;
-      for (int j = i; j < k0 + p.topk; ++j)
-        if (t.slot_expert[j] == a) w += p.weights[j];
+      float w = p.weights[i];
+      if (again) {    // the token's slots with this expert in their order, by the first of them
+        bool other = false;
+        for (int j = tok * p.topk; j < i; ++j) other |= t.slot_expert[j] == a;
+        if (other) continue;
+        for (int j = i + 1; j < (tok + 1) * p.topk; ++j)
+          if (t.slot_expert[j] == a) w += p.weights[j];
+      }
       const int row = t.first_row[a] + rank_below(t.tokens[a], tok);
       t.weight[row] = w;
       t.row_expert[row] = (uint16_t)a;
-      t.row_token[row] = (uint16_t)tok;
     }
-    __syncthreads();
   }
 }
 
@@ -132,9 +136,8 @@ __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
-// `bytes` of the four come from memory, the rest are zeros.
-__device__ __forceinline__ void copy4(uint32_t to, const void* from, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -277,36 +280,41 @@ __device__ __forceinline__ float row_top(const void* src, int source, int k, int
   for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
   return top;
 }
-// Warps of a row where a panel has `rows` of them.
-__device__ __forceinline__ int warps_per_row(int rows) { return rows == 1 ? 8 : rows == 2 ? 4 : rows <= 4 ? 2 : 1; }
+// Warps of a row where `warps` of them fill a panel of `rows`.
+__device__ __forceinline__ int warps_per_row(int rows, int warps) { return rows >= warps ? 1 : warps / rows; }
 
 // ---- weights: a warp's ring ------------------------------------------------------------
 // fp8: a lane reads the bytes that it fetched.  4 bits: a lane fetches 16 bytes of a row, which is a group of 32 values, and
 // reads a word of each of the row's four groups; the groups' places are swapped so that the eight rows of a read fall on
-// different banks.  The scales of a row are fetched and made fp32 by one lane per row.
+// different banks.  Scales are fetched as words, neighbouring rows by neighbouring lanes (those of 4-bit formats are laid out
+// for that: as they come, a step's would be 2 or 4 bytes of every row, which kept the load units busy for longer than the
+// weights did), and made fp32 by one lane per row.
 
-// The lane's part of 64 rows of one expert's matrix.
+// The lane's part of the rows of one expert's matrix that a warp takes at once.
 struct FewRows {
-  const uint8_t* w;              // its 16 bytes of step 0 in row g (lane = 4 g + t)
-  int64_t to[2 * kTiles];        // from there to rows g + 8 i
-  const uint8_t* s[kTiles / 2];  // first byte of the scales of the rows that it looks after, lane + 32 i
-  int tiles;                     // that there are
+  const uint8_t* w;                       // its 16 bytes of step 0 in row g (lane = 4 g + t)
+  int64_t to[2 * kTiles];                 // from there to rows g + 8 i
+  const uint8_t* s[kRows / 32];           // scales of step 0 of the rows that it looks after, places lane + 32 i
+  bool there[kRows / 32];                 // whether these rows are
+  int tiles;                              // that there are
 };
 // The matrix as a whole.
 struct FewLayout {
-  int row_bytes, scale_bytes, group;
+  int row_bytes, group;
+  int64_t word_step;     // bytes from one word of a row's scales to the next
   bool f16;
   __device__ __forceinline__ FewLayout(const FewMatrix& m, int f, bool half) {
     row_bytes = f == kFewFp8 ? m.k : m.k / 2;
-    scale_bytes = f == kFewFp8 ? m.k / 128 * 4 : f == kFewFp4 ? m.k / 32 : m.k / m.group * 2;
     group = m.group;
+    word_step = f == kFewFp8 ? 4 : 4 * (int64_t)m.n;
     f16 = half;
   }
 };
-// Byte of a row's scales where those of step s begin.
+// Scales of step 0 of row n.  4 bits: [experts][words][n], words as in few_scale_words.
 template <int F>
-__device__ __forceinline__ int scale_offset(const FewLayout& l, int s) {
-  return F == kFewFp8 ? s >> 1 << 2 : F == kFewFp4 ? 4 * s : (s * 128) / l.group * 2;
+__device__ __forceinline__ const uint8_t* scales_of(const FewMatrix& m, int64_t e, int n) {
+  if (F == kFewFp8) return reinterpret_cast<const uint8_t*>(m.scale) + ((e * (m.n / 128) + n / 128) * (m.k / 128)) * 4;
+  return reinterpret_cast<const uint8_t*>(m.scale) + (e * few_scale_words(m.format, m.group, m.k) * m.n + n) * 4;
 }
 
 // Fetches step s into a slot.
@@ -325,43 +333,41 @@ __device__ __forceinline__ void copy_step(uint32_t slot, const FewRows& r, const
       copy16(to + i * 1024 + 512, w + r.to[2 * i + 1]);
     }
   }
-  // the words that hold the step's scales (they need not begin at one), as far as the row goes
-  const int off = scale_offset<F>(l, s);
+  // (a word serves two steps of fp8, whose blocks are 128 long, and of int4 with one scale of 16 bits per step)
+  const bool two = F == kFewInt4Fine && l.group == 32;
+  const int word = F == kFewFp8 || F == kFewInt4 ? s >> 1 : two ? 2 * s : s;
 #pragma unroll
-  for (int j = 0; j < kTiles / 2; ++j) {
-    if (2 * j >= r.tiles) break;
-    const int skip = F == kFewFp8 ? 0 : (int)((uintptr_t)r.s[j] + off) & 3;
-    const uint8_t* from = r.s[j] + off - skip;
-    const int left = l.scale_bytes - off + skip;
+  for (int j = 0; j < kRows / 32; ++j) {
+    if (!r.there[j]) continue;
 #pragma unroll
     for (int i = 0; i < S::kScaleWords; ++i)
-      copy4(slot + kRows * 64 + ((j * 32 + lane) * S::kScaleWords + i) * 4, i == 0 || left > 4 * i ? from + 4 * i : from, max(0, min(4, left - 4 * i)));
+      if (i == 0 || two) copy4(slot + kRows * 64 + ((j * 32 + lane) * S::kScaleWords + i) * 4, r.s[j] + (word + i) * l.word_step);
   }
 }
 
-// The scales of the step in the slot, of the rows that the lane looks after, as fp32.  low: the two lowest bits of their addresses.
+// The scales of step s, which is in the slot, as fp32.
 template <int F>
-__device__ __forceinline__ void spread_scales(uint32_t to, uint32_t slot, const int (&low)[kTiles / 2], int tiles, const FewLayout& l, int s) {
+__device__ __forceinline__ void spread_scales(uint32_t to, uint32_t slot, const FewLayout& l, int s) {
   using S = FewShape<F>;
 #pragma unroll
-  for (int j = 0; j < kTiles / 2; ++j) {
-    if (2 * j >= tiles) break;
+  for (int j = 0; j < kRows / 32; ++j) {
     const int row = j * 32 + (threadIdx.x & 31);
-    const uint32_t w = slot + kRows * 64 + row * S::kScaleWords * 4;
-    const int shift = F == kFewFp4 ? low[j] * 8 : ((low[j] + scale_offset<F>(l, s)) & 3) * 8;
+    const uint32_t at = slot + kRows * 64 + row * S::kScaleWords * 4, v = lds4(at);
     auto value = [&](uint32_t h) { return l.f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16); };
     if constexpr (F == kFewFp4) {
       // 2^(byte - 127): the byte is the exponent (0 gives zero for 2^-127, 255 infinity for NaN)
-      const uint32_t v = __funnelshift_r(lds4(w), lds4(w + 4), shift);
       sts16(to + row * 16, __uint_as_float((v & 255u) << 23), __uint_as_float((v << 15) & 0x7f800000u),
             __uint_as_float((v << 7) & 0x7f800000u), __uint_as_float((v >> 1) & 0x7f800000u));
     } else if constexpr (F == kFewInt4) {
-      sts4(to + row * 4, value((lds4(w) >> shift) & 0xffffu));
+      sts4(to + row * 4, value(s & 1 ? v >> 16 : v & 0xffffu));
     } else if constexpr (F == kFewInt4Fine) {
-      const uint32_t mid = lds4(w + 4), lo = __funnelshift_r(lds4(w), mid, shift), hi = __funnelshift_r(mid, lds4(w + 8), shift);
-      const float a = value(lo & 0xffffu), b = value(lo >> 16);
-      const bool fine = l.group == 32;
-      sts16(to + row * 16, a, fine ? b : a, fine ? value(hi & 0xffffu) : b, fine ? value(hi >> 16) : b);
+      const float a = value(v & 0xffffu), b = value(v >> 16);
+      if (l.group == 32) {
+        const uint32_t h = lds4(at + 4);
+        sts16(to + row * 16, a, b, value(h & 0xffffu), value(h >> 16));
+      } else {
+        sts16(to + row * 16, a, a, b, b);
+      }
     }
   }
 }
@@ -373,8 +379,8 @@ struct FewTokens {
 };
 
 // acc += W x of the step in the slot, for the first `Tiles` tiles (what one of them has not got is something finite or not, in
-// rows that nobody reads).
-template <int F, int NT, int Tiles>
+// rows that nobody reads).  kHalves: scales lie as [8 rows g of all tiles][8 rows g + 8 of all tiles], else row by row.
+template <int F, int NT, int Tiles, bool kHalves>
 __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint32_t slot, uint32_t scales,
                                               const FewTokens (&x)[NT], int s) {
   using S = FewShape<F>;
@@ -386,6 +392,7 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
     for (int q = 0; q < S::kBlocks; ++q) v[q][n] = lds16(x[n].at + (s * S::kBlocks + q) * x[n].block);
 #pragma unroll
   for (int i = 0; i < Tiles; ++i) {
+    const int at_lo = kHalves ? 8 * i + g : 16 * i + g, at_hi = at_lo + (kHalves ? kRows / 2 : 8);   // places of the scales
     float d[NT][4];
     auto add = [&](float a, float b) {
 #pragma unroll
@@ -411,16 +418,15 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
           else mma(d[n], a0, a1, a2, a3, w & 1 ? b.z : b.x, w & 1 ? b.w : b.y);
         }
       }
-      const uint32_t sc = slot + kRows * 64 + (16 * i + g) * 4;
-      add(ldsf(sc), ldsf(sc + 32));
+      add(ldsf(slot + kRows * 64 + at_lo * 4), ldsf(slot + kRows * 64 + at_hi * 4));
     } else {
       uint4 lo, hi;
       if constexpr (S::kScales == 4) {
-        lo = lds16(scales + (16 * i + g) * 16);
-        hi = lds16(scales + (16 * i + 8 + g) * 16);
+        lo = lds16(scales + at_lo * 16);
+        hi = lds16(scales + at_hi * 16);
       } else {
-        lo.w = lds4(scales + (16 * i + g) * 4);
-        hi.w = lds4(scales + (16 * i + 8 + g) * 4);
+        lo.w = lds4(scales + at_lo * 4);
+        hi.w = lds4(scales + at_hi * 4);
       }
       const uint32_t w = slot + i * 1024 + g * 64 + t * 4;
 #pragma unroll
@@ -444,16 +450,15 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
 }
 
 // Takes the step in the slot and fetches the next one into it.
-template <int F, int NT, typename Next>
-__device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], uint32_t ring, int& slot, const int (&low)[kTiles / 2], int tiles,
-                                          const FewLayout& l, const FewTokens (&x)[NT], int s, int panel_step, Next next) {
+template <int F, int NT, bool kHalves, typename Next>
+__device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], uint32_t ring, int& slot, int tiles, const FewLayout& l, const FewTokens (&x)[NT], int s, int panel_step, Next next) {
   using S = FewShape<F>;
   const uint32_t scales = ring + S::kDepth * S::kSlot, at = ring + slot * S::kSlot;
   copies_wait<S::kDepth - 1>();
-  if (F != kFewFp8) spread_scales<F>(scales, at, low, tiles, l, s);
+  if (F != kFewFp8) spread_scales<F>(scales, at, l, s);
   __syncwarp();
-  if (tiles > kTiles / 2) multiply_step<F, NT, kTiles>(acc, at, scales, x, panel_step);
-  else multiply_step<F, NT, kTiles / 2>(acc, at, scales, x, panel_step);
+  if (tiles > kTiles / 2) multiply_step<F, NT, kTiles, kHalves>(acc, at, scales, x, panel_step);
+  else multiply_step<F, NT, kTiles / 2, kHalves>(acc, at, scales, x, panel_step);
   __syncwarp();
   next(slot);
   slot = slot + 1 == S::kDepth ? 0 : slot + 1;
@@ -476,7 +481,25 @@ struct FewLaunch {
 
 constexpr int kTableBytes = (sizeof(FewTable) + 127) / 128 * 128;
 // Sums of the warps, for their owner to add up.
-template <int NT> struct RedShape { static constexpr int kWarpFloats = kTiles * NT * 4 * 32, kBytes = kWarps * kWarpFloats * 4; };
+template <int NT> struct RedShape {
+  static constexpr int kTile = NT * 4 * 32 + 1;      // (off the banks of the tile before)
+  static constexpr int kWarpFloats = kTiles * kTile, kBytes = (kWarps * kWarpFloats * 4 + 127) / 128 * 128;
+  // Where the sums of row `row` (of a tile's 16) and column `col` are.
+  static __device__ __forceinline__ int at(int tile, int row, int col) {
+    return tile * kTile + ((col >> 3) * 4 + (row >> 3) * 2 + (col & 1)) * 32 + (row & 7) * 4 + ((col & 7) >> 1);
+  }
+};
+// A warp's sums to its place.
+template <int NT>
+__device__ __forceinline__ void store_sums(float* red, const float (&acc)[kTiles][NT][4]) {
+  float* const to = red + (threadIdx.x >> 5) * RedShape<NT>::kWarpFloats + (threadIdx.x & 31);
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) to[i * RedShape<NT>::kTile + (n * 4 + c) * 32] = acc[i][n][c];
+}
 template <int F, int NT> struct UpShape {
   static constexpr int kFixed = kTableBytes + 512 + kMaxSlots * 4 + RedShape<NT>::kBytes + kWarps * FewShape<F>::kRing;
 };
@@ -502,58 +525,91 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
   uint8_t* const panel = smem + UpShape<F, NT>::kFixed;
   pdl_wait();
   pdl_trigger();
-  if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0;
-  for (int i = tid; i < p.tokens * p.topk; i += kThreads) h_top[i] = 0;
-  if (blockIdx.x == 0)   // (the second kernel counts from there)
-    for (int i = tid; i < kFewMaxColumns; i += kThreads) launch.arrived[i] = 0;
-  build_table<false>(table, p);
   const FewMatrix& m = p.w13;
   const FewLayout layout(m, F, launch.f16);
   const int steps = (p.hidden + S::kK - 1) / S::kK, per_expert = p.inter / 8;
-  const int64_t all = (int64_t)table.active * per_expert;
+  const int most = launch.panel_bytes / (steps * S::kK * 2);      // rows that the panel holds
+  const bool whole = most >= p.tokens;                            // all tokens
+  if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0;
+  // The panel's row `row`: token `token`, by `parts` warps that have barrier `id` to themselves.
+  auto fill_row = [&](int row, int rows, int token, bool there, int warps, int id) {
+    const int parts = warps_per_row(rows, warps), part = (warp + warps - kWarps) % parts, k8 = steps * (S::kK / 8);
+    const int source = launch.f16 ? kFromF16 : kFromBf16;
+    const uint8_t* x = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)token * p.hidden * 2;
+    float top = there ? row_top(x, source, p.hidden, 0, k8, part, parts) : 0.f;
+    if (parts > 1) {
+      if (lane == 0) tops[warp] = top;
+      group_sync(id, warps * 32);
+      for (int i = 0; i < parts; ++i) top = max_nan(top, tops[warp - part + i]);
+    }
+    if (there) {
+      float inv;
+      const float scale = row_scale(top, inv);
+      if (lane == 0 && part == 0) inverse[row] = inv;
+      convert_row<F>(panel, row, rows, x, source, p.hidden, 0, k8, scale, part, parts);
+    }
+  };
+  // Rows in turn; where there are fewer than warps, all at once with several warps each.
+  auto fill_panel = [&](uint32_t now, int warps, int id) {
+    const int rows = __popc(now), parts = warps_per_row(rows, warps), first = (warp + warps - kWarps) / parts, step = warps / parts;
+#pragma unroll 1
+    for (int row = first, turn = 0; turn < rows; row += step, turn += step) {
+      uint32_t left = now;
+      for (int i = 0; i < row && left; ++i) left &= left - 1;
+      fill_row(row, rows, left ? __ffs(left) - 1 : 0, row < rows, warps, id);
+    }
+  };
+  if (warp == 0) {
+    build_table<false>(table, p);
+  } else {
+    for (int i = tid - 32; i < p.tokens * p.topk; i += kThreads - 32) h_top[i] = 0;
+    if (blockIdx.x == 0)   // (the second kernel counts from there)
+      for (int i = tid - 32; i < kFewMaxColumns; i += kThreads - 32) launch.arrived[i] = 0;
+    if (whole) fill_panel((1u << p.tokens) - 1u, kWarps - 1, 1);
+  }
+  __syncthreads();
+  const uint32_t all = (uint32_t)(table.active * per_expert);     // (times the blocks below 2^32: takes_nk)
   const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
   const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
-  const int most = launch.panel_bytes / (steps * S::kK * 2);      // rows that the panel holds
 
+#pragma unroll 1
   for (int from = begin; from < end;) {
-    // as many experts as have their tokens in the panel at once; one with more tokens than that goes through its
-    // features again with the rest of them
-    const int a0 = from / per_expert;
-    uint32_t tokens = table.tokens[a0];
-    int to = min(end, (a0 + 1) * per_expert);
-    if (__popc(tokens) <= most) {
-      for (int a = a0 + 1; to < end && __popc(tokens | table.tokens[a]) <= most; ++a) {
-        tokens |= table.tokens[a];
-        to = min(end, (a + 1) * per_expert);
+    // As many experts as have their tokens in the panel at once; one with more tokens than that goes through its
+    // features again with the rest of them.
+    uint32_t tokens = (1u << p.tokens) - 1u;
+    int to = end;
+    if (!whole) {
+      const int a0 = from / per_expert;
+      tokens = table.tokens[a0];
+      to = min(end, (a0 + 1) * per_expert);
+      if (__popc(tokens) <= most) {
+        for (int a = a0 + 1; to < end && __popc(tokens | table.tokens[a]) <= most; ++a) {
+          tokens |= table.tokens[a];
+          to = min(end, (a + 1) * per_expert);
+        }
       }
     }
     // Warps of a group: few where there are many tiles, as every tile's sums cost a barrier of the group; many where there
     // are few, so that all have work.
-    int group = kWarps;
+    int shift = 0;
     {
       int least = 1 << 30;
 #pragma unroll
-      for (int w = 1; w <= kWarps; w *= 2) {
-        const int pieces = ((to - from) * w + kWarps - 1) / kWarps, tiles = (pieces + kTiles - 1) / kTiles;
-        const int cost = (steps + w - 1) / w * (pieces + tiles) + tiles * (w > 1 ? 8 : 4);
-        if (cost < least) { least = cost; group = w; }
+      for (int w = 0; (1 << w) <= kWarps; ++w) {
+        const int pieces = (((to - from) << w) + kWarps - 1) / kWarps, tiles = (pieces + kTiles - 1) / kTiles;
+        const int cost = ((steps + (1 << w) - 1) >> w) * (pieces + tiles) + tiles * (w > 0 ? 8 : 4);
+        if (cost < least) { least = cost; shift = w; }
       }
     }
-    const int groups = kWarps / group, mine_of = warp / group, member = warp % group;
-    const int my_from = from + (to - from) * mine_of / groups, my_to = from + (to - from) * (mine_of + 1) / groups;
+    const int group = 1 << shift, mine_of = warp >> shift, member = warp & (group - 1);
+    const int my_from = from + (((to - from) * mine_of << shift) / kWarps), my_to = from + (((to - from) * (mine_of + 1) << shift) / kWarps);
 
+#pragma unroll 1
     for (uint32_t rest = tokens; rest;) {
       uint32_t now = rest;
       while (__popc(now) > most) now &= ~(1u << (31 - __clz(now)));
       rest &= ~now;
-      const int rows = __popc(now);
 
-      // scales of the rows that the lane looks after, where features [f, f + 8 tiles) begin
-      auto scale_row = [&](int64_t e, int f, int tiles, int j) {
-        const int row = j * 32 + lane, piece = row < 16 * tiles ? row >> 4 : 0, fs = f + piece * 8 + (row & 7), up = (row >> 3) & 1;
-        const int64_t n = pairs ? 2 * fs + up : fs + up * p.inter;
-        return reinterpret_cast<const uint8_t*>(m.scale) + (F == kFewFp8 ? e * (m.n / 128) + n / 128 : e * m.n + n) * layout.scale_bytes;
-      };
       auto tile_rows = [&](FewRows& r, int a, int f, int last) {       // of the tiles that begin with feature f
         const int64_t e = table.expert[a], rb = layout.row_bytes;
         r.tiles = min(kTiles, last);
@@ -564,7 +620,12 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
           r.to[2 * i + 1] = r.to[2 * i] + (pairs ? rb : p.inter * rb);
         }
 #pragma unroll
-        for (int j = 0; j < kTiles / 2; ++j) r.s[j] = scale_row(e, f, r.tiles, j);
+        for (int j = 0; j < kRows / 32; ++j) {
+          // gates in the first half of the places, ups in the second
+          const int place = j * 32 + lane, up = place >= kRows / 2, fs = place % (kRows / 2);
+          r.there[j] = fs < 8 * r.tiles;
+          r.s[j] = scales_of<F>(m, e, r.there[j] ? (pairs ? 2 * (f + fs) + up : f + fs + up * p.inter) : 0);
+        }
       };
       // the ring begins to fill
       // of the step that is fetched next: its tiles' first piece (of all, and within its expert), the expert
@@ -587,43 +648,22 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         }
         copies_end();
       };
+      int a = next_a, u = next_u;
       if (next < my_to) tile_rows(fetch, next_a, next_u * 8, min(per_expert - next_u, my_to - next));
       settle();
 #pragma unroll 1
       for (int i = 0; i < S::kDepth; ++i) copy_next(i);
-
-      // the panel
-      {
-        const int parts = warps_per_row(rows), part = warp % parts;
-        const int source = launch.f16 ? kFromF16 : kFromBf16, k8 = steps * (S::kK / 8);
-        for (int row = warp / parts, q0 = 0; q0 < rows; q0 += kWarps / parts, row += kWarps / parts) {   // (once where a row has several warps)
-          uint32_t left_tokens = now;
-          for (int i = 0; i < row; ++i) left_tokens &= left_tokens - 1;
-          const bool there = row < rows;
-          const uint8_t* x = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)(there ? __ffs(left_tokens) - 1 : 0) * p.hidden * 2;
-          float top = there ? row_top(x, source, p.hidden, 0, k8, part, parts) : 0.f;
-          if (parts > 1) {
-            if (lane == 0) tops[warp] = top;
-            __syncthreads();
-            for (int i = 0; i < parts; ++i) top = max_nan(top, tops[row * parts + i]);
-          }
-          if (there) {
-            float inv;
-            const float scale = row_scale(top, inv);
-            if (lane == 0 && part == 0) inverse[row] = inv;
-            convert_row<F>(panel, row, rows, x, source, p.hidden, 0, k8, scale, part, parts);
-          }
-        }
+      if (!whole) {
+        fill_panel(now, kWarps, 0);
         __syncthreads();
       }
+      const int rows = whole ? p.tokens : __popc(now);
 
-      int slot = 0, cs = member, a = my_from / per_expert, u = my_from - a * per_expert;
+      int slot = 0, cs = member;
+#pragma unroll 1
       for (int first = my_from; first < my_to;) {
         const int tiles = min(kTiles, min(per_expert - u, my_to - first));
         const uint32_t mine = table.tokens[a] & now;
-        int low[kTiles / 2];
-#pragma unroll
-        for (int j = 0; j < kTiles / 2; ++j) low[j] = F == kFewFp8 ? 0 : (int)((uintptr_t)scale_row(table.expert[a], u * 8, tiles, j) & 3);
         FewTokens x[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -632,53 +672,43 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
           x[n].block = used ? rows * 64 : 0;
         }
         float acc[kTiles][NT][4] = {};
-        for (; cs < steps; cs += group) take_step<F, NT>(acc, ring, slot, low, tiles, layout, x, cs, cs, copy_next);
+#pragma unroll 1
+        for (; cs < steps; cs += group) take_step<F, NT, true>(acc, ring, slot, tiles, layout, x, cs, cs, copy_next);
         cs -= steps;
-        auto finish = [&](int i, int col, int f_in_tile, float gate, float up) {
-          if (i >= tiles || !((mine >> col) & 1)) return;
-          const float inv = inverse[rank_below(now, col)];
-          const int f = (u + i) * 8 + f_in_tile;
-          gate *= inv;
-          up *= inv;
-          if (m.bias) {
-            const int64_t at = (int64_t)table.expert[a] * m.n;
-            gate += load16(m.bias, at + (pairs ? 2 * f : f), launch.f16);
-            up += load16(m.bias, at + (pairs ? 2 * f + 1 : p.inter + f), launch.f16);
-          }
-          const int row = table.first_row[a] + rank_below(table.tokens[a], col);
-          const float h = gated(p, gate, up);
-          p.h[(int64_t)row * p.inter + f] = h;
-          atomicMax(&h_top[row], __float_as_uint(h) & 0x7fffffffu);
-        };
-        if (group == 1) {
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) finish(i, 8 * n + 2 * t + c, g, acc[i][n][c], acc[i][n][c + 2]);
-        } else {
-          constexpr int kWarpFloats = RedShape<NT>::kWarpFloats;
-          float* const to_red = red + warp * kWarpFloats + lane;
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) to_red[((i * NT + n) * 4 + c) * 32] = acc[i][n][c];
-          group_sync(1 + mine_of, group * 32);
-          for (int j = member * 32 + lane; j < kTiles * NT * 64; j += group * 32) {
-            const int l2 = j & 31, c = (j >> 5) & 1, n = (j >> 6) % NT, i = (j >> 6) / NT;
+        // The tile's sums: a lane has a feature, the members take the tokens in turn.
+        store_sums<NT>(red, acc);
+        if (group > 1) group_sync(1 + mine_of, group * 32);
+        else __syncwarp();
+        const int i = lane >> 3, f = (u + i) * 8 + (lane & 7);
+        int turn = 0;
+        for (uint32_t left = mine; left; left &= left - 1, ++turn) {
+          if ((turn & (group - 1)) != member) continue;
+          const int col = __ffs(left) - 1, row = table.first_row[a] + rank_below(table.tokens[a], col);
+          float h = 0.f;
+          if (i < tiles) {
+            const float* from_red = red + (warp - member) * RedShape<NT>::kWarpFloats;
             float gate = 0.f, up = 0.f;
-            const float* from_red = red + (warp - member) * kWarpFloats + ((i * NT + n) * 4 + c) * 32 + l2;
             for (int w = 0; w < group; ++w) {
-              gate += from_red[w * kWarpFloats];
-              up += from_red[w * kWarpFloats + 64];
+              gate += from_red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(i, lane & 7, col)];
+              up += from_red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(i, 8 + (lane & 7), col)];
             }
-            finish(i, 8 * n + 2 * (l2 & 3) + c, l2 >> 2, gate, up);
+            const float inv = inverse[rank_below(now, col)];
+            gate *= inv;
+            up *= inv;
+            if (m.bias) {
+              const int64_t at = (int64_t)table.expert[a] * m.n;
+              gate += load16(m.bias, at + (pairs ? 2 * f : f), launch.f16);
+              up += load16(m.bias, at + (pairs ? 2 * f + 1 : p.inter + f), launch.f16);
+            }
+            h = gated(p, gate, up);
+            p.h[(int64_t)row * p.inter + f] = h;
           }
-          group_sync(1 + mine_of, group * 32);   // the sums' place is free again
+          uint32_t top = __float_as_uint(h) & 0x7fffffffu;
+          top = __reduce_max_sync(0xffffffffu, top);
+          if (lane == 0) atomicMax(&h_top[row], top);
         }
+        if (group > 1) group_sync(1 + mine_of, group * 32);   // the sums' place is free again
+        else __syncwarp();
         first += tiles;
         u += tiles;
         if (u == per_expert) { u = 0; ++a; }
@@ -711,14 +741,15 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   uint8_t* const panel = smem + DownShape<F>::kFixed;
   float* const red = reinterpret_cast<float*>(panel);                     // (after the last panel)
   // What routed the tokens was complete before the kernel ahead of this one let it start.
-  if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0;
-  build_table<true>(table, p);
+  if (warp == 0) build_table<true>(table, p);
+  else if (tid < 48) reinterpret_cast<uint32_t*>(zeros)[tid - 32] = 0;
+  __syncthreads();
   const FewMatrix& m = p.w2;
   const FewLayout layout(m, F, launch.f16);
   const int steps = (p.inter + S::kK - 1) / S::kK;
   const int columns = gridDim.x / launch.splits, column = blockIdx.x % columns, split = blockIdx.x / columns;
-  const int row_begin = (int)((int64_t)p.hidden * column / columns), row_end = (int)((int64_t)p.hidden * (column + 1) / columns);
-  const int64_t total = (int64_t)table.active * steps;
+  const int row_begin = (int)((uint32_t)p.hidden * column / columns), row_end = (int)((uint32_t)p.hidden * (column + 1) / columns);
+  const uint32_t total = (uint32_t)(table.active * steps);
   const int step_begin = (int)(total * split / launch.splits), step_end = (int)(total * (split + 1) / launch.splits);
   const int per_expert = p.inter / 8;                                     // (as the first kernel deals its features out)
   const int room = launch.panel_bytes / (S::kK * 2);                      // rows times steps that the panel holds
@@ -753,19 +784,18 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   };
   for (int r0 = row_begin; r0 < row_end || !waited; r0 += kRows) {
     const int rows_here = max(0, min(kRows, row_end - r0)), tiles = (rows_here + 15) / 16;
-    auto scale_row = [&](int a, int j) {
-      const int64_t n = r0 + min(j * 32 + lane, rows_here - 1), e = table.expert[a];
-      return reinterpret_cast<const uint8_t*>(m.scale) + (F == kFewFp8 ? e * (m.n / 128) + n / 128 : e * m.n + n) * layout.scale_bytes;
-    };
     FewRows fetch;
     fetch.tiles = tiles;
 #pragma unroll
     for (int i = 0; i < 2 * kTiles; ++i)
       fetch.to[i] = (int64_t)max(0, min(8 * i + g, rows_here - 1)) * layout.row_bytes;   // (what a tile has not got is the last row again)
-    auto expert_rows = [&](int a) {
-      fetch.w = reinterpret_cast<const uint8_t*>(m.w) + ((int64_t)table.expert[a] * m.n + r0) * layout.row_bytes + t * 16;
 #pragma unroll
-      for (int j = 0; j < kTiles / 2; ++j) fetch.s[j] = scale_row(a, j);
+    for (int j = 0; j < kRows / 32; ++j) fetch.there[j] = j * 32 + lane < rows_here;
+    auto expert_rows = [&](int a) {
+      const int64_t e = table.expert[a];
+      fetch.w = reinterpret_cast<const uint8_t*>(m.w) + (e * m.n + r0) * layout.row_bytes + t * 16;
+#pragma unroll
+      for (int j = 0; j < kRows / 32; ++j) fetch.s[j] = scales_of<F>(m, e, fetch.there[j] ? r0 + j * 32 + lane : r0);
     };
     // The step that is fetched next, the end of this warp's stretch, and where the panel after that begins.
     int fetch_a = 0, fetch_s = 0, left = 0, panel_a = step_begin / steps, panel_s = step_begin - panel_a * steps;
@@ -811,16 +841,17 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       const int last = s1 > 0 ? a1 : a1 - 1;           // the last expert with steps in the panel
       const int row0 = table.first_row[a0], rows = table.first_row[last + 1] - row0;
       {
-        const int parts = warps_per_row(rows), row = warp / parts, part = warp % parts;
-        for (int q0 = 0; q0 < rows; q0 += kWarps / parts) {   // (once where a row has several warps)
+        const int parts = warps_per_row(rows, kWarps), row = warp / parts, part = warp % parts;   // (several warps have a row where there are fewer rows)
+#pragma unroll 1
+        for (int q0 = 0; q0 < rows; q0 += kWarps / parts) {
           const int r = row0 + q0 + row;
           const bool there = q0 + row < rows;
           const int a = there ? table.row_expert[r] : a0;
           const int k8_0 = (a == a0 ? s0 : 0) * (S::kK / 8), k8_1 = (a == a1 ? s1 : steps) * (S::kK / 8);
-          if (there) {
+          if (there && row < kWarps / parts) {
             // the largest |h| of the row, over the blocks of the first kernel that had features of its expert
-            const int64_t all = (int64_t)table.active * per_expert, g1 = launch.up_blocks;
-            const int c0 = (int)((((int64_t)a * per_expert + 1) * g1 - 1) / all), c1 = (int)(((int64_t)(a + 1) * per_expert * g1 - 1) / all);
+            const uint32_t all = (uint32_t)(table.active * per_expert), g1 = launch.up_blocks;
+            const int c0 = (int)((((uint32_t)(a * per_expert) + 1) * g1 - 1) / all), c1 = (int)(((uint32_t)((a + 1) * per_expert) * g1 - 1) / all);
             float top = 0.f;
             for (int c = c0 + lane; c <= c1; c += 32)   // (with less than a piece a block, some have none)
               if (all * c / g1 < all * (c + 1) / g1) top = max_nan(top, launch.top[(int64_t)c * (p.tokens * p.topk) + r]);
@@ -848,9 +879,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
           const int before = a == a0 ? 0 : (table.first_row[a0 + 1] - row0) * (steps - s0) + (row - table.first_row[a0 + 1]) * steps;
           const uint32_t base = smem_at(panel) + (before - (a == a0 ? s0 : 0) * n_rows) * (S::kK * 2);
           const uint32_t mine = table.tokens[a];
-          int low[kTiles / 2];
-#pragma unroll
-          for (int j = 0; j < kTiles / 2; ++j) low[j] = F == kFewFp8 ? 0 : (int)((uintptr_t)scale_row(a, j) & 3);
           FewTokens x[NT];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -859,7 +887,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
             x[n].block = used ? n_rows * 64 : 0;
           }
           float acc[kTiles][NT][4] = {};
-          for (; pos < end; ++pos) take_step<F, NT>(acc, ring, slot, low, tiles, layout, x, pos - a * steps, pos - a * steps, copy_next);
+#pragma unroll 1
+          for (; pos < end; ++pos) take_step<F, NT, false>(acc, ring, slot, tiles, layout, x, pos - a * steps, pos - a * steps, copy_next);
           // (columns of tokens without this expert are left out: a weight that is not finite would get into them)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
@@ -880,23 +909,16 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       s0 = s1;
       __syncthreads();   // the panel is free again
     }
-    constexpr int kWarpFloats = RedShape<NT>::kWarpFloats;
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) red[warp * kWarpFloats + ((i * NT + n) * 4 + c) * 32 + lane] = out[i][n][c];
+    store_sums<NT>(red, out);
     copies_wait<0>();
     __syncthreads();
     for (int j = tid; j < kRows * p.tokens; j += kThreads) {
       // consecutive threads, consecutive features of a token
       const int row = j % kRows, token = j / kRows;
       if (row >= rows_here) continue;
-      const int at = (((row >> 4) * NT + (token >> 3)) * 4 + ((row >> 3) & 1) * 2 + (token & 1)) * 32 + (row & 7) * 4 + ((token & 7) >> 1);
       float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += red[w * kWarpFloats + at];
+      for (int w = 0; w < kWarps; ++w) v += red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(row >> 4, row & 15, token)];
       const int64_t to = (int64_t)token * p.hidden + r0 + row;
       if (launch.splits == 1) finish(v, token, r0 + row);
       else launch.part[(int64_t)split * p.tokens * p.hidden + to] = v;

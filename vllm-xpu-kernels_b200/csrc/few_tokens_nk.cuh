@@ -54,6 +54,7 @@ struct FewTable {
   int slot_expert[kMaxSlots];      // the slot's expert, as an index of the active ones (-1: none)
   uint16_t row_expert[kMaxSlots];
   float weight[kMaxSlots];         // of a row: the sum over the slots that name its expert
+  float slot_weight[kMaxSlots];
 };
 
 __device__ __forceinline__ int rank_below(uint32_t mask, int bit) { return __popc(mask & ((1u << bit) - 1u)); }
@@ -69,6 +70,7 @@ __device__ __forceinline__ void build_table(FewTable& t, const FewParams& p) {
   for (int i = lane; i < slots; i += 32) {
     const int e = local_expert(p, i);
     t.slot_expert[i] = e;
+    if (kWeights) t.slot_weight[i] = p.weights[i];
     if (e >= 0) atomicOr(&t.bits[e >> 5], 1u << (e & 31));
   }
   __syncwarp();
@@ -116,13 +118,13 @@ __device__ __forceinline__ void build_table(FewTable& t, const FewParams& p) {
     for (int i = lane; i < slots; i += 32) {
       const int a = t.slot_expert[i], tok = i / p.topk;
       if (a < 0) continue;
-      float w = p.weights[i];
+      float w = t.slot_weight[i];
       if (again) {    // the token's slots with this expert in their order, by the first of them
         bool other = false;
         for (int j = tok * p.topk; j < i; ++j) other |= t.slot_expert[j] == a;
         if (other) continue;
         for (int j = i + 1; j < (tok + 1) * p.topk; ++j)
-          if (t.slot_expert[j] == a) w += p.weights[j];
+          if (t.slot_expert[j] == a) w += t.slot_weight[j];
       }
       const int row = t.first_row[a] + rank_below(t.tokens[a], tok);
       t.weight[row] = w;
@@ -213,27 +215,6 @@ __device__ __forceinline__ uint32_t panel_at(int k8, int row, int rows) {   // k
   return (uint32_t)(((block * rows + row) * 4 + t) * 16);
 }
 
-enum FewSource { kFromBf16, kFromF16, kFromF32 };
-__device__ __forceinline__ void load8(float (&v)[8], const void* row, int source, int k8) {
-  if (source == kFromF32) {
-    const float4 a = reinterpret_cast<const float4*>(row)[2 * k8], b = reinterpret_cast<const float4*>(row)[2 * k8 + 1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    return;
-  }
-  const vec16 w = reinterpret_cast<const vec16*>(row)[k8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (source == kFromBf16) {
-      v[2 * i] = __uint_as_float(w.w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w.w[i] & 0xffff0000u);
-    } else {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w.w[i]));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  }
-}
-
 // The power of two by which a row is multiplied on its way to float16, its largest magnitude then between 2^14 and 2^15, and
 // its inverse.  Magnitudes below 2^-100 are taken for that; a row that is not finite stays as it is.
 __device__ __forceinline__ float row_scale(float top, float& inverse) {
@@ -244,44 +225,64 @@ __device__ __forceinline__ float row_scale(float top, float& inverse) {
   return __uint_as_float((uint32_t)(254 - (e - 14)) << 23);
 }
 
-// One row's part of a panel: values [k8_0, k8_1) * 8 of a source row of `k` values (zeros beyond it), by `parts` warps of
-// which this is `part`.
+// Eight values as a lane wants them: int4 pairs are four apart.
 template <int F>
-__device__ __forceinline__ void convert_row(uint8_t* panel, int row, int rows, const void* src, int source, int k, int k8_0, int k8_1,
-                                            float scale, int part, int parts) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll 4
-  for (int j = k8_0 + part * 32 + lane; j < k8_1; j += parts * 32) {
-    float v[8] = {};
-    if (8 * j < k) load8(v, src, source, j);
-    uint32_t o[4];
+__device__ __forceinline__ uint4 scaled8(const float (&v)[8], float scale) {
+  constexpr bool kApart = F == kFewInt4 || F == kFewInt4Fine;
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = kApart ? __floats2half2_rn(v[i] * scale, v[i + 4] * scale) : __floats2half2_rn(v[2 * i] * scale, v[2 * i + 1] * scale);
+    o[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Tokens of the set `now` into a panel, in two passes with a barrier between them: the rows as they are and their largest
+// magnitudes (as bits, which order like the magnitudes, NaN last), then each row times its scale as float16.  A warp takes 256
+// values of a row at a time, four such pieces together (the loads' latency is what a pass costs).
+template <int F>
+__device__ __forceinline__ void panel_raw(uint8_t* panel, uint32_t* tops, const FewParams& p, uint32_t now, int k8, int member, int members) {
+  const int lane = threadIdx.x & 31, pieces = (k8 + 31) / 32, rows = __popc(now), items = rows * pieces;
+#pragma unroll 1
+  for (int first = member; first < items; first += 4 * members) {
+    vec16 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      // int4 pairs are four apart
-      const float x = F == kFewInt4 || F == kFewInt4Fine ? v[i] : v[2 * i], y = F == kFewInt4 || F == kFewInt4Fine ? v[i + 4] : v[2 * i + 1];
-      const __half2 h = __floats2half2_rn(x * scale, y * scale);
-      o[i] = *reinterpret_cast<const uint32_t*>(&h);
+      const int item = first + i * members, row = item / pieces, j = (item - row * pieces) * 32 + lane;
+      uint32_t left = now;
+      for (int r = 0; r < row; ++r) left &= left - 1;
+      v[i] = vec16{{0, 0, 0, 0}};
+      if (item < items && 8 * j < p.hidden) v[i] = ld16(reinterpret_cast<const uint16_t*>(p.x) + (int64_t)(__ffs(left) - 1) * p.hidden + 8 * j);
     }
-    *reinterpret_cast<uint4*>(panel + panel_at<F>(j - k8_0, row, rows)) = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int item = first + i * members, row = item / pieces, j = (item - row * pieces) * 32 + lane;
+      if (item >= items) break;
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = __vmaxu2(top, v[i].w[k] & 0x7fff7fffu);
+      top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+      if (lane == 0) atomicMax(&tops[row], top);
+      if (j < k8) *reinterpret_cast<vec16*>(panel + panel_at<F>(j, row, rows)) = v[i];
+    }
   }
 }
-__device__ __forceinline__ float row_top(const void* src, int source, int k, int k8_0, int k8_1, int part, int parts) {
-  const int lane = threadIdx.x & 31;
-  float top = 0.f;
-#pragma unroll 4
-  for (int j = k8_0 + part * 32 + lane; j < k8_1; j += parts * 32) {
-    if (8 * j >= k) break;
-    float v[8];
-    load8(v, src, source, j);
+template <int F>
+__device__ __forceinline__ void panel_scaled(uint8_t* panel, const uint32_t* tops, float* inverse, int rows, int k8, bool f16) {
+  auto value = [&](uint32_t h) { return f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16); };
+  for (int i = threadIdx.x; i < rows * k8; i += kThreads) {
+    const int row = i / k8, j = i - row * k8;
+    vec16* const at = reinterpret_cast<vec16*>(panel + panel_at<F>(j, row, rows));
+    const vec16 raw = *at;
+    float v[8], inv;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[i]));
+    for (int k = 0; k < 4; ++k) { v[2 * k] = value(raw.w[k] & 0xffffu); v[2 * k + 1] = value(raw.w[k] >> 16); }
+    const float scale = row_scale(value(tops[row]), inv);
+    if (j == 0) inverse[row] = inv;
+    *reinterpret_cast<uint4*>(at) = scaled8<F>(v, scale);
   }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
-  return top;
 }
-// Warps of a row where `warps` of them fill a panel of `rows`.
-__device__ __forceinline__ int warps_per_row(int rows, int warps) { return rows >= warps ? 1 : warps / rows; }
 
 // ---- weights: a warp's ring ------------------------------------------------------------
 // fp8: a lane reads the bytes that it fetched.  4 bits: a lane fetches 16 bytes of a row, which is a group of 32 values, and
@@ -504,7 +505,7 @@ template <int F, int NT> struct UpShape {
   static constexpr int kFixed = kTableBytes + 512 + kMaxSlots * 4 + RedShape<NT>::kBytes + kWarps * FewShape<F>::kRing;
 };
 template <int F> struct DownShape {
-  static constexpr int kFixed = kTableBytes + 128 + kMaxSlots * 4 + kWarps * FewShape<F>::kRing;
+  static constexpr int kFixed = kTableBytes + 128 + 2 * kMaxSlots * 4 + kWarps * FewShape<F>::kRing;
 };
 
 // h[row] = act(W13 x + b13).  The features of all active experts, in pieces of eight (a tile's rows: eight gates and their
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
   extern __shared__ __align__(128) uint8_t smem[];
   FewTable& table = *reinterpret_cast<FewTable*>(smem);
   float* const inverse = reinterpret_cast<float*>(smem + kTableBytes);   // of the panel's rows' scales
-  float* const tops = inverse + 32;                                       // (per warp)
+  uint32_t* const tops = reinterpret_cast<uint32_t*>(inverse + 32);       // of the panel's rows: largest magnitude
   uint8_t* const zeros = smem + kTableBytes + 256;                        // a token's values where there is no token
   uint32_t* const h_top = reinterpret_cast<uint32_t*>(smem + kTableBytes + 512);   // largest |h| per row (bits: NaN counts as largest)
   float* const red = reinterpret_cast<float*>(smem + kTableBytes + 512 + kMaxSlots * 4);
@@ -530,42 +531,19 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
   const int steps = (p.hidden + S::kK - 1) / S::kK, per_expert = p.inter / 8;
   const int most = launch.panel_bytes / (steps * S::kK * 2);      // rows that the panel holds
   const bool whole = most >= p.tokens;                            // all tokens
-  if (tid < 16) reinterpret_cast<uint32_t*>(zeros)[tid] = 0;
-  // The panel's row `row`: token `token`, by `parts` warps that have barrier `id` to themselves.
-  auto fill_row = [&](int row, int rows, int token, bool there, int warps, int id) {
-    const int parts = warps_per_row(rows, warps), part = (warp + warps - kWarps) % parts, k8 = steps * (S::kK / 8);
-    const int source = launch.f16 ? kFromF16 : kFromBf16;
-    const uint8_t* x = reinterpret_cast<const uint8_t*>(p.x) + (int64_t)token * p.hidden * 2;
-    float top = there ? row_top(x, source, p.hidden, 0, k8, part, parts) : 0.f;
-    if (parts > 1) {
-      if (lane == 0) tops[warp] = top;
-      group_sync(id, warps * 32);
-      for (int i = 0; i < parts; ++i) top = max_nan(top, tops[warp - part + i]);
-    }
-    if (there) {
-      float inv;
-      const float scale = row_scale(top, inv);
-      if (lane == 0 && part == 0) inverse[row] = inv;
-      convert_row<F>(panel, row, rows, x, source, p.hidden, 0, k8, scale, part, parts);
-    }
-  };
-  // Rows in turn; where there are fewer than warps, all at once with several warps each.
-  auto fill_panel = [&](uint32_t now, int warps, int id) {
-    const int rows = __popc(now), parts = warps_per_row(rows, warps), first = (warp + warps - kWarps) / parts, step = warps / parts;
-#pragma unroll 1
-    for (int row = first, turn = 0; turn < rows; row += step, turn += step) {
-      uint32_t left = now;
-      for (int i = 0; i < row && left; ++i) left &= left - 1;
-      fill_row(row, rows, left ? __ffs(left) - 1 : 0, row < rows, warps, id);
-    }
-  };
+  const int k8 = steps * (S::kK / 8);
+  if (tid < 16) {
+    reinterpret_cast<uint32_t*>(zeros)[tid] = 0;
+    tops[tid] = 0;
+  }
+  __syncthreads();
   if (warp == 0) {
     build_table<false>(table, p);
   } else {
     for (int i = tid - 32; i < p.tokens * p.topk; i += kThreads - 32) h_top[i] = 0;
     if (blockIdx.x == 0)   // (the second kernel counts from there)
       for (int i = tid - 32; i < kFewMaxColumns; i += kThreads - 32) launch.arrived[i] = 0;
-    if (whole) fill_panel((1u << p.tokens) - 1u, kWarps - 1, 1);
+    if (whole) panel_raw<F>(panel, tops, p, (1u << p.tokens) - 1u, k8, warp - 1, kWarps - 1);
   }
   __syncthreads();
   const uint32_t all = (uint32_t)(table.active * per_expert);     // (times the blocks below 2^32: takes_nk)
@@ -653,11 +631,14 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       settle();
 #pragma unroll 1
       for (int i = 0; i < S::kDepth; ++i) copy_next(i);
+      const int rows = __popc(now);
       if (!whole) {
-        fill_panel(now, kWarps, 0);
+        panel_raw<F>(panel, tops, p, now, k8, warp, kWarps);
         __syncthreads();
       }
-      const int rows = whole ? p.tokens : __popc(now);
+      panel_scaled<F>(panel, tops, inverse, rows, k8, launch.f16);
+      __syncthreads();
+      if (!whole && tid < 16) tops[tid] = 0;
 
       int slot = 0, cs = member;
 #pragma unroll 1
@@ -736,8 +717,9 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   int& last_one = *reinterpret_cast<int*>(smem + kTableBytes);
   uint8_t* const zeros = smem + kTableBytes + 64;
   float* const coef = reinterpret_cast<float*>(smem + kTableBytes + 128);   // of the panel's rows: routing weight and the inverse of the scale
+  float* const scales = coef + kMaxSlots;                                     // ... and the scale
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_at(smem) + kTableBytes + 128 + kMaxSlots * 4 + warp * S::kRing;
+  const uint32_t ring = smem_at(smem) + kTableBytes + 128 + 2 * kMaxSlots * 4 + warp * S::kRing;
   uint8_t* const panel = smem + DownShape<F>::kFixed;
   float* const red = reinterpret_cast<float*>(panel);                     // (after the last panel)
   // What routed the tokens was complete before the kernel ahead of this one let it start.
@@ -758,6 +740,13 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   // How far a panel reaches that begins with step s0 of expert a0: whole experts, then as many steps of the next one as
   // there is room for (at least one).
   auto panel_end = [&](int a0, int s0, int& a1, int& s1) {
+    const int ae = step_end / steps, se = step_end - ae * steps;      // all that is left, if it fits
+    const int need = ae == a0 ? (table.first_row[a0 + 1] - table.first_row[a0]) * (se - s0)
+                              : (table.first_row[a0 + 1] - table.first_row[a0]) * (steps - s0) + (table.first_row[ae] - table.first_row[a0 + 1]) * steps +
+                                    (se > 0 ? (table.first_row[ae + 1] - table.first_row[ae]) * se : 0);
+    a1 = ae;
+    s1 = se;
+    if (need <= room) return;
     int free = room;
     a1 = a0;
     s1 = s0;
@@ -775,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
     if (m.bias) {
       for (int k = 0; k < p.topk; ++k) {
         const int a = table.slot_expert[token * p.topk + k];
-        if (a >= 0) v = fmaf(p.weights[token * p.topk + k], load16(m.bias, (int64_t)table.expert[a] * m.n + n, launch.f16), v);
+        if (a >= 0) v = fmaf(table.slot_weight[token * p.topk + k], load16(m.bias, (int64_t)table.expert[a] * m.n + n, launch.f16), v);
       }
     }
     const int64_t to = (int64_t)token * p.hidden + n;
@@ -840,32 +829,61 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       panel_end(a0, s0, a1, s1);
       const int last = s1 > 0 ? a1 : a1 - 1;           // the last expert with steps in the panel
       const int row0 = table.first_row[a0], rows = table.first_row[last + 1] - row0;
-      {
-        const int parts = warps_per_row(rows, kWarps), row = warp / parts, part = warp % parts;   // (several warps have a row where there are fewer rows)
-#pragma unroll 1
-        for (int q0 = 0; q0 < rows; q0 += kWarps / parts) {
-          const int r = row0 + q0 + row;
-          const bool there = q0 + row < rows;
-          const int a = there ? table.row_expert[r] : a0;
-          const int k8_0 = (a == a0 ? s0 : 0) * (S::kK / 8), k8_1 = (a == a1 ? s1 : steps) * (S::kK / 8);
-          if (there && row < kWarps / parts) {
-            // the largest |h| of the row, over the blocks of the first kernel that had features of its expert
-            const uint32_t all = (uint32_t)(table.active * per_expert), g1 = launch.up_blocks;
-            const int c0 = (int)((((uint32_t)(a * per_expert) + 1) * g1 - 1) / all), c1 = (int)(((uint32_t)((a + 1) * per_expert) * g1 - 1) / all);
-            float top = 0.f;
-            for (int c = c0 + lane; c <= c1; c += 32)   // (with less than a piece a block, some have none)
-              if (all * c / g1 < all * (c + 1) / g1) top = max_nan(top, launch.top[(int64_t)c * (p.tokens * p.topk) + r]);
+      // Rows' scales, eight lanes a row, from the largest |h| that the blocks of the first kernel with features of its expert
+      // have found; then their values, 256 of a row at a time by a warp, two such pieces together.
+      for (int i = tid / 8; i < (rows + kThreads / 8 - 1) / (kThreads / 8) * (kThreads / 8); i += kThreads / 8) {
+        const int r = row0 + min(i, rows - 1), a = table.row_expert[r];
+        const uint32_t all = (uint32_t)(table.active * per_expert), g1 = launch.up_blocks;
+        const int c0 = (int)((((uint32_t)(a * per_expert) + 1) * g1 - 1) / all), c1 = (int)(((uint32_t)((a + 1) * per_expert) * g1 - 1) / all);
+        float top = 0.f;
+        for (int c = c0 + (tid & 7); c <= c1; c += 8)   // (with less than a piece a block, some have none)
+          if (all * c / g1 < all * (c + 1) / g1) top = max_nan(top, launch.top[c * (p.tokens * p.topk) + r]);
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float* h = p.h + (int64_t)r * p.inter;
-            float inv;
-            const float scale = row_scale(top, inv);
-            if (lane == 0 && part == 0) coef[q0 + row] = table.weight[r] * inv;
-            // rows of earlier experts in the panel: the first one's with the steps that it has there
-            const int before = a == a0 ? 0 : (table.first_row[a0 + 1] - row0) * (steps - s0) + (table.first_row[a] - table.first_row[a0 + 1]) * steps;
-            convert_row<F>(panel + (int64_t)before * (S::kK * 2), r - table.first_row[a], table.first_row[a + 1] - table.first_row[a], h,
-                           kFromF32, p.inter, k8_0, k8_1, scale, part, parts);
-          }
+        for (int d = 4; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+        float inv;
+        const float scale = row_scale(top, inv);
+        if ((tid & 7) == 0 && i < rows) {
+          coef[i] = table.weight[r] * inv;
+          scales[i] = scale;
+        }
+      }
+      __syncthreads();
+      {
+        // the first expert's rows have the steps from s0 on, the last one's those up to s1
+        constexpr int kPiece = S::kK / 8;
+        const int n0 = table.first_row[a0 + 1] - row0, n2 = last > a0 ? rows - (table.first_row[last] - row0) : 0, n1 = rows - n0 - n2;
+        const int len0 = ((a0 == last && s1 > 0 ? s1 : steps) - s0) * kPiece, len1 = steps * kPiece, len2 = (s1 > 0 ? s1 : steps) * kPiece;
+        const int p0 = (len0 + 31) / 32, p1 = (len1 + 31) / 32, p2 = (len2 + 31) / 32, items = n0 * p0 + n1 * p1 + n2 * p2;
+        // an item's row (of the panel), its piece, where the piece's values come from and go to
+        struct Item { int row, j; const float* from; uint8_t* to; };
+        auto item_of = [&](int item) {
+          Item it = {0, 0, nullptr, nullptr};
+          if (item >= items) return it;
+          int len, k8_0 = 0;
+          if (item < n0 * p0) { it.row = item / p0; it.j = item - it.row * p0; len = len0; k8_0 = s0 * kPiece; }
+          else if (item < n0 * p0 + n1 * p1) { item -= n0 * p0; it.row = item / p1; it.j = item - it.row * p1; it.row += n0; len = len1; }
+          else { item -= n0 * p0 + n1 * p1; it.row = item / p2; it.j = item - it.row * p2; it.row += n0 + n1; len = len2; }
+          it.j = it.j * 32 + lane;
+          if (it.j >= len) return it;
+          const int r = row0 + it.row, a = table.row_expert[r], e0 = table.first_row[a], n = table.first_row[a + 1] - e0;
+          const int before = a == a0 ? 0 : n0 * (steps - s0) + (e0 - row0 - n0) * steps;   // rows times steps of earlier experts in the panel
+          it.to = panel + (int64_t)before * (S::kK * 2) + panel_at<F>(it.j, r - e0, n);
+          if (8 * (k8_0 + it.j) < p.inter) it.from = p.h + (int64_t)r * p.inter + 8 * (k8_0 + it.j);
+          return it;
+        };
+#pragma unroll 1
+        for (int first = warp; first < items; first += 2 * kWarps) {
+          const Item i0 = item_of(first), i1 = item_of(first + kWarps);
+          float4 v[4] = {};
+          if (i0.from) { v[0] = reinterpret_cast<const float4*>(i0.from)[0]; v[1] = reinterpret_cast<const float4*>(i0.from)[1]; }
+          if (i1.from) { v[2] = reinterpret_cast<const float4*>(i1.from)[0]; v[3] = reinterpret_cast<const float4*>(i1.from)[1]; }
+          auto put = [&](const Item& it, const float4& a, const float4& b) {
+            if (it.to == nullptr) return;
+            const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            *reinterpret_cast<uint4*>(it.to) = scaled8<F>(x, scales[it.row]);
+          };
+          put(i0, v[0], v[1]);
+          put(i1, v[2], v[3]);
         }
         __syncthreads();
       }

@@ -120,11 +120,10 @@ int launch_block_per_sm(const char* name, int grid, int smem, cudaStream_t st, c
 
 // Where things are in the workspace: h, then what the blocks of the two kernels tell one another.
 struct FewWorkspace {
-  size_t top, arrived, part, bytes;
+  size_t arrived, part, bytes;
   FewWorkspace(int64_t tokens, int64_t topk, int64_t hidden, int64_t inter) {
     auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    top = up(tokens * topk * inter * sizeof(float));
-    arrived = top + up((size_t)kFewMaxBlocks * tokens * topk * sizeof(float));
+    arrived = up(tokens * topk * inter * sizeof(float));
     part = arrived + kFewMaxColumns * sizeof(uint32_t);
     bytes = part + up((size_t)splits(hidden, kFewMaxBlocks) * tokens * hidden * sizeof(float));
   }
@@ -138,14 +137,14 @@ struct FewWorkspace {
 template <int F, int NT>
 int launch_nk(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   constexpr int k = FewShape<F>::kK, up_room = kMaxSmem - UpShape<F, NT>::kFixed, down_room = kMaxSmem - DownShape<F>::kFixed;
-  const int up_row = (p.hidden + k - 1) / k * k * 2, down_row = (p.inter + k - 1) / k * k * 2;
+  constexpr int step = FewShape<F>::kPanelBytes;
+  const int up_row = (p.hidden + k - 1) / k * step, down_row = (p.inter + k - 1) / k * step;
   l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
-  l.up_blocks = ctas;
   l.splits = FewWorkspace::splits(p.hidden, ctas);
   int rc = launch_block_per_sm<few_up_kernel<F, NT>>("few_up_kernel", ctas, UpShape<F, NT>::kFixed + l.panel_bytes, st, p, l);
   if (rc != B200MOE_OK) return rc;
   const int64_t want = (int64_t)p.tokens * p.topk * down_row;
-  l.panel_bytes = (int)(want < down_room ? want : down_room / 256 * 256);
+  l.panel_bytes = (int)(want < down_room ? want : down_room);
   if (l.panel_bytes < RedShape<NT>::kBytes) l.panel_bytes = RedShape<NT>::kBytes;
   return launch_block_per_sm<few_down_kernel<F, NT>>("few_down_kernel", ctas / l.splits * l.splits, DownShape<F>::kFixed + l.panel_bytes, st, p, l);
 }
@@ -233,7 +232,6 @@ extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200mo
     FewLaunch l = {};
     l.f16 = a->dtype == B200MOE_F16;
     const FewWorkspace ws(p.tokens, p.topk, p.hidden, p.inter);
-    l.top = (float*)((char*)a->workspace + ws.top);
     l.arrived = (uint32_t*)((char*)a->workspace + ws.arrived);
     l.part = (float*)((char*)a->workspace + ws.part);
     if (p.w13.format == B200MOE_W_FP8_BLOCK_NK) return launch_nk<kFewFp8>(p, l, ctas, as_stream(stream));

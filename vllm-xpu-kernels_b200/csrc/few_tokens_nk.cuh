@@ -7,8 +7,8 @@
 // through a warp's own ring in shared memory (cp.async) into the registers that the matrix instruction reads, with one
 // conversion to float16 on the way, which holds every code of the three formats exactly.  The sum over k does not mind its order,
 // so a lane's 16 bytes of a row go into the instruction as they come and the tokens are laid out to match.  Scales of weights
-// multiply sums of their group in fp32.  Tokens and activations are float16 with a power of two per row, which keeps a
-// bfloat16 as it is and rounds h to 11 bits.
+// multiply sums of their group in fp32.  Tokens and activations are float16 with a power of two per 64 or 128 values of a row,
+// which keeps a bfloat16 as it is and rounds h to 11 bits.
 //
 // tcgen05 would have to get its weights converted in shared or tensor memory, a second pass for every byte, and its tile
 // of 128 features leaves most SMs without work at one token.
@@ -34,6 +34,7 @@ enum FewFormat { kFewFp8, kFewFp4, kFewInt4Fine, kFewInt4 };   // Fine: groups o
 template <int F> struct FewShape {
   static constexpr int kK = F == kFewFp8 ? 64 : 128;             // values of a row
   static constexpr int kBlocks = kK / 32;                        // of the panel: a lane's eight values, two instructions
+  static constexpr int kPanelBytes = kK * 2 + 4;                 // of the panel: a row's values of a step and their scale
   static constexpr int kScaleWords = F == kFewInt4Fine ? 2 : 1;  // that hold a row's scales of a step
   static constexpr int kScales = F == kFewFp8 ? 0 : F == kFewInt4 ? 1 : 4;                       // of a row and step, made fp32 (fp8: are so)
   static constexpr int kSlot = kRows * (64 + 4 * kScaleWords);
@@ -207,7 +208,7 @@ __device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a
 // ---- tokens and activations as float16 -------------------------------------------------
 // A panel holds rows of values in the order in which the lanes want them: per step blocks of [row][4 lanes][8 values].
 // Where k sits: fp8 lanes hold 16 bytes of a row, 16 values; 4-bit formats hand a group of 32 values out to the four lanes,
-// eight each.
+// eight each.  Behind them, per row and step, the inverse of what the values have been multiplied by.
 template <int F>
 __device__ __forceinline__ uint32_t panel_at(int k8, int row, int rows) {   // k8: k / 8
   const int block = F == kFewFp8 ? (k8 >> 3) * 2 + (k8 & 1) : k8 >> 2;
@@ -215,10 +216,10 @@ __device__ __forceinline__ uint32_t panel_at(int k8, int row, int rows) {   // k
   return (uint32_t)(((block * rows + row) * 4 + t) * 16);
 }
 
-// The power of two by which a row is multiplied on its way to float16, its largest magnitude then between 2^14 and 2^15, and
-// its inverse.  Magnitudes below 2^-100 are taken for that; a row that is not finite stays as it is.
-__device__ __forceinline__ float row_scale(float top, float& inverse) {
-  int e = (int)(__float_as_uint(top) >> 23);   // (no sign)
+// The power of two by which values are multiplied on their way to float16, their largest magnitude then between 2^14 and 2^15,
+// and its inverse.  Magnitudes below 2^-100 are taken for that; what is not finite stays as it is.
+__device__ __forceinline__ float step_scale(uint32_t top, float& inverse) {   // top: bits of the largest magnitude
+  int e = (int)(top >> 23);
   if (e == 255) e = 127 + 14;
   e = max(e, 127 - 100);
   inverse = __uint_as_float((uint32_t)(e - 14) << 23);
@@ -238,49 +239,72 @@ __device__ __forceinline__ uint4 scaled8(const float (&v)[8], float scale) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// Tokens of the set `now` into a panel, in two passes with a barrier between them: the rows as they are and their largest
-// magnitudes (as bits, which order like the magnitudes, NaN last), then each row times its scale as float16.  A warp takes 256
-// values of a row at a time, four such pieces together (the loads' latency is what a pass costs).
-template <int F>
-__device__ __forceinline__ void panel_raw(uint8_t* panel, uint32_t* tops, const FewParams& p, uint32_t now, int k8, int member, int members) {
-  const int lane = threadIdx.x & 31, pieces = (k8 + 31) / 32, rows = __popc(now), items = rows * pieces;
+enum FewSource { kFromBf16, kFromF16, kFromF32 };
+// `len` eighths of a row (what is beyond `values` values is zero) into a panel, by `parts` warps of which this is `part`.  A warp
+// asks for four times 256 values at once: the loads' latency is what this costs.
+template <int F, int Source>
+__device__ __forceinline__ void fill_row(uint8_t* panel, float* scales, const void* from, int values, int len, int row, int rows, int part, int parts) {
+  constexpr int kLanes = FewShape<F>::kK / 8;      // of a step
+  constexpr int kWords = Source == kFromF32 ? 2 : 1;
+  const int lane = threadIdx.x & 31, stride = 32 * parts;
 #pragma unroll 1
-  for (int first = member; first < items; first += 4 * members) {
-    vec16 v[4];
+  for (int j0 = part * 32 + lane; j0 - lane < len; j0 += 4 * stride) {
+    vec16 raw[4][kWords];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int item = first + i * members, row = item / pieces, j = (item - row * pieces) * 32 + lane;
-      uint32_t left = now;
-      for (int r = 0; r < row; ++r) left &= left - 1;
-      v[i] = vec16{{0, 0, 0, 0}};
-      if (item < items && 8 * j < p.hidden) v[i] = ld16(reinterpret_cast<const uint16_t*>(p.x) + (int64_t)(__ffs(left) - 1) * p.hidden + 8 * j);
+      const int j = j0 + i * stride;
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) {
+        raw[i][k] = vec16{{0, 0, 0, 0}};
+        if (j < len && 8 * j < values) raw[i][k] = reinterpret_cast<const vec16*>(from)[j * kWords + k];
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int item = first + i * members, row = item / pieces, j = (item - row * pieces) * 32 + lane;
-      if (item >= items) break;
-      uint32_t top = 0;
+      const int j = j0 + i * stride;
+      float v[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) top = __vmaxu2(top, v[i].w[k] & 0x7fff7fffu);
-      top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-      if (lane == 0) atomicMax(&tops[row], top);
-      if (j < k8) *reinterpret_cast<vec16*>(panel + panel_at<F>(j, row, rows)) = v[i];
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (Source == kFromF32) {
+          v[k] = __uint_as_float(raw[i][0].w[k]);
+          v[4 + k] = __uint_as_float(raw[i][kWords - 1].w[k]);
+        } else if constexpr (Source == kFromBf16) {
+          v[2 * k] = __uint_as_float(raw[i][0].w[k] << 16);
+          v[2 * k + 1] = __uint_as_float(raw[i][0].w[k] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&raw[i][0].w[k]));
+          v[2 * k] = f.x;
+          v[2 * k + 1] = f.y;
+        }
+      }
+      uint32_t top = 0;        // (as bits: magnitudes in their order, NaN last)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+#pragma unroll
+      for (int d = 1; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+      float inv;
+      const float scale = step_scale(top, inv);
+      if (j < len) {
+        *reinterpret_cast<uint4*>(panel + panel_at<F>(j, row, rows)) = scaled8<F>(v, scale);
+        if ((j & (kLanes - 1)) == 0) scales[j / kLanes * rows + row] = inv;
+      }
     }
   }
 }
+// Warps of a row where `warps` of them fill a panel of `rows`.
+__device__ __forceinline__ int warps_per_row(int rows, int warps) { return rows >= warps ? 1 : warps / rows; }
+
+// Tokens of the set `now` into a panel.
 template <int F>
-__device__ __forceinline__ void panel_scaled(uint8_t* panel, const uint32_t* tops, float* inverse, int rows, int k8, bool f16) {
-  auto value = [&](uint32_t h) { return f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16); };
-  for (int i = threadIdx.x; i < rows * k8; i += kThreads) {
-    const int row = i / k8, j = i - row * k8;
-    vec16* const at = reinterpret_cast<vec16*>(panel + panel_at<F>(j, row, rows));
-    const vec16 raw = *at;
-    float v[8], inv;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) { v[2 * k] = value(raw.w[k] & 0xffffu); v[2 * k + 1] = value(raw.w[k] >> 16); }
-    const float scale = row_scale(value(tops[row]), inv);
-    if (j == 0) inverse[row] = inv;
-    *reinterpret_cast<uint4*>(at) = scaled8<F>(v, scale);
+__device__ __forceinline__ void fill_tokens(uint8_t* panel, float* scales, const FewParams& p, uint32_t now, int len, bool f16, int member, int members) {
+  const int rows = __popc(now), parts = warps_per_row(rows, members);
+#pragma unroll 1
+  for (int row = member / parts; row < rows; row += members / parts) {
+    uint32_t left = now;
+    for (int r = 0; r < row; ++r) left &= left - 1;
+    const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x) + (int64_t)(__ffs(left) - 1) * p.hidden;
+    if (f16) fill_row<F, kFromF16>(panel, scales, x, p.hidden, len, row, rows, member % parts, parts);
+    else fill_row<F, kFromBf16>(panel, scales, x, p.hidden, len, row, rows, member % parts, parts);
   }
 }
 
@@ -377,7 +401,22 @@ __device__ __forceinline__ void spread_scales(uint32_t to, uint32_t slot, const 
 // Without a token: zeros, and no way.
 struct FewTokens {
   uint32_t at, block;
+  uint32_t scale[2], step;   // the scales of the lane's columns of sums, and the way to the next step's
 };
+template <int NT>
+__device__ __forceinline__ void find_tokens(FewTokens (&x)[NT], uint32_t used, uint32_t in_panel, uint32_t panel, uint32_t scales, uint32_t zeros, int rows) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const bool there = (used >> (8 * n + g)) & 1;
+    x[n].at = there ? panel + rank_below(in_panel, 8 * n + g) * 64 + t * 16 : zeros;
+    x[n].block = there ? rows * 64 : 0;
+    // (columns without a token: any scale, nobody reads them)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) x[n].scale[c] = scales + min(rank_below(in_panel, 8 * n + 2 * t + c), rows - 1) * 4;
+    x[n].step = rows * 4;
+  }
+}
 
 // acc += W x of the step in the slot, for the first `Tiles` tiles (what one of them has not got is something finite or not, in
 // rows that nobody reads).  kHalves: scales lie as [8 rows g of all tiles][8 rows g + 8 of all tiles], else row by row.
@@ -387,21 +426,25 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
   using S = FewShape<F>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint4 v[S::kBlocks][NT];
+  float sx[NT][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) sx[n][c] = ldsf(x[n].scale[c] + s * x[n].step);
 #pragma unroll
     for (int q = 0; q < S::kBlocks; ++q) v[q][n] = lds16(x[n].at + (s * S::kBlocks + q) * x[n].block);
+  }
 #pragma unroll
   for (int i = 0; i < Tiles; ++i) {
     const int at_lo = kHalves ? 8 * i + g : 16 * i + g, at_hi = at_lo + (kHalves ? kRows / 2 : 8);   // places of the scales
-    float d[NT][4];
+    float d[NT][4], sum[NT][4] = {};   // products of a group of weights, and the step's
     auto add = [&](float a, float b) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        acc[i][n][0] = fmaf(a, d[n][0], acc[i][n][0]);
-        acc[i][n][1] = fmaf(a, d[n][1], acc[i][n][1]);
-        acc[i][n][2] = fmaf(b, d[n][2], acc[i][n][2]);
-        acc[i][n][3] = fmaf(b, d[n][3], acc[i][n][3]);
+        sum[n][0] = fmaf(a, d[n][0], sum[n][0]);
+        sum[n][1] = fmaf(a, d[n][1], sum[n][1]);
+        sum[n][2] = fmaf(b, d[n][2], sum[n][2]);
+        sum[n][3] = fmaf(b, d[n][3], sum[n][3]);
       }
     };
     if constexpr (F == kFewFp8) {
@@ -447,6 +490,10 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
                                              __uint_as_float(q == 0 ? hi.x : q == 1 ? hi.y : q == 2 ? hi.z : hi.w));
       }
     }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf(sx[n][c & 1], sum[n][c], acc[i][n][c]);
   }
 }
 
@@ -473,9 +520,7 @@ __device__ __forceinline__ float load16(const void* p, int64_t i, bool f16) {
 struct FewLaunch {
   int panel_bytes;       // of shared memory for the panel
   bool f16;
-  int up_blocks;         // of the first kernel
   int splits;            // of the second kernel's steps: it has hidden / splits columns of blocks
-  float* top;            // [up_blocks][tokens * topk]: largest |h| that a block of the first kernel has found, per row of h
   uint32_t* arrived;     // per column of blocks of the second kernel
   float* part;           // [splits][tokens][hidden]: partial sums, with more than one split
 };
@@ -484,6 +529,7 @@ constexpr int kTableBytes = (sizeof(FewTable) + 127) / 128 * 128;
 // Sums of the warps, for their owner to add up.
 template <int NT> struct RedShape {
   static constexpr int kTile = NT * 4 * 32 + 1;      // (off the banks of the tile before)
+  static constexpr int kBuffers = NT == 1 ? 2 : 1;   // (two where there is room: one barrier a tile)
   static constexpr int kWarpFloats = kTiles * kTile, kBytes = (kWarps * kWarpFloats * 4 + 127) / 128 * 128;
   // Where the sums of row `row` (of a tile's 16) and column `col` are.
   static __device__ __forceinline__ int at(int tile, int row, int col) {
@@ -502,10 +548,11 @@ __device__ __forceinline__ void store_sums(float* red, const float (&acc)[kTiles
       for (int c = 0; c < 4; ++c) to[i * RedShape<NT>::kTile + (n * 4 + c) * 32] = acc[i][n][c];
 }
 template <int F, int NT> struct UpShape {
-  static constexpr int kFixed = kTableBytes + 512 + kMaxSlots * 4 + RedShape<NT>::kBytes + kWarps * FewShape<F>::kRing;
+  static constexpr int kSums = RedShape<NT>::kBuffers * RedShape<NT>::kBytes;
+  static constexpr int kFixed = kTableBytes + 128 + kSums + kWarps * FewShape<F>::kRing;
 };
 template <int F> struct DownShape {
-  static constexpr int kFixed = kTableBytes + 128 + 2 * kMaxSlots * 4 + kWarps * FewShape<F>::kRing;
+  static constexpr int kFixed = kTableBytes + 128 + kWarps * FewShape<F>::kRing;
 };
 
 // h[row] = act(W13 x + b13).  The features of all active experts, in pieces of eight (a tile's rows: eight gates and their
@@ -516,34 +563,27 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
   using S = FewShape<F>;
   extern __shared__ __align__(128) uint8_t smem[];
   FewTable& table = *reinterpret_cast<FewTable*>(smem);
-  float* const inverse = reinterpret_cast<float*>(smem + kTableBytes);   // of the panel's rows' scales
-  uint32_t* const tops = reinterpret_cast<uint32_t*>(inverse + 32);       // of the panel's rows: largest magnitude
-  uint8_t* const zeros = smem + kTableBytes + 256;                        // a token's values where there is no token
-  uint32_t* const h_top = reinterpret_cast<uint32_t*>(smem + kTableBytes + 512);   // largest |h| per row (bits: NaN counts as largest)
-  float* const red = reinterpret_cast<float*>(smem + kTableBytes + 512 + kMaxSlots * 4);
+  uint8_t* const zeros = smem + kTableBytes;                              // a token's values where there is no token
+  float* const red = reinterpret_cast<float*>(smem + kTableBytes + 128);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_at(smem) + kTableBytes + 512 + kMaxSlots * 4 + RedShape<NT>::kBytes + warp * S::kRing;
+  const uint32_t ring = smem_at(smem) + kTableBytes + 128 + UpShape<F, NT>::kSums + warp * S::kRing;
   uint8_t* const panel = smem + UpShape<F, NT>::kFixed;
   pdl_wait();
   pdl_trigger();
   const FewMatrix& m = p.w13;
   const FewLayout layout(m, F, launch.f16);
   const int steps = (p.hidden + S::kK - 1) / S::kK, per_expert = p.inter / 8;
-  const int most = launch.panel_bytes / (steps * S::kK * 2);      // rows that the panel holds
+  const int most = launch.panel_bytes / (steps * S::kPanelBytes); // rows that the panel holds
   const bool whole = most >= p.tokens;                            // all tokens
   const int k8 = steps * (S::kK / 8);
-  if (tid < 16) {
-    reinterpret_cast<uint32_t*>(zeros)[tid] = 0;
-    tops[tid] = 0;
-  }
-  __syncthreads();
+  auto scales_after = [&](uint8_t* at, int rows) { return reinterpret_cast<float*>(at + rows * steps * (S::kK * 2)); };
   if (warp == 0) {
     build_table<false>(table, p);
   } else {
-    for (int i = tid - 32; i < p.tokens * p.topk; i += kThreads - 32) h_top[i] = 0;
+    if (tid < 48) reinterpret_cast<uint32_t*>(zeros)[tid - 32] = 0;
     if (blockIdx.x == 0)   // (the second kernel counts from there)
       for (int i = tid - 32; i < kFewMaxColumns; i += kThreads - 32) launch.arrived[i] = 0;
-    if (whole) panel_raw<F>(panel, tops, p, (1u << p.tokens) - 1u, k8, warp - 1, kWarps - 1);
+    if (whole) fill_tokens<F>(panel, scales_after(panel, p.tokens), p, (1u << p.tokens) - 1u, k8, launch.f16, warp - 1, kWarps - 1);
   }
   __syncthreads();
   const uint32_t all = (uint32_t)(table.active * per_expert);     // (times the blocks below 2^32: takes_nk)
@@ -568,17 +608,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       }
     }
     // Warps of a group: few where there are many tiles, as every tile's sums cost a barrier of the group; many where there
-    // are few, so that all have work.
-    int shift = 0;
-    {
-      int least = 1 << 30;
-#pragma unroll
-      for (int w = 0; (1 << w) <= kWarps; ++w) {
-        const int pieces = (((to - from) << w) + kWarps - 1) / kWarps, tiles = (pieces + kTiles - 1) / kTiles;
-        const int cost = ((steps + (1 << w) - 1) >> w) * (pieces + tiles) + tiles * (w > 0 ? 8 : 4);
-        if (cost < least) { least = cost; shift = w; }
-      }
-    }
+    // are few, so that all have work and end together.  Both kernels, 1 / 2 / 4 / 8 warps, us: 62 pieces a block (MXFP4, 23
+    // steps) 90.5 / 87.0 / 89.1 / 92.7; 53 (fp8, 32 steps) 102 / 99.7 / 100 / 108; 22 (fp8, 112 steps) 151 / 136 / 125 / 126; 14
+    // (the same) 105 / 84 / 76 / 73; 10 (MXFP4) 31.4 / 29.1 / 29.8 / 29.3.
+    const int shift = to - from >= 40 ? 1 : to - from >= 18 ? 2 : 3;
     const int group = 1 << shift, mine_of = warp >> shift, member = warp & (group - 1);
     const int my_from = from + (((to - from) * mine_of << shift) / kWarps), my_to = from + (((to - from) * (mine_of + 1) << shift) / kWarps);
 
@@ -633,63 +666,50 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       for (int i = 0; i < S::kDepth; ++i) copy_next(i);
       const int rows = __popc(now);
       if (!whole) {
-        panel_raw<F>(panel, tops, p, now, k8, warp, kWarps);
+        fill_tokens<F>(panel, scales_after(panel, rows), p, now, k8, launch.f16, warp, kWarps);
         __syncthreads();
       }
-      panel_scaled<F>(panel, tops, inverse, rows, k8, launch.f16);
-      __syncthreads();
-      if (!whole && tid < 16) tops[tid] = 0;
 
-      int slot = 0, cs = member;
+      int slot = 0, cs = member, tile = 0;
 #pragma unroll 1
       for (int first = my_from; first < my_to;) {
         const int tiles = min(kTiles, min(per_expert - u, my_to - first));
         const uint32_t mine = table.tokens[a] & now;
         FewTokens x[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const bool used = (mine >> (8 * n + g)) & 1;
-          x[n].at = used ? smem_at(panel) + rank_below(now, 8 * n + g) * 64 + t * 16 : smem_at(zeros);
-          x[n].block = used ? rows * 64 : 0;
-        }
+        find_tokens<NT>(x, mine, now, smem_at(panel), smem_at(scales_after(panel, rows)), smem_at(zeros), rows);
         float acc[kTiles][NT][4] = {};
 #pragma unroll 1
         for (; cs < steps; cs += group) take_step<F, NT, true>(acc, ring, slot, tiles, layout, x, cs, cs, copy_next);
         cs -= steps;
         // The tile's sums: a lane has a feature, the members take the tokens in turn.
-        store_sums<NT>(red, acc);
+        float* const sums = red + (RedShape<NT>::kBuffers == 2 && (tile & 1) ? RedShape<NT>::kBytes / 4 : 0);
+        store_sums<NT>(sums, acc);
         if (group > 1) group_sync(1 + mine_of, group * 32);
         else __syncwarp();
         const int i = lane >> 3, f = (u + i) * 8 + (lane & 7);
-        int turn = 0;
+        int turn = tile;
         for (uint32_t left = mine; left; left &= left - 1, ++turn) {
           if ((turn & (group - 1)) != member) continue;
           const int col = __ffs(left) - 1, row = table.first_row[a] + rank_below(table.tokens[a], col);
-          float h = 0.f;
           if (i < tiles) {
-            const float* from_red = red + (warp - member) * RedShape<NT>::kWarpFloats;
+            const float* from_red = sums + (warp - member) * RedShape<NT>::kWarpFloats;
             float gate = 0.f, up = 0.f;
             for (int w = 0; w < group; ++w) {
               gate += from_red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(i, lane & 7, col)];
               up += from_red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(i, 8 + (lane & 7), col)];
             }
-            const float inv = inverse[rank_below(now, col)];
-            gate *= inv;
-            up *= inv;
             if (m.bias) {
               const int64_t at = (int64_t)table.expert[a] * m.n;
               gate += load16(m.bias, at + (pairs ? 2 * f : f), launch.f16);
               up += load16(m.bias, at + (pairs ? 2 * f + 1 : p.inter + f), launch.f16);
             }
-            h = gated(p, gate, up);
-            p.h[(int64_t)row * p.inter + f] = h;
+            p.h[(int64_t)row * p.inter + f] = gated(p, gate, up);
           }
-          uint32_t top = __float_as_uint(h) & 0x7fffffffu;
-          top = __reduce_max_sync(0xffffffffu, top);
-          if (lane == 0) atomicMax(&h_top[row], top);
         }
-        if (group > 1) group_sync(1 + mine_of, group * 32);   // the sums' place is free again
+        // the sums' place is free again: the next tile has another one, and that one's barrier is behind this one's reads
+        if (RedShape<NT>::kBuffers == 1 && group > 1) group_sync(1 + mine_of, group * 32);
         else __syncwarp();
+        ++tile;
         first += tiles;
         u += tiles;
         if (u == per_expert) { u = 0; ++a; }
@@ -698,10 +718,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       __syncthreads();   // the panel is free again
     }
     from = to;
-  }
-  if (begin < end) {
-    const int r0 = table.first_row[begin / per_expert], r1 = table.first_row[(end - 1) / per_expert + 1];
-    for (int r = r0 + tid; r < r1; r += kThreads) launch.top[(int64_t)blockIdx.x * (p.tokens * p.topk) + r] = __uint_as_float(h_top[r]);
   }
 }
 
@@ -716,10 +732,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   FewTable& table = *reinterpret_cast<FewTable*>(smem);
   int& last_one = *reinterpret_cast<int*>(smem + kTableBytes);
   uint8_t* const zeros = smem + kTableBytes + 64;
-  float* const coef = reinterpret_cast<float*>(smem + kTableBytes + 128);   // of the panel's rows: routing weight and the inverse of the scale
-  float* const scales = coef + kMaxSlots;                                     // ... and the scale
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_at(smem) + kTableBytes + 128 + 2 * kMaxSlots * 4 + warp * S::kRing;
+  const uint32_t ring = smem_at(smem) + kTableBytes + 128 + warp * S::kRing;
   uint8_t* const panel = smem + DownShape<F>::kFixed;
   float* const red = reinterpret_cast<float*>(panel);                     // (after the last panel)
   // What routed the tokens was complete before the kernel ahead of this one let it start.
@@ -733,8 +747,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   const int row_begin = (int)((uint32_t)p.hidden * column / columns), row_end = (int)((uint32_t)p.hidden * (column + 1) / columns);
   const uint32_t total = (uint32_t)(table.active * steps);
   const int step_begin = (int)(total * split / launch.splits), step_end = (int)(total * (split + 1) / launch.splits);
-  const int per_expert = p.inter / 8;                                     // (as the first kernel deals its features out)
-  const int room = launch.panel_bytes / (S::kK * 2);                      // rows times steps that the panel holds
+  const int room = launch.panel_bytes / S::kPanelBytes;                   // rows times steps that the panel holds
+  float* const scales = reinterpret_cast<float*>(panel + room * (S::kK * 2));
   bool waited = false;
 
   // How far a panel reaches that begins with step s0 of expert a0: whole experts, then as many steps of the next one as
@@ -760,13 +774,24 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       ++a1;
     }
   };
-  auto finish = [&](float v, int token, int n) {
-    if (m.bias) {
-      for (int k = 0; k < p.topk; ++k) {
-        const int a = table.slot_expert[token * p.topk + k];
-        if (a >= 0) v = fmaf(table.slot_weight[token * p.topk + k], load16(m.bias, (int64_t)table.expert[a] * m.n + n, launch.f16), v);
+  // Routing weights times biases of a token's experts.
+  auto biases = [&](int token, int n) {
+    float v = 0.f;
+    for (int k0 = 0; k0 < p.topk; k0 += 4) {
+      float w[4], b[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int slot = token * p.topk + k0 + k, a = k0 + k < p.topk ? table.slot_expert[slot] : -1;
+        w[k] = a >= 0 ? table.slot_weight[slot] : 0.f;
+        b[k] = a >= 0 ? load16(m.bias, (int64_t)table.expert[a] * m.n + n, launch.f16) : 0.f;
       }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (w[k] != 0.f) v = fmaf(w[k], b[k], v);
     }
+    return v;
+  };
+  auto finish = [&](float v, int token, int n) {
     const int64_t to = (int64_t)token * p.hidden + n;
     if (launch.f16) reinterpret_cast<__half*>(p.out)[to] = __float2half_rn(v);
     else reinterpret_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(v);
@@ -817,6 +842,14 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
     if (rows_here > 0) next_stretch();
 #pragma unroll 1
     for (int i = 0; i < S::kDepth; ++i) copy_next(i);
+    // Biases while the ring fills, by the blocks with the first share.
+    constexpr int kMine = kRows * B200MOE_FEW_TOKENS / kThreads;
+    float bias[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int row = tid % kRows, token = tid / kRows + i * (kThreads / kRows);
+      bias[i] = m.bias && split == 0 && token < p.tokens && row < rows_here ? biases(token, r0 + row) : 0.f;
+    }
     if (!waited) {
       pdl_wait();
       pdl_trigger();
@@ -829,61 +862,17 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       panel_end(a0, s0, a1, s1);
       const int last = s1 > 0 ? a1 : a1 - 1;           // the last expert with steps in the panel
       const int row0 = table.first_row[a0], rows = table.first_row[last + 1] - row0;
-      // Rows' scales, eight lanes a row, from the largest |h| that the blocks of the first kernel with features of its expert
-      // have found; then their values, 256 of a row at a time by a warp, two such pieces together.
-      for (int i = tid / 8; i < (rows + kThreads / 8 - 1) / (kThreads / 8) * (kThreads / 8); i += kThreads / 8) {
-        const int r = row0 + min(i, rows - 1), a = table.row_expert[r];
-        const uint32_t all = (uint32_t)(table.active * per_expert), g1 = launch.up_blocks;
-        const int c0 = (int)((((uint32_t)(a * per_expert) + 1) * g1 - 1) / all), c1 = (int)(((uint32_t)((a + 1) * per_expert) * g1 - 1) / all);
-        float top = 0.f;
-        for (int c = c0 + (tid & 7); c <= c1; c += 8)   // (with less than a piece a block, some have none)
-          if (all * c / g1 < all * (c + 1) / g1) top = max_nan(top, launch.top[c * (p.tokens * p.topk) + r]);
-#pragma unroll
-        for (int d = 4; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
-        float inv;
-        const float scale = row_scale(top, inv);
-        if ((tid & 7) == 0 && i < rows) {
-          coef[i] = table.weight[r] * inv;
-          scales[i] = scale;
-        }
-      }
-      __syncthreads();
       {
-        // the first expert's rows have the steps from s0 on, the last one's those up to s1
+        // (the first expert's rows have the steps from s0 on, the last one's those up to s1)
         constexpr int kPiece = S::kK / 8;
-        const int n0 = table.first_row[a0 + 1] - row0, n2 = last > a0 ? rows - (table.first_row[last] - row0) : 0, n1 = rows - n0 - n2;
-        const int len0 = ((a0 == last && s1 > 0 ? s1 : steps) - s0) * kPiece, len1 = steps * kPiece, len2 = (s1 > 0 ? s1 : steps) * kPiece;
-        const int p0 = (len0 + 31) / 32, p1 = (len1 + 31) / 32, p2 = (len2 + 31) / 32, items = n0 * p0 + n1 * p1 + n2 * p2;
-        // an item's row (of the panel), its piece, where the piece's values come from and go to
-        struct Item { int row, j; const float* from; uint8_t* to; };
-        auto item_of = [&](int item) {
-          Item it = {0, 0, nullptr, nullptr};
-          if (item >= items) return it;
-          int len, k8_0 = 0;
-          if (item < n0 * p0) { it.row = item / p0; it.j = item - it.row * p0; len = len0; k8_0 = s0 * kPiece; }
-          else if (item < n0 * p0 + n1 * p1) { item -= n0 * p0; it.row = item / p1; it.j = item - it.row * p1; it.row += n0; len = len1; }
-          else { item -= n0 * p0 + n1 * p1; it.row = item / p2; it.j = item - it.row * p2; it.row += n0 + n1; len = len2; }
-          it.j = it.j * 32 + lane;
-          if (it.j >= len) return it;
-          const int r = row0 + it.row, a = table.row_expert[r], e0 = table.first_row[a], n = table.first_row[a + 1] - e0;
-          const int before = a == a0 ? 0 : n0 * (steps - s0) + (e0 - row0 - n0) * steps;   // rows times steps of earlier experts in the panel
-          it.to = panel + (int64_t)before * (S::kK * 2) + panel_at<F>(it.j, r - e0, n);
-          if (8 * (k8_0 + it.j) < p.inter) it.from = p.h + (int64_t)r * p.inter + 8 * (k8_0 + it.j);
-          return it;
-        };
+        const int parts = warps_per_row(rows, kWarps), n0 = table.first_row[a0 + 1] - row0;
 #pragma unroll 1
-        for (int first = warp; first < items; first += 2 * kWarps) {
-          const Item i0 = item_of(first), i1 = item_of(first + kWarps);
-          float4 v[4] = {};
-          if (i0.from) { v[0] = reinterpret_cast<const float4*>(i0.from)[0]; v[1] = reinterpret_cast<const float4*>(i0.from)[1]; }
-          if (i1.from) { v[2] = reinterpret_cast<const float4*>(i1.from)[0]; v[3] = reinterpret_cast<const float4*>(i1.from)[1]; }
-          auto put = [&](const Item& it, const float4& a, const float4& b) {
-            if (it.to == nullptr) return;
-            const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            *reinterpret_cast<uint4*>(it.to) = scaled8<F>(x, scales[it.row]);
-          };
-          put(i0, v[0], v[1]);
-          put(i1, v[2], v[3]);
+        for (int row = warp / parts; row < rows; row += kWarps / parts) {
+          const int r = row0 + row, a = table.row_expert[r], e0 = table.first_row[a], n = table.first_row[a + 1] - e0;
+          const int k8_0 = (a == a0 ? s0 : 0) * kPiece, len = (a == a1 ? s1 : steps) * kPiece - k8_0;
+          const int before = a == a0 ? 0 : n0 * (steps - s0) + (e0 - row0 - n0) * steps;   // rows times steps of earlier experts
+          fill_row<F, kFromF32>(panel + before * (S::kK * 2), scales + before, p.h + (int64_t)r * p.inter + 8 * k8_0, p.inter - 8 * k8_0, len,
+                                r - e0, n, warp % parts, parts);
         }
         __syncthreads();
       }
@@ -896,14 +885,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
           // rows of earlier experts in the panel, as above
           const int before = a == a0 ? 0 : (table.first_row[a0 + 1] - row0) * (steps - s0) + (row - table.first_row[a0 + 1]) * steps;
           const uint32_t base = smem_at(panel) + (before - (a == a0 ? s0 : 0) * n_rows) * (S::kK * 2);
+          const uint32_t base_scales = smem_at(scales) + (before - (a == a0 ? s0 : 0) * n_rows) * 4;
           const uint32_t mine = table.tokens[a];
           FewTokens x[NT];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const bool used = (mine >> (8 * n + g)) & 1;
-            x[n].at = used ? base + rank_below(mine, 8 * n + g) * 64 + t * 16 : smem_at(zeros);
-            x[n].block = used ? n_rows * 64 : 0;
-          }
+          find_tokens<NT>(x, mine, mine, base, base_scales, smem_at(zeros), n_rows);
           float acc[kTiles][NT][4] = {};
 #pragma unroll 1
           for (; pos < end; ++pos) take_step<F, NT, false>(acc, ring, slot, tiles, layout, x, pos - a * steps, pos - a * steps, copy_next);
@@ -914,7 +899,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
             for (int c = 0; c < 2; ++c) {
               const int token = 8 * n + 2 * t + c;
               if (!((mine >> token) & 1)) continue;
-              const float w = coef[row - row0 + rank_below(mine, token)];
+              const float w = table.weight[row + rank_below(mine, token)];
 #pragma unroll
               for (int i = 0; i < kTiles; ++i) {
                 out[i][n][c] = fmaf(w, acc[i][n][c], out[i][n][c]);
@@ -930,11 +915,12 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
     store_sums<NT>(red, out);
     copies_wait<0>();
     __syncthreads();
-    for (int j = tid; j < kRows * p.tokens; j += kThreads) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
       // consecutive threads, consecutive features of a token
-      const int row = j % kRows, token = j / kRows;
-      if (row >= rows_here) continue;
-      float v = 0.f;
+      const int row = tid % kRows, token = tid / kRows + i * (kThreads / kRows);
+      if (row >= rows_here || token >= p.tokens) continue;
+      float v = bias[i];
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) v += red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(row >> 4, row & 15, token)];
       const int64_t to = (int64_t)token * p.hidden + r0 + row;
@@ -954,7 +940,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   for (int j = tid; j < width * p.tokens; j += kThreads) {
     const int row = row_begin + j % width, token = j / width;
     float v = 0.f;
-    for (int i = 0; i < launch.splits; ++i) v += __ldcg(launch.part + ((int64_t)i * p.tokens + token) * p.hidden + row);
+    const float* from = launch.part + (int64_t)token * p.hidden + row;
+    const int64_t next = (int64_t)p.tokens * p.hidden;
+#pragma unroll 4
+    for (int i = 0; i < launch.splits; ++i) v += __ldcg(from + i * next);
     finish(v, token, row);
   }
 }

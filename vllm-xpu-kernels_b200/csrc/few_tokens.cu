@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(256) few_up_simple_kernel(FewParams p) {
       g += to_f32<T>(b[(int64_t)e * p.w13.n + ng]);
       u += to_f32<T>(b[(int64_t)e * p.w13.n + nu]);
     }
-    p.h[(int64_t)slot * p.inter + f] = gated(p, g, u);
+    p.h[(int64_t)slot * p.inter + f] = gated(p.act, p.alpha, p.limit, p.clamp, g, u);
   }
 }
 

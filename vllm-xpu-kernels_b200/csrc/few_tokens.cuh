@@ -59,21 +59,21 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 __device__ __forceinline__ float clamp_nan(float v, float limit) { return max_nan(min_nan(v, limit), -limit); }
 
 // The gated activation in fp32, unrounded.
-__device__ __forceinline__ float gated(const FewParams& p, float g, float u) {
-  if (p.clamp > 0.f) {
-    g = min_nan(g, p.clamp);
-    u = clamp_nan(u, p.clamp);
+__device__ __forceinline__ float gated(int act, float alpha, float limit, float clamp, float g, float u) {
+  if (clamp > 0.f) {
+    g = min_nan(g, clamp);
+    u = clamp_nan(u, clamp);
   }
-  switch (p.act) {
+  switch (act) {
     case B200MOE_ACT_SILU: return g / (1.0f + expf(-g)) * u;
     case B200MOE_ACT_GELU: return 0.5f * g * (1.0f + erff(g * 0.70710678118654752440f)) * u;
     case B200MOE_ACT_GELU_TANH:
       return 0.5f * g * (1.0f + tanhf(0.79788456080286535588f * (g + 0.044715f * (g * g * g)))) * u;
     case B200MOE_ACT_SWIGLUOAI:
-      g = min_nan(g, p.limit);
-      u = clamp_nan(u, p.limit);
-      return (u + 1.0f) * (g / (1.0f + expf(-g * p.alpha)));
-    default: return min_nan(g / (1.0f + expf(-g)), p.limit) * clamp_nan(u, p.limit);
+      g = min_nan(g, limit);
+      u = clamp_nan(u, limit);
+      return (u + 1.0f) * (g / (1.0f + expf(-g * alpha)));
+    default: return min_nan(g / (1.0f + expf(-g)), limit) * clamp_nan(u, limit);
   }
 }
 

@@ -239,13 +239,15 @@ __device__ __forceinline__ uint4 scaled8(const float (&v)[8], float scale) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-enum FewSource { kFromBf16, kFromF16, kFromF32 };
 // `len` eighths of a row (what is beyond `values` values is zero) into a panel, by `parts` warps of which this is `part`.  A warp
-// asks for four times 256 values at once: the loads' latency is what this costs.
-template <int F, int Source>
-__device__ __forceinline__ void fill_row(uint8_t* panel, float* scales, const void* from, int values, int len, int row, int rows, int part, int parts) {
+// asks for four times 256 values at once: the loads' latency is what this costs.  (Functions that run once in a while are not
+// inlined: both kernels' code together has to stay in the SM's instruction cache.  With 160 KB of it every launch began
+// with some 3 us of misses.)
+template <int F, bool kF32>
+__device__ __noinline__ void fill_row(uint8_t* panel, float* scales, const void* from, int values, int len, int row, int rows, int part, int parts,
+                                      bool f16) {
   constexpr int kLanes = FewShape<F>::kK / 8;      // of a step
-  constexpr int kWords = Source == kFromF32 ? 2 : 1;
+  constexpr int kWords = kF32 ? 2 : 1;
   const int lane = threadIdx.x & 31, stride = 32 * parts;
 #pragma unroll 1
   for (int j0 = part * 32 + lane; j0 - lane < len; j0 += 4 * stride) {
@@ -265,16 +267,13 @@ __device__ __forceinline__ void fill_row(uint8_t* panel, float* scales, const vo
       float v[8];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if constexpr (Source == kFromF32) {
+        if constexpr (kF32) {
           v[k] = __uint_as_float(raw[i][0].w[k]);
           v[4 + k] = __uint_as_float(raw[i][kWords - 1].w[k]);
-        } else if constexpr (Source == kFromBf16) {
-          v[2 * k] = __uint_as_float(raw[i][0].w[k] << 16);
-          v[2 * k + 1] = __uint_as_float(raw[i][0].w[k] & 0xffff0000u);
         } else {
           const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&raw[i][0].w[k]));
-          v[2 * k] = f.x;
-          v[2 * k + 1] = f.y;
+          v[2 * k] = f16 ? f.x : __uint_as_float(raw[i][0].w[k] << 16);
+          v[2 * k + 1] = f16 ? f.y : __uint_as_float(raw[i][0].w[k] & 0xffff0000u);
         }
       }
       uint32_t top = 0;        // (as bits: magnitudes in their order, NaN last)
@@ -296,15 +295,15 @@ __device__ __forceinline__ int warps_per_row(int rows, int warps) { return rows 
 
 // Tokens of the set `now` into a panel.
 template <int F>
-__device__ __forceinline__ void fill_tokens(uint8_t* panel, float* scales, const FewParams& p, uint32_t now, int len, bool f16, int member, int members) {
+__device__ __noinline__ void fill_tokens(uint8_t* panel, float* scales, const void* from, int hidden, uint32_t now, int len, bool f16,
+                                          int member, int members) {
   const int rows = __popc(now), parts = warps_per_row(rows, members);
 #pragma unroll 1
   for (int row = member / parts; row < rows; row += members / parts) {
     uint32_t left = now;
     for (int r = 0; r < row; ++r) left &= left - 1;
-    const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x) + (int64_t)(__ffs(left) - 1) * p.hidden;
-    if (f16) fill_row<F, kFromF16>(panel, scales, x, p.hidden, len, row, rows, member % parts, parts);
-    else fill_row<F, kFromBf16>(panel, scales, x, p.hidden, len, row, rows, member % parts, parts);
+    const uint16_t* x = reinterpret_cast<const uint16_t*>(from) + (int64_t)(__ffs(left) - 1) * hidden;
+    fill_row<F, false>(panel, scales, x, hidden, len, row, rows, member % parts, parts, f16);
   }
 }
 
@@ -326,20 +325,21 @@ struct FewRows {
 // The matrix as a whole.
 struct FewLayout {
   int row_bytes, group;
-  int64_t word_step;     // bytes from one word of a row's scales to the next
+  int words, word_step;  // of a row's scales (4 bits), and bytes from one to the next
   bool f16;
   __device__ __forceinline__ FewLayout(const FewMatrix& m, int f, bool half) {
     row_bytes = f == kFewFp8 ? m.k : m.k / 2;
     group = m.group;
-    word_step = f == kFewFp8 ? 4 : 4 * (int64_t)m.n;
+    words = f == kFewFp8 ? 0 : few_scale_words(m.format, m.group, m.k);
+    word_step = f == kFewFp8 ? 4 : 4 * m.n;
     f16 = half;
   }
 };
 // Scales of step 0 of row n.  4 bits: [experts][words][n], words as in few_scale_words.
 template <int F>
-__device__ __forceinline__ const uint8_t* scales_of(const FewMatrix& m, int64_t e, int n) {
-  if (F == kFewFp8) return reinterpret_cast<const uint8_t*>(m.scale) + ((e * (m.n / 128) + n / 128) * (m.k / 128)) * 4;
-  return reinterpret_cast<const uint8_t*>(m.scale) + (e * few_scale_words(m.format, m.group, m.k) * m.n + n) * 4;
+__device__ __forceinline__ const uint8_t* scales_of(const FewMatrix& m, const FewLayout& l, int e, int n) {
+  if (F == kFewFp8) return reinterpret_cast<const uint8_t*>(m.scale) + (int64_t)(e * (m.n >> 7) + (n >> 7)) * (m.k >> 5);
+  return reinterpret_cast<const uint8_t*>(m.scale) + (int64_t)(e * l.words) * (4 * m.n) + n * 4;
 }
 
 // Fetches step s into a slot.
@@ -366,7 +366,7 @@ __device__ __forceinline__ void copy_step(uint32_t slot, const FewRows& r, const
     if (!r.there[j]) continue;
 #pragma unroll
     for (int i = 0; i < S::kScaleWords; ++i)
-      if (i == 0 || two) copy4(slot + kRows * 64 + ((j * 32 + lane) * S::kScaleWords + i) * 4, r.s[j] + (word + i) * l.word_step);
+      if (i == 0 || two) copy4(slot + kRows * 64 + ((j * 32 + lane) * S::kScaleWords + i) * 4, r.s[j] + (int64_t)(word + i) * l.word_step);
   }
 }
 
@@ -512,6 +512,9 @@ __device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], uint32_t 
   slot = slot + 1 == S::kDepth ? 0 : slot + 1;
 }
 
+__device__ __noinline__ float gated_once(int act, float alpha, float limit, float clamp, float gate, float up) {
+  return gated(act, alpha, limit, clamp, gate, up);
+}
 __device__ __forceinline__ float load16(const void* p, int64_t i, bool f16) {
   return f16 ? __half2float(reinterpret_cast<const __half*>(p)[i]) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
 }
@@ -583,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
     if (tid < 48) reinterpret_cast<uint32_t*>(zeros)[tid - 32] = 0;
     if (blockIdx.x == 0)   // (the second kernel counts from there)
       for (int i = tid - 32; i < kFewMaxColumns; i += kThreads - 32) launch.arrived[i] = 0;
-    if (whole) fill_tokens<F>(panel, scales_after(panel, p.tokens), p, (1u << p.tokens) - 1u, k8, launch.f16, warp - 1, kWarps - 1);
+    if (whole) fill_tokens<F>(panel, scales_after(panel, p.tokens), p.x, p.hidden, (1u << p.tokens) - 1u, k8, launch.f16, warp - 1, kWarps - 1);
   }
   __syncthreads();
   const uint32_t all = (uint32_t)(table.active * per_expert);     // (times the blocks below 2^32: takes_nk)
@@ -621,52 +624,51 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       while (__popc(now) > most) now &= ~(1u << (31 - __clz(now)));
       rest &= ~now;
 
-      auto tile_rows = [&](FewRows& r, int a, int f, int last) {       // of the tiles that begin with feature f
-        const int64_t e = table.expert[a], rb = layout.row_bytes;
-        r.tiles = min(kTiles, last);
-        r.w = reinterpret_cast<const uint8_t*>(m.w) + (e * m.n + (pairs ? 2 * (f + g) : f + g)) * rb + t * 16;
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          r.to[2 * i] = (pairs ? 16 : 8) * i * rb;
-          r.to[2 * i + 1] = r.to[2 * i] + (pairs ? rb : p.inter * rb);
-        }
-#pragma unroll
-        for (int j = 0; j < kRows / 32; ++j) {
-          // gates in the first half of the places, ups in the second
-          const int place = j * 32 + lane, up = place >= kRows / 2, fs = place % (kRows / 2);
-          r.there[j] = fs < 8 * r.tiles;
-          r.s[j] = scales_of<F>(m, e, r.there[j] ? (pairs ? 2 * (f + fs) + up : f + fs + up * p.inter) : 0);
-        }
-      };
-      // the ring begins to fill
-      // of the step that is fetched next: its tiles' first piece (of all, and within its expert), the expert
+      // The ring begins to fill.  Of the step that is fetched next: its tiles' first piece (of all, and within its expert),
+      // the expert, and whether its rows have been found.
       int next = my_from, next_a = my_from / per_expert, next_u = my_from - next_a * per_expert, s = member;
+      int a = next_a, u = next_u;
+      bool found = false;
       FewRows fetch;
-      auto settle = [&]() {
-        while (s >= steps && next < my_to) {
-          s -= steps;
-          next += fetch.tiles;
-          next_u += fetch.tiles;
-          if (next_u == per_expert) { next_u = 0; ++next_a; }
-          if (next < my_to) tile_rows(fetch, next_a, next_u * 8, min(per_expert - next_u, my_to - next));
-        }
-      };
+      fetch.tiles = 0;
       auto copy_next = [&](int slot) {
+        while (next < my_to && (s >= steps || !found)) {
+          if (found) {
+            s -= steps;
+            next += fetch.tiles;
+            next_u += fetch.tiles;
+            if (next_u == per_expert) { next_u = 0; ++next_a; }
+            if (next >= my_to) break;
+          }
+          const int e = table.expert[next_a], f = next_u * 8, rb = layout.row_bytes;
+          found = true;
+          fetch.tiles = min(kTiles, min(per_expert - next_u, my_to - next));
+          fetch.w = reinterpret_cast<const uint8_t*>(m.w) + (int64_t)(e * m.n + (pairs ? 2 * (f + g) : f + g)) * rb + t * 16;
+          const int64_t other = pairs ? rb : (int64_t)p.inter * rb;
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) {
+            fetch.to[2 * i] = (int64_t)((pairs ? 16 : 8) * i) * rb;
+            fetch.to[2 * i + 1] = fetch.to[2 * i] + other;
+          }
+#pragma unroll
+          for (int j = 0; j < kRows / 32; ++j) {
+            // gates in the first half of the places, ups in the second
+            const int place = j * 32 + lane, up = place >= kRows / 2, fs = place % (kRows / 2);
+            fetch.there[j] = fs < 8 * fetch.tiles;
+            fetch.s[j] = scales_of<F>(m, layout, e, fetch.there[j] ? (pairs ? 2 * (f + fs) + up : f + fs + up * p.inter) : 0);
+          }
+        }
         if (next < my_to) {
           copy_step<F>(ring + slot * S::kSlot, fetch, layout, s);
           s += group;
-          settle();
         }
         copies_end();
       };
-      int a = next_a, u = next_u;
-      if (next < my_to) tile_rows(fetch, next_a, next_u * 8, min(per_expert - next_u, my_to - next));
-      settle();
 #pragma unroll 1
       for (int i = 0; i < S::kDepth; ++i) copy_next(i);
       const int rows = __popc(now);
       if (!whole) {
-        fill_tokens<F>(panel, scales_after(panel, rows), p, now, k8, launch.f16, warp, kWarps);
+        fill_tokens<F>(panel, scales_after(panel, rows), p.x, p.hidden, now, k8, launch.f16, warp, kWarps);
         __syncthreads();
       }
 
@@ -703,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
               gate += load16(m.bias, at + (pairs ? 2 * f : f), launch.f16);
               up += load16(m.bias, at + (pairs ? 2 * f + 1 : p.inter + f), launch.f16);
             }
-            p.h[(int64_t)row * p.inter + f] = gated(p, gate, up);
+            p.h[(int64_t)row * p.inter + f] = gated_once(p.act, p.alpha, p.limit, p.clamp, gate, up);
           }
         }
         // the sums' place is free again: the next tile has another one, and that one's barrier is behind this one's reads
@@ -719,6 +721,24 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
     }
     from = to;
   }
+}
+
+// Routing weights times biases of a token's experts, for output n.
+__device__ __noinline__ float weighted_bias(const FewTable& table, const FewMatrix& m, int topk, bool f16, int token, int n) {
+  float v = 0.f;
+  for (int k0 = 0; k0 < topk; k0 += 4) {
+    float w[4], b[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int slot = token * topk + k0 + k, a = k0 + k < topk ? table.slot_expert[slot] : -1;
+      w[k] = a >= 0 ? table.slot_weight[slot] : 0.f;
+      b[k] = a >= 0 ? load16(m.bias, (int64_t)table.expert[a] * m.n + n, f16) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (w[k] != 0.f) v = fmaf(w[k], b[k], v);
+  }
+  return v;
 }
 
 // out = sum over experts of weight * (W2 h + b2).  A block has some rows of W2 and a share of the steps over all active
@@ -774,23 +794,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       ++a1;
     }
   };
-  // Routing weights times biases of a token's experts.
-  auto biases = [&](int token, int n) {
-    float v = 0.f;
-    for (int k0 = 0; k0 < p.topk; k0 += 4) {
-      float w[4], b[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int slot = token * p.topk + k0 + k, a = k0 + k < p.topk ? table.slot_expert[slot] : -1;
-        w[k] = a >= 0 ? table.slot_weight[slot] : 0.f;
-        b[k] = a >= 0 ? load16(m.bias, (int64_t)table.expert[a] * m.n + n, launch.f16) : 0.f;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (w[k] != 0.f) v = fmaf(w[k], b[k], v);
-    }
-    return v;
-  };
   auto finish = [&](float v, int token, int n) {
     const int64_t to = (int64_t)token * p.hidden + n;
     if (launch.f16) reinterpret_cast<__half*>(p.out)[to] = __float2half_rn(v);
@@ -805,15 +808,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       fetch.to[i] = (int64_t)max(0, min(8 * i + g, rows_here - 1)) * layout.row_bytes;   // (what a tile has not got is the last row again)
 #pragma unroll
     for (int j = 0; j < kRows / 32; ++j) fetch.there[j] = j * 32 + lane < rows_here;
-    auto expert_rows = [&](int a) {
-      const int64_t e = table.expert[a];
-      fetch.w = reinterpret_cast<const uint8_t*>(m.w) + (e * m.n + r0) * layout.row_bytes + t * 16;
-#pragma unroll
-      for (int j = 0; j < kRows / 32; ++j) fetch.s[j] = scales_of<F>(m, e, fetch.there[j] ? r0 + j * 32 + lane : r0);
-    };
-    // The step that is fetched next, the end of this warp's stretch, and where the panel after that begins.
+    // The step that is fetched next, how many are left of this warp's stretch, and where the panel after that begins.
     int fetch_a = 0, fetch_s = 0, left = 0, panel_a = step_begin / steps, panel_s = step_begin - panel_a * steps;
-    auto next_stretch = [&]() {
+    bool found = false;
+    auto copy_next = [&](int slot) {
       while (left == 0 && panel_a * steps + panel_s < step_end) {
         int a1, s1;
         panel_end(panel_a, panel_s, a1, s1);
@@ -823,23 +821,23 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
         fetch_s = from + mine - fetch_a * steps;
         panel_a = a1;
         panel_s = s1;
-        if (left > 0) expert_rows(fetch_a);
+        found = false;
       }
-    };
-    auto copy_next = [&](int slot) {
-      if (left > 0) {
+      if (left > 0 && rows_here > 0) {
+        if (fetch_s == steps) { fetch_s = 0; ++fetch_a; found = false; }
+        if (!found) {
+          const int e = table.expert[fetch_a];
+          fetch.w = reinterpret_cast<const uint8_t*>(m.w) + (int64_t)(e * m.n + r0) * layout.row_bytes + t * 16;
+#pragma unroll
+          for (int j = 0; j < kRows / 32; ++j) fetch.s[j] = scales_of<F>(m, layout, e, fetch.there[j] ? r0 + j * 32 + lane : r0);
+          found = true;
+        }
         copy_step<F>(ring + slot * S::kSlot, fetch, layout, fetch_s);
         ++fetch_s;
-        if (--left == 0) {
-          next_stretch();
-        } else if (fetch_s == steps) {
-          fetch_s = 0;
-          expert_rows(++fetch_a);
-        }
+        --left;
       }
       copies_end();
     };
-    if (rows_here > 0) next_stretch();
 #pragma unroll 1
     for (int i = 0; i < S::kDepth; ++i) copy_next(i);
     // Biases while the ring fills, by the blocks with the first share.
@@ -848,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int row = tid % kRows, token = tid / kRows + i * (kThreads / kRows);
-      bias[i] = m.bias && split == 0 && token < p.tokens && row < rows_here ? biases(token, r0 + row) : 0.f;
+      bias[i] = m.bias && split == 0 && token < p.tokens && row < rows_here ? weighted_bias(table, m, p.topk, launch.f16, token, r0 + row) : 0.f;
     }
     if (!waited) {
       pdl_wait();
@@ -871,8 +869,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
           const int r = row0 + row, a = table.row_expert[r], e0 = table.first_row[a], n = table.first_row[a + 1] - e0;
           const int k8_0 = (a == a0 ? s0 : 0) * kPiece, len = (a == a1 ? s1 : steps) * kPiece - k8_0;
           const int before = a == a0 ? 0 : n0 * (steps - s0) + (e0 - row0 - n0) * steps;   // rows times steps of earlier experts
-          fill_row<F, kFromF32>(panel + before * (S::kK * 2), scales + before, p.h + (int64_t)r * p.inter + 8 * k8_0, p.inter - 8 * k8_0, len,
-                                r - e0, n, warp % parts, parts);
+          fill_row<F, true>(panel + before * (S::kK * 2), scales + before, p.h + (int64_t)r * p.inter + 8 * k8_0, p.inter - 8 * k8_0, len,
+                            r - e0, n, warp % parts, parts, false);
         }
         __syncthreads();
       }

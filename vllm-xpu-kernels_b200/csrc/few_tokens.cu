@@ -135,32 +135,40 @@ struct FewWorkspace {
 };
 
 template <int F, int NT>
-int launch_nk(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
+int launch_mma(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   constexpr int k = FewShape<F>::kK, up_room = kMaxSmem - UpShape<F, NT>::kFixed, down_room = kMaxSmem - DownShape<F>::kFixed;
-  constexpr int step = FewShape<F>::kPanelBytes;
-  const int up_row = (p.hidden + k - 1) / k * step, down_row = (p.inter + k - 1) / k * step;
+  const int up_row = (p.hidden + k - 1) / k * FewShape<F>::kPanelBytes(1);
+  const int down_row = (p.inter + k - 1) / k * FewShape<F>::kPanelBytes(FewShape<F>::kTerms);
   l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
-  l.splits = FewWorkspace::splits(p.hidden, ctas);
+  int columns = (p.hidden + kRows - 1) / kRows;
+  if (by_column(F)) {
+    if (columns > ctas) columns = ctas;
+    l.splits = ctas / columns;
+  } else {
+    l.splits = FewWorkspace::splits(p.hidden, ctas);
+    columns = ctas / l.splits;
+  }
   int rc = launch_block_per_sm<few_up_kernel<F, NT>>("few_up_kernel", ctas, UpShape<F, NT>::kFixed + l.panel_bytes, st, p, l);
   if (rc != B200MOE_OK) return rc;
   const int64_t want = (int64_t)p.tokens * p.topk * down_row;
   l.panel_bytes = (int)(want < down_room ? want : down_room);
   if (l.panel_bytes < RedShape<NT>::kBytes) l.panel_bytes = RedShape<NT>::kBytes;
-  return launch_block_per_sm<few_down_kernel<F, NT>>("few_down_kernel", ctas / l.splits * l.splits, DownShape<F>::kFixed + l.panel_bytes, st, p, l);
+  return launch_block_per_sm<few_down_kernel<F, NT>>("few_down_kernel", columns * l.splits, DownShape<F>::kFixed + l.panel_bytes, st, p, l);
 }
 
 template <int F>
-int launch_nk(const FewParams& p, const FewLaunch& l, int ctas, cudaStream_t st) {
-  return p.tokens <= 8 ? launch_nk<F, 1>(p, l, ctas, st) : launch_nk<F, 2>(p, l, ctas, st);
+int launch_mma(const FewParams& p, const FewLaunch& l, int ctas, cudaStream_t st) {
+  return p.tokens <= 8 ? launch_mma<F, 1>(p, l, ctas, st) : launch_mma<F, 2>(p, l, ctas, st);
 }
 
 // Sizes and addresses that these kernels can take; one row of tokens has to fit a block's shared memory.
-bool takes_nk(const FewParams& p) {
-  const int f = p.w13.format;
-  if (f != B200MOE_W_FP8_BLOCK_NK && f != B200MOE_W_MXFP4_NK && f != B200MOE_W_INT4_NK) return false;
+bool takes_mma(const FewParams& p) {
+  const bool by_columns = p.w13.format == B200MOE_W_BF16_KN;
+  if (p.w13.format == B200MOE_W_FP8_BLOCK_KN) return false;
   for (const void* a : {p.x, p.w13.w, p.w13.scale, p.w2.w, p.w2.scale})
     if (((uintptr_t)a & 15) != 0) return false;
-  return p.hidden % 32 == 0 && p.inter % 32 == 0 && p.hidden <= 16384 && p.inter <= 65536;
+  const int whole = by_columns ? 8 : 32;
+  return p.hidden % whole == 0 && p.inter % whole == 0 && p.hidden <= 16384 && p.inter <= 65536;
 }
 
 bool known_format(int f) {
@@ -228,16 +236,18 @@ extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200mo
   p.w2 = {a->w2, a->w2_scale, a->w2_bias, a->w2_format, a->w2_group, a->hidden, a->inter};
   int ctas = a->max_ctas > 0 && a->max_ctas < sm_count() ? a->max_ctas : sm_count();
   if (ctas > kFewMaxBlocks) ctas = kFewMaxBlocks;
-  if (takes_nk(p)) {
+  if (takes_mma(p)) {
     FewLaunch l = {};
     l.f16 = a->dtype == B200MOE_F16;
     const FewWorkspace ws(p.tokens, p.topk, p.hidden, p.inter);
     l.arrived = (uint32_t*)((char*)a->workspace + ws.arrived);
     l.part = (float*)((char*)a->workspace + ws.part);
-    if (p.w13.format == B200MOE_W_FP8_BLOCK_NK) return launch_nk<kFewFp8>(p, l, ctas, as_stream(stream));
-    if (p.w13.format == B200MOE_W_MXFP4_NK) return launch_nk<kFewFp4>(p, l, ctas, as_stream(stream));
+    if (p.w13.format == B200MOE_W_BF16_KN)
+      return l.f16 ? launch_mma<kFewF16>(p, l, ctas, as_stream(stream)) : launch_mma<kFewBf16>(p, l, ctas, as_stream(stream));
+    if (p.w13.format == B200MOE_W_FP8_BLOCK_NK) return launch_mma<kFewFp8>(p, l, ctas, as_stream(stream));
+    if (p.w13.format == B200MOE_W_MXFP4_NK) return launch_mma<kFewFp4>(p, l, ctas, as_stream(stream));
     const bool fine = p.w13.group < 128 || p.w2.group < 128;
-    return fine ? launch_nk<kFewInt4Fine>(p, l, ctas, as_stream(stream)) : launch_nk<kFewInt4>(p, l, ctas, as_stream(stream));
+    return fine ? launch_mma<kFewInt4Fine>(p, l, ctas, as_stream(stream)) : launch_mma<kFewInt4>(p, l, ctas, as_stream(stream));
   }
   return a->dtype == B200MOE_BF16 ? launch_simple<__nv_bfloat16>(p, as_stream(stream)) : launch_simple<__half>(p, as_stream(stream));
 }

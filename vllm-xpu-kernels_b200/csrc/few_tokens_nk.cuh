@@ -28,16 +28,21 @@ constexpr int kFewMaxBlocks = 160;      // of a kernel (one per SM)
 constexpr int kFewMaxColumns = kFewMaxBlocks;
 constexpr int kMaxSlots = kFewMaxTopk * B200MOE_FEW_TOKENS;   // routed slots of a call
 
-enum FewFormat { kFewFp8, kFewFp4, kFewInt4Fine, kFewInt4 };   // Fine: groups of 32 or 64
+enum FewFormat { kFewFp8, kFewFp4, kFewInt4Fine, kFewInt4, kFewBf16, kFewF16 };   // Fine: groups of 32 or 64
+__host__ __device__ constexpr bool by_column(int f) { return f == kFewBf16 || f == kFewF16; }     // stored as [K, N]
 
-// A step of a warp is 64 bytes of its 64 rows.
+// A step of a warp is 64 bytes of its 64 rows; of weights stored by column 32 rows of 128 bytes.
 template <int F> struct FewShape {
-  static constexpr int kK = F == kFewFp8 ? 64 : 128;             // values of a row
+  static constexpr int kK = by_column(F) ? 32 : F == kFewFp8 ? 64 : 128;      // values of k
   static constexpr int kBlocks = kK / 32;                        // of the panel: a lane's eight values, two instructions
-  static constexpr int kPanelBytes = kK * 2 + 4;                 // of the panel: a row's values of a step and their scale
+  // Of the panel: a row's values of a step and their scale.  h next to 16-bit weights is there twice, as the type has it
+  // and what that leaves of it: with one rounding to 16 bits the results would be 1.4 times as far from the formula's as
+  // their own rounding puts them.
+  __host__ __device__ static constexpr int kPanelBytes(int terms) { return terms * kK * 2 + 4; }
+  static constexpr int kTerms = by_column(F) ? 2 : 1;            // of h
   static constexpr int kScaleWords = F == kFewInt4Fine ? 2 : 1;  // that hold a row's scales of a step
-  static constexpr int kScales = F == kFewFp8 ? 0 : F == kFewInt4 ? 1 : 4;                       // of a row and step, made fp32 (fp8: are so)
-  static constexpr int kSlot = kRows * (64 + 4 * kScaleWords);
+  static constexpr int kScales = F == kFewFp8 || by_column(F) ? 0 : F == kFewInt4 ? 1 : 4;                       // of a row and step, made fp32 (fp8: are so)
+  static constexpr int kSlot = kRows * (64 + (by_column(F) ? 0 : 4 * kScaleWords));
   static constexpr int kDepth = 3;
   static constexpr int kRing = kDepth * kSlot + kRows * kScales * 4;
 };
@@ -139,6 +144,10 @@ __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+// `bytes` of the 16 come from memory, the rest are zeros.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
@@ -199,6 +208,10 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 // The first product of a sum.
 __device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
@@ -208,10 +221,10 @@ __device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a
 // ---- tokens and activations as float16 -------------------------------------------------
 // A panel holds rows of values in the order in which the lanes want them: per step blocks of [row][4 lanes][8 values].
 // Where k sits: fp8 lanes hold 16 bytes of a row, 16 values; 4-bit formats hand a group of 32 values out to the four lanes,
-// eight each.  Behind them, per row and step, the inverse of what the values have been multiplied by.
+// eight each, and weights by column 32 rows.  Behind them, per row and step, the inverse of what the values have been multiplied by.
 template <int F>
-__device__ __forceinline__ uint32_t panel_at(int k8, int row, int rows) {   // k8: k / 8
-  const int block = F == kFewFp8 ? (k8 >> 3) * 2 + (k8 & 1) : k8 >> 2;
+__device__ __forceinline__ uint32_t panel_at(int k8, int row, int rows, int terms) {   // k8: k / 8; a second term is a block on
+  const int block = (F == kFewFp8 ? (k8 >> 3) * 2 + (k8 & 1) : k8 >> 2) * terms;
   const int t = F == kFewFp8 ? (k8 >> 1) & 3 : k8 & 3;
   return (uint32_t)(((block * rows + row) * 4 + t) * 16);
 }
@@ -228,13 +241,18 @@ __device__ __forceinline__ float step_scale(uint32_t top, float& inverse) {   //
 
 // Eight values as a lane wants them: int4 pairs are four apart.
 template <int F>
-__device__ __forceinline__ uint4 scaled8(const float (&v)[8], float scale) {
+__device__ __forceinline__ uint4 packed8(const float (&v)[8]) {
   constexpr bool kApart = F == kFewInt4 || F == kFewInt4Fine;
   uint32_t o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 h = kApart ? __floats2half2_rn(v[i] * scale, v[i + 4] * scale) : __floats2half2_rn(v[2 * i] * scale, v[2 * i + 1] * scale);
-    o[i] = *reinterpret_cast<const uint32_t*>(&h);
+    if constexpr (F == kFewBf16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      o[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __half2 h = kApart ? __floats2half2_rn(v[i], v[i + 4]) : __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      o[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
@@ -281,10 +299,30 @@ __device__ __noinline__ void fill_row(uint8_t* panel, float* scales, const void*
       for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
 #pragma unroll
       for (int d = 1; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-      float inv;
-      const float scale = step_scale(top, inv);
+      float inv = 1.f;
+      if constexpr (F != kFewBf16) {
+        const float scale = step_scale(top, inv);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= scale;
+      }
       if (j < len) {
-        *reinterpret_cast<uint4*>(panel + panel_at<F>(j, row, rows)) = scaled8<F>(v, scale);
+        constexpr int kTerms = kF32 ? FewShape<F>::kTerms : 1;
+        uint8_t* const at = panel + panel_at<F>(j, row, rows, kTerms);
+        const uint4 o = packed8<F>(v);
+        *reinterpret_cast<uint4*>(at) = o;
+        if constexpr (kTerms == 2) {
+          const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+          float rest[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+            const float x = F == kFewBf16 ? __uint_as_float(w[k] << 16) : f.x, y = F == kFewBf16 ? __uint_as_float(w[k] & 0xffff0000u) : f.y;
+            // (what is not finite leaves nothing)
+            rest[2 * k] = fabsf(v[2 * k]) < INFINITY ? v[2 * k] - x : 0.f;
+            rest[2 * k + 1] = fabsf(v[2 * k + 1]) < INFINITY ? v[2 * k + 1] - y : 0.f;
+          }
+          *reinterpret_cast<uint4*>(at + rows * 64) = packed8<F>(rest);
+        }
         if ((j & (kLanes - 1)) == 0) scales[j / kLanes * rows + row] = inv;
       }
     }
@@ -316,19 +354,20 @@ __device__ __noinline__ void fill_tokens(uint8_t* panel, float* scales, const vo
 
 // The lane's part of the rows of one expert's matrix that a warp takes at once.
 struct FewRows {
-  const uint8_t* w;                       // its 16 bytes of step 0 in row g (lane = 4 g + t)
-  int64_t to[2 * kTiles];                 // from there to rows g + 8 i
+  const uint8_t* w;                       // its 16 bytes of step 0 in row g (lane = 4 g + t); by column: in row 8 t of k
+  int64_t to[2 * kTiles];                 // from there to rows g + 8 i (by column: not used)
   const uint8_t* s[kRows / 32];           // scales of step 0 of the rows that it looks after, places lane + 32 i
   bool there[kRows / 32];                 // whether these rows are
   int tiles;                              // that there are
 };
 // The matrix as a whole.
 struct FewLayout {
-  int row_bytes, group;
+  int row_bytes, group, k;
   int words, word_step;  // of a row's scales (4 bits), and bytes from one to the next
   bool f16;
   __device__ __forceinline__ FewLayout(const FewMatrix& m, int f, bool half) {
-    row_bytes = f == kFewFp8 ? m.k : m.k / 2;
+    row_bytes = by_column(f) ? 2 * m.n : f == kFewFp8 ? m.k : m.k / 2;
+    k = m.k;
     group = m.group;
     words = f == kFewFp8 ? 0 : few_scale_words(m.format, m.group, m.k);
     word_step = f == kFewFp8 ? 4 : 4 * m.n;
@@ -347,6 +386,16 @@ template <int F>
 __device__ __forceinline__ void copy_step(uint32_t slot, const FewRows& r, const FewLayout& l, int s) {
   using S = FewShape<F>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if constexpr (by_column(F)) {
+    // eight rows of k, 16 bytes of each; rows beyond the last one are zeros
+    if (!r.there[0]) return;
+    const uint8_t* w = r.w + (int64_t)(s * S::kK) * l.row_bytes;
+    const int left = l.k - s * S::kK - 8 * t;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      copy16(slot + i * 512 + lane * 16, i < left ? w + (int64_t)i * l.row_bytes : r.w, i < left ? 16 : 0);
+    return;
+  }
   const uint8_t* w = r.w + s * 64;
   // What is beyond a row of 4-bit codes stays what it was: any code is finite, and its tokens' values are zeros.
   if (F == kFewFp8 || s * 64 + t * 16 < l.row_bytes) {
@@ -497,15 +546,61 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
   }
 }
 
+// The same for weights by column: a lane has eight features of eight rows of k; two rows side by side make the pairs of k that
+// the instruction wants (rows g and g + 8 of product i are the lane's features 2 i and 2 i + 1).
+template <int F, int NT, int kTerms>
+__device__ __forceinline__ void multiply_columns(float (&acc)[kTiles][NT][4], uint32_t slot, const FewTokens (&x)[NT], int s) {
+  const int lane = threadIdx.x & 31;
+  uint4 v[kTerms][NT];
+  float d[kTiles][NT][4] = {};
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int q = 0; q < kTerms; ++q) v[q][n] = lds16(x[n].at + (s * kTerms + q) * x[n].block);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t r[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 w = lds16(slot + (4 * h + i) * 512 + lane * 16);
+      r[i][0] = w.x; r[i][1] = w.y; r[i][2] = w.z; r[i][3] = w.w;
+    }
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      const uint32_t a0 = __byte_perm(r[0][i], r[1][i], 0x5410), a1 = __byte_perm(r[0][i], r[1][i], 0x7632);
+      const uint32_t a2 = __byte_perm(r[2][i], r[3][i], 0x5410), a3 = __byte_perm(r[2][i], r[3][i], 0x7632);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int q = 0; q < kTerms; ++q) {
+          const uint32_t b0 = h ? v[q][n].z : v[q][n].x, b1 = h ? v[q][n].w : v[q][n].y;
+          if constexpr (F == kFewBf16) mma_bf16(acc[i][n], a0, a1, a2, a3, b0, b1);
+          else mma(d[i][n], a0, a1, a2, a3, b0, b1);
+        }
+    }
+  }
+  if constexpr (F == kFewF16) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float s0 = ldsf(x[n].scale[0] + s * x[n].step), s1 = ldsf(x[n].scale[1] + s * x[n].step);
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf(c & 1 ? s1 : s0, d[i][n][c], acc[i][n][c]);
+    }
+  }
+}
+
 // Takes the step in the slot and fetches the next one into it.
 template <int F, int NT, bool kHalves, typename Next>
 __device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], uint32_t ring, int& slot, int tiles, const FewLayout& l, const FewTokens (&x)[NT], int s, int panel_step, Next next) {
   using S = FewShape<F>;
   const uint32_t scales = ring + S::kDepth * S::kSlot, at = ring + slot * S::kSlot;
   copies_wait<S::kDepth - 1>();
-  if (F != kFewFp8) spread_scales<F>(scales, at, l, s);
+  if (F != kFewFp8 && !by_column(F)) spread_scales<F>(scales, at, l, s);
   __syncwarp();
-  if (tiles > kTiles / 2) multiply_step<F, NT, kTiles, kHalves>(acc, at, scales, x, panel_step);
+  if constexpr (by_column(F)) multiply_columns<F, NT, kHalves ? 1 : FewShape<F>::kTerms>(acc, at, x, panel_step);
+  else if (tiles > kTiles / 2) multiply_step<F, NT, kTiles, kHalves>(acc, at, scales, x, panel_step);
   else multiply_step<F, NT, kTiles / 2, kHalves>(acc, at, scales, x, panel_step);
   __syncwarp();
   next(slot);
@@ -539,6 +634,17 @@ template <int NT> struct RedShape {
     return tile * kTile + ((col >> 3) * 4 + (row >> 3) * 2 + (col & 1)) * 32 + (row & 7) * 4 + ((col & 7) >> 1);
   }
 };
+// Tile and row of the sums of a column of W13's part (gate or up of feature f of the 32), and of output c of the 64.
+template <int F>
+__device__ __forceinline__ int2 sums_of(int f, bool up, bool pairs) {
+  if (!by_column(F)) return make_int2(f >> 3, (f & 7) + (up ? 8 : 0));
+  if (pairs) return make_int2(f & 3, (f >> 2) + (up ? 8 : 0));
+  return make_int2((f & 7) >> 1, (f >> 3) + (up ? 4 : 0) + (f & 1 ? 8 : 0));
+}
+template <int F>
+__device__ __forceinline__ int2 sums_of(int c) {
+  return by_column(F) ? make_int2((c & 7) >> 1, (c >> 3) + (c & 1 ? 8 : 0)) : make_int2(c >> 4, c & 15);
+}
 // A warp's sums to its place.
 template <int NT>
 __device__ __forceinline__ void store_sums(float* red, const float (&acc)[kTiles][NT][4]) {
@@ -576,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
   const FewMatrix& m = p.w13;
   const FewLayout layout(m, F, launch.f16);
   const int steps = (p.hidden + S::kK - 1) / S::kK, per_expert = p.inter / 8;
-  const int most = launch.panel_bytes / (steps * S::kPanelBytes); // rows that the panel holds
+  const int most = launch.panel_bytes / (steps * S::kPanelBytes(1)); // rows that the panel holds
   const bool whole = most >= p.tokens;                            // all tokens
   const int k8 = steps * (S::kK / 8);
   auto scales_after = [&](uint8_t* at, int rows) { return reinterpret_cast<float*>(at + rows * steps * (S::kK * 2)); };
@@ -589,8 +695,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
     if (whole) fill_tokens<F>(panel, scales_after(panel, p.tokens), p.x, p.hidden, (1u << p.tokens) - 1u, k8, launch.f16, warp - 1, kWarps - 1);
   }
   __syncthreads();
-  const uint32_t all = (uint32_t)(table.active * per_expert);     // (times the blocks below 2^32: takes_nk)
-  const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+  // (by column: blocks begin and end at whole 32-byte sectors, at whole tiles where there are enough)
+  const uint32_t unit = !by_column(F) || per_expert % 2 ? 1 : per_expert % 4 || table.active * per_expert < 16 * gridDim.x ? 2 : 4;
+  const uint32_t all = (uint32_t)(table.active * per_expert) / unit;     // (times the blocks below 2^32: takes_mma)
+  const int begin = (int)(all * blockIdx.x / gridDim.x * unit), end = (int)(all * (blockIdx.x + 1) / gridDim.x * unit);
   const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
 
 #pragma unroll 1
@@ -615,8 +723,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
     // steps) 90.5 / 87.0 / 89.1 / 92.7; 53 (fp8, 32 steps) 102 / 99.7 / 100 / 108; 22 (fp8, 112 steps) 151 / 136 / 125 / 126; 14
     // (the same) 105 / 84 / 76 / 73; 10 (MXFP4) 31.4 / 29.1 / 29.8 / 29.3.
     const int shift = to - from >= 40 ? 1 : to - from >= 18 ? 2 : 3;
-    const int group = 1 << shift, mine_of = warp >> shift, member = warp & (group - 1);
-    const int my_from = from + (((to - from) * mine_of << shift) / kWarps), my_to = from + (((to - from) * (mine_of + 1) << shift) / kWarps);
+    const int group = 1 << shift, mine_of = warp >> shift, member = warp & (group - 1), units = (to - from) / (int)unit;
+    const int my_from = from + ((units * mine_of << shift) / kWarps) * (int)unit, my_to = from + ((units * (mine_of + 1) << shift) / kWarps) * (int)unit;
 
 #pragma unroll 1
     for (uint32_t rest = tokens; rest;) {
@@ -643,6 +751,13 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
           const int e = table.expert[next_a], f = next_u * 8, rb = layout.row_bytes;
           found = true;
           fetch.tiles = min(kTiles, min(per_expert - next_u, my_to - next));
+          if constexpr (by_column(F)) {
+            // gates in the first half of the 64 columns, ups in the second; pairs as they are
+            const int col = pairs ? 2 * f + 8 * g : g < 4 ? f + 8 * g : p.inter + f + 8 * (g - 4);
+            fetch.there[0] = pairs ? g < 2 * fetch.tiles : (g & 3) < fetch.tiles;
+            fetch.w = reinterpret_cast<const uint8_t*>(m.w) + ((int64_t)e * m.k + 8 * t) * rb + col * 2;
+            continue;
+          }
           fetch.w = reinterpret_cast<const uint8_t*>(m.w) + (int64_t)(e * m.n + (pairs ? 2 * (f + g) : f + g)) * rb + t * 16;
           const int64_t other = pairs ? rb : (int64_t)p.inter * rb;
 #pragma unroll
@@ -689,6 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         if (group > 1) group_sync(1 + mine_of, group * 32);
         else __syncwarp();
         const int i = lane >> 3, f = (u + i) * 8 + (lane & 7);
+        const int2 at_gate = sums_of<F>(lane, false, pairs), at_up = sums_of<F>(lane, true, pairs);
         int turn = tile;
         for (uint32_t left = mine; left; left &= left - 1, ++turn) {
           if ((turn & (group - 1)) != member) continue;
@@ -697,8 +813,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
             const float* from_red = sums + (warp - member) * RedShape<NT>::kWarpFloats;
             float gate = 0.f, up = 0.f;
             for (int w = 0; w < group; ++w) {
-              gate += from_red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(i, lane & 7, col)];
-              up += from_red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(i, 8 + (lane & 7), col)];
+              gate += from_red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(at_gate.x, at_gate.y, col)];
+              up += from_red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(at_up.x, at_up.y, col)];
             }
             if (m.bias) {
               const int64_t at = (int64_t)table.expert[a] * m.n;
@@ -764,11 +880,13 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   const FewLayout layout(m, F, launch.f16);
   const int steps = (p.inter + S::kK - 1) / S::kK;
   const int columns = gridDim.x / launch.splits, column = blockIdx.x % columns, split = blockIdx.x / columns;
-  const int row_begin = (int)((uint32_t)p.hidden * column / columns), row_end = (int)((uint32_t)p.hidden * (column + 1) / columns);
+  // (by column: whole 64 of them, one block's 64 after the other's)
+  const int row_begin = by_column(F) ? column * kRows : (int)((uint32_t)p.hidden * column / columns);
+  const int row_end = by_column(F) ? p.hidden : (int)((uint32_t)p.hidden * (column + 1) / columns);
   const uint32_t total = (uint32_t)(table.active * steps);
   const int step_begin = (int)(total * split / launch.splits), step_end = (int)(total * (split + 1) / launch.splits);
-  const int room = launch.panel_bytes / S::kPanelBytes;                   // rows times steps that the panel holds
-  float* const scales = reinterpret_cast<float*>(panel + room * (S::kK * 2));
+  const int room = launch.panel_bytes / S::kPanelBytes(S::kTerms);        // rows times steps that the panel holds
+  float* const scales = reinterpret_cast<float*>(panel + room * (S::kTerms * S::kK * 2));
   bool waited = false;
 
   // How far a panel reaches that begins with step s0 of expert a0: whole experts, then as many steps of the next one as
@@ -799,7 +917,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
     if (launch.f16) reinterpret_cast<__half*>(p.out)[to] = __float2half_rn(v);
     else reinterpret_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(v);
   };
-  for (int r0 = row_begin; r0 < row_end || !waited; r0 += kRows) {
+  for (int r0 = row_begin; r0 < row_end || !waited; r0 += by_column(F) ? columns * kRows : kRows) {
     const int rows_here = max(0, min(kRows, row_end - r0)), tiles = (rows_here + 15) / 16;
     FewRows fetch;
     fetch.tiles = tiles;
@@ -807,7 +925,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
     for (int i = 0; i < 2 * kTiles; ++i)
       fetch.to[i] = (int64_t)max(0, min(8 * i + g, rows_here - 1)) * layout.row_bytes;   // (what a tile has not got is the last row again)
 #pragma unroll
-    for (int j = 0; j < kRows / 32; ++j) fetch.there[j] = j * 32 + lane < rows_here;
+    for (int j = 0; j < kRows / 32; ++j) fetch.there[j] = by_column(F) ? 8 * g < rows_here : j * 32 + lane < rows_here;
     // The step that is fetched next, how many are left of this warp's stretch, and where the panel after that begins.
     int fetch_a = 0, fetch_s = 0, left = 0, panel_a = step_begin / steps, panel_s = step_begin - panel_a * steps;
     bool found = false;
@@ -827,9 +945,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
         if (fetch_s == steps) { fetch_s = 0; ++fetch_a; found = false; }
         if (!found) {
           const int e = table.expert[fetch_a];
-          fetch.w = reinterpret_cast<const uint8_t*>(m.w) + (int64_t)(e * m.n + r0) * layout.row_bytes + t * 16;
+          fetch.w = by_column(F) ? reinterpret_cast<const uint8_t*>(m.w) + ((int64_t)e * m.k + 8 * t) * layout.row_bytes + (r0 + 8 * g) * 2
+                                 : reinterpret_cast<const uint8_t*>(m.w) + (int64_t)(e * m.n + r0) * layout.row_bytes + t * 16;
 #pragma unroll
-          for (int j = 0; j < kRows / 32; ++j) fetch.s[j] = scales_of<F>(m, layout, e, fetch.there[j] ? r0 + j * 32 + lane : r0);
+          for (int j = 0; j < kRows / 32; ++j)
+            if (!by_column(F)) fetch.s[j] = scales_of<F>(m, layout, e, fetch.there[j] ? r0 + j * 32 + lane : r0);
           found = true;
         }
         copy_step<F>(ring + slot * S::kSlot, fetch, layout, fetch_s);
@@ -869,7 +989,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
           const int r = row0 + row, a = table.row_expert[r], e0 = table.first_row[a], n = table.first_row[a + 1] - e0;
           const int k8_0 = (a == a0 ? s0 : 0) * kPiece, len = (a == a1 ? s1 : steps) * kPiece - k8_0;
           const int before = a == a0 ? 0 : n0 * (steps - s0) + (e0 - row0 - n0) * steps;   // rows times steps of earlier experts
-          fill_row<F, true>(panel + before * (S::kK * 2), scales + before, p.h + (int64_t)r * p.inter + 8 * k8_0, p.inter - 8 * k8_0, len,
+          fill_row<F, true>(panel + before * (S::kTerms * S::kK * 2), scales + before, p.h + (int64_t)r * p.inter + 8 * k8_0, p.inter - 8 * k8_0, len,
                             r - e0, n, warp % parts, parts, false);
         }
         __syncthreads();
@@ -882,7 +1002,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
           const int row = table.first_row[a], n_rows = table.first_row[a + 1] - row, end = min(stop, (a + 1) * steps);
           // rows of earlier experts in the panel, as above
           const int before = a == a0 ? 0 : (table.first_row[a0 + 1] - row0) * (steps - s0) + (row - table.first_row[a0 + 1]) * steps;
-          const uint32_t base = smem_at(panel) + (before - (a == a0 ? s0 : 0) * n_rows) * (S::kK * 2);
+          const uint32_t base = smem_at(panel) + (before - (a == a0 ? s0 : 0) * n_rows) * (S::kTerms * S::kK * 2);
           const uint32_t base_scales = smem_at(scales) + (before - (a == a0 ? s0 : 0) * n_rows) * 4;
           const uint32_t mine = table.tokens[a];
           FewTokens x[NT];
@@ -920,7 +1040,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       if (row >= rows_here || token >= p.tokens) continue;
       float v = bias[i];
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(row >> 4, row & 15, token)];
+      for (int w = 0; w < kWarps; ++w) v += red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(sums_of<F>(row).x, sums_of<F>(row).y, token)];
       const int64_t to = (int64_t)token * p.hidden + r0 + row;
       if (launch.splits == 1) finish(v, token, r0 + row);
       else launch.part[(int64_t)split * p.tokens * p.hidden + to] = v;
@@ -934,7 +1054,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   __syncthreads();
   if (!last_one) return;
   __threadfence();
-  const int width = row_end - row_begin;
+  const int width = min(row_end - row_begin, by_column(F) ? kRows : row_end);
   for (int j = tid; j < width * p.tokens; j += kThreads) {
     const int row = row_begin + j % width, token = j / width;
     float v = 0.f;

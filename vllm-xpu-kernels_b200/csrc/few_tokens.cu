@@ -118,6 +118,8 @@ int launch_block_per_sm(const char* name, int grid, int smem, cudaStream_t st, c
   return B200MOE_OK;
 }
 
+constexpr int kMaxSide = 4;      // warps side by side in the second kernel
+
 // Where things are in the workspace: h, then what the blocks of the two kernels tell one another.
 struct FewWorkspace {
   size_t arrived, part, bytes;
@@ -127,9 +129,9 @@ struct FewWorkspace {
     part = arrived + kFewMaxColumns * sizeof(uint32_t);
     bytes = part + up((size_t)splits(hidden, kFewMaxBlocks) * tokens * hidden * sizeof(float));
   }
-  // Shares of the second kernel's steps: as many as make `ctas` blocks with up to 64 rows each.
-  static int splits(int64_t hidden, int ctas) {
-    const int64_t n = (int64_t)ctas * kRows / hidden;
+  // Shares of the second kernel's steps: as many as make `ctas` blocks with up to `rows` rows each.
+  static int splits(int64_t hidden, int ctas, int rows = kMaxSide * kRows) {
+    const int64_t n = (int64_t)ctas * rows / hidden;
     return n < 1 ? 1 : n > ctas ? ctas : (int)n;
   }
 };
@@ -140,12 +142,13 @@ int launch_mma(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   const int up_row = (p.hidden + k - 1) / k * FewShape<F>::kPanelBytes(1);
   const int down_row = (p.inter + k - 1) / k * FewShape<F>::kPanelBytes(FewShape<F>::kTerms);
   l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
-  int columns = (p.hidden + kRows - 1) / kRows;
+  l.side = p.hidden > 2 * kRows ? 4 : p.hidden > kRows ? 2 : 1;
+  int columns = (p.hidden + l.side * kRows - 1) / (l.side * kRows);
   if (by_column(F)) {
     if (columns > ctas) columns = ctas;
     l.splits = ctas / columns;
   } else {
-    l.splits = FewWorkspace::splits(p.hidden, ctas);
+    l.splits = FewWorkspace::splits(p.hidden, ctas, kRows);
     columns = ctas / l.splits;
   }
   int rc = launch_block_per_sm<few_up_kernel<F, NT>>("few_up_kernel", ctas, UpShape<F, NT>::kFixed + l.panel_bytes, st, p, l);

@@ -618,7 +618,8 @@ __device__ __forceinline__ float load16(const void* p, int64_t i, bool f16) {
 struct FewLaunch {
   int panel_bytes;       // of shared memory for the panel
   bool f16;
-  int splits;            // of the second kernel's steps: it has hidden / splits columns of blocks
+  int splits;            // shares of the second kernel's steps: blocks / splits have the same rows
+  int side;              // by column: warps side by side in the second kernel (1, 2, 4)
   uint32_t* arrived;     // per column of blocks of the second kernel
   float* part;           // [splits][tokens][hidden]: partial sums, with more than one split
 };
@@ -724,7 +725,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
     // (the same) 105 / 84 / 76 / 73; 10 (MXFP4) 31.4 / 29.1 / 29.8 / 29.3.
     const int shift = to - from >= 40 ? 1 : to - from >= 18 ? 2 : 3;
     const int group = 1 << shift, mine_of = warp >> shift, member = warp & (group - 1), units = (to - from) / (int)unit;
-    const int my_from = from + ((units * mine_of << shift) / kWarps) * (int)unit, my_to = from + ((units * (mine_of + 1) << shift) / kWarps) * (int)unit;
+    // Groups have a stretch of the pieces each; by column neighbouring tiles, so that a row of k is read in long runs: what
+    // they take together is `wide` pieces, of which the group's begin with `skip`.
+    const int my_from = by_column(F) ? from : from + ((units * mine_of << shift) / kWarps) * (int)unit;
+    const int my_to = by_column(F) ? to : from + ((units * (mine_of + 1) << shift) / kWarps) * (int)unit;
+    const int wide = by_column(F) ? kWarps / group * kTiles : kTiles, skip = by_column(F) ? mine_of * kTiles : 0;
 
 #pragma unroll 1
     for (uint32_t rest = tokens; rest;) {
@@ -732,8 +737,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       while (__popc(now) > most) now &= ~(1u << (31 - __clz(now)));
       rest &= ~now;
 
-      // The ring begins to fill.  Of the step that is fetched next: its tiles' first piece (of all, and within its expert),
-      // the expert, and whether its rows have been found.
+      // The ring begins to fill.  Of the step that is fetched next: the first piece of its `wide` (of all, and within its
+      // expert), the expert, and whether its rows have been found.
       int next = my_from, next_a = my_from / per_expert, next_u = my_from - next_a * per_expert, s = member;
       int a = next_a, u = next_u;
       bool found = false;
@@ -743,14 +748,22 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         while (next < my_to && (s >= steps || !found)) {
           if (found) {
             s -= steps;
-            next += fetch.tiles;
-            next_u += fetch.tiles;
+            const int n = min(wide, min(per_expert - next_u, my_to - next));
+            next += n;
+            next_u += n;
             if (next_u == per_expert) { next_u = 0; ++next_a; }
             if (next >= my_to) break;
           }
-          const int e = table.expert[next_a], f = next_u * 8, rb = layout.row_bytes;
-          found = true;
-          fetch.tiles = min(kTiles, min(per_expert - next_u, my_to - next));
+          fetch.tiles = min(kTiles, min(wide, min(per_expert - next_u, my_to - next)) - skip);
+          found = fetch.tiles > 0;
+          if (!found) {      // (nothing for this group)
+            const int n = min(wide, min(per_expert - next_u, my_to - next));
+            next += n;
+            next_u += n;
+            if (next_u == per_expert) { next_u = 0; ++next_a; }
+            continue;
+          }
+          const int e = table.expert[next_a], f = (next_u + skip) * 8, rb = layout.row_bytes;
           if constexpr (by_column(F)) {
             // gates in the first half of the 64 columns, ups in the second; pairs as they are
             const int col = pairs ? 2 * f + 8 * g : g < 4 ? f + 8 * g : p.inter + f + 8 * (g - 4);
@@ -790,7 +803,13 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       int slot = 0, cs = member, tile = 0;
 #pragma unroll 1
       for (int first = my_from; first < my_to;) {
-        const int tiles = min(kTiles, min(per_expert - u, my_to - first));
+        const int step_on = min(wide, min(per_expert - u, my_to - first)), tiles = min(kTiles, step_on - skip);
+        if (tiles <= 0) {
+          first += step_on;
+          u += step_on;
+          if (u == per_expert) { u = 0; ++a; }
+          continue;
+        }
         const uint32_t mine = table.tokens[a] & now;
         FewTokens x[NT];
         find_tokens<NT>(x, mine, now, smem_at(panel), smem_at(scales_after(panel, rows)), smem_at(zeros), rows);
@@ -803,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         store_sums<NT>(sums, acc);
         if (group > 1) group_sync(1 + mine_of, group * 32);
         else __syncwarp();
-        const int i = lane >> 3, f = (u + i) * 8 + (lane & 7);
+        const int i = lane >> 3, f = (u + skip + i) * 8 + (lane & 7);
         const int2 at_gate = sums_of<F>(lane, false, pairs), at_up = sums_of<F>(lane, true, pairs);
         int turn = tile;
         for (uint32_t left = mine; left; left &= left - 1, ++turn) {
@@ -828,8 +847,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         if (RedShape<NT>::kBuffers == 1 && group > 1) group_sync(1 + mine_of, group * 32);
         else __syncwarp();
         ++tile;
-        first += tiles;
-        u += tiles;
+        first += step_on;
+        u += step_on;
         if (u == per_expert) { u = 0; ++a; }
       }
       copies_wait<0>();
@@ -860,7 +879,8 @@ __device__ __noinline__ float weighted_bias(const FewTable& table, const FewMatr
 // out = sum over experts of weight * (W2 h + b2).  A block has some rows of W2 and a share of the steps over all active
 // experts: of rows up to 64, so that few blocks need the same values of h, and of steps what makes as many blocks as there are
 // SMs.  It goes through its steps with as many of h's values at a time as its panel holds, each warp with a stretch of them.
-// Of the blocks with the same rows the last one to be done adds the partial sums up, in their order.
+// Of the blocks with the same rows the last one to be done adds the partial sums up, in their order.  By column a block has
+// up to four times 64, side by side by warps that share their steps' values of h.
 template <int F, int NT>
 __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewLaunch launch) {
   using S = FewShape<F>;
@@ -880,8 +900,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   const FewLayout layout(m, F, launch.f16);
   const int steps = (p.inter + S::kK - 1) / S::kK;
   const int columns = gridDim.x / launch.splits, column = blockIdx.x % columns, split = blockIdx.x / columns;
-  // (by column: whole 64 of them, one block's 64 after the other's)
-  const int row_begin = by_column(F) ? column * kRows : (int)((uint32_t)p.hidden * column / columns);
+  // (by column: whole 64 of them, one block's after the other's)
+  const int side = by_column(F) ? launch.side : 1, members = kWarps / side, member = warp / side, mine_side = warp % side;
+  const int block_rows = side * kRows;
+  const int row_begin = by_column(F) ? column * block_rows : (int)((uint32_t)p.hidden * column / columns);
   const int row_end = by_column(F) ? p.hidden : (int)((uint32_t)p.hidden * (column + 1) / columns);
   const uint32_t total = (uint32_t)(table.active * steps);
   const int step_begin = (int)(total * split / launch.splits), step_end = (int)(total * (split + 1) / launch.splits);
@@ -917,8 +939,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
     if (launch.f16) reinterpret_cast<__half*>(p.out)[to] = __float2half_rn(v);
     else reinterpret_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(v);
   };
-  for (int r0 = row_begin; r0 < row_end || !waited; r0 += by_column(F) ? columns * kRows : kRows) {
-    const int rows_here = max(0, min(kRows, row_end - r0)), tiles = (rows_here + 15) / 16;
+  for (int block_r0 = row_begin; block_r0 < row_end || !waited; block_r0 += by_column(F) ? columns * block_rows : kRows) {
+    const int r0 = block_r0 + mine_side * kRows, rows_here = max(0, min(kRows, row_end - r0)), tiles = (rows_here + 15) / 16;
     FewRows fetch;
     fetch.tiles = tiles;
 #pragma unroll
@@ -933,8 +955,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       while (left == 0 && panel_a * steps + panel_s < step_end) {
         int a1, s1;
         panel_end(panel_a, panel_s, a1, s1);
-        const int from = panel_a * steps + panel_s, all = a1 * steps + s1 - from, mine = all * warp / kWarps;
-        left = all * (warp + 1) / kWarps - mine;
+        const int from = panel_a * steps + panel_s, all = a1 * steps + s1 - from, mine = all * member / members;
+        left = all * (member + 1) / members - mine;
         fetch_a = (from + mine) / steps;
         fetch_s = from + mine - fetch_a * steps;
         panel_a = a1;
@@ -960,13 +982,13 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
     };
 #pragma unroll 1
     for (int i = 0; i < S::kDepth; ++i) copy_next(i);
-    // Biases while the ring fills, by the blocks with the first share.
+    // Biases while the ring fills, by the blocks with the first share (by column: when they are needed).
     constexpr int kMine = kRows * B200MOE_FEW_TOKENS / kThreads;
     float bias[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int row = tid % kRows, token = tid / kRows + i * (kThreads / kRows);
-      bias[i] = m.bias && split == 0 && token < p.tokens && row < rows_here ? weighted_bias(table, m, p.topk, launch.f16, token, r0 + row) : 0.f;
+      bias[i] = !by_column(F) && m.bias && split == 0 && token < p.tokens && row < rows_here ? weighted_bias(table, m, p.topk, launch.f16, token, r0 + row) : 0.f;
     }
     if (!waited) {
       pdl_wait();
@@ -996,8 +1018,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       }
       {
         const int from = a0 * steps + s0, all = a1 * steps + s1 - from;
-        int pos = from + all * warp / kWarps;
-        const int stop = rows_here > 0 ? from + all * (warp + 1) / kWarps : 0;
+        int pos = from + all * member / members;
+        const int stop = rows_here > 0 ? from + all * (member + 1) / members : 0;
         for (int a = pos / steps; pos < stop; ++a) {
           const int row = table.first_row[a], n_rows = table.first_row[a + 1] - row, end = min(stop, (a + 1) * steps);
           // rows of earlier experts in the panel, as above
@@ -1033,28 +1055,44 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
     store_sums<NT>(red, out);
     copies_wait<0>();
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      // consecutive threads, consecutive features of a token
-      const int row = tid % kRows, token = tid / kRows + i * (kThreads / kRows);
-      if (row >= rows_here || token >= p.tokens) continue;
-      float v = bias[i];
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(sums_of<F>(row).x, sums_of<F>(row).y, token)];
-      const int64_t to = (int64_t)token * p.hidden + r0 + row;
-      if (launch.splits == 1) finish(v, token, r0 + row);
+    auto put = [&](float v, int token, int row) {
+      const int64_t to = (int64_t)token * p.hidden + row;
+      if (launch.splits == 1) finish(v, token, row);
       else launch.part[(int64_t)split * p.tokens * p.hidden + to] = v;
+    };
+    // consecutive threads, consecutive features of a token
+    if constexpr (by_column(F)) {
+      for (int j = tid; j < block_rows * p.tokens; j += kThreads) {
+        const int row = j % block_rows, token = j / block_rows;
+        if (block_r0 + row >= row_end) continue;
+        const int2 at = sums_of<F>(row % kRows);
+        float v = m.bias && split == 0 ? weighted_bias(table, m, p.topk, launch.f16, token, block_r0 + row) : 0.f;
+        for (int w = row / kRows; w < kWarps; w += side) v += red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(at.x, at.y, token)];
+        put(v, token, block_r0 + row);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int row = tid % kRows, token = tid / kRows + i * (kThreads / kRows);
+        if (row >= rows_here || token >= p.tokens) continue;
+        float v = bias[i];
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) v += red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(sums_of<F>(row).x, sums_of<F>(row).y, token)];
+        put(v, token, r0 + row);
+      }
     }
     __syncthreads();
   }
   if (launch.splits == 1) return;
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) last_one = atomicAdd(&launch.arrived[column], 1u) == (uint32_t)launch.splits - 1;
+  // (the barrier puts the block's partial sums ahead of the fence, and what the others have published ahead of the reads)
+  if (tid == 0) {
+    __threadfence();
+    last_one = atomicAdd(&launch.arrived[column], 1u) == (uint32_t)launch.splits - 1;
+    __threadfence();
+  }
   __syncthreads();
   if (!last_one) return;
-  __threadfence();
-  const int width = min(row_end - row_begin, by_column(F) ? kRows : row_end);
+  const int width = min(row_end - row_begin, by_column(F) ? block_rows : row_end);
   for (int j = tid; j < width * p.tokens; j += kThreads) {
     const int row = row_begin + j % width, token = j / width;
     float v = 0.f;

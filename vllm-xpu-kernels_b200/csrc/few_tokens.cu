@@ -118,7 +118,7 @@ int launch_block_per_sm(const char* name, int grid, int smem, cudaStream_t st, c
   return B200MOE_OK;
 }
 
-constexpr int kMaxSide = 4;      // warps side by side in the second kernel
+constexpr int kMaxSide = 8;      // warps side by side in the second kernel
 
 // Where things are in the workspace: h, then what the blocks of the two kernels tell one another.
 struct FewWorkspace {

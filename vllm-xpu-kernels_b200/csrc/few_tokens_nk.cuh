@@ -624,6 +624,14 @@ struct FewLaunch {
   float* part;           // [splits][tokens][hidden]: partial sums, with more than one split
 };
 
+// The tiles that the warps of a block take together: where they are among the pieces, and a warp's part.
+struct FewPlace {
+  int at, a, u;           // the first piece: of all, its expert (of the active ones), and within that
+  int pieces;             // that the block's warps take together (by column) or the group takes (else)
+  int shift, member;      // log2 of the warps of a group, and which one this is
+  int skip, tiles;        // the group's pieces: where they begin, how many (none: 0 or less)
+};
+
 constexpr int kTableBytes = (sizeof(FewTable) + 127) / 128 * 128;
 // Sums of the warps, for their owner to add up.
 template <int NT> struct RedShape {
@@ -724,12 +732,34 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
     // steps) 90.5 / 87.0 / 89.1 / 92.7; 53 (fp8, 32 steps) 102 / 99.7 / 100 / 108; 22 (fp8, 112 steps) 151 / 136 / 125 / 126; 14
     // (the same) 105 / 84 / 76 / 73; 10 (MXFP4) 31.4 / 29.1 / 29.8 / 29.3.
     const int shift = to - from >= 40 ? 1 : to - from >= 18 ? 2 : 3;
-    const int group = 1 << shift, mine_of = warp >> shift, member = warp & (group - 1), units = (to - from) / (int)unit;
-    // Groups have a stretch of the pieces each; by column neighbouring tiles, so that a row of k is read in long runs: what
-    // they take together is `wide` pieces, of which the group's begin with `skip`.
-    const int my_from = by_column(F) ? from : from + ((units * mine_of << shift) / kWarps) * (int)unit;
-    const int my_to = by_column(F) ? to : from + ((units * (mine_of + 1) << shift) / kWarps) * (int)unit;
-    const int wide = by_column(F) ? kWarps / group * kTiles : kTiles, skip = by_column(F) ? mine_of * kTiles : 0;
+    // Groups have a stretch of the pieces each.  By column all warps work side by side instead, so that rows of k are read in
+    // long runs, and where fewer pieces are left than warps times tiles several have the same ones.
+    const int my_from = by_column(F) ? from : from + (((to - from) * (warp >> shift) << shift) / kWarps);
+    const int my_to = by_column(F) ? to : from + (((to - from) * ((warp >> shift) + 1) << shift) / kWarps);
+    auto place = [&](FewPlace& at) {
+      const int left = min(per_expert - at.u, my_to - at.at);
+      at.shift = shift;
+      at.skip = 0;
+      at.pieces = min(kTiles, left);
+      if constexpr (by_column(F)) {
+        at.shift = left > 4 * kTiles ? 0 : left > 2 * kTiles ? 1 : left > kTiles ? 2 : 3;
+        at.pieces = min(kWarps * kTiles, left);
+        at.skip = (warp >> at.shift) * kTiles;
+      }
+      at.member = warp & ((1 << at.shift) - 1);
+      at.tiles = min(kTiles, at.pieces - at.skip);
+    };
+    auto place_after = [&](FewPlace& at) {
+      at.at += at.pieces;
+      at.u += at.pieces;
+      if (at.u == per_expert) { at.u = 0; ++at.a; }
+      if (at.at < my_to) place(at);
+    };
+    FewPlace start;
+    start.at = my_from;
+    start.a = my_from / per_expert;
+    start.u = my_from - start.a * per_expert;
+    if (my_from < my_to) place(start);
 
 #pragma unroll 1
     for (uint32_t rest = tokens; rest;) {
@@ -737,33 +767,23 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       while (__popc(now) > most) now &= ~(1u << (31 - __clz(now)));
       rest &= ~now;
 
-      // The ring begins to fill.  Of the step that is fetched next: the first piece of its `wide` (of all, and within its
-      // expert), the expert, and whether its rows have been found.
-      int next = my_from, next_a = my_from / per_expert, next_u = my_from - next_a * per_expert, s = member;
-      int a = next_a, u = next_u;
+      // The ring begins to fill.  The step that is fetched next, and whether its rows have been found.
+      FewPlace next = start;
+      int s = start.member;
       bool found = false;
       FewRows fetch;
-      fetch.tiles = 0;
       auto copy_next = [&](int slot) {
-        while (next < my_to && (s >= steps || !found)) {
-          if (found) {
-            s -= steps;
-            const int n = min(wide, min(per_expert - next_u, my_to - next));
-            next += n;
-            next_u += n;
-            if (next_u == per_expert) { next_u = 0; ++next_a; }
-            if (next >= my_to) break;
+        while (next.at < my_to && (s >= steps || !found)) {
+          if (found || next.tiles <= 0) {     // (without tiles for this group: on to the next ones)
+            s -= found ? steps : 0;
+            place_after(next);
+            if (by_column(F)) s = next.member;
+            found = false;
+            if (next.at >= my_to || next.tiles <= 0) continue;
           }
-          fetch.tiles = min(kTiles, min(wide, min(per_expert - next_u, my_to - next)) - skip);
-          found = fetch.tiles > 0;
-          if (!found) {      // (nothing for this group)
-            const int n = min(wide, min(per_expert - next_u, my_to - next));
-            next += n;
-            next_u += n;
-            if (next_u == per_expert) { next_u = 0; ++next_a; }
-            continue;
-          }
-          const int e = table.expert[next_a], f = (next_u + skip) * 8, rb = layout.row_bytes;
+          found = true;
+          fetch.tiles = next.tiles;
+          const int e = table.expert[next.a], f = (next.u + next.skip) * 8, rb = layout.row_bytes;
           if constexpr (by_column(F)) {
             // gates in the first half of the 64 columns, ups in the second; pairs as they are
             const int col = pairs ? 2 * f + 8 * g : g < 4 ? f + 8 * g : p.inter + f + 8 * (g - 4);
@@ -786,9 +806,9 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
             fetch.s[j] = scales_of<F>(m, layout, e, fetch.there[j] ? (pairs ? 2 * (f + fs) + up : f + fs + up * p.inter) : 0);
           }
         }
-        if (next < my_to) {
+        if (next.at < my_to) {
           copy_step<F>(ring + slot * S::kSlot, fetch, layout, s);
-          s += group;
+          s += 1 << next.shift;
         }
         copies_end();
       };
@@ -800,16 +820,12 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         __syncthreads();
       }
 
-      int slot = 0, cs = member, tile = 0;
+      int slot = 0, cs = start.member, tile = 0;
 #pragma unroll 1
-      for (int first = my_from; first < my_to;) {
-        const int step_on = min(wide, min(per_expert - u, my_to - first)), tiles = min(kTiles, step_on - skip);
-        if (tiles <= 0) {
-          first += step_on;
-          u += step_on;
-          if (u == per_expert) { u = 0; ++a; }
-          continue;
-        }
+      for (FewPlace at = start; at.at < my_to; place_after(at)) {
+        const int tiles = at.tiles, group = 1 << at.shift, a = at.a;
+        if (tiles <= 0) continue;
+        if (by_column(F)) cs = at.member;
         const uint32_t mine = table.tokens[a] & now;
         FewTokens x[NT];
         find_tokens<NT>(x, mine, now, smem_at(panel), smem_at(scales_after(panel, rows)), smem_at(zeros), rows);
@@ -818,18 +834,21 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         for (; cs < steps; cs += group) take_step<F, NT, true>(acc, ring, slot, tiles, layout, x, cs, cs, copy_next);
         cs -= steps;
         // The tile's sums: a lane has a feature, the members take the tokens in turn.
-        float* const sums = red + (RedShape<NT>::kBuffers == 2 && (tile & 1) ? RedShape<NT>::kBytes / 4 : 0);
+        // (by column the warps of a group need not have had the same number of tiles)
+        float* const sums = red + (RedShape<NT>::kBuffers == 2 && !by_column(F) && (tile & 1) ? RedShape<NT>::kBytes / 4 : 0);
         store_sums<NT>(sums, acc);
-        if (group > 1) group_sync(1 + mine_of, group * 32);
+        // (a barrier for each group of each size)
+        const int barrier = by_column(F) ? (kWarps >> at.shift) + (warp >> at.shift) : 1 + (warp >> at.shift);
+        if (group > 1) group_sync(barrier, group * 32);
         else __syncwarp();
-        const int i = lane >> 3, f = (u + skip + i) * 8 + (lane & 7);
+        const int i = lane >> 3, f = (at.u + at.skip + i) * 8 + (lane & 7);
         const int2 at_gate = sums_of<F>(lane, false, pairs), at_up = sums_of<F>(lane, true, pairs);
-        int turn = tile;
+        int turn = by_column(F) ? 0 : tile;
         for (uint32_t left = mine; left; left &= left - 1, ++turn) {
-          if ((turn & (group - 1)) != member) continue;
+          if ((turn & (group - 1)) != at.member) continue;
           const int col = __ffs(left) - 1, row = table.first_row[a] + rank_below(table.tokens[a], col);
           if (i < tiles) {
-            const float* from_red = sums + (warp - member) * RedShape<NT>::kWarpFloats;
+            const float* from_red = sums + (warp - at.member) * RedShape<NT>::kWarpFloats;
             float gate = 0.f, up = 0.f;
             for (int w = 0; w < group; ++w) {
               gate += from_red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(at_gate.x, at_gate.y, col)];
@@ -844,12 +863,9 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
           }
         }
         // the sums' place is free again: the next tile has another one, and that one's barrier is behind this one's reads
-        if (RedShape<NT>::kBuffers == 1 && group > 1) group_sync(1 + mine_of, group * 32);
+        if ((RedShape<NT>::kBuffers == 1 || by_column(F)) && group > 1) group_sync(barrier, group * 32);
         else __syncwarp();
         ++tile;
-        first += step_on;
-        u += step_on;
-        if (u == per_expert) { u = 0; ++a; }
       }
       copies_wait<0>();
       __syncthreads();   // the panel is free again

@@ -638,6 +638,7 @@ typedef struct {
   float act_alpha, act_limit;
   float clamp_limit;          /* >0: gate = min(gate, L), up = clamp(up, +-L) first    */
   int max_ctas;               /* >0: at most this many CTAs; 0: one per SM            */
+  int32_t* status;            /* as in b200moe_gemm_args                              */
 } b200moe_few_tokens_args;
 int b200moe_few_tokens_scale_words(b200moe_weight_format format, int group_size, int k);
 size_t b200moe_few_tokens_workspace_bytes(int num_tokens, int topk, int hidden, int inter);

@@ -102,19 +102,19 @@ int launch_simple(const FewParams& p, cudaStream_t st) {
 }
 
 // ---- weights by output feature ---------------------------------------------------------
-constexpr int kMaxSmem = 232448;   // of a block
+constexpr int kMaxBlockSmem = 232448;
 
 // The attribute is set once per kernel and device, and always to the most that a block may have, so that calls with
 // different needs do not get into each other's way.
-template <void (*Kern)(FewParams, FewLaunch)>
-int launch_block_per_sm(const char* name, int grid, int smem, cudaStream_t st, const FewParams& p, const FewLaunch& l) {
+template <auto Kern, typename... Maps>
+int launch_block_per_sm(const char* name, int grid, int smem, cudaStream_t st, const FewParams& p, const FewLaunch& l, const Maps&... maps) {
   static std::atomic<bool> done[kMaxDevices];
   const int dev = current_device();
   if (!done[dev].load(std::memory_order_acquire)) {
-    B200_CUDA_OK(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    B200_CUDA_OK(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBlockSmem));
     done[dev].store(true, std::memory_order_release);
   }
-  B200_LAUNCHED(name, launch_pdl(true, Kern, dim3(grid), dim3(kThreads), smem, st, p, l));
+  B200_LAUNCHED(name, launch_pdl(true, Kern, dim3(grid), dim3(kThreads), smem, st, p, l, maps...));
   return B200MOE_OK;
 }
 
@@ -136,9 +136,26 @@ struct FewWorkspace {
   }
 };
 
+// The map of a matrix for loads of `box` rows (by column: columns) of a step.
+template <int F>
+int few_map(CUtensorMap* map, const FewMatrix& m, int experts, int box) {
+  if (by_column(F)) {
+    const cuuint64_t dims[3] = {(cuuint64_t)m.n, (cuuint64_t)m.k, (cuuint64_t)experts};
+    const cuuint64_t strides[2] = {(cuuint64_t)m.n * 2, (cuuint64_t)m.n * m.k * 2};
+    const cuuint32_t boxes[3] = {(cuuint32_t)box, (cuuint32_t)FewShape<F>::kK, 1};
+    return encode_map(map, F == kFewBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, m.w, dims, strides, boxes,
+                      box == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+  }
+  const cuuint64_t row = F == kFewFp8 ? m.k : m.k / 2;
+  const cuuint64_t dims[3] = {row, (cuuint64_t)m.n, (cuuint64_t)experts};
+  const cuuint64_t strides[2] = {row, row * m.n};
+  const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1};
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, m.w, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 template <int F, int NT>
 int launch_mma(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
-  constexpr int k = FewShape<F>::kK, up_room = kMaxSmem - UpShape<F, NT>::kFixed, down_room = kMaxSmem - DownShape<F>::kFixed;
+  constexpr int k = FewShape<F>::kK, up_room = kMaxBlockSmem - UpShape<F, NT>::kFixed, down_room = kMaxBlockSmem - DownShape<F>::kFixed;
   const int up_row = (p.hidden + k - 1) / k * FewShape<F>::kPanelBytes(1);
   const int down_row = (p.inter + k - 1) / k * FewShape<F>::kPanelBytes(FewShape<F>::kTerms);
   l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
@@ -151,12 +168,22 @@ int launch_mma(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
     l.splits = FewWorkspace::splits(p.hidden, ctas, kRows);
     columns = ctas / l.splits;
   }
-  int rc = launch_block_per_sm<few_up_kernel<F, NT>>("few_up_kernel", ctas, UpShape<F, NT>::kFixed + l.panel_bytes, st, p, l);
+  // Loads: rows of 64 bytes (codes) of 32 gates, 32 ups or 64 features in pairs, and of a piece's; by column 32 rows of the
+  // same columns.  In the second kernel the rows that a block has, by column 64.
+  const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
+  l.box = by_column(F) ? kRows : min(kRows, (p.hidden + columns - 1) / columns);
+  CUtensorMap up_map, piece_map, down_map;
+  int rc = few_map<F>(&up_map, p.w13, p.experts, pairs ? 64 : 32);
+  if (rc == B200MOE_OK) rc = by_column(F) ? B200MOE_OK : few_map<F>(&piece_map, p.w13, p.experts, pairs ? 16 : 8);
+  if (rc == B200MOE_OK) rc = few_map<F>(&down_map, p.w2, p.experts, l.box);
+  if (rc != B200MOE_OK) return rc;
+  if (by_column(F)) piece_map = up_map;
+  rc = launch_block_per_sm<few_up_kernel<F, NT>>("few_up_kernel", ctas, UpShape<F, NT>::kFixed + l.panel_bytes, st, p, l, up_map, piece_map);
   if (rc != B200MOE_OK) return rc;
   const int64_t want = (int64_t)p.tokens * p.topk * down_row;
   l.panel_bytes = (int)(want < down_room ? want : down_room);
   if (l.panel_bytes < RedShape<NT>::kBytes) l.panel_bytes = RedShape<NT>::kBytes;
-  return launch_block_per_sm<few_down_kernel<F, NT>>("few_down_kernel", columns * l.splits, DownShape<F>::kFixed + l.panel_bytes, st, p, l);
+  return launch_block_per_sm<few_down_kernel<F, NT>>("few_down_kernel", columns * l.splits, DownShape<F>::kFixed + l.panel_bytes, st, p, l, down_map);
 }
 
 template <int F>
@@ -242,6 +269,7 @@ extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200mo
   if (takes_mma(p)) {
     FewLaunch l = {};
     l.f16 = a->dtype == B200MOE_F16;
+    l.status = a->status;
     const FewWorkspace ws(p.tokens, p.topk, p.hidden, p.inter);
     l.arrived = (uint32_t*)((char*)a->workspace + ws.arrived);
     l.part = (float*)((char*)a->workspace + ws.part);

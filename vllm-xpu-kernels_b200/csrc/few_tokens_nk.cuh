@@ -4,7 +4,7 @@
 //   D[features, tokens] += W[16 features, 16 k] x^T[16 k, 8 tokens]     (mma.sync, fp32 accumulation)
 //
 // A few tokens leave the layer to the bandwidth of its weights: every byte of an active expert passes once, from L2
-// through a warp's own ring in shared memory (cp.async) into the registers that the matrix instruction reads, with one
+// through a warp's own ring in shared memory (TMA) into the registers that the matrix instruction reads, with one
 // conversion to float16 on the way, which holds every code of the three formats exactly.  The sum over k does not mind its order,
 // so a lane's 16 bytes of a row go into the instruction as they come and the tokens are laid out to match.  Scales of weights
 // multiply sums of their group in fp32.  Tokens and activations are float16 with a power of two per 64 or 128 values of a row,
@@ -14,9 +14,9 @@
 // of 128 features leaves most SMs without work at one token.
 #pragma once
 
-#include <cuda_fp4.h>
-
 #include "few_tokens.cuh"
+#include "gemm_tc_common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace b200moe {
 namespace {
@@ -24,6 +24,7 @@ namespace {
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kTiles = 4;        // tiles of 16 rows that a warp takes at once
 constexpr int kRows = 16 * kTiles;
+constexpr int kSlotBytes = kRows * 64;    // of a warp's ring: the weights of a step
 constexpr int kFewMaxBlocks = 160;      // of a kernel (one per SM)
 constexpr int kFewMaxColumns = kFewMaxBlocks;
 constexpr int kMaxSlots = kFewMaxTopk * B200MOE_FEW_TOKENS;   // routed slots of a call
@@ -42,9 +43,11 @@ template <int F> struct FewShape {
   static constexpr int kTerms = by_column(F) ? 2 : 1;            // of h
   static constexpr int kScaleWords = F == kFewInt4Fine ? 2 : 1;  // that hold a row's scales of a step
   static constexpr int kScales = F == kFewFp8 || by_column(F) ? 0 : F == kFewInt4 ? 1 : 4;                       // of a row and step, made fp32 (fp8: are so)
-  static constexpr int kSlot = kRows * (64 + (by_column(F) ? 0 : 4 * kScaleWords));
   static constexpr int kDepth = 3;
-  static constexpr int kRing = kDepth * kSlot + kRows * kScales * 4;
+  static constexpr int kRing = kDepth * kSlotBytes;
+  // behind the rings of all warps, per warp: scales of the steps in the ring as they come, and as fp32
+  static constexpr int kSlotScales = by_column(F) ? 0 : kRows * 4 * kScaleWords;
+  static constexpr int kRingScales = kDepth * kSlotScales + kRows * kScales * 4;
 };
 
 // ---- which experts a call uses ------------------------------------------------------
@@ -141,13 +144,6 @@ __device__ __forceinline__ void build_table(FewTable& t, const FewParams& p) {
 
 // ---- loads ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
-// `bytes` of the 16 come from memory, the rest are zeros.
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
@@ -221,11 +217,11 @@ __device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a
 // ---- tokens and activations as float16 -------------------------------------------------
 // A panel holds rows of values in the order in which the lanes want them: per step blocks of [row][4 lanes][8 values].
 // Where k sits: fp8 lanes hold 16 bytes of a row, 16 values; 4-bit formats hand a group of 32 values out to the four lanes,
-// eight each, and weights by column 32 rows.  Behind them, per row and step, the inverse of what the values have been multiplied by.
+// eight each; weights by column have 32 rows, of which a lane multiplies 2 t, 2 t + 1 and every eighth after these.  Behind them, per row and step, the inverse of what the values have been multiplied by.
 template <int F>
 __device__ __forceinline__ uint32_t panel_at(int k8, int row, int rows, int terms) {   // k8: k / 8; a second term is a block on
   const int block = (F == kFewFp8 ? (k8 >> 3) * 2 + (k8 & 1) : k8 >> 2) * terms;
-  const int t = F == kFewFp8 ? (k8 >> 1) & 3 : k8 & 3;
+  const int t = by_column(F) ? 0 : F == kFewFp8 ? (k8 >> 1) & 3 : k8 & 3;     // (by column: all four, see store8)
   return (uint32_t)(((block * rows + row) * 4 + t) * 16);
 }
 
@@ -255,6 +251,20 @@ __device__ __forceinline__ uint4 packed8(const float (&v)[8]) {
     }
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Eighth j of a row to its place: at the panel's place for it, or by column a word to each of the four lanes.
+template <int F>
+__device__ __forceinline__ void store8(uint8_t* at, int j, const uint4& o) {
+  if constexpr (by_column(F)) {
+    uint32_t* const w = reinterpret_cast<uint32_t*>(at) + (j & 3);
+    w[0] = o.x;
+    w[4] = o.y;
+    w[8] = o.z;
+    w[12] = o.w;
+  } else {
+    *reinterpret_cast<uint4*>(at) = o;
+  }
 }
 
 // `len` eighths of a row (what is beyond `values` values is zero) into a panel, by `parts` warps of which this is `part`.  A warp
@@ -309,7 +319,7 @@ __device__ __noinline__ void fill_row(uint8_t* panel, float* scales, const void*
         constexpr int kTerms = kF32 ? FewShape<F>::kTerms : 1;
         uint8_t* const at = panel + panel_at<F>(j, row, rows, kTerms);
         const uint4 o = packed8<F>(v);
-        *reinterpret_cast<uint4*>(at) = o;
+        store8<F>(at, j, o);
         if constexpr (kTerms == 2) {
           const uint32_t w[4] = {o.x, o.y, o.z, o.w};
           float rest[8];
@@ -321,7 +331,7 @@ __device__ __noinline__ void fill_row(uint8_t* panel, float* scales, const void*
             rest[2 * k] = fabsf(v[2 * k]) < INFINITY ? v[2 * k] - x : 0.f;
             rest[2 * k + 1] = fabsf(v[2 * k + 1]) < INFINITY ? v[2 * k + 1] - y : 0.f;
           }
-          *reinterpret_cast<uint4*>(at + rows * 64) = packed8<F>(rest);
+          store8<F>(at + rows * 64, j, packed8<F>(rest));
         }
         if ((j & (kLanes - 1)) == 0) scales[j / kLanes * rows + row] = inv;
       }
@@ -346,19 +356,28 @@ __device__ __noinline__ void fill_tokens(uint8_t* panel, float* scales, const vo
 }
 
 // ---- weights: a warp's ring ------------------------------------------------------------
-// fp8: a lane reads the bytes that it fetched.  4 bits: a lane fetches 16 bytes of a row, which is a group of 32 values, and
-// reads a word of each of the row's four groups; the groups' places are swapped so that the eight rows of a read fall on
-// different banks.  Scales are fetched as words, neighbouring rows by neighbouring lanes (those of 4-bit formats are laid out
-// for that: as they come, a step's would be 2 or 4 bytes of every row, which kept the load units busy for longer than the
-// weights did), and made fp32 by one lane per row.
+// One lane asks for a step's weights by TMA, whose swizzle puts the 16-byte pieces of a row where the lanes' reads fall on
+// different banks: rows of 64 bytes (a lane reads one of the four pieces, or a word of each: a group of 32 4-bit codes is
+// handed out to four lanes), by column rows of 128 or two halves of 64.  Scales are fetched as words, neighbouring rows
+// by neighbouring lanes (those of 4-bit formats are laid out for that: as they come, a step's would be 2 or 4 bytes of every
+// row, which kept the load units busy for longer than the weights did), and made fp32 by one lane per row.
+// (With every lane fetching its own pieces, MXFP4 took a third more instructions, and every first touch of a page held up
+// the warps: both kernels at one MXFP4 token 28.7 us, 16-bit weights at 16 tokens, whose rows are far apart, 765 us.)
 
-// The lane's part of the rows of one expert's matrix that a warp takes at once.
+// Where the rows of a step lie in a slot, and their scales: rows g and g + 8 of tile i.
+struct FewOrder {
+  int tile, half;             // bytes from one tile to the next, from row g to g + 8
+  int place, place_half;      // the same for places of scales
+};
+__device__ __forceinline__ FewOrder row_order() { return {1024, 512, 16, 8}; }          // 64 rows
+__device__ __forceinline__ FewOrder halves_order() { return {512, 2048, 8, 32}; }       // 32 gates, 32 ups
+
+// What a warp fetches: the rows of one expert's matrix that it takes at once.
 struct FewRows {
-  const uint8_t* w;                       // its 16 bytes of step 0 in row g (lane = 4 g + t); by column: in row 8 t of k
-  int64_t to[2 * kTiles];                 // from there to rows g + 8 i (by column: not used)
-  const uint8_t* s[kRows / 32];           // scales of step 0 of the rows that it looks after, places lane + 32 i
-  bool there[kRows / 32];                 // whether these rows are
+  int e, row;                             // expert, first row (feature)
   int tiles;                              // that there are
+  const uint8_t* s[kRows / 32];           // scales of step 0 of the rows that the lane looks after, places lane + 32 i
+  bool there[kRows / 32];                 // whether these rows are
 };
 // The matrix as a whole.
 struct FewLayout {
@@ -381,32 +400,11 @@ __device__ __forceinline__ const uint8_t* scales_of(const FewMatrix& m, const Fe
   return reinterpret_cast<const uint8_t*>(m.scale) + (int64_t)(e * l.words) * (4 * m.n) + n * 4;
 }
 
-// Fetches step s into a slot.
+// Fetches the scales of step s.
 template <int F>
-__device__ __forceinline__ void copy_step(uint32_t slot, const FewRows& r, const FewLayout& l, int s) {
+__device__ __forceinline__ void copy_scales(uint32_t to, const FewRows& r, const FewLayout& l, int s) {
   using S = FewShape<F>;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  if constexpr (by_column(F)) {
-    // eight rows of k, 16 bytes of each; rows beyond the last one are zeros
-    if (!r.there[0]) return;
-    const uint8_t* w = r.w + (int64_t)(s * S::kK) * l.row_bytes;
-    const int left = l.k - s * S::kK - 8 * t;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      copy16(slot + i * 512 + lane * 16, i < left ? w + (int64_t)i * l.row_bytes : r.w, i < left ? 16 : 0);
-    return;
-  }
-  const uint8_t* w = r.w + s * 64;
-  // What is beyond a row of 4-bit codes stays what it was: any code is finite, and its tokens' values are zeros.
-  if (F == kFewFp8 || s * 64 + t * 16 < l.row_bytes) {
-    const uint32_t to = slot + (F == kFewFp8 ? lane * 16 : g * 64 + ((t ^ (g >> 1)) << 4));
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-      if (i >= r.tiles) break;
-      copy16(to + i * 1024, w + r.to[2 * i]);
-      copy16(to + i * 1024 + 512, w + r.to[2 * i + 1]);
-    }
-  }
+  const int lane = threadIdx.x & 31;
   // (a word serves two steps of fp8, whose blocks are 128 long, and of int4 with one scale of 16 bits per step)
   const bool two = F == kFewInt4Fine && l.group == 32;
   const int word = F == kFewFp8 || F == kFewInt4 ? s >> 1 : two ? 2 * s : s;
@@ -415,18 +413,43 @@ __device__ __forceinline__ void copy_step(uint32_t slot, const FewRows& r, const
     if (!r.there[j]) continue;
 #pragma unroll
     for (int i = 0; i < S::kScaleWords; ++i)
-      if (i == 0 || two) copy4(slot + kRows * 64 + ((j * 32 + lane) * S::kScaleWords + i) * 4, r.s[j] + (int64_t)(word + i) * l.word_step);
+      if (i == 0 || two) copy4(to + ((j * 32 + lane) * S::kScaleWords + i) * 4, r.s[j] + (int64_t)(word + i) * l.word_step);
   }
 }
 
-// The scales of step s, which is in the slot, as fp32.
+// A warp's ring, one slot after the other.
+struct FewRing {
+  uint32_t slots, bars;      // shared addresses: of slot 0, of its barrier
+  uint32_t scales;           // of the scales of slot 0
+  int slot, parity;          // that is taken next
+  volatile int* gave_up;
+  int32_t* status;
+};
+// Waits for a slot; a wait that runs out sets the status word, and the kernel goes on with what is there (later waits, one for
+// every copy in flight, are short then).
+static __device__ __noinline__ void ring_wait_long(uint32_t bar, int parity, volatile int* gave_up, int32_t* status) {
+  const long long budget = *gave_up ? 1000000 : ptx::kWaitBudgetCycles, t0 = clock64();
+  while (!ptx::mbar_try_wait_s(bar, parity)) {
+    if (clock64() - t0 > budget) {
+      *gave_up = 1;
+      if (status) *reinterpret_cast<volatile int32_t*>(status) = 1;
+      return;
+    }
+  }
+}
+__device__ __forceinline__ void ring_wait(const FewRing& r) {
+  const uint32_t bar = r.bars + r.slot * 8;
+  if (!ptx::mbar_try_wait_s(bar, r.parity)) ring_wait_long(bar, r.parity, r.gave_up, r.status);
+}
+
+// The scales of step s as fp32.
 template <int F>
-__device__ __forceinline__ void spread_scales(uint32_t to, uint32_t slot, const FewLayout& l, int s) {
+__device__ __forceinline__ void spread_scales(uint32_t to, uint32_t from, const FewLayout& l, int s) {
   using S = FewShape<F>;
 #pragma unroll
   for (int j = 0; j < kRows / 32; ++j) {
     const int row = j * 32 + (threadIdx.x & 31);
-    const uint32_t at = slot + kRows * 64 + row * S::kScaleWords * 4, v = lds4(at);
+    const uint32_t at = from + row * S::kScaleWords * 4, v = lds4(at);
     auto value = [&](uint32_t h) { return l.f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16); };
     if constexpr (F == kFewFp4) {
       // 2^(byte - 127): the byte is the exponent (0 gives zero for 2^-127, 255 infinity for NaN)
@@ -468,9 +491,9 @@ __device__ __forceinline__ void find_tokens(FewTokens (&x)[NT], uint32_t used, u
 }
 
 // acc += W x of the step in the slot, for the first `Tiles` tiles (what one of them has not got is something finite or not, in
-// rows that nobody reads).  kHalves: scales lie as [8 rows g of all tiles][8 rows g + 8 of all tiles], else row by row.
-template <int F, int NT, int Tiles, bool kHalves>
-__device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint32_t slot, uint32_t scales,
+// rows that nobody reads).
+template <int F, int NT, int Tiles>
+__device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint32_t slot, uint32_t scales, const FewOrder& order,
                                               const FewTokens (&x)[NT], int s) {
   using S = FewShape<F>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -485,7 +508,7 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
   }
 #pragma unroll
   for (int i = 0; i < Tiles; ++i) {
-    const int at_lo = kHalves ? 8 * i + g : 16 * i + g, at_hi = at_lo + (kHalves ? kRows / 2 : 8);   // places of the scales
+    const int at_lo = i * order.place + g, at_hi = at_lo + order.place_half;     // places of the scales
     float d[NT][4], sum[NT][4] = {};   // products of a group of weights, and the step's
     auto add = [&](float a, float b) {
 #pragma unroll
@@ -497,7 +520,8 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
       }
     };
     if constexpr (F == kFewFp8) {
-      const uint4 lo = lds16(slot + i * 1024 + lane * 16), hi = lds16(slot + i * 1024 + 512 + lane * 16);
+      const uint32_t at = slot + i * order.tile + g * 64 + ((t ^ (g >> 1)) << 4);
+      const uint4 lo = lds16(at), hi = lds16(at + order.half);
       const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -511,7 +535,7 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
           else mma(d[n], a0, a1, a2, a3, w & 1 ? b.z : b.x, w & 1 ? b.w : b.y);
         }
       }
-      add(ldsf(slot + kRows * 64 + at_lo * 4), ldsf(slot + kRows * 64 + at_hi * 4));
+      add(ldsf(scales + at_lo * 4), ldsf(scales + at_hi * 4));
     } else {
       uint4 lo, hi;
       if constexpr (S::kScales == 4) {
@@ -521,11 +545,11 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
         lo.w = lds4(scales + at_lo * 4);
         hi.w = lds4(scales + at_hi * 4);
       }
-      const uint32_t w = slot + i * 1024 + g * 64 + t * 4;
+      const uint32_t w = slot + i * order.tile + g * 64 + t * 4;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int at = (q ^ (g >> 1)) << 4;
-        const uint32_t wl = lds4(w + at), wh = lds4(w + at + 512);
+        const uint32_t wl = lds4(w + at), wh = lds4(w + at + order.half);
         uint32_t al[4], ah[4];
         if constexpr (F == kFewFp4) { e2m1x8_to_h2(wl, al); e2m1x8_to_h2(wh, ah); }
         else { s4x8_to_h2(wl, al); s4x8_to_h2(wh, ah); }
@@ -547,22 +571,26 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
 }
 
 // The same for weights by column: a lane has eight features of eight rows of k; two rows side by side make the pairs of k that
-// the instruction wants (rows g and g + 8 of product i are the lane's features 2 i and 2 i + 1).
+// the instruction wants (rows g and g + 8 of product i are the lane's features 2 i and 2 i + 1).  halves: 32 and 32 columns
+// (gates, ups) behind one another, else 64.
 template <int F, int NT, int kTerms>
-__device__ __forceinline__ void multiply_columns(float (&acc)[kTiles][NT][4], uint32_t slot, const FewTokens (&x)[NT], int s) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void multiply_columns(float (&acc)[kTiles][NT][4], uint32_t slot, bool halves, const FewTokens (&x)[NT], int s) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint4 v[kTerms][NT];
   float d[kTiles][NT][4] = {};
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int q = 0; q < kTerms; ++q) v[q][n] = lds16(x[n].at + (s * kTerms + q) * x[n].block);
+  // rows 2 t and 2 t + 1 of eight; the next eight rows are 512 or 1024 bytes on
+  const uint32_t at0 = halves ? slot + (g >> 2) * 2048 + t * 128 + (((g & 3) ^ t) << 4) : slot + t * 256 + ((g ^ (2 * t)) << 4);
+  const uint32_t at1 = halves ? at0 + 64 : slot + t * 256 + 128 + ((g ^ (2 * t + 1)) << 4), next = halves ? 512 : 1024;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t r[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint4 w = lds16(slot + (4 * h + i) * 512 + lane * 16);
+      const uint4 w = lds16((i & 1 ? at1 : at0) + (2 * h + (i >> 1)) * next);
       r[i][0] = w.x; r[i][1] = w.y; r[i][2] = w.z; r[i][3] = w.w;
     }
 #pragma unroll
@@ -591,20 +619,50 @@ __device__ __forceinline__ void multiply_columns(float (&acc)[kTiles][NT][4], ui
   }
 }
 
-// Takes the step in the slot and fetches the next one into it.
-template <int F, int NT, bool kHalves, typename Next>
-__device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], uint32_t ring, int& slot, int tiles, const FewLayout& l, const FewTokens (&x)[NT], int s, int panel_step, Next next) {
+// Takes the step in the ring's slot and fetches the next one into it.
+template <int F, int NT, int kTerms, typename Next>
+__device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], FewRing& ring, int tiles, const FewOrder& order, bool halves, const FewLayout& l,
+                                          const FewTokens (&x)[NT], int s, Next next) {
   using S = FewShape<F>;
-  const uint32_t scales = ring + S::kDepth * S::kSlot, at = ring + slot * S::kSlot;
+  const uint32_t at = ring.slots + ring.slot * kSlotBytes;
+  uint32_t scales = ring.scales + ring.slot * S::kSlotScales;
   copies_wait<S::kDepth - 1>();
-  if (F != kFewFp8 && !by_column(F)) spread_scales<F>(scales, at, l, s);
+  if (!by_column(F) && F != kFewFp8) {
+    const uint32_t to = ring.scales + S::kDepth * S::kSlotScales;
+    spread_scales<F>(to, scales, l, s);
+    scales = to;
+  }
   __syncwarp();
-  if constexpr (by_column(F)) multiply_columns<F, NT, kHalves ? 1 : FewShape<F>::kTerms>(acc, at, x, panel_step);
-  else if (tiles > kTiles / 2) multiply_step<F, NT, kTiles, kHalves>(acc, at, scales, x, panel_step);
-  else multiply_step<F, NT, kTiles / 2, kHalves>(acc, at, scales, x, panel_step);
+  ring_wait(ring);
+  if constexpr (by_column(F)) multiply_columns<F, NT, kTerms>(acc, at, halves, x, s);
+  else if (tiles > kTiles / 2) multiply_step<F, NT, kTiles>(acc, at, scales, order, x, s);
+  else multiply_step<F, NT, kTiles / 2>(acc, at, scales, order, x, s);
   __syncwarp();
-  next(slot);
-  slot = slot + 1 == S::kDepth ? 0 : slot + 1;
+  next(ring.slot);
+  if (++ring.slot == S::kDepth) {
+    ring.slot = 0;
+    ring.parity ^= 1;
+  }
+}
+// Sets a warp's ring up.
+template <int F>
+__device__ __forceinline__ FewRing make_ring(uint8_t* rings, uint8_t* scales, uint64_t* bars, int* gave_up, int32_t* status) {
+  using S = FewShape<F>;
+  const int warp = threadIdx.x >> 5;
+  FewRing r;
+  r.slots = smem_at(rings) + warp * S::kRing;
+  r.scales = smem_at(scales) + warp * S::kRingScales;
+  r.bars = smem_at(bars + warp * S::kDepth);
+  r.slot = r.parity = 0;
+  r.gave_up = gave_up;
+  r.status = status;
+  if ((threadIdx.x & 31) == 0) {
+    for (int i = 0; i < S::kDepth; ++i) ptx::mbar_init(bars + warp * S::kDepth + i, 1);
+    ptx::fence_barrier_init();
+    ptx::fence_proxy_async();
+  }
+  __syncwarp();
+  return r;
 }
 
 __device__ __noinline__ float gated_once(int act, float alpha, float limit, float clamp, float gate, float up) {
@@ -622,6 +680,8 @@ struct FewLaunch {
   int side;              // by column: warps side by side in the second kernel (1, 2, 4)
   uint32_t* arrived;     // per column of blocks of the second kernel
   float* part;           // [splits][tokens][hidden]: partial sums, with more than one split
+  int box;               // rows (by column: columns) that a load of the second kernel brings
+  int32_t* status;       // for waits that run out, or NULL
 };
 
 // The tiles that the warps of a block take together: where they are among the pieces, and a warp's part.
@@ -646,7 +706,7 @@ template <int NT> struct RedShape {
 // Tile and row of the sums of a column of W13's part (gate or up of feature f of the 32), and of output c of the 64.
 template <int F>
 __device__ __forceinline__ int2 sums_of(int f, bool up, bool pairs) {
-  if (!by_column(F)) return make_int2(f >> 3, (f & 7) + (up ? 8 : 0));
+  if (!by_column(F)) return pairs ? make_int2(f >> 3, 2 * (f & 7) + (up ? 1 : 0)) : make_int2(f >> 3, (f & 7) + (up ? 8 : 0));
   if (pairs) return make_int2(f & 3, (f >> 2) + (up ? 8 : 0));
   return make_int2((f & 7) >> 1, (f >> 3) + (up ? 4 : 0) + (f & 1 ? 8 : 0));
 }
@@ -665,27 +725,42 @@ __device__ __forceinline__ void store_sums(float* red, const float (&acc)[kTiles
 #pragma unroll
       for (int c = 0; c < 4; ++c) to[i * RedShape<NT>::kTile + (n * 4 + c) * 32] = acc[i][n][c];
 }
+// Shared memory: the rings, barriers, zeros, flags, the table, scales in the rings, sums, the panel.
+template <int F> struct FewSmem {
+  using S = FewShape<F>;
+  static constexpr int kBars = kWarps * S::kRing, kZeros = kBars + 256, kFlags = kZeros + 64, kTable = kFlags + 64;
+  static constexpr int kScales = kTable + kTableBytes, kRest = (kScales + kWarps * S::kRingScales + 127) / 128 * 128;
+  static_assert(kWarps * S::kDepth * 8 <= 256, "barriers");
+};
 template <int F, int NT> struct UpShape {
   static constexpr int kSums = RedShape<NT>::kBuffers * RedShape<NT>::kBytes;
-  static constexpr int kFixed = kTableBytes + 128 + kSums + kWarps * FewShape<F>::kRing;
+  static constexpr int kFixed = FewSmem<F>::kRest + kSums;
 };
 template <int F> struct DownShape {
-  static constexpr int kFixed = kTableBytes + 128 + kWarps * FewShape<F>::kRing;
+  static constexpr int kFixed = FewSmem<F>::kRest;
 };
 
 // h[row] = act(W13 x + b13).  The features of all active experts, in pieces of eight (a tile's rows: eight gates and their
 // eight ups), are dealt out evenly to the blocks, and within a block to groups of warps; the warps of a group take the
 // steps of its tiles in turn and add their sums up in shared memory.
 template <int F, int NT>
-__global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLaunch launch) {
+__global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLaunch launch, const __grid_constant__ CUtensorMap map,
+                                                           const __grid_constant__ CUtensorMap piece_map) {
   using S = FewShape<F>;
-  extern __shared__ __align__(128) uint8_t smem[];
-  FewTable& table = *reinterpret_cast<FewTable*>(smem);
-  uint8_t* const zeros = smem + kTableBytes;                              // a token's values where there is no token
-  float* const red = reinterpret_cast<float*>(smem + kTableBytes + 128);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_at(smem) + kTableBytes + 128 + UpShape<F, NT>::kSums + warp * S::kRing;
+  using M = FewSmem<F>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  FewTable& table = *reinterpret_cast<FewTable*>(smem + M::kTable);
+  uint8_t* const zeros = smem + M::kZeros;                                // a token's values where there is no token
+  int* const gave_up = reinterpret_cast<int*>(smem + M::kFlags);
+  float* const red = reinterpret_cast<float*>(smem + M::kRest);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  FewRing ring = make_ring<F>(smem, smem + M::kScales, reinterpret_cast<uint64_t*>(smem + M::kBars), gave_up, launch.status);
   uint8_t* const panel = smem + UpShape<F, NT>::kFixed;
+  if (tid == 0) {
+    *gave_up = 0;
+    ptx::prefetch_tensormap(&map);
+    if (!by_column(F)) ptx::prefetch_tensormap(&piece_map);
+  }
   pdl_wait();
   pdl_trigger();
   const FewMatrix& m = p.w13;
@@ -709,6 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
   const uint32_t all = (uint32_t)(table.active * per_expert) / unit;     // (times the blocks below 2^32: takes_mma)
   const int begin = (int)(all * blockIdx.x / gridDim.x * unit), end = (int)(all * (blockIdx.x + 1) / gridDim.x * unit);
   const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
+  const FewOrder order = pairs ? row_order() : halves_order();
 
 #pragma unroll 1
   for (int from = begin; from < end;) {
@@ -783,44 +859,57 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
           }
           found = true;
           fetch.tiles = next.tiles;
-          const int e = table.expert[next.a], f = (next.u + next.skip) * 8, rb = layout.row_bytes;
-          if constexpr (by_column(F)) {
-            // gates in the first half of the 64 columns, ups in the second; pairs as they are
-            const int col = pairs ? 2 * f + 8 * g : g < 4 ? f + 8 * g : p.inter + f + 8 * (g - 4);
-            fetch.there[0] = pairs ? g < 2 * fetch.tiles : (g & 3) < fetch.tiles;
-            fetch.w = reinterpret_cast<const uint8_t*>(m.w) + ((int64_t)e * m.k + 8 * t) * rb + col * 2;
-            continue;
-          }
-          fetch.w = reinterpret_cast<const uint8_t*>(m.w) + (int64_t)(e * m.n + (pairs ? 2 * (f + g) : f + g)) * rb + t * 16;
-          const int64_t other = pairs ? rb : (int64_t)p.inter * rb;
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i) {
-            fetch.to[2 * i] = (int64_t)((pairs ? 16 : 8) * i) * rb;
-            fetch.to[2 * i + 1] = fetch.to[2 * i] + other;
-          }
+          fetch.e = table.expert[next.a];
+          fetch.row = (next.u + next.skip) * 8;
 #pragma unroll
           for (int j = 0; j < kRows / 32; ++j) {
-            // gates in the first half of the places, ups in the second
+            if (by_column(F)) break;
+            // gates in the first half of the places, ups in the second; pairs as they are
             const int place = j * 32 + lane, up = place >= kRows / 2, fs = place % (kRows / 2);
-            fetch.there[j] = fs < 8 * fetch.tiles;
-            fetch.s[j] = scales_of<F>(m, layout, e, fetch.there[j] ? (pairs ? 2 * (f + fs) + up : f + fs + up * p.inter) : 0);
+            fetch.there[j] = pairs ? place < 16 * fetch.tiles : fs < 8 * fetch.tiles;
+            const int n = pairs ? 2 * fetch.row + place : fetch.row + fs + up * p.inter;
+            fetch.s[j] = scales_of<F>(m, layout, fetch.e, fetch.there[j] ? n : 0);
           }
         }
         if (next.at < my_to) {
-          copy_step<F>(ring + slot * S::kSlot, fetch, layout, s);
+          if (lane == 0) {
+            const uint32_t to = ring.slots + slot * kSlotBytes, bar = ring.bars + slot * 8;
+            const int x = by_column(F) ? fetch.row : s * 64, y = by_column(F) ? s * S::kK : fetch.row;
+            ptx::fence_proxy_async();      // (the warp has read what was there)
+            if (by_column(F) || fetch.tiles == kTiles) {
+              ptx::mbar_expect_tx_s(bar, kSlotBytes);
+              if (pairs) {
+                ptx::tma_load_3d_s(to, &map, bar, by_column(F) ? 2 * x : x, by_column(F) ? y : 2 * y, fetch.e);
+              } else {
+                ptx::tma_load_3d_s(to, &map, bar, x, y, fetch.e);
+                ptx::tma_load_3d_s(to + 2048, &map, bar, by_column(F) ? p.inter + x : x, by_column(F) ? y : p.inter + y, fetch.e);
+              }
+            } else {                       // the tiles that there are, one by one
+              ptx::mbar_expect_tx_s(bar, fetch.tiles * 1024);
+              for (int i = 0; i < fetch.tiles; ++i) {
+                if (pairs) {
+                  ptx::tma_load_3d_s(to + i * 1024, &piece_map, bar, x, 2 * (y + 8 * i), fetch.e);
+                } else {
+                  ptx::tma_load_3d_s(to + i * 512, &piece_map, bar, x, y + 8 * i, fetch.e);
+                  ptx::tma_load_3d_s(to + 2048 + i * 512, &piece_map, bar, x, p.inter + y + 8 * i, fetch.e);
+                }
+              }
+            }
+          }
+          if (!by_column(F)) copy_scales<F>(ring.scales + slot * S::kSlotScales, fetch, layout, s);
           s += 1 << next.shift;
         }
         copies_end();
       };
 #pragma unroll 1
-      for (int i = 0; i < S::kDepth; ++i) copy_next(i);
+      for (int i = 0; i < S::kDepth; ++i) copy_next((ring.slot + i) % S::kDepth);
       const int rows = __popc(now);
       if (!whole) {
         fill_tokens<F>(panel, scales_after(panel, rows), p.x, p.hidden, now, k8, launch.f16, warp, kWarps);
         __syncthreads();
       }
 
-      int slot = 0, cs = start.member, tile = 0;
+      int cs = start.member, tile = 0;
 #pragma unroll 1
       for (FewPlace at = start; at.at < my_to; place_after(at)) {
         const int tiles = at.tiles, group = 1 << at.shift, a = at.a;
@@ -831,7 +920,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         find_tokens<NT>(x, mine, now, smem_at(panel), smem_at(scales_after(panel, rows)), smem_at(zeros), rows);
         float acc[kTiles][NT][4] = {};
 #pragma unroll 1
-        for (; cs < steps; cs += group) take_step<F, NT, true>(acc, ring, slot, tiles, layout, x, cs, cs, copy_next);
+        for (; cs < steps; cs += group) take_step<F, NT, 1>(acc, ring, tiles, order, !pairs, layout, x, cs, copy_next);
         cs -= steps;
         // The tile's sums: a lane has a feature, the members take the tokens in turn.
         // (by column the warps of a group need not have had the same number of tiles)
@@ -898,16 +987,22 @@ __device__ __noinline__ float weighted_bias(const FewTable& table, const FewMatr
 // Of the blocks with the same rows the last one to be done adds the partial sums up, in their order.  By column a block has
 // up to four times 64, side by side by warps that share their steps' values of h.
 template <int F, int NT>
-__global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewLaunch launch) {
+__global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewLaunch launch, const __grid_constant__ CUtensorMap map) {
   using S = FewShape<F>;
-  extern __shared__ __align__(128) uint8_t smem[];
-  FewTable& table = *reinterpret_cast<FewTable*>(smem);
-  int& last_one = *reinterpret_cast<int*>(smem + kTableBytes);
-  uint8_t* const zeros = smem + kTableBytes + 64;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_at(smem) + kTableBytes + 128 + warp * S::kRing;
+  using M = FewSmem<F>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  FewTable& table = *reinterpret_cast<FewTable*>(smem + M::kTable);
+  uint8_t* const zeros = smem + M::kZeros;
+  int* const gave_up = reinterpret_cast<int*>(smem + M::kFlags);
+  int& last_one = *reinterpret_cast<int*>(smem + M::kFlags + 4);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = lane & 3;
+  FewRing ring = make_ring<F>(smem, smem + M::kScales, reinterpret_cast<uint64_t*>(smem + M::kBars), gave_up, launch.status);
   uint8_t* const panel = smem + DownShape<F>::kFixed;
   float* const red = reinterpret_cast<float*>(panel);                     // (after the last panel)
+  if (tid == 0) {
+    *gave_up = 0;
+    ptx::prefetch_tensormap(&map);
+  }
   // What routed the tokens was complete before the kernel ahead of this one let it start.
   if (warp == 0) build_table<true>(table, p);
   else if (tid < 48) reinterpret_cast<uint32_t*>(zeros)[tid - 32] = 0;
@@ -958,12 +1053,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   for (int block_r0 = row_begin; block_r0 < row_end || !waited; block_r0 += by_column(F) ? columns * block_rows : kRows) {
     const int r0 = block_r0 + mine_side * kRows, rows_here = max(0, min(kRows, row_end - r0)), tiles = (rows_here + 15) / 16;
     FewRows fetch;
-    fetch.tiles = tiles;
 #pragma unroll
-    for (int i = 0; i < 2 * kTiles; ++i)
-      fetch.to[i] = (int64_t)max(0, min(8 * i + g, rows_here - 1)) * layout.row_bytes;   // (what a tile has not got is the last row again)
-#pragma unroll
-    for (int j = 0; j < kRows / 32; ++j) fetch.there[j] = by_column(F) ? 8 * g < rows_here : j * 32 + lane < rows_here;
+    for (int j = 0; j < kRows / 32; ++j) fetch.there[j] = j * 32 + lane < rows_here;
     // The step that is fetched next, how many are left of this warp's stretch, and where the panel after that begins.
     int fetch_a = 0, fetch_s = 0, left = 0, panel_a = step_begin / steps, panel_s = step_begin - panel_a * steps;
     bool found = false;
@@ -982,22 +1073,26 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       if (left > 0 && rows_here > 0) {
         if (fetch_s == steps) { fetch_s = 0; ++fetch_a; found = false; }
         if (!found) {
-          const int e = table.expert[fetch_a];
-          fetch.w = by_column(F) ? reinterpret_cast<const uint8_t*>(m.w) + ((int64_t)e * m.k + 8 * t) * layout.row_bytes + (r0 + 8 * g) * 2
-                                 : reinterpret_cast<const uint8_t*>(m.w) + (int64_t)(e * m.n + r0) * layout.row_bytes + t * 16;
+          fetch.e = table.expert[fetch_a];
 #pragma unroll
           for (int j = 0; j < kRows / 32; ++j)
-            if (!by_column(F)) fetch.s[j] = scales_of<F>(m, layout, e, fetch.there[j] ? r0 + j * 32 + lane : r0);
+            if (!by_column(F)) fetch.s[j] = scales_of<F>(m, layout, fetch.e, fetch.there[j] ? r0 + j * 32 + lane : r0);
           found = true;
         }
-        copy_step<F>(ring + slot * S::kSlot, fetch, layout, fetch_s);
+        if (lane == 0) {
+          const uint32_t bar = ring.bars + slot * 8;
+          ptx::fence_proxy_async();        // (the warp has read what was there)
+          ptx::mbar_expect_tx_s(bar, launch.box * 64);
+          ptx::tma_load_3d_s(ring.slots + slot * kSlotBytes, &map, bar, by_column(F) ? r0 : fetch_s * 64, by_column(F) ? fetch_s * S::kK : r0, fetch.e);
+        }
+        if (!by_column(F)) copy_scales<F>(ring.scales + slot * S::kSlotScales, fetch, layout, fetch_s);
         ++fetch_s;
         --left;
       }
       copies_end();
     };
 #pragma unroll 1
-    for (int i = 0; i < S::kDepth; ++i) copy_next(i);
+    for (int i = 0; i < S::kDepth; ++i) copy_next((ring.slot + i) % S::kDepth);
     // Biases while the ring fills, by the blocks with the first share (by column: when they are needed).
     constexpr int kMine = kRows * B200MOE_FEW_TOKENS / kThreads;
     float bias[kMine];
@@ -1012,7 +1107,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       waited = true;
     }
     float out[kTiles][NT][4] = {};
-    int slot = 0;
     for (int a0 = step_begin / steps, s0 = step_begin - a0 * steps; a0 * steps + s0 < step_end;) {
       int a1, s1;
       panel_end(a0, s0, a1, s1);
@@ -1047,7 +1141,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
           find_tokens<NT>(x, mine, mine, base, base_scales, smem_at(zeros), n_rows);
           float acc[kTiles][NT][4] = {};
 #pragma unroll 1
-          for (; pos < end; ++pos) take_step<F, NT, false>(acc, ring, slot, tiles, layout, x, pos - a * steps, pos - a * steps, copy_next);
+          for (; pos < end; ++pos) take_step<F, NT, S::kTerms>(acc, ring, tiles, row_order(), false, layout, x, pos - a * steps, copy_next);
           // (columns of tokens without this expert are left out: a weight that is not finite would get into them)
 #pragma unroll
           for (int n = 0; n < NT; ++n)

@@ -625,6 +625,8 @@ PyObject* layer_few(PyObject*, PyObject* const* a, Py_ssize_t n) {
   g.max_ctas = (int)int_arg(a[6]);
   const c10::cuda::CUDAGuard guard(x.device());
   const auto stream = at::cuda::getCurrentCUDAStream();
+  g.status = device_status_word(x.get_device());
+  raise_if_timed_out(g.status);   // an earlier call on this device gave up a wait
   WithoutGil gil;
   {
     g.workspace_bytes = b200moe_few_tokens_workspace_bytes((int)T, (int)K, (int)H, (int)k2);

@@ -107,11 +107,11 @@ def reference(x, weights, ids, w13, b13, w2, b2, act, clamp, emap, h_half, half)
 
 class Case:
     def __init__(self, native, recipe, T, H, I, E, K, dtype=BF16, act="silu", bias=False, clamp=None, group=128, seed=0, ranks=1, rank=0,
-                 few=True, **kw):
+                 few=True, group2=None, **kw):
         g = gen(seed)
         self.T, self.H, self.dtype = T, H, dtype
         self.w13, self.s13, self.d13 = make_matrix(recipe, g, E, 2 * I, H, dtype, group)
-        self.w2, self.s2, self.d2 = make_matrix(recipe, g, E, H, I, dtype, group)
+        self.w2, self.s2, self.d2 = make_matrix(recipe, g, E, H, I, dtype, group2 or group)
         rnd = lambda *s: torch.randn(*s, generator=g, device=DEV)  # noqa: E731
         self.b13 = (rnd(E, 2 * I) * 0.1).to(dtype) if bias else None
         self.b2 = (rnd(E, H) * 0.1).to(dtype) if bias else None
@@ -164,6 +164,13 @@ def test_formats_and_sizes(native, recipe, H, I, E, K, group, dtype):
 
 
 @pytest.mark.parametrize("T", range(1, 17))
+@pytest.mark.parametrize("group,group2", [(32, 128), (128, 32), (64, 256), (256, 64), (32, 64), (128, 256)])
+def test_int4_groups_of_both(native, group, group2):
+    """The two matrices may have groups of different lengths."""
+    c = Case(native, "int4", 5, 768, 512, 6, 3, group=group, group2=group2, seed=group + group2)
+    c.check(c.run())
+
+
 @pytest.mark.parametrize("recipe", ["w16", "fp8", "mxfp4", "int4"])
 def test_every_number_of_tokens(native, recipe, T):
     c = Case(native, recipe, T, 256, 256, 6, 3, seed=T)

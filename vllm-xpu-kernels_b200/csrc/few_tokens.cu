@@ -149,8 +149,8 @@ int few_map(CUtensorMap* map, const FewMatrix& m, int experts, int box) {
   const cuuint64_t row = F == kFewFp8 ? m.k : m.k / 2;
   const cuuint64_t dims[3] = {row, (cuuint64_t)m.n, (cuuint64_t)experts};
   const cuuint64_t strides[2] = {row, row * m.n};
-  const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1};
-  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, m.w, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_64B);
+  const cuuint32_t boxes[3] = {128, (cuuint32_t)box, 1};
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, m.w, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int F, int NT>
@@ -168,7 +168,7 @@ int launch_mma(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
     l.splits = FewWorkspace::splits(p.hidden, ctas, kRows);
     columns = ctas / l.splits;
   }
-  // Loads: rows of 64 bytes (codes) of 32 gates, 32 ups or 64 features in pairs, and of a piece's; by column 32 rows of the
+  // Loads: rows of 128 bytes (codes) of 32 gates, 32 ups or 64 features in pairs, and of a piece's; by column 32 rows of the
   // same columns.  In the second kernel the rows that a block has, by column 64.
   const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
   l.box = by_column(F) ? kRows : min(kRows, (p.hidden + columns - 1) / columns);

@@ -24,7 +24,6 @@ namespace {
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kTiles = 4;        // tiles of 16 rows that a warp takes at once
 constexpr int kRows = 16 * kTiles;
-constexpr int kSlotBytes = kRows * 64;    // of a warp's ring: the weights of a step
 constexpr int kFewMaxBlocks = 160;      // of a kernel (one per SM)
 constexpr int kFewMaxColumns = kFewMaxBlocks;
 constexpr int kMaxSlots = kFewMaxTopk * B200MOE_FEW_TOKENS;   // routed slots of a call
@@ -32,18 +31,19 @@ constexpr int kMaxSlots = kFewMaxTopk * B200MOE_FEW_TOKENS;   // routed slots of
 enum FewFormat { kFewFp8, kFewFp4, kFewInt4Fine, kFewInt4, kFewBf16, kFewF16 };   // Fine: groups of 32 or 64
 __host__ __device__ constexpr bool by_column(int f) { return f == kFewBf16 || f == kFewF16; }     // stored as [K, N]
 
-// A step of a warp is 64 bytes of its 64 rows; of weights stored by column 32 rows of 128 bytes.
+// A step of a warp is 128 bytes of its 64 rows; of weights stored by column 32 rows of 128 bytes.
 template <int F> struct FewShape {
-  static constexpr int kK = by_column(F) ? 32 : F == kFewFp8 ? 64 : 128;      // values of k
+  static constexpr int kK = by_column(F) ? 32 : F == kFewFp8 ? 128 : 256;     // values of k
+  static constexpr int kHalfBlocks = by_column(F) ? 1 : F == kFewFp8 ? 2 : 4;  // of the panel, per 64 bytes of a weight row
   static constexpr int kBlocks = kK / 32;                        // of the panel: a lane's eight values, two instructions
   // Of the panel: a row's values of a step and their scale.  h next to 16-bit weights is there twice, as the type has it
   // and what that leaves of it: with one rounding to 16 bits the results would be 1.4 times as far from the formula's as
   // their own rounding puts them.
   __host__ __device__ static constexpr int kPanelBytes(int terms) { return terms * kK * 2 + 4; }
   static constexpr int kTerms = by_column(F) ? 2 : 1;            // of h
-  static constexpr int kScaleWords = F == kFewInt4Fine ? 2 : 1;  // that hold a row's scales of a step
-  static constexpr int kScales = F == kFewFp8 || by_column(F) ? 0 : F == kFewInt4 ? 1 : 4;                       // of a row and step, made fp32 (fp8: are so)
-  static constexpr int kDepth = 3;
+  static constexpr int kScaleWords = F == kFewInt4Fine ? 4 : F == kFewFp4 ? 2 : 1;  // that hold a row's scales of a step
+  static constexpr int kScales = F == kFewFp8 || by_column(F) ? 0 : F == kFewInt4 ? 2 : 8;                       // of a row and step, made fp32 (fp8: are so)
+  static constexpr int kSlotBytes = by_column(F) ? 4096 : 8192, kDepth = by_column(F) ? 3 : 2;
   static constexpr int kRing = kDepth * kSlotBytes;
   // behind the rings of all warps, per warp: scales of the steps in the ring as they come, and as fp32
   static constexpr int kSlotScales = by_column(F) ? 0 : kRows * 4 * kScaleWords;
@@ -274,7 +274,7 @@ __device__ __forceinline__ void store8(uint8_t* at, int j, const uint4& o) {
 template <int F, bool kF32>
 __device__ __noinline__ void fill_row(uint8_t* panel, float* scales, const void* from, int values, int len, int row, int rows, int part, int parts,
                                       bool f16) {
-  constexpr int kLanes = FewShape<F>::kK / 8;      // of a step
+  constexpr int kLanes = FewShape<F>::kK / 8;      // of a step (at most 32)
   constexpr int kWords = kF32 ? 2 : 1;
   const int lane = threadIdx.x & 31, stride = 32 * parts;
 #pragma unroll 1
@@ -357,8 +357,9 @@ __device__ __noinline__ void fill_tokens(uint8_t* panel, float* scales, const vo
 
 // ---- weights: a warp's ring ------------------------------------------------------------
 // One lane asks for a step's weights by TMA, whose swizzle puts the 16-byte pieces of a row where the lanes' reads fall on
-// different banks: rows of 64 bytes (a lane reads one of the four pieces, or a word of each: a group of 32 4-bit codes is
-// handed out to four lanes), by column rows of 128 or two halves of 64.  Scales are fetched as words, neighbouring rows
+// different banks: rows of 128 bytes (a lane reads one of four pieces, or a word of each: a group of 32 4-bit codes is
+// handed out to four lanes; rows of 64 bytes kept the copy unit from the memory's rate, fp8 at one token 91 us, 74 without
+// it), by column rows of 128 or two halves of 64.  Scales are fetched as words, neighbouring rows
 // by neighbouring lanes (those of 4-bit formats are laid out for that: as they come, a step's would be 2 or 4 bytes of every
 // row, which kept the load units busy for longer than the weights did), and made fp32 by one lane per row.
 // (With every lane fetching its own pieces, MXFP4 took a third more instructions, and every first touch of a page held up
@@ -369,8 +370,12 @@ struct FewOrder {
   int tile, half;             // bytes from one tile to the next, from row g to g + 8
   int place, place_half;      // the same for places of scales
 };
-__device__ __forceinline__ FewOrder row_order() { return {1024, 512, 16, 8}; }          // 64 rows
-__device__ __forceinline__ FewOrder halves_order() { return {512, 2048, 8, 32}; }       // 32 gates, 32 ups
+__device__ __forceinline__ FewOrder row_order() { return {2048, 1024, 16, 8}; }         // 64 rows
+__device__ __forceinline__ FewOrder halves_order() { return {1024, 4096, 8, 32}; }      // 32 gates, 32 ups
+// Row of eight that the instruction's row g is: of the lanes that read 16 bytes at once (two rows g) one is in the first
+// four, so that the swizzle takes them to different banks.
+__device__ __forceinline__ int row_of(int g) { return (g >> 1) | ((g & 1) << 2); }
+__device__ __forceinline__ int g_of(int row) { return ((row & 3) << 1) | (row >> 2); }
 
 // What a warp fetches: the rows of one expert's matrix that it takes at once.
 struct FewRows {
@@ -405,15 +410,15 @@ template <int F>
 __device__ __forceinline__ void copy_scales(uint32_t to, const FewRows& r, const FewLayout& l, int s) {
   using S = FewShape<F>;
   const int lane = threadIdx.x & 31;
-  // (a word serves two steps of fp8, whose blocks are 128 long, and of int4 with one scale of 16 bits per step)
-  const bool two = F == kFewInt4Fine && l.group == 32;
-  const int word = F == kFewFp8 || F == kFewInt4 ? s >> 1 : two ? 2 * s : s;
+  // (the other matrix of kFewInt4Fine may have groups of 128 and more: a word for 256 values)
+  const int words = F == kFewInt4Fine ? (l.group == 32 ? 4 : l.group == 64 ? 2 : 1) : S::kScaleWords, word = s * words;
 #pragma unroll
   for (int j = 0; j < kRows / 32; ++j) {
     if (!r.there[j]) continue;
 #pragma unroll
     for (int i = 0; i < S::kScaleWords; ++i)
-      if (i == 0 || two) copy4(to + ((j * 32 + lane) * S::kScaleWords + i) * 4, r.s[j] + (int64_t)(word + i) * l.word_step);
+      // (a row's last step may have fewer; what they stand for is beyond the row)
+      if (i < words && (by_column(F) || F == kFewFp8 || word + i < l.words)) copy4(to + ((j * 32 + lane) * S::kScaleWords + i) * 4, r.s[j] + (int64_t)(word + i) * l.word_step);
   }
 }
 
@@ -449,21 +454,35 @@ __device__ __forceinline__ void spread_scales(uint32_t to, uint32_t from, const 
 #pragma unroll
   for (int j = 0; j < kRows / 32; ++j) {
     const int row = j * 32 + (threadIdx.x & 31);
-    const uint32_t at = from + row * S::kScaleWords * 4, v = lds4(at);
+    const uint32_t at = from + row * S::kScaleWords * 4;
     auto value = [&](uint32_t h) { return l.f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16); };
-    if constexpr (F == kFewFp4) {
-      // 2^(byte - 127): the byte is the exponent (0 gives zero for 2^-127, 255 infinity for NaN)
-      sts16(to + row * 16, __uint_as_float((v & 255u) << 23), __uint_as_float((v << 15) & 0x7f800000u),
-            __uint_as_float((v << 7) & 0x7f800000u), __uint_as_float((v >> 1) & 0x7f800000u));
-    } else if constexpr (F == kFewInt4) {
-      sts4(to + row * 4, value(s & 1 ? v >> 16 : v & 0xffffu));
-    } else if constexpr (F == kFewInt4Fine) {
-      const float a = value(v & 0xffffu), b = value(v >> 16);
-      if (l.group == 32) {
-        const uint32_t h = lds4(at + 4);
-        sts16(to + row * 16, a, b, value(h & 0xffffu), value(h >> 16));
-      } else {
-        sts16(to + row * 16, a, a, b, b);
+    if constexpr (F == kFewInt4) {
+      const uint32_t v = lds4(at);
+      sts4(to + row * 8, value(v & 0xffffu));
+      sts4(to + row * 8 + 4, value(v >> 16));
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {       // the halves of the step
+        const uint32_t place = to + (h * kRows + row) * 16;
+        if constexpr (F == kFewFp4) {
+          // 2^(byte - 127): the byte is the exponent (0 gives zero for 2^-127, 255 infinity for NaN).  Beyond the row: zeros,
+          // as whatever is there must not make a NaN of them.
+          const uint32_t v = 2 * s + h < l.words ? lds4(at + 4 * h) : 0;
+          sts16(place, __uint_as_float((v & 255u) << 23), __uint_as_float((v << 15) & 0x7f800000u), __uint_as_float((v << 7) & 0x7f800000u),
+                __uint_as_float((v >> 1) & 0x7f800000u));
+        } else if constexpr (F == kFewInt4Fine) {
+          if (l.group == 32) {
+            const uint32_t v = 4 * s + 2 * h < l.words ? lds4(at + 8 * h) : 0, w = 4 * s + 2 * h < l.words ? lds4(at + 8 * h + 4) : 0;
+            sts16(place, value(v & 0xffffu), value(v >> 16), value(w & 0xffffu), value(w >> 16));
+          } else if (l.group == 64) {
+            const uint32_t v = 2 * s + h < l.words ? lds4(at + 4 * h) : 0;
+            const float a = value(v & 0xffffu), b = value(v >> 16);
+            sts16(place, a, a, b, b);
+          } else {
+            const float a = value(lds4(at) >> 16 * h & 0xffffu);
+            sts16(place, a, a, a, a);
+          }
+        }
       }
     }
   }
@@ -496,77 +515,81 @@ template <int F, int NT, int Tiles>
 __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint32_t slot, uint32_t scales, const FewOrder& order,
                                               const FewTokens (&x)[NT], int s) {
   using S = FewShape<F>;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint4 v[S::kBlocks][NT];
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, row = row_of(g);
   float sx[NT][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) sx[n][c] = ldsf(x[n].scale[c] + s * x[n].step);
-#pragma unroll
-    for (int q = 0; q < S::kBlocks; ++q) v[q][n] = lds16(x[n].at + (s * S::kBlocks + q) * x[n].block);
-  }
-#pragma unroll
-  for (int i = 0; i < Tiles; ++i) {
-    const int at_lo = i * order.place + g, at_hi = at_lo + order.place_half;     // places of the scales
-    float d[NT][4], sum[NT][4] = {};   // products of a group of weights, and the step's
-    auto add = [&](float a, float b) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        sum[n][0] = fmaf(a, d[n][0], sum[n][0]);
-        sum[n][1] = fmaf(a, d[n][1], sum[n][1]);
-        sum[n][2] = fmaf(b, d[n][2], sum[n][2]);
-        sum[n][3] = fmaf(b, d[n][3], sum[n][3]);
-      }
-    };
-    if constexpr (F == kFewFp8) {
-      const uint32_t at = slot + i * order.tile + g * 64 + ((t ^ (g >> 1)) << 4);
-      const uint4 lo = lds16(at), hi = lds16(at + order.half);
-      const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t a0, a1, a2, a3;
-        e4m3x4_to_h2(wl[w], a0, a2);
-        e4m3x4_to_h2(wh[w], a1, a3);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint4 b = v[w >> 1][n];
-          if (w == 0) mma_first(d[n], a0, a1, a2, a3, b.x, b.y);
-          else mma(d[n], a0, a1, a2, a3, w & 1 ? b.z : b.x, w & 1 ? b.w : b.y);
-        }
-      }
-      add(ldsf(scales + at_lo * 4), ldsf(scales + at_hi * 4));
-    } else {
-      uint4 lo, hi;
-      if constexpr (S::kScales == 4) {
-        lo = lds16(scales + at_lo * 16);
-        hi = lds16(scales + at_hi * 16);
-      } else {
-        lo.w = lds4(scales + at_lo * 4);
-        hi.w = lds4(scales + at_hi * 4);
-      }
-      const uint32_t w = slot + i * order.tile + g * 64 + t * 4;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int at = (q ^ (g >> 1)) << 4;
-        const uint32_t wl = lds4(w + at), wh = lds4(w + at + order.half);
-        uint32_t al[4], ah[4];
-        if constexpr (F == kFewFp4) { e2m1x8_to_h2(wl, al); e2m1x8_to_h2(wh, ah); }
-        else { s4x8_to_h2(wl, al); s4x8_to_h2(wh, ah); }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (S::kScales == 4 || q == 0) mma_first(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
-          else mma(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
-          mma(d[n], al[2], ah[2], al[3], ah[3], v[q][n].z, v[q][n].w);
-        }
-        if (S::kScales == 4 || q == 3) add(__uint_as_float(q == 0 ? lo.x : q == 1 ? lo.y : q == 2 ? lo.z : lo.w),
-                                             __uint_as_float(q == 0 ? hi.x : q == 1 ? hi.y : q == 2 ? hi.z : hi.w));
-      }
-    }
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {       // the row's first and second 64 bytes
+    uint4 v[S::kHalfBlocks][NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf(sx[n][c & 1], sum[n][c], acc[i][n][c]);
+      for (int q = 0; q < S::kHalfBlocks; ++q) v[q][n] = lds16(x[n].at + (s * S::kBlocks + h * S::kHalfBlocks + q) * x[n].block);
+#pragma unroll
+    for (int i = 0; i < Tiles; ++i) {
+      const int at_lo = i * order.place + row, at_hi = at_lo + order.place_half;     // places of the scales
+      float d[NT][4], sum[NT][4] = {};   // products of a group of weights, and the half's
+      auto add = [&](float a, float b) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          sum[n][0] = fmaf(a, d[n][0], sum[n][0]);
+          sum[n][1] = fmaf(a, d[n][1], sum[n][1]);
+          sum[n][2] = fmaf(b, d[n][2], sum[n][2]);
+          sum[n][3] = fmaf(b, d[n][3], sum[n][3]);
+        }
+      };
+      if constexpr (F == kFewFp8) {
+        const uint32_t at = slot + i * order.tile + row * 128 + (((4 * h + t) ^ row) << 4);
+        const uint4 lo = lds16(at), hi = lds16(at + order.half);
+        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_to_h2(wl[w], a0, a2);
+          e4m3x4_to_h2(wh[w], a1, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 b = v[w >> 1][n];
+            if (w == 0) mma_first(d[n], a0, a1, a2, a3, b.x, b.y);
+            else mma(d[n], a0, a1, a2, a3, w & 1 ? b.z : b.x, w & 1 ? b.w : b.y);
+          }
+        }
+        add(ldsf(scales + at_lo * 4), ldsf(scales + at_hi * 4));
+      } else {
+        uint4 lo, hi;
+        if constexpr (S::kScales == 8) {
+          lo = lds16(scales + (h * kRows + at_lo) * 16);
+          hi = lds16(scales + (h * kRows + at_hi) * 16);
+        } else {
+          lo.w = lds4(scales + at_lo * 8 + h * 4);
+          hi.w = lds4(scales + at_hi * 8 + h * 4);
+        }
+        const uint32_t w = slot + i * order.tile + row * 128 + t * 4;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int at = ((4 * h + q) ^ row) << 4;
+          const uint32_t wl = lds4(w + at), wh = lds4(w + at + order.half);
+          uint32_t al[4], ah[4];
+          if constexpr (F == kFewFp4) { e2m1x8_to_h2(wl, al); e2m1x8_to_h2(wh, ah); }
+          else { s4x8_to_h2(wl, al); s4x8_to_h2(wh, ah); }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if (S::kScales == 8 || q == 0) mma_first(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
+            else mma(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
+            mma(d[n], al[2], ah[2], al[3], ah[3], v[q][n].z, v[q][n].w);
+          }
+          if (S::kScales == 8 || q == 3) add(__uint_as_float(q == 0 ? lo.x : q == 1 ? lo.y : q == 2 ? lo.z : lo.w),
+                                               __uint_as_float(q == 0 ? hi.x : q == 1 ? hi.y : q == 2 ? hi.z : hi.w));
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf(sx[n][c & 1], sum[n][c], acc[i][n][c]);
+    }
   }
 }
 
@@ -624,7 +647,7 @@ template <int F, int NT, int kTerms, typename Next>
 __device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], FewRing& ring, int tiles, const FewOrder& order, bool halves, const FewLayout& l,
                                           const FewTokens (&x)[NT], int s, Next next) {
   using S = FewShape<F>;
-  const uint32_t at = ring.slots + ring.slot * kSlotBytes;
+  const uint32_t at = ring.slots + ring.slot * S::kSlotBytes;
   uint32_t scales = ring.scales + ring.slot * S::kSlotScales;
   copies_wait<S::kDepth - 1>();
   if (!by_column(F) && F != kFewFp8) {
@@ -703,16 +726,19 @@ template <int NT> struct RedShape {
     return tile * kTile + ((col >> 3) * 4 + (row >> 3) * 2 + (col & 1)) * 32 + (row & 7) * 4 + ((col & 7) >> 1);
   }
 };
-// Tile and row of the sums of a column of W13's part (gate or up of feature f of the 32), and of output c of the 64.
+// Tile and row (of the instruction) of the sums of a column of W13's part (gate or up of feature f of the 32), and of output c of the 64.
 template <int F>
 __device__ __forceinline__ int2 sums_of(int f, bool up, bool pairs) {
-  if (!by_column(F)) return pairs ? make_int2(f >> 3, 2 * (f & 7) + (up ? 1 : 0)) : make_int2(f >> 3, (f & 7) + (up ? 8 : 0));
+  if (!by_column(F)) {
+    const int row = pairs ? 2 * (f & 7) + (up ? 1 : 0) : (f & 7) + (up ? 8 : 0);
+    return make_int2(f >> 3, (row & 8) + g_of(row & 7));
+  }
   if (pairs) return make_int2(f & 3, (f >> 2) + (up ? 8 : 0));
   return make_int2((f & 7) >> 1, (f >> 3) + (up ? 4 : 0) + (f & 1 ? 8 : 0));
 }
 template <int F>
 __device__ __forceinline__ int2 sums_of(int c) {
-  return by_column(F) ? make_int2((c & 7) >> 1, (c >> 3) + (c & 1 ? 8 : 0)) : make_int2(c >> 4, c & 15);
+  return by_column(F) ? make_int2((c & 7) >> 1, (c >> 3) + (c & 1 ? 8 : 0)) : make_int2(c >> 4, (c & 8) + g_of(c & 7));
 }
 // A warp's sums to its place.
 template <int NT>
@@ -873,25 +899,25 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         }
         if (next.at < my_to) {
           if (lane == 0) {
-            const uint32_t to = ring.slots + slot * kSlotBytes, bar = ring.bars + slot * 8;
-            const int x = by_column(F) ? fetch.row : s * 64, y = by_column(F) ? s * S::kK : fetch.row;
+            const uint32_t to = ring.slots + slot * S::kSlotBytes, bar = ring.bars + slot * 8;
+            const int x = by_column(F) ? fetch.row : s * 128, y = by_column(F) ? s * S::kK : fetch.row;
             ptx::fence_proxy_async();      // (the warp has read what was there)
             if (by_column(F) || fetch.tiles == kTiles) {
-              ptx::mbar_expect_tx_s(bar, kSlotBytes);
+              ptx::mbar_expect_tx_s(bar, S::kSlotBytes);
               if (pairs) {
                 ptx::tma_load_3d_s(to, &map, bar, by_column(F) ? 2 * x : x, by_column(F) ? y : 2 * y, fetch.e);
               } else {
                 ptx::tma_load_3d_s(to, &map, bar, x, y, fetch.e);
-                ptx::tma_load_3d_s(to + 2048, &map, bar, by_column(F) ? p.inter + x : x, by_column(F) ? y : p.inter + y, fetch.e);
+                ptx::tma_load_3d_s(to + S::kSlotBytes / 2, &map, bar, by_column(F) ? p.inter + x : x, by_column(F) ? y : p.inter + y, fetch.e);
               }
             } else {                       // the tiles that there are, one by one
-              ptx::mbar_expect_tx_s(bar, fetch.tiles * 1024);
+              ptx::mbar_expect_tx_s(bar, fetch.tiles * 2048);
               for (int i = 0; i < fetch.tiles; ++i) {
                 if (pairs) {
-                  ptx::tma_load_3d_s(to + i * 1024, &piece_map, bar, x, 2 * (y + 8 * i), fetch.e);
+                  ptx::tma_load_3d_s(to + i * 2048, &piece_map, bar, x, 2 * (y + 8 * i), fetch.e);
                 } else {
-                  ptx::tma_load_3d_s(to + i * 512, &piece_map, bar, x, y + 8 * i, fetch.e);
-                  ptx::tma_load_3d_s(to + 2048 + i * 512, &piece_map, bar, x, p.inter + y + 8 * i, fetch.e);
+                  ptx::tma_load_3d_s(to + i * 1024, &piece_map, bar, x, y + 8 * i, fetch.e);
+                  ptx::tma_load_3d_s(to + 4096 + i * 1024, &piece_map, bar, x, p.inter + y + 8 * i, fetch.e);
                 }
               }
             }
@@ -1082,8 +1108,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
         if (lane == 0) {
           const uint32_t bar = ring.bars + slot * 8;
           ptx::fence_proxy_async();        // (the warp has read what was there)
-          ptx::mbar_expect_tx_s(bar, launch.box * 64);
-          ptx::tma_load_3d_s(ring.slots + slot * kSlotBytes, &map, bar, by_column(F) ? r0 : fetch_s * 64, by_column(F) ? fetch_s * S::kK : r0, fetch.e);
+          ptx::mbar_expect_tx_s(bar, launch.box * (by_column(F) ? 64 : 128));
+          ptx::tma_load_3d_s(ring.slots + slot * S::kSlotBytes, &map, bar, by_column(F) ? r0 : fetch_s * 128, by_column(F) ? fetch_s * S::kK : r0, fetch.e);
         }
         if (!by_column(F)) copy_scales<F>(ring.scales + slot * S::kSlotScales, fetch, layout, fetch_s);
         ++fetch_s;

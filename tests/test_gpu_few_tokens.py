@@ -163,7 +163,6 @@ def test_formats_and_sizes(native, recipe, H, I, E, K, group, dtype):
         c.check(c.run())
 
 
-@pytest.mark.parametrize("T", range(1, 17))
 @pytest.mark.parametrize("group,group2", [(32, 128), (128, 32), (64, 256), (256, 64), (32, 64), (128, 256)])
 def test_int4_groups_of_both(native, group, group2):
     """The two matrices may have groups of different lengths."""
@@ -171,6 +170,7 @@ def test_int4_groups_of_both(native, group, group2):
     c.check(c.run())
 
 
+@pytest.mark.parametrize("T", range(1, 17))
 @pytest.mark.parametrize("recipe", ["w16", "fp8", "mxfp4", "int4"])
 def test_every_number_of_tokens(native, recipe, T):
     c = Case(native, recipe, T, 256, 256, 6, 3, seed=T)

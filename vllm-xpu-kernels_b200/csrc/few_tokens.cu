@@ -107,18 +107,18 @@ constexpr int kMaxBlockSmem = 232448;
 // The attribute is set once per kernel and device, and always to the most that a block may have, so that calls with
 // different needs do not get into each other's way.
 template <auto Kern, typename... Maps>
-int launch_block_per_sm(const char* name, int grid, int smem, cudaStream_t st, const FewParams& p, const FewLaunch& l, const Maps&... maps) {
+int launch_block_per_sm(const char* name, int grid, int threads, int smem, cudaStream_t st, const FewParams& p, const FewLaunch& l, const Maps&... maps) {
   static std::atomic<bool> done[kMaxDevices];
   const int dev = current_device();
   if (!done[dev].load(std::memory_order_acquire)) {
     B200_CUDA_OK(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBlockSmem));
     done[dev].store(true, std::memory_order_release);
   }
-  B200_LAUNCHED(name, launch_pdl(true, Kern, dim3(grid), dim3(kThreads), smem, st, p, l, maps...));
+  B200_LAUNCHED(name, launch_pdl(true, Kern, dim3(grid), dim3(threads), smem, st, p, l, maps...));
   return B200MOE_OK;
 }
 
-constexpr int kMaxSide = 8;      // warps side by side in the second kernel
+constexpr int kMaxBlockRows = 512;      // of W2 that a block of the second kernel can have at once
 
 // Where things are in the workspace: h, then what the blocks of the two kernels tell one another.
 struct FewWorkspace {
@@ -130,7 +130,7 @@ struct FewWorkspace {
     bytes = part + up((size_t)splits(hidden, kFewMaxBlocks) * tokens * hidden * sizeof(float));
   }
   // Shares of the second kernel's steps: as many as make `ctas` blocks with up to `rows` rows each.
-  static int splits(int64_t hidden, int ctas, int rows = kMaxSide * kRows) {
+  static int splits(int64_t hidden, int ctas, int rows = kMaxBlockRows) {
     const int64_t n = (int64_t)ctas * rows / hidden;
     return n < 1 ? 1 : n > ctas ? ctas : (int)n;
   }
@@ -155,35 +155,44 @@ int few_map(CUtensorMap* map, const FewMatrix& m, int experts, int box) {
 
 template <int F, int NT>
 int launch_mma(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
-  constexpr int k = FewShape<F>::kK, up_room = kMaxBlockSmem - UpShape<F, NT>::kFixed, down_room = kMaxBlockSmem - DownShape<F>::kFixed;
+  constexpr int k = FewShape<F>::kK, up_fixed = by_column(F) ? UpShape<F, NT>::kFixed : UpRowsShape<F, NT>::kFixed, up_room = kMaxBlockSmem - up_fixed, down_room = kMaxBlockSmem - DownShape<F>::kFixed;
   const int up_row = (p.hidden + k - 1) / k * FewShape<F>::kPanelBytes(1);
   const int down_row = (p.inter + k - 1) / k * FewShape<F>::kPanelBytes(FewShape<F>::kTerms);
   l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
-  l.side = p.hidden > 2 * kRows ? 4 : p.hidden > kRows ? 2 : 1;
-  int columns = (p.hidden + l.side * kRows - 1) / (l.side * kRows);
+  int columns;
   if (by_column(F)) {
+    constexpr int kRows = FewShape<F>::kRows;
+    l.box = kRows;
+    l.side = p.hidden > 2 * kRows ? 4 : p.hidden > kRows ? 2 : 1;
+    columns = (p.hidden + l.side * kRows - 1) / (l.side * kRows);
     if (columns > ctas) columns = ctas;
     l.splits = ctas / columns;
   } else {
-    l.splits = FewWorkspace::splits(p.hidden, ctas, kRows);
+    l.splits = FewWorkspace::splits(p.hidden, ctas, kBlockRows);
     columns = ctas / l.splits;
+    // a block's rows in as few turns as they need, and halved in each
+    const int rows = (p.hidden + columns - 1) / columns, turns = (rows + kBlockRows - 1) / kBlockRows;
+    l.side = 2;
+    l.box = (rows + 2 * turns - 1) / (2 * turns);
   }
   // Loads: rows of 128 bytes (codes) of 32 gates, 32 ups or 64 features in pairs, and of a piece's; by column 32 rows of the
   // same columns.  In the second kernel the rows that a block has, by column 64.
   const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
-  l.box = by_column(F) ? kRows : min(kRows, (p.hidden + columns - 1) / columns);
   CUtensorMap up_map, piece_map, down_map;
-  int rc = few_map<F>(&up_map, p.w13, p.experts, pairs ? 64 : 32);
+  int rc = few_map<F>(&up_map, p.w13, p.experts, FewShape<F>::kRows / (pairs ? 1 : 2));
   if (rc == B200MOE_OK) rc = by_column(F) ? B200MOE_OK : few_map<F>(&piece_map, p.w13, p.experts, pairs ? 16 : 8);
   if (rc == B200MOE_OK) rc = few_map<F>(&down_map, p.w2, p.experts, l.box);
   if (rc != B200MOE_OK) return rc;
-  if (by_column(F)) piece_map = up_map;
-  rc = launch_block_per_sm<few_up_kernel<F, NT>>("few_up_kernel", ctas, UpShape<F, NT>::kFixed + l.panel_bytes, st, p, l, up_map, piece_map);
+  if constexpr (by_column(F))
+    rc = launch_block_per_sm<few_up_columns_kernel<F, NT>>("few_up_columns_kernel", ctas, FewShape<F>::kThreads, up_fixed + l.panel_bytes, st, p, l, up_map);
+  else
+    rc = launch_block_per_sm<few_up_rows_kernel<F, NT>>("few_up_rows_kernel", ctas, FewShape<F>::kThreads, up_fixed + l.panel_bytes, st, p, l, up_map,
+                                                        piece_map);
   if (rc != B200MOE_OK) return rc;
   const int64_t want = (int64_t)p.tokens * p.topk * down_row;
   l.panel_bytes = (int)(want < down_room ? want : down_room);
-  if (l.panel_bytes < RedShape<NT>::kBytes) l.panel_bytes = RedShape<NT>::kBytes;
-  return launch_block_per_sm<few_down_kernel<F, NT>>("few_down_kernel", columns * l.splits, DownShape<F>::kFixed + l.panel_bytes, st, p, l, down_map);
+  if (l.panel_bytes < RedShape<F, NT>::kBytes) l.panel_bytes = RedShape<F, NT>::kBytes;
+  return launch_block_per_sm<few_down_kernel<F, NT>>("few_down_kernel", columns * l.splits, FewShape<F>::kThreads, DownShape<F>::kFixed + l.panel_bytes, st, p, l, down_map);
 }
 
 template <int F>

@@ -21,9 +21,6 @@
 namespace b200moe {
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kTiles = 4;        // tiles of 16 rows that a warp takes at once
-constexpr int kRows = 16 * kTiles;
 constexpr int kFewMaxBlocks = 160;      // of a kernel (one per SM)
 constexpr int kFewMaxColumns = kFewMaxBlocks;
 constexpr int kMaxSlots = kFewMaxTopk * B200MOE_FEW_TOKENS;   // routed slots of a call
@@ -31,8 +28,12 @@ constexpr int kMaxSlots = kFewMaxTopk * B200MOE_FEW_TOKENS;   // routed slots of
 enum FewFormat { kFewFp8, kFewFp4, kFewInt4Fine, kFewInt4, kFewBf16, kFewF16 };   // Fine: groups of 32 or 64
 __host__ __device__ constexpr bool by_column(int f) { return f == kFewBf16 || f == kFewF16; }     // stored as [K, N]
 
-// A step of a warp is 128 bytes of its 64 rows; of weights stored by column 32 rows of 128 bytes.
+// A step of a warp is 4 KB: 128 bytes of its 32 rows; of weights stored by column 32 rows of 128 bytes.  Codes are turned into
+// float16 by every warp for itself, between loads from shared memory and products that depend on one another, and 16 warps
+// hide that where 8 with twice the rows did not
 template <int F> struct FewShape {
+  static constexpr int kWarps = by_column(F) ? 8 : 12, kThreads = 32 * kWarps;
+  static constexpr int kTiles = by_column(F) ? 4 : 2, kRows = 16 * kTiles;     // tiles of 16 rows that a warp takes at once
   static constexpr int kK = by_column(F) ? 32 : F == kFewFp8 ? 128 : 256;     // values of k
   static constexpr int kHalfBlocks = by_column(F) ? 1 : F == kFewFp8 ? 2 : 4;  // of the panel, per 64 bytes of a weight row
   static constexpr int kBlocks = kK / 32;                        // of the panel: a lane's eight values, two instructions
@@ -43,7 +44,7 @@ template <int F> struct FewShape {
   static constexpr int kTerms = by_column(F) ? 2 : 1;            // of h
   static constexpr int kScaleWords = F == kFewInt4Fine ? 4 : F == kFewFp4 ? 2 : 1;  // that hold a row's scales of a step
   static constexpr int kScales = F == kFewFp8 || by_column(F) ? 0 : F == kFewInt4 ? 2 : 8;                       // of a row and step, made fp32 (fp8: are so)
-  static constexpr int kSlotBytes = by_column(F) ? 4096 : 8192, kDepth = by_column(F) ? 3 : 2;
+  static constexpr int kSlotBytes = 4096, kDepth = by_column(F) ? 3 : 2;
   static constexpr int kRing = kDepth * kSlotBytes;
   // behind the rings of all warps, per warp: scales of the steps in the ring as they come, and as fp32
   static constexpr int kSlotScales = by_column(F) ? 0 : kRows * 4 * kScaleWords;
@@ -370,8 +371,8 @@ struct FewOrder {
   int tile, half;             // bytes from one tile to the next, from row g to g + 8
   int place, place_half;      // the same for places of scales
 };
-__device__ __forceinline__ FewOrder row_order() { return {2048, 1024, 16, 8}; }         // 64 rows
-__device__ __forceinline__ FewOrder halves_order() { return {1024, 4096, 8, 32}; }      // 32 gates, 32 ups
+__device__ __forceinline__ FewOrder row_order() { return {2048, 1024, 16, 8}; }         // 32 rows
+__device__ __forceinline__ FewOrder halves_order() { return {1024, 2048, 8, 16}; }      // 16 gates, 16 ups
 // Row of eight that the instruction's row g is: of the lanes that read 16 bytes at once (two rows g) one is in the first
 // four, so that the swizzle takes them to different banks.
 __device__ __forceinline__ int row_of(int g) { return (g >> 1) | ((g & 1) << 2); }
@@ -381,8 +382,8 @@ __device__ __forceinline__ int g_of(int row) { return ((row & 3) << 1) | (row >>
 struct FewRows {
   int e, row;                             // expert, first row (feature)
   int tiles;                              // that there are
-  const uint8_t* s[kRows / 32];           // scales of step 0 of the rows that the lane looks after, places lane + 32 i
-  bool there[kRows / 32];                 // whether these rows are
+  const uint8_t* s;                       // scales of step 0 of the row that the lane looks after
+  bool there;                             // whether it is
 };
 // The matrix as a whole.
 struct FewLayout {
@@ -412,14 +413,11 @@ __device__ __forceinline__ void copy_scales(uint32_t to, const FewRows& r, const
   const int lane = threadIdx.x & 31;
   // (the other matrix of kFewInt4Fine may have groups of 128 and more: a word for 256 values)
   const int words = F == kFewInt4Fine ? (l.group == 32 ? 4 : l.group == 64 ? 2 : 1) : S::kScaleWords, word = s * words;
+  if (!r.there) return;
 #pragma unroll
-  for (int j = 0; j < kRows / 32; ++j) {
-    if (!r.there[j]) continue;
-#pragma unroll
-    for (int i = 0; i < S::kScaleWords; ++i)
-      // (a row's last step may have fewer; what they stand for is beyond the row)
-      if (i < words && (by_column(F) || F == kFewFp8 || word + i < l.words)) copy4(to + ((j * 32 + lane) * S::kScaleWords + i) * 4, r.s[j] + (int64_t)(word + i) * l.word_step);
-  }
+  for (int i = 0; i < S::kScaleWords; ++i)
+    // (a row's last step may have fewer; what they stand for is beyond the row)
+    if (i < words && (F == kFewFp8 || word + i < l.words)) copy4(to + (lane * S::kScaleWords + i) * 4, r.s + (int64_t)(word + i) * l.word_step);
 }
 
 // A warp's ring, one slot after the other.
@@ -429,6 +427,7 @@ struct FewRing {
   int slot, parity;          // that is taken next
   volatile int* gave_up;
   int32_t* status;
+  uint64_t once;             // L2 policy of the weights
 };
 // Waits for a slot; a wait that runs out sets the status word, and the kernel goes on with what is there (later waits, one for
 // every copy in flight, are short then).
@@ -451,37 +450,34 @@ __device__ __forceinline__ void ring_wait(const FewRing& r) {
 template <int F>
 __device__ __forceinline__ void spread_scales(uint32_t to, uint32_t from, const FewLayout& l, int s) {
   using S = FewShape<F>;
+  const int row = threadIdx.x & 31;
+  const uint32_t at = from + row * S::kScaleWords * 4;
+  auto value = [&](uint32_t h) { return l.f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16); };
+  if constexpr (F == kFewInt4) {
+    const uint32_t v = lds4(at);
+    sts4(to + row * 8, value(v & 0xffffu));
+    sts4(to + row * 8 + 4, value(v >> 16));
+  } else {
 #pragma unroll
-  for (int j = 0; j < kRows / 32; ++j) {
-    const int row = j * 32 + (threadIdx.x & 31);
-    const uint32_t at = from + row * S::kScaleWords * 4;
-    auto value = [&](uint32_t h) { return l.f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16); };
-    if constexpr (F == kFewInt4) {
-      const uint32_t v = lds4(at);
-      sts4(to + row * 8, value(v & 0xffffu));
-      sts4(to + row * 8 + 4, value(v >> 16));
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {       // the halves of the step
-        const uint32_t place = to + (h * kRows + row) * 16;
-        if constexpr (F == kFewFp4) {
-          // 2^(byte - 127): the byte is the exponent (0 gives zero for 2^-127, 255 infinity for NaN).  Beyond the row: zeros,
-          // as whatever is there must not make a NaN of them.
+    for (int h = 0; h < 2; ++h) {       // the halves of the step
+      const uint32_t place = to + (h * S::kRows + row) * 16;
+      if constexpr (F == kFewFp4) {
+        // 2^(byte - 127): the byte is the exponent (0 gives zero for 2^-127, 255 infinity for NaN).  Beyond the row: zeros,
+        // as whatever is there must not make a NaN of them.
+        const uint32_t v = 2 * s + h < l.words ? lds4(at + 4 * h) : 0;
+        sts16(place, __uint_as_float((v & 255u) << 23), __uint_as_float((v << 15) & 0x7f800000u), __uint_as_float((v << 7) & 0x7f800000u),
+              __uint_as_float((v >> 1) & 0x7f800000u));
+      } else if constexpr (F == kFewInt4Fine) {
+        if (l.group == 32) {
+          const uint32_t v = 4 * s + 2 * h < l.words ? lds4(at + 8 * h) : 0, w = 4 * s + 2 * h < l.words ? lds4(at + 8 * h + 4) : 0;
+          sts16(place, value(v & 0xffffu), value(v >> 16), value(w & 0xffffu), value(w >> 16));
+        } else if (l.group == 64) {
           const uint32_t v = 2 * s + h < l.words ? lds4(at + 4 * h) : 0;
-          sts16(place, __uint_as_float((v & 255u) << 23), __uint_as_float((v << 15) & 0x7f800000u), __uint_as_float((v << 7) & 0x7f800000u),
-                __uint_as_float((v >> 1) & 0x7f800000u));
-        } else if constexpr (F == kFewInt4Fine) {
-          if (l.group == 32) {
-            const uint32_t v = 4 * s + 2 * h < l.words ? lds4(at + 8 * h) : 0, w = 4 * s + 2 * h < l.words ? lds4(at + 8 * h + 4) : 0;
-            sts16(place, value(v & 0xffffu), value(v >> 16), value(w & 0xffffu), value(w >> 16));
-          } else if (l.group == 64) {
-            const uint32_t v = 2 * s + h < l.words ? lds4(at + 4 * h) : 0;
-            const float a = value(v & 0xffffu), b = value(v >> 16);
-            sts16(place, a, a, b, b);
-          } else {
-            const float a = value(lds4(at) >> 16 * h & 0xffffu);
-            sts16(place, a, a, a, a);
-          }
+          const float a = value(v & 0xffffu), b = value(v >> 16);
+          sts16(place, a, a, b, b);
+        } else {
+          const float a = value(lds4(at) >> 16 * h & 0xffffu);
+          sts16(place, a, a, a, a);
         }
       }
     }
@@ -512,7 +508,7 @@ __device__ __forceinline__ void find_tokens(FewTokens (&x)[NT], uint32_t used, u
 // acc += W x of the step in the slot, for the first `Tiles` tiles (what one of them has not got is something finite or not, in
 // rows that nobody reads).
 template <int F, int NT, int Tiles>
-__device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint32_t slot, uint32_t scales, const FewOrder& order,
+__device__ __forceinline__ void multiply_step(float (&acc)[FewShape<F>::kTiles][NT][4], uint32_t slot, uint32_t scales, const FewOrder& order,
                                               const FewTokens (&x)[NT], int s) {
   using S = FewShape<F>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, row = row_of(g);
@@ -561,8 +557,8 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
       } else {
         uint4 lo, hi;
         if constexpr (S::kScales == 8) {
-          lo = lds16(scales + (h * kRows + at_lo) * 16);
-          hi = lds16(scales + (h * kRows + at_hi) * 16);
+          lo = lds16(scales + (h * S::kRows + at_lo) * 16);
+          hi = lds16(scales + (h * S::kRows + at_hi) * 16);
         } else {
           lo.w = lds4(scales + at_lo * 8 + h * 4);
           hi.w = lds4(scales + at_hi * 8 + h * 4);
@@ -597,7 +593,8 @@ __device__ __forceinline__ void multiply_step(float (&acc)[kTiles][NT][4], uint3
 // the instruction wants (rows g and g + 8 of product i are the lane's features 2 i and 2 i + 1).  halves: 32 and 32 columns
 // (gates, ups) behind one another, else 64.
 template <int F, int NT, int kTerms>
-__device__ __forceinline__ void multiply_columns(float (&acc)[kTiles][NT][4], uint32_t slot, bool halves, const FewTokens (&x)[NT], int s) {
+__device__ __forceinline__ void multiply_columns(float (&acc)[FewShape<F>::kTiles][NT][4], uint32_t slot, bool halves, const FewTokens (&x)[NT], int s) {
+  constexpr int kTiles = FewShape<F>::kTiles;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint4 v[kTerms][NT];
   float d[kTiles][NT][4] = {};
@@ -644,7 +641,7 @@ __device__ __forceinline__ void multiply_columns(float (&acc)[kTiles][NT][4], ui
 
 // Takes the step in the ring's slot and fetches the next one into it.
 template <int F, int NT, int kTerms, typename Next>
-__device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], FewRing& ring, int tiles, const FewOrder& order, bool halves, const FewLayout& l,
+__device__ __forceinline__ void take_step(float (&acc)[FewShape<F>::kTiles][NT][4], FewRing& ring, int tiles, const FewOrder& order, bool halves, const FewLayout& l,
                                           const FewTokens (&x)[NT], int s, Next next) {
   using S = FewShape<F>;
   const uint32_t at = ring.slots + ring.slot * S::kSlotBytes;
@@ -658,8 +655,8 @@ __device__ __forceinline__ void take_step(float (&acc)[kTiles][NT][4], FewRing& 
   __syncwarp();
   ring_wait(ring);
   if constexpr (by_column(F)) multiply_columns<F, NT, kTerms>(acc, at, halves, x, s);
-  else if (tiles > kTiles / 2) multiply_step<F, NT, kTiles>(acc, at, scales, order, x, s);
-  else multiply_step<F, NT, kTiles / 2>(acc, at, scales, order, x, s);
+  else if (tiles > S::kTiles / 2) multiply_step<F, NT, S::kTiles>(acc, at, scales, order, x, s);
+  else multiply_step<F, NT, S::kTiles / 2>(acc, at, scales, order, x, s);
   __syncwarp();
   next(ring.slot);
   if (++ring.slot == S::kDepth) {
@@ -679,6 +676,7 @@ __device__ __forceinline__ FewRing make_ring(uint8_t* rings, uint8_t* scales, ui
   r.slot = r.parity = 0;
   r.gave_up = gave_up;
   r.status = status;
+  r.once = ptx::l2_evict_first();
   if ((threadIdx.x & 31) == 0) {
     for (int i = 0; i < S::kDepth; ++i) ptx::mbar_init(bars + warp * S::kDepth + i, 1);
     ptx::fence_barrier_init();
@@ -700,33 +698,33 @@ struct FewLaunch {
   int panel_bytes;       // of shared memory for the panel
   bool f16;
   int splits;            // shares of the second kernel's steps: blocks / splits have the same rows
-  int side;              // by column: warps side by side in the second kernel (1, 2, 4)
+  int side;              // warps side by side in the second kernel (1, 2, 4)
   uint32_t* arrived;     // per column of blocks of the second kernel
   float* part;           // [splits][tokens][hidden]: partial sums, with more than one split
-  int box;               // rows (by column: columns) that a load of the second kernel brings
+  int box;               // rows (by column: columns) of a warp of the second kernel, which a load brings
   int32_t* status;       // for waits that run out, or NULL
 };
 
 // The tiles that the warps of a block take together: where they are among the pieces, and a warp's part.
 struct FewPlace {
   int at, a, u;           // the first piece: of all, its expert (of the active ones), and within that
-  int pieces;             // that the block's warps take together (by column) or the group takes (else)
-  int shift, member;      // log2 of the warps of a group, and which one this is
+  int pieces;             // that the block's warps take together
+  int shift, member;      // log2 of the warps of a group with the same ones, and which one this is
   int skip, tiles;        // the group's pieces: where they begin, how many (none: 0 or less)
 };
 
+constexpr int kBlockRows = 64;      // of W2 that a block of the second kernel has at once (by column: its own rule)
 constexpr int kTableBytes = (sizeof(FewTable) + 127) / 128 * 128;
 // Sums of the warps, for their owner to add up.
-template <int NT> struct RedShape {
+template <int F, int NT> struct RedShape {
   static constexpr int kTile = NT * 4 * 32 + 1;      // (off the banks of the tile before)
-  static constexpr int kBuffers = NT == 1 ? 2 : 1;   // (two where there is room: one barrier a tile)
-  static constexpr int kWarpFloats = kTiles * kTile, kBytes = (kWarps * kWarpFloats * 4 + 127) / 128 * 128;
+  static constexpr int kWarpFloats = FewShape<F>::kTiles * kTile, kBytes = (FewShape<F>::kWarps * kWarpFloats * 4 + 127) / 128 * 128;
   // Where the sums of row `row` (of a tile's 16) and column `col` are.
   static __device__ __forceinline__ int at(int tile, int row, int col) {
     return tile * kTile + ((col >> 3) * 4 + (row >> 3) * 2 + (col & 1)) * 32 + (row & 7) * 4 + ((col & 7) >> 1);
   }
 };
-// Tile and row (of the instruction) of the sums of a column of W13's part (gate or up of feature f of the 32), and of output c of the 64.
+// Tile and row (of the instruction) of the sums of a warp's gate or up f, and of its output c.
 template <int F>
 __device__ __forceinline__ int2 sums_of(int f, bool up, bool pairs) {
   if (!by_column(F)) {
@@ -741,39 +739,41 @@ __device__ __forceinline__ int2 sums_of(int c) {
   return by_column(F) ? make_int2((c & 7) >> 1, (c >> 3) + (c & 1 ? 8 : 0)) : make_int2(c >> 4, (c & 8) + g_of(c & 7));
 }
 // A warp's sums to its place.
-template <int NT>
-__device__ __forceinline__ void store_sums(float* red, const float (&acc)[kTiles][NT][4]) {
-  float* const to = red + (threadIdx.x >> 5) * RedShape<NT>::kWarpFloats + (threadIdx.x & 31);
+template <int F, int NT>
+__device__ __forceinline__ void store_sums(float* red, const float (&acc)[FewShape<F>::kTiles][NT][4]) {
+  float* const to = red + (threadIdx.x >> 5) * RedShape<F, NT>::kWarpFloats + (threadIdx.x & 31);
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i)
+  for (int i = 0; i < FewShape<F>::kTiles; ++i)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) to[i * RedShape<NT>::kTile + (n * 4 + c) * 32] = acc[i][n][c];
+      for (int c = 0; c < 4; ++c) to[i * RedShape<F, NT>::kTile + (n * 4 + c) * 32] = acc[i][n][c];
 }
 // Shared memory: the rings, barriers, zeros, flags, the table, scales in the rings, sums, the panel.
 template <int F> struct FewSmem {
   using S = FewShape<F>;
-  static constexpr int kBars = kWarps * S::kRing, kZeros = kBars + 256, kFlags = kZeros + 64, kTable = kFlags + 64;
-  static constexpr int kScales = kTable + kTableBytes, kRest = (kScales + kWarps * S::kRingScales + 127) / 128 * 128;
-  static_assert(kWarps * S::kDepth * 8 <= 256, "barriers");
+  static constexpr int kBars = S::kWarps * S::kRing, kZeros = kBars + 256, kFlags = kZeros + 64, kTable = kFlags + 64;
+  static constexpr int kScales = kTable + kTableBytes, kRest = (kScales + S::kWarps * S::kRingScales + 127) / 128 * 128;
+  static_assert(S::kWarps * S::kDepth * 8 <= 256, "barriers");
 };
 template <int F, int NT> struct UpShape {
-  static constexpr int kSums = RedShape<NT>::kBuffers * RedShape<NT>::kBytes;
+  static constexpr int kSums = RedShape<F, NT>::kBytes;
   static constexpr int kFixed = FewSmem<F>::kRest + kSums;
 };
 template <int F> struct DownShape {
   static constexpr int kFixed = FewSmem<F>::kRest;
 };
 
+// ---- the first kernel where weights are stored by column ---------------------------------------
 // h[row] = act(W13 x + b13).  The features of all active experts, in pieces of eight (a tile's rows: eight gates and their
-// eight ups), are dealt out evenly to the blocks, and within a block to groups of warps; the warps of a group take the
-// steps of its tiles in turn and add their sums up in shared memory.
+// eight ups), are dealt out evenly to the blocks.  Within a block all warps work side by side, so that rows of k are read in
+// long runs; where fewer pieces are left than warps times tiles several have the same ones, take their steps in turn and add
+// their sums up in shared memory.
 template <int F, int NT>
-__global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLaunch launch, const __grid_constant__ CUtensorMap map,
-                                                           const __grid_constant__ CUtensorMap piece_map) {
+__global__ void __launch_bounds__(FewShape<F>::kThreads, 1) few_up_columns_kernel(FewParams p, FewLaunch launch, const __grid_constant__ CUtensorMap map) {
   using S = FewShape<F>;
   using M = FewSmem<F>;
+  constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kTiles = S::kTiles, kRows = S::kRows;
   extern __shared__ __align__(1024) uint8_t smem[];
   FewTable& table = *reinterpret_cast<FewTable*>(smem + M::kTable);
   uint8_t* const zeros = smem + M::kZeros;                                // a token's values where there is no token
@@ -785,7 +785,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
   if (tid == 0) {
     *gave_up = 0;
     ptx::prefetch_tensormap(&map);
-    if (!by_column(F)) ptx::prefetch_tensormap(&piece_map);
   }
   pdl_wait();
   pdl_trigger();
@@ -805,12 +804,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
     if (whole) fill_tokens<F>(panel, scales_after(panel, p.tokens), p.x, p.hidden, (1u << p.tokens) - 1u, k8, launch.f16, warp - 1, kWarps - 1);
   }
   __syncthreads();
-  // (by column: blocks begin and end at whole 32-byte sectors, at whole tiles where there are enough)
-  const uint32_t unit = !by_column(F) || per_expert % 2 ? 1 : per_expert % 4 || table.active * per_expert < 16 * gridDim.x ? 2 : 4;
+  // (blocks begin and end at whole 32-byte sectors, at whole tiles where there are enough)
+  const uint32_t unit = per_expert % 2 ? 1 : per_expert % 4 || table.active * per_expert < 16 * gridDim.x ? 2 : 4;
   const uint32_t all = (uint32_t)(table.active * per_expert) / unit;     // (times the blocks below 2^32: takes_mma)
   const int begin = (int)(all * blockIdx.x / gridDim.x * unit), end = (int)(all * (blockIdx.x + 1) / gridDim.x * unit);
   const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
-  const FewOrder order = pairs ? row_order() : halves_order();
 
 #pragma unroll 1
   for (int from = begin; from < end;) {
@@ -829,25 +827,11 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         }
       }
     }
-    // Warps of a group: few where there are many tiles, as every tile's sums cost a barrier of the group; many where there
-    // are few, so that all have work and end together.  Both kernels, 1 / 2 / 4 / 8 warps, us: 62 pieces a block (MXFP4, 23
-    // steps) 90.5 / 87.0 / 89.1 / 92.7; 53 (fp8, 32 steps) 102 / 99.7 / 100 / 108; 22 (fp8, 112 steps) 151 / 136 / 125 / 126; 14
-    // (the same) 105 / 84 / 76 / 73; 10 (MXFP4) 31.4 / 29.1 / 29.8 / 29.3.
-    const int shift = to - from >= 40 ? 1 : to - from >= 18 ? 2 : 3;
-    // Groups have a stretch of the pieces each.  By column all warps work side by side instead, so that rows of k are read in
-    // long runs, and where fewer pieces are left than warps times tiles several have the same ones.
-    const int my_from = by_column(F) ? from : from + (((to - from) * (warp >> shift) << shift) / kWarps);
-    const int my_to = by_column(F) ? to : from + (((to - from) * ((warp >> shift) + 1) << shift) / kWarps);
     auto place = [&](FewPlace& at) {
-      const int left = min(per_expert - at.u, my_to - at.at);
-      at.shift = shift;
-      at.skip = 0;
-      at.pieces = min(kTiles, left);
-      if constexpr (by_column(F)) {
-        at.shift = left > 4 * kTiles ? 0 : left > 2 * kTiles ? 1 : left > kTiles ? 2 : 3;
-        at.pieces = min(kWarps * kTiles, left);
-        at.skip = (warp >> at.shift) * kTiles;
-      }
+      const int left = min(per_expert - at.u, to - at.at);
+      at.shift = left > 4 * kTiles ? 0 : left > 2 * kTiles ? 1 : left > kTiles ? 2 : 3;
+      at.pieces = min(kWarps * kTiles, left);
+      at.skip = (warp >> at.shift) * kTiles;
       at.member = warp & ((1 << at.shift) - 1);
       at.tiles = min(kTiles, at.pieces - at.skip);
     };
@@ -855,13 +839,13 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       at.at += at.pieces;
       at.u += at.pieces;
       if (at.u == per_expert) { at.u = 0; ++at.a; }
-      if (at.at < my_to) place(at);
+      if (at.at < to) place(at);
     };
     FewPlace start;
-    start.at = my_from;
-    start.a = my_from / per_expert;
-    start.u = my_from - start.a * per_expert;
-    if (my_from < my_to) place(start);
+    start.at = from;
+    start.a = from / per_expert;
+    start.u = from - start.a * per_expert;
+    place(start);
 
 #pragma unroll 1
     for (uint32_t rest = tokens; rest;) {
@@ -875,55 +859,234 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
       bool found = false;
       FewRows fetch;
       auto copy_next = [&](int slot) {
-        while (next.at < my_to && (s >= steps || !found)) {
+        while (next.at < to && (s >= steps || !found)) {
           if (found || next.tiles <= 0) {     // (without tiles for this group: on to the next ones)
-            s -= found ? steps : 0;
             place_after(next);
-            if (by_column(F)) s = next.member;
+            s = next.member;
             found = false;
-            if (next.at >= my_to || next.tiles <= 0) continue;
+            if (next.at >= to || next.tiles <= 0) continue;
           }
           found = true;
-          fetch.tiles = next.tiles;
           fetch.e = table.expert[next.a];
           fetch.row = (next.u + next.skip) * 8;
-#pragma unroll
-          for (int j = 0; j < kRows / 32; ++j) {
-            if (by_column(F)) break;
-            // gates in the first half of the places, ups in the second; pairs as they are
-            const int place = j * 32 + lane, up = place >= kRows / 2, fs = place % (kRows / 2);
-            fetch.there[j] = pairs ? place < 16 * fetch.tiles : fs < 8 * fetch.tiles;
-            const int n = pairs ? 2 * fetch.row + place : fetch.row + fs + up * p.inter;
-            fetch.s[j] = scales_of<F>(m, layout, fetch.e, fetch.there[j] ? n : 0);
-          }
         }
-        if (next.at < my_to) {
+        if (next.at < to) {
           if (lane == 0) {
-            const uint32_t to = ring.slots + slot * S::kSlotBytes, bar = ring.bars + slot * 8;
-            const int x = by_column(F) ? fetch.row : s * 128, y = by_column(F) ? s * S::kK : fetch.row;
+            const uint32_t to_slot = ring.slots + slot * S::kSlotBytes, bar = ring.bars + slot * 8;
             ptx::fence_proxy_async();      // (the warp has read what was there)
-            if (by_column(F) || fetch.tiles == kTiles) {
-              ptx::mbar_expect_tx_s(bar, S::kSlotBytes);
-              if (pairs) {
-                ptx::tma_load_3d_s(to, &map, bar, by_column(F) ? 2 * x : x, by_column(F) ? y : 2 * y, fetch.e);
-              } else {
-                ptx::tma_load_3d_s(to, &map, bar, x, y, fetch.e);
-                ptx::tma_load_3d_s(to + S::kSlotBytes / 2, &map, bar, by_column(F) ? p.inter + x : x, by_column(F) ? y : p.inter + y, fetch.e);
-              }
-            } else {                       // the tiles that there are, one by one
-              ptx::mbar_expect_tx_s(bar, fetch.tiles * 2048);
-              for (int i = 0; i < fetch.tiles; ++i) {
-                if (pairs) {
-                  ptx::tma_load_3d_s(to + i * 2048, &piece_map, bar, x, 2 * (y + 8 * i), fetch.e);
-                } else {
-                  ptx::tma_load_3d_s(to + i * 1024, &piece_map, bar, x, y + 8 * i, fetch.e);
-                  ptx::tma_load_3d_s(to + 4096 + i * 1024, &piece_map, bar, x, p.inter + y + 8 * i, fetch.e);
-                }
-              }
+            ptx::mbar_expect_tx_s(bar, S::kSlotBytes);
+            if (pairs) {
+              ptx::tma_load_3d_hint_s(to_slot, &map, bar, 2 * fetch.row, s * S::kK, fetch.e, ring.once);
+            } else {
+              ptx::tma_load_3d_hint_s(to_slot, &map, bar, fetch.row, s * S::kK, fetch.e, ring.once);
+              ptx::tma_load_3d_hint_s(to_slot + S::kSlotBytes / 2, &map, bar, p.inter + fetch.row, s * S::kK, fetch.e, ring.once);
             }
           }
-          if (!by_column(F)) copy_scales<F>(ring.scales + slot * S::kSlotScales, fetch, layout, s);
           s += 1 << next.shift;
+        }
+      };
+#pragma unroll 1
+      for (int i = 0; i < S::kDepth; ++i) copy_next((ring.slot + i) % S::kDepth);
+      const int rows = __popc(now);
+      if (!whole) {
+        fill_tokens<F>(panel, scales_after(panel, rows), p.x, p.hidden, now, k8, launch.f16, warp, kWarps);
+        __syncthreads();
+      }
+
+#pragma unroll 1
+      for (FewPlace at = start; at.at < to; place_after(at)) {
+        const int tiles = at.tiles, group = 1 << at.shift, a = at.a;
+        if (tiles <= 0) continue;
+        const uint32_t mine = table.tokens[a] & now;
+        FewTokens x[NT];
+        find_tokens<NT>(x, mine, now, smem_at(panel), smem_at(scales_after(panel, rows)), smem_at(zeros), rows);
+        float acc[kTiles][NT][4] = {};
+#pragma unroll 1
+        for (int cs = at.member; cs < steps; cs += group) take_step<F, NT, 1>(acc, ring, tiles, row_order(), !pairs, layout, x, cs, copy_next);
+        // The tile's sums: a lane has a feature, the members take the tokens in turn.
+        store_sums<F, NT>(red, acc);
+        // (a barrier for each group of each size)
+        const int barrier = (kWarps >> at.shift) + (warp >> at.shift);
+        if (group > 1) group_sync(barrier, group * 32);
+        else __syncwarp();
+        const int i = lane >> 3, f = (at.u + at.skip + i) * 8 + (lane & 7);
+        const int2 at_gate = sums_of<F>(lane, false, pairs), at_up = sums_of<F>(lane, true, pairs);
+        int turn = 0;
+        for (uint32_t left = mine; left; left &= left - 1, ++turn) {
+          if ((turn & (group - 1)) != at.member) continue;
+          const int col = __ffs(left) - 1, row = table.first_row[a] + rank_below(table.tokens[a], col);
+          if (i < tiles) {
+            const float* from_red = red + (warp - at.member) * RedShape<F, NT>::kWarpFloats;
+            float gate = 0.f, up = 0.f;
+            for (int w = 0; w < group; ++w) {
+              gate += from_red[w * RedShape<F, NT>::kWarpFloats + RedShape<F, NT>::at(at_gate.x, at_gate.y, col)];
+              up += from_red[w * RedShape<F, NT>::kWarpFloats + RedShape<F, NT>::at(at_up.x, at_up.y, col)];
+            }
+            if (m.bias) {
+              const int64_t at = (int64_t)table.expert[a] * m.n;
+              gate += load16(m.bias, at + (pairs ? 2 * f : f), launch.f16);
+              up += load16(m.bias, at + (pairs ? 2 * f + 1 : p.inter + f), launch.f16);
+            }
+            p.h[(int64_t)row * p.inter + f] = gated_once(p.act, p.alpha, p.limit, p.clamp, gate, up);
+          }
+        }
+        // the sums' place is free again
+        if (group > 1) group_sync(barrier, group * 32);
+        else __syncwarp();
+      }
+      __syncthreads();   // the panel is free again
+    }
+    from = to;
+  }
+}
+
+// ---- the first kernel where weights are stored by output feature ------------------------------
+// Columns of a partial sum's entry: 36 floats, so that a store's 32 lanes (eight rows of four columns) hit 32 banks.
+constexpr int kEntryColumn = 36;
+template <int F, int NT> struct UpRowsShape {
+  static constexpr int kSums = NT == 1 ? 24 * 1024 : 36 * 1024;
+  static constexpr int kFixed = FewSmem<F>::kRest + kSums;
+  static_assert(kSums >= (FewShape<F>::kWarps + 1) * kEntryColumn * 4 * 8 * NT, "a set with all its tokens");
+};
+
+// A block's features of one pass: pieces of eight (a tile's rows: eight gates and their eight ups), up to two of one expert to a
+// set, which a warp takes at once.
+struct FewPieces {
+  int per_expert, from, to;     // pieces of an expert; first and last of the pass
+  int a0, u0, sets0, per;       // where the first one is; sets of the first expert and of every other one
+  __device__ __forceinline__ FewPieces(int per_expert, int from, int to) : per_expert(per_expert), from(from), to(to) {
+    a0 = from / per_expert;
+    u0 = from - a0 * per_expert;
+    sets0 = (min(per_expert - u0, to - from) + 1) >> 1;
+    per = (per_expert + 1) >> 1;
+  }
+  __device__ __forceinline__ int sets() const {
+    const int rest = to - from - (per_expert - u0);     // behind the first expert
+    if (rest <= 0) return sets0;
+    const int experts = rest / per_expert;
+    return sets0 + experts * per + ((rest - experts * per_expert + 1) >> 1);
+  }
+  // Set j: its expert (of the active ones), its first piece there, and how many it has.
+  __device__ __forceinline__ void find(int j, int& a, int& u, int& tiles) const {
+    a = a0;
+    u = u0 + 2 * j;
+    int end = per_expert;
+    if (j >= sets0) {
+      const int i = (j - sets0) / per;
+      a = a0 + 1 + i;
+      u = 2 * (j - sets0 - i * per);
+    }
+    end = min(end, to - (from - u0) - (a - a0) * per_expert);
+    tiles = min(2, end - u);
+  }
+};
+
+// h[row] = act(W13 x + b13).  The pieces of all active experts are dealt out evenly to the blocks.  A block's sets times the
+// steps of a row are one list, of which each warp takes a stretch; what it adds up of a set goes into shared memory, and
+// at the end of the pass all that there is of a set is added up in the warps' order: one barrier a pass instead of one a set (which cost
+// 4 to 10 us of the kernel).
+template <int F, int NT>
+__global__ void __launch_bounds__(FewShape<F>::kThreads, 1) few_up_rows_kernel(FewParams p, FewLaunch launch, const __grid_constant__ CUtensorMap map,
+                                                                               const __grid_constant__ CUtensorMap piece_map) {
+  using S = FewShape<F>;
+  using M = FewSmem<F>;
+  constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kTiles = S::kTiles;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  FewTable& table = *reinterpret_cast<FewTable*>(smem + M::kTable);
+  uint8_t* const zeros = smem + M::kZeros;                                // a token's values where there is no token
+  int* const gave_up = reinterpret_cast<int*>(smem + M::kFlags);
+  float* const sums = reinterpret_cast<float*>(smem + M::kRest);
+  uint8_t* const panel = smem + UpRowsShape<F, NT>::kFixed;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  FewRing ring = make_ring<F>(smem, smem + M::kScales, reinterpret_cast<uint64_t*>(smem + M::kBars), gave_up, launch.status);
+  if (tid == 0) {
+    *gave_up = 0;
+    ptx::prefetch_tensormap(&map);
+    ptx::prefetch_tensormap(&piece_map);
+  }
+  pdl_wait();
+  pdl_trigger();
+  const FewMatrix& m = p.w13;
+  const FewLayout layout(m, F, launch.f16);
+  const int steps = (p.hidden + S::kK - 1) / S::kK, per_expert = p.inter / 8;
+  const int most = launch.panel_bytes / (steps * S::kPanelBytes(1)); // rows that the panel holds
+  const bool whole = most >= p.tokens;                            // all tokens
+  const int k8 = steps * (S::kK / 8);
+  auto scales_after = [&](uint8_t* at, int rows) { return reinterpret_cast<float*>(at + rows * steps * (S::kK * 2)); };
+  if (warp == 0) {
+    build_table<false>(table, p);
+  } else {
+    if (tid < 48) reinterpret_cast<uint32_t*>(zeros)[tid - 32] = 0;
+    if (blockIdx.x == 0)   // (the second kernel counts from there)
+      for (int i = tid - 32; i < kFewMaxColumns; i += kThreads - 32) launch.arrived[i] = 0;
+    if (whole) fill_tokens<F>(panel, scales_after(panel, p.tokens), p.x, p.hidden, (1u << p.tokens) - 1u, k8, launch.f16, warp - 1, kWarps - 1);
+  }
+  __syncthreads();
+  const uint32_t all = (uint32_t)(table.active * per_expert);     // (times the blocks below 2^32: takes_mma)
+  const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+  const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
+  const FewOrder order = pairs ? row_order() : halves_order();
+
+#pragma unroll 1
+  for (int from = begin; from < end;) {
+    // As many experts as have their tokens in the panel at once and their sums in shared memory; one with more tokens than
+    // the panel holds goes through its features again with the rest of them.
+    int to = from, deep = 0;       // deep: the most tokens that an expert has
+    uint32_t tokens = 0;
+    for (int a = from / per_expert; to < end; ++a) {
+      const uint32_t with = tokens | table.tokens[a];
+      const int n = max(deep, min(__popc(table.tokens[a]), most));
+      const int room = UpRowsShape<F, NT>::kSums / (kEntryColumn * 4 * n) - kWarps;             // sets
+      if (tokens && (__popc(with) > most || room <= (to - from) / 2 + a - from / per_expert)) break;
+      tokens = with;
+      deep = n;
+      // (an expert before this one may have left a set with one piece, and this one may)
+      to = min(min(end, (a + 1) * per_expert), from + 2 * (room - (a - from / per_expert)));
+      if (to < min(end, (a + 1) * per_expert)) break;
+    }
+    if (whole) tokens = (1u << p.tokens) - 1u;
+    const FewPieces pieces(per_expert, from, to);
+    const int total = pieces.sets() * steps;
+    const int workers = min(kWarps, total);
+    const int pos0 = total * min(warp, workers) / workers, pos1 = total * min(warp + 1, workers) / workers;
+    const int j0 = pos0 / steps, s0 = pos0 - j0 * steps;
+
+#pragma unroll 1
+    for (uint32_t rest = tokens; rest;) {
+      uint32_t now = rest;
+      while (__popc(now) > most) now &= ~(1u << (31 - __clz(now)));
+      rest &= ~now;
+
+      // The ring begins to fill: the set and step that are fetched next, and how many after them.
+      FewRows fetch;
+      int fetch_j = j0, fetch_s = s0, left = pos1 - pos0;
+      bool found = false;
+      auto copy_next = [&](int slot) {
+        if (left > 0) {
+          if (fetch_s == steps) { fetch_s = 0; ++fetch_j; found = false; }
+          if (!found) {
+            int a;
+            pieces.find(fetch_j, a, fetch.row, fetch.tiles);
+            fetch.row *= 8;
+            fetch.e = table.expert[a];
+            // gates in the first half of the places, ups in the second; pairs as they are
+            const int up = lane >= S::kRows / 2, fs = lane % (S::kRows / 2);
+            fetch.there = pairs ? lane < 16 * fetch.tiles : fs < 8 * fetch.tiles;
+            const int n = pairs ? 2 * fetch.row + lane : fetch.row + fs + up * p.inter;
+            fetch.s = scales_of<F>(m, layout, fetch.e, fetch.there ? n : 0);
+            found = true;
+          }
+          if (lane == 0) {
+            const uint32_t at = ring.slots + slot * S::kSlotBytes, bar = ring.bars + slot * 8;
+            const CUtensorMap* from_map = fetch.tiles == kTiles ? &map : &piece_map;
+            ptx::fence_proxy_async();      // (the warp has read what was there)
+            ptx::mbar_expect_tx_s(bar, fetch.tiles * 2048);
+            ptx::tma_load_3d_hint_s(at, from_map, bar, fetch_s * 128, pairs ? 2 * fetch.row : fetch.row, fetch.e, ring.once);
+            if (!pairs) ptx::tma_load_3d_hint_s(at + S::kSlotBytes / 2, from_map, bar, fetch_s * 128, p.inter + fetch.row, fetch.e, ring.once);
+          }
+          copy_scales<F>(ring.scales + slot * S::kSlotScales, fetch, layout, fetch_s);
+          ++fetch_s;
+          --left;
         }
         copies_end();
       };
@@ -935,55 +1098,70 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(FewParams p, FewLau
         __syncthreads();
       }
 
-      int cs = start.member, tile = 0;
 #pragma unroll 1
-      for (FewPlace at = start; at.at < my_to; place_after(at)) {
-        const int tiles = at.tiles, group = 1 << at.shift, a = at.a;
-        if (tiles <= 0) continue;
-        if (by_column(F)) cs = at.member;
+      for (int pos = pos0, j = j0, s = s0; pos < pos1; ++j, s = 0) {
+        int a, u, tiles;
+        pieces.find(j, a, u, tiles);
         const uint32_t mine = table.tokens[a] & now;
         FewTokens x[NT];
         find_tokens<NT>(x, mine, now, smem_at(panel), smem_at(scales_after(panel, rows)), smem_at(zeros), rows);
         float acc[kTiles][NT][4] = {};
+        const int stop = min(steps, s + pos1 - pos);
+        pos += stop - s;
 #pragma unroll 1
-        for (; cs < steps; cs += group) take_step<F, NT, 1>(acc, ring, tiles, order, !pairs, layout, x, cs, copy_next);
-        cs -= steps;
-        // The tile's sums: a lane has a feature, the members take the tokens in turn.
-        // (by column the warps of a group need not have had the same number of tiles)
-        float* const sums = red + (RedShape<NT>::kBuffers == 2 && !by_column(F) && (tile & 1) ? RedShape<NT>::kBytes / 4 : 0);
-        store_sums<NT>(sums, acc);
-        // (a barrier for each group of each size)
-        const int barrier = by_column(F) ? (kWarps >> at.shift) + (warp >> at.shift) : 1 + (warp >> at.shift);
-        if (group > 1) group_sync(barrier, group * 32);
-        else __syncwarp();
-        const int i = lane >> 3, f = (at.u + at.skip + i) * 8 + (lane & 7);
-        const int2 at_gate = sums_of<F>(lane, false, pairs), at_up = sums_of<F>(lane, true, pairs);
-        int turn = by_column(F) ? 0 : tile;
-        for (uint32_t left = mine; left; left &= left - 1, ++turn) {
-          if ((turn & (group - 1)) != at.member) continue;
-          const int col = __ffs(left) - 1, row = table.first_row[a] + rank_below(table.tokens[a], col);
-          if (i < tiles) {
-            const float* from_red = sums + (warp - at.member) * RedShape<NT>::kWarpFloats;
-            float gate = 0.f, up = 0.f;
-            for (int w = 0; w < group; ++w) {
-              gate += from_red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(at_gate.x, at_gate.y, col)];
-              up += from_red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(at_up.x, at_up.y, col)];
+        for (; s < stop; ++s) take_step<F, NT, 1>(acc, ring, tiles, order, !pairs, layout, x, s, copy_next);
+        // sets and warps begin a new entry each
+        float* const entry = sums + (j + warp) * (kEntryColumn * deep);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int token = 8 * n + 2 * (lane & 3) + c;
+            if (!((mine >> token) & 1)) continue;
+            float* const to_entry = entry + rank_below(mine, token) * kEntryColumn + (lane >> 2);
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+              to_entry[i * 16] = acc[i][n][c];
+              to_entry[i * 16 + 8] = acc[i][n][c + 2];
             }
-            if (m.bias) {
-              const int64_t at = (int64_t)table.expert[a] * m.n;
-              gate += load16(m.bias, at + (pairs ? 2 * f : f), launch.f16);
-              up += load16(m.bias, at + (pairs ? 2 * f + 1 : p.inter + f), launch.f16);
-            }
-            p.h[(int64_t)row * p.inter + f] = gated_once(p.act, p.alpha, p.limit, p.clamp, gate, up);
           }
-        }
-        // the sums' place is free again: the next tile has another one, and that one's barrier is behind this one's reads
-        if ((RedShape<NT>::kBuffers == 1 || by_column(F)) && group > 1) group_sync(barrier, group * 32);
-        else __syncwarp();
-        ++tile;
       }
       copies_wait<0>();
-      __syncthreads();   // the panel is free again
+      __syncthreads();   // the sums are complete, and the panel is free again
+      // A warp has a set, a lane one of its 16 features, for one token of two.
+#pragma unroll 1
+      for (int j = warp; j * steps < total; j += kWarps) {
+        int a, u, tiles;
+        pieces.find(j, a, u, tiles);
+        const int f = 8 * u + (lane & 15), first = table.first_row[a];
+        const uint32_t have = table.tokens[a], mine = have & now;
+        // the warps that had the set's first and last step
+        const int w0 = (workers * (j * steps + 1) - 1) / total, w1 = (workers * (j + 1) * steps - 1) / total;
+        if ((lane & 15) >= 8 * tiles) continue;
+        float bias_gate = 0.f, bias_up = 0.f;
+        if (m.bias) {
+          const int64_t at = (int64_t)table.expert[a] * m.n;
+          bias_gate = load16(m.bias, at + (pairs ? 2 * f : f), launch.f16);
+          bias_up = load16(m.bias, at + (pairs ? 2 * f + 1 : p.inter + f), launch.f16);
+        }
+        const int2 at_gate = sums_of<F>(lane & 15, false, pairs), at_up = sums_of<F>(lane & 15, true, pairs);
+        const float* const gates = sums + (at_gate.x * 16 + at_gate.y), * const ups = sums + (at_up.x * 16 + at_up.y);
+        uint32_t later = mine;
+        if (lane >= 16) later &= later - 1;
+        for (int rank = lane >> 4; later; rank += 2) {
+          const int token = __ffs(later) - 1;
+          float gate = bias_gate, up = bias_up;
+          for (int w = w0; w <= w1; ++w) {
+            const int at = ((j + w) * deep + rank) * kEntryColumn;
+            gate += gates[at];
+            up += ups[at];
+          }
+          p.h[(int64_t)(first + rank_below(have, token)) * p.inter + f] = gated_once(p.act, p.alpha, p.limit, p.clamp, gate, up);
+          later &= later - 1;
+          later &= later - 1;
+        }
+      }
+      if (rest || to < end) __syncthreads();   // the sums' place is free again
     }
     from = to;
   }
@@ -1013,9 +1191,10 @@ __device__ __noinline__ float weighted_bias(const FewTable& table, const FewMatr
 // Of the blocks with the same rows the last one to be done adds the partial sums up, in their order.  By column a block has
 // up to four times 64, side by side by warps that share their steps' values of h.
 template <int F, int NT>
-__global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewLaunch launch, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(FewShape<F>::kThreads, 1) few_down_kernel(FewParams p, FewLaunch launch, const __grid_constant__ CUtensorMap map) {
   using S = FewShape<F>;
   using M = FewSmem<F>;
+  constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kTiles = S::kTiles, kRows = S::kRows;
   extern __shared__ __align__(1024) uint8_t smem[];
   FewTable& table = *reinterpret_cast<FewTable*>(smem + M::kTable);
   uint8_t* const zeros = smem + M::kZeros;
@@ -1038,8 +1217,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
   const int steps = (p.inter + S::kK - 1) / S::kK;
   const int columns = gridDim.x / launch.splits, column = blockIdx.x % columns, split = blockIdx.x / columns;
   // (by column: whole 64 of them, one block's after the other's)
-  const int side = by_column(F) ? launch.side : 1, members = kWarps / side, member = warp / side, mine_side = warp % side;
-  const int block_rows = side * kRows;
+  const int side = launch.side, members = kWarps / side, member = warp / side, mine_side = warp % side;
+  const int warp_rows = launch.box, block_rows = side * warp_rows;
   const int row_begin = by_column(F) ? column * block_rows : (int)((uint32_t)p.hidden * column / columns);
   const int row_end = by_column(F) ? p.hidden : (int)((uint32_t)p.hidden * (column + 1) / columns);
   const uint32_t total = (uint32_t)(table.active * steps);
@@ -1076,11 +1255,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
     if (launch.f16) reinterpret_cast<__half*>(p.out)[to] = __float2half_rn(v);
     else reinterpret_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(v);
   };
-  for (int block_r0 = row_begin; block_r0 < row_end || !waited; block_r0 += by_column(F) ? columns * block_rows : kRows) {
-    const int r0 = block_r0 + mine_side * kRows, rows_here = max(0, min(kRows, row_end - r0)), tiles = (rows_here + 15) / 16;
+  for (int block_r0 = row_begin; block_r0 < row_end || !waited; block_r0 += by_column(F) ? columns * block_rows : block_rows) {
+    const int r0 = block_r0 + mine_side * warp_rows, rows_here = max(0, min(warp_rows, row_end - r0)), tiles = (rows_here + 15) / 16;
     FewRows fetch;
-#pragma unroll
-    for (int j = 0; j < kRows / 32; ++j) fetch.there[j] = j * 32 + lane < rows_here;
+    fetch.there = lane < rows_here;
     // The step that is fetched next, how many are left of this warp's stretch, and where the panel after that begins.
     int fetch_a = 0, fetch_s = 0, left = 0, panel_a = step_begin / steps, panel_s = step_begin - panel_a * steps;
     bool found = false;
@@ -1100,16 +1278,14 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
         if (fetch_s == steps) { fetch_s = 0; ++fetch_a; found = false; }
         if (!found) {
           fetch.e = table.expert[fetch_a];
-#pragma unroll
-          for (int j = 0; j < kRows / 32; ++j)
-            if (!by_column(F)) fetch.s[j] = scales_of<F>(m, layout, fetch.e, fetch.there[j] ? r0 + j * 32 + lane : r0);
+          if (!by_column(F)) fetch.s = scales_of<F>(m, layout, fetch.e, fetch.there ? r0 + lane : r0);
           found = true;
         }
         if (lane == 0) {
           const uint32_t bar = ring.bars + slot * 8;
           ptx::fence_proxy_async();        // (the warp has read what was there)
-          ptx::mbar_expect_tx_s(bar, launch.box * (by_column(F) ? 64 : 128));
-          ptx::tma_load_3d_s(ring.slots + slot * S::kSlotBytes, &map, bar, by_column(F) ? r0 : fetch_s * 128, by_column(F) ? fetch_s * S::kK : r0, fetch.e);
+          ptx::mbar_expect_tx_s(bar, warp_rows * (by_column(F) ? 64 : 128));
+          ptx::tma_load_3d_hint_s(ring.slots + slot * S::kSlotBytes, &map, bar, by_column(F) ? r0 : fetch_s * 128, by_column(F) ? fetch_s * S::kK : r0, fetch.e, ring.once);
         }
         if (!by_column(F)) copy_scales<F>(ring.scales + slot * S::kSlotScales, fetch, layout, fetch_s);
         ++fetch_s;
@@ -1120,12 +1296,14 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
 #pragma unroll 1
     for (int i = 0; i < S::kDepth; ++i) copy_next((ring.slot + i) % S::kDepth);
     // Biases while the ring fills, by the blocks with the first share (by column: when they are needed).
-    constexpr int kMine = kRows * B200MOE_FEW_TOKENS / kThreads;
+    constexpr int kMine = (B200MOE_FEW_TOKENS * kBlockRows + kThreads - 1) / kThreads;
+    const int block_rows_here = min(block_rows, row_end - block_r0), my_row = tid % kBlockRows, my_token = tid / kBlockRows;
     float bias[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      const int row = tid % kRows, token = tid / kRows + i * (kThreads / kRows);
-      bias[i] = !by_column(F) && m.bias && split == 0 && token < p.tokens && row < rows_here ? weighted_bias(table, m, p.topk, launch.f16, token, r0 + row) : 0.f;
+      const int token = my_token + i * (kThreads / kBlockRows);
+      bias[i] = !by_column(F) && m.bias && split == 0 && token < p.tokens && my_row < block_rows_here
+                    ? weighted_bias(table, m, p.topk, launch.f16, token, block_r0 + my_row) : 0.f;
     }
     if (!waited) {
       pdl_wait();
@@ -1188,7 +1366,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
       s0 = s1;
       __syncthreads();   // the panel is free again
     }
-    store_sums<NT>(red, out);
+    store_sums<F, NT>(red, out);
     copies_wait<0>();
     __syncthreads();
     auto put = [&](float v, int token, int row) {
@@ -1203,18 +1381,20 @@ __global__ void __launch_bounds__(kThreads, 1) few_down_kernel(FewParams p, FewL
         if (block_r0 + row >= row_end) continue;
         const int2 at = sums_of<F>(row % kRows);
         float v = m.bias && split == 0 ? weighted_bias(table, m, p.topk, launch.f16, token, block_r0 + row) : 0.f;
-        for (int w = row / kRows; w < kWarps; w += side) v += red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(at.x, at.y, token)];
+        for (int w = row / kRows; w < kWarps; w += side) v += red[w * RedShape<F, NT>::kWarpFloats + RedShape<F, NT>::at(at.x, at.y, token)];
         put(v, token, block_r0 + row);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        const int row = tid % kRows, token = tid / kRows + i * (kThreads / kRows);
-        if (row >= rows_here || token >= p.tokens) continue;
+        const int token = my_token + i * (kThreads / kBlockRows);
+        if (my_row >= block_rows_here || token >= p.tokens) continue;
+        const int which = my_row >= warp_rows ? 1 : 0;
+        const int2 at = sums_of<F>(my_row - which * warp_rows);
         float v = bias[i];
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) v += red[w * RedShape<NT>::kWarpFloats + RedShape<NT>::at(sums_of<F>(row).x, sums_of<F>(row).y, token)];
-        put(v, token, r0 + row);
+        for (int w = 0; w < kWarps / 2; ++w) v += red[(2 * w + which) * RedShape<F, NT>::kWarpFloats + RedShape<F, NT>::at(at.x, at.y, token)];
+        put(v, token, block_r0 + my_row);
       }
     }
     __syncthreads();

@@ -6,7 +6,8 @@
 // Weights are taken as they are stored; activations stay in 16 bits or more, sums in fp32.
 #include "common.cuh"
 #include "few_tokens.cuh"
-#include "few_tokens_nk.cuh"
+#include "few_tokens_columns.cuh"
+#include "few_tokens_rows.cuh"
 
 namespace b200moe {
 namespace {
@@ -101,7 +102,7 @@ int launch_simple(const FewParams& p, cudaStream_t st) {
   return B200MOE_OK;
 }
 
-// ---- weights by output feature ---------------------------------------------------------
+// ---- on the tensor cores ------------------------------------------------------------------
 constexpr int kMaxBlockSmem = 232448;
 
 // The attribute is set once per kernel and device, and always to the most that a block may have, so that calls with
@@ -126,7 +127,7 @@ struct FewWorkspace {
   FewWorkspace(int64_t tokens, int64_t topk, int64_t hidden, int64_t inter) {
     auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     arrived = up(tokens * topk * inter * sizeof(float));
-    part = arrived + kFewMaxColumns * sizeof(uint32_t);
+    part = arrived + kFewMaxBlocks * sizeof(uint32_t);
     bytes = part + up((size_t)splits(hidden, kFewMaxBlocks) * tokens * hidden * sizeof(float));
   }
   // Shares of the second kernel's steps: as many as make `ctas` blocks with up to `rows` rows each.
@@ -136,63 +137,96 @@ struct FewWorkspace {
   }
 };
 
-// The map of a matrix for loads of `box` rows (by column: columns) of a step.
+// The map of a matrix for loads of `box` rows (by column: columns) of a step, and that of its scales (4 bits).
 template <int F>
 int few_map(CUtensorMap* map, const FewMatrix& m, int experts, int box) {
-  if (by_column(F)) {
+  if constexpr (by_column(F)) {
     const cuuint64_t dims[3] = {(cuuint64_t)m.n, (cuuint64_t)m.k, (cuuint64_t)experts};
     const cuuint64_t strides[2] = {(cuuint64_t)m.n * 2, (cuuint64_t)m.n * m.k * 2};
-    const cuuint32_t boxes[3] = {(cuuint32_t)box, (cuuint32_t)FewShape<F>::kK, 1};
+    const cuuint32_t boxes[3] = {(cuuint32_t)box, (cuuint32_t)ColumnShape<F>::kK, 1};
     return encode_map(map, F == kFewBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, m.w, dims, strides, boxes,
                       box == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+  } else {
+    const cuuint64_t row = F == kFewFp8 ? m.k : m.k / 2;
+    const cuuint64_t dims[3] = {row, (cuuint64_t)m.n, (cuuint64_t)experts};
+    const cuuint64_t strides[2] = {row, row * m.n};
+    const cuuint32_t boxes[3] = {128, (cuuint32_t)box, 1};
+    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, m.w, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_128B);
   }
-  const cuuint64_t row = F == kFewFp8 ? m.k : m.k / 2;
-  const cuuint64_t dims[3] = {row, (cuuint64_t)m.n, (cuuint64_t)experts};
-  const cuuint64_t strides[2] = {row, row * m.n};
-  const cuuint32_t boxes[3] = {128, (cuuint32_t)box, 1};
-  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, m.w, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int few_scale_map(CUtensorMap* map, const FewMatrix& m, int experts, int box) {
+  const cuuint64_t words = few_scale_words(m.format, m.group, m.k);
+  const cuuint64_t dims[3] = {(cuuint64_t)m.n, words, (cuuint64_t)experts};
+  const cuuint64_t strides[2] = {(cuuint64_t)m.n * 4, (cuuint64_t)m.n * 4 * words};
+  const int step = m.format == B200MOE_W_MXFP4_NK ? 2 : m.group == 32 ? 4 : m.group == 64 ? 2 : 1;       // words of 256 values
+  const cuuint32_t boxes[3] = {(cuuint32_t)box, (cuuint32_t)step, 1};
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, m.scale, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+int at_least(int a, int b) { return a < b ? b : a; }
+
+// The kernels' shared memory: what they always need, and a panel of tokens or h.
 template <int F, int NT>
-int launch_mma(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
-  constexpr int k = FewShape<F>::kK, up_fixed = by_column(F) ? UpShape<F, NT>::kFixed : UpRowsShape<F, NT>::kFixed, up_room = kMaxBlockSmem - up_fixed, down_room = kMaxBlockSmem - DownShape<F>::kFixed;
-  const int up_row = (p.hidden + k - 1) / k * FewShape<F>::kPanelBytes(1);
-  const int down_row = (p.inter + k - 1) / k * FewShape<F>::kPanelBytes(FewShape<F>::kTerms);
+int launch_columns(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
+  using S = ColumnShape<F>;
+  constexpr int up_fixed = UpColumnsShape<F, NT>::kFixed, up_room = kMaxBlockSmem - up_fixed, down_room = kMaxBlockSmem - S::kRest;
+  const int up_row = (p.hidden + S::kK - 1) / S::kK * S::kPanelBytes(1), down_row = (p.inter + S::kK - 1) / S::kK * S::kPanelBytes(S::kTerms);
+  static_assert(up_room >= 16384 / S::kK * S::kPanelBytes(1), "a token");
   l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
-  int columns;
-  if (by_column(F)) {
-    constexpr int kRows = FewShape<F>::kRows;
-    l.box = kRows;
-    l.side = p.hidden > 2 * kRows ? 4 : p.hidden > kRows ? 2 : 1;
-    columns = (p.hidden + l.side * kRows - 1) / (l.side * kRows);
-    if (columns > ctas) columns = ctas;
-    l.splits = ctas / columns;
-  } else {
-    l.splits = FewWorkspace::splits(p.hidden, ctas, kBlockRows);
-    columns = ctas / l.splits;
-    // a block's rows in as few turns as they need, and halved in each
-    const int rows = (p.hidden + columns - 1) / columns, turns = (rows + kBlockRows - 1) / kBlockRows;
-    l.side = 2;
-    l.box = (rows + 2 * turns - 1) / (2 * turns);
-  }
-  // Loads: rows of 128 bytes (codes) of 32 gates, 32 ups or 64 features in pairs, and of a piece's; by column 32 rows of the
-  // same columns.  In the second kernel the rows that a block has, by column 64.
-  const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
-  CUtensorMap up_map, piece_map, down_map;
-  int rc = few_map<F>(&up_map, p.w13, p.experts, FewShape<F>::kRows / (pairs ? 1 : 2));
-  if (rc == B200MOE_OK) rc = by_column(F) ? B200MOE_OK : few_map<F>(&piece_map, p.w13, p.experts, pairs ? 16 : 8);
-  if (rc == B200MOE_OK) rc = few_map<F>(&down_map, p.w2, p.experts, l.box);
-  if (rc != B200MOE_OK) return rc;
-  if constexpr (by_column(F))
-    rc = launch_block_per_sm<few_up_columns_kernel<F, NT>>("few_up_columns_kernel", ctas, FewShape<F>::kThreads, up_fixed + l.panel_bytes, st, p, l, up_map);
-  else
-    rc = launch_block_per_sm<few_up_rows_kernel<F, NT>>("few_up_rows_kernel", ctas, FewShape<F>::kThreads, up_fixed + l.panel_bytes, st, p, l, up_map,
-                                                        piece_map);
-  if (rc != B200MOE_OK) return rc;
+  l.box = S::kRows;
+  l.side = p.hidden > 2 * S::kRows ? 4 : p.hidden > S::kRows ? 2 : 1;
+  l.columns = min(ctas, (p.hidden + l.side * S::kRows - 1) / (l.side * S::kRows));
+  l.splits = ctas / l.columns;
   const int64_t want = (int64_t)p.tokens * p.topk * down_row;
-  l.panel_bytes = (int)(want < down_room ? want : down_room);
-  if (l.panel_bytes < RedShape<F, NT>::kBytes) l.panel_bytes = RedShape<F, NT>::kBytes;
-  return launch_block_per_sm<few_down_kernel<F, NT>>("few_down_kernel", columns * l.splits, FewShape<F>::kThreads, DownShape<F>::kFixed + l.panel_bytes, st, p, l, down_map);
+  const int down_panel = at_least((int)(want < down_room ? want : down_room), RedShape<F, NT>::kBytes);
+  l.room = down_panel / S::kPanelBytes(S::kTerms);
+  // loads of 32 gates, 32 ups or 64 columns in pairs; of 64 columns of W2
+  CUtensorMap up_map, down_map;
+  int rc = few_map<F>(&up_map, p.w13, p.experts, p.act == B200MOE_ACT_SWIGLUOAI ? 64 : 32);
+  if (rc == B200MOE_OK) rc = few_map<F>(&down_map, p.w2, p.experts, l.box);
+  if (rc == B200MOE_OK)
+    rc = launch_block_per_sm<few_up_columns_kernel<F, NT>>("few_up_columns_kernel", ctas, S::kThreads, up_fixed + l.panel_bytes, st, p, l, up_map);
+  if (rc != B200MOE_OK) return rc;
+  return launch_block_per_sm<few_down_columns_kernel<F, NT>>("few_down_columns_kernel", l.columns * l.splits, S::kThreads, S::kRest + down_panel, st, p, l,
+                                                             down_map);
+}
+template <int F, int NT>
+int launch_rows(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
+  using S = RowShape<F>;
+  constexpr int up_fixed = UpRowsShape<F, NT>::kFixed, up_room = kMaxBlockSmem - up_fixed, down_room = kMaxBlockSmem - S::kRest;
+  const int up_row = (p.hidden + S::kK - 1) / S::kK * S::kPanelBytes, down_row = (p.inter + S::kK - 1) / S::kK * S::kPanelBytes;
+  static_assert(up_room >= 16384 / S::kK * S::kPanelBytes, "a token");
+  l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
+  l.splits = FewWorkspace::splits(p.hidden, ctas, kBlockRows);
+  l.columns = ctas / l.splits;
+  // a block's rows in as few turns as they need, and halved in each; scales from a multiple of four rows on
+  const int rows = (p.hidden + l.columns - 1) / l.columns, turns = (rows + kBlockRows - 1) / kBlockRows;
+  l.side = 2;
+  l.box = (rows + 2 * turns - 1) / (2 * turns);
+  l.scale_box = (l.box + 3 + 3) / 4 * 4;
+  const int64_t want = (int64_t)p.tokens * p.topk * down_row;
+  const int down_panel = at_least((int)(want < down_room ? want : down_room), S::kWarps * 8 * NT * kSumColumn * 4);
+  l.room = down_panel / S::kPanelBytes;
+  CUtensorMap up_map, down_map, up_scales, down_scales;
+  int rc = few_map<F>(&up_map, p.w13, p.experts, 16);
+  if (rc == B200MOE_OK) rc = few_map<F>(&down_map, p.w2, p.experts, l.box);
+  if constexpr (F == kFewFp8) {      // (these have no use for maps)
+    up_scales = up_map;
+    down_scales = down_map;
+  } else {
+    if (rc == B200MOE_OK) rc = few_scale_map(&up_scales, p.w13, p.experts, 16);
+    if (rc == B200MOE_OK) rc = few_scale_map(&down_scales, p.w2, p.experts, l.scale_box);
+  }
+  if (rc == B200MOE_OK)
+    rc = launch_block_per_sm<few_up_rows_kernel<F, NT>>("few_up_rows_kernel", ctas, S::kThreads, up_fixed + l.panel_bytes, st, p, l, up_map, up_scales);
+  if (rc != B200MOE_OK) return rc;
+  return launch_block_per_sm<few_down_rows_kernel<F, NT>>("few_down_rows_kernel", l.columns * l.splits, S::kThreads, S::kRest + down_panel, st, p, l,
+                                                          down_map, down_scales);
+}
+template <int F, int NT>
+int launch_mma(const FewParams& p, const FewLaunch& l, int ctas, cudaStream_t st) {
+  if constexpr (by_column(F)) return launch_columns<F, NT>(p, l, ctas, st);
+  else return launch_rows<F, NT>(p, l, ctas, st);
 }
 
 template <int F>

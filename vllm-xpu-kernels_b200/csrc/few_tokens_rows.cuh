@@ -286,10 +286,16 @@ __device__ __forceinline__ void find_row_tokens(RowTokens (&x)[NT], uint32_t use
 // instructions instead of five.)  What the 8 adds, 8 times the sum of x, is where the sums begin.
 __device__ __forceinline__ void u4x8_to_h2(uint32_t w, uint32_t (&o)[4]) {
   const uint32_t h = w >> 8;
-  o[0] = (w & 0x000f000fu) ^ 0x00080008u;
-  o[1] = (w & 0x00f000f0u) ^ 0x00800080u;
-  o[2] = (h & 0x000f000fu) ^ 0x00080008u;
-  o[3] = (h & 0x00f000f0u) ^ 0x00800080u;
+  // (a & b) ^ c in one instruction; left to the compiler it is two
+  auto masked = [](uint32_t v, uint32_t mask, uint32_t flip) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(v), "r"(mask), "r"(flip));
+    return r;
+  };
+  o[0] = masked(w, 0x000f000fu, 0x00080008u);
+  o[1] = masked(w, 0x00f000f0u, 0x00800080u);
+  o[2] = masked(h, 0x000f000fu, 0x00080008u);
+  o[3] = masked(h, 0x00f000f0u, 0x00800080u);
 }
 
 // acc += W x of the step in the slot (rows and columns that there are not: something finite or not that nobody reads).
@@ -316,31 +322,38 @@ __device__ __forceinline__ void multiply_rows(float (&acc)[2][NT][4], uint32_t s
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[q][n] = lds16(xa[n] + q * x[n].block);
     const uint32_t at[2] = {rows + ((t ^ row) << 4), rows + ((t ^ row ^ 4) << 4)};
+    // (the tiles in turn: products of one depend on one another)
+    float d[2][NT][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float d[NT][4];
+    for (int h = 0; h < 2; ++h) {
+      uint4 lo[2], hi[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 lo = lds16(at[h] + i * 1024), hi = lds16(at[h] + i * 1024 + 2048);
-        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+      for (int i = 0; i < 2; ++i) {
+        lo[i] = lds16(at[h] + i * 1024);
+        hi[i] = lds16(at[h] + i * 1024 + 2048);
+      }
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
           uint32_t a0, a1, a2, a3;
-          e4m3x4_to_h2(wl[w], a0, a2);
-          e4m3x4_to_h2(wh[w], a1, a3);
+          e4m3x4_to_h2(w == 0 ? lo[i].x : w == 1 ? lo[i].y : w == 2 ? lo[i].z : lo[i].w, a0, a2);
+          e4m3x4_to_h2(w == 0 ? hi[i].x : w == 1 ? hi[i].y : w == 2 ? hi[i].z : hi[i].w, a1, a3);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const uint4 b = v[2 * h + (w >> 1)][n];
-            if (h == 0 && w == 0) mma_first(d[n], a0, a1, a2, a3, b.x, b.y);
-            else mma(d[n], a0, a1, a2, a3, w & 1 ? b.z : b.x, w & 1 ? b.w : b.y);
+            if (h == 0 && w == 0) mma_first(d[i][n], a0, a1, a2, a3, b.x, b.y);
+            else mma(d[i][n], a0, a1, a2, a3, w & 1 ? b.z : b.x, w & 1 ? b.w : b.y);
           }
         }
-      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
       const float a = ldsf(scales + (i * 8 + row) * 4), b = ldsf(scales + (i * 8 + row) * 4 + 64);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf((c < 2 ? a : b) * sx[n][c & 1], d[n][c], acc[i][n][c]);
+        for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf((c < 2 ? a : b) * sx[n][c & 1], d[i][n][c], acc[i][n][c]);
     }
   } else {
     const uint32_t piece = rows + (F == kFewInt4 ? (t ^ row) << 4 : (row << 4) + t * 4);
@@ -361,63 +374,78 @@ __device__ __forceinline__ void multiply_rows(float (&acc)[2][NT][4], uint32_t s
             for (int c = 0; c < 2; ++c) first[g][n][c] = ldsf(xf[n][c] + (1 + h * (S::kSums / 2) + g) * x[n].next);
       }
       const uint32_t half = piece ^ (h << 6);
+      float d[2][NT][4];
+      if constexpr (F == kFewInt4) {
+        uint4 lo[2], hi[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float d[NT][4];
-        if constexpr (F == kFewInt4) {
-          const uint4 lo = lds16(half + i * 1024), hi = lds16(half + i * 1024 + 2048);
-          const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+        for (int i = 0; i < 2; ++i) {
+          lo[i] = lds16(half + i * 1024);
+          hi[i] = lds16(half + i * 1024 + 2048);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) d[n][c] = first[0][n][c & 1];
+            for (int c = 0; c < 4; ++c) d[i][n][c] = first[0][n][c & 1];
+        }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
             uint32_t al[4], ah[4];
-            u4x8_to_h2(wl[q], al);
-            u4x8_to_h2(wh[q], ah);
+            u4x8_to_h2(q == 0 ? lo[i].x : q == 1 ? lo[i].y : q == 2 ? lo[i].z : lo[i].w, al);
+            u4x8_to_h2(q == 0 ? hi[i].x : q == 1 ? hi[i].y : q == 2 ? hi[i].z : hi[i].w, ah);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              mma(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
-              mma(d[n], al[2], ah[2], al[3], ah[3], v[q][n].z, v[q][n].w);
+              mma(d[i][n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
+              mma(d[i][n], al[2], ah[2], al[3], ah[3], v[q][n].z, v[q][n].w);
             }
           }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
           const float a = ldsf(scales + h * 128 + (i * 8 + row) * 4), b = ldsf(scales + h * 128 + (i * 8 + row) * 4 + 64);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf((c < 2 ? a : b) * sx[n][c & 1], d[n][c], acc[i][n][c]);
-        } else {
-          const uint4 a4 = lds16(scales + (h * 32 + i * 8 + row) * 16), b4 = lds16(scales + (h * 32 + i * 8 + row) * 16 + 256);
-          const uint32_t as[4] = {a4.x, a4.y, a4.z, a4.w}, bs[4] = {b4.x, b4.y, b4.z, b4.w};
-          float sum[NT][4];
+            for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf((c < 2 ? a : b) * sx[n][c & 1], d[i][n][c], acc[i][n][c]);
+        }
+      } else {
+        float sum[2][NT][4];
+        uint4 as[2], bs[2];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+        for (int i = 0; i < 2; ++i) {
+          as[i] = lds16(scales + (h * 32 + i * 8 + row) * 16);
+          bs[i] = lds16(scales + (h * 32 + i * 8 + row) * 16 + 256);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
             const uint32_t w = (half ^ (q << 4)) + i * 1024;
             const uint32_t wl = lds4(w), wh = lds4(w + 2048);
             uint32_t al[4], ah[4];
             if constexpr (F == kFewFp4) { e2m1x8_to_h2(wl, al); e2m1x8_to_h2(wh, ah); }
             else { u4x8_to_h2(wl, al); u4x8_to_h2(wh, ah); }
-            const float a = __uint_as_float(as[q]), b = __uint_as_float(bs[q]);
+            const float a = __uint_as_float(q == 0 ? as[i].x : q == 1 ? as[i].y : q == 2 ? as[i].z : as[i].w);
+            const float b = __uint_as_float(q == 0 ? bs[i].x : q == 1 ? bs[i].y : q == 2 ? bs[i].z : bs[i].w);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               if constexpr (F == kFewFp4) {
-                mma_first(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
+                mma_first(d[i][n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
               } else {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) d[n][c] = first[q][n][c & 1];
-                mma(d[n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
+                for (int c = 0; c < 4; ++c) d[i][n][c] = first[q][n][c & 1];
+                mma(d[i][n], al[0], ah[0], al[1], ah[1], v[q][n].x, v[q][n].y);
               }
-              mma(d[n], al[2], ah[2], al[3], ah[3], v[q][n].z, v[q][n].w);
+              mma(d[i][n], al[2], ah[2], al[3], ah[3], v[q][n].z, v[q][n].w);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) sum[n][c] = q == 0 ? (c < 2 ? a : b) * d[n][c] : fmaf(c < 2 ? a : b, d[n][c], sum[n][c]);
+              for (int c = 0; c < 4; ++c) sum[i][n][c] = q == 0 ? (c < 2 ? a : b) * d[i][n][c] : fmaf(c < 2 ? a : b, d[i][n][c], sum[i][n][c]);
             }
           }
 #pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf(sx[n][c & 1], sum[n][c], acc[i][n][c]);
-        }
+            for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf(sx[n][c & 1], sum[i][n][c], acc[i][n][c]);
       }
     }
   }

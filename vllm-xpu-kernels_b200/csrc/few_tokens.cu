@@ -193,7 +193,8 @@ int launch_columns(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
 template <int F, int NT>
 int launch_rows(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   using S = RowShape<F>;
-  constexpr int up_fixed = UpRowsShape<F, NT>::kFixed, up_room = kMaxBlockSmem - up_fixed, down_room = kMaxBlockSmem - S::kRest;
+  constexpr int up_fixed = UpRowsShape<F, NT>::kFixed, up_room = kMaxBlockSmem - up_fixed;
+  const int down_fixed = S::kRest + down_sums_bytes(p.tokens, S::kWarps), down_room = kMaxBlockSmem - down_fixed;
   const int up_row = (p.hidden + S::kK - 1) / S::kK * S::kPanelBytes, down_row = (p.inter + S::kK - 1) / S::kK * S::kPanelBytes;
   static_assert(up_room >= 16384 / S::kK * S::kPanelBytes, "a token");
   l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
@@ -205,7 +206,7 @@ int launch_rows(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   l.box = (rows + 2 * turns - 1) / (2 * turns);
   l.scale_box = (l.box + 3 + 3) / 4 * 4;
   const int64_t want = (int64_t)p.tokens * p.topk * down_row;
-  const int down_panel = at_least((int)(want < down_room ? want : down_room), S::kWarps * 8 * NT * kSumColumn * 4);
+  const int down_panel = (int)(want < down_room ? want : down_room);
   l.room = down_panel / S::kPanelBytes;
   CUtensorMap up_map, down_map, up_scales, down_scales;
   int rc = few_map<F>(&up_map, p.w13, p.experts, 16);
@@ -220,7 +221,7 @@ int launch_rows(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   if (rc == B200MOE_OK)
     rc = launch_block_per_sm<few_up_rows_kernel<F, NT>>("few_up_rows_kernel", ctas, S::kThreads, up_fixed + l.panel_bytes, st, p, l, up_map, up_scales);
   if (rc != B200MOE_OK) return rc;
-  return launch_block_per_sm<few_down_rows_kernel<F, NT>>("few_down_rows_kernel", l.columns * l.splits, S::kThreads, S::kRest + down_panel, st, p, l,
+  return launch_block_per_sm<few_down_rows_kernel<F, NT>>("few_down_rows_kernel", l.columns * l.splits, S::kThreads, down_fixed + down_panel, st, p, l,
                                                           down_map, down_scales);
 }
 template <int F, int NT>

@@ -125,11 +125,11 @@ __device__ __noinline__ void fill_token(uint8_t* panel, float* floats, const voi
 }
 // Tokens of the set `now` into a panel.
 template <int F>
-__device__ __noinline__ void fill_tokens_rows(uint8_t* panel, float* floats, const void* from, int hidden, uint32_t now, int len, bool f16) {
-  constexpr int kWarps = RowShape<F>::kWarps;
-  const int warp = threadIdx.x >> 5, rows = __popc(now), parts = warps_per_row(rows, kWarps);
+__device__ __noinline__ void fill_tokens_rows(uint8_t* panel, float* floats, const void* from, int hidden, uint32_t now, int len, bool f16, int warp,
+                                              int warps) {
+  const int rows = __popc(now), parts = warps_per_row(rows, warps);
 #pragma unroll 1
-  for (int row = warp / parts; row < rows; row += kWarps / parts) {
+  for (int row = warp < warps / parts * parts ? warp / parts : rows; row < rows; row += warps / parts) {
     uint32_t left = now;
     for (int r = 0; r < row; ++r) left &= left - 1;
     const uint16_t* x = reinterpret_cast<const uint16_t*>(from) + (int64_t)(__ffs(left) - 1) * hidden;
@@ -260,26 +260,32 @@ __device__ __forceinline__ void spread_scales(uint32_t to, uint32_t from, const 
 }
 
 // Where a lane finds the values of its columns' tokens in the panel: the first block and the way to the next one.  Without a
-// token: zeros, and no way.
+// token: zeros, and no way.  An expert's tokens have columns in their order, so that up to eight need one instruction, whichever they
+// are.
 struct RowTokens {
   uint32_t at, block;
   uint32_t floats[2], next;   // of the lane's columns of sums: the step's scale (its sums behind it), and the way to the next one
 };
-template <int F, int NT>
-__device__ __forceinline__ void find_row_tokens(RowTokens (&x)[NT], uint32_t used, uint32_t in_panel, uint32_t panel, uint32_t floats, uint32_t zeros,
-                                                int rows) {
+// `count` tokens; row(i): the panel's row of the expert's token i.
+template <int NT, typename Row>
+__device__ __forceinline__ void find_row_tokens(RowTokens (&x)[NT], int count, uint32_t panel, uint32_t floats, uint32_t zeros, int rows, Row row) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const bool there = (used >> (8 * n + g)) & 1;
-    x[n].at = there ? panel + rank_below(in_panel, 8 * n + g) * 64 + t * 16 : zeros;
+    const bool there = 8 * n + g < count;
+    x[n].at = there ? panel + row(8 * n + g) * 64 + t * 16 : zeros;
     x[n].block = there ? rows * 64 : 0;
-    // (columns without a token: those of any, nobody reads them)
+    // (columns without a token: those of the last one, nobody reads them)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) x[n].floats[c] = floats + min(rank_below(in_panel, 8 * n + 2 * t + c), rows - 1) * 4;
+    for (int c = 0; c < 2; ++c) x[n].floats[c] = floats + row(min(8 * n + 2 * t + c, count - 1)) * 4;
     x[n].next = rows * 4;
   }
 }
+__device__ __forceinline__ int nth_bit(uint32_t bits, int n) {
+  for (int i = 0; i < n; ++i) bits &= bits - 1;
+  return __ffs(bits) - 1;
+}
+template <int N> struct Int { static constexpr int value = N; };
 
 // Eight two's-complement nibbles -> float16 pairs (0,4) (1,5) (2,6) (3,7) of (n + 8) 2^-24, every other pair times 16: n ^ 8 = n + 8 is
 // unsigned, and a small whole number is a float16 below the normal ones.  (Made signed numbers one by one it is nine
@@ -508,6 +514,9 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
   const FewMatrix& m = p.w13;
   const int steps = (p.hidden + S::kK - 1) / S::kK, per_expert = p.inter / 16;
   const int most = launch.panel_bytes / (steps * S::kPanelBytes); // rows that the panel holds
+  // A few values are laid out while one warp finds the experts, which takes as long as a round of loads; more than that would keep
+  // the weights from being asked for, and comes after it.
+  const bool early = most >= p.tokens && p.tokens * p.hidden <= (kWarps - 1) * 1024;
   const RowScales layout = {scale_words_of_step(m), (lane >> 4) * S::kUps + (lane & 15) * 4, 64, launch.f16};
   if (warp == 0) {
     build_table<false>(table, p);
@@ -515,8 +524,13 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
     if (tid < 48) reinterpret_cast<uint32_t*>(zeros)[tid - 32] = 0;
     if (blockIdx.x == 0)   // (the second kernel counts from there)
       for (int i = tid - 32; i < kFewMaxBlocks; i += kThreads - 32) launch.arrived[i] = 0;
-    const char* const x = reinterpret_cast<const char*>(p.x);
-    for (int i = (tid - 32) * 128; i < p.tokens * p.hidden * 2; i += (kThreads - 32) * 128) prefetch_l2(x + i);
+    if (early) {
+      fill_tokens_rows<F>(panel, reinterpret_cast<float*>(panel + p.tokens * steps * (S::kK * 2)), p.x, p.hidden, (1u << p.tokens) - 1u,
+                          steps * (S::kK / 8), launch.f16, warp - 1, kWarps - 1);
+    } else {
+      const char* const x = reinterpret_cast<const char*>(p.x);
+      for (int i = (tid - 32) * 128; i < p.tokens * p.hidden * 2; i += (kThreads - 32) * 128) prefetch_l2(x + i);
+    }
   }
   __syncthreads();
   const uint32_t all = (uint32_t)(table.active * per_expert);     // (times the blocks below 2^32: takes_mma)
@@ -540,6 +554,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
       to = min(stop, from + room);
       if (to < stop) break;
     }
+    if (early) tokens = (1u << p.tokens) - 1u;
     const int total = (to - from) * steps, workers = min(kWarps, total);
     const int pos0 = total * min(warp, workers) / workers, pos1 = total * min(warp + 1, workers) / workers;
     const int j0 = pos0 / steps, s0 = pos0 - j0 * steps;
@@ -589,34 +604,40 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
       for (int i = 0; i < S::kDepth; ++i) copy_next((ring.slot + i) % S::kDepth);
       const int rows = __popc(now);
       float* const floats = reinterpret_cast<float*>(panel + rows * steps * (S::kK * 2));
-      fill_tokens_rows<F>(panel, floats, p.x, p.hidden, now, steps * (S::kK / 8), launch.f16);
-      __syncthreads();
+      if (!early) {
+        fill_tokens_rows<F>(panel, floats, p.x, p.hidden, now, steps * (S::kK / 8), launch.f16, warp, kWarps);
+        __syncthreads();
+      }
 
 #pragma unroll 1
       for (int pos = pos0, j = j0, s = s0; pos < pos1; ++j, s = 0) {
         const uint32_t mine = table.tokens[(from + j) / per_expert] & now;
-        RowTokens x[NT];
-        find_row_tokens<F, NT>(x, mine, now, smem_at(panel), smem_at(floats), smem_at(zeros), rows);
-        float acc[2][NT][4] = {};
-        const int stop = min(steps, s + pos1 - pos);
+        const int count = __popc(mine), stop = min(steps, s + pos1 - pos);
         pos += stop - s;
-#pragma unroll 1
-        for (; s < stop; ++s) take_rows<F, NT>(acc, ring, layout, x, s, copy_next);
         // sets and warps begin a new entry each
-        float* const entry = sums + (j + warp) * (kSumColumn * deep);
+        float* const entry = sums + (j + warp) * (kSumColumn * deep) + (lane >> 2);
+        auto take = [&](auto width) {
+          constexpr int N = decltype(width)::value;
+          RowTokens x[N];
+          find_row_tokens<N>(x, count, smem_at(panel), smem_at(floats), smem_at(zeros), rows, [&](int i) { return rank_below(now, nth_bit(mine, i)); });
+          float acc[2][N][4] = {};
+#pragma unroll 1
+          for (; s < stop; ++s) take_rows<F, N>(acc, ring, layout, x, s, copy_next);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < N; ++n)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int token = 8 * n + 2 * (lane & 3) + c;
-            if (!((mine >> token) & 1)) continue;
-            float* const column = entry + rank_below(mine, token) * kSumColumn + (lane >> 2);
+            for (int c = 0; c < 2; ++c) {
+              const int column = 8 * n + 2 * (lane & 3) + c;
+              if (column >= count) continue;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              column[i * 16] = acc[i][n][c];
-              column[i * 16 + 8] = acc[i][n][c + 2];
+              for (int i = 0; i < 2; ++i) {
+                entry[column * kSumColumn + i * 16] = acc[i][n][c];
+                entry[column * kSumColumn + i * 16 + 8] = acc[i][n][c + 2];
+              }
             }
-          }
+        };
+        if (NT == 1 || count <= 8) take(Int<1>{});
+        else take(Int<NT>{});
       }
       // A warp has a set, a lane one of its features, for one token of two.  What does not need the sums is there before the
       // barrier, and for the next set before the sums of this one.
@@ -670,6 +691,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
 
 // ---- the second kernel -------------------------------------------------------------------
 constexpr int kBlockRows = 64;      // of W2 that a block has at once
+__host__ __device__ __forceinline__ int down_sums_bytes(int tokens, int warps) { return (warps * tokens * kSumColumn * 4 + 127) / 128 * 128; }
 
 // out = sum over experts of weight * (W2 h + b2).  A block has some rows of W2 and a share of the steps over all active
 // experts: of rows up to 64, so that few blocks need the same values of h, and of steps what makes as many blocks as there are
@@ -688,8 +710,9 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = lane & 3;
   FewRing ring = make_ring(smem, S::kSlot, S::kDepth, smem + S::kScales, S::kWarpScales, reinterpret_cast<uint64_t*>(smem + S::kBars), gave_up,
                            launch.status);
-  uint8_t* const panel = smem + S::kRest;
-  float* const red = reinterpret_cast<float*>(panel);                     // (after the last panel)
+  // every warp's sums, by token, and the panel
+  float* const sums = reinterpret_cast<float*>(smem + S::kRest), * const my_sums = sums + warp * p.tokens * kSumColumn + (lane >> 2);
+  uint8_t* const panel = smem + S::kRest + down_sums_bytes(p.tokens, kWarps);
   if (tid == 0) {
     *gave_up = 0;
     ptx::prefetch_tensormap(&map);
@@ -770,7 +793,8 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
       pdl_trigger();
       waited = true;
     }
-    float out[2][NT][4] = {};
+    for (int i = lane; i < p.tokens * kSumColumn; i += 32) sums[warp * p.tokens * kSumColumn + i] = 0.f;
+    __syncwarp();
     for (int a0 = share.begin / steps, s0 = share.begin - a0 * steps; a0 * steps + s0 < share.end;) {
       int a1, s1;
       share.panel_end(table, launch.room, a0, s0, a1, s1);
@@ -799,42 +823,36 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
           // rows of earlier experts in the panel, as above
           const int before = (a == a0 ? 0 : (table.first_row[a0 + 1] - row0) * (steps - s0) + (row - table.first_row[a0 + 1]) * steps) - (a == a0 ? s0 : 0) * n_rows;
           const uint32_t mine = table.tokens[a];
-          RowTokens x[NT];
-          find_row_tokens<F, NT>(x, mine, mine, smem_at(panel) + before * (S::kK * 2), smem_at(floats) + before * (S::kFloats * 4), smem_at(zeros), n_rows);
-          float acc[2][NT][4] = {};
+          auto take = [&](auto width) {
+            constexpr int N = decltype(width)::value;
+            RowTokens x[N];
+            find_row_tokens<N>(x, n_rows, smem_at(panel) + before * (S::kK * 2), smem_at(floats) + before * (S::kFloats * 4), smem_at(zeros), n_rows,
+                               [](int i) { return i; });
+            float acc[2][N][4] = {};
 #pragma unroll 1
-          for (; pos < end; ++pos) take_rows<F, NT>(acc, ring, layout, x, pos - a * steps, copy_next);
-          // (columns of tokens without this expert are left out: a weight that is not finite would get into them)
+            for (; pos < end; ++pos) take_rows<F, N>(acc, ring, layout, x, pos - a * steps, copy_next);
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int token = 8 * n + 2 * t + c;
-              if (!((mine >> token) & 1)) continue;
-              const float w = table.weight[row + rank_below(mine, token)];
+              for (int c = 0; c < 2; ++c) {
+                const int column = 8 * n + 2 * t + c;
+                if (column >= n_rows) continue;
+                const float w = table.weight[row + column];
+                float* const to = my_sums + nth_bit(mine, column) * kSumColumn;
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                out[i][n][c] = fmaf(w, acc[i][n][c], out[i][n][c]);
-                out[i][n][c + 2] = fmaf(w, acc[i][n][c + 2], out[i][n][c + 2]);
+                for (int i = 0; i < 2; ++i) {
+                  to[i * 16] = fmaf(w, acc[i][n][c], to[i * 16]);
+                  to[i * 16 + 8] = fmaf(w, acc[i][n][c + 2], to[i * 16 + 8]);
+                }
               }
-            }
+          };
+          if (NT == 1 || n_rows <= 8) take(Int<1>{});
+          else take(Int<NT>{});
         }
       }
       a0 = a1;
       s0 = s1;
       __syncthreads();   // the panel is free again
-    }
-    {
-      float* const to = red + warp * (8 * NT * kSumColumn) + (lane >> 2);
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            to[(8 * n + 2 * t + c) * kSumColumn + i * 16] = out[i][n][c];
-            to[(8 * n + 2 * t + c) * kSumColumn + i * 16 + 8] = out[i][n][c + 2];
-          }
     }
     if (F == kFewFp8) copies_wait<0>();
     __syncthreads();
@@ -846,7 +864,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
       if (my_row >= block_rows_here || token >= p.tokens) continue;
       float v = bias[i];
 #pragma unroll
-      for (int w = 0; w < kMembers; ++w) v += red[(2 * w + which) * (8 * NT * kSumColumn) + token * kSumColumn + my_sum];
+      for (int w = 0; w < kMembers; ++w) v += sums[((2 * w + which) * p.tokens + token) * kSumColumn + my_sum];
       if (launch.splits == 1) finish(v, token, block_r0 + my_row);
       else launch.part[((int64_t)share.split * p.tokens + token) * p.hidden + block_r0 + my_row] = v;
     }

@@ -4,6 +4,8 @@
 //   down:  out[t] = sum_k w[t,k] (W2[e] h[s] + b2[e])
 //
 // Weights are taken as they are stored; activations stay in 16 bits or more, sums in fp32.
+#include <algorithm>
+
 #include "common.cuh"
 #include "few_tokens.cuh"
 #include "few_tokens_columns.cuh"
@@ -119,7 +121,9 @@ int launch_block_per_sm(const char* name, int grid, int threads, int smem, cudaS
   return B200MOE_OK;
 }
 
-constexpr int kMaxBlockRows = 512;      // of W2 that a block of the second kernel can have at once
+// Shares of the second kernel's steps for the same rows, at most: the last of their blocks adds all of them up, some 0.2 us each and
+// round of 256 sums (148 of them for 256 columns: 217 us at 16 tokens).
+constexpr int kMaxSplits = 9;
 
 // Where things are in the workspace: h, then what the blocks of the two kernels tell one another.
 struct FewWorkspace {
@@ -128,14 +132,14 @@ struct FewWorkspace {
     auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     arrived = up(tokens * topk * inter * sizeof(float));
     part = arrived + kFewMaxBlocks * sizeof(uint32_t);
-    bytes = part + up((size_t)splits(hidden, kFewMaxBlocks) * tokens * hidden * sizeof(float));
-  }
-  // Shares of the second kernel's steps: as many as make `ctas` blocks with up to `rows` rows each.
-  static int splits(int64_t hidden, int ctas, int rows = kMaxBlockRows) {
-    const int64_t n = (int64_t)ctas * rows / hidden;
-    return n < 1 ? 1 : n > ctas ? ctas : (int)n;
+    bytes = part + up((size_t)kMaxSplits * tokens * hidden * sizeof(float));
   }
 };
+// As many as make `ctas` blocks with up to `rows` rows each.
+int few_splits(int64_t hidden, int ctas, int rows) {
+  const int64_t n = (int64_t)ctas * rows / hidden;
+  return n < 1 ? 1 : (int)std::min<int64_t>(n, std::min(ctas, kMaxSplits));
+}
 
 // The map of a matrix for loads of `box` rows (by column: columns) of a step, and that of its scales (4 bits).
 template <int F>
@@ -174,9 +178,11 @@ int launch_columns(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   static_assert(up_room >= 16384 / S::kK * S::kPanelBytes(1), "a token");
   l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
   l.box = S::kRows;
-  l.side = p.hidden > 2 * S::kRows ? 4 : p.hidden > S::kRows ? 2 : 1;
+  // as many side by side as leave no more shares than that
+  l.side = 4;
+  while (l.side > 1 && (p.hidden + l.side * S::kRows - 1) / (l.side * S::kRows) * kMaxSplits * 4 < ctas * 3) l.side /= 2;
   l.columns = min(ctas, (p.hidden + l.side * S::kRows - 1) / (l.side * S::kRows));
-  l.splits = ctas / l.columns;
+  l.splits = min(ctas / l.columns, kMaxSplits);
   const int64_t want = (int64_t)p.tokens * p.topk * down_row;
   const int down_panel = at_least((int)(want < down_room ? want : down_room), RedShape<F, NT>::kBytes);
   l.room = down_panel / S::kPanelBytes(S::kTerms);
@@ -198,8 +204,8 @@ int launch_rows(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   const int up_row = (p.hidden + S::kK - 1) / S::kK * S::kPanelBytes, down_row = (p.inter + S::kK - 1) / S::kK * S::kPanelBytes;
   static_assert(up_room >= 16384 / S::kK * S::kPanelBytes, "a token");
   l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
-  l.splits = FewWorkspace::splits(p.hidden, ctas, kBlockRows);
-  l.columns = ctas / l.splits;
+  l.splits = few_splits(p.hidden, ctas, kBlockRows);
+  l.columns = min(ctas / l.splits, (p.hidden + 15) / 16);
   // a block's rows in as few turns as they need, and halved in each; scales from a multiple of four rows on
   const int rows = (p.hidden + l.columns - 1) / l.columns, turns = (rows + kBlockRows - 1) / kBlockRows;
   l.side = 2;

@@ -320,14 +320,27 @@ __device__ __forceinline__ void sum_splits(const FewLaunch& launch, const FewPar
   }
   __syncthreads();
   if (!last_one) return;
-  for (int j = threadIdx.x; j < width * p.tokens; j += blockDim.x) {
-    const int token = j / width, row = row_begin + j - token * width;
-    float v = 0.f;
-    const float* from = launch.part + (int64_t)token * p.hidden + row;
-    const int64_t next = (int64_t)p.tokens * p.hidden;
-#pragma unroll 4
-    for (int i = 0; i < launch.splits; ++i) v += __ldcg(from + i * next);
-    finish(v, token, row);
+  // (four outputs of a thread at once, whose loads are in flight together)
+  const int64_t next = (int64_t)p.tokens * p.hidden;
+  const int all = width * p.tokens, stride = blockDim.x;
+#pragma unroll 1
+  for (int j0 = threadIdx.x; j0 < all; j0 += 4 * stride) {
+    const float* from[4];
+    float v[4] = {};
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+      const int j = min(j0 + o * stride, all - 1), token = j / width;
+      from[o] = launch.part + (int64_t)token * p.hidden + row_begin + j - token * width;
+    }
+#pragma unroll 3
+    for (int i = 0; i < launch.splits; ++i)
+#pragma unroll
+      for (int o = 0; o < 4; ++o) v[o] += __ldcg(from[o] + i * next);
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+      const int j = j0 + o * stride, token = j / width;
+      if (j < all) finish(v[o], token, row_begin + j - token * width);
+    }
   }
 }
 

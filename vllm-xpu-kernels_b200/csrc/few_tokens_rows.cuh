@@ -537,156 +537,188 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
   const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
   const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
 
-#pragma unroll 1
-  for (int from = begin; from < end;) {
-    // A pass: as many experts as have their tokens in the panel at once and their sums in shared memory; one with more tokens
-    // than the panel holds goes through its features again with the rest of them.
-    int to = from, deep = 0;       // deep: the most tokens that an expert has
-    uint32_t tokens = 0;
-    const int a_first = from / per_expert;
-    for (int a = a_first; to < end; ++a) {
-      const uint32_t with = tokens | table.tokens[a];
-      const int n = max(deep, min(__popc(table.tokens[a]), most)), stop = min(end, (a + 1) * per_expert);
-      const int room = UpRowsShape<F, NT>::kSums / (kSumColumn * 4 * n) - kWarps;             // sets
-      if (tokens && (__popc(with) > most || room <= to - from)) break;
-      tokens = with;
-      deep = n;
-      to = min(stop, from + room);
-      if (to < stop) break;
+  // A pass: as many experts as have their tokens in the panel at once and their sums in shared memory; one with more tokens
+  // than the panel holds goes through its features again with the rest of them.
+  struct Pass {
+    int from, to, deep;            // sets; the most tokens that an expert has
+    uint32_t now, rest;            // tokens in the panel, and of a later pass over the same sets
+    int total, workers;            // steps, and the warps that have any
+    __device__ __forceinline__ int start(int warp) const { return total * min(warp, workers) / workers; }
+  };
+  auto plan = [&](int from, int to, uint32_t rest) {       // from the set `from` on, or the rest of the tokens
+    Pass pass;
+    pass.from = from;
+    pass.deep = min(__popc(rest), most);
+    if (!rest) {
+      const int a_first = from / per_expert;
+      to = from;
+      for (int a = a_first; to < end; ++a) {
+        const uint32_t with = rest | table.tokens[a];
+        const int n = max(pass.deep, min(__popc(table.tokens[a]), most)), stop = min(end, (a + 1) * per_expert);
+        const int room = UpRowsShape<F, NT>::kSums / (kSumColumn * 4 * n) - kWarps;             // sets
+        if (rest && (__popc(with) > most || room <= to - from)) break;
+        rest = with;
+        pass.deep = n;
+        to = min(stop, from + room);
+        if (to < stop) break;
+      }
+      if (early) rest = (1u << p.tokens) - 1u;
     }
-    if (early) tokens = (1u << p.tokens) - 1u;
-    const int total = (to - from) * steps, workers = min(kWarps, total);
-    const int pos0 = total * min(warp, workers) / workers, pos1 = total * min(warp + 1, workers) / workers;
-    const int j0 = pos0 / steps, s0 = pos0 - j0 * steps;
+    pass.to = to;
+    pass.now = rest;
+    while (__popc(pass.now) > most) pass.now &= ~(1u << (31 - __clz(pass.now)));
+    pass.rest = rest & ~pass.now;
+    pass.total = (to - from) * steps;
+    pass.workers = min(kWarps, pass.total);
+    return pass;
+  };
 
-#pragma unroll 1
-    for (uint32_t rest = tokens; rest;) {
-      uint32_t now = rest;
-      while (__popc(now) > most) now &= ~(1u << (31 - __clz(now)));
-      rest &= ~now;
-
-      // The ring begins to fill: the set and step that are fetched next, and how many after them.
-      int fetch_j = j0 - 1, fetch_s = steps, left = pos1 - pos0, e = 0, row = 0;
-      const uint8_t* scale = nullptr;
-      auto copy_next = [&](int slot) {
-        if (left > 0) {
-          if (fetch_s == steps) {
-            ++fetch_j;
-            fetch_s = fetch_j == j0 ? s0 : 0;
-            const int a = (from + fetch_j) / per_expert;
-            row = 16 * (from + fetch_j - a * per_expert);
-            e = table.expert[a];
-            if (F == kFewFp8) scale = fp8_scale(m, e, pairs ? 2 * row + lane : row + (lane & 15) + (lane >= 16 ? p.inter : 0)) + fetch_s * 4;
-          }
-          const uint32_t scales = ring.scales + slot * S::kSlotScales;
-          if (lane == 0) {
-            const uint32_t at = ring.slots + slot * S::kSlot, bar = ring.bars + slot * 8;
-            const int y0 = pairs ? 2 * row : row, y1 = pairs ? 2 * row + 16 : p.inter + row;
-            ptx::fence_proxy_async();      // (the warp has read what was there)
-            ptx::mbar_expect_tx_s(bar, S::kSlot + (F == kFewFp8 ? 0 : layout.words * 128));
-            ptx::tma_load_3d_hint_s(at, &map, bar, fetch_s * 128, y0, e, ring.once);
-            ptx::tma_load_3d_hint_s(at + S::kSlot / 2, &map, bar, fetch_s * 128, y1, e, ring.once);
-            if (F != kFewFp8) {
-              ptx::tma_load_3d_hint_s(scales, &scale_map, bar, y0, fetch_s * layout.words, e, ring.once);
-              ptx::tma_load_3d_hint_s(scales + S::kUps, &scale_map, bar, y1, fetch_s * layout.words, e, ring.once);
-            }
-          }
-          if (F == kFewFp8) {
-            copy4(scales + lane * 4, scale);
-            scale += 4;
-          }
-          ++fetch_s;
-          --left;
-        }
-        if (F == kFewFp8) copies_end();
-      };
-#pragma unroll 1
-      for (int i = 0; i < S::kDepth; ++i) copy_next((ring.slot + i) % S::kDepth);
-      const int rows = __popc(now);
-      float* const floats = reinterpret_cast<float*>(panel + rows * steps * (S::kK * 2));
-      if (!early) {
-        fill_tokens_rows<F>(panel, floats, p.x, p.hidden, now, steps * (S::kK / 8), launch.f16, warp, kWarps);
-        __syncthreads();
+  // The set and step that are fetched next, and how many after them.
+  int fetch_j = 0, fetch_s = 0, fetch_s0 = 0, left = 0, e = 0, row = 0;
+  const uint8_t* scale = nullptr;
+  auto copy_next = [&](int slot) {
+    if (left > 0) {
+      if (fetch_s == steps) {
+        fetch_s = fetch_s0;
+        fetch_s0 = 0;
+        const int a = fetch_j / per_expert;
+        row = 16 * (fetch_j - a * per_expert);
+        ++fetch_j;
+        e = table.expert[a];
+        if (F == kFewFp8) scale = fp8_scale(m, e, pairs ? 2 * row + lane : row + (lane & 15) + (lane >= 16 ? p.inter : 0)) + fetch_s * 4;
       }
-
-#pragma unroll 1
-      for (int pos = pos0, j = j0, s = s0; pos < pos1; ++j, s = 0) {
-        const uint32_t mine = table.tokens[(from + j) / per_expert] & now;
-        const int count = __popc(mine), stop = min(steps, s + pos1 - pos);
-        pos += stop - s;
-        // sets and warps begin a new entry each
-        float* const entry = sums + (j + warp) * (kSumColumn * deep) + (lane >> 2);
-        auto take = [&](auto width) {
-          constexpr int N = decltype(width)::value;
-          RowTokens x[N];
-          find_row_tokens<N>(x, count, smem_at(panel), smem_at(floats), smem_at(zeros), rows, [&](int i) { return rank_below(now, nth_bit(mine, i)); });
-          float acc[2][N][4] = {};
-#pragma unroll 1
-          for (; s < stop; ++s) take_rows<F, N>(acc, ring, layout, x, s, copy_next);
-#pragma unroll
-          for (int n = 0; n < N; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int column = 8 * n + 2 * (lane & 3) + c;
-              if (column >= count) continue;
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                entry[column * kSumColumn + i * 16] = acc[i][n][c];
-                entry[column * kSumColumn + i * 16 + 8] = acc[i][n][c + 2];
-              }
-            }
-        };
-        if (NT == 1 || count <= 8) take(Int<1>{});
-        else take(Int<NT>{});
-      }
-      // A warp has a set, a lane one of its features, for one token of two.  What does not need the sums is there before the
-      // barrier, and for the next set before the sums of this one.
-      struct { int a, f, w0, w1; float gate, up; } set;
-      auto look_up = [&](int j) {
-        set.a = (from + j) / per_expert;
-        set.f = 16 * (from + j - set.a * per_expert) + (lane & 15);
-        // the warps that had the set's first and last step
-        set.w0 = (workers * (j * steps + 1) - 1) / total;
-        set.w1 = (workers * (j + 1) * steps - 1) / total;
-        set.gate = set.up = 0.f;
-        if (m.bias) {
-          const int64_t at = (int64_t)table.expert[set.a] * m.n;
-          set.gate = load16(m.bias, at + (pairs ? 2 * set.f : set.f), launch.f16);
-          set.up = load16(m.bias, at + (pairs ? 2 * set.f + 1 : p.inter + set.f), launch.f16);
-        }
-      };
-      const int sets = to - from, gate_row = pairs ? 2 * (lane & 15) : lane & 15, up_row = pairs ? gate_row + 1 : 16 + gate_row;
-      const float* const gates = sums + sum_of_row(gate_row), * const ups = sums + sum_of_row(up_row);
-      if (warp < sets) look_up(warp);
-      if (F == kFewFp8) copies_wait<0>();
-      __syncthreads();   // the sums are complete, and the panel is free again
-#pragma unroll 1
-      for (int j = warp; j < sets; j += kWarps) {
-        const auto here = set;
-        if (j + kWarps < sets) look_up(j + kWarps);
-        const uint32_t have = table.tokens[here.a];
-        uint32_t later = have & now;
-        for (int rank = 0; later; rank += 2) {        // (two tokens: the lower and the upper half of the warp)
-          const uint32_t after = later & (later - 1);
-          const int my_rank = rank + (lane >> 4), token = __ffs(lane < 16 ? later : after) - 1;
-          float v = 0.f;
-          if (token >= 0) {
-            float gate = here.gate, up = here.up;
-            for (int w = here.w0; w <= here.w1; ++w) {
-              const int at = ((j + w) * deep + my_rank) * kSumColumn;
-              gate += gates[at];
-              up += ups[at];
-            }
-            v = gated_once(p.act, p.alpha, p.limit, p.clamp, gate, up);
-          }
-          store_h(p.h, table.first_row[here.a] + (token >= 0 ? rank_below(have, token) : 0), here.f, p.inter, p.tokens * p.topk, v, token >= 0);
-          later = after & (after - 1);
+      const uint32_t scales = ring.scales + slot * S::kSlotScales;
+      if (lane == 0) {
+        const uint32_t at = ring.slots + slot * S::kSlot, bar = ring.bars + slot * 8;
+        const int y0 = pairs ? 2 * row : row, y1 = pairs ? 2 * row + 16 : p.inter + row;
+        ptx::fence_proxy_async();      // (the warp has read what was there)
+        ptx::mbar_expect_tx_s(bar, S::kSlot + (F == kFewFp8 ? 0 : layout.words * 128));
+        ptx::tma_load_3d_hint_s(at, &map, bar, fetch_s * 128, y0, e, ring.once);
+        ptx::tma_load_3d_hint_s(at + S::kSlot / 2, &map, bar, fetch_s * 128, y1, e, ring.once);
+        if (F != kFewFp8) {
+          ptx::tma_load_3d_hint_s(scales, &scale_map, bar, y0, fetch_s * layout.words, e, ring.once);
+          ptx::tma_load_3d_hint_s(scales + S::kUps, &scale_map, bar, y1, fetch_s * layout.words, e, ring.once);
         }
       }
-      if (rest || to < end) __syncthreads();   // the sums' place is free again
+      if (F == kFewFp8) {
+        copy4(scales + lane * 4, scale);
+        scale += 4;
+      }
+      ++fetch_s;
+      --left;
     }
-    from = to;
+    if (F == kFewFp8) copies_end();
+  };
+  auto start_fetch = [&](const Pass& pass) {
+    const int pos = pass.start(warp), j = pos / steps;
+    left = pass.start(warp + 1) - pos;
+    fetch_j = pass.from + j;
+    fetch_s0 = pos - j * steps;
+    fetch_s = steps;
+#pragma unroll 1
+    for (int i = 0; i < S::kDepth; ++i) copy_next((ring.slot + i) % S::kDepth);
+  };
+  auto lay_out = [&](uint32_t now) {
+    fill_tokens_rows<F>(panel, reinterpret_cast<float*>(panel + __popc(now) * steps * (S::kK * 2)), p.x, p.hidden, now, steps * (S::kK / 8), launch.f16,
+                        warp, kWarps);
+  };
+  Pass pass = plan(begin, begin, 0);
+  if (begin < end) {
+    start_fetch(pass);
+    if (!early) {
+      lay_out(pass.now);
+      __syncthreads();
+    }
   }
+#pragma unroll 1
+  while (pass.from < end) {
+    const int from = pass.from, total = pass.total, workers = pass.workers, deep = pass.deep, rows = __popc(pass.now);
+    const int pos0 = pass.start(warp), pos1 = pass.start(warp + 1), j0 = pos0 / steps, s0 = pos0 - j0 * steps;
+    const uint32_t now = pass.now;
+    const float* const floats = reinterpret_cast<float*>(panel + rows * steps * (S::kK * 2));
+#pragma unroll 1
+    for (int pos = pos0, j = j0, s = s0; pos < pos1; ++j, s = 0) {
+      const uint32_t mine = table.tokens[(from + j) / per_expert] & now;
+      const int count = __popc(mine), stop = min(steps, s + pos1 - pos);
+      pos += stop - s;
+      // sets and warps begin a new entry each
+      float* const entry = sums + (j + warp) * (kSumColumn * deep) + (lane >> 2);
+      auto take = [&](auto width) {
+        constexpr int N = decltype(width)::value;
+        RowTokens x[N];
+        find_row_tokens<N>(x, count, smem_at(panel), smem_at(floats), smem_at(zeros), rows, [&](int i) { return rank_below(now, nth_bit(mine, i)); });
+        float acc[2][N][4] = {};
+#pragma unroll 1
+        for (; s < stop; ++s) take_rows<F, N>(acc, ring, layout, x, s, copy_next);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int column = 8 * n + 2 * (lane & 3) + c;
+            if (column >= count) continue;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              entry[column * kSumColumn + i * 16] = acc[i][n][c];
+              entry[column * kSumColumn + i * 16 + 8] = acc[i][n][c + 2];
+            }
+          }
+      };
+      if (NT == 1 || count <= 8) take(Int<1>{});
+      else take(Int<NT>{});
+    }
+    // A warp has a set, a lane one of its features, for one token of two.  What does not need the sums is there before the
+    // barrier, and for the next set before the sums of this one.
+    struct { int a, f, w0, w1; float gate, up; } set;
+    auto look_up = [&](int j) {
+      set.a = (from + j) / per_expert;
+      set.f = 16 * (from + j - set.a * per_expert) + (lane & 15);
+      // the warps that had the set's first and last step
+      set.w0 = (workers * (j * steps + 1) - 1) / total;
+      set.w1 = (workers * (j + 1) * steps - 1) / total;
+      set.gate = set.up = 0.f;
+      if (m.bias) {
+        const int64_t at = (int64_t)table.expert[set.a] * m.n;
+        set.gate = load16(m.bias, at + (pairs ? 2 * set.f : set.f), launch.f16);
+        set.up = load16(m.bias, at + (pairs ? 2 * set.f + 1 : p.inter + set.f), launch.f16);
+      }
+    };
+    const int sets = pass.to - from, gate_row = pairs ? 2 * (lane & 15) : lane & 15, up_row = pairs ? gate_row + 1 : 16 + gate_row;
+    const float* const gates = sums + sum_of_row(gate_row), * const ups = sums + sum_of_row(up_row);
+    if (warp < sets) look_up(warp);
+    // the next pass's weights are on their way meanwhile
+    const Pass next = pass.rest ? plan(from, pass.to, pass.rest) : plan(pass.to, pass.to, 0);
+    if (next.from < end) start_fetch(next);
+    __syncthreads();   // the sums are complete, and the panel is free again
+#pragma unroll 1
+    for (int j = warp; j < sets; j += kWarps) {
+      const auto here = set;
+      if (j + kWarps < sets) look_up(j + kWarps);
+      const uint32_t have = table.tokens[here.a];
+      uint32_t later = have & now;
+      for (int rank = 0; later; rank += 2) {        // (two tokens: the lower and the upper half of the warp)
+        const uint32_t after = later & (later - 1);
+        const int my_rank = rank + (lane >> 4), token = __ffs(lane < 16 ? later : after) - 1;
+        float v = 0.f;
+        if (token >= 0) {
+          float gate = here.gate, up = here.up;
+          for (int w = here.w0; w <= here.w1; ++w) {
+            const int at = ((j + w) * deep + my_rank) * kSumColumn;
+            gate += gates[at];
+            up += ups[at];
+          }
+          v = gated_once(p.act, p.alpha, p.limit, p.clamp, gate, up);
+        }
+        store_h(p.h, table.first_row[here.a] + (token >= 0 ? rank_below(have, token) : 0), here.f, p.inter, p.tokens * p.topk, v, token >= 0);
+        later = after & (after - 1);
+      }
+    }
+    if (next.from < end) {
+      if (!early) lay_out(next.now);
+      __syncthreads();   // the sums' place is free again
+    }
+    pass = next;
+  }
+  if (F == kFewFp8) copies_wait<0>();
 }
 
 // ---- the second kernel -------------------------------------------------------------------

@@ -170,6 +170,24 @@ def test_int4_groups_of_both(native, group, group2):
     c.check(c.run())
 
 
+@pytest.mark.parametrize("recipe", ["w16", "fp8", "mxfp4", "int4"])
+@pytest.mark.parametrize("H,I,experts", [(8192, 256, 1), (16384, 128, 2), (256, 8192, 1), (256, 4096, 3)])
+def test_more_tokens_than_a_block_holds(native, recipe, H, I, experts):
+    """Tokens that a block's shared memory holds a part of, all with the same experts: several passes over the features, several
+    stretches of h."""
+    c = Case(native, recipe, 16, H, I, 4, 1, group=128, seed=H + I)
+    c.ids[:, 0] = torch.arange(16, device=DEV, dtype=torch.int32) % experts
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("recipe", ["w16", "fp8", "mxfp4", "int4"])
+@pytest.mark.parametrize("T", [2, 13])
+def test_more_experts_than_blocks(native, recipe, T):
+    """Blocks whose features belong to many experts: small ones, most of them with one token."""
+    c = Case(native, recipe, T, 128, 128, 300, 24, group=64, seed=T)
+    c.check(c.run())
+
+
 @pytest.mark.parametrize("T", range(1, 17))
 @pytest.mark.parametrize("recipe", ["w16", "fp8", "mxfp4", "int4"])
 def test_every_number_of_tokens(native, recipe, T):

@@ -151,6 +151,10 @@ enum ScaleMode { kNoScales, kRowScale, kGroupScales };
 // Rows are read once and stay in registers between their sums and the result.  blockDim = (threads of a row, rows of a
 // block); a thread has V pieces of N values, blockDim.x pieces apart.  A resident block takes row after row and asks for
 // the next one before it waits for its sums.
+// Bound by the bytes of a row, each moved once: 8192 rows of 7168 bf16 values with residual, output and e4m3 rows 86 us, 6.1
+// TB/s (a block per row with 16-byte pieces and its values read twice 228 us).  Where only e4m3 rows are written there are fewer bytes
+// for the same chain of sums, scale and codes: 8192 rows of 4096 float16 values 33 us, 3.0 TB/s.  With few rows the launch is what it
+// costs: one row 2.2 us in a graph.
 template <typename T, typename W, int N, int V, int kMode>
 __global__ void __launch_bounds__(1024) rms_norm_kernel(RmsParams p) {
   __shared__ float2 red[2][32];
@@ -302,7 +306,12 @@ int launch_rms_norm(const RmsParams& p, cudaStream_t st) {
   constexpr int N = 32 / sizeof(T), kSingles = 8;
   if (pieces_fit(p, N, sizeof(T), sizeof(W))) return launch_mode<T, W, N, 1>(p, st);
   if (pieces_fit(p, N / 2, sizeof(T), sizeof(W))) return launch_mode<T, W, N / 2, 1>(p, st);
-  if (p.hidden <= 1024 * kSingles && (p.q == nullptr || p.group == 0)) return launch_mode<T, W, 1, kSingles>(p, st);
+  // Rows that cannot be cut into pieces: kept in registers value by value where that saves the second way through them, whose latency
+  // counts with few rows; with many the kernel below has more of them on an SM.  us, in registers / below: 1411 bf16 values, 61 rows
+  // 4.9 / 7.4, 256 rows 6.6 / 8.1, 1001 rows 11.3 / 10.6, 8192 rows 82 / 63; 5001 values, 61 rows 6.0 / 20, 8192 rows 402 / 188;
+  // 99 values, 8192 rows 9.4 / 15.9.
+  if (p.hidden <= 1024 * kSingles && (p.rows <= 512 || p.hidden < 256) && (p.q == nullptr || p.group == 0))
+    return launch_mode<T, W, 1, kSingles>(p, st);
   B200_LAUNCHED("rms_norm_scalar_kernel",
                 launch_pdl(p.rows <= kEarlyLaunchRows, rms_norm_scalar_kernel<T, W>, dim3((unsigned)p.rows), dim3(256), 0, st, p));
   return B200MOE_OK;

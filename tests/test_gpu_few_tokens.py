@@ -331,6 +331,51 @@ def test_streams_graphs_and_workspaces(native):
     c.check(graphs[0][1])
 
 
+@pytest.mark.parametrize("recipe", ["fp8", "mxfp4"])
+def test_decoding_steps(native, recipe):
+    """What a decoder block does between its attention and the next one's, as it would be called: norm with the residual's
+    addition, router, layer for a few tokens; with the same results eagerly and replayed, over steps that follow one another."""
+    from gpu_utils import topk_softmax
+    T, H, E, K = 5, 512, 16, 4
+    c = Case(native, recipe, T, H, 256, E, K, seed=11)
+    router, weight = torch.randn(H, E, device=DEV) * H ** -0.5, torch.rand(H, device=DEV) + 0.5
+    hidden, residual = torch.zeros(T, H, dtype=BF16, device=DEV), torch.zeros(T, H, dtype=BF16, device=DEV)
+    rows, q, s = torch.empty_like(hidden), torch.empty(T, H, dtype=torch.float8_e4m3fn, device=DEV), torch.empty(T, H // 128, device=DEV)
+
+    def step():
+        torch.ops._C.b200_add_rms_norm(hidden, residual, weight, 1e-6, rows, q, s, 128)
+        w, ids, _ = topk_softmax((rows.float() @ router).contiguous(), K, True)
+        c.layer.apply(hidden, rows, w, ids)
+        return w, ids
+
+    start = c.x.clone()
+    hidden.copy_(start)
+    residual.copy_(start * 0.5)
+    eager = []
+    for _ in range(3):
+        before = (hidden.double() + residual.double()).to(BF16)
+        w, ids = step()
+        assert torch.equal(residual, before)
+        want = before.double() * (before.double().square().mean(-1, keepdim=True) + 1e-6).rsqrt() * weight.double()
+        # fp32 on the way (2^-18), then half a step of bfloat16
+        assert ((rows.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -18) * want.abs()).all()
+        back = q.double().view(T, H // 128, 128) * s.double()[..., None]
+        # half a step of e4m3 and of the scale's reciprocal; below the normal codes half of 2^-9 scales
+        assert ((back.view(T, H) - want).abs() <= (2.0 ** -4 + 2.0 ** -18) * want.abs() + 2.0 ** -10 * s.double().repeat_interleave(128, 1)).all()
+        c.x, c.weights, c.ids = rows, w, ids
+        c.check(hidden)
+        eager.append(hidden.clone())
+    torch.cuda.synchronize()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    hidden.copy_(start)
+    residual.copy_(start * 0.5)
+    for want in eager:
+        graph.replay()
+        assert torch.equal(hidden, want)
+
+
 def test_a_limit_on_the_blocks_changes_nothing(native):
     for recipe in ("w16", "fp8", "mxfp4"):
         c = Case(native, recipe, 7, 512, 384, 8, 3, seed=1)

@@ -36,6 +36,15 @@ template <int F> struct RowShape {
   static_assert(kWarps * kDepth * 8 <= 256, "barriers");
 };
 
+// The largest value of a step's lanes (half a warp, or a warp: one instruction).
+template <int kLanes>
+__device__ __forceinline__ uint32_t max_of_step(uint32_t v) {
+  if constexpr (kLanes == 32) return __reduce_max_sync(0xffffffffu, v);
+#pragma unroll
+  for (int d = 1; d < kLanes; d <<= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+
 // ---- tokens and activations as float16 -------------------------------------------------
 // A panel holds rows of values in the order in which the lanes want them: per step blocks of [row][4 lanes][8 values].  fp8
 // lanes hold 16 bytes of a row, 16 values; of int4 16 bytes, 32 values; where groups are 32 values they are handed out to
@@ -109,8 +118,7 @@ __device__ __noinline__ void fill_token(uint8_t* panel, float* floats, const voi
         v[2 * k + 1] = f16 ? f.y : __uint_as_float(raw[i].w[k] & 0xffff0000u);
         top = max(top, max(__float_as_uint(v[2 * k]) & 0x7fffffffu, __float_as_uint(v[2 * k + 1]) & 0x7fffffffu));
       }
-#pragma unroll
-      for (int d = 1; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+      top = max_of_step<kLanes>(top);
       float inverse;
       const float scale = step_scale(top, inverse);
       uint32_t o[4];
@@ -181,9 +189,7 @@ __device__ __noinline__ void fill_h(uint8_t* panel, float* floats, void* h, int 
     for (int i = 0; i < 4; ++i) {
       const int j = j0 + i * stride;
       if (j - lane >= len) break;
-      int top = e[i];
-#pragma unroll
-      for (int d = 1; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const int top = (int)max_of_step<kLanes>(e[i]);
       // (2^(e - top) as float16; below 2^-24 nothing is left)
       const int down = top - e[i];
       const __half f = __ushort_as_half(down < 15 ? (unsigned short)((15 - down) << 10) : down < 25 ? (unsigned short)(1 << (24 - down)) : (unsigned short)0);

@@ -294,6 +294,7 @@ __global__ void __launch_bounds__(ColumnShape<F>::kThreads, 1) few_up_columns_ke
     *gave_up = 0;
     ptx::prefetch_tensormap(&map);
   }
+  prefetch_call(p, tid, kThreads);
   pdl_wait();
   pdl_trigger();
   const FewMatrix& m = p.w13;

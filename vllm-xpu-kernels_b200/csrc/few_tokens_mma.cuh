@@ -157,6 +157,17 @@ __device__ __forceinline__ void sts4(uint32_t a, float x) { asm volatile("st.sha
 // Barrier of some of the block's warps.
 __device__ __forceinline__ void group_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
+// What a call is given, into L2 while the kernels ahead of it finish (nothing is read yet: they may still write it).
+__device__ __forceinline__ void prefetch_call(const FewParams& p, int tid, int threads) {
+  const int slots = p.tokens * p.topk;
+  const char* const ids = reinterpret_cast<const char*>(p.ids), * const x = reinterpret_cast<const char*>(p.x);
+  for (int i = tid * 128; i < slots * (p.ids64 ? 8 : 4); i += threads * 128) prefetch_l2(ids + i);
+  for (int i = tid * 128; i < slots * 4; i += threads * 128) prefetch_l2(reinterpret_cast<const char*>(p.weights) + i);
+  if (p.expert_map)
+    for (int i = tid * 32; i < p.id_limit; i += threads * 32) prefetch_l2(p.expert_map + i);
+  for (int i = tid * 128; i < p.tokens * p.hidden * 2; i += threads * 128) prefetch_l2(x + i);
+}
+
 // ---- conversions and products ------------------------------------------------------------
 // Four e4m3 codes of a word -> float16 pairs (0,1) (2,3).  (One instruction each; through the header's function, which takes
 // and returns halves of registers, seven for the two.)

@@ -515,6 +515,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
     ptx::prefetch_tensormap(&map);
     if (F != kFewFp8) ptx::prefetch_tensormap(&scale_map);
   }
+  prefetch_call(p, tid, kThreads);
   pdl_wait();
   pdl_trigger();
   const FewMatrix& m = p.w13;
@@ -530,13 +531,9 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
     if (tid < 48) reinterpret_cast<uint32_t*>(zeros)[tid - 32] = 0;
     if (blockIdx.x == 0)   // (the second kernel counts from there)
       for (int i = tid - 32; i < kFewMaxBlocks; i += kThreads - 32) launch.arrived[i] = 0;
-    if (early) {
+    if (early)
       fill_tokens_rows<F>(panel, reinterpret_cast<float*>(panel + p.tokens * steps * (S::kK * 2)), p.x, p.hidden, (1u << p.tokens) - 1u,
                           steps * (S::kK / 8), launch.f16, warp - 1, kWarps - 1);
-    } else {
-      const char* const x = reinterpret_cast<const char*>(p.x);
-      for (int i = (tid - 32) * 128; i < p.tokens * p.hidden * 2; i += (kThreads - 32) * 128) prefetch_l2(x + i);
-    }
   }
   __syncthreads();
   const uint32_t all = (uint32_t)(table.active * per_expert);     // (times the blocks below 2^32: takes_mma)

@@ -6,7 +6,14 @@
 // act(W13 x + b13), the second W2 h and what is made of it.
 //
 // tcgen05 would have to get its weights converted in shared or tensor memory, a second pass for every byte, and its tile
-// of 128 features leaves most SMs without work at one token.
+// of 128 features leaves most SMs without work at one token.  mma.sync is far from its limit here (0.4 instructions a cycle
+// and SM: 12 to 26 % of the time in use).
+//
+// What a call costs beyond its bytes (7 tokens of MXFP4 2880 x 2880, four of 128 experts, 80 us for 52 us of weights): finding the
+// experts 2.3 us in each kernel, the first weights' way 1, tokens and h on their way to shared memory 3 and 4, the sums of
+// the first kernel 2 to 4, of the second 1, the last of a column's blocks 1 to 2, and the kernels' ends, where blocks that
+// shared the memory evenly finish up to 4 us apart.  Asking for W2 ahead from the first kernel's end into L2 gained nothing (the second
+// kernel's loop is as long, the first one's 3 to 8 us longer), nor did both kernels on an SM at once with half the registers.
 #pragma once
 
 #include "few_tokens.cuh"
@@ -41,7 +48,7 @@ struct FewLaunch {
 struct FewTable {
   uint32_t bits[32];
   int before[32];
-  int active, rows;
+  int active;
   int expert[kMaxSlots];
   uint32_t tokens[kMaxSlots];
   int first_row[kMaxSlots + 1];
@@ -105,7 +112,7 @@ __device__ __forceinline__ void build_table(FewTable& t, const FewParams& p) {
     if (a < t.active) t.first_row[a] = base + sum - n;
     base += __shfl_sync(0xffffffffu, sum, 31);
   }
-  if (lane == 0) { t.first_row[t.active] = base; t.rows = base; }
+  if (lane == 0) t.first_row[t.active] = base;
   __syncwarp();
   if (kWeights) {
 #pragma unroll 1

@@ -186,6 +186,9 @@ int launch_columns(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   const int64_t want = (int64_t)p.tokens * p.topk * down_row;
   const int down_panel = at_least((int)(want < down_room ? want : down_room), RedShape<F, NT>::kBytes);
   l.room = down_panel / S::kPanelBytes(S::kTerms);
+  l.by_columns = FewDiv(l.columns);
+  l.by_splits = FewDiv(l.splits);
+  l.by_down_steps = FewDiv((p.inter + S::kK - 1) / S::kK);
   // loads of 32 gates, 32 ups or 64 columns in pairs; of 64 columns of W2
   CUtensorMap up_map, down_map;
   int rc = few_map<F>(&up_map, p.w13, p.experts, p.act == B200MOE_ACT_SWIGLUOAI ? 64 : 32);
@@ -214,6 +217,13 @@ int launch_rows(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   const int64_t want = (int64_t)p.tokens * p.topk * down_row;
   const int down_panel = (int)(want < down_room ? want : down_room);
   l.room = down_panel / S::kPanelBytes;
+  l.most = l.panel_bytes / up_row;
+  l.by_sets = FewDiv(p.inter / 16);
+  l.by_steps = FewDiv((p.hidden + S::kK - 1) / S::kK);
+  l.by_ctas = FewDiv(ctas);
+  l.by_columns = FewDiv(l.columns);
+  l.by_splits = FewDiv(l.splits);
+  l.by_down_steps = FewDiv((p.inter + S::kK - 1) / S::kK);
   CUtensorMap up_map, down_map, up_scales, down_scales;
   int rc = few_map<F>(&up_map, p.w13, p.experts, 16);
   if (rc == B200MOE_OK) rc = few_map<F>(&down_map, p.w2, p.experts, l.box);
@@ -311,6 +321,7 @@ extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200mo
   p.expert_map = a->expert_map; p.out = a->out; p.h = (float*)a->workspace;
   p.tokens = a->num_tokens; p.hidden = a->hidden; p.inter = a->inter; p.topk = a->topk;
   p.experts = a->num_experts; p.id_limit = a->expert_map ? a->total_experts : a->num_experts;
+  p.by_topk = FewDiv(a->topk);
   p.act = a->activation; p.alpha = a->act_alpha; p.limit = a->act_limit; p.clamp = a->clamp_limit;
   p.w13 = {a->w13, a->w13_scale, a->w13_bias, a->w13_format, a->w13_group, 2 * a->inter, a->hidden};
   p.w2 = {a->w2, a->w2_scale, a->w2_bias, a->w2_format, a->w2_group, a->hidden, a->inter};

@@ -16,6 +16,21 @@ struct FewMatrix {
   int n, k;
 };
 
+// Division by a number that the host knows: a quotient that is at most one too small, and put right.  (The device's own
+// takes some 20 instructions, and these kernels' way to their first loads is code that runs once.)
+struct FewDiv {
+  uint32_t d, m;
+  FewDiv() = default;
+  __host__ __device__ explicit FewDiv(uint32_t d) : d(d), m(0xffffffffu / d) {}
+};
+__device__ __forceinline__ int operator/(uint32_t n, const FewDiv& by) {
+  const uint32_t q = __umulhi(n, by.m);
+  return (int)(n - q * by.d >= by.d ? q + 1 : q);
+}
+__device__ __forceinline__ int operator/(int n, const FewDiv& by) { return (uint32_t)n / by; }
+// The same of small numbers (quotients and remainders below 2^20).
+__device__ __forceinline__ int small_div(int n, int d) { return (int)__fdividef((float)n + 0.5f, (float)d); }
+
 struct FewParams {
   const void* x;               // [tokens, hidden]
   const void* ids;             // [tokens, topk]
@@ -27,6 +42,7 @@ struct FewParams {
   int act;
   float alpha, limit, clamp;
   bool ids64;
+  FewDiv by_topk;
   FewMatrix w13, w2;
 };
 

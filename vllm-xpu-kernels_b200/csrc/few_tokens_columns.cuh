@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(ColumnShape<F>::kThreads, 1) few_down_columns_
   else if (tid < 48) reinterpret_cast<uint32_t*>(zeros)[tid - 32] = 0;
   __syncthreads();
   const FewMatrix& m = p.w2;
-  const FewShare share(table, p.inter, S::kK, launch);
+  const FewShare share(table, launch);
   const int steps = share.steps, step_begin = share.begin, step_end = share.end, row_begin = share.column * launch.side * kRows, row_end = p.hidden;
   const int side = launch.side, members = kWarps / side, member = warp / side, mine_side = warp % side, block_rows = side * kRows;
   float* const scales = reinterpret_cast<float*>(panel + launch.room * (S::kTerms * S::kK * 2));

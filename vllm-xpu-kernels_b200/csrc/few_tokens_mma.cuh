@@ -37,6 +37,9 @@ struct FewLaunch {
   int box;               // rows (by column: columns) of one of its warps, which a load brings
   int scale_box;         // rows of a load of its scales (4 bits)
   int room;              // rows of h times steps that its panel holds
+  int most;              // tokens that the first kernel's panel holds
+  FewDiv by_sets, by_steps, by_ctas;                // the first kernel's: sets of an expert, steps of a row, blocks
+  FewDiv by_columns, by_splits, by_down_steps;      // the second one's
   uint32_t* arrived;     // per column of its blocks
   float* part;           // [splits][tokens][hidden]: partial sums, with more than one split
   int32_t* status;       // for waits that run out, or NULL
@@ -90,7 +93,7 @@ __device__ __forceinline__ void build_table(FewTable& t, const FewParams& p) {
   bool again = false;      // a token that names an expert twice
 #pragma unroll 1
   for (int i = lane; i < slots; i += 32) {
-    const int e = t.slot_expert[i], tok = i / p.topk;
+    const int e = t.slot_expert[i], tok = i / p.by_topk;
     if (e < 0) continue;
     const int a = t.before[e >> 5] + rank_below(t.bits[e >> 5], e & 31);
     t.slot_expert[i] = a;
@@ -117,7 +120,7 @@ __device__ __forceinline__ void build_table(FewTable& t, const FewParams& p) {
   if (kWeights) {
 #pragma unroll 1
     for (int i = lane; i < slots; i += 32) {
-      const int a = t.slot_expert[i], tok = i / p.topk;
+      const int a = t.slot_expert[i], tok = i / p.by_topk;
       if (a < 0) continue;
       float w = t.slot_weight[i];
       if (again) {    // the token's slots with this expert in their order, by the first of them
@@ -214,7 +217,7 @@ __device__ __forceinline__ float step_scale(uint32_t top, float& inverse) {   //
 }
 
 // Warps of a row where `warps` of them fill a panel of `rows`.
-__device__ __forceinline__ int warps_per_row(int rows, int warps) { return rows >= warps ? 1 : warps / rows; }
+__device__ __forceinline__ int warps_per_row(int rows, int warps) { return rows >= warps ? 1 : small_div(warps, rows); }
 
 // ---- a warp's ring --------------------------------------------------------------------
 // A warp's ring, one slot after the other.
@@ -293,19 +296,21 @@ __device__ __noinline__ float weighted_bias(const FewTable& table, const FewMatr
 // What a block of the second kernel has to do: its column of blocks, and its share of the steps over all active experts.
 struct FewShare {
   int steps;                   // of an expert
+  FewDiv by_steps;
   int column, split, begin, end;
-  __device__ __forceinline__ FewShare(const FewTable& t, int inter, int step, const FewLaunch& l) {
-    steps = (inter + step - 1) / step;
-    split = blockIdx.x / l.columns;
+  __device__ __forceinline__ FewShare(const FewTable& t, const FewLaunch& l) {
+    steps = l.by_down_steps.d;
+    by_steps = l.by_down_steps;
+    split = blockIdx.x / l.by_columns;
     column = blockIdx.x - split * l.columns;
     const uint32_t total = (uint32_t)(t.active * steps);
-    begin = (int)(total * split / l.splits);
-    end = (int)(total * (split + 1) / l.splits);
+    begin = total * split / l.by_splits;
+    end = total * (split + 1) / l.by_splits;
   }
   // How far a panel reaches that begins with step s0 of expert a0: whole experts, then as many steps of the next one as
   // there is room for (at least one).
   __device__ __forceinline__ void panel_end(const FewTable& t, int room, int a0, int s0, int& a1, int& s1) const {
-    const int ae = end / steps, se = end - ae * steps;      // all that is left, if it fits
+    const int ae = end / by_steps, se = end - ae * steps;      // all that is left, if it fits
     const int need = ae == a0 ? (t.first_row[a0 + 1] - t.first_row[a0]) * (se - s0)
                               : (t.first_row[a0 + 1] - t.first_row[a0]) * (steps - s0) + (t.first_row[ae] - t.first_row[a0 + 1]) * steps +
                                     (se > 0 ? (t.first_row[ae + 1] - t.first_row[ae]) * se : 0);
@@ -316,7 +321,7 @@ struct FewShare {
     a1 = a0;
     s1 = s0;
     while (a1 * steps + s1 < end) {
-      const int n = t.first_row[a1 + 1] - t.first_row[a1], fit = min(min(steps - s1, end - a1 * steps - s1), free / n);
+      const int n = t.first_row[a1 + 1] - t.first_row[a1], fit = min(min(steps - s1, end - a1 * steps - s1), small_div(free, n));
       if (fit == 0) break;
       free -= fit * n;
       s1 += fit;
@@ -347,7 +352,7 @@ __device__ __forceinline__ void sum_splits(const FewLaunch& launch, const FewPar
     float v[4] = {};
 #pragma unroll
     for (int o = 0; o < 4; ++o) {
-      const int j = min(j0 + o * stride, all - 1), token = j / width;
+      const int j = min(j0 + o * stride, all - 1), token = small_div(j, width);
       from[o] = launch.part + (int64_t)token * p.hidden + row_begin + j - token * width;
     }
 #pragma unroll 3
@@ -356,7 +361,7 @@ __device__ __forceinline__ void sum_splits(const FewLaunch& launch, const FewPar
       for (int o = 0; o < 4; ++o) v[o] += __ldcg(from[o] + i * next);
 #pragma unroll
     for (int o = 0; o < 4; ++o) {
-      const int j = j0 + o * stride, token = j / width;
+      const int j = j0 + o * stride, token = small_div(j, width);
       if (j < all) finish(v[o], token, row_begin + j - token * width);
     }
   }

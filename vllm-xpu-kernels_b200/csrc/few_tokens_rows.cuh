@@ -141,12 +141,13 @@ template <int F>
 __device__ __noinline__ void fill_tokens_rows(uint8_t* panel, float* floats, const void* from, int hidden, uint32_t now, int len, bool f16, int warp,
                                               int warps) {
   const int rows = __popc(now), parts = warps_per_row(rows, warps);
+  const int together = small_div(warps, parts), mine = small_div(warp, parts), part = warp - mine * parts;      // rows at once, and this warp's
 #pragma unroll 1
-  for (int row = warp < warps / parts * parts ? warp / parts : rows; row < rows; row += warps / parts) {
+  for (int row = mine < together ? mine : rows; row < rows; row += together) {
     uint32_t left = now;
     for (int r = 0; r < row; ++r) left &= left - 1;
     const uint16_t* x = reinterpret_cast<const uint16_t*>(from) + (int64_t)(__ffs(left) - 1) * hidden;
-    fill_token<F>(panel, floats, x, hidden, len, row, rows, warp % parts, parts, f16);
+    fill_token<F>(panel, floats, x, hidden, len, row, rows, part, parts, f16);
   }
 }
 
@@ -293,7 +294,7 @@ __device__ __forceinline__ void find_row_tokens(RowTokens (&x)[NT], int count, u
   }
 }
 __device__ __forceinline__ int nth_bit(uint32_t bits, int n) {
-  for (int i = 0; i < n; ++i) bits &= bits - 1;
+  while (n-- > 0) bits &= bits - 1;
   return __ffs(bits) - 1;
 }
 template <int N> struct Int { static constexpr int value = N; };
@@ -524,8 +525,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
   pdl_wait();
   pdl_trigger();
   const FewMatrix& m = p.w13;
-  const int steps = (p.hidden + S::kK - 1) / S::kK, per_expert = p.inter / 16;
-  const int most = launch.panel_bytes / (steps * S::kPanelBytes); // rows that the panel holds
+  const int steps = launch.by_steps.d, per_expert = launch.by_sets.d, most = launch.most;
   // A few values are laid out while one warp finds the experts, which takes as long as a round of loads; more than that would keep
   // the weights from being asked for, and comes after it.
   const bool early = most >= p.tokens && p.tokens * p.hidden <= (kWarps - 1) * 1024;
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
   }
   __syncthreads();
   const uint32_t all = (uint32_t)(table.active * per_expert);     // (times the blocks below 2^32: takes_mma)
-  const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+  const int begin = all * blockIdx.x / launch.by_ctas, end = all * (blockIdx.x + 1) / launch.by_ctas;
   const bool pairs = p.act == B200MOE_ACT_SWIGLUOAI;
 
   // A pass: as many experts as have their tokens in the panel at once and their sums in shared memory; one with more tokens
@@ -550,20 +550,23 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
   struct Pass {
     int from, to, deep;            // sets; the most tokens that an expert has
     uint32_t now, rest;            // tokens in the panel, and of a later pass over the same sets
-    int total, workers;            // steps, and the warps that have any
-    __device__ __forceinline__ int start(int warp) const { return total * min(warp, workers) / workers; }
+    int total;                     // steps
+    FewDiv by_total;
+    // A warp's first step; fewer steps than warps: one each.
+    __device__ __forceinline__ int start(int warp) const { return total >= kWarps ? total * warp / kWarps : min(warp, total); }
+    __device__ __forceinline__ int warp_of(int step) const { return total >= kWarps ? (kWarps * (step + 1) - 1) / by_total : step; }
   };
   auto plan = [&](int from, int to, uint32_t rest) {       // from the set `from` on, or the rest of the tokens
     Pass pass;
     pass.from = from;
     pass.deep = min(__popc(rest), most);
     if (!rest) {
-      const int a_first = from / per_expert;
+      const int a_first = from / launch.by_sets;
       to = from;
       for (int a = a_first; to < end; ++a) {
         const uint32_t with = rest | table.tokens[a];
         const int n = max(pass.deep, min(__popc(table.tokens[a]), most)), stop = min(end, (a + 1) * per_expert);
-        const int room = UpRowsShape<F, NT>::kSums / (kSumColumn * 4 * n) - kWarps;             // sets
+        const int room = small_div(UpRowsShape<F, NT>::kSums / (kSumColumn * 4), n) - kWarps;             // sets
         if (rest && (__popc(with) > most || room <= to - from)) break;
         rest = with;
         pass.deep = n;
@@ -577,7 +580,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
     while (__popc(pass.now) > most) pass.now &= ~(1u << (31 - __clz(pass.now)));
     pass.rest = rest & ~pass.now;
     pass.total = (to - from) * steps;
-    pass.workers = min(kWarps, pass.total);
+    pass.by_total = FewDiv(max(pass.total, 1));
     return pass;
   };
 
@@ -589,7 +592,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
       if (fetch_s == steps) {
         fetch_s = fetch_s0;
         fetch_s0 = 0;
-        const int a = fetch_j / per_expert;
+        const int a = fetch_j / launch.by_sets;
         row = 16 * (fetch_j - a * per_expert);
         ++fetch_j;
         e = table.expert[a];
@@ -618,7 +621,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
     if (F == kFewFp8) copies_end();
   };
   auto start_fetch = [&](const Pass& pass) {
-    const int pos = pass.start(warp), j = pos / steps;
+    const int pos = pass.start(warp), j = pos / launch.by_steps;
     left = pass.start(warp + 1) - pos;
     fetch_j = pass.from + j;
     fetch_s0 = pos - j * steps;
@@ -640,13 +643,13 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
   }
 #pragma unroll 1
   while (pass.from < end) {
-    const int from = pass.from, total = pass.total, workers = pass.workers, deep = pass.deep, rows = __popc(pass.now);
-    const int pos0 = pass.start(warp), pos1 = pass.start(warp + 1), j0 = pos0 / steps, s0 = pos0 - j0 * steps;
+    const int from = pass.from, deep = pass.deep, rows = __popc(pass.now);
+    const int pos0 = pass.start(warp), pos1 = pass.start(warp + 1), j0 = pos0 / launch.by_steps, s0 = pos0 - j0 * steps;
     const uint32_t now = pass.now;
     const float* const floats = reinterpret_cast<float*>(panel + rows * steps * (S::kK * 2));
 #pragma unroll 1
     for (int pos = pos0, j = j0, s = s0; pos < pos1; ++j, s = 0) {
-      const uint32_t mine = table.tokens[(from + j) / per_expert] & now;
+      const uint32_t mine = table.tokens[(from + j) / launch.by_sets] & now;
       const int count = __popc(mine), stop = min(steps, s + pos1 - pos);
       pos += stop - s;
       // sets and warps begin a new entry each
@@ -678,11 +681,11 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(F
     // barrier, and for the next set before the sums of this one.
     struct { int a, f, w0, w1; float gate, up; } set;
     auto look_up = [&](int j) {
-      set.a = (from + j) / per_expert;
+      set.a = (from + j) / launch.by_sets;
       set.f = 16 * (from + j - set.a * per_expert) + (lane & 15);
       // the warps that had the set's first and last step
-      set.w0 = (workers * (j * steps + 1) - 1) / total;
-      set.w1 = (workers * (j + 1) * steps - 1) / total;
+      set.w0 = pass.warp_of(j * steps);
+      set.w1 = pass.warp_of((j + 1) * steps - 1);
       set.gate = set.up = 0.f;
       if (m.bias) {
         const int64_t at = (int64_t)table.expert[set.a] * m.n;
@@ -763,9 +766,9 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
   else if (tid < 48) reinterpret_cast<uint32_t*>(zeros)[tid - 32] = 0;
   __syncthreads();
   const FewMatrix& m = p.w2;
-  const FewShare share(table, p.inter, S::kK, launch);
+  const FewShare share(table, launch);
   const int steps = share.steps, member = warp >> 1, warp_rows = launch.box;
-  const int row_begin = (int)((uint32_t)p.hidden * share.column / launch.columns), row_end = (int)((uint32_t)p.hidden * (share.column + 1) / launch.columns);
+  const int row_begin = (uint32_t)p.hidden * share.column / launch.by_columns, row_end = (uint32_t)p.hidden * (share.column + 1) / launch.by_columns;
   float* const floats = reinterpret_cast<float*>(panel + launch.room * (S::kK * 2));
   bool waited = false;
   auto finish = [&](float v, int token, int n) {
@@ -777,7 +780,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
     const int r0 = block_r0 + (warp & 1) * warp_rows, rows_here = max(0, min(warp_rows, row_end - r0));
     const RowScales layout = {scale_words_of_step(m), ((r0 & 3) + lane) * 4, launch.scale_box * 4, launch.f16};
     // The step that is fetched next, how many are left of this warp's stretch, and where the panel after that begins.
-    int fetch_a = 0, fetch_s = 0, left = 0, panel_a = share.begin / steps, panel_s = share.begin - panel_a * steps, e = 0;
+    int fetch_a = 0, fetch_s = 0, left = 0, panel_a = share.begin / share.by_steps, panel_s = share.begin - panel_a * steps, e = 0;
     bool found = false;
     const uint8_t* scale = nullptr;
     auto copy_next = [&](int slot) {
@@ -786,7 +789,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
         share.panel_end(table, launch.room, panel_a, panel_s, a1, s1);
         const int from = panel_a * steps + panel_s, all = a1 * steps + s1 - from, mine = all * member / kMembers;
         left = all * (member + 1) / kMembers - mine;
-        fetch_a = (from + mine) / steps;
+        fetch_a = (from + mine) / share.by_steps;
         fetch_s = from + mine - fetch_a * steps;
         panel_a = a1;
         panel_s = s1;
@@ -835,7 +838,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
     }
     for (int i = lane; i < p.tokens * kSumColumn; i += 32) sums[warp * p.tokens * kSumColumn + i] = 0.f;
     __syncwarp();
-    for (int a0 = share.begin / steps, s0 = share.begin - a0 * steps; a0 * steps + s0 < share.end;) {
+    for (int a0 = share.begin / share.by_steps, s0 = share.begin - a0 * steps; a0 * steps + s0 < share.end;) {
       int a1, s1;
       share.panel_end(table, launch.room, a0, s0, a1, s1);
       const int last = s1 > 0 ? a1 : a1 - 1;           // the last expert with steps in the panel
@@ -844,13 +847,14 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
         // (the first expert's rows have the steps from s0 on, the last one's those up to s1)
         constexpr int kPiece = S::kK / 8;
         const int parts = warps_per_row(rows, kWarps), n0 = table.first_row[a0 + 1] - row0;
+        const int together = small_div(kWarps, parts), mine = small_div(warp, parts), part = warp - mine * parts;
 #pragma unroll 1
-        for (int row = warp / parts; row < rows; row += kWarps / parts) {
+        for (int row = mine; row < rows; row += together) {
           const int r = row0 + row, a = table.row_expert[r], e0 = table.first_row[a], n = table.first_row[a + 1] - e0;
           const int k8_0 = (a == a0 ? s0 : 0) * kPiece, len = (a == a1 ? s1 : steps) * kPiece - k8_0;
           const int before = a == a0 ? 0 : n0 * (steps - s0) + (e0 - row0 - n0) * steps;   // rows times steps of earlier experts
           fill_h<F>(panel + before * (S::kK * 2), floats + before * S::kFloats, p.h, r, 8 * k8_0, p.inter, p.tokens * p.topk, len, r - e0, n,
-                    warp % parts, parts);
+                    part, parts);
         }
         __syncthreads();
       }
@@ -858,7 +862,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
         const int from = a0 * steps + s0, all = a1 * steps + s1 - from;
         int pos = from + all * member / kMembers;
         const int stop = rows_here > 0 ? from + all * (member + 1) / kMembers : 0;
-        for (int a = pos / steps; pos < stop; ++a) {
+        for (int a = pos / share.by_steps; pos < stop; ++a) {
           const int row = table.first_row[a], n_rows = table.first_row[a + 1] - row, end = min(stop, (a + 1) * steps);
           // rows of earlier experts in the panel, as above
           const int before = (a == a0 ? 0 : (table.first_row[a0 + 1] - row0) * (steps - s0) + (row - table.first_row[a0 + 1]) * steps) - (a == a0 ? s0 : 0) * n_rows;

@@ -281,7 +281,7 @@ template <int F, int NT> struct UpColumnsShape {
 // long runs; where fewer pieces are left than warps times tiles several have the same ones, take their steps in turn and add
 // their sums up in shared memory.
 template <int F, int NT>
-__global__ void __launch_bounds__(ColumnShape<F>::kThreads, 1) few_up_columns_kernel(FewParams p, FewLaunch launch, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(ColumnShape<F>::kThreads, 1) few_up_columns_kernel(const __grid_constant__ FewParams p, const __grid_constant__ FewLaunch launch, const __grid_constant__ CUtensorMap map) {
   using S = ColumnShape<F>;
   constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kTiles = S::kTiles;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(ColumnShape<F>::kThreads, 1) few_up_columns_ke
 // through its steps with as many of h's values at a time as its panel holds, each group of warps with a stretch of them.  Of the blocks
 // with the same columns the last one to be done adds the partial sums up, in their order.
 template <int F, int NT>
-__global__ void __launch_bounds__(ColumnShape<F>::kThreads, 1) few_down_columns_kernel(FewParams p, FewLaunch launch, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(ColumnShape<F>::kThreads, 1) few_down_columns_kernel(const __grid_constant__ FewParams p, const __grid_constant__ FewLaunch launch, const __grid_constant__ CUtensorMap map) {
   using S = ColumnShape<F>;
   constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kTiles = S::kTiles, kRows = S::kRows;
   extern __shared__ __align__(1024) uint8_t smem[];

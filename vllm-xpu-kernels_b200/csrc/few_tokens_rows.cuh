@@ -503,7 +503,7 @@ template <int F, int NT> struct UpRowsShape {
 // of a set goes into shared memory, and at the end of a pass all that there is of a set is added up in the warps' order: one
 // barrier a pass instead of one a set (which cost 4 to 10 us of the kernel).
 template <int F, int NT>
-__global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(FewParams p, FewLaunch launch, const __grid_constant__ CUtensorMap map,
+__global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(const __grid_constant__ FewParams p, const __grid_constant__ FewLaunch launch, const __grid_constant__ CUtensorMap map,
                                                                                const __grid_constant__ CUtensorMap scale_map) {
   using S = RowShape<F>;
   constexpr int kWarps = S::kWarps, kThreads = S::kThreads;
@@ -741,7 +741,7 @@ __host__ __device__ __forceinline__ int down_sums_bytes(int tokens, int warps) {
 // SMs.  It goes through its steps with as many of h's values at a time as its panel holds, each warp with a stretch of them,
 // half of the rows each.  Of the blocks with the same rows the last one to be done adds the partial sums up, in their order.
 template <int F, int NT>
-__global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel(FewParams p, FewLaunch launch, const __grid_constant__ CUtensorMap map,
+__global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel(const __grid_constant__ FewParams p, const __grid_constant__ FewLaunch launch, const __grid_constant__ CUtensorMap map,
                                                                                  const __grid_constant__ CUtensorMap scale_map) {
   using S = RowShape<F>;
   constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kMembers = kWarps / 2;

@@ -551,10 +551,9 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(c
     int from, to, deep;            // sets; the most tokens that an expert has
     uint32_t now, rest;            // tokens in the panel, and of a later pass over the same sets
     int total;                     // steps
-    FewDiv by_total;
     // A warp's first step; fewer steps than warps: one each.
     __device__ __forceinline__ int start(int warp) const { return total >= kWarps ? total * warp / kWarps : min(warp, total); }
-    __device__ __forceinline__ int warp_of(int step) const { return total >= kWarps ? (kWarps * (step + 1) - 1) / by_total : step; }
+    __device__ __forceinline__ int warp_of(int step, const FewDiv& by_total) const { return total >= kWarps ? (kWarps * (step + 1) - 1) / by_total : step; }
   };
   auto plan = [&](int from, int to, uint32_t rest) {       // from the set `from` on, or the rest of the tokens
     Pass pass;
@@ -580,7 +579,6 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(c
     while (__popc(pass.now) > most) pass.now &= ~(1u << (31 - __clz(pass.now)));
     pass.rest = rest & ~pass.now;
     pass.total = (to - from) * steps;
-    pass.by_total = FewDiv(max(pass.total, 1));
     return pass;
   };
 
@@ -646,6 +644,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(c
     const int from = pass.from, deep = pass.deep, rows = __popc(pass.now);
     const int pos0 = pass.start(warp), pos1 = pass.start(warp + 1), j0 = pos0 / launch.by_steps, s0 = pos0 - j0 * steps;
     const uint32_t now = pass.now;
+    const FewDiv by_total(pass.total);
     const float* const floats = reinterpret_cast<float*>(panel + rows * steps * (S::kK * 2));
 #pragma unroll 1
     for (int pos = pos0, j = j0, s = s0; pos < pos1; ++j, s = 0) {
@@ -684,8 +683,8 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(c
       set.a = (from + j) / launch.by_sets;
       set.f = 16 * (from + j - set.a * per_expert) + (lane & 15);
       // the warps that had the set's first and last step
-      set.w0 = pass.warp_of(j * steps);
-      set.w1 = pass.warp_of((j + 1) * steps - 1);
+      set.w0 = pass.warp_of(j * steps, by_total);
+      set.w1 = pass.warp_of((j + 1) * steps - 1, by_total);
       set.gate = set.up = 0.f;
       if (m.bias) {
         const int64_t at = (int64_t)table.expert[set.a] * m.n;
@@ -821,16 +820,11 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
     };
 #pragma unroll 1
     for (int i = 0; i < S::kDepth; ++i) copy_next((ring.slot + i) % S::kDepth);
-    // Biases while the ring fills, by the blocks with the first share.
-    constexpr int kMine = (B200MOE_FEW_TOKENS * kBlockRows + kThreads - 1) / kThreads;
     const int block_rows_here = min(2 * warp_rows, row_end - block_r0), my_row = tid % kBlockRows, my_token = tid / kBlockRows;
-    float bias[kMine];
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int token = my_token + i * (kThreads / kBlockRows);
-      bias[i] = m.bias && share.split == 0 && token < p.tokens && my_row < block_rows_here
-                    ? weighted_bias(table, m, p.topk, launch.f16, token, block_r0 + my_row) : 0.f;
-    }
+    const bool with_bias = m.bias && share.split == 0;           // (by the blocks with the first share)
+    if (with_bias)
+      for (int i = tid; i < 2 * table.active; i += kThreads)     // into L2: what is needed once the products are done
+        prefetch_l2(reinterpret_cast<const uint16_t*>(m.bias) + (int64_t)table.expert[i >> 1] * m.n + ((i & 1) ? block_r0 + block_rows_here - 1 : block_r0));
     if (!waited) {
       pdl_wait();
       pdl_trigger();
@@ -896,7 +890,15 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
       }
       a0 = a1;
       s0 = s1;
-      __syncthreads();   // the panel is free again
+      if (a0 * steps + s0 < share.end) __syncthreads();   // the panel is free again
+    }
+    // Biases while other warps are still at work.
+    constexpr int kMine = (B200MOE_FEW_TOKENS * kBlockRows + kThreads - 1) / kThreads;
+    float bias[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int token = my_token + i * (kThreads / kBlockRows);
+      bias[i] = with_bias && token < p.tokens && my_row < block_rows_here ? weighted_bias(table, m, p.topk, launch.f16, token, block_r0 + my_row) : 0.f;
     }
     if (F == kFewFp8) copies_wait<0>();
     __syncthreads();

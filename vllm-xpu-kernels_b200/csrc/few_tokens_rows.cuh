@@ -676,10 +676,12 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(c
       if (NT == 1 || count <= 8) take(Int<1>{});
       else take(Int<NT>{});
     }
-    // A warp has a set, a lane one of its features, for one token of two.  What does not need the sums is there before the
-    // barrier, and for the next set before the sums of this one.
+    // Half a warp has a set, a lane one of its features.  What does not need the sums is there before the barrier, and for the
+    // next set before the sums of this one.
     struct { int a, f, w0, w1; float gate, up; } set;
+    const int sets = pass.to - from;
     auto look_up = [&](int j) {
+      j = min(j, sets - 1);
       set.a = (from + j) / launch.by_sets;
       set.f = 16 * (from + j - set.a * per_expert) + (lane & 15);
       // the warps that had the set's first and last step
@@ -692,34 +694,34 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(c
         set.up = load16(m.bias, at + (pairs ? 2 * set.f + 1 : p.inter + set.f), launch.f16);
       }
     };
-    const int sets = pass.to - from, gate_row = pairs ? 2 * (lane & 15) : lane & 15, up_row = pairs ? gate_row + 1 : 16 + gate_row;
+    const int gate_row = pairs ? 2 * (lane & 15) : lane & 15, up_row = pairs ? gate_row + 1 : 16 + gate_row;
     const float* const gates = sums + sum_of_row(gate_row), * const ups = sums + sum_of_row(up_row);
-    if (warp < sets) look_up(warp);
+    if (2 * warp < sets) look_up(2 * warp + (lane >> 4));
     // the next pass's weights are on their way meanwhile
     const Pass next = pass.rest ? plan(from, pass.to, pass.rest) : plan(pass.to, pass.to, 0);
     if (next.from < end) start_fetch(next);
     __syncthreads();   // the sums are complete, and the panel is free again
 #pragma unroll 1
-    for (int j = warp; j < sets; j += kWarps) {
+    for (int j0 = 2 * warp; j0 < sets; j0 += 2 * kWarps) {
       const auto here = set;
-      if (j + kWarps < sets) look_up(j + kWarps);
+      const int j = j0 + (lane >> 4);
+      if (j0 + 2 * kWarps < sets) look_up(j + 2 * kWarps);
       const uint32_t have = table.tokens[here.a];
-      uint32_t later = have & now;
-      for (int rank = 0; later; rank += 2) {        // (two tokens: the lower and the upper half of the warp)
-        const uint32_t after = later & (later - 1);
-        const int my_rank = rank + (lane >> 4), token = __ffs(lane < 16 ? later : after) - 1;
+      uint32_t later = j < sets ? have & now : 0;
+      for (int rank = 0; __any_sync(0xffffffffu, later != 0); ++rank) {
+        const int token = __ffs(later) - 1;
         float v = 0.f;
         if (token >= 0) {
           float gate = here.gate, up = here.up;
           for (int w = here.w0; w <= here.w1; ++w) {
-            const int at = ((j + w) * deep + my_rank) * kSumColumn;
+            const int at = ((j + w) * deep + rank) * kSumColumn;
             gate += gates[at];
             up += ups[at];
           }
           v = gated_once(p.act, p.alpha, p.limit, p.clamp, gate, up);
         }
         store_h(p.h, table.first_row[here.a] + (token >= 0 ? rank_below(have, token) : 0), here.f, p.inter, p.tokens * p.topk, v, token >= 0);
-        later = after & (after - 1);
+        later &= later - 1;
       }
     }
     if (next.from < end) {

@@ -9,9 +9,9 @@
 // of 128 features leaves most SMs without work at one token.  mma.sync is far from its limit here (0.4 instructions a cycle
 // and SM: 12 to 26 % of the time in use).
 //
-// What a call costs beyond its bytes (7 tokens of MXFP4 2880 x 2880, four of 128 experts, 80 us for 52 us of weights): finding the
-// experts 2.3 us in each kernel, the first weights' way 1, tokens and h on their way to shared memory 3 and 4, the sums of
-// the first kernel 2 to 4, of the second 1, the last of a column's blocks 1 to 2, and the kernels' ends, where blocks that
+// What a call costs beyond its bytes (7 tokens of MXFP4 2880 x 2880, four of 128 experts, 75 us for 52 us of weights): finding the
+// experts 1.3 us in each kernel (with more than 32 routed slots 2.3), the first weights' way 2, tokens and h on their way to shared
+// memory 2.5 each, the sums of the first kernel 2 to 3, of the second 1, the last of a column's blocks 1, and the kernels' ends, where blocks that
 // shared the memory evenly finish up to 4 us apart.  Asking for W2 ahead from the first kernel's end into L2 gained nothing (the second
 // kernel's loop is as long, the first one's 3 to 8 us longer), nor did both kernels on an SM at once with half the registers.
 #pragma once

@@ -7,7 +7,7 @@
 // holds every code of the three formats exactly), and the tokens are laid out to match.  Scales of weights multiply the sums of
 // their group in fp32.
 //
-// Bound by the weights' bytes with few tokens of large experts: 7168 x 2048 fp8, 8 of 256 experts, one token 67 us, 5.3 TB/s (its
+// Bound by the weights' bytes with few tokens of large experts: 7168 x 2048 fp8, 8 of 256 experts, one token 65 us, 5.4 TB/s (its
 // main loops alone 6.5); with small ones by what a call costs besides (few_tokens_mma.cuh).  MXFP4 and int4 come near the issue rate: a byte is
 // two conversions, and its products are as many as those of two bytes of fp8 (2880 x 2880, 7 tokens: 50 % of the issue slots, 44 % of the
 // ALU's cycles; int4 4 tokens 53 % of the ALU's).

@@ -48,8 +48,8 @@ __device__ __forceinline__ float scale_of(float amax, bool ue8m0) {
   return ue8m0 ? up_to_pow2(s) : s;
 }
 
-// Any size, stride and alignment: a block per row, one value at a time.  Every thread comes back to its own values
-// only, so that `out` may be the input's memory.
+// Any size, stride and alignment: a block per row, one value at a time, four of a thread asked for together.  Every thread
+// comes back to its own values only, so that `out` may be the input's memory.
 template <typename T, typename W>
 __global__ void __launch_bounds__(256) rms_norm_scalar_kernel(RmsParams p) {
   pdl_trigger();
@@ -63,18 +63,30 @@ __global__ void __launch_bounds__(256) rms_norm_scalar_kernel(RmsParams p) {
   const W* w = reinterpret_cast<const W*>(p.weight);
   float sum = 0.f, top = 0.f;
   // A warp owns whole groups, so that what it wrote to the residual is what it reads again.
-  const int group = p.q && p.group ? p.group : 32;
+  const int group = p.q && p.group ? p.group : 128;
   for (int g0 = warp * group; g0 < p.hidden; g0 += 8 * group) {
     const int end = min(g0 + group, p.hidden);
-    for (int i = g0 + lane; i < end; i += 32) {
-      float v = to_f32<T>(x[i]);
-      if (res) {
-        const T t = from_f32<T>(v + to_f32<T>(res[i]));
-        res[i] = t;
-        v = to_f32<T>(t);
+    for (int i0 = g0 + lane; i0 < end; i0 += 128) {
+      float v[4], r[4], f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + 32 * k;
+        v[k] = i < end ? to_f32<T>(x[i]) : 0.f;
+        r[k] = res && i < end ? to_f32<T>(res[i]) : 0.f;
+        f[k] = w && i < end ? to_f32<W>(w[i]) : 1.f;
       }
-      sum = fmaf(v, v, sum);
-      top = max_nan(top, fabsf(w ? v * to_f32<W>(w[i]) : v));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + 32 * k;
+        if (i >= end) break;
+        if (res) {
+          const T t = from_f32<T>(v[k] + r[k]);
+          res[i] = t;
+          v[k] = to_f32<T>(t);
+        }
+        sum = fmaf(v[k], v[k], sum);
+        top = max_nan(top, fabsf(v[k] * f[k]));
+      }
     }
   }
 #pragma unroll
@@ -101,6 +113,7 @@ __global__ void __launch_bounds__(256) rms_norm_scalar_kernel(RmsParams p) {
     const int end = min(g0 + group, p.hidden);
     if (q && p.group) {
       float m = 0.f;
+#pragma unroll 4
       for (int i = g0 + lane; i < end; i += 32) {
         const float n = to_f32<T>(s[i]) * rs;
         m = max_nan(m, fabsf(w ? n * to_f32<W>(w[i]) : n));
@@ -111,11 +124,21 @@ __global__ void __launch_bounds__(256) rms_norm_scalar_kernel(RmsParams p) {
       inv = __fdiv_rn(1.0f, scale);
       if (lane == 0) p.scales[r * p.s_stride_row + (int64_t)(g0 / group) * p.s_stride_group] = scale;
     }
-    for (int i = g0 + lane; i < end; i += 32) {
-      const float n = to_f32<T>(s[i]) * rs;
-      const float y = w ? n * to_f32<W>(w[i]) : n;
-      if (out) out[i] = from_f32<T>(y);
-      if (q) q[i] = f32_to_e4m3(y * inv);
+    for (int i0 = g0 + lane; i0 < end; i0 += 128) {
+      float y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + 32 * k;
+        const float n = i < end ? to_f32<T>(s[i]) * rs : 0.f;
+        y[k] = w && i < end ? n * to_f32<W>(w[i]) : n;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + 32 * k;
+        if (i >= end) break;
+        if (out) out[i] = from_f32<T>(y[k]);
+        if (q) q[i] = f32_to_e4m3(y[k] * inv);
+      }
     }
   }
 }
@@ -306,11 +329,11 @@ int launch_rms_norm(const RmsParams& p, cudaStream_t st) {
   constexpr int N = 32 / sizeof(T), kSingles = 8;
   if (pieces_fit(p, N, sizeof(T), sizeof(W))) return launch_mode<T, W, N, 1>(p, st);
   if (pieces_fit(p, N / 2, sizeof(T), sizeof(W))) return launch_mode<T, W, N / 2, 1>(p, st);
-  // Rows that cannot be cut into pieces: kept in registers value by value where that saves the second way through them, whose latency
-  // counts with few rows; with many the kernel below has more of them on an SM.  us, in registers / below: 1411 bf16 values, 61 rows
-  // 4.9 / 7.4, 256 rows 6.6 / 8.1, 1001 rows 11.3 / 10.6, 8192 rows 82 / 63; 5001 values, 61 rows 6.0 / 20, 8192 rows 402 / 188;
-  // 99 values, 8192 rows 9.4 / 15.9.
-  if (p.hidden <= 1024 * kSingles && (p.rows <= 512 || p.hidden < 256) && (p.q == nullptr || p.group == 0))
+  // Rows that cannot be cut into pieces: kept in registers value by value where that saves the second way through long rows, whose
+  // latency counts with few of them, or where many short ones would have a block each.  us, in registers / below: 1411 bf16 values,
+  // 61 rows 5.0 / 5.0, 256 rows 6.5 / 5.8, 8192 rows 82 / 64; 5001 values, 61 rows 6.0 / 10.0, 256 rows 11.9 / 12.9, 1001 rows 45 /
+  // 28; 99 values, 1001 rows 4.3 / 4.0, 8192 rows 9.4 / 18.
+  if (p.hidden <= 1024 * kSingles && (p.hidden > 2048 ? p.rows <= 256 : p.hidden < 256 && p.rows > 1024) && (p.q == nullptr || p.group == 0))
     return launch_mode<T, W, 1, kSingles>(p, st);
   B200_LAUNCHED("rms_norm_scalar_kernel",
                 launch_pdl(p.rows <= kEarlyLaunchRows, rms_norm_scalar_kernel<T, W>, dim3((unsigned)p.rows), dim3(256), 0, st, p));

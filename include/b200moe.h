@@ -620,10 +620,12 @@ typedef struct {
   void* out;                  /* [num_tokens, hidden] dtype                           */
   /* weights [num_experts, ...]: 16-bit [E,K,N] (of dtype), block-scaled fp8 (either
      layout), MXFP4 or int4, as b200moe_grouped_gemm takes them; biases [E,N] of dtype or
-     NULL; N x K of w13 is 2*inter x hidden, of w2 hidden x inter.  The scales of MXFP4 and
-     int4 weights are laid out anew: 32-bit words [num_experts][words][N] (4 e8m0 bytes,
-     or two 16-bit scales; groups of 256 as two of 128; in the order of k, the last ones
-     filled up with zeros), words = b200moe_few_tokens_scale_words                      */
+     NULL; N x K of w13 is 2*inter x hidden, of w2 hidden x inter.  Scales as
+     b200moe_grouped_gemm takes them with b200moe_few_tokens_layer_as_stored; with
+     b200moe_few_tokens_layer those of MXFP4 and int4 weights are laid out anew by the
+     caller: 32-bit words [num_experts][words][N] (4 e8m0 bytes, or two 16-bit scales;
+     groups of 256 as two of 128; in the order of k, the last ones filled up with zeros),
+     words = b200moe_few_tokens_scale_words                                             */
   const void *w13, *w13_scale, *w13_bias;
   const void *w2, *w2_scale, *w2_bias;
   void* workspace;            /* b200moe_few_tokens_workspace_bytes, 16-byte aligned; its
@@ -643,6 +645,7 @@ typedef struct {
 int b200moe_few_tokens_scale_words(b200moe_weight_format format, int group_size, int k);
 size_t b200moe_few_tokens_workspace_bytes(int num_tokens, int topk, int hidden, int inter);
 int b200moe_few_tokens_layer(const b200moe_few_tokens_args* args, b200moe_stream stream);
+int b200moe_few_tokens_layer_as_stored(const b200moe_few_tokens_args* args, b200moe_stream stream);
 
 /* ------------------------------------------------------------------------- */
 /* Expert parallelism over peer memory                                        */

@@ -14,6 +14,11 @@
 namespace b200moe {
 namespace {
 
+// Byte i of the scales of a 4-bit matrix's row.
+__device__ __forceinline__ const uint8_t* scale_at(const FewMatrix& w, int64_t e, int n, int i) {
+  return reinterpret_cast<const uint8_t*>(w.scale) + e * w.n * w.scales.bytes + (int64_t)n * w.scales.row + (int64_t)(i / 4) * w.scales.next + i % 4;
+}
+
 // One weight, W_e[n, k], in fp32.
 template <typename T>
 __device__ __forceinline__ float weight_at(const FewMatrix& w, int64_t e, int n, int k) {
@@ -29,13 +34,11 @@ __device__ __forceinline__ float weight_at(const FewMatrix& w, int64_t e, int n,
     case B200MOE_W_INT4_NK: {
       const uint8_t q = b[(e * N + n) * (K / 2) + k / 2];
       const int v = (int)(((k & 1) ? (q >> 4) : (q & 15)) ^ 8) - 8;
-      const int i = k / (w.group < 128 ? w.group : 128);   // of the row's 16-bit scales, two a word
-      return (float)v * to_f32<T>(reinterpret_cast<const T*>(w.scale)[((e * few_scale_words(w.format, w.group, w.k) + i / 2) * N + n) * 2 + i % 2]);
+      return (float)v * to_f32<T>(*reinterpret_cast<const T*>(scale_at(w, e, n, k / (512 / w.scales.step) * 2)));
     }
     default: {
       const uint8_t q = b[(e * N + n) * (K / 2) + k / 2];
-      return e2m1_to_f32((k & 1) ? (q >> 4) : (q & 15)) *
-             e8m0_to_f32(reinterpret_cast<const uint8_t*>(w.scale)[((e * few_scale_words(w.format, 0, w.k) + k / 128) * N + n) * 4 + k / 32 % 4]);
+      return e2m1_to_f32((k & 1) ? (q >> 4) : (q & 15)) * e8m0_to_f32(*scale_at(w, e, n, k / 32));
     }
   }
 }
@@ -141,7 +144,7 @@ int few_splits(int64_t hidden, int ctas, int rows) {
   return n < 1 ? 1 : (int)std::min<int64_t>(n, std::min(ctas, kMaxSplits));
 }
 
-// The map of a matrix for loads of `box` rows (by column: columns) of a step, and that of its scales (4 bits).
+// The map of a matrix for loads of `box` rows (by column: columns) of a step.
 template <int F>
 int few_map(CUtensorMap* map, const FewMatrix& m, int experts, int box) {
   if constexpr (by_column(F)) {
@@ -158,15 +161,6 @@ int few_map(CUtensorMap* map, const FewMatrix& m, int experts, int box) {
     return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, m.w, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_128B);
   }
 }
-int few_scale_map(CUtensorMap* map, const FewMatrix& m, int experts, int box) {
-  const cuuint64_t words = few_scale_words(m.format, m.group, m.k);
-  const cuuint64_t dims[3] = {(cuuint64_t)m.n, words, (cuuint64_t)experts};
-  const cuuint64_t strides[2] = {(cuuint64_t)m.n * 4, (cuuint64_t)m.n * 4 * words};
-  const int step = m.format == B200MOE_W_MXFP4_NK ? 2 : m.group == 32 ? 4 : m.group == 64 ? 2 : 1;       // words of 256 values
-  const cuuint32_t boxes[3] = {(cuuint32_t)box, (cuuint32_t)step, 1};
-  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, m.scale, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_NONE);
-}
-
 int at_least(int a, int b) { return a < b ? b : a; }
 
 // The kernels' shared memory: what they always need, and a panel of tokens or h.
@@ -209,11 +203,10 @@ int launch_rows(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   l.panel_bytes = min(p.tokens * up_row, up_room / up_row * up_row);
   l.splits = few_splits(p.hidden, ctas, kBlockRows);
   l.columns = min(ctas / l.splits, (p.hidden + 15) / 16);
-  // a block's rows in as few turns as they need, and halved in each; scales from a multiple of four rows on
+  // a block's rows in as few turns as they need, and halved in each
   const int rows = (p.hidden + l.columns - 1) / l.columns, turns = (rows + kBlockRows - 1) / kBlockRows;
   l.side = 2;
   l.box = (rows + 2 * turns - 1) / (2 * turns);
-  l.scale_box = (l.box + 3 + 3) / 4 * 4;
   const int64_t want = (int64_t)p.tokens * p.topk * down_row;
   const int down_panel = (int)(want < down_room ? want : down_room);
   l.room = down_panel / S::kPanelBytes;
@@ -224,21 +217,14 @@ int launch_rows(const FewParams& p, FewLaunch l, int ctas, cudaStream_t st) {
   l.by_columns = FewDiv(l.columns);
   l.by_splits = FewDiv(l.splits);
   l.by_down_steps = FewDiv((p.inter + S::kK - 1) / S::kK);
-  CUtensorMap up_map, down_map, up_scales, down_scales;
+  CUtensorMap up_map, down_map;
   int rc = few_map<F>(&up_map, p.w13, p.experts, 16);
   if (rc == B200MOE_OK) rc = few_map<F>(&down_map, p.w2, p.experts, l.box);
-  if constexpr (F == kFewFp8) {      // (these have no use for maps)
-    up_scales = up_map;
-    down_scales = down_map;
-  } else {
-    if (rc == B200MOE_OK) rc = few_scale_map(&up_scales, p.w13, p.experts, 16);
-    if (rc == B200MOE_OK) rc = few_scale_map(&down_scales, p.w2, p.experts, l.scale_box);
-  }
   if (rc == B200MOE_OK)
-    rc = launch_block_per_sm<few_up_rows_kernel<F, NT>>("few_up_rows_kernel", ctas, S::kThreads, up_fixed + l.panel_bytes, st, p, l, up_map, up_scales);
+    rc = launch_block_per_sm<few_up_rows_kernel<F, NT>>("few_up_rows_kernel", ctas, S::kThreads, up_fixed + l.panel_bytes, st, p, l, up_map);
   if (rc != B200MOE_OK) return rc;
   return launch_block_per_sm<few_down_rows_kernel<F, NT>>("few_down_rows_kernel", l.columns * l.splits, S::kThreads, down_fixed + down_panel, st, p, l,
-                                                          down_map, down_scales);
+                                                          down_map);
 }
 template <int F, int NT>
 int launch_mma(const FewParams& p, const FewLaunch& l, int ctas, cudaStream_t st) {
@@ -297,7 +283,10 @@ extern "C" size_t b200moe_few_tokens_workspace_bytes(int num_tokens, int topk, i
   return FewWorkspace(num_tokens, topk, hidden, inter).bytes;
 }
 
-extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200moe_stream stream) {
+namespace b200moe {
+namespace {
+
+int few_tokens_layer(const b200moe_few_tokens_args* a, b200moe_stream stream, bool scales_by_step) {
   B200_CHECK_ARG(a != nullptr, "few_tokens_layer: null arguments");
   B200_CHECK_ARG(a->dtype == B200MOE_BF16 || a->dtype == B200MOE_F16, "few_tokens_layer: hidden states must be bfloat16 or float16");
   B200_CHECK_ARG(a->num_tokens >= 0 && a->num_tokens <= B200MOE_FEW_TOKENS, "few_tokens_layer: at most %d tokens", B200MOE_FEW_TOKENS);
@@ -323,8 +312,10 @@ extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200mo
   p.experts = a->num_experts; p.id_limit = a->expert_map ? a->total_experts : a->num_experts;
   p.by_topk = FewDiv(a->topk);
   p.act = a->activation; p.alpha = a->act_alpha; p.limit = a->act_limit; p.clamp = a->clamp_limit;
-  p.w13 = {a->w13, a->w13_scale, a->w13_bias, a->w13_format, a->w13_group, 2 * a->inter, a->hidden};
-  p.w2 = {a->w2, a->w2_scale, a->w2_bias, a->w2_format, a->w2_group, a->hidden, a->inter};
+  p.w13 = {a->w13, a->w13_scale, a->w13_bias, a->w13_format, a->w13_group, 2 * a->inter, a->hidden,
+           few_scales(a->w13_format, a->w13_group, 2 * a->inter, a->hidden, scales_by_step)};
+  p.w2 = {a->w2, a->w2_scale, a->w2_bias, a->w2_format, a->w2_group, a->hidden, a->inter,
+          few_scales(a->w2_format, a->w2_group, a->hidden, a->inter, scales_by_step)};
   int ctas = a->max_ctas > 0 && a->max_ctas < sm_count() ? a->max_ctas : sm_count();
   if (ctas > kFewMaxBlocks) ctas = kFewMaxBlocks;
   if (takes_mma(p)) {
@@ -342,4 +333,13 @@ extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200mo
     return fine ? launch_mma<kFewInt4Fine>(p, l, ctas, as_stream(stream)) : launch_mma<kFewInt4>(p, l, ctas, as_stream(stream));
   }
   return a->dtype == B200MOE_BF16 ? launch_simple<__nv_bfloat16>(p, as_stream(stream)) : launch_simple<__half>(p, as_stream(stream));
+}
+
+}  // namespace
+}  // namespace b200moe
+
+extern "C" int b200moe_few_tokens_layer(const b200moe_few_tokens_args* a, b200moe_stream stream) { return few_tokens_layer(a, stream, true); }
+
+extern "C" int b200moe_few_tokens_layer_as_stored(const b200moe_few_tokens_args* a, b200moe_stream stream) {
+  return few_tokens_layer(a, stream, false);
 }

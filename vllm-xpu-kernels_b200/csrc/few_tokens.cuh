@@ -8,12 +8,21 @@ namespace {
 
 constexpr int kFewMaxTopk = 32, kFewMaxExperts = 1024;
 
+// Where the scales of a 4-bit matrix are, in bytes: as they are stored, rows [E][n] one behind the other, or laid out by step, in
+// words of four bytes [E][words][n] (b200moe_few_tokens_scale_words).  A step is 256 values.
+struct FewScales {
+  int row, bytes;        // from one row's to the next row's, and of a row (by step: of all its words)
+  int step;              // of a row and step
+  int next;              // from four of a row's bytes to the next four
+};
+
 struct FewMatrix {
   const void* w;
   const void* scale;
   const void* bias;      // [E, n] in the activation type, or NULL
   int format, group;     // b200moe_weight_format; int4: values per scale
   int n, k;
+  FewScales scales;      // 4-bit weights
 };
 
 // Division by a number that the host knows: a quotient that is at most one too small, and put right.  (The device's own
@@ -46,11 +55,17 @@ struct FewParams {
   FewMatrix w13, w2;
 };
 
-// Words of four bytes that hold a row's scales of a 4-bit matrix, in the order of k: one e8m0 byte per 32 values, or one
-// 16-bit scale per group (per 128 values where groups are longer), as many as whole steps of 128 values take.
+// Words of four bytes that hold a row's scales of a 4-bit matrix laid out by step, in the order of k: one e8m0 byte per 32 values,
+// or one 16-bit scale per group (per 128 values where groups are longer), as many as whole steps of 128 values take.
 __host__ __device__ __forceinline__ int few_scale_words(int format, int group, int k) {
   const int steps = (k + 127) / 128;
   return format == B200MOE_W_MXFP4_NK || group == 64 ? steps : group == 32 ? 2 * steps : (steps + 1) / 2;
+}
+inline FewScales few_scales(int format, int group, int n, int k, bool by_step) {
+  const int values = format == B200MOE_W_MXFP4_NK ? 32 : group, size = format == B200MOE_W_MXFP4_NK ? 1 : 2;
+  if (format != B200MOE_W_MXFP4_NK && format != B200MOE_W_INT4_NK) return {};
+  if (!by_step) return {k / values * size, k / values * size, 256 / values * size, 4};
+  return {4, 4 * few_scale_words(format, group, k), 256 / (values < 128 ? values : 128) * size, 4 * n};
 }
 
 // The slot's expert among the local ones, -1 if it has none here.

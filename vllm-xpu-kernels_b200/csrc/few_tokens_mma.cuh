@@ -35,7 +35,6 @@ struct FewLaunch {
   int columns, splits;   // of the second kernel: blocks with different rows, and shares of the steps for each of them
   int side;              // by column: its warps side by side (1, 2, 4)
   int box;               // rows (by column: columns) of one of its warps, which a load brings
-  int scale_box;         // rows of a load of its scales (4 bits)
   int room;              // rows of h times steps that its panel holds
   int most;              // tokens that the first kernel's panel holds
   FewDiv by_sets, by_steps, by_ctas;                // the first kernel's: sets of an expert, steps of a row, blocks
@@ -195,6 +194,10 @@ __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+// The same of a word's first `bytes` bytes (0: nothing is read); the others are zeros.
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }

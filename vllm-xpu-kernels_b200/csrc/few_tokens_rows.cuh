@@ -28,13 +28,11 @@ template <int F> struct RowShape {
   static constexpr int kFloats = 1 + kSums;                     // per row and step behind the panel: the scale, these sums
   static constexpr int kPanelBytes = kK * 2 + kFloats * 4;      // of the panel: a row's step
   static constexpr int kDepth = 2, kSlot = 4096;
-  static constexpr int kWords = F == kFewInt4Fine ? 4 : F == kFewFp4 ? 2 : 1;    // that hold a row's scales of a step, at most
-  // Behind the rings, per warp: scales of the steps in the ring as they come (first kernel: gates, then ups), and as fp32.
-  static constexpr int kUps = F == kFewFp8 ? 64 : kWords * 64 > 128 ? kWords * 64 : 128;
-  static constexpr int kSlotScales = F == kFewFp8 ? 128 : F == kFewInt4Fine ? 640 : F == kFewFp4 ? 384 : 256;
-  static constexpr int kSpread = F == kFewFp8 ? 0 : F == kFewInt4 ? 256 : 1024;
+  // Words of four bytes that a row's scales of a step (4 bits) are part of, at most: they may begin at any byte.
+  static constexpr int kWords = F == kFewInt4Fine ? 5 : F == kFewFp4 ? 3 : F == kFewInt4 ? 2 : 1;
+  // Behind the rings, per warp: scales of the steps in the ring as they come, a word of every row after the other, and as fp32.
+  static constexpr int kSlotScales = kWords * 128, kSpread = F == kFewFp8 ? 0 : F == kFewInt4 ? 256 : 1024;
   static constexpr int kWarpScales = kDepth * kSlotScales + kSpread;
-  static_assert(F == kFewFp8 || (kSlotScales >= 2 * kUps && kSlotScales >= kWords * 144 && kSlotScales % 128 == 0), "scales of a slot");
   // Shared memory: the rings, barriers, zeros, flags, the table, scales; the rest is the kernels'.
   static constexpr int kBars = kWarps * kDepth * kSlot, kZeros = kBars + 256, kFlags = kZeros + 64, kTable = kFlags + 64;
   static constexpr int kScales = kTable + kTableBytes, kRest = (kScales + kWarps * kWarpScales + 127) / 128 * 128;
@@ -224,47 +222,104 @@ __device__ __forceinline__ int sum_of_row(int row) { return ((row >> 3) & 1) * 1
 // Columns of sums are 36 floats apart, so that a store's 32 lanes (eight rows of four columns) hit 32 banks.
 constexpr int kSumColumn = 36;
 
-// Scales of 4-bit weights come with them: [experts][words][n], neighbouring rows side by side (as they are in a layer, a
-// step's would be 2 or 4 bytes of every row).  fp8: one per 128 values and 128 rows; a lane fetches that of its row.
+// Scales come by cp.async and are read where the caller has them at every call.  4-bit weights have 2 to 16 bytes of a row and step, at
+// any byte (a row of 2880 MXFP4 values has 90), which are part of up to five words of four bytes; the words of a row are
+// fetched by neighbouring lanes, so that an instruction has few lines to find (a row a lane: 7 MXFP4 tokens 87 us, so 81),
+// and what a row's first word has ahead of its scales is taken off when they are read.  fp8: one per 128 values and 128 rows; a lane
+// fetches that of its row.
+template <int F>
 struct RowScales {
-  int words;                   // per step
-  int at, stride;              // of the lane's row in a slot: bytes to the first word, and from one to the next
+  int words;                          // of a row and step
+  int step;                           // bytes per step
+  int advance;                        // bytes from a step's to the next one's
+  int ahead;                          // of the lane's row: bytes ahead of the first step's scales in their first word
   bool f16;
+  int place[RowShape<F>::kWords];     // of the lane's words in the expert's scales, without the step (-1: none)
 };
-__device__ __forceinline__ int scale_words_of_step(const FewMatrix& m) {
-  return m.format == B200MOE_W_MXFP4_NK ? 2 : m.format != B200MOE_W_INT4_NK ? 1 : m.group == 32 ? 4 : m.group == 64 ? 2 : 1;
+// Slot rows up to `rows`; row(i): the matrix's row of slot row i, or one that is 16 times something below it.
+template <int F, typename Row>
+__device__ __forceinline__ RowScales<F> row_scales(const FewMatrix& m, int rows, bool f16, Row row) {
+  const FewScales& s = m.scales;
+  RowScales<F> l;
+  const int lane = threadIdx.x & 31;
+  l.step = s.step;
+  l.advance = s.step / 4 * s.next + s.step % 4;
+  l.words = s.step == 2 ? 1 : s.step / 4 + (s.row & 3 ? 1 : 0);      // (two bytes at an even place are part of one word)
+  l.ahead = row(lane) * s.row & 3;
+  l.f16 = f16;
+#pragma unroll
+  for (int i = 0; i < RowShape<F>::kWords; ++i) {
+    const int j = 32 * i + lane, r = small_div(j, l.words);
+    l.place[i] = i < l.words && r < rows ? row(r) * s.row + (j - r * l.words) * s.next : -1;
+  }
+  return l;
+}
+// The scales of a slot's rows from a step on.
+struct ScalesFrom {
+  const uint8_t* at;       // the step's of the expert, or of a row that is 16 times something
+  int left;                // bytes of a row from there on
+};
+__device__ __forceinline__ ScalesFrom scales_from(const FewMatrix& m, int e, int row16, int step) {
+  const FewScales& s = m.scales;
+  const int first = step * s.step;
+  return {reinterpret_cast<const uint8_t*>(m.scale) + ((int64_t)e * m.n * s.bytes + (int64_t)row16 * s.row + (int64_t)(first / 4) * s.next + first % 4),
+          s.bytes - first};
+}
+// A step's words to their places in a slot; on to the next step.
+template <int F>
+__device__ __forceinline__ void copy_scales(uint32_t to, ScalesFrom& from, const RowScales<F>& l) {
+  to += (threadIdx.x & 31) * 4;
+  if (from.left >= l.step + 3) {
+#pragma unroll
+    for (int i = 0; i < RowShape<F>::kWords; ++i)
+      if (l.place[i] >= 0) copy4(to + i * 128, reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(from.at + l.place[i]) & ~(uintptr_t)3));
+  } else {      // the row's end: nothing from behind it
+#pragma unroll
+    for (int i = 0; i < RowShape<F>::kWords; ++i) {
+      if (l.place[i] < 0) continue;
+      const int j = 32 * i + (threadIdx.x & 31), word = j - small_div(j, l.words) * l.words;
+      const uint8_t* const at = from.at + l.place[i];
+      const int ahead = (int)(reinterpret_cast<uintptr_t>(at) & 3), bytes = max(min(from.left + ahead - 4 * word, 4), 0);
+      copy4(to + i * 128, bytes > 0 ? at - ahead : reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(from.at) & ~(uintptr_t)3), bytes);
+    }
+  }
+  from.at += l.advance;
+  from.left -= l.step;
 }
 __device__ __forceinline__ const uint8_t* fp8_scale(const FewMatrix& m, int e, int n) {
   return reinterpret_cast<const uint8_t*>(m.scale) + (int64_t)(e * (m.n >> 7) + (n >> 7)) * (m.k >> 5);
 }
-// The scales of a step as fp32, four per row and half of the step (int4 with groups from 128 on: one).
+// The scales of step s as fp32, four per row and half of the step (int4 with groups from 128 on: one).
 template <int F>
-__device__ __forceinline__ void spread_scales(uint32_t to, uint32_t from, const RowScales& l) {
-  const int row = threadIdx.x & 31;
-  const uint32_t at = from + l.at;
+__device__ __forceinline__ void spread_scales(uint32_t to, uint32_t from, const RowScales<F>& l, int s) {
+  const int row = threadIdx.x & 31, shift = (l.ahead + (F == kFewFp4 ? 0 : s * l.step) & 3) * 8;
+  const uint32_t at = from + row * l.words * 4;
+  // (the word behind a row's last one has nothing of its scales)
+  auto word = [&](int i) { return __funnelshift_r(lds4(at + i * 4), lds4(at + (i + 1) * 4), shift); };
   auto value = [&](uint32_t h) { return kCodeScale * (l.f16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16)); };
   if constexpr (F == kFewInt4) {
-    const uint32_t v = lds4(at);
-    sts4(to + row * 4, value(v & 0xffffu));
-    sts4(to + 128 + row * 4, value(v >> 16));
+    const uint32_t v = word(0);
+    const float a = value(v & 0xffffu);
+    sts4(to + row * 4, a);
+    sts4(to + 128 + row * 4, l.step == 2 ? a : value(v >> 16));
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t place = to + (h * 32 + row) * 16;
       if constexpr (F == kFewFp4) {
         // 2^(byte - 127): the byte is the exponent (0 gives zero for 2^-127, 255 infinity for NaN).  Beyond the row: zeros.
-        const uint32_t v = lds4(at + h * l.stride);
+        const uint32_t v = word(h);
         sts16(place, __uint_as_float((v & 255u) << 23), __uint_as_float((v << 15) & 0x7f800000u), __uint_as_float((v << 7) & 0x7f800000u),
               __uint_as_float((v >> 1) & 0x7f800000u));
-      } else if (l.words == 4) {
-        const uint32_t v = lds4(at + 2 * h * l.stride), w = lds4(at + (2 * h + 1) * l.stride);
+      } else if (l.step == 16) {
+        const uint32_t v = word(2 * h), w = word(2 * h + 1);
         sts16(place, value(v & 0xffffu), value(v >> 16), value(w & 0xffffu), value(w >> 16));
-      } else if (l.words == 2) {
-        const uint32_t v = lds4(at + h * l.stride);
+      } else if (l.step == 8) {
+        const uint32_t v = word(h);
         const float a = value(v & 0xffffu), b = value(v >> 16);
         sts16(place, a, a, b, b);
       } else {      // (the matrix next to one with finer groups)
-        const float a = value(lds4(at) >> 16 * h & 0xffffu);
+        const float a = value(word(0) >> (l.step == 2 ? 0 : 16 * h) & 0xffffu);
         sts16(place, a, a, a, a);
       }
     }
@@ -471,14 +526,14 @@ __device__ __forceinline__ void multiply_rows(float (&acc)[2][NT][4], uint32_t s
 
 // Takes the step in the ring's slot and fetches the next one into it.
 template <int F, int NT, typename Next>
-__device__ __forceinline__ void take_rows(float (&acc)[2][NT][4], FewRing& ring, const RowScales& l, const RowTokens (&x)[NT], int s, Next next) {
+__device__ __forceinline__ void take_rows(float (&acc)[2][NT][4], FewRing& ring, const RowScales<F>& l, const RowTokens (&x)[NT], int s, Next next) {
   using S = RowShape<F>;
   uint32_t scales = ring.scales + ring.slot * S::kSlotScales;
-  if (F == kFewFp8) copies_wait<S::kDepth - 1>();
+  copies_wait<S::kDepth - 1>();
   ring_wait(ring);
   if (F != kFewFp8) {
     const uint32_t to = ring.scales + S::kDepth * S::kSlotScales;
-    spread_scales<F>(to, scales, l);
+    spread_scales<F>(to, scales, l, s);
     scales = to;
   }
   __syncwarp();
@@ -503,8 +558,7 @@ template <int F, int NT> struct UpRowsShape {
 // of a set goes into shared memory, and at the end of a pass all that there is of a set is added up in the warps' order: one
 // barrier a pass instead of one a set (which cost 4 to 10 us of the kernel).
 template <int F, int NT>
-__global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(const __grid_constant__ FewParams p, const __grid_constant__ FewLaunch launch, const __grid_constant__ CUtensorMap map,
-                                                                               const __grid_constant__ CUtensorMap scale_map) {
+__global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(const __grid_constant__ FewParams p, const __grid_constant__ FewLaunch launch, const __grid_constant__ CUtensorMap map) {
   using S = RowShape<F>;
   constexpr int kWarps = S::kWarps, kThreads = S::kThreads;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -519,7 +573,6 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(c
   if (tid == 0) {
     *gave_up = 0;
     ptx::prefetch_tensormap(&map);
-    if (F != kFewFp8) ptx::prefetch_tensormap(&scale_map);
   }
   prefetch_call(p, tid, kThreads);
   pdl_wait();
@@ -529,7 +582,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(c
   // A few values are laid out while one warp finds the experts, which takes as long as a round of loads; more than that would keep
   // the weights from being asked for, and comes after it.
   const bool early = most >= p.tokens && p.tokens * p.hidden <= (kWarps - 1) * 1024;
-  const RowScales layout = {scale_words_of_step(m), (lane >> 4) * S::kUps + (lane & 15) * 4, 64, launch.f16};
+  const RowScales<F> layout = row_scales<F>(m, 32, launch.f16, [&](int r) { return p.act == B200MOE_ACT_SWIGLUOAI || r < 16 ? r : p.inter + r - 16; });
   if (warp == 0) {
     build_table<false>(table, p);
   } else {
@@ -585,6 +638,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(c
   // The set and step that are fetched next, and how many after them.
   int fetch_j = 0, fetch_s = 0, fetch_s0 = 0, left = 0, e = 0, row = 0;
   const uint8_t* scale = nullptr;
+  ScalesFrom scales_at = {};
   auto copy_next = [&](int slot) {
     if (left > 0) {
       if (fetch_s == steps) {
@@ -595,28 +649,27 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(c
         ++fetch_j;
         e = table.expert[a];
         if (F == kFewFp8) scale = fp8_scale(m, e, pairs ? 2 * row + lane : row + (lane & 15) + (lane >= 16 ? p.inter : 0)) + fetch_s * 4;
+        else scales_at = scales_from(m, e, pairs ? 2 * row : row, fetch_s);
       }
       const uint32_t scales = ring.scales + slot * S::kSlotScales;
       if (lane == 0) {
         const uint32_t at = ring.slots + slot * S::kSlot, bar = ring.bars + slot * 8;
         const int y0 = pairs ? 2 * row : row, y1 = pairs ? 2 * row + 16 : p.inter + row;
         ptx::fence_proxy_async();      // (the warp has read what was there)
-        ptx::mbar_expect_tx_s(bar, S::kSlot + (F == kFewFp8 ? 0 : layout.words * 128));
+        ptx::mbar_expect_tx_s(bar, S::kSlot);
         ptx::tma_load_3d_hint_s(at, &map, bar, fetch_s * 128, y0, e, ring.once);
         ptx::tma_load_3d_hint_s(at + S::kSlot / 2, &map, bar, fetch_s * 128, y1, e, ring.once);
-        if (F != kFewFp8) {
-          ptx::tma_load_3d_hint_s(scales, &scale_map, bar, y0, fetch_s * layout.words, e, ring.once);
-          ptx::tma_load_3d_hint_s(scales + S::kUps, &scale_map, bar, y1, fetch_s * layout.words, e, ring.once);
-        }
       }
-      if (F == kFewFp8) {
+      if constexpr (F == kFewFp8) {
         copy4(scales + lane * 4, scale);
         scale += 4;
+      } else {
+        copy_scales<F>(scales, scales_at, layout);
       }
       ++fetch_s;
       --left;
     }
-    if (F == kFewFp8) copies_end();
+    copies_end();
   };
   auto start_fetch = [&](const Pass& pass) {
     const int pos = pass.start(warp), j = pos / launch.by_steps;
@@ -730,7 +783,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_up_rows_kernel(c
     }
     pass = next;
   }
-  if (F == kFewFp8) copies_wait<0>();
+  copies_wait<0>();
 }
 
 // ---- the second kernel -------------------------------------------------------------------
@@ -742,8 +795,7 @@ __host__ __device__ __forceinline__ int down_sums_bytes(int tokens, int warps) {
 // SMs.  It goes through its steps with as many of h's values at a time as its panel holds, each warp with a stretch of them,
 // half of the rows each.  Of the blocks with the same rows the last one to be done adds the partial sums up, in their order.
 template <int F, int NT>
-__global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel(const __grid_constant__ FewParams p, const __grid_constant__ FewLaunch launch, const __grid_constant__ CUtensorMap map,
-                                                                                 const __grid_constant__ CUtensorMap scale_map) {
+__global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel(const __grid_constant__ FewParams p, const __grid_constant__ FewLaunch launch, const __grid_constant__ CUtensorMap map) {
   using S = RowShape<F>;
   constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kMembers = kWarps / 2;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -760,7 +812,6 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
   if (tid == 0) {
     *gave_up = 0;
     ptx::prefetch_tensormap(&map);
-    if (F != kFewFp8) ptx::prefetch_tensormap(&scale_map);
   }
   // What routed the tokens was complete before the kernel ahead of this one let it start.
   if (warp == 0) build_table<true>(table, p);
@@ -779,11 +830,12 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
   };
   for (int block_r0 = row_begin; block_r0 < row_end; block_r0 += 2 * warp_rows) {
     const int r0 = block_r0 + (warp & 1) * warp_rows, rows_here = max(0, min(warp_rows, row_end - r0));
-    const RowScales layout = {scale_words_of_step(m), ((r0 & 3) + lane) * 4, launch.scale_box * 4, launch.f16};
+    const RowScales<F> layout = row_scales<F>(m, rows_here, launch.f16, [&](int r) { return r0 + r; });
     // The step that is fetched next, how many are left of this warp's stretch, and where the panel after that begins.
     int fetch_a = 0, fetch_s = 0, left = 0, panel_a = share.begin / share.by_steps, panel_s = share.begin - panel_a * steps, e = 0;
     bool found = false;
     const uint8_t* scale = nullptr;
+    ScalesFrom scales_at = {};
     auto copy_next = [&](int slot) {
       while (left == 0 && panel_a * steps + panel_s < share.end) {
         int a1, s1;
@@ -801,24 +853,26 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
         if (!found) {
           e = table.expert[fetch_a];
           if (F == kFewFp8) scale = fp8_scale(m, e, min(r0 + lane, p.hidden - 1)) + fetch_s * 4;
+          else scales_at = scales_from(m, e, 0, fetch_s);
           found = true;
         }
         const uint32_t scales = ring.scales + slot * S::kSlotScales;
         if (lane == 0) {
           const uint32_t bar = ring.bars + slot * 8;
           ptx::fence_proxy_async();        // (the warp has read what was there)
-          ptx::mbar_expect_tx_s(bar, warp_rows * 128 + (F == kFewFp8 ? 0 : layout.words * launch.scale_box * 4));
+          ptx::mbar_expect_tx_s(bar, warp_rows * 128);
           ptx::tma_load_3d_hint_s(ring.slots + slot * S::kSlot, &map, bar, fetch_s * 128, r0, e, ring.once);
-          if (F != kFewFp8) ptx::tma_load_3d_hint_s(scales, &scale_map, bar, r0 & ~3, fetch_s * layout.words, e, ring.once);
         }
-        if (F == kFewFp8) {
+        if constexpr (F == kFewFp8) {
           copy4(scales + lane * 4, scale);
           scale += 4;
+        } else {
+          copy_scales<F>(scales, scales_at, layout);
         }
         ++fetch_s;
         --left;
       }
-      if (F == kFewFp8) copies_end();
+      copies_end();
     };
 #pragma unroll 1
     for (int i = 0; i < S::kDepth; ++i) copy_next((ring.slot + i) % S::kDepth);
@@ -902,7 +956,7 @@ __global__ void __launch_bounds__(RowShape<F>::kThreads, 1) few_down_rows_kernel
       const int token = my_token + i * (kThreads / kBlockRows);
       bias[i] = with_bias && token < p.tokens && my_row < block_rows_here ? weighted_bias(table, m, p.topk, launch.f16, token, block_r0 + my_row) : 0.f;
     }
-    if (F == kFewFp8) copies_wait<0>();
+    copies_wait<0>();
     __syncthreads();
     // consecutive threads, consecutive features of a token
     const int which = my_row >= warp_rows ? 1 : 0, my_sum = sum_of_row((my_row - which * warp_rows) & 31);

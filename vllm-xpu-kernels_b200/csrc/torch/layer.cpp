@@ -564,12 +564,11 @@ PyObject* layer_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// layer_few(plan, output, hidden, topk_weights, topk_ids, expert_map | None, max_ctas, persistent, w13 step scales | None,
-// w2 step scales | None): the whole layer in two kernels, for up to B200MOE_FEW_TOKENS tokens.  Step scales: those of MXFP4 and
-// int4 weights as fused_moe_interface.step_scales lays them out.
+// layer_few(plan, output, hidden, topk_weights, topk_ids, expert_map | None, max_ctas, persistent): the whole layer in two
+// kernels, for up to B200MOE_FEW_TOKENS tokens.
 PyObject* layer_few(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK(n == 10, "layer_few takes 10 arguments");
+  TORCH_CHECK(n == 8, "layer_few takes 8 arguments");
   const Plan& p = *plan_arg(a[0]);
   const at::Tensor &y = tensor_arg(a[1], "output"), &x = tensor_arg(a[2], "hidden_states"), &w = tensor_arg(a[3], "topk_weights"),
                    &ids = tensor_arg(a[4], "topk_ids");
@@ -607,16 +606,8 @@ PyObject* layer_few(PyObject*, PyObject* const* a, Py_ssize_t n) {
   g.expert_map = map.has_value() ? map->data_ptr<int32_t>() : nullptr;
   g.w13 = p.w13.data_ptr(); g.w13_format = weights.d13.format; g.w13_group = weights.d13.group;
   g.w2 = p.w2.data_ptr(); g.w2_format = weights.d2.format; g.w2_group = weights.d2.group;
-  auto scale_of = [&](const std::optional<at::Tensor>& scale, PyObject* arg, const WeightDesc& d, int64_t N, int64_t K) -> const void* {
-    if (d.format != B200MOE_W_MXFP4_NK && d.format != B200MOE_W_INT4_NK) return scale.has_value() ? scale->data_ptr() : nullptr;
-    const at::Tensor& s = tensor_arg(arg, "step scales");
-    TORCH_CHECK(s.scalar_type() == at::kInt && s.is_contiguous() && s.device() == x.device() && s.dim() == 3 && s.size(0) == p.experts &&
-                    s.size(1) == b200moe_few_tokens_scale_words(d.format, d.group, (int)K) && s.size(2) == N,
-                "step scales must be int32 [num_experts, words, N] of the layer's weights");
-    return s.data_ptr();
-  };
-  g.w13_scale = scale_of(p.s13, a[8], weights.d13, 2 * p.inter, H);
-  g.w2_scale = scale_of(p.s2, a[9], weights.d2, H, k2);
+  g.w13_scale = p.s13.has_value() ? p.s13->data_ptr() : nullptr;
+  g.w2_scale = p.s2.has_value() ? p.s2->data_ptr() : nullptr;
   g.w13_bias = p.b13.has_value() ? p.b13->data_ptr() : nullptr;
   g.w2_bias = p.b2.has_value() ? p.b2->data_ptr() : nullptr;
   g.num_tokens = (int)T; g.hidden = (int)H; g.inter = (int)k2; g.topk = (int)K;
@@ -632,7 +623,7 @@ PyObject* layer_few(PyObject*, PyObject* const* a, Py_ssize_t n) {
     g.workspace_bytes = b200moe_few_tokens_workspace_bytes((int)T, (int)K, (int)H, (int)k2);
     const Workspace workspace(stream, g.workspace_bytes, a[7] == Py_True);
     g.workspace = workspace.mem.data_ptr();
-    check_status(b200moe_few_tokens_layer(&g, (b200moe_stream)stream.stream()));
+    check_status(b200moe_few_tokens_layer_as_stored(&g, (b200moe_stream)stream.stream()));
   }
   gil.end();
   Py_RETURN_NONE;

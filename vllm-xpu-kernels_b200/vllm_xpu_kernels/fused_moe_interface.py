@@ -148,8 +148,8 @@ def _signed_nibbles(w):
 
 
 def step_scales(scale, k):
-    """The scales of MXFP4 (``[E, N, k / 32]`` e8m0 bytes) or int4 weights (``[E, N, k / group]``, 16 bits) as the kernels for
-    a few tokens read them: int32 words ``[E, words, N]``, each with the four bytes of 128 values, or two 16-bit scales
+    """The scales of MXFP4 (``[E, N, k / 32]`` e8m0 bytes) or int4 weights (``[E, N, k / group]``, 16 bits) as
+    ``b200moe_few_tokens_layer`` of the C ABI takes them (a layer object reads them as they are): int32 words ``[E, words, N]``, each with the four bytes of 128 values, or two 16-bit scales
     (groups of 256 as two of 128); whole steps of 128 values, the rest zeros."""
     if scale.element_size() == 2:
         group = max(k // scale.shape[-1], 1)
@@ -243,7 +243,6 @@ class XpuFusedMoe:
     """
 
     few_tokens = False       # (also of layers that were saved before there was a choice)
-    _step_scales = None
 
     def __init__(
         self,
@@ -373,7 +372,6 @@ class XpuFusedMoe:
         if few_tokens and self._act_kind == "relu2_no_mul":
             raise NotImplementedError("few_tokens: no kernel for the relu2_no_mul activation")
         self.few_tokens = few_tokens
-        self._step_scales = None
         self._native_plan = None
 
         self.expert_map = expert_map
@@ -403,11 +401,10 @@ class XpuFusedMoe:
         object.__setattr__(self, name, value)
         if name in _PLAN_FIELDS:
             object.__setattr__(self, "_native_plan", None)
-            object.__setattr__(self, "_step_scales", None)
 
     def __getstate__(self):
         """What a copy takes along: everything but the native plan, which it makes anew from its own tensors."""
-        return {**self.__dict__, "_native_plan": None, "_step_scales": None}
+        return {**self.__dict__, "_native_plan": None}
 
     @property
     def act_func(self):
@@ -434,23 +431,13 @@ class XpuFusedMoe:
         self._apply_kernel(output, hidden_states, topk_weights, topk_ids,
                            expert_map, a1q_scale)
 
-    def _few_scales(self):
-        """`step_scales` of the layer's weights, made on first use and anew when the scales' contents have changed."""
-        s13, s2 = self.gemm1_wei_scales, self.gemm2_wei_scales
-        kept = self._step_scales
-        if kept is None or kept[0] != s13._version or kept[1] != s2._version:
-            kept = (s13._version, s2._version, step_scales(s13, 2 * self.w13.shape[-1]), step_scales(s2, 2 * self.w2.shape[-1]))
-            self._step_scales = kept
-        return kept[2:]
-
     def _apply_few_tokens(self, output, hidden_states, topk_weights, topk_ids, expert_map):
         if expert_map is None and self.ep_size > 1:
             expert_map = self.expert_map
         if self.stage_hook is not None:
             self.stage_hook("routing")
-        s13, s2 = self._few_scales() if self.is_mxfp4 or self.is_int4 else (None, None)
         _xpu_C.layer_few(self._native_plan or self._plan(), output, hidden_states, topk_weights, topk_ids, expert_map,
-                         self.gemm_max_ctas, self.persistent_workspace, s13, s2)
+                         self.gemm_max_ctas, self.persistent_workspace)
         if self.stage_hook is not None:
             self.stage_hook("experts")
 

@@ -290,8 +290,10 @@ struct Experts {
       if (p.clamp > 0) {
         at::Tensor t = at::from_blob(ws + g1, {M, 2 * I},
                                      at::TensorOptions().dtype(out_scalar).device(at::kCUDA, device));
-        t.narrow(1, 0, I).clamp_max_(p.clamp);
-        t.narrow(1, I, I).clamp_(-p.clamp, p.clamp);
+        // gates and ups are halves of the features, or with SwigluOAI every other one, as for the epilogues
+        const bool pairs = p.act == kSwigluOai;
+        (pairs ? t.slice(1, 0, 2 * I, 2) : t.narrow(1, 0, I)).clamp_max_(p.clamp);
+        (pairs ? t.slice(1, 1, 2 * I, 2) : t.narrow(1, I, I)).clamp_(-p.clamp, p.clamp);
       }
       if (p.block_fp8 && p.act == kSilu && I % 128 == 0) {
         // SiLU, multiply and the 1x128 e4m3 quantisation of gemm2's input in one pass over the rows

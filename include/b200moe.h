@@ -554,9 +554,9 @@ int b200moe_quant_mxfp8_ex(const void* x, b200moe_dtype dtype, void* q, void* s,
  * which has the norm and the quantisation as separate steps):
  *   s = T(input + residual), written back to `residual`   (s = input if it is NULL)
  *   y = s / sqrt(mean(s^2) + eps) * weight                (fp32; weight NULL: 1)
- *   out = T(y);  q = e4m3(y / scale), per group of a row
+ *   out = T(y);  q = e4m3(y * (1 / scale)), per group of a row
  *   scale = max(amax|y| / 448, 1 / (448*512)), with scale_ue8m0 rounded up to a power
- *   of two; NaN if the group holds a NaN or an infinity.
+ *   of two; NaN if the group holds a NaN or an infinity.  Finite rows of any magnitude.
  * `out` may be the input (same pointer and stride); no other buffers may overlap. */
 typedef struct {
   const void* input;      /* [rows, hidden] dtype, row stride in elements            */

@@ -4,11 +4,13 @@
 //
 //   s = T(input + residual), stored as the new residual      (s = input without one)
 //   y = s / sqrt(mean(s^2) + eps) * weight                   (fp32, mean over the row)
-//   out = T(y);   per group of a row: scale = max(amax|y| / 448, 1 / (448 * 512)), q = e4m3(y / scale)
+//   out = T(y);   per group of a row: scale = max(amax|y| / 448, 1 / (448 * 512)), q = e4m3(y * (1 / scale))
 //
 // The sum that is normalised is the rounded one, which the next reader of the residual sees too; y goes
 // to the 8-bit rows before its rounding to T.  Scales and codes are those of per_token_group_fp8_quant on y,
 // except that NaN and infinities stay visible: the scale of a group that holds one is NaN.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace b200moe {
@@ -27,6 +29,7 @@ struct RmsParams {
   int hidden, group;
   float eps;
   bool ue8m0;
+  uint32_t least;      // bits of the least sum of squares that eps does not cover (see row_factor)
 };
 
 // Maximum that keeps a NaN.
@@ -46,6 +49,92 @@ __device__ __forceinline__ float up_to_pow2(float x) {
 __device__ __forceinline__ float scale_of(float amax, bool ue8m0) {
   const float s = max_nan(__fdiv_rn(amax, kE4m3Max), kLeastScale);
   return ue8m0 ? up_to_pow2(s) : s;
+}
+
+// The squares of a row are summed in fp32, which does not hold them where values are beyond some 2^63 (nor, with an eps that does
+// not cover them, where all are below 2^-62).  Such a row is taken again times this power of two, with eps times its square; 1
+// elsewhere.  fp32 holds the squares of any float16.
+__device__ __forceinline__ float row_factor(float sum, float eps) {
+  if (sum == INFINITY) return 0x1p-80f;
+  return sum < 0x1p-80f && eps < 0x1p-80f ? 0x1p100f : 1.f;
+}
+// Whether it is 1 (false also where the sum is a NaN): from `least` on, and finite.
+template <typename T>
+__device__ __forceinline__ bool sum_holds(float sum, uint32_t least) {
+  return std::is_same_v<T, __half> || __float_as_uint(sum) - least < 0x7f800000u - least;
+}
+
+// All of such a row of rms_norm_kernel behind the residual's addition, by the threads that have summed it: one value at a time, from
+// memory.  (Out of line and behind all of a block's ordinary rows: 8192 rows of 2880 values, which have none, take 41 us, 39 without this
+// and 46 to 60 with it in their loop.)
+template <typename T, typename W>
+__device__ __noinline__ void norm_scaled_row(const RmsParams& p, int64_t r, float2* red) {
+  const int tx = threadIdx.x, lane = tx & 31, warp = tx >> 5, warps = blockDim.x >> 5;
+  const T* const s = p.residual ? reinterpret_cast<const T*>(p.residual) + r * p.residual_stride
+                                : reinterpret_cast<const T*>(p.input) + r * p.input_stride;
+  const W* const w = reinterpret_cast<const W*>(p.weight);
+  // (numbers that the compiler knows: with one in a register the kernel is given all 16 barriers, of which an SM has too few for
+  // five blocks.  A block has two rows of two warps at most.)
+  auto row_sync = [&]() {
+    if (warps == 1) __syncwarp();
+    else if (threadIdx.y == 0) asm volatile("bar.sync 1, %0;" ::"r"((int)blockDim.x) : "memory");
+    else asm volatile("bar.sync 2, %0;" ::"r"((int)blockDim.x) : "memory");
+  };
+  float sum, top, by = 1.f;
+  for (int pass = 0; pass < 2; ++pass) {       // which factor it is, and the sums with it
+    row_sync();      // the residual is written, and what `red` held has been read
+    sum = top = 0.f;
+#pragma unroll 1
+    for (int i = tx; i < p.hidden; i += blockDim.x) {
+      const float v = to_f32<T>(s[i]) * by;
+      sum = fmaf(v, v, sum);
+      top = max_nan(top, fabsf(w ? v * to_f32<W>(w[i]) : v));
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+    }
+    if (lane == 0) red[warp] = make_float2(sum, top);
+    row_sync();
+    sum = top = 0.f;
+    for (int i = 0; i < warps; ++i) {
+      sum += red[i].x;
+      top = max_nan(top, red[i].y);
+    }
+    if (pass == 0) by = row_factor(sum, p.eps);
+  }
+  const float rs = rsqrtf(sum / (float)p.hidden + p.eps * by * by);
+  float scale = scale_of(top * rs, p.ue8m0);
+  if (p.q && p.group == 0 && tx == 0) p.scales[r * p.s_stride_row] = scale;
+  T* const out = p.out ? reinterpret_cast<T*>(p.out) + r * p.out_stride : nullptr;
+  uint8_t* const q = p.q ? p.q + r * p.q_stride : nullptr;
+  auto value = [&](int i) {
+    const float n = to_f32<T>(s[i]) * by * rs;
+    return w ? n * to_f32<W>(w[i]) : n;
+  };
+  // (a lane writes only what it reads itself: `out` may be the input)
+  const int group = p.q && p.group ? p.group : 128;
+#pragma unroll 1
+  for (int g0 = warp * group; g0 < p.hidden; g0 += warps * group) {
+    const int end = min(g0 + group, p.hidden);
+    if (q && p.group) {
+      float m = 0.f;
+#pragma unroll 1
+      for (int i = g0 + lane; i < end; i += 32) m = max_nan(m, fabsf(value(i)));
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+      scale = scale_of(m, p.ue8m0);
+      if (lane == 0) p.scales[r * p.s_stride_row + (int64_t)(g0 / group) * p.s_stride_group] = scale;
+    }
+    const float inv = __fdiv_rn(1.0f, scale);
+#pragma unroll 1
+    for (int i = g0 + lane; i < end; i += 32) {
+      const float y = value(i);
+      if (out) out[i] = from_f32<T>(y);
+      if (q) q[i] = f32_to_e4m3(y * inv);
+    }
+  }
 }
 
 // Any size, stride and alignment: a block per row, one value at a time, four of a thread asked for together.  Every thread
@@ -89,18 +178,37 @@ __global__ void __launch_bounds__(256) rms_norm_scalar_kernel(RmsParams p) {
       }
     }
   }
+  auto join = [&]() {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+    for (int d = 16; d > 0; d >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+    }
+    if (lane == 0) { red_sum[warp] = sum; red_max[warp] = top; }
+    __syncthreads();
+    sum = 0.f;
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { sum += red_sum[i]; top = max_nan(top, red_max[i]); }
+  };
+  join();
+  const float by = sum_holds<T>(sum, p.least) ? 1.f : row_factor(sum, p.eps);
+  if (by != 1.f) {       // (the same for all threads)
+    __syncthreads();
+    sum = top = 0.f;
+#pragma unroll 1
+    for (int g0 = warp * group; g0 < p.hidden; g0 += 8 * group) {
+      const int end = min(g0 + group, p.hidden);
+#pragma unroll 1
+      for (int i = g0 + lane; i < end; i += 32) {
+        const float v = to_f32<T>(s[i]) * by;
+        sum = fmaf(v, v, sum);
+        top = max_nan(top, fabsf(w ? v * to_f32<W>(w[i]) : v));
+      }
+    }
+    join();
   }
-  if (lane == 0) { red_sum[warp] = sum; red_max[warp] = top; }
-  __syncthreads();
-  sum = 0.f;
-  top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { sum += red_sum[i]; top = max_nan(top, red_max[i]); }
-  const float rs = rsqrtf(sum / (float)p.hidden + p.eps);
+  const float rs = rsqrtf(sum / (float)p.hidden + p.eps * by * by);
   float scale = 0.f, inv = 0.f;
   if (p.q && p.group == 0) {
     scale = scale_of(top * rs, p.ue8m0);
@@ -115,7 +223,7 @@ __global__ void __launch_bounds__(256) rms_norm_scalar_kernel(RmsParams p) {
       float m = 0.f;
 #pragma unroll 4
       for (int i = g0 + lane; i < end; i += 32) {
-        const float n = to_f32<T>(s[i]) * rs;
+        const float n = to_f32<T>(s[i]) * by * rs;
         m = max_nan(m, fabsf(w ? n * to_f32<W>(w[i]) : n));
       }
 #pragma unroll
@@ -129,7 +237,7 @@ __global__ void __launch_bounds__(256) rms_norm_scalar_kernel(RmsParams p) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int i = i0 + 32 * k;
-        const float n = i < end ? to_f32<T>(s[i]) * rs : 0.f;
+        const float n = i < end ? to_f32<T>(s[i]) * by * rs : 0.f;
         y[k] = w && i < end ? n * to_f32<W>(w[i]) : n;
       }
 #pragma unroll
@@ -179,7 +287,7 @@ enum ScaleMode { kNoScales, kRowScale, kGroupScales };
 // for the same chain of sums, scale and codes: 8192 rows of 4096 float16 values 33 us, 3.0 TB/s.  With few rows the launch is what it
 // costs: one row 2.2 us in a graph.
 template <typename T, typename W, int N, int V, int kMode>
-__global__ void __launch_bounds__(1024) rms_norm_kernel(RmsParams p) {
+__global__ void __launch_bounds__(1024) rms_norm_kernel(const __grid_constant__ RmsParams p) {
   __shared__ float2 red[2][32];
   pdl_trigger();
   pdl_wait();
@@ -201,6 +309,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(RmsParams p) {
     }
   };
   int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  uint32_t again = 0;      // turns whose row is left for later (see row_factor)
   ask(r);
   // (the rows of a block run through the same number of turns, so that its barrier is met by all)
   for (int64_t first = (int64_t)blockIdx.x * blockDim.y, turn = 0; first < p.rows; first += step, r += step, ++turn) {
@@ -242,17 +351,19 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(RmsParams p) {
         if (kMode == kRowScale) top = max_nan(top, o.y);
       }
     }
+    const bool here = r < p.rows && sum_holds<T>(sum, p.least);      // (the same for all threads of a row)
+    if (!here) again |= 1u << turn;
     const float rs = rsqrtf(sum / (float)p.hidden + p.eps);
     float scale = 0.f, inv = 0.f;
     if (kMode == kRowScale) {
       scale = scale_of(top * rs, p.ue8m0);
       inv = __fdiv_rn(1.0f, scale);
-      if (tx == 0 && r < p.rows) p.scales[r * p.s_stride_row] = scale;
+      if (tx == 0 && here) p.scales[r * p.s_stride_row] = scale;
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int j = tx + i * blockDim.x;
-      const bool mine = r < p.rows && j < pieces;
+      const bool mine = here && j < pieces;
       float y[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) {
@@ -292,16 +403,26 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(RmsParams p) {
       }
     }
   }
+  if constexpr (!std::is_same_v<T, __half>) {
+#pragma unroll 1
+    for (; again; again &= again - 1) {
+      r = ((int64_t)blockIdx.x + (int64_t)(__ffs(again) - 1) * gridDim.x) * blockDim.y + threadIdx.y;
+      if (r < p.rows) norm_scaled_row<T, W>(p, r, red[0] + threadIdx.y * warps);
+    }
+  }
 }
 
+constexpr int kMostTurns = 32;      // (of a block: a bit each)
 template <typename T, typename W, int N, int V, int kMode>
 int launch_rows(const RmsParams& p, cudaStream_t st) {
   const int threads = ((p.hidden / N + V - 1) / V + 31) / 32 * 32;
   int rows = 1;   // of a block: at least 128 threads where there are rows for every SM
   while (rows * threads < 128 && p.rows > (int64_t)rows * sm_count()) rows *= 2;
   const int64_t blocks = (p.rows + rows - 1) / rows, resident = (int64_t)sm_count() * (1024 / (rows * threads));
+  const int64_t least = (blocks + kMostTurns - 1) / kMostTurns;
   B200_LAUNCHED("rms_norm_kernel", launch_pdl(p.rows <= kEarlyLaunchRows, rms_norm_kernel<T, W, N, V, kMode>,
-                                              dim3((unsigned)(blocks < resident ? blocks : resident)), dim3(threads, rows), 0, st, p));
+                                              dim3((unsigned)(blocks < resident ? blocks : resident < least ? least : resident)), dim3(threads, rows), 0,
+                                              st, p));
   return B200MOE_OK;
 }
 template <typename T, typename W, int N, int V>
@@ -358,7 +479,8 @@ extern "C" int b200moe_add_rms_norm(const b200moe_rms_norm_args* a, b200moe_stre
   B200_CHECK_ARG(a->out != nullptr || a->q != nullptr, "add_rms_norm: nothing to write");
   RmsParams p = {a->input, a->residual, a->weight, a->out, (uint8_t*)a->q, a->scales, a->rows, a->input_stride,
                  a->residual_stride, a->out_stride, a->q_stride, a->s_stride_row, a->s_stride_group, a->hidden,
-                 a->group_size == a->hidden ? 0 : a->group_size, a->eps, a->scale_ue8m0 != 0};
+                 a->group_size == a->hidden ? 0 : a->group_size, a->eps, a->scale_ue8m0 != 0,
+                 a->eps < 0x1p-80f ? 0x17800000u : 0u};
   const bool wide = a->weight != nullptr && a->weight_dtype == B200MOE_F32;
   B200_DISPATCH_FLOAT(a->dtype, "add_rms_norm", {
     return wide ? launch_rms_norm<scalar_t, float>(p, as_stream(stream)) : launch_rms_norm<scalar_t, scalar_t>(p, as_stream(stream));

@@ -256,17 +256,34 @@ int64_t row_stride(const at::Tensor& t, const char* name) {
   return stride;
 }
 
-// Whether the memory that the rows of a and b span overlaps.
-bool rows_overlap(const at::Tensor& a, const at::Tensor& b) {
-  auto span = [](const at::Tensor& t) {
-    int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    const char* p = (const char*)t.data_ptr();
-    return std::make_pair(p, p + (last + 1) * t.element_size());
-  };
-  if (a.numel() == 0 || b.numel() == 0) return false;
-  const auto x = span(a), y = span(b);
-  return x.first < y.second && y.first < x.second;
+// Memory as `n` pieces of `length` bytes, `stride` bytes apart.
+struct Pieces {
+  const char* at;
+  int64_t n, stride, length;
+  const char* end() const { return at + (n - 1) * stride + length; }
+};
+Pieces pieces_of_rows(const at::Tensor& t, int64_t row_stride) {
+  const int64_t hidden = t.size(-1), rows = hidden ? t.numel() / hidden : 0, size = t.element_size();
+  return {(const char*)t.data_ptr(), row_stride == 0 ? std::min<int64_t>(rows, 1) : rows, row_stride * size, hidden * size};
+}
+// ... of scales [rows, groups], by row or by group, whichever is dense, else all that they span.
+Pieces pieces_of_scales(const at::Tensor& t) {
+  const int64_t rows = t.size(0), groups = t.size(1), size = t.element_size();
+  const char* const at = (const char*)t.data_ptr();
+  if (t.numel() == 0) return {at, 0, 0, 0};
+  if (groups == 1 || t.stride(1) == 1) return {at, rows, t.stride(0) * size, groups * size};
+  if (rows == 1 || t.stride(0) == 1) return {at, groups, t.stride(1) * size, rows * size};
+  return {at, 1, 0, ((rows - 1) * t.stride(0) + (groups - 1) * t.stride(1) + 1) * size};
+}
+// Whether a and b share bytes.  (Pieces of different strides whose spans overlap are taken to.)
+bool overlap(const Pieces& a, const Pieces& b) {
+  if (a.n == 0 || b.n == 0 || a.length == 0 || b.length == 0 || a.at >= b.end() || b.at >= a.end()) return false;
+  if (a.n > 1 && b.n > 1 && a.stride != b.stride) return true;
+  // columns of one buffer: where b's pieces are, modulo the stride
+  const int64_t stride = a.n > 1 ? a.stride : b.stride;
+  if ((a.n == 1 && b.n == 1) || stride <= 0) return true;
+  const int64_t d = ((b.at - a.at) % stride + stride) % stride;
+  return d < a.length || d + b.length > stride;
 }
 
 // residual += input, norm, weight; the result in the input's dtype (out) and as e4m3 rows with scales (out_q, scales).
@@ -301,7 +318,8 @@ void b200_add_rms_norm(const at::Tensor& input, const std::optional<at::Tensor>&
     a.residual = residual->data_ptr();
     a.residual_stride = row_stride(*residual, "residual");
     TORCH_CHECK(rows <= 1 || a.residual_stride >= hidden, "b200_add_rms_norm: the rows of residual must not overlap");
-    TORCH_CHECK(!rows_overlap(input, *residual), "b200_add_rms_norm: residual must not overlap the input");
+    TORCH_CHECK(!overlap(pieces_of_rows(input, a.input_stride), pieces_of_rows(*residual, a.residual_stride)),
+                "b200_add_rms_norm: residual must not overlap the input");
   }
   if (weight.has_value()) {
     TORCH_CHECK(weight->dim() == 1 && weight->size(0) == hidden && weight->is_contiguous(),
@@ -315,7 +333,7 @@ void b200_add_rms_norm(const at::Tensor& input, const std::optional<at::Tensor>&
     a.out = out->data_ptr();
     a.out_stride = row_stride(*out, "out");
     TORCH_CHECK(rows <= 1 || a.out_stride >= hidden, "b200_add_rms_norm: the rows of out must not overlap");
-    TORCH_CHECK(!rows_overlap(*out, input) || (a.out == a.input && (rows <= 1 || a.out_stride == a.input_stride)),
+    TORCH_CHECK(!overlap(pieces_of_rows(*out, a.out_stride), pieces_of_rows(input, a.input_stride)) || (a.out == a.input && (rows <= 1 || a.out_stride == a.input_stride)),
                 "b200_add_rms_norm: out must be the input or not overlap it");
   }
   if (out_q.has_value()) {
@@ -327,6 +345,9 @@ void b200_add_rms_norm(const at::Tensor& input, const std::optional<at::Tensor>&
                 "b200_add_rms_norm: scales must be float32 [rows, hidden_size / group_size]");
     TORCH_CHECK((rows <= 1 || scales->stride(0) != 0) && (groups <= 1 || scales->stride(1) != 0),
                 "b200_add_rms_norm: scales must not be expanded");
+    const int64_t apart = std::max(scales->stride(0), scales->stride(1)), next = std::min(scales->stride(0), scales->stride(1));
+    TORCH_CHECK(rows <= 1 || groups <= 1 || apart > ((scales->stride(0) == next ? rows : groups) - 1) * next,
+                "b200_add_rms_norm: scales must not overlap themselves");
     a.q = out_q->data_ptr();
     a.q_stride = row_stride(*out_q, "out_q");
     TORCH_CHECK(rows <= 1 || a.q_stride >= hidden, "b200_add_rms_norm: the rows of out_q must not overlap");
@@ -336,15 +357,17 @@ void b200_add_rms_norm(const at::Tensor& input, const std::optional<at::Tensor>&
     a.group_size = (int)group_size;
     a.scale_ue8m0 = scale_ue8m0;
   }
-  const at::Tensor* written[] = {residual.has_value() ? &*residual : nullptr, out.has_value() ? &*out : nullptr,
-                                 out_q.has_value() ? &*out_q : nullptr, scales.has_value() ? &*scales : nullptr};
+  const Pieces none = {nullptr, 0, 0, 0}, read = pieces_of_rows(input, a.input_stride);
+  const Pieces weights = weight.has_value() ? pieces_of_rows(*weight, hidden) : none;
+  const Pieces written[] = {residual.has_value() ? pieces_of_rows(*residual, a.residual_stride) : none,
+                            out.has_value() ? pieces_of_rows(*out, a.out_stride) : none,
+                            out_q.has_value() ? pieces_of_rows(*out_q, a.q_stride) : none,
+                            scales.has_value() ? pieces_of_scales(*scales) : none};
   for (int i = 0; i < 4; ++i) {
-    if (written[i] == nullptr) continue;
     for (int j = 0; j < i; ++j)
-      TORCH_CHECK(written[j] == nullptr || !rows_overlap(*written[i], *written[j]),
-                  "b200_add_rms_norm: the tensors that are written must not overlap");
-    TORCH_CHECK(i == 1 || !rows_overlap(*written[i], input), "b200_add_rms_norm: only out may be the input");
-    TORCH_CHECK(!weight.has_value() || !rows_overlap(*written[i], *weight), "b200_add_rms_norm: weight must not be written");
+      TORCH_CHECK(!overlap(written[i], written[j]), "b200_add_rms_norm: the tensors that are written must not overlap");
+    TORCH_CHECK(i == 1 || !overlap(written[i], read), "b200_add_rms_norm: only out may be the input");
+    TORCH_CHECK(!overlap(written[i], weights), "b200_add_rms_norm: weight must not be written");
   }
   if (rows == 0 || hidden == 0) return;
   const c10::cuda::CUDAGuard guard(input.device());

@@ -151,7 +151,10 @@ struct Weights {
   WeightDesc d13, d2;
   bool i4;                    // int4 weights whose shapes the block-scaled kernel takes (gemm_tc_i4.cu)
 };
-Weights describe(const Plan& p, int64_t hidden, at::ScalarType out_dtype) {
+Weights describe(const Plan& p, int64_t hidden, at::ScalarType out_dtype, at::Device device) {
+  TORCH_CHECK(p.w13.device() == device && p.w2.device() == device, "weights must be on the device of hidden_states");
+  for (const auto* t : {&p.s13, &p.s2, &p.b13, &p.b2})
+    TORCH_CHECK(!t->has_value() || (*t)->device() == device, "scales and biases must be on the device of hidden_states");
   const at::ScalarType a = (p.block_fp8 || p.mx) ? at::kFloat8_e4m3fn : out_dtype;
   const int64_t k2 = p.inter * p.inter_scale;
   Weights w;
@@ -442,7 +445,7 @@ PyObject* layer_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const c10::cuda::CUDAGuard guard(x.device());
   const auto stream = at::cuda::getCurrentCUDAStream();
   const b200moe_stream st = (b200moe_stream)stream.stream();
-  const Weights weights = describe(p, H, od);
+  const Weights weights = describe(p, H, od, x.device());
   raise_if_timed_out(device_status_word(x.get_device()));   // an earlier call on this device gave up a wait
   if (o.rows_hint == 0 && map.has_value() && p.total_experts > p.experts)
     o.rows_hint = std::max<int64_t>(1, M * p.experts / p.total_experts);   // the other ranks' share is masked
@@ -550,7 +553,7 @@ PyObject* layer_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   const c10::cuda::CUDAGuard guard(x.device());
   const auto stream = at::cuda::getCurrentCUDAStream();
-  const Weights weights = describe(p, H, y.scalar_type());
+  const Weights weights = describe(p, H, y.scalar_type(), x.device());
   raise_if_timed_out(device_status_word(x.get_device()));
   WithoutGil gil;
   Experts e{p, weights, o, gil, out, y.scalar_type(), M, H, (int)segments, (int)x.get_device(),
@@ -592,13 +595,13 @@ PyObject* layer_few(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK(map->scalar_type() == at::kInt && map->is_contiguous(), "expert_map must be int32");
     TORCH_CHECK(map->size(0) == p.total_experts, "expert_map must be [total_experts_num]");
   }
-  for (const at::Tensor* t : {&y, &w, &ids, map.has_value() ? &*map : &x, &p.w13, &p.w2})
+  for (const at::Tensor* t : {&y, &w, &ids, map.has_value() ? &*map : &x})
     TORCH_CHECK(t->device() == x.device(), "all tensors of a layer call must be on the device of hidden_states");
   const int64_t k2 = p.inter * p.inter_scale;
   TORCH_CHECK_NOT_IMPLEMENTED(p.inter_scale == 1, "the layer for a few tokens has no relu2_no_mul");
   Plan q = p;   // (weights are read as they are: no quantised activations to go with them)
   q.block_fp8 = q.mx = false;
-  const Weights weights = describe(q, H, y.scalar_type());
+  const Weights weights = describe(q, H, y.scalar_type(), x.device());
   if (T == 0) Py_RETURN_NONE;
   static const b200moe_activation acts[] = {B200MOE_ACT_SILU, B200MOE_ACT_GELU, B200MOE_ACT_GELU_TANH, B200MOE_ACT_SWIGLUOAI,
                                             B200MOE_ACT_SILU, B200MOE_ACT_SWIGLUSTEP};

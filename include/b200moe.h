@@ -633,7 +633,8 @@ typedef struct {
   size_t workspace_bytes;
   b200moe_weight_format w13_format, w2_format;
   int w13_group, w2_group;    /* int4: values per scale                               */
-  int num_tokens, hidden, inter, topk, num_experts, total_experts;
+  int num_tokens, hidden, inter;
+  int topk, num_experts, total_experts; /* topk <= 32, num_experts <= 1024            */
   b200moe_dtype dtype;        /* BF16 or F16                                          */
   b200moe_dtype ids_dtype;
   b200moe_activation activation;

@@ -35,6 +35,7 @@ REF_FUSED_MOE_ENV = "VLLM_XPU_FUSED_MOE_USE_REF"
 USE_MXFP4_FP8_ENV = "VLLM_XPU_FUSED_MOE_USE_MXFP4_FP8"
 FP8_BLOCK_SIZE = 128
 FEW_TOKENS = 16          # tokens up to which few_tokens=True takes the form of two kernels
+FEW_TOKENS_TOPK = 32     # experts a token that this form takes
 FP8_FUSED_MIN_ROWS = 12   # routed rows per expert from which fuse_activation=True takes the fused form of fp8 layers
 
 
@@ -238,7 +239,7 @@ class XpuFusedMoe:
     activations are not quantised (``mxfp4_activations`` and the fp8 activations of
     block-scaled layers concern the other calls), so results differ from the other form's in
     rounding and are the more accurate.  For 16-bit, block-scaled fp8, MXFP4 and int4
-    weights and every activation but ``relu2_no_mul``; calls with ``a1q_scale`` and larger
+    weights, up to 32 experts a token and every activation but ``relu2_no_mul``; calls with ``a1q_scale`` and larger
     ones run as without it.
     """
 
@@ -371,6 +372,8 @@ class XpuFusedMoe:
             raise NotImplementedError("few_tokens: 16-bit, block-scaled fp8, MXFP4 and int4 weights only")
         if few_tokens and self._act_kind == "relu2_no_mul":
             raise NotImplementedError("few_tokens: no kernel for the relu2_no_mul activation")
+        if few_tokens and n_experts_per_token > FEW_TOKENS_TOPK:
+            raise NotImplementedError(f"few_tokens: up to {FEW_TOKENS_TOPK} experts a token")
         self.few_tokens = few_tokens
         self._native_plan = None
 

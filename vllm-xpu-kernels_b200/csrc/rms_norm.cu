@@ -52,8 +52,8 @@ __device__ __forceinline__ float scale_of(float amax, bool ue8m0) {
 }
 
 // The squares of a row are summed in fp32, which does not hold them where values are beyond some 2^63 (nor, with an eps that does
-// not cover them, where all are below 2^-62).  Such a row is taken again times this power of two, with eps times its square; 1
-// elsewhere.  fp32 holds the squares of any float16.
+// not cover them, where all are below 2^-62).  Such a row is summed again times this power of two, and normalised so, with eps
+// times its square; 1 elsewhere.  fp32 holds the squares of any float16.
 __device__ __forceinline__ float row_factor(float sum, float eps) {
   if (sum == INFINITY) return 0x1p-80f;
   return sum < 0x1p-80f && eps < 0x1p-80f ? 0x1p100f : 1.f;
@@ -62,79 +62,6 @@ __device__ __forceinline__ float row_factor(float sum, float eps) {
 template <typename T>
 __device__ __forceinline__ bool sum_holds(float sum, uint32_t least) {
   return std::is_same_v<T, __half> || __float_as_uint(sum) - least < 0x7f800000u - least;
-}
-
-// All of such a row of rms_norm_kernel behind the residual's addition, by the threads that have summed it: one value at a time, from
-// memory.  (Out of line and behind all of a block's ordinary rows: 8192 rows of 2880 values, which have none, take 41 us, 39 without this
-// and 46 to 60 with it in their loop.)
-template <typename T, typename W>
-__device__ __noinline__ void norm_scaled_row(const RmsParams& p, int64_t r, float2* red) {
-  const int tx = threadIdx.x, lane = tx & 31, warp = tx >> 5, warps = blockDim.x >> 5;
-  const T* const s = p.residual ? reinterpret_cast<const T*>(p.residual) + r * p.residual_stride
-                                : reinterpret_cast<const T*>(p.input) + r * p.input_stride;
-  const W* const w = reinterpret_cast<const W*>(p.weight);
-  // (numbers that the compiler knows: with one in a register the kernel is given all 16 barriers, of which an SM has too few for
-  // five blocks.  A block has two rows of two warps at most.)
-  auto row_sync = [&]() {
-    if (warps == 1) __syncwarp();
-    else if (threadIdx.y == 0) asm volatile("bar.sync 1, %0;" ::"r"((int)blockDim.x) : "memory");
-    else asm volatile("bar.sync 2, %0;" ::"r"((int)blockDim.x) : "memory");
-  };
-  float sum, top, by = 1.f;
-  for (int pass = 0; pass < 2; ++pass) {       // which factor it is, and the sums with it
-    row_sync();      // the residual is written, and what `red` held has been read
-    sum = top = 0.f;
-#pragma unroll 1
-    for (int i = tx; i < p.hidden; i += blockDim.x) {
-      const float v = to_f32<T>(s[i]) * by;
-      sum = fmaf(v, v, sum);
-      top = max_nan(top, fabsf(w ? v * to_f32<W>(w[i]) : v));
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
-    }
-    if (lane == 0) red[warp] = make_float2(sum, top);
-    row_sync();
-    sum = top = 0.f;
-    for (int i = 0; i < warps; ++i) {
-      sum += red[i].x;
-      top = max_nan(top, red[i].y);
-    }
-    if (pass == 0) by = row_factor(sum, p.eps);
-  }
-  const float rs = rsqrtf(sum / (float)p.hidden + p.eps * by * by);
-  float scale = scale_of(top * rs, p.ue8m0);
-  if (p.q && p.group == 0 && tx == 0) p.scales[r * p.s_stride_row] = scale;
-  T* const out = p.out ? reinterpret_cast<T*>(p.out) + r * p.out_stride : nullptr;
-  uint8_t* const q = p.q ? p.q + r * p.q_stride : nullptr;
-  auto value = [&](int i) {
-    const float n = to_f32<T>(s[i]) * by * rs;
-    return w ? n * to_f32<W>(w[i]) : n;
-  };
-  // (a lane writes only what it reads itself: `out` may be the input)
-  const int group = p.q && p.group ? p.group : 128;
-#pragma unroll 1
-  for (int g0 = warp * group; g0 < p.hidden; g0 += warps * group) {
-    const int end = min(g0 + group, p.hidden);
-    if (q && p.group) {
-      float m = 0.f;
-#pragma unroll 1
-      for (int i = g0 + lane; i < end; i += 32) m = max_nan(m, fabsf(value(i)));
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-      scale = scale_of(m, p.ue8m0);
-      if (lane == 0) p.scales[r * p.s_stride_row + (int64_t)(g0 / group) * p.s_stride_group] = scale;
-    }
-    const float inv = __fdiv_rn(1.0f, scale);
-#pragma unroll 1
-    for (int i = g0 + lane; i < end; i += 32) {
-      const float y = value(i);
-      if (out) out[i] = from_f32<T>(y);
-      if (q) q[i] = f32_to_e4m3(y * inv);
-    }
-  }
 }
 
 // Any size, stride and alignment: a block per row, one value at a time, four of a thread asked for together.  Every thread
@@ -282,12 +209,14 @@ enum ScaleMode { kNoScales, kRowScale, kGroupScales };
 // Rows are read once and stay in registers between their sums and the result.  blockDim = (threads of a row, rows of a
 // block); a thread has V pieces of N values, blockDim.x pieces apart.  A resident block takes row after row and asks for
 // the next one before it waits for its sums.
-// Bound by the bytes of a row, each moved once: 8192 rows of 7168 bf16 values with residual, output and e4m3 rows 86 us, 6.1
+// Bound by the bytes of a row, each moved once: 8192 rows of 7168 bf16 values with residual, output and e4m3 rows 86.5 us, 6.1
 // TB/s (a block per row with 16-byte pieces and its values read twice 228 us).  Where only e4m3 rows are written there are fewer bytes
-// for the same chain of sums, scale and codes: 8192 rows of 4096 float16 values 33 us, 3.0 TB/s.  With few rows the launch is what it
+// for the same chain of sums, scale and codes: 8192 rows of 4096 float16 values 34 us, 2.9 TB/s.  With few rows the launch is what it
 // costs: one row 2.2 us in a graph.
-template <typename T, typename W, int N, int V, int kMode>
-__global__ void __launch_bounds__(1024) rms_norm_kernel(const __grid_constant__ RmsParams p) {
+// Of rows that are summed again (see row_factor) the values in registers are scaled.
+constexpr int kFewThreads = 448;
+template <typename T, typename W, int N, int V, int kMode, int kMost>
+__global__ void __launch_bounds__(kMost, kMost == 1024 ? 1 : 2) rms_norm_kernel(RmsParams p) {
   __shared__ float2 red[2][32];
   pdl_trigger();
   pdl_wait();
@@ -308,8 +237,14 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const __grid_constant__ 
       }
     }
   };
+  // Of a row's threads: a block has two rows of two warps at most.  (Numbers that the compiler knows: for one in a register the kernel is
+  // given all 16 barriers, of which an SM has too few for five blocks.)
+  auto row_sync = [&]() {
+    if (warps == 1) __syncwarp();
+    else if (threadIdx.y == 0) asm volatile("bar.sync 1, %0;" ::"r"((int)blockDim.x) : "memory");
+    else asm volatile("bar.sync 2, %0;" ::"r"((int)blockDim.x) : "memory");
+  };
   int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  uint32_t again = 0;      // turns whose row is left for later (see row_factor)
   ask(r);
   // (the rows of a block run through the same number of turns, so that its barrier is met by all)
   for (int64_t first = (int64_t)blockIdx.x * blockDim.y, turn = 0; first < p.rows; first += step, r += step, ++turn) {
@@ -336,34 +271,56 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const __grid_constant__ 
       }
     }
     ask(r + step);
+    auto join = [&](auto sync) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (kMode == kRowScale) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
-    }
-    if (warps > 1) {   // two buffers in turn: one barrier a row
-      if (lane == 0) red[turn & 1][warp] = make_float2(sum, top);
-      __syncthreads();
-      sum = 0.f;
-      for (int i = 0; i < warps; ++i) {
-        const float2 o = red[turn & 1][threadIdx.y * warps + i];
-        sum += o.x;
-        if (kMode == kRowScale) top = max_nan(top, o.y);
+      for (int d = 16; d > 0; d >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (kMode == kRowScale) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
       }
+      if (warps > 1) {   // two buffers in turn: one barrier a row
+        if (lane == 0) red[turn & 1][warp] = make_float2(sum, top);
+        sync();
+        sum = 0.f;
+        for (int i = 0; i < warps; ++i) {
+          const float2 o = red[turn & 1][threadIdx.y * warps + i];
+          sum += o.x;
+          if (kMode == kRowScale) top = max_nan(top, o.y);
+        }
+      }
+    };
+    join([] { __syncthreads(); });
+    float eps = p.eps;
+    if (!sum_holds<T>(sum, p.least)) {      // (the same for all threads of a row)
+      const float by = row_factor(sum, p.eps);
+      row_sync();
+      sum = top = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int j = tx + i * blockDim.x;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const float s = to_f32<T>(v[i].e[k]) * by;
+          v[i].e[k] = from_f32<T>(s);
+          if (r < p.rows && j < pieces) {
+            sum = fmaf(s, s, sum);
+            if (kMode == kRowScale) top = max_nan(top, fabsf(w ? s * to_f32<W>(wv[i].e[k]) : s));
+          }
+        }
+      }
+      join(row_sync);
+      eps = eps * by * by;
     }
-    const bool here = r < p.rows && sum_holds<T>(sum, p.least);      // (the same for all threads of a row)
-    if (!here) again |= 1u << turn;
-    const float rs = rsqrtf(sum / (float)p.hidden + p.eps);
+    const float rs = rsqrtf(sum / (float)p.hidden + eps);
     float scale = 0.f, inv = 0.f;
     if (kMode == kRowScale) {
       scale = scale_of(top * rs, p.ue8m0);
       inv = __fdiv_rn(1.0f, scale);
-      if (tx == 0 && here) p.scales[r * p.s_stride_row] = scale;
+      if (tx == 0 && r < p.rows) p.scales[r * p.s_stride_row] = scale;
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int j = tx + i * blockDim.x;
-      const bool mine = here && j < pieces;
+      const bool mine = r < p.rows && j < pieces;
       float y[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) {
@@ -403,26 +360,20 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const __grid_constant__ 
       }
     }
   }
-  if constexpr (!std::is_same_v<T, __half>) {
-#pragma unroll 1
-    for (; again; again &= again - 1) {
-      r = ((int64_t)blockIdx.x + (int64_t)(__ffs(again) - 1) * gridDim.x) * blockDim.y + threadIdx.y;
-      if (r < p.rows) norm_scaled_row<T, W>(p, r, red[0] + threadIdx.y * warps);
-    }
-  }
 }
 
-constexpr int kMostTurns = 32;      // (of a block: a bit each)
 template <typename T, typename W, int N, int V, int kMode>
 int launch_rows(const RmsParams& p, cudaStream_t st) {
   const int threads = ((p.hidden / N + V - 1) / V + 31) / 32 * 32;
   int rows = 1;   // of a block: at least 128 threads where there are rows for every SM
   while (rows * threads < 128 && p.rows > (int64_t)rows * sm_count()) rows *= 2;
-  const int64_t blocks = (p.rows + rows - 1) / rows, resident = (int64_t)sm_count() * (1024 / (rows * threads));
-  const int64_t least = (blocks + kMostTurns - 1) / kMostTurns;
-  B200_LAUNCHED("rms_norm_kernel", launch_pdl(p.rows <= kEarlyLaunchRows, rms_norm_kernel<T, W, N, V, kMode>,
-                                              dim3((unsigned)(blocks < resident ? blocks : resident < least ? least : resident)), dim3(threads, rows), 0,
-                                              st, p));
+  // Blocks of up to 448 threads are given 72 registers each, of which an SM has enough for two: with 64, as a block of 1024 needs, 8192 rows
+  // of 7168 bf16 values take 92 us instead of 86.5, of 4096 57 instead of 50, of 512 7.9 instead of 7.0.
+  const int most = rows * threads <= kFewThreads ? 2 * kFewThreads : 1024;
+  const int64_t blocks = (p.rows + rows - 1) / rows, resident = (int64_t)sm_count() * (most / (rows * threads));
+  const dim3 grid((unsigned)(blocks < resident ? blocks : resident));
+  const auto kernel = rows * threads <= kFewThreads ? rms_norm_kernel<T, W, N, V, kMode, kFewThreads> : rms_norm_kernel<T, W, N, V, kMode, 1024>;
+  B200_LAUNCHED("rms_norm_kernel", launch_pdl(p.rows <= kEarlyLaunchRows, kernel, grid, dim3(threads, rows), 0, st, p));
   return B200MOE_OK;
 }
 template <typename T, typename W, int N, int V>
@@ -452,8 +403,8 @@ int launch_rms_norm(const RmsParams& p, cudaStream_t st) {
   if (pieces_fit(p, N / 2, sizeof(T), sizeof(W))) return launch_mode<T, W, N / 2, 1>(p, st);
   // Rows that cannot be cut into pieces: kept in registers value by value where that saves the second way through long rows, whose
   // latency counts with few of them, or where many short ones would have a block each.  us, in registers / below: 1411 bf16 values,
-  // 61 rows 5.0 / 5.0, 256 rows 6.5 / 5.8, 8192 rows 82 / 64; 5001 values, 61 rows 6.0 / 10.0, 256 rows 11.9 / 12.9, 1001 rows 45 /
-  // 28; 99 values, 1001 rows 4.3 / 4.0, 8192 rows 9.4 / 18.
+  // 61 rows 4.9 / 4.8, 256 rows 6.5 / 5.7, 8192 rows 81 / 51; 5001 values, 61 rows 6.0 / 9.6, 256 rows 11.7 / 12.7, 1001 rows 45 /
+  // 20; 99 values, 1001 rows 4.3 / 3.8, 8192 rows 9.4 / 17.5.
   if (p.hidden <= 1024 * kSingles && (p.hidden > 2048 ? p.rows <= 256 : p.hidden < 256 && p.rows > 1024) && (p.q == nullptr || p.group == 0))
     return launch_mode<T, W, 1, kSingles>(p, st);
   B200_LAUNCHED("rms_norm_scalar_kernel",

@@ -9,7 +9,7 @@
 // of 128 features leaves most SMs without work at one token.  mma.sync is far from its limit here (0.4 instructions a cycle
 // and SM: 12 to 26 % of the time in use).
 //
-// What a call costs beyond its bytes (7 tokens of MXFP4 2880 x 2880, four of 128 experts, 75 us for 52 us of weights): finding the
+// What a call costs beyond its bytes (7 tokens of MXFP4 2880 x 2880, four of 128 experts, 81 us for 52 us of weights): finding the
 // experts 1.3 us in each kernel (with more than 32 routed slots 2.3), the first weights' way 2, tokens and h on their way to shared
 // memory 2.5 each, the sums of the first kernel 2 to 3, of the second 1, the last of a column's blocks 1, and the kernels' ends, where blocks that
 // shared the memory evenly finish up to 4 us apart.  Asking for W2 ahead from the first kernel's end into L2 gained nothing (the second

@@ -8,9 +8,10 @@
 // their group in fp32.
 //
 // Bound by the weights' bytes with few tokens of large experts: 7168 x 2048 fp8, 8 of 256 experts, one token 65 us, 5.4 TB/s (its
-// main loops alone 6.5); with small ones by what a call costs besides (few_tokens_mma.cuh).  MXFP4 and int4 come near the issue rate: a byte is
-// two conversions, and its products are as many as those of two bytes of fp8 (2880 x 2880, 7 tokens: 50 % of the issue slots, 44 % of the
-// ALU's cycles; int4 4 tokens 53 % of the ALU's).
+// main loops alone 6.5); with small ones by what a call costs besides (few_tokens_mma.cuh).  MXFP4 and int4 take more instructions for a
+// byte (two conversions, and the products of two bytes of fp8), but no unit bounds them: 2880 x 2880, 7 tokens, first and second kernel 52 and
+// 43 % of the issue slots, 43 and 35 % of the ALU's cycles, 50 and 38 % of the shared-memory pipe's; int4 4 tokens 49 and 42, 50 and 40,
+// 50 and 38.  What they wait for are one another's results: 12 warps hide that in part.
 #pragma once
 
 #include "few_tokens_mma.cuh"

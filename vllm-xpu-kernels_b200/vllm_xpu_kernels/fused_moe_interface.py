@@ -235,8 +235,9 @@ class XpuFusedMoe:
     ``few_tokens`` (not in the reference; keyword only, default False): calls of
     ``apply`` with up to ``FEW_TOKENS`` tokens run as two kernels instead of a chain of five or
     more: one that multiplies with ``w13`` and applies the activation, one that
-    multiplies with ``w2`` and adds the experts up.  Weights are used as they are stored,
-    activations are not quantised (``mxfp4_activations`` and the fp8 activations of
+    multiplies with ``w2`` and adds the experts up.  Weights and scales are read where they are
+    stored, at every call (block-scaled fp8 stored ``[E,K,N]``, and sizes or addresses that are not
+    multiples of 16 bytes, by kernels that take many times as long as the other form's); activations are not quantised (``mxfp4_activations`` and the fp8 activations of
     block-scaled layers concern the other calls), so results differ from the other form's in
     rounding and are the more accurate.  For 16-bit, block-scaled fp8, MXFP4 and int4
     weights, up to 32 experts a token and every activation but ``relu2_no_mul``; calls with ``a1q_scale`` and larger

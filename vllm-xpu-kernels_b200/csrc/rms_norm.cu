@@ -51,9 +51,9 @@ __device__ __forceinline__ float scale_of(float amax, bool ue8m0) {
   return ue8m0 ? up_to_pow2(s) : s;
 }
 
-// The squares of a row are summed in fp32, which does not hold them where values are beyond some 2^63 (nor, with an eps that does
-// not cover them, where all are below 2^-62).  Such a row is summed again times this power of two, and normalised so, with eps
-// times its square; 1 elsewhere.  fp32 holds the squares of any float16.
+// The squares of a row are summed in fp32, which does not hold them where values are beyond some 2^63, nor to its precision where their
+// sum is below 2^-80 (which counts where eps is, too).  Such a row is summed again times this power of two, and normalised so, with
+// eps times its square; 1 elsewhere.  fp32 holds the squares of any float16.
 __device__ __forceinline__ float row_factor(float sum, float eps) {
   if (sum == INFINITY) return 0x1p-80f;
   return sum < 0x1p-80f && eps < 0x1p-80f ? 0x1p100f : 1.f;

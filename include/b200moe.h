@@ -328,8 +328,13 @@ typedef enum {
   B200MOE_W_FP8E5M2_TENSOR_KN = 6, /* fp8 e5m2 [E,K,N] + fp32 scale [E]               */
   B200MOE_W_INT4_NK = 7,  /* two's-complement 4-bit pairs [E,N,K/2] (low nibble = even k)
                              + scales [E,N,K/group_size] in the activation dtype   */
-  B200MOE_W_MXFP8_KN = 8  /* fp8 e4m3 [E,K,N] + e8m0 bytes [E,K/32,N] (one per 32 K rows) */
+  B200MOE_W_MXFP8_KN = 8, /* fp8 e4m3 [E,K,N] + e8m0 bytes [E,K/32,N] (one per 32 K rows) */
+  B200MOE_W_INT8_NK = 9   /* int8 [E,N,K] + fp32 scales [E,N]; rows int8 (I8) with fp32 scales [M]:
+                             sums in int32, K divisible by 16 and at most B200MOE_INT8_MAX_K;
+                             EPI_NONE or EPI_SILU_MUL, d_dtype BF16, F16 or F32                */
 } b200moe_weight_format;
+
+#define B200MOE_INT8_MAX_K 131071 /* products of two int8 values that a 32-bit sum holds: (2^31 - 1) / 128^2 */
 
 typedef enum {
   B200MOE_EPI_NONE = 0,      /* D = acc (+bias)                                     */
@@ -356,7 +361,8 @@ typedef struct {
                              b200moe_quant_mxfp8; int4 weights (FP8_E4M3_X2, _X3
                              and their _EVENS_FIRST forms): such words and fp32
                              block sums [K/128][M] behind them, the output of
-                             b200moe_quant_mxfp8_ex; else NULL                  */
+                             b200moe_quant_mxfp8_ex; int8 weights (I8 rows): fp32
+                             [M], the output of b200moe_quant_int8_rows; else NULL */
   const void* w;          /* weights, layout per w_format                         */
   b200moe_weight_format w_format;
   const void* w_scale;    /* per w_format, else NULL                              */
@@ -400,7 +406,8 @@ typedef struct {
                              permutation.  16-bit and block-scaled fp8 weights.     */
   void* d_scale;          /* FP8_E4M3 output: fp32 scales [M, N/256]; planes: their
                              scale words [planes][ceil(N/2 / 128)][M]; else NULL    */
-  b200moe_dtype mid_dtype;/* FP8_E4M3 output: BF16 or F16, the type the
+  b200moe_dtype mid_dtype;/* F32 output (int8 weights): the bias's type, BF16 or F16.
+                             FP8_E4M3 output: BF16 or F16, the type the
                              pre-activation values (and the bias) have: they are
                              rounded to it before the activation, as the unfused
                              GEMM's output would be                                */
@@ -416,6 +423,64 @@ typedef struct {
 } b200moe_gemm_args;
 
 int b200moe_grouped_gemm(const b200moe_gemm_args* args, b200moe_stream stream);
+
+/* ------------------------------------------------------------------------- */
+/* Dense layers beside the routed experts (shared experts, dense blocks)      */
+/* ------------------------------------------------------------------------- */
+
+/* Rows as 8-bit integers with one scale each: v = in, or with `gated` silu(gate) * up of rows
+ * [gate(hidden) | up(hidden)]; scale = max(amax|v|, 1e-10) / 127, q = rint(v / scale) in fp32.  A row with a
+ * NaN or an infinity has a scale that is not finite.  in [rows, hidden (gated: 2 hidden)] F32, F16 or BF16,
+ * in_stride / q_stride elements from row to row; scales [rows].  rows_per_segment (int32 [num_segments], device) or NULL:
+ * only the first sum(rows_per_segment) rows are read and written.  No counterpart op in the reference. */
+int b200moe_quant_int8_rows(const void* in, b200moe_dtype dtype, int64_t in_stride, int8_t* q, int64_t q_stride,
+                            float* scales, int64_t rows, int hidden, int gated, const int32_t* rows_per_segment,
+                            int num_segments, b200moe_stream stream);
+
+/* The matrix product in 8-bit integers with a scale for each row of either operand:
+ *   d[m, n] = (sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n] (+ bias[n])
+ * The sum is exact (int32).  Zero-initialise the struct. */
+typedef struct {
+  const int8_t* x;        /* [rows, k], 16-byte aligned, x_stride (a multiple of 16) from row to row */
+  const float* x_scale;   /* [rows]                                                  */
+  const int8_t* w;        /* [n, k], 16-byte aligned                                 */
+  const float* w_scale;   /* [n]                                                     */
+  const void* bias;       /* [n] bias_dtype, or NULL                                 */
+  void* d;                /* [rows, n] d_dtype, d_stride from row to row             */
+  int64_t rows, x_stride, d_stride;
+  int n, k;               /* k: a multiple of 16, at most B200MOE_INT8_MAX_K         */
+  b200moe_dtype d_dtype;  /* F32, F16 or BF16                                        */
+  b200moe_dtype bias_dtype; /* F16 or BF16                                           */
+  int32_t* status;        /* as in b200moe_gemm_args, or NULL                        */
+} b200moe_int8_linear_args;
+int b200moe_int8_linear(const b200moe_int8_linear_args* args, b200moe_stream stream);
+
+/* Both projections of a gated feed-forward block, its activation and the product, and the gradients:
+ *   [g | u] = x w^T,  out = silu(g) * u                                w [2 inter, hidden], gate rows first
+ *   dg = grad u s (1 + g (1 - s)),  du = grad g s,  s = sigmoid(g)
+ *   grad_x = [dg | du] w,  grad_w = [dg | du]^T x
+ * Sums are fp32; g and u stay fp32 until the activation, and in `pre`; dg and du are rounded to dtype.  The forward pass
+ * reads x, w and writes out and, unless it is NULL, pre; the backward pass reads grad, pre, x, w and writes those of grad_x
+ * and grad_w that are not NULL.  All matrices but w, pre and grad_w may have rows that are further apart than they are
+ * long (strides in elements).  Zero-initialise the struct. */
+typedef struct {
+  const void* x;          /* [rows, hidden], 16-byte aligned, stride a multiple of 8  */
+  const void* w;          /* [2 inter, hidden], 16-byte aligned                       */
+  void* out;              /* [rows, inter]                                            */
+  float* pre;             /* [rows, 2 inter] fp32: g and u                            */
+  const void* grad;       /* [rows, inter]                                            */
+  void* grad_x;           /* [rows, hidden]                                           */
+  void* grad_w;           /* [2 inter, hidden]                                        */
+  void* workspace;        /* backward: ..._workspace_bytes, 16-byte aligned           */
+  size_t workspace_bytes;
+  int64_t rows, x_stride, out_stride, grad_stride, grad_x_stride;
+  int inter, hidden;      /* hidden: a multiple of 8                                  */
+  b200moe_dtype dtype;    /* F16 or BF16, of all matrices but pre                     */
+  int32_t* status;        /* as in b200moe_gemm_args, or NULL                         */
+} b200moe_gated_linear_args;
+int b200moe_gated_linear(const b200moe_gated_linear_args* args, b200moe_stream stream);
+size_t b200moe_gated_linear_backward_workspace_bytes(int64_t rows, int inter);
+int b200moe_gated_linear_backward(const b200moe_gated_linear_args* args, b200moe_stream stream);
 
 /* ------------------------------------------------------------------------- */
 /* Activations, quantisation, reductions                                      */

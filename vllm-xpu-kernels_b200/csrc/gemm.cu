@@ -13,6 +13,7 @@ int grouped_gemm_tc_dq(const b200moe_gemm_args* a, cudaStream_t st);
 int grouped_gemm_tc_mx(const b200moe_gemm_args* a, cudaStream_t st);
 int grouped_gemm_tc_i4(const b200moe_gemm_args* a, cudaStream_t st);
 int grouped_gemm_check(const b200moe_gemm_args* a, cudaStream_t st);
+int grouped_gemm_i8(const b200moe_gemm_args* a, cudaStream_t st);
 }  // namespace b200moe
 
 using namespace b200moe;
@@ -23,6 +24,7 @@ extern "C" int b200moe_grouped_gemm(const b200moe_gemm_args* a, b200moe_stream s
   B200_CHECK_ARG(a->m >= 0 && a->n >= 0 && a->k > 0 && a->num_experts >= 1,
                  "grouped_gemm: bad sizes (m=%lld n=%d k=%d experts=%d)", (long long)a->m, a->n,
                  a->k, a->num_experts);
+  if (a->w_format == B200MOE_W_INT8_NK) return grouped_gemm_i8(a, as_stream(stream));
   // the SwigluOAI form's output as the planes that the next GEMM takes
   const bool d_planes = a->epilogue == B200MOE_EPI_SWIGLUOAI && a->d_dtype == a->a_dtype &&
                         (a->d_dtype == B200MOE_FP8_E4M3 || a->d_dtype == B200MOE_FP8_E4M3_X2) &&

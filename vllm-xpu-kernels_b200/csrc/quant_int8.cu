@@ -1,0 +1,185 @@
+// Rows as 8-bit integers with one scale each, as the int8 GEMM takes its activations:
+//
+//   v = x, or silu(gate) * up of a row [gate | up];  scale = max(amax|v|, 1e-10) / 127;  q = rint(v / scale)
+//
+// in fp32 with IEEE divisions (ties of rint go to even, so that a row's codes are the ones that the same formula
+// in torch operations gives).  A row that holds a NaN or an infinity gets a scale that is not finite and codes that are zero
+// where it holds it: every output of the product that it goes into is a NaN.
+#include "common.cuh"
+
+namespace b200moe {
+namespace {
+
+constexpr float kLeastAmax = 1e-10f;
+
+struct QuantInt8Params {
+  const void* in;
+  int8_t* q;
+  float* scales;
+  const int32_t* rows_per_segment;   // or NULL: all rows
+  int64_t rows, in_stride, q_stride;
+  int hidden, num_segments;
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t code_of(float v, float scale) {
+  // (a NaN, from a scale that is not finite, becomes 0; the limits are for quotients of subnormal scales)
+  const float r = rintf(__fdiv_rn(v, scale));
+  return r == r ? (uint32_t)(int)fminf(fmaxf(r, -127.f), 127.f) & 0xffu : 0u;
+}
+__device__ __forceinline__ float gated_value(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+__device__ __forceinline__ float scale_of(float amax) { return __fdiv_rn(max_nan(amax, kLeastAmax), 127.f); }
+
+__device__ __forceinline__ int64_t rows_in_use(const QuantInt8Params& p) {
+  if (p.rows_per_segment == nullptr) return p.rows;
+  int64_t used = 0;   // (every warp for itself; plain loads: the kernel before this one may have written the counts)
+  for (int e = threadIdx.x & 31; e < p.num_segments; e += 32) used += max(p.rows_per_segment[e], 0);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) used += __shfl_xor_sync(0xffffffffu, used, off);
+  return used < p.rows ? used : p.rows;
+}
+
+// Largest |v| of a row over its `threads` threads (a multiple of 32); `part` holds a value per warp of the block.
+__device__ __forceinline__ float row_max(float amax, int threads, float* part) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  if (threads == 32) return amax;
+  const int warp = threadIdx.x >> 5, warps = threads >> 5, first = warp / warps * warps;
+  if ((threadIdx.x & 31) == 0) part[warp] = amax;
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  amax = lane < warps ? part[first + lane] : 0.f;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  return amax;
+}
+
+// Rows whose 16-byte pieces are aligned, up to kPieces of them a thread, which stay in registers between the
+// maximum and the codes: every byte is read once.
+constexpr int kPieces = 4;
+template <typename T, bool kGated>
+__global__ void __launch_bounds__(1024)
+quant_int8_rows_kernel(const QuantInt8Params p, int threads) {
+  constexpr int N = 16 / sizeof(T);
+  __shared__ float part[32];
+  pdl_trigger();
+  pdl_wait();
+  const int sub = threadIdx.x / threads, t = threadIdx.x - sub * threads;
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / threads) + sub;
+  const bool live = row < rows_in_use(p);
+  const int nvec = p.hidden / N;
+  const T* in = reinterpret_cast<const T*>(p.in) + row * p.in_stride;
+  vec16 a[kPieces], b[kGated ? kPieces : 1];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int c = t + i * threads;
+    if (live && c < nvec) {
+      a[i] = ld16(in + (int64_t)c * N);
+      if (kGated) b[i] = ld16(in + p.hidden + (int64_t)c * N);
+    }
+  }
+  float amax = 0.f;
+  float v[kGated ? kPieces * N : 1];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    if (live && t + i * threads < nvec) {
+      const T* x = reinterpret_cast<const T*>(&a[i]);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        float y = to_f32<T>(x[k]);
+        if (kGated) {
+          y = gated_value(y, to_f32<T>(reinterpret_cast<const T*>(&b[i])[k]));
+          v[kGated ? i * N + k : 0] = y;
+        }
+        amax = max_nan(amax, fabsf(y));
+      }
+    }
+  }
+  const float scale = scale_of(row_max(amax, threads, part));
+  if (!live) return;
+  if (t == 0) p.scales[row] = scale;
+  int8_t* q = p.q + row * p.q_stride;
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int c = t + i * threads;
+    if (c < nvec) {
+      const T* x = reinterpret_cast<const T*>(&a[i]);
+      uint32_t w[N / 4];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const uint32_t code = code_of(kGated ? v[kGated ? i * N + k : 0] : to_f32<T>(x[k]), scale);
+        w[k / 4] = (k % 4 ? w[k / 4] : 0u) | code << (8 * (k % 4));
+      }
+      if (N == 8) *reinterpret_cast<uint2*>(q + (int64_t)c * N) = make_uint2(w[0], w[N / 4 - 1]);
+      else *reinterpret_cast<uint32_t*>(q + (int64_t)c * N) = w[0];
+    }
+  }
+}
+
+// Any length and alignment, value by value; rows are read twice.
+template <typename T, bool kGated>
+__global__ void __launch_bounds__(1024)
+quant_int8_any_kernel(const QuantInt8Params p) {
+  __shared__ float part[32];
+  pdl_trigger();
+  pdl_wait();
+  const int64_t row = blockIdx.x;
+  if (row >= rows_in_use(p)) return;
+  const T* in = reinterpret_cast<const T*>(p.in) + row * p.in_stride;
+  auto value = [&](int c) {
+    const float y = to_f32<T>(in[c]);
+    return kGated ? gated_value(y, to_f32<T>(in[(int64_t)p.hidden + c])) : y;
+  };
+  float amax = 0.f;
+  for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) amax = max_nan(amax, fabsf(value(c)));
+  const float scale = scale_of(row_max(amax, blockDim.x, part));
+  if (threadIdx.x == 0) p.scales[row] = scale;
+  for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) p.q[row * p.q_stride + c] = (int8_t)code_of(value(c), scale);
+}
+
+template <typename T, bool kGated>
+int launch(const QuantInt8Params& p, cudaStream_t st) {
+  constexpr int N = 16 / sizeof(T);
+  const int nvec = p.hidden / N;
+  const bool early = p.rows <= kEarlyLaunchRows;
+  const bool whole = p.hidden % N == 0 && p.in_stride % N == 0 && p.q_stride % N == 0 && ((uintptr_t)p.in & 15) == 0 &&
+                     ((uintptr_t)p.q & (N - 1)) == 0 && nvec <= kPieces * 1024;
+  if (!whole) {
+    const int threads = p.hidden >= 1024 ? 1024 : (p.hidden + 31) / 32 * 32;
+    B200_LAUNCHED("quant_int8_any_kernel",
+                  launch_pdl(early, quant_int8_any_kernel<T, kGated>, dim3((unsigned)p.rows), dim3(threads), 0, st, p));
+    return B200MOE_OK;
+  }
+  // Threads of a row: one piece each for a few rows (latency), all four of them for many.
+  const int pieces = p.rows <= 256 ? 1 : kPieces;
+  int threads = ((nvec + pieces - 1) / pieces + 31) / 32 * 32;
+  if (threads > 1024) threads = 1024;
+  const int per_block = threads >= 256 ? 1 : 256 / threads;
+  const int64_t blocks = (p.rows + per_block - 1) / per_block;
+  B200_LAUNCHED("quant_int8_rows_kernel", launch_pdl(early, quant_int8_rows_kernel<T, kGated>, dim3((unsigned)blocks),
+                                                     dim3(threads * per_block), 0, st, p, threads));
+  return B200MOE_OK;
+}
+
+}  // namespace
+}  // namespace b200moe
+
+using namespace b200moe;
+
+extern "C" int b200moe_quant_int8_rows(const void* in, b200moe_dtype dtype, int64_t in_stride, int8_t* q, int64_t q_stride,
+                                       float* scales, int64_t rows, int hidden, int gated, const int32_t* rows_per_segment,
+                                       int num_segments, b200moe_stream stream) {
+  B200_CHECK_ARG(rows >= 0 && rows <= 0x7fffffff && hidden >= 0, "quant_int8_rows: negative or too large size");
+  B200_CHECK_ARG(rows_per_segment == nullptr || num_segments >= 0, "quant_int8_rows: negative number of segments");
+  if (rows == 0 || hidden == 0) return B200MOE_OK;
+  B200_CHECK_ARG(in && q && scales, "quant_int8_rows: null pointer");
+  const QuantInt8Params p = {in, q, scales, rows_per_segment, rows, in_stride, q_stride, hidden, num_segments};
+  int rc = B200MOE_OK;
+  B200_DISPATCH_FLOAT(dtype, "quant_int8_rows",
+                      rc = gated ? launch<scalar_t, true>(p, as_stream(stream)) : launch<scalar_t, false>(p, as_stream(stream)));
+  return rc;
+}

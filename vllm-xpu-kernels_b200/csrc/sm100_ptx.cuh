@@ -673,6 +673,25 @@ __device__ __forceinline__ void umma_f16_pair_block(uint32_t tmem_d, uint64_t ad
         "n"(3 * kAStep), "n"(kBStep), "n"(2 * kBStep), "n"(3 * kBStep)
       : "memory");
 }
+// 8-bit integers (both signed, int32 sums): kind::i8, K = 32 bytes an instruction as for the other 8-bit types.
+__host__ __device__ constexpr uint32_t make_idesc_i8(uint32_t M, uint32_t N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+template <int kAStep, int kBStep>
+__device__ __forceinline__ void umma_i8_pair_block(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                   uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred pa;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\tsetp.ne.b32 pa, %4, 0;\n\t"
+      "add.u64 a1, %1, %5;\n\tadd.u64 a2, %1, %6;\n\tadd.u64 a3, %1, %7;\n\t"
+      "add.u64 b1, %2, %8;\n\tadd.u64 b2, %2, %9;\n\tadd.u64 b3, %2, %10;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, pa;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], a1, b1, %3, 1;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], a2, b2, %3, 1;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], a3, b3, %3, 1;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "n"(kAStep), "n"(2 * kAStep),
+        "n"(3 * kAStep), "n"(kBStep), "n"(2 * kBStep), "n"(3 * kBStep)
+      : "memory");
+}
 // One arrival on the barrier at `bar`'s offset in both CTAs of the pair once the pair's MMAs
 // issued so far have completed.
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {

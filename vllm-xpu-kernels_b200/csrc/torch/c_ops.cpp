@@ -238,24 +238,6 @@ void silu_and_mul_quant(at::Tensor& out, at::Tensor& input, at::Tensor& scale) {
                                           scale.data_ptr<float>(), rows, (int)d, current_stream()));
 }
 
-// Rows [..., hidden] whose last dimension is dense and whose rows are evenly spaced: the row stride in elements.
-int64_t row_stride(const at::Tensor& t, const char* name) {
-  const int64_t hidden = t.size(-1);
-  if (t.numel() == 0) return hidden;
-  TORCH_CHECK(hidden == 1 || t.stride(-1) == 1, "b200_add_rms_norm: the last dimension of ", name, " must be contiguous");
-  if (t.dim() == 1) return hidden;
-  int64_t at = t.dim() - 2;
-  while (at > 0 && t.size(at) == 1) --at;       // (the stride of a single row says nothing)
-  const int64_t stride = t.size(at) == 1 ? hidden : t.stride(at);
-  int64_t next = stride * t.size(at);
-  for (int64_t d = at - 1; d >= 0; --d) {
-    if (t.size(d) == 1) continue;
-    TORCH_CHECK(t.stride(d) == next, "b200_add_rms_norm: the rows of ", name, " must be evenly spaced");
-    next *= t.size(d);
-  }
-  return stride;
-}
-
 // Memory as `n` pieces of `length` bytes, `stride` bytes apart.
 struct Pieces {
   const char* at;
@@ -313,10 +295,10 @@ void b200_add_rms_norm(const at::Tensor& input, const std::optional<at::Tensor>&
   a.hidden = (int)hidden;
   a.eps = (float)epsilon;
   a.input = input.data_ptr();
-  a.input_stride = row_stride(input, "input");
+  a.input_stride = row_stride(input, "b200_add_rms_norm", "input");
   if (residual.has_value()) {
     a.residual = residual->data_ptr();
-    a.residual_stride = row_stride(*residual, "residual");
+    a.residual_stride = row_stride(*residual, "b200_add_rms_norm", "residual");
     TORCH_CHECK(rows <= 1 || a.residual_stride >= hidden, "b200_add_rms_norm: the rows of residual must not overlap");
     TORCH_CHECK(!overlap(pieces_of_rows(input, a.input_stride), pieces_of_rows(*residual, a.residual_stride)),
                 "b200_add_rms_norm: residual must not overlap the input");
@@ -331,7 +313,7 @@ void b200_add_rms_norm(const at::Tensor& input, const std::optional<at::Tensor>&
   }
   if (out.has_value()) {
     a.out = out->data_ptr();
-    a.out_stride = row_stride(*out, "out");
+    a.out_stride = row_stride(*out, "b200_add_rms_norm", "out");
     TORCH_CHECK(rows <= 1 || a.out_stride >= hidden, "b200_add_rms_norm: the rows of out must not overlap");
     TORCH_CHECK(!overlap(pieces_of_rows(*out, a.out_stride), pieces_of_rows(input, a.input_stride)) || (a.out == a.input && (rows <= 1 || a.out_stride == a.input_stride)),
                 "b200_add_rms_norm: out must be the input or not overlap it");
@@ -349,7 +331,7 @@ void b200_add_rms_norm(const at::Tensor& input, const std::optional<at::Tensor>&
     TORCH_CHECK(rows <= 1 || groups <= 1 || apart > ((scales->stride(0) == next ? rows : groups) - 1) * next,
                 "b200_add_rms_norm: scales must not overlap themselves");
     a.q = out_q->data_ptr();
-    a.q_stride = row_stride(*out_q, "out_q");
+    a.q_stride = row_stride(*out_q, "b200_add_rms_norm", "out_q");
     TORCH_CHECK(rows <= 1 || a.q_stride >= hidden, "b200_add_rms_norm: the rows of out_q must not overlap");
     a.scales = scales->data_ptr<float>();
     a.s_stride_row = scales->stride(0);
@@ -374,9 +356,44 @@ void b200_add_rms_norm(const at::Tensor& input, const std::optional<at::Tensor>&
   check_status(b200moe_add_rms_norm(&a, current_stream()));
 }
 
+// Rows as int8 codes with a scale each; `gated`: of silu(gate) * up of rows [gate | up].
+void quant_int8_rows(const at::Tensor& input, const at::Tensor& out, const at::Tensor& scales, bool gated, const char* op) {
+  check_cuda(input, "input");
+  TORCH_CHECK(input.dim() >= 1 && out.dim() == input.dim(), op, ": input must be [..., ", gated ? "2 * " : "", "hidden_size], out [..., hidden_size]");
+  const int64_t hidden = out.size(-1);
+  TORCH_CHECK(input.size(-1) == (gated ? 2 * hidden : hidden) &&
+                  input.sizes().slice(0, input.dim() - 1) == out.sizes().slice(0, out.dim() - 1),
+              op, ": input must be [..., ", gated ? "2 * " : "", "hidden_size], out [..., hidden_size]");
+  int64_t rows = 1;
+  for (int64_t d = 0; d + 1 < out.dim(); ++d) rows *= out.size(d);
+  TORCH_CHECK(hidden <= 0x3fffffff && rows <= 0x7fffffff, op, ": input is too large");
+  const b200moe_dtype dtype = float_dtype(input, op);
+  TORCH_CHECK(out.scalar_type() == at::kChar, op, ": out must be int8");
+  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.is_contiguous() && scales.numel() == rows, op,
+              ": scales must be contiguous float32, one a row");
+  TORCH_CHECK(out.device() == input.device() && scales.device() == input.device(), op, ": all tensors must be on the input's device");
+  const int64_t in_stride = row_stride(input, op, "input"), q_stride = row_stride(out, op, "out");
+  TORCH_CHECK(rows <= 1 || q_stride >= hidden, op, ": the rows of out must not overlap");
+  const Pieces s = {(const char*)scales.data_ptr(), scales.numel() ? 1 : 0, 0, scales.numel() * 4};
+  const Pieces q = pieces_of_rows(out, q_stride), in = pieces_of_rows(input, in_stride);
+  TORCH_CHECK(!overlap(q, in) && !overlap(s, in) && !overlap(s, q), op, ": tensors must not overlap");
+  if (rows == 0 || hidden == 0) return;
+  const c10::cuda::CUDAGuard guard(input.device());
+  check_status(b200moe_quant_int8_rows(input.data_ptr(), dtype, in_stride, (int8_t*)out.data_ptr(), q_stride, scales.data_ptr<float>(),
+                                       rows, (int)hidden, gated, nullptr, 0, current_stream()));
+}
+void b200_quant_int8_rows(const at::Tensor& input, const at::Tensor& out, const at::Tensor& scales) {
+  quant_int8_rows(input, out, scales, false, "b200_quant_int8_rows");
+}
+void b200_silu_and_mul_quant_int8_rows(const at::Tensor& out, const at::Tensor& input, const at::Tensor& scales) {
+  quant_int8_rows(input, out, scales, true, "b200_silu_and_mul_quant_int8_rows");
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(_C, m) {
+  m.def("b200_quant_int8_rows(Tensor input, Tensor(a!) out, Tensor(b!) scales) -> ()");
+  m.def("b200_silu_and_mul_quant_int8_rows(Tensor(a!) out, Tensor input, Tensor(b!) scales) -> ()");
   m.def("gelu_and_mul(Tensor! out, Tensor input) -> ()");
   m.def("gelu_tanh_and_mul(Tensor! out, Tensor input) -> ()");
   m.def("relu2_no_mul(Tensor! out, Tensor! input) -> ()");
@@ -420,6 +437,8 @@ TORCH_LIBRARY_IMPL(_C, CUDA, m) {
   m.impl("swigluoai_and_mul", &swigluoai_and_mul);
   m.impl("per_token_group_fp8_quant", &per_token_group_fp8_quant);
   m.impl("b200_add_rms_norm", &b200_add_rms_norm);
+  m.impl("b200_quant_int8_rows", &b200_quant_int8_rows);
+  m.impl("b200_silu_and_mul_quant_int8_rows", &b200_silu_and_mul_quant_int8_rows);
   m.impl("b200_quant_mxfp8", &b200_quant_mxfp8);
   m.impl("gelu_and_mul", &gelu_and_mul);
   m.impl("gelu_tanh_and_mul", &gelu_tanh_and_mul);

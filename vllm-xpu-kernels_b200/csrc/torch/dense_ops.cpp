@@ -1,0 +1,199 @@
+// The dense layers beside the routed experts: torch.ops._xpu_C.b200_int8_linear, b200_gated_linear and
+// b200_gated_linear_backward over the C ABI.  No counterpart in the reference, which multiplies dense layers by library calls.
+#include <ATen/MemoryOverlap.h>
+
+#include "layer.h"
+
+using namespace b200shim;
+
+namespace {
+
+void same_device(const at::Tensor& t, const at::Tensor& input, const char* op, const char* name) {
+  TORCH_CHECK(t.device() == input.device(), op, ": ", name, " must be on the input's device");
+}
+void writable(const at::Tensor& t, const char* op, const char* name, std::initializer_list<const at::Tensor*> others) {
+  TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, op, ": ", name, " must not be expanded");
+  for (const at::Tensor* o : others)
+    if (o != nullptr && o->defined()) {
+      const auto s = at::get_overlap_status(t, *o);
+      TORCH_CHECK(s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial, op, ": ", name,
+                  " must not share memory with another tensor of the call");
+    }
+}
+bool same_leading(const at::Tensor& a, const at::Tensor& b) {
+  return a.dim() == b.dim() && a.sizes().slice(0, a.dim() - 1) == b.sizes().slice(0, b.dim() - 1);
+}
+int64_t rows_of(const at::Tensor& t) {
+  int64_t rows = 1;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) rows *= t.size(d);
+  return rows;
+}
+int32_t* status_word(const at::Tensor& like) {
+  int32_t* word = device_status_word(like.get_device());
+  raise_if_timed_out(word);   // an earlier call on this device gave up a wait
+  return word;
+}
+
+// out = input weight^T with 8-bit integers: input int8 rows with their scales, or rows that are quantised on the way.
+void b200_int8_linear(const at::Tensor& out, const at::Tensor& input, const std::optional<at::Tensor>& input_scales,
+                      const at::Tensor& weight, const at::Tensor& weight_scales, const std::optional<at::Tensor>& bias) {
+  const char* const op = "b200_int8_linear";
+  check_cuda(input, "input");
+  TORCH_CHECK(input.dim() >= 1 && out.dim() >= 1 && weight.dim() == 2, op, ": input must be [..., K], weight [N, K], out [..., N]");
+  const int64_t K = input.size(-1), N = weight.size(0), rows = rows_of(input);
+  TORCH_CHECK(weight.size(1) == K, op, ": input and weight must have the same K");
+  TORCH_CHECK(same_leading(out, input) && out.size(-1) == N, op, ": out must be [..., N]");
+  TORCH_CHECK(rows <= 0x7fffffff && N <= 0x7fffffff && K <= B200MOE_INT8_MAX_K, op, ": too large (K is at most ", B200MOE_INT8_MAX_K, ")");
+  TORCH_CHECK(weight.scalar_type() == at::kChar && weight.is_contiguous(), op, ": weight must be contiguous int8");
+  TORCH_CHECK(weight_scales.scalar_type() == at::kFloat && weight_scales.is_contiguous() && weight_scales.numel() == N, op,
+              ": weight_scales must be contiguous float32 [N]");
+  TORCH_CHECK(K > 0 && K % 16 == 0, op, ": K must be a multiple of 16");
+  for (const auto& [t, name] : {std::pair<const at::Tensor&, const char*>{out, "out"}, {weight, "weight"}, {weight_scales, "weight_scales"}})
+    same_device(t, input, op, name);
+  const bool codes = input.scalar_type() == at::kChar;
+  TORCH_CHECK(codes == input_scales.has_value(), op, ": int8 rows come with input_scales, other rows without");
+  b200moe_int8_linear_args a = {};
+  a.d_dtype = float_dtype(out, op);
+  if (bias.has_value()) {
+    same_device(*bias, input, op, "bias");
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N && bias->is_contiguous(), op, ": bias must be contiguous [N]");
+    TORCH_CHECK(bias->scalar_type() == at::kHalf || bias->scalar_type() == at::kBFloat16, op, ": bias must be float16 or bfloat16");
+    a.bias = bias->data_ptr();
+    a.bias_dtype = float_dtype(*bias, op);
+  }
+  if (codes) {
+    same_device(*input_scales, input, op, "input_scales");
+    TORCH_CHECK(input_scales->scalar_type() == at::kFloat && input_scales->is_contiguous() && input_scales->numel() == rows, op,
+                ": input_scales must be contiguous float32, one a row");
+  } else {
+    float_dtype(input, op);
+  }
+  const int64_t in_stride = row_stride(input, op, "input");
+  a.d_stride = row_stride(out, op, "out");
+  TORCH_CHECK(rows <= 1 || a.d_stride >= N, op, ": the rows of out must not overlap");
+  writable(out, op, "out", {&input, &weight, &weight_scales, bias.has_value() ? &*bias : nullptr, codes ? &*input_scales : nullptr});
+  if (rows == 0 || N == 0) return;
+  const c10::cuda::CUDAGuard guard(input.device());
+  a.status = status_word(input);
+  at::Tensor q, s;
+  if (codes) {
+    a.x = (const int8_t*)input.data_ptr();
+    a.x_scale = input_scales->data_ptr<float>();
+    a.x_stride = in_stride;
+  } else {
+    q = at::empty({rows, K}, input.options().dtype(at::kChar));
+    s = at::empty({rows}, input.options().dtype(at::kFloat));
+    check_status(b200moe_quant_int8_rows(input.data_ptr(), float_dtype(input, op), in_stride, (int8_t*)q.data_ptr(), K,
+                                         s.data_ptr<float>(), rows, (int)K, 0, nullptr, 0, current_stream()));
+    a.x = (const int8_t*)q.data_ptr();
+    a.x_scale = s.data_ptr<float>();
+    a.x_stride = K;
+  }
+  a.w = (const int8_t*)weight.data_ptr();
+  a.w_scale = weight_scales.data_ptr<float>();
+  a.d = out.data_ptr();
+  a.rows = rows; a.n = (int)N; a.k = (int)K;
+  check_status(b200moe_int8_linear(&a, current_stream()));
+}
+
+// What the gated product's passes have in common; weight [2 I, H], gate rows first.
+b200moe_gated_linear_args gated_args(const at::Tensor& input, const at::Tensor& weight, const char* op) {
+  check_cuda(input, "input");
+  TORCH_CHECK(input.dim() >= 1 && weight.dim() == 2, op, ": input must be [..., H], weight [2 I, H]");
+  TORCH_CHECK(weight.size(1) == input.size(-1) && weight.size(0) % 2 == 0, op, ": weight must be [2 I, H] for an input [..., H]");
+  TORCH_CHECK(input.scalar_type() == at::kBFloat16 || input.scalar_type() == at::kHalf, op, ": only float16 and bfloat16 are supported");
+  TORCH_CHECK(weight.scalar_type() == input.scalar_type(), op, ": weight must have the input's dtype");
+  TORCH_CHECK(weight.is_contiguous(), op, ": weight must be contiguous");
+  same_device(weight, input, op, "weight");
+  b200moe_gated_linear_args a = {};
+  const int64_t rows = rows_of(input);
+  TORCH_CHECK(rows <= 0x7fffffff && weight.size(0) <= 0x3fffffff && weight.size(1) <= 0x7fffffff, op, ": too large");
+  a.x = input.data_ptr(); a.w = weight.data_ptr();
+  a.rows = rows; a.inter = (int)(weight.size(0) / 2); a.hidden = (int)weight.size(1);
+  a.x_stride = row_stride(input, op, "input");
+  a.dtype = float_dtype(input, op);
+  TORCH_CHECK(a.hidden % 8 == 0 && a.x_stride % 8 == 0, op, ": rows must be multiples of 8 values apart and long");
+  return a;
+}
+void check_pre(const at::Tensor& pre, const at::Tensor& input, const b200moe_gated_linear_args& a, const char* op) {
+  same_device(pre, input, op, "pre");
+  TORCH_CHECK(pre.scalar_type() == at::kFloat && pre.is_contiguous() && pre.numel() == a.rows * 2 * a.inter &&
+                  (pre.dim() == 0 || pre.size(-1) == 2 * (int64_t)a.inter),
+              op, ": pre must be contiguous float32 [..., 2 I]");
+}
+
+void b200_gated_linear(const at::Tensor& out, const at::Tensor& input, const at::Tensor& weight, const std::optional<at::Tensor>& pre) {
+  const char* const op = "b200_gated_linear";
+  b200moe_gated_linear_args a = gated_args(input, weight, op);
+  same_device(out, input, op, "out");
+  TORCH_CHECK(same_leading(out, input) && out.size(-1) == a.inter, op, ": out must be [..., I]");
+  TORCH_CHECK(out.scalar_type() == input.scalar_type(), op, ": out must have the input's dtype");
+  a.out = out.data_ptr();
+  a.out_stride = row_stride(out, op, "out");
+  TORCH_CHECK(a.rows <= 1 || a.out_stride >= a.inter, op, ": the rows of out must not overlap");
+  writable(out, op, "out", {&input, &weight, pre.has_value() ? &*pre : nullptr});
+  if (pre.has_value()) {
+    check_pre(*pre, input, a, op);
+    writable(*pre, op, "pre", {&input, &weight});
+    a.pre = pre->data_ptr<float>();
+  }
+  TORCH_CHECK(a.hidden > 0, op, ": rows have no values");
+  if (a.rows == 0 || a.inter == 0) return;
+  const c10::cuda::CUDAGuard guard(input.device());
+  a.status = status_word(input);
+  check_status(b200moe_gated_linear(&a, current_stream()));
+}
+
+void b200_gated_linear_backward(const at::Tensor& grad_out, const at::Tensor& pre, const at::Tensor& input, const at::Tensor& weight,
+                                const std::optional<at::Tensor>& grad_input, const std::optional<at::Tensor>& grad_weight) {
+  const char* const op = "b200_gated_linear_backward";
+  b200moe_gated_linear_args a = gated_args(input, weight, op);
+  same_device(grad_out, input, op, "grad_out");
+  TORCH_CHECK(same_leading(grad_out, input) && grad_out.size(-1) == a.inter, op, ": grad_out must be [..., I]");
+  TORCH_CHECK(grad_out.scalar_type() == input.scalar_type(), op, ": grad_out must have the input's dtype");
+  check_pre(pre, input, a, op);
+  a.grad = grad_out.data_ptr();
+  a.grad_stride = row_stride(grad_out, op, "grad_out");
+  a.pre = pre.data_ptr<float>();
+  if (grad_input.has_value()) {
+    const at::Tensor& t = *grad_input;
+    same_device(t, input, op, "grad_input");
+    TORCH_CHECK(t.sizes() == input.sizes() && t.scalar_type() == input.scalar_type(), op, ": grad_input must have the input's shape and dtype");
+    a.grad_x = t.data_ptr();
+    a.grad_x_stride = row_stride(t, op, "grad_input");
+    TORCH_CHECK(a.rows <= 1 || a.grad_x_stride >= a.hidden, op, ": the rows of grad_input must not overlap");
+    writable(t, op, "grad_input", {&grad_out, &pre, &input, &weight, grad_weight.has_value() ? &*grad_weight : nullptr});
+  }
+  if (grad_weight.has_value()) {
+    const at::Tensor& t = *grad_weight;
+    same_device(t, input, op, "grad_weight");
+    TORCH_CHECK(t.sizes() == weight.sizes() && t.scalar_type() == weight.scalar_type() && t.is_contiguous(), op,
+                ": grad_weight must be contiguous, with the weight's shape and dtype");
+    a.grad_w = t.data_ptr();
+    writable(t, op, "grad_weight", {&grad_out, &pre, &input, &weight});
+  }
+  const c10::cuda::CUDAGuard guard(input.device());
+  a.status = status_word(input);
+  a.workspace_bytes = b200moe_gated_linear_backward_workspace_bytes(a.rows, a.inter);
+  const at::Tensor workspace = at::empty({(int64_t)a.workspace_bytes}, input.options().dtype(at::kByte));
+  a.workspace = workspace.data_ptr();
+  check_status(b200moe_gated_linear_backward(&a, current_stream()));
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(_xpu_C, m) {
+  m.def(
+      "b200_int8_linear(Tensor(a!) out, Tensor input, Tensor? input_scales, Tensor weight, Tensor weight_scales, "
+      "Tensor? bias=None) -> ()");
+  m.def("b200_gated_linear(Tensor(a!) out, Tensor input, Tensor weight, Tensor(b!)? pre=None) -> ()");
+  m.def(
+      "b200_gated_linear_backward(Tensor grad_out, Tensor pre, Tensor input, Tensor weight, Tensor(a!)? grad_input, "
+      "Tensor(b!)? grad_weight) -> ()");
+}
+
+TORCH_LIBRARY_IMPL(_xpu_C, CUDA, m) {
+  m.impl("b200_int8_linear", &b200_int8_linear);
+  m.impl("b200_gated_linear", &b200_gated_linear);
+  m.impl("b200_gated_linear_backward", &b200_gated_linear_backward);
+}

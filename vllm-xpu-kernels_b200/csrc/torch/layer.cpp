@@ -150,6 +150,7 @@ b200moe_dtype dtype16(at::ScalarType t, const char* what) {
 struct Weights {
   WeightDesc d13, d2;
   bool i4;                    // int4 weights whose shapes the block-scaled kernel takes (gemm_tc_i4.cu)
+  bool i8;                    // int8 weights: rows are quantised to int8 ahead of either GEMM
 };
 Weights describe(const Plan& p, int64_t hidden, at::ScalarType out_dtype, at::Device device) {
   TORCH_CHECK(p.w13.device() == device && p.w2.device() == device, "weights must be on the device of hidden_states");
@@ -172,6 +173,8 @@ Weights describe(const Plan& p, int64_t hidden, at::ScalarType out_dtype, at::De
     return d.format == B200MOE_W_INT4_NK && (d.group == 128 || d.group == 256) && k % 128 == 0;
   };
   w.i4 = i4_ok(w.d13, hidden) && i4_ok(w.d2, k2);
+  TORCH_CHECK(w.d13.int8 == w.d2.int8, "w13 and w2 must both be int8 or neither");
+  w.i8 = w.d13.int8;
   return w;
 }
 
@@ -216,6 +219,13 @@ struct Experts {
   }
   void lay_out_second(Layout& l) {
     const int64_t I = p.inter, I2 = o.form == kUnfused ? inter2() : I;
+    if (weights.i8) {
+      if (o.form == kEpilogue) act = l.take(M * I * 4);
+      else if (p.act != kSilu) act = l.take(M * I2 * 2);
+      act_q = l.take(M * I2);
+      act_s = l.take(M * 4);
+      return;
+    }
     const bool direct_fp8 = p.block_fp8 && (o.form == kFp8 || (p.act == kSilu && I % 128 == 0));
     if (!direct_fp8 && !gated_quant() && !planes_out()) act = l.take(M * I2 * 2);
     if (p.block_fp8) {
@@ -267,13 +277,28 @@ struct Experts {
     check_status(b200moe_grouped_gemm(&g, stream));
   }
 
+  // Int8 layers: rows between the GEMMs are quantised from the activation's fp32 values where gemm1's epilogue applies it
+  // (16-bit ones would move every twentieth code), else from 16 bits as the activation kernels take and give them.
+  void quantise_int8(uint8_t* ws, const void* from, b200moe_dtype type, int64_t stride, int gated) const {
+    check_status(b200moe_quant_int8_rows(from, type, stride, (int8_t*)(ws + act_q), inter2(), (float*)(ws + act_s), M, (int)inter2(),
+                                         gated, nullptr, 0, stream));
+  }
   void run(uint8_t* ws, const void* a, const void* a_scale, const int32_t* rows, void* d) const {
     const int64_t I = p.inter, I2 = inter2();
+    if (weights.i8 && o.form == kEpilogue) {
+      gemm(true, a, B200MOE_I8, a_scale, ws + act, B200MOE_F32, nullptr, rows, B200MOE_EPI_SILU_MUL);
+      mark(o, gil, "gemm1");
+      quantise_int8(ws, ws + act, B200MOE_F32, I, 0);
+      mark(o, gil, "activation");
+      gemm(false, ws + act_q, B200MOE_I8, ws + act_s, d, out, nullptr, rows, B200MOE_EPI_NONE);
+      mark(o, gil, "gemm2");
+      return;
+    }
     const b200moe_dtype mx_dtype =
         sums ? (planes == 3 ? B200MOE_FP8_E4M3_X3_EVENS_FIRST : B200MOE_FP8_E4M3_X2_EVENS_FIRST) :
         planes == 2 ? B200MOE_FP8_E4M3_X2 : B200MOE_FP8_E4M3;
     const int terms = planes + (sums ? B200MOE_PLANES_EVENS_FIRST : 0);
-    const b200moe_dtype a_dtype = a_fp8 ? B200MOE_FP8_E4M3 : planes_in ? mx_dtype : out;
+    const b200moe_dtype a_dtype = weights.i8 ? B200MOE_I8 : a_fp8 ? B200MOE_FP8_E4M3 : planes_in ? mx_dtype : out;
     bool fp8_ready = false, planes_ready = false;
     if (o.form == kFp8) {
       gemm(true, a, a_dtype, a_scale, ws + act_q, B200MOE_FP8_E4M3, ws + act_s, rows, B200MOE_EPI_SILU_MUL);
@@ -298,7 +323,9 @@ struct Experts {
         (pairs ? t.slice(1, 0, 2 * I, 2) : t.narrow(1, 0, I)).clamp_max_(p.clamp);
         (pairs ? t.slice(1, 1, 2 * I, 2) : t.narrow(1, I, I)).clamp_(-p.clamp, p.clamp);
       }
-      if (p.block_fp8 && p.act == kSilu && I % 128 == 0) {
+      if (weights.i8 && p.act == kSilu) {
+        quantise_int8(ws, ws + g1, out, 2 * I, 1);
+      } else if (p.block_fp8 && p.act == kSilu && I % 128 == 0) {
         // SiLU, multiply and the 1x128 e4m3 quantisation of gemm2's input in one pass over the rows
         // that the experts' segments use (the buffers may be sized for a worst case)
         check_status(b200moe_silu_and_mul_per_block_quant_ragged(ws + act_q, (float*)(ws + act_s), ws + g1, out, M,
@@ -321,7 +348,10 @@ struct Experts {
       }
     }
     mark(o, gil, "activation");
-    if (p.block_fp8) {
+    if (weights.i8) {
+      if (p.act != kSilu) quantise_int8(ws, ws + act, out, I2, 0);
+      gemm(false, ws + act_q, B200MOE_I8, ws + act_s, d, out, nullptr, rows, B200MOE_EPI_NONE);
+    } else if (p.block_fp8) {
       if (!fp8_ready)
         check_status(b200moe_per_token_group_fp8_quant(ws + act, out, ws + act_q, (float*)(ws + act_s), M, (int)I2, 128,
                                                        1e-10f, 0, I2 / 128, 1, stream));
@@ -449,6 +479,8 @@ PyObject* layer_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   raise_if_timed_out(device_status_word(x.get_device()));   // an earlier call on this device gave up a wait
   if (o.rows_hint == 0 && map.has_value() && p.total_experts > p.experts)
     o.rows_hint = std::max<int64_t>(1, M * p.experts / p.total_experts);   // the other ranks' share is masked
+  TORCH_CHECK_NOT_IMPLEMENTED(!weights.i8 || (!a1q.has_value() && o.form != kFp8),
+                              "int8 layers quantise their rows themselves: pass 16-bit hidden_states without a1q_scale");
   const bool quant_fp8 = p.block_fp8 && !a1q.has_value();
   // (the block-scaled int4 kernel has no activation in its epilogue)
   const bool i4 = weights.i4 && o.form == kUnfused &&
@@ -469,8 +501,13 @@ PyObject* layer_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const size_t sort_bytes = b200moe_sort_workspace_bytes(M, (int)p.experts);
   const size_t sort_at = l.take(sort_bytes);
   const size_t a_at = l.end;
-  size_t as_at = a_at;
-  if (quant_fp8) {
+  size_t as_at = a_at, token_at = a_at, token_s_at = a_at;
+  if (weights.i8) {
+    l.take(M * H);
+    as_at = l.take(M * 4);
+    token_at = l.take(T * H);
+    token_s_at = l.take(T * 4);
+  } else if (quant_fp8) {
     l.take(M * H);
     as_at = l.take(M * (H / 128) * 4);
   } else if (planes_in) {
@@ -489,7 +526,14 @@ PyObject* layer_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   uint8_t* ws = workspace.mem.data_ptr<uint8_t>();
   int32_t *rows = (int32_t*)(ws + rows_at), *row_map = (int32_t*)(ws + map_at);
   const int32_t* emap = map.has_value() ? map->data_ptr<int32_t>() : nullptr;
-  if (quant_fp8)
+  if (weights.i8) {
+    // a token is quantised once, then copied to its experts' rows
+    check_status(b200moe_quant_int8_rows(x.data_ptr(), float_dtype(x, "hidden_states"), H, (int8_t*)(ws + token_at), H,
+                                         (float*)(ws + token_s_at), T, (int)H, 0, nullptr, 0, st));
+    check_status(b200moe_remap_hidden_states(ws + token_at, ws + token_s_at, ws + a_at, ws + as_at, emap, rows, row_map, ids.data_ptr(),
+                                             index_dtype(ids), T, (int)H, 1, 1, 4, (int)K, (int)p.total_experts, (int)p.experts,
+                                             ws + sort_at, sort_bytes, st));
+  } else if (quant_fp8)
     check_status(b200moe_remap_quant_fp8(x.data_ptr(), float_dtype(x, "b200_remap_quant_fp8"), ws + a_at,
                                          (float*)(ws + as_at), emap, rows, row_map, ids.data_ptr(), index_dtype(ids), T,
                                          (int)H, (int)K, (int)p.total_experts, (int)p.experts, ws + sort_at, sort_bytes,
@@ -506,7 +550,7 @@ PyObject* layer_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
         a1q.has_value() ? (int)a1q->size(1) : 0, a1q.has_value() ? (int)a1q->element_size() : 0, (int)K,
         (int)p.total_experts, (int)p.experts, ws + sort_at, sort_bytes, st));
   mark(o, gil, "permute");
-  e.run(ws, ws + a_at, (a_fp8 || planes_in) ? ws + as_at : nullptr, rows, ws + d_at);
+  e.run(ws, ws + a_at, (a_fp8 || planes_in || weights.i8) ? ws + as_at : nullptr, rows, ws + d_at);
   if (gather) {
     check_status(b200moe_moe_gather(y->data_ptr(), ws + d_at, w->data_ptr<float>(), row_map, out, T, (int)H, (int)K, st));
     mark(o, gil, "gather");
@@ -554,6 +598,7 @@ PyObject* layer_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const c10::cuda::CUDAGuard guard(x.device());
   const auto stream = at::cuda::getCurrentCUDAStream();
   const Weights weights = describe(p, H, y.scalar_type(), x.device());
+  TORCH_CHECK_NOT_IMPLEMENTED(!weights.i8, "grouped rows: 16-bit or block-scaled fp8 weights only");
   raise_if_timed_out(device_status_word(x.get_device()));
   WithoutGil gil;
   Experts e{p, weights, o, gil, out, y.scalar_type(), M, H, (int)segments, (int)x.get_device(),
@@ -602,6 +647,7 @@ PyObject* layer_few(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Plan q = p;   // (weights are read as they are: no quantised activations to go with them)
   q.block_fp8 = q.mx = false;
   const Weights weights = describe(q, H, y.scalar_type(), x.device());
+  TORCH_CHECK_NOT_IMPLEMENTED(!weights.i8, "the layer for a few tokens has no int8 weights");
   if (T == 0) Py_RETURN_NONE;
   static const b200moe_activation acts[] = {B200MOE_ACT_SILU, B200MOE_ACT_GELU, B200MOE_ACT_GELU_TANH, B200MOE_ACT_SWIGLUOAI,
                                             B200MOE_ACT_SILU, B200MOE_ACT_SWIGLUSTEP};

@@ -15,7 +15,7 @@ void raise_if_timed_out(int32_t* word);
 struct WeightDesc {
   b200moe_weight_format format;
   int group;          // int4: K elements per scale
-  bool fp8, mxfp4, fp8_block;
+  bool fp8, mxfp4, fp8_block, int8;
 };
 WeightDesc describe_weights(const at::Tensor& w, const std::optional<at::Tensor>& scale, int64_t N, int64_t K,
                             int64_t num_experts, int64_t layout, at::ScalarType activation_dtype);

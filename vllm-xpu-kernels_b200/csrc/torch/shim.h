@@ -64,6 +64,24 @@ inline void check_cuda(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
 }
 
+// Rows [..., n] whose last dimension is dense and whose rows are evenly spaced: the row stride in elements.
+inline int64_t row_stride(const at::Tensor& t, const char* op, const char* name) {
+  const int64_t n = t.size(-1);
+  if (t.numel() == 0) return n;
+  TORCH_CHECK(n == 1 || t.stride(-1) == 1, op, ": the last dimension of ", name, " must be contiguous");
+  if (t.dim() == 1) return n;
+  int64_t at = t.dim() - 2;
+  while (at > 0 && t.size(at) == 1) --at;       // (the stride of a single row says nothing)
+  const int64_t stride = t.size(at) == 1 ? n : t.stride(at);
+  int64_t next = stride * t.size(at);
+  for (int64_t d = at - 1; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    TORCH_CHECK(t.stride(d) == next, op, ": the rows of ", name, " must be evenly spaced");
+    next *= t.size(d);
+  }
+  return stride;
+}
+
 // Scratch for the multi-block sort path; empty when the single-block path runs.
 inline at::Tensor sort_workspace(const at::Tensor& like, int64_t numel, int64_t buckets) {
   const size_t bytes = b200moe_sort_workspace_bytes(numel, (int)buckets);

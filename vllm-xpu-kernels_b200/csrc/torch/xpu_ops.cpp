@@ -52,7 +52,9 @@ WeightDesc describe_weights(const at::Tensor& ptr_B, const std::optional<at::Ten
   const auto B_dtype = ptr_B.scalar_type();
   const bool is_weight_fp8 = (B_dtype == at::kFloat8_e4m3fn) || (B_dtype == at::kFloat8_e5m2);
   const bool is_B_mxfp4 = (B_dtype == at::kFloat4_e2m1fn_x2) && ptr_B_scale.has_value();
-  const bool is_B_int4 = (B_dtype == at::kChar) && ptr_B_scale.has_value();
+  // int8 weights have one fp32 scale an output channel, int4 pairs 16-bit scales per group of K
+  const bool is_B_int8 = (B_dtype == at::kChar) && ptr_B_scale.has_value() && ptr_B_scale->scalar_type() == at::kFloat;
+  const bool is_B_int4 = (B_dtype == at::kChar) && ptr_B_scale.has_value() && !is_B_int8;
   // fp8 weights with one-byte (e8m0) scales: the "mxfp8" recipe of
   // vllm_xpu_kernels/fused_moe_interface.py:47-61, weights [E,K,N], scales [E,K/32,N]
   const bool is_B_mxfp8 = is_weight_fp8 && ptr_B_scale.has_value() && ptr_B_scale->element_size() == 1;
@@ -64,7 +66,10 @@ WeightDesc describe_weights(const at::Tensor& ptr_B, const std::optional<at::Ten
   const int64_t B_E = ptr_B.size(0);
   int64_t B_K = ptr_B.size(1), B_N = ptr_B.size(2);
   b200moe_weight_format fmt;
-  if (is_B_int4) {
+  if (is_B_int8) {
+    B_K = ptr_B.size(2); B_N = ptr_B.size(1);
+    fmt = B200MOE_W_INT8_NK;
+  } else if (is_B_int4) {
     B_K = ptr_B.size(2) * 2; B_N = ptr_B.size(1);
     fmt = B200MOE_W_INT4_NK;
   } else if (is_B_mxfp4) {
@@ -91,7 +96,12 @@ WeightDesc describe_weights(const at::Tensor& ptr_B, const std::optional<at::Ten
   TORCH_CHECK(B_K == K, "ptr_A K dimension must match ptr_B logical K dimension and K");
   TORCH_CHECK(B_N == N, "ptr_B logical N dimension must match ptr_D N dimension and N");
   int64_t group_size = 0;
-  if (is_B_int4) {
+  if (is_B_int8) {
+    TORCH_CHECK(ptr_B_scale->is_contiguous(), "ptr_scales must be contiguous");
+    TORCH_CHECK(ptr_B_scale->numel() == num_experts * N && ptr_B_scale->dim() >= 2 && ptr_B_scale->size(0) == num_experts &&
+                    ptr_B_scale->size(1) == N, "ptr_scales of int8 must be float32 [num_experts, N]");
+    TORCH_CHECK(K % 16 == 0 && K <= B200MOE_INT8_MAX_K, "int8 grouped GEMM requires K divisible by 16 and at most ", B200MOE_INT8_MAX_K);
+  } else if (is_B_int4) {
     TORCH_CHECK(ptr_B_scale->is_contiguous(), "ptr_scales must be contiguous");
     TORCH_CHECK(ptr_B_scale->dim() == 3, "ptr_scales of int4 must be 3D [num_experts, group_num, N]");
     TORCH_CHECK(ptr_B_scale->size(0) == num_experts, "ptr_scales.size(0) of int4 must match num_experts");
@@ -133,7 +143,7 @@ WeightDesc describe_weights(const at::Tensor& ptr_B, const std::optional<at::Ten
     TORCH_CHECK(B_dtype == A_dtype, "w16a16 grouped gemm needs weights of the activation dtype");
   }
 
-  return {fmt, (int)group_size, is_weight_fp8, is_B_mxfp4, is_B_fp8_block};
+  return {fmt, (int)group_size, is_weight_fp8, is_B_mxfp4, is_B_fp8_block, is_B_int8};
 }
 
 }  // namespace b200shim
@@ -176,13 +186,19 @@ at::Tensor grouped_gemm_impl(at::Tensor& ptr_A, const std::optional<at::Tensor>&
     TORCH_CHECK(ptr_bias->size(0) == num_experts, "ptr_bias.size(0) must match num_experts");
     TORCH_CHECK(ptr_bias->size(1) == N, "ptr_bias.size(1) must match N");
     TORCH_CHECK(ptr_bias->scalar_type() == ptr_D.scalar_type() ||
-                    (ptr_D.scalar_type() == at::kFloat8_e4m3fn &&
+                    ((ptr_D.scalar_type() == at::kFloat8_e4m3fn || (w.int8 && ptr_D.scalar_type() == at::kFloat)) &&
                      ptr_bias->scalar_type() == (mid_f16 ? at::kHalf : at::kBFloat16)),
                 "ptr_bias must have ptr_D's dtype");
   }
   b200moe_gemm_args g = {};
   g.a = ptr_A.data_ptr();
-  if (A_dtype == at::kFloat8_e4m3fn) {
+  if (w.int8) {
+    TORCH_CHECK(A_dtype == at::kChar && ptr_A_scale.has_value() && ptr_A_scale->scalar_type() == at::kFloat &&
+                    ptr_A_scale->is_contiguous() && ptr_A_scale->numel() == A_total_M,
+                "int8 weights need int8 ptr_A and ptr_A_scale float32 [Total_M]");
+    g.a_dtype = B200MOE_I8;
+    g.a_scale = ptr_A_scale->data_ptr();
+  } else if (A_dtype == at::kFloat8_e4m3fn) {
     TORCH_CHECK((w.fp8 || w.mxfp4) && ptr_A_scale.has_value(),
                 "fp8 activations need fp8 or mxfp4 weights and ptr_A_scale");
     g.a_dtype = B200MOE_FP8_E4M3;
@@ -209,8 +225,8 @@ at::Tensor grouped_gemm_impl(at::Tensor& ptr_A, const std::optional<at::Tensor>&
     g.a_dtype = A_dtype == at::kBFloat16 ? B200MOE_BF16 : B200MOE_F16;
   }
   const bool d_quant = ptr_D.scalar_type() == at::kFloat8_e4m3fn;
-  TORCH_CHECK(ptr_D.scalar_type() == at::kBFloat16 || ptr_D.scalar_type() == at::kHalf || d_quant,
-              "ptr_D must be bfloat16 or float16");
+  TORCH_CHECK(ptr_D.scalar_type() == at::kBFloat16 || ptr_D.scalar_type() == at::kHalf || d_quant ||
+                  (w.int8 && ptr_D.scalar_type() == at::kFloat), "ptr_D must be bfloat16 or float16");
   if (d_quant) {
     // extended op only: quantised output of the fused SiLU epilogue, scales [Total_M, N / 256]
     TORCH_CHECK(allow_segments && epilogue == 1 && ptr_D_scale.has_value() && w.fp8_block &&
@@ -224,7 +240,7 @@ at::Tensor grouped_gemm_impl(at::Tensor& ptr_A, const std::optional<at::Tensor>&
   g.w_scale = ptr_B_scale.has_value() ? ptr_B_scale->data_ptr() : nullptr;
   g.bias = ptr_bias.has_value() ? ptr_bias->data_ptr() : nullptr;
   g.d = ptr_D.data_ptr();
-  g.d_dtype = d_quant ? B200MOE_FP8_E4M3 : (ptr_D.scalar_type() == at::kBFloat16 ? B200MOE_BF16 : B200MOE_F16);
+  g.d_dtype = d_quant ? B200MOE_FP8_E4M3 : ptr_D.scalar_type() == at::kFloat ? B200MOE_F32 : (ptr_D.scalar_type() == at::kBFloat16 ? B200MOE_BF16 : B200MOE_F16);
   g.d_scale = d_quant ? ptr_D_scale->data_ptr() : nullptr;
   g.mid_dtype = mid_f16 ? B200MOE_F16 : B200MOE_BF16;
   g.rows_per_expert = rows_per_expert.data_ptr<int32_t>();

@@ -14,7 +14,9 @@ csrc/xpu/grouped_gemm/xe_2/grouped_gemm_xe2_interface.hpp:200-223):
 
 * bf16 / fp16 and per-tensor fp8:  ``[E, K, N]`` (the transposed checkpoint);
 * block fp8 (fp32 scales ``[E, N/128, K/128]``): ``[E, N, K]`` or ``[E, K, N]``;
-* MXFP4 (``float4_e2m1fn_x2``): ``[E, N, K/2]`` with e8m0 scales ``[E, N, K/32]``.
+* MXFP4 (``float4_e2m1fn_x2``): ``[E, N, K/2]`` with e8m0 scales ``[E, N, K/32]``;
+* int8 (not in the reference): ``[E, N, K]`` with fp32 scales ``[E, N]``, one an output channel.  Rows are
+  quantised to int8 with one scale each ahead of either GEMM; K divisible by 16.
 """
 import os
 from typing import Optional
@@ -51,8 +53,10 @@ def _is_env_enabled(env_name: str, default: str = "0") -> bool:
     return value in ("1", "ON", "TRUE", "YES", "Y")
 
 
-def _get_recipe(is_fp8, is_mxfp8, is_mxfp4, is_int4, is_block_fp8):
-    if is_mxfp8:
+def _get_recipe(is_fp8, is_mxfp8, is_mxfp4, is_int4, is_block_fp8, is_int8=False):
+    if is_int8:
+        return "int8"
+    elif is_mxfp8:
         return "mxfp8"
     elif is_block_fp8:
         return "fp8block"
@@ -245,6 +249,7 @@ class XpuFusedMoe:
     """
 
     few_tokens = False       # (also of layers that were saved before there was a choice)
+    is_int8 = False          # (the same)
 
     def __init__(
         self,
@@ -279,7 +284,12 @@ class XpuFusedMoe:
                 f"{REF_FUSED_MOE_ENV} selects the reference's eager qdq simulation, "
                 "which this build does not ship: only the CUDA kernels run")
 
-        self.inter_size = _get_inter_size(w13, w13_scales, is_int4, is_mxfp4, is_block_fp8)
+        is_int8 = w13.dtype == torch.int8 and w13_scales is not None and w13_scales.dtype == torch.float32
+        if is_int8 and few_tokens:
+            raise NotImplementedError("few_tokens: 16-bit, block-scaled fp8, MXFP4 and int4 weights only")
+        if is_int8 and (w2.dtype != torch.int8 or w2_scales is None):
+            raise ValueError("int8 layers need int8 w13 and w2, and the scales of both")
+        self.inter_size = _get_inter_size(w13, w13_scales, is_int4 or is_int8, is_mxfp4, is_block_fp8)
         if is_int4 and not getattr(w13, "xpu_fused_moe", False):
             # uint4 with the default zero point 8 -> two's-complement int4 (reference
             # implement_zp, :135-162: u4 - 8 re-encoded per nibble, i.e. bit 3 flipped).
@@ -289,7 +299,7 @@ class XpuFusedMoe:
             w13, w2 = _signed_nibbles(w13), _signed_nibbles(w2)
         self.w13 = w13
         self.w2 = w2
-        if not (is_fp8 or is_mxfp4 or is_mxfp8 or is_block_fp8 or is_int4):
+        if not (is_fp8 or is_mxfp4 or is_mxfp8 or is_block_fp8 or is_int4 or is_int8):
             self.gemm1_wei_scales = None
             self.gemm2_wei_scales = None
         else:
@@ -311,8 +321,9 @@ class XpuFusedMoe:
         self.is_mxfp4 = is_mxfp4
         self.is_mxfp8 = is_mxfp8
         self.is_block_fp8 = is_block_fp8
+        self.is_int8 = is_int8
         self.gemm1_clamp_limit = gemm1_clamp_limit
-        self.recipe = _get_recipe(is_fp8, is_mxfp8, is_mxfp4, is_int4, is_block_fp8)
+        self.recipe = _get_recipe(is_fp8, is_mxfp8, is_mxfp4, is_int4, is_block_fp8, is_int8)
         self._use_ref = False
         # block-scaled fp8 with SiLU: the token-major tensor-core kernel can apply the activation and the
         # 1x128 e4m3 quantisation of gemm2's input in its epilogue (same values as the two-kernel form).
@@ -332,7 +343,7 @@ class XpuFusedMoe:
         # tiles.  With whole 128-feature tiles (I % 128 == 0) the fused form is taken at every
         # size; otherwise up to 96 routed rows per expert, where 128-token tiles are picked anyway
         # (fuse_activation=True forces it at every size).
-        is_16bit = not (is_fp8 or is_mxfp4 or is_mxfp8 or is_block_fp8 or is_int4)
+        is_16bit = not (is_fp8 or is_mxfp4 or is_mxfp8 or is_block_fp8 or is_int4 or is_int8)
         # SwigluOAI keeps gate and up of a feature on neighbouring accumulator lanes: one accumulator,
         # every tile size, so it is fused at every size.
         self._w16_fused_ok = (is_16bit and self._act_kind in ("silu", "swigluoai") and self.inter_size % 16 == 0
@@ -341,7 +352,9 @@ class XpuFusedMoe:
                                             or self.inter_size % 128 == 0) else 96
         if fuse_activation is None:
             # fused where the tensor-core kernel of this recipe has the epilogue
-            fuse_activation = self.is_mxfp4 and self._act_kind == "swigluoai"
+            # (int8: SiLU, whose fp32 values the rows of gemm2 are quantised from)
+            fuse_activation = ((self.is_mxfp4 and self._act_kind == "swigluoai") or
+                               (self.is_int8 and self._act_kind == "silu"))
         if is_block_fp8:
             fuse_activation = False     # (the fp8 form is chosen per call: fuses_activation)
         self.fuse_activation = fuse_activation
@@ -367,7 +380,7 @@ class XpuFusedMoe:
                             and hidden % 16 == 0 and self.inter_size % 8 == 0)
         if self.mx_acts and self._act_kind == "silu" and fuse_activation:
             raise ValueError("the block-scaled MXFP4 GEMM has no fused SiLU epilogue")
-        if fuse_activation and self._act_kind not in ("silu", "swigluoai"):
+        if fuse_activation and self._act_kind not in (("silu",) if is_int8 else ("silu", "swigluoai")):
             raise ValueError(f"no fused epilogue for the {self._act_kind} activation")
         if few_tokens and (is_fp8 or is_mxfp8):
             raise NotImplementedError("few_tokens: 16-bit, block-scaled fp8, MXFP4 and int4 weights only")
@@ -471,7 +484,7 @@ class XpuFusedMoe:
         if self.is_block_fp8:
             if rows.dtype != torch.float8_e4m3fn or a1q_scale is None:
                 raise ValueError("apply_sorted with block-scaled fp8 weights takes fp8 rows and a1q_scale")
-        elif self.is_fp8 or self.is_mxfp4 or self.is_mxfp8 or self.is_int4:
+        elif self.is_fp8 or self.is_mxfp4 or self.is_mxfp8 or self.is_int4 or self.is_int8:
             raise NotImplementedError("apply_sorted: 16-bit or block-scaled fp8 weights only")
         if rows.shape[0] == 0:
             return

@@ -439,20 +439,25 @@ int b200moe_quant_int8_rows(const void* in, b200moe_dtype dtype, int64_t in_stri
 
 /* The matrix product in 8-bit integers with a scale for each row of either operand:
  *   d[m, n] = (sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n] (+ bias[n])
- * The sum is exact (int32).  Zero-initialise the struct. */
+ * The sum is exact (int32).  Rows of 16 or 32 bits are quantised on the way, as b200moe_quant_int8_rows does it: a
+ * few of them by the product's kernel itself, more into the workspace.  Zero-initialise the struct. */
 typedef struct {
-  const int8_t* x;        /* [rows, k], 16-byte aligned, x_stride (a multiple of 16) from row to row */
-  const float* x_scale;   /* [rows]                                                  */
+  const void* x;          /* [rows, k], x_stride from row to row; int8: 16-byte aligned, stride a multiple of 16 */
+  const float* x_scale;   /* int8 rows: [rows]                                       */
   const int8_t* w;        /* [n, k], 16-byte aligned                                 */
   const float* w_scale;   /* [n]                                                     */
   const void* bias;       /* [n] bias_dtype, or NULL                                 */
   void* d;                /* [rows, n] d_dtype, d_stride from row to row             */
   int64_t rows, x_stride, d_stride;
   int n, k;               /* k: a multiple of 16, at most B200MOE_INT8_MAX_K         */
+  b200moe_dtype x_dtype;  /* I8, F32, F16 or BF16                                    */
   b200moe_dtype d_dtype;  /* F32, F16 or BF16                                        */
   b200moe_dtype bias_dtype; /* F16 or BF16                                           */
+  void* workspace;        /* rows that are not int8: ..._workspace_bytes, 16-byte aligned */
+  size_t workspace_bytes;
   int32_t* status;        /* as in b200moe_gemm_args, or NULL                        */
 } b200moe_int8_linear_args;
+size_t b200moe_int8_linear_workspace_bytes(int64_t rows, int k);
 int b200moe_int8_linear(const b200moe_int8_linear_args* args, b200moe_stream stream);
 
 /* Both projections of a gated feed-forward block, its activation and the product, and the gradients:

@@ -15,7 +15,7 @@ P, I, L, Z = ct.c_void_p, ct.c_int, ct.c_int64, ct.c_size_t
 class Int8LinearArgs(ct.Structure):
     """b200moe_int8_linear_args of include/b200moe.h."""
     _fields_ = [("x", P), ("x_scale", P), ("w", P), ("w_scale", P), ("bias", P), ("d", P), ("rows", L), ("x_stride", L), ("d_stride", L),
-                ("n", I), ("k", I), ("d_dtype", I), ("bias_dtype", I), ("status", P)]
+                ("n", I), ("k", I), ("x_dtype", I), ("d_dtype", I), ("bias_dtype", I), ("workspace", P), ("workspace_bytes", Z), ("status", P)]
 
 
 class GatedLinearArgs(ct.Structure):
@@ -53,12 +53,12 @@ def test_struct_layout(tmp_path, cls, name):
     assert got == [getattr(cls, f).offset for f, _ in cls._fields_] + [ct.sizeof(cls)]
 
 
-LINEAR = dict(x=256, x_scale=256, w=256, w_scale=256, d=256, rows=4, x_stride=64, d_stride=8, n=8, k=64, d_dtype=2)
+LINEAR = dict(x=256, x_scale=256, w=256, w_scale=256, d=256, rows=4, x_stride=64, d_stride=8, n=8, k=64, x_dtype=10, d_dtype=2)
 
 
 @pytest.mark.parametrize("change,message", [
     (dict(rows=-1), b"negative or too large"), (dict(rows=1 << 31), b"negative or too large"), (dict(n=-1), b"negative or too large"),
-    (dict(k=-16), b"negative or too large"), (dict(k=131072), b"at most 131071"), (dict(k=0), b"multiples of 16"),
+    (dict(k=-16), b"negative or too large"), (dict(k=131072), b"at most 131071"), (dict(k=0), b"multiples of 16"), (dict(x_dtype=3), b"input must be"),
     (dict(k=24), b"multiples of 16"), (dict(x_stride=72), b"multiples of 16"), (dict(d_dtype=3), b"out must be"),
     (dict(bias=256, bias_dtype=0), b"bias must be"), (dict(x=None), b"null pointer"), (dict(w_scale=None), b"null pointer"),
     (dict(x=264), b"16-byte aligned"), (dict(w=264), b"16-byte aligned"),
@@ -66,6 +66,15 @@ LINEAR = dict(x=256, x_scale=256, w=256, w_scale=256, d=256, rows=4, x_stride=64
 def test_int8_linear_refused_before_any_launch(lib, change, message):
     assert lib.b200moe_int8_linear(ct.byref(_filled(Int8LinearArgs, **{**LINEAR, **change})), None) == -1
     assert message in lib.b200moe_last_error()
+
+
+def test_int8_linear_workspace(lib):
+    lib.b200moe_int8_linear_workspace_bytes.restype = Z
+    assert lib.b200moe_int8_linear_workspace_bytes(L(300), 64) == 300 * 68
+    assert lib.b200moe_int8_linear_workspace_bytes(L(0), 64) == 0
+    for more in (dict(), dict(workspace=256, workspace_bytes=300 * 68 - 1), dict(workspace=264, workspace_bytes=300 * 68)):
+        assert lib.b200moe_int8_linear(ct.byref(_filled(Int8LinearArgs, **{**LINEAR, "x_dtype": 2, "rows": 300, **more})), None) == -4
+        assert b"workspace" in lib.b200moe_last_error()
 
 
 def test_nothing_to_do_is_no_launch(lib):
@@ -141,6 +150,7 @@ def test_schemas_and_no_cpu_path(native):
     assert schema(X.b200_gated_linear) == (["out", "input", "weight", "pre"], ["out", "pre"])
     assert schema(X.b200_gated_linear_backward) == (["grad_out", "pre", "input", "weight", "grad_input", "grad_weight"],
                                                     ["grad_input", "grad_weight"])
+    assert schema(X.b200_gated_product) == (["input", "weight"], [])
     x, w = torch.ones(2, 16, dtype=torch.bfloat16), torch.ones(8, 16, dtype=torch.bfloat16)
     from vllm_xpu_kernels.gated_linear import gated_linear
     with pytest.raises(NotImplementedError):

@@ -84,19 +84,41 @@ int check_gated(const b200moe_gated_linear_args* a) {
 
 using namespace b200moe;
 
+extern "C" size_t b200moe_int8_linear_workspace_bytes(int64_t rows, int k) {
+  return rows <= 0 || k <= 0 ? 0 : (size_t)rows * k + (size_t)rows * 4;
+}
+
 extern "C" int b200moe_int8_linear(const b200moe_int8_linear_args* a, b200moe_stream stream) {
   B200_CHECK_ARG(a != nullptr, "int8_linear: null argument struct");
   B200_CHECK_ARG(a->rows >= 0 && a->rows <= 0x7fffffff && a->n >= 0 && a->k >= 0, "int8_linear: negative or too large size");
   B200_CHECK_ARG(a->k <= B200MOE_INT8_MAX_K, "int8_linear: K must be at most %d, so that sums fit 32 bits", B200MOE_INT8_MAX_K);
-  B200_CHECK_ARG(a->k > 0 && a->k % 16 == 0 && a->x_stride % 16 == 0, "int8_linear: rows must be multiples of 16 values apart and long");
+  B200_CHECK_ARG(a->k > 0 && a->k % 16 == 0, "int8_linear: rows must be multiples of 16 values long");
+  B200_CHECK_ARG(a->x_dtype == B200MOE_I8 || a->x_dtype == B200MOE_F32 || a->x_dtype == B200MOE_F16 || a->x_dtype == B200MOE_BF16,
+                 "int8_linear: input must be int8, float32, float16 or bfloat16");
+  B200_CHECK_ARG(a->x_dtype != B200MOE_I8 || a->x_stride % 16 == 0, "int8_linear: int8 rows must be multiples of 16 values apart");
   B200_CHECK_ARG(a->d_dtype == B200MOE_BF16 || a->d_dtype == B200MOE_F16 || a->d_dtype == B200MOE_F32,
                  "int8_linear: out must be float32, float16 or bfloat16");
   B200_CHECK_ARG(a->bias == nullptr || a->bias_dtype == B200MOE_BF16 || a->bias_dtype == B200MOE_F16,
                  "int8_linear: bias must be float16 or bfloat16");
   if (a->rows == 0 || a->n == 0) return B200MOE_OK;
-  B200_CHECK_ARG(a->x && a->x_scale && a->w && a->w_scale && a->d, "int8_linear: null pointer");
-  B200_CHECK_ARG(aligned16(a->x) && aligned16(a->w), "int8_linear: input and weight must be 16-byte aligned");
+  const bool codes = a->x_dtype == B200MOE_I8;
+  B200_CHECK_ARG(a->x && (a->x_scale || !codes) && a->w && a->w_scale && a->d, "int8_linear: null pointer");
+  B200_CHECK_ARG((aligned16(a->x) || !codes) && aligned16(a->w), "int8_linear: input and weight must be 16-byte aligned");
   DenseJob j = {};
+  j.x_dtype = B200MOE_I8;
+  const int size = dtype_bytes(a->x_dtype);
+  if (!codes && dense_rows_quantises(a->rows, a->k) && aligned16(a->x) && a->x_stride * size % 16 == 0) {
+    j.x_dtype = a->x_dtype;
+  } else if (!codes) {
+    if (a->workspace == nullptr || a->workspace_bytes < b200moe_int8_linear_workspace_bytes(a->rows, a->k) || !aligned16(a->workspace))
+      return fail(B200MOE_E_WORKSPACE, "int8_linear: workspace missing, too small or not 16-byte aligned");
+    int8_t* const q = (int8_t*)a->workspace;
+    float* const s = (float*)(q + a->rows * a->k);
+    if (int rc = b200moe_quant_int8_rows(a->x, a->x_dtype, a->x_stride, q, a->k, s, a->rows, a->k, 0, nullptr, 0, stream)) return rc;
+    b200moe_int8_linear_args b = *a;
+    b.x = q; b.x_scale = s; b.x_dtype = B200MOE_I8; b.x_stride = a->k;
+    return b200moe_int8_linear(&b, stream);
+  }
   j.x = a->x; j.w = a->w; j.x_scale = a->x_scale; j.w_scale = a->w_scale; j.bias = a->bias; j.d = a->d; j.status = a->status;
   j.m = a->rows; j.x_stride = a->x_stride; j.w_stride = a->k; j.d_stride = a->d_stride; j.n = a->n; j.k = a->k; j.experts = 1;
   j.type = kDenseI8; j.d_dtype = a->d_dtype; j.bias_f16 = a->bias_dtype == B200MOE_F16; j.early = a->rows <= kEarlyLaunchRows;
@@ -182,7 +204,7 @@ int grouped_gemm_i8(const b200moe_gemm_args* a, cudaStream_t st) {
   j.m = a->m; j.x_stride = a->k; j.w_stride = a->k; j.n = a->n; j.k = a->k; j.experts = a->num_experts;
   j.d_stride = gated ? a->n / 2 : a->n;
   j.rows_hint = (int)(a->rows_hint > 0 && a->rows_hint < a->m ? a->rows_hint : 0);
-  j.max_ctas = a->max_ctas; j.type = kDenseI8; j.gated = gated; j.d_dtype = a->d_dtype;
+  j.max_ctas = a->max_ctas; j.type = kDenseI8; j.x_dtype = B200MOE_I8; j.gated = gated; j.d_dtype = a->d_dtype;
   j.bias_f16 = (f32 ? a->mid_dtype : a->d_dtype) == B200MOE_F16;
   j.clamp = gated ? a->clamp_limit : 0.f;
   j.early = a->m <= kEarlyLaunchRows;

@@ -4,6 +4,7 @@
 
 #include "common.cuh"
 #include "gemm_tc_common.cuh"
+#include "quant_int8.cuh"
 
 namespace b200moe {
 
@@ -26,6 +27,7 @@ struct DenseJob {
   int rows_hint;                  // rows expected in use, or 0
   int max_ctas;
   DenseType type;
+  b200moe_dtype x_dtype;          // int8 weights: I8, or the type of rows that the kernel quantises itself (x_scale NULL; few values)
   bool gated;
   b200moe_dtype d_dtype;          // F32, BF16, F16
   bool bias_f16;
@@ -34,13 +36,19 @@ struct DenseJob {
 };
 
 int dense_rows(const DenseJob& j, cudaStream_t st);      // dense_rows.cu
+// Whether dense_rows takes rows of 16 or 32 bits and int8 weights, every block making the codes for itself: up to so many values
+// that takes less time than a kernel of its own.
+constexpr int kQuantValues = 16384;
+bool dense_rows_quantises(int64_t rows, int k);
 int dense_tc(const DenseJob& j, cudaStream_t st);        // dense_tc.cu
 
-// Rows an expert from which the kernel for many rows takes a call.
-constexpr int kDenseFewRows = 16;
+// Rows (an expert) up to which the kernel for a few rows takes a call.  By expert, layer calls, that kernel / the one for many, us:
+// 8 experts of 4096 x 14336, 4 rows 246 / 257, 15 rows 365 / 265; 128 of 2048 x 768, 1 row 86.8 / 88.6, 8 rows 172 / 147; 8 of
+// 2048 x 1408, 4 rows 28.4 / 36.3, 16 rows 39.8 / 36.8.
+constexpr int kDenseFewRows = 16, kGroupedFewRows = 5;
 inline int dense(const DenseJob& j, cudaStream_t st) {
   const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m;
-  return (rows + j.experts - 1) / j.experts <= kDenseFewRows ? dense_rows(j, st) : dense_tc(j, st);
+  return (rows + j.experts - 1) / j.experts <= (j.rows_per_expert != nullptr ? kGroupedFewRows : kDenseFewRows) ? dense_rows(j, st) : dense_tc(j, st);
 }
 
 namespace {

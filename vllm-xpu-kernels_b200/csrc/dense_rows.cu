@@ -1,14 +1,20 @@
-// Products of a few rows with int8 weights, or with the 16-bit weights of a gated block: every weight is read once, straight into
-// the registers of the matrix instruction.
+// Products of a few rows with int8 weights, or with the 16-bit weights of a gated block: every weight is read once.
 //
 //   int8:   D[m, n] = (sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n] (+ bias[n])      sums in int32, exact
 //   gated:  D[m, i] = silu(g) * u, g and u the products with rows i and I + i of W          sums in fp32
 //
-// The order of k inside a sum is free as long as both operands share it, so a lane loads 16 consecutive bytes of a weight row
-// (and of a token's) and takes them for the four words that mma.sync wants of it, two instructions for 64 bytes of a row: no shared
-// memory, no shuffle and no repacking stand between the load and the product.  A block owns 32 features (16 gates and their
-// 16 ups) and up to 16 tokens; its eight warps share the row's bytes out among themselves, 128 at a time, and add their sums up in shared
-// memory.  What bounds it is the weights' way from HBM.
+// The order of k inside a sum is free as long as both operands share it, so a lane takes 16 consecutive bytes of a weight row
+// (and of a token's) for the four words that mma.sync wants of it, two instructions for 64 bytes of a row, and no shuffle or
+// repacking stands between the load and the product.  A block owns 16 weight rows (gated: 8 gates and their 8 ups) and up to 16
+// tokens at a time; a team of its eight warps (all of them for few tiles or long rows, one or two for many short ones) shares the
+// rows' bytes out, 128 at a time (a unit), and adds its sums up in shared memory.
+//
+// What bounds it is the weights' way from HBM, so what counts is bytes in flight: every lane has its own slots in shared memory, which
+// cp.async fills several units ahead, across tiles, and which only this lane reads again, so that nothing but its own wait stands
+// between the two.
+//
+// Up to eight tokens of one set of weights lie in shared memory as a whole (a panel): with every block asking L2 for the same lines
+// of one token at the same time, unit after unit, a token of 7168 x 2048 took longer than sixteen (18.6 and 13.9 us).
 #include "dense.cuh"
 
 namespace b200moe {
@@ -16,13 +22,18 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kUnit = 128;      // bytes of a row that a warp takes at a time
+constexpr int kPanelBytes = 32768;   // of a panel: two blocks stay on an SM
 
 struct RowsParams {
   DenseJob j;
   int64_t x_pitch, w_pitch;     // bytes from row to row
   int k_bytes;                  // bytes of a row
-  int f_tiles;                  // tiles of 32 weight rows (gated: 16 and 16)
-  int t_tiles;                  // dense: tiles of tokens
+  int units;                    // of a row
+  int f_tiles;                  // tiles of 16 weight rows (gated: 8 and 8)
+  int t_tiles;                  // one set of weights: tiles of tokens
+  int team;                     // warps of a tile: 1, 2, 4 or 8
+  int panel_pitch;              // bytes from row to row of a panel
+  bool near;                    // tokens go through L1
 };
 
 template <int kType>
@@ -47,169 +58,324 @@ __device__ __forceinline__ void mma(uint32_t (&d)[4], uint32_t a0, uint32_t a1, 
     for (int i = 0; i < 4; ++i) d[i] = __float_as_uint(f[i]);
   }
 }
-// Weights: read once, and constant while the kernel runs.
-__device__ __forceinline__ uint4 ld_weights(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+__device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, bool there) {   // (zeros where there is nothing)
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+// ... of a token, which the SM's other tiles read as well
+__device__ __forceinline__ void copy16_token(uint32_t to, const uint8_t* from, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
+
+// The codes of up to eight rows, by the whole block: 8, 4, 2 or 1 warps a row.
+__device__ __forceinline__ void quantise_rows(const RowsParams& p, uint8_t* codes, float* scales, float* part) {
+  const DenseJob& j = p.j;
+  const int m = (int)j.m, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int each = m == 1 ? 8 : m == 2 ? 4 : m <= 4 ? 2 : 1, row = warp / each, threads = 32 * each, t = (warp % each) * 32 + lane;
+  const int size = j.x_dtype == B200MOE_F32 ? 4 : 2, per = 16 / size, pieces = j.k / per;
+  const uint8_t* x = reinterpret_cast<const uint8_t*>(j.x) + (int64_t)min(row, m - 1) * j.x_stride * size;
+  auto values = [&](int c, float (&v)[8]) {
+    const vec16 a = ld16(x + (int64_t)c * 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (j.x_dtype == B200MOE_F32) v[i] = i < 4 ? __uint_as_float(a.w[i & 3]) : 0.f;
+      else if (j.x_dtype == B200MOE_BF16) v[i] = __uint_as_float(i & 1 ? a.w[i / 2] & 0xffff0000u : a.w[i / 2] << 16);
+      else v[i] = __half2float(reinterpret_cast<const __half*>(&a)[i]);
+    }
+  };
+  float amax = 0.f;
+#pragma unroll 4
+  for (int c = t; c < pieces; c += threads) {
+    float v[8];
+    values(c, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = max_nan(amax, fabsf(v[i]));
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  if (lane == 0) part[warp] = amax;
+  __syncthreads();
+  for (int i = 0; i < each; ++i) amax = max_nan(amax, part[warp / each * each + i]);
+  const Int8Scale s(amax);
+  if (row < m) {
+    if (t == 0) scales[row] = s.scale;
+#pragma unroll 4
+    for (int c = t; c < pieces; c += threads) {
+      float v[8];
+      values(c, v);
+      uint32_t w[2];
+      s.codes<2>(v, w);
+      if (per == 8) *reinterpret_cast<uint2*>(codes + row * p.panel_pitch + c * 8) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(codes + row * p.panel_pitch + c * 4) = w[0];
+    }
+  }
+  __syncthreads();
 }
 
-// NT: tiles of 8 tokens.
-template <int kType, bool kGated, int NT>
+// Up to eight rows as they are, zeros up to a whole unit.
+__device__ __forceinline__ void copy_rows(const RowsParams& p, uint8_t* panel) {
+  const uint8_t* x = reinterpret_cast<const uint8_t*>(p.j.x);
+  const int pieces = p.units * (kUnit / 16), total = (int)p.j.m * pieces;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < total; i += 32 * kWarps) {
+    const int row = i / pieces, c = (i - row * pieces) * 16;
+    const vec16 v = c < p.k_bytes ? ld16(x + row * p.x_pitch + c) : vec16{{0, 0, 0, 0}};
+    *reinterpret_cast<vec16*>(panel + row * p.panel_pitch + c) = v;
+  }
+  __syncthreads();
+}
+
+template <int NT>
+struct alignas(128) Fixed {
+  uint32_t sums[2][kWarps][NT][4][32];
+  float x_scales[8], part[kWarps];      // of rows that are quantised on the way
+};
+
+// Where tokens come from: beside the weights through the lanes' slots, or from a panel of the rows or of their codes.
+enum Tokens { kRing, kPanel, kCodes };
+
+// NT: tiles of 8 tokens.  kAhead: units in flight.
+template <int kType, bool kGated, int NT, int kAhead, int kTokens>
 __global__ void __launch_bounds__(32 * kWarps, 2)
-dense_rows_kernel(const RowsParams p) {
+dense_rows_kernel(const __grid_constant__ RowsParams p) {
   constexpr int BT = 8 * NT;
-  __shared__ uint32_t sums[kWarps][2][NT][4][32];
-  extern __shared__ __align__(16) uint8_t walk_mem[];
+  constexpr int kSlots = 4 + (kTokens == kRing ? 2 * NT : 0);      // 16-byte pieces of a unit that a lane has
+  extern __shared__ __align__(128) uint8_t dyn[];
+  Fixed<NT>& fixed = *reinterpret_cast<Fixed<NT>*>(dyn);
+  auto& sums = fixed.sums;
   const DenseJob& j = p.j;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const bool grouped = j.rows_per_expert != nullptr;
-  pdl_trigger();
-  pdl_wait();
-  TileWalk walk = {};
-  int total = p.f_tiles * p.t_tiles;
-  if (grouped) {
-    if (warp == 0) build_tile_walk<BT>(j.rows_per_expert, j.experts, p.f_tiles, walk_mem);
-    __syncthreads();
-    walk = tile_walk_at(walk_mem, j.experts);
-    total = walk.total;
-  }
-  const int half = kGated ? j.n >> 1 : 16;        // from the tile's first 16 weight rows to its other 16
+  const int team = warp / p.team, in_team = warp - team * p.team, teams = kWarps / p.team;   // (p.team divides kWarps)
+  const bool grouped = kTokens == kRing && j.rows_per_expert != nullptr;
+  uint8_t* const behind = dyn + sizeof(Fixed<NT>) + kWarps * kAhead * kSlots * 512;      // the panel, or the tile walk
+  const uint32_t ring = ptx::smem_u32(dyn) + sizeof(Fixed<NT>) + warp * kAhead * kSlots * 512 + lane * 16;
+  const uint32_t panel = ptx::smem_u32(behind) + min(g, (int)min(j.m, (int64_t)8) - 1) * p.panel_pitch + 16 * q;
+  const int half = kGated ? j.n >> 1 : 8;         // from the tile's first 8 weight rows to its other 8
   const int limit = kGated ? j.n >> 1 : j.n;      // features
   const uint8_t *w = reinterpret_cast<const uint8_t*>(j.w), *x = reinterpret_cast<const uint8_t*>(j.x);
-  int cursor = 0;
-  for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
-    TileInfo ti;
+  TileWalk walk = {};
+  int total = p.f_tiles * p.t_tiles;
+  const int first_tile = team * gridDim.x + blockIdx.x, step = teams * gridDim.x;   // (neighbouring blocks: neighbouring tiles)
+  auto locate = [&](int tile, int& cursor, TileInfo& ti) {
     if (grouped) {
       locate_tile<BT>(walk, tile, cursor, ti);
-    } else {
-      ti.e = 0;
-      ti.n_tile = p.t_tiles == 1 ? tile : tile / p.t_tiles;
-      ti.row0 = (tile - ti.n_tile * p.t_tiles) * BT;
-      ti.valid = (int)(j.m - ti.row0 < BT ? j.m - ti.row0 : BT);
+      return;
     }
-    const int f0 = ti.n_tile * (kGated ? 16 : 32);
-    // this lane's weight rows: g and g + 8 of both sixteens; rows past the end read the last one, and are not stored
-    const uint8_t* wr[4];
+    ti.e = 0;
+    ti.n_tile = p.t_tiles == 1 ? tile : tile / p.t_tiles;
+    ti.row0 = (tile - ti.n_tile * p.t_tiles) * BT;
+    ti.valid = (int)(j.m - ti.row0 < BT ? j.m - ti.row0 : BT);
+  };
+  pdl_trigger();
+  if (grouped) {
+    pdl_wait();
+    if (warp == 0) build_tile_walk<BT>(j.rows_per_expert, j.experts, p.f_tiles, behind);
+    __syncthreads();
+    walk = tile_walk_at(behind, j.experts);
+    total = walk.total;
+  }
+
+  // where the copies are: tile, unit and addresses of this lane's rows in it
+  int next_tile = first_tile, next_unit = in_team, next_cursor = 0;
+  const uint8_t *wr[2], *xr[NT];
+  auto at_tile = [&]() {
+    if (next_tile >= total) return;
+    TileInfo ti;
+    locate(next_tile, next_cursor, ti);
+    // (rows past the end read the last one, and are not stored)
+    const int f = ti.n_tile * (kGated ? 8 : 16) + g;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int f = f0 + g + 8 * (i & 1);
-      const int row = kGated ? min(f, limit - 1) + (i >> 1) * half : min(f + (i >> 1) * half, limit - 1);
-      wr[i] = w + ((int64_t)ti.e * j.n + row) * p.w_pitch;
+    for (int i = 0; i < 2; ++i) {
+      const int row = kGated ? min(f, limit - 1) + i * half : min(f + i * half, limit - 1);
+      wr[i] = w + ((int64_t)ti.e * j.n + row) * p.w_pitch + 16 * q;
     }
-    const uint8_t* xr[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-      xr[i] = x + min((int64_t)ti.row0 + min(g + 8 * i, ti.valid - 1), j.m - 1) * p.x_pitch;
-    uint32_t acc[2][NT][4] = {};
-    uint4 a[2][4];
-    auto load = [&](int at) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int k = at + 64 * s + 16 * q;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[s][i] = k < p.k_bytes ? ld_weights(wr[i] + k) : make_uint4(0, 0, 0, 0);
-      }
-    };
-    int at = warp * kUnit;
-    if (at < p.k_bytes) load(at);
-    for (; at < p.k_bytes; at += kWarps * kUnit) {
-      uint4 b[2][NT], c[2][4];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int k = at + 64 * s + 16 * q;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) b[s][i] = k < p.k_bytes ? *reinterpret_cast<const uint4*>(xr[i] + k) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[s][i] = a[s][i];
-      }
-      if (at + kWarps * kUnit < p.k_bytes) load(at + kWarps * kUnit);
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            mma<kType>(acc[h][i], c[s][2 * h].x, c[s][2 * h + 1].x, c[s][2 * h].y, c[s][2 * h + 1].y, b[s][i].x, b[s][i].y);
-            mma<kType>(acc[h][i], c[s][2 * h].z, c[s][2 * h + 1].z, c[s][2 * h].w, c[s][2 * h + 1].w, b[s][i].z, b[s][i].w);
-          }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
+    if (kTokens == kRing) {
 #pragma unroll
       for (int i = 0; i < NT; ++i)
+        xr[i] = x + min((int64_t)ti.row0 + min(g + 8 * i, ti.valid - 1), j.m - 1) * p.x_pitch + 16 * q;
+    }
+  };
+  auto copy = [&](uint32_t slot) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sums[warp][h][i][r][lane] = acc[h][i][r];
-    __syncthreads();
-    auto sum = [&](int h, int f, int t) {   // of feature f (of 16) and token t
-      const int r = (f >> 3) * 2 + (t & 1), l = (f & 7) * 4 + ((t & 7) >> 1);
-      if (kType == kDenseI8) {
-        int v = 0;
+    for (int s = 0; s < 2; ++s) {
+      const int k = next_unit * kUnit + 64 * s;
+      const bool there = k + 16 * q < p.k_bytes;
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) v += (int)sums[i][h][t >> 3][r][l];
-        return (float)v;
-      }
-      float v = 0.f;
+      for (int i = 0; i < 2; ++i) copy16(slot + (2 * s + i) * 512, wr[i] + k, there);
+      if (kTokens == kRing) {
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) v += __uint_as_float(sums[i][h][t >> 3][r][l]);
-      return v;
-    };
-    auto value = [&](int h, int f, int t) {   // with scales and bias
-      float v = sum(h, f, t);
-      const int64_t at = (int64_t)ti.e * j.n + f0 + f + h * half;
-      if (kType == kDenseI8) v = v * j.x_scale[ti.row0 + t] * j.w_scale[at];
-      if (j.bias != nullptr) v += load_bias(j.bias, j.bias_f16, at);
-      return v;
-    };
-    for (int i = threadIdx.x; i < (kGated ? 16 : 32) * BT; i += 32 * kWarps) {
-      const int f = i & 15, h = kGated ? 0 : (i >> 4) & 1, t = i >> (kGated ? 4 : 5);
-      const int64_t row = (int64_t)ti.row0 + t;
-      if (t >= ti.valid || row >= j.m || f0 + f + (kGated ? 0 : h * half) >= limit) continue;
-      if (kGated) {
-        const float gate = value(0, f, t), up = value(1, f, t);
-        if (j.pre != nullptr) {
-          j.pre[row * j.n + f0 + f] = gate;
-          j.pre[row * j.n + half + f0 + f] = up;
+        for (int i = 0; i < NT; ++i) {
+          if (p.near) copy16_token(slot + (4 + NT * s + i) * 512, xr[i] + k, there);
+          else copy16(slot + (4 + NT * s + i) * 512, xr[i] + k, there);
         }
-        store_as(j.d, j.d_dtype, row * j.d_stride + f0 + f, gated_product(gate, up, j.clamp));
-      } else {
-        store_as(j.d, j.d_dtype, row * j.d_stride + f0 + f + h * half, value(h, f, t));
       }
     }
-    if (tile + (int)gridDim.x < total) __syncthreads();   // the sums are read before they are written again
+    next_unit += p.team;
+    if (next_unit < p.units) return;
+    next_unit = in_team;
+    next_tile += step;
+    at_tile();
+  };
+  const bool mine = in_team < p.units;               // (a row of fewer units than warps)
+  at_tile();
+  if (!grouped) {
+    // The first weights on their way to L2 while the kernel before this one ends.  (Only there: that kernel may be the one that
+    // writes them, and L2 is where its writes are seen.)
+    if (mine && next_tile < total && q == 0) {
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const int k = (in_team + a * p.team) * kUnit;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (k < p.k_bytes) asm volatile("prefetch.global.L2 [%0];" ::"l"(wr[i] + k));
+      }
+    }
+    pdl_wait();
+  }
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) {
+    if (mine && next_tile < total) copy(ring + a * kSlots * 512);
+    commit();
+  }
+  if (kTokens == kCodes) quantise_rows(p, behind, fixed.x_scales, fixed.part);
+  if (kTokens == kPanel) copy_rows(p, behind);
+
+  // the outputs of this thread: one feature of the 8 (and of which 8), every some tokens
+  const int tt = in_team * 32 + lane, f = tt & 7, h = kGated ? 0 : (tt >> 3) & 1;
+  const int t0 = tt >> (kGated ? 3 : 4), t_step = 2 * p.team * (kGated ? 2 : 1);
+  int slot = 0, cursor = 0, parity = 0;
+  for (int tile = first_tile; tile < total; tile += step, parity ^= 1) {
+    TileInfo ti;
+    locate(tile, cursor, ti);
+    // scales and biases are on their way while the weights are
+    const int feat = ti.n_tile * (kGated ? 8 : 16) + f + h * half;
+    const int64_t at = (int64_t)ti.e * j.n + feat;
+    float ws[2] = {1.f, 1.f}, bias[2] = {0.f, 0.f};
+    if (feat < limit) {
+#pragma unroll
+      for (int i = 0; i < (kGated ? 2 : 1); ++i) {
+        if (kType == kDenseI8) ws[i] = j.w_scale[at + i * half];
+        if (j.bias != nullptr) bias[i] = load_bias(j.bias, j.bias_f16, at + i * half);
+      }
+    }
+    uint32_t acc[NT][4] = {};
+    for (int unit = in_team; unit < p.units; unit += p.team) {
+      const uint32_t from = ring + slot * kSlots * 512;
+      wait_but<kAhead - 1>();
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const uint4 a = ptx::lds128(from + 2 * s * 512), b = ptx::lds128(from + (2 * s + 1) * 512);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const uint4 t = kTokens == kRing ? ptx::lds128(from + (4 + NT * s + i) * 512) : ptx::lds128(panel + unit * kUnit + 64 * s);
+          mma<kType>(acc[i], a.x, b.x, a.y, b.y, t.x, t.y);
+          mma<kType>(acc[i], a.z, b.z, a.w, b.w, t.z, t.w);
+        }
+      }
+      // (the slot has been read: the products above took its values)
+      if (next_tile < total) copy(from);
+      commit();
+      if (++slot == kAhead) slot = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sums[parity][warp][i][r][lane] = acc[i][r];
+    // (one barrier a tile: the sums of the tile before are in the other half)
+    if (p.team == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * p.team) : "memory");
+    if (feat >= limit) continue;
+    for (int t = t0; t < ti.valid; t += t_step) {
+      const int64_t row = (int64_t)ti.row0 + t;
+      if (row >= j.m) break;
+      const float xs = kType != kDenseI8 ? 1.f : kTokens == kCodes ? fixed.x_scales[t] : j.x_scale[row];
+      auto value = [&](int i) {
+        const int r = 2 * (h + i) + (t & 1), l = f * 4 + ((t & 7) >> 1);
+        if (kType == kDenseI8) {
+          int sum = 0;
+          for (int n = 0; n < p.team; ++n) sum += (int)sums[parity][team * p.team + n][t >> 3][r][l];
+          return (float)sum * xs * ws[i] + bias[i];
+        }
+        float v = 0.f;
+        for (int n = 0; n < p.team; ++n) v += __uint_as_float(sums[parity][team * p.team + n][t >> 3][r][l]);
+        return v + bias[i];
+      };
+      float v = value(0);
+      if (kGated) {
+        const float up = value(1);
+        if (j.pre != nullptr) {
+          j.pre[row * j.n + feat] = v;
+          j.pre[row * j.n + half + feat] = up;
+        }
+        v = gated_product(v, up, j.clamp);
+      }
+      store_as(j.d, j.d_dtype, row * j.d_stride + feat, v);
+    }
   }
 }
 
-template <int kType, bool kGated, int NT>
-int launch(const RowsParams& p, cudaStream_t st) {
+template <int kType, bool kGated, int NT, int kAhead, int kTokens>
+int launch(RowsParams& p, cudaStream_t st) {
   constexpr int BT = 8 * NT;
   const DenseJob& j = p.j;
-  const size_t smem = j.rows_per_expert != nullptr ? tile_walk_bytes(j.experts) : 0;
-  const int64_t tiles = ((j.m + BT - 1) / BT + (j.rows_per_expert != nullptr ? std::min<int64_t>(j.m, j.experts) : 0)) * p.f_tiles;
-  int64_t grid = (j.max_ctas > 0 ? std::min(j.max_ctas, sm_count()) : sm_count()) * 2;
-  grid = std::max<int64_t>(1, std::min(grid, tiles));
-  B200_LAUNCHED("dense_rows_kernel", launch_pdl(j.early, dense_rows_kernel<kType, kGated, NT>, dim3((unsigned)grid), dim3(32 * kWarps),
-                                                smem, st, p));
+  auto kern = dense_rows_kernel<kType, kGated, NT, kAhead, kTokens>;
+  static SmemConfig configured;
+  if (int rc = configured.ensure(kern)) return rc;
+  const size_t smem = sizeof(Fixed<NT>) + (size_t)kWarps * kAhead * (4 + (kTokens == kRing ? 2 * NT : 0)) * 512 +
+                      (kTokens != kRing ? (size_t)j.m * p.panel_pitch : j.rows_per_expert != nullptr ? tile_walk_bytes(j.experts) : 0);
+  const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m;
+  const int64_t tiles = j.rows_per_expert != nullptr ? (rows / BT + std::min<int64_t>(rows, j.experts)) * p.f_tiles
+                                                     : (int64_t)p.t_tiles * p.f_tiles;
+  const int64_t blocks = (j.max_ctas > 0 ? std::min(j.max_ctas, sm_count()) : sm_count()) * 2;
+  // Warps of a team: rounds of tiles times the units of a warp, and as much as kTileCost units for what a tile costs besides.
+  constexpr int kTileCost = 4;
+  int64_t best = -1;
+  for (int team = kWarps; team >= 1; team /= 2) {
+    const int64_t teams = blocks * (kWarps / team), rounds = (tiles + teams - 1) / teams;
+    const int64_t cost = rounds * ((p.units + team - 1) / team + kTileCost);
+    if (best < 0 || cost < best) { best = cost; p.team = team; }
+  }
+  const int64_t grid = std::max<int64_t>(1, std::min(blocks, (tiles * p.team + kWarps - 1) / kWarps));
+  B200_LAUNCHED("dense_rows_kernel", launch_pdl(j.early, kern, dim3((unsigned)grid), dim3(32 * kWarps), smem, st, p));
   return B200MOE_OK;
 }
 template <int kType, bool kGated>
 int launch_tokens(RowsParams& p, cudaStream_t st) {
-  const int64_t rows = p.j.rows_hint > 0 && p.j.rows_hint < p.j.m ? p.j.rows_hint : p.j.m;
-  const bool eight = (rows + p.j.experts - 1) / p.j.experts <= (p.j.rows_per_expert != nullptr ? 4 : 8);
-  p.t_tiles = (int)((p.j.m + (eight ? 7 : 15)) / (eight ? 8 : 16));
-  return eight ? launch<kType, kGated, 1>(p, st) : launch<kType, kGated, 2>(p, st);
+  const DenseJob& j = p.j;
+  const bool one_set = j.rows_per_expert == nullptr;
+  if (one_set && j.m <= 8 && j.m * p.panel_pitch <= kPanelBytes) {
+    p.t_tiles = 1;
+    return launch<kType, kGated, 1, 4, kPanel>(p, st);
+  }
+  const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m;
+  const bool eight = (rows + j.experts - 1) / j.experts <= (one_set ? 8 : 4);
+  p.t_tiles = (int)((j.m + (eight ? 7 : 15)) / (eight ? 8 : 16));
+  // Tokens that L1 holds are asked of L2 once an SM: one token of two experts of 4096 x 28672 102.7 us without, 45.3 with L1, 15 tokens
+  // each of eight 288 and 216; 16 x 4096 x 7168 (115 KB of tokens) 11.9 and 13.2.
+  p.near = std::min<int64_t>((rows + j.experts - 1) / j.experts, 16) * p.k_bytes <= 65536;
+  return eight ? launch<kType, kGated, 1, 4, kRing>(p, st) : launch<kType, kGated, 2, 3, kRing>(p, st);
 }
 
 }  // namespace
+
+bool dense_rows_quantises(int64_t rows, int k) { return rows <= 8 && rows * k <= kQuantValues; }
 
 int dense_rows(const DenseJob& j, cudaStream_t st) {
   RowsParams p = {};
   p.j = j;
   const int size = j.type == kDenseI8 ? 1 : 2;
   p.k_bytes = j.k * size;
+  p.units = (p.k_bytes + kUnit - 1) / kUnit;
   p.x_pitch = j.x_stride * size;
   p.w_pitch = j.w_stride * size;
-  p.f_tiles = j.gated ? (j.n / 2 + 15) / 16 : (j.n + 31) / 32;
+  p.panel_pitch = p.units * kUnit + 64;      // (half of the banks from row to row)
+  p.f_tiles = j.gated ? (j.n / 2 + 7) / 8 : (j.n + 15) / 16;
+  if (j.type == kDenseI8 && j.x_dtype != B200MOE_I8) {
+    p.t_tiles = 1;
+    return launch<kDenseI8, false, 1, 4, kCodes>(p, st);
+  }
   if (j.type == kDenseI8) return j.gated ? launch_tokens<kDenseI8, true>(p, st) : launch_tokens<kDenseI8, false>(p, st);
   if (!j.gated) return fail(B200MOE_E_UNSUPPORTED, "dense_rows: 16-bit products are gated");
   return j.type == kDenseBf16 ? launch_tokens<kDenseBf16, true>(p, st) : launch_tokens<kDenseF16, true>(p, st);

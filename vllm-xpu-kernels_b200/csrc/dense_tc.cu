@@ -5,13 +5,18 @@
 //   D[m, i] = silu(g) * u,  g = X W[i]^T, u = X W[I + i]^T                      kind::i8 or kind::f16 (sums in fp32)
 //   D = A B^T                                                                  kind::f16, either operand also stored by column
 //
-// A cluster of two CTAs shares a tile of 256 rows x 256 weight rows: each brings its 128 rows of X and one half of the
+// A cluster of two CTAs shares a tile of 256 rows x up to 256 weight rows: each brings its 128 rows of X and one half of the
 // weight rows (128 bytes of k at a time, 32 KB a CTA) into its shared memory by TMA, the even CTA issues tcgen05.mma with
 // cta_group::2 for both, and each CTA's tensor memory receives its own rows' 128 x 256 sums, twice, so that the epilogue of a tile
 // overlaps the products of the next.  Rows of X lie on the lanes: a thread of the epilogue owns one row, its
 // scale is one register, and gate and up of a gated tile (128 gates and their 128 ups are the tile's 256 weight rows) meet in one thread.
 //
-//   warp 0: TMA producer;  warp 1: MMA issuer (even CTA), tensor memory;  warps 2-9: epilogue, a half of the columns each four
+// How wide a tile is follows from what the pairs have to do (tile_width below): 256 weight rows share the rows of X best, fewer leave
+// fewer pairs idle in the last round.  Of a tile with few rows only those are brought in (what lies behind them in shared
+// memory makes sums of rows that nobody stores).
+//
+//   warps 0 and 10: TMA producers of W and X;  warp 1: MMA issuer (even CTA), tensor memory;  warps 2-9: epilogue, every second 32
+//   columns each four
 //
 // Every wait on an mbarrier is bounded, as in the grouped GEMMs (gemm_tc.cu).
 #include <algorithm>
@@ -23,11 +28,11 @@ namespace b200moe {
 namespace {
 
 constexpr int kEpi = 8;                           // epilogue warps
-constexpr int kThreads = 64 + 32 * kEpi;
-constexpr int kTile = 256;                        // rows of X, and of W, of a pair's tile
+constexpr int kThreads = 96 + 32 * kEpi;
+constexpr int kTile = 256;                        // rows of X of a pair's tile, and the most rows of W
 constexpr int kOperand = 128 * 128;               // bytes of an operand in a stage: 128 rows of 128 bytes
-constexpr int kStage = 2 * kOperand;
-constexpr int kStages = 6;
+constexpr int kRing = 6 * 2 * kOperand;           // bytes of all stages
+constexpr int kMaxStages = 9;                     // (of tiles of 64 weight rows)
 
 enum Form { kPlain, kScaled, kGated };
 
@@ -43,6 +48,9 @@ struct TcDense {
   int n, experts;
   int num_kb;
   int m_tiles, n_tiles;
+  int width;                // weight rows of a tile: a multiple of 32, gated of 64
+  int stages, stage_bytes, w_bytes;   // w_bytes: of a CTA's weight rows in a stage
+  int x_box;                // rows that a load of X brings
   uint32_t idesc;
   b200moe_dtype d_dtype;
   int bias_f16;
@@ -51,17 +59,18 @@ struct TcDense {
 };
 
 struct Ctrl {
-  uint64_t full[kStages];
-  uint64_t empty[kStages];
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint32_t tmem_base;
   int abort_flag;
   alignas(16) float scale[kEpi][128];    // per epilogue warp: of the weight rows that it has columns of
   alignas(16) float bias[kEpi][128];
+  alignas(16) uint8_t narrow[kEpi][32 * 32];   // 32 bytes of each of a warp's rows, for stores that are not aligned
   alignas(16) uint8_t walk[tile_walk_bytes(kMaxExperts)];
 };
-constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + sizeof(Ctrl);
+constexpr size_t kSmem = 1024 + (size_t)kRing + sizeof(Ctrl);
 static_assert(kSmem <= kMaxSmem, "shared memory");
 
 // Tiles of one set of weights: eight tiles of rows side by side, so that pairs that run at the same time share both operands in L2.
@@ -75,45 +84,76 @@ __device__ __forceinline__ void locate_dense(const TcDense& p, int t, TileInfo& 
   ti.valid = (int)(p.m - ti.row0 < kTile ? p.m - ti.row0 : kTile);
 }
 
-// 32 consecutive values of a row, of which those below `limit` exist.
-__device__ __forceinline__ void store_32(void* d, b200moe_dtype t, int64_t row_at, int col, int limit, const float (&v)[32], int wide) {
-  if (col >= limit) return;
+// A warp's 32 rows x 32 columns, a row a lane, of which the first `rows` rows and the columns below `limit` exist: in pieces of 32 or
+// 16 bytes where they are aligned, else through shared memory, so that lanes that store together are neighbours in a row.
+// (Odd row lengths, value by value from the row's own lane: 1001 x 2011 x 2032 48 us.)
+__device__ __forceinline__ void store_32(void* d, b200moe_dtype t, int64_t row_at, int64_t stride, int rows, int col, int limit,
+                                         const float (&v)[32], int wide, uint32_t narrow) {
+  const int lane = threadIdx.x & 31;
   if (t == B200MOE_F32) {
+    if (wide != 0) {
+      float* to = reinterpret_cast<float*>(d) + row_at + lane * stride + col;
+      if (lane >= rows) return;
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        if (wide == 32) {
+          if (col + i < limit)
+            ptx::stg256(to + i, {__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]),
+                                 __float_as_uint(v[i + 4]), __float_as_uint(v[i + 5]), __float_as_uint(v[i + 6]), __float_as_uint(v[i + 7])});
+        } else {
+#pragma unroll
+          for (int k = i; k < i + 8; k += 4)
+            if (col + k < limit) *reinterpret_cast<float4*>(to + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+        }
+      }
+      return;
+    }
     float* to = reinterpret_cast<float*>(d) + row_at + col;
-    if (wide == 32) {
 #pragma unroll
-      for (int i = 0; i < 32; i += 8)
-        if (col + i < limit)
-          ptx::stg256(to + i, {__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]),
-                               __float_as_uint(v[i + 4]), __float_as_uint(v[i + 5]), __float_as_uint(v[i + 6]), __float_as_uint(v[i + 7])});
-    } else if (wide == 16) {
+    for (int i = 0; i < 32; i += 8) {
+      ptx::sts128(narrow + lane * 32, make_uint4(__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3])));
+      ptx::sts128(narrow + lane * 32 + 16, make_uint4(__float_as_uint(v[i + 4]), __float_as_uint(v[i + 5]), __float_as_uint(v[i + 6]), __float_as_uint(v[i + 7])));
+      __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 32; i += 4)
-        if (col + i < limit) *reinterpret_cast<float4*>(to + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (col + i < limit) to[i] = v[i];
+      for (int n = 0; n < 8; ++n) {
+        const int r = 4 * n + (lane >> 3), c = i + (lane & 7);
+        if (r < rows && col + c < limit) to[r * stride + c] = ptx::lds32f(narrow + r * 32 + (lane & 7) * 4);
+      }
+      __syncwarp();
     }
     return;
   }
-  uint16_t* to = reinterpret_cast<uint16_t*>(d) + row_at + col;
   const int f16 = t == B200MOE_F16;
   uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = (uint32_t)bits16(v[2 * i], f16) | (uint32_t)bits16(v[2 * i + 1], f16) << 16;
-  if (wide == 32) {
+  if (wide != 0) {
+    uint16_t* to = reinterpret_cast<uint16_t*>(d) + row_at + lane * stride + col;
+    if (lane >= rows) return;
 #pragma unroll
-    for (int i = 0; i < 16; i += 8)
-      if (col + 2 * i < limit) ptx::stg256(to + 2 * i, {w[i], w[i + 1], w[i + 2], w[i + 3], w[i + 4], w[i + 5], w[i + 6], w[i + 7]});
-  } else if (wide == 16) {
+    for (int i = 0; i < 16; i += 8) {
+      if (wide == 32) {
+        if (col + 2 * i < limit) ptx::stg256(to + 2 * i, {w[i], w[i + 1], w[i + 2], w[i + 3], w[i + 4], w[i + 5], w[i + 6], w[i + 7]});
+      } else {
 #pragma unroll
-    for (int i = 0; i < 16; i += 4)
-      if (col + 2 * i < limit) *reinterpret_cast<uint4*>(to + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-  } else {
+        for (int k = i; k < i + 8; k += 4)
+          if (col + 2 * k < limit) *reinterpret_cast<uint4*>(to + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+      }
+    }
+    return;
+  }
+  uint16_t* to = reinterpret_cast<uint16_t*>(d) + row_at + col;
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (col + i < limit) to[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+  for (int i = 0; i < 16; i += 8) {
+    ptx::sts128(narrow + lane * 32, make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
+    ptx::sts128(narrow + lane * 32 + 16, make_uint4(w[i + 4], w[i + 5], w[i + 6], w[i + 7]));
+    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+      const int r = 2 * n + (lane >> 4), c = 2 * i + (lane & 15);
+      if (r < rows && col + c < limit) to[r * stride + c] = ptx::lds16(narrow + r * 32 + (lane & 15) * 2);
+    }
+    __syncwarp();
   }
 }
 
@@ -125,7 +165,7 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   constexpr bool kScales = kI8 || kForm == kScaled;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + kStages * kStage);
+  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + kRing);
   volatile int* abort_flag = &ctrl->abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t cta = ptx::cluster_ctarank();
@@ -143,7 +183,7 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
     ptx::tmem_alloc_pair(&ctrl->tmem_base, 512);
     ptx::tmem_relinquish_pair();
   } else if (warp == 2 && lane == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kMaxStages; ++s) {
       ptx::mbar_init(&ctrl->full[s], 1);
       ptx::mbar_init(&ctrl->empty[s], 1);
     }
@@ -174,8 +214,11 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
     else locate_dense(p, t, ti);
   };
 
-  if (warp == 0) {
-    // ------------------------------ TMA producer ------------------------------
+  if (warp == 0 || warp == 2 + kEpi) {
+    // ------------------------------ TMA producers -----------------------------
+    // W by the one, X by the other: a load costs its thread some 100 cycles, a K block of a tile with few rows hardly more
+    // in the tensor cores.
+    const bool is_w = warp == 0;
     if (ptx::elect_one()) {
       uint32_t s = 0, ph = 1;
       bool ok = true;
@@ -183,31 +226,43 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       const uint32_t bar0 = ptx::map_to_cta(full0, 0);   // the even CTA's barriers count the bytes of both CTAs
       const uint32_t st0 = ptx::smem_u32(smem);
       uint32_t st = st0;
+      auto first_row = [&](const TileInfo& ti) {   // of W, of this CTA
+        return kForm == kGated ? (cta == 0 ? 0 : half) + ti.n_tile * (p.width >> 1) : ti.n_tile * p.width + (int)cta * (p.width >> 1);
+      };
       for (int t = walker; t < total && ok; t += walkers) {
         TileInfo ti;
         locate(t, ti);
         // rows past the end are filled with zeros
         const int row = ti.row0 + (int)cta * 128;
-        const int n0 = kForm == kGated ? (cta == 0 ? 0 : half) + ti.n_tile * 128 : (ti.n_tile * 2 + (int)cta) * 128;
+        const int n0 = first_row(ti);
+        // loads of X in either CTA: as many as the tile's rows take
+        auto boxes = [&](int c) {
+          const int rows = min(max(ti.valid - 128 * c, 0), 128);
+          return kXMn ? 2 : (rows + p.x_box - 1) / p.x_box;
+        };
+        const int mine = boxes((int)cta);
+        const uint32_t box_bytes = kXMn ? kOperand / 2 : p.x_box * 128;
+        const uint32_t tx = 2 * p.w_bytes + (boxes(0) + boxes(1)) * box_bytes;
         for (int kb = 0; kb < p.num_kb; ++kb) {
           if (!ptx::paced::mbar_wait_s(empty0 + 8 * s, ph, abort_flag)) { ok = false; break; }
-          if (cta == 0) ptx::mbar_expect_tx_s(full0 + 8 * s, 2 * kStage);
+          if (is_w && cta == 0) ptx::mbar_expect_tx_s(full0 + 8 * s, tx);
           const uint32_t bar = bar0 + 8 * s;
           const int k0 = kb * kPerKb;
-          if (kXMn) {
-            ptx::tma_load_2d_pair(st, &tmap_x, bar, row, k0);
-            ptx::tma_load_2d_pair(st + kOperand / 2, &tmap_x, bar, row + 64, k0);
-          } else {
-            ptx::tma_load_2d_pair(st, &tmap_x, bar, k0, row);
-          }
-          if (kWMn) {
+          if (!is_w) {
+            if (kXMn) {
+              ptx::tma_load_2d_pair(st, &tmap_x, bar, row, k0);
+              ptx::tma_load_2d_pair(st + kOperand / 2, &tmap_x, bar, row + 64, k0);
+            } else {
+              for (int b = 0; b < mine; ++b) ptx::tma_load_2d_pair(st + b * box_bytes, &tmap_x, bar, k0, row + b * p.x_box);
+            }
+          } else if (kWMn) {
             ptx::tma_load_3d_pair(st + kOperand, &tmap_w, bar, n0, k0, ti.e);
-            ptx::tma_load_3d_pair(st + kOperand + kOperand / 2, &tmap_w, bar, n0 + 64, k0, ti.e);
+            if (p.w_bytes > kOperand / 2) ptx::tma_load_3d_pair(st + kOperand + kOperand / 2, &tmap_w, bar, n0 + 64, k0, ti.e);
           } else {
             ptx::tma_load_3d_pair(st + kOperand, &tmap_w, bar, k0, n0, ti.e);
           }
-          st += kStage;
-          if (++s == (uint32_t)kStages) { s = 0; ph ^= 1; st = st0; }
+          st += p.stage_bytes;
+          if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; st = st0; }
         }
       }
     }
@@ -224,6 +279,7 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       const uint64_t xdesc0 = ptx::make_smem_desc(ptx::smem_u32(smem), kXMn ? 8192u : 16u, 1024);
       const uint64_t wdesc0 = ptx::make_smem_desc(ptx::smem_u32(smem) + kOperand, kWMn ? 8192u : 16u, 1024);
       uint64_t xdesc = xdesc0, wdesc = wdesc0;
+      const uint64_t stage16 = p.stage_bytes >> 4;
       for (int t = walker; t < total && ok; t += walkers) {
         const uint32_t a = acc_it & 1;
         if (!ptx::mbar_wait_s(acc_empty0 + 8 * a, ((acc_it >> 1) & 1) ^ 1, abort_flag)) break;
@@ -234,9 +290,9 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
           if (kI8) ptx::umma_i8_pair_block<kXStep, kWStep>(tmem_base + a * kTile, xdesc, wdesc, p.idesc, kb > 0 ? 1u : 0u);
           else ptx::umma_f16_pair_block<kXStep, kWStep>(tmem_base + a * kTile, xdesc, wdesc, p.idesc, kb > 0 ? 1u : 0u);
           ptx::umma_commit_pair(empty0 + 8 * s);
-          xdesc += kStage >> 4;
-          wdesc += kStage >> 4;
-          if (++s == (uint32_t)kStages) { s = 0; ph ^= 1; xdesc = xdesc0; wdesc = wdesc0; }
+          xdesc += stage16;
+          wdesc += stage16;
+          if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; xdesc = xdesc0; wdesc = wdesc0; }
         }
         if (ok) { ptx::umma_commit_pair(acc_full0 + 8 * a); ++acc_it; }
       }
@@ -248,15 +304,16 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
     const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
     const uint32_t acc_empty0 = ptx::map_to_cta(ptx::smem_u32(&ctrl->acc_empty[0]), 0);
     const uint32_t scale0 = ptx::smem_u32(ctrl->scale[warp - 2]), bias0 = ptx::smem_u32(ctrl->bias[warp - 2]);
+    const uint32_t narrow = ptx::smem_u32(ctrl->narrow[warp - 2]);
     uint32_t acc_it = 0;
     for (int t = walker; t < total; t += walkers) {
       TileInfo ti;
       locate(t, ti);
       const uint32_t a = acc_it & 1;
-      const int in_tile = (int)cta * 128 + quarter * 32 + lane;
-      const int64_t row = (int64_t)ti.row0 + in_tile;
-      const bool live = in_tile < ti.valid && row < p.m;
-      const int j0 = ti.n_tile * (kForm == kGated ? 128 : kTile);        // the tile's first feature
+      const int row0 = (int)cta * 128 + quarter * 32;      // this warp's first row in the tile
+      const int64_t first = (int64_t)ti.row0 + row0;
+      const int rows = (int)min((int64_t)min(ti.valid - row0, 32), p.m - first);
+      const int features = kForm == kGated ? p.width >> 1 : p.width, j0 = ti.n_tile * features;
       const int limit = kForm == kGated ? half : p.n;
       float xs = 1.f;
       if (kScales) {
@@ -264,13 +321,14 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int l = lane + 32 * i;
-          const int f = j0 + (kForm == kGated ? side * 64 + (l & 63) : side * 128 + l);
-          const int64_t at = (int64_t)ti.e * p.n + f + (kForm == kGated && l >= 64 ? half : 0);
-          ptx::sts32f(scale0 + 4 * l, f < limit ? p.w_scale[at] : 0.f);
-          ptx::sts32f(bias0 + 4 * l, f < limit && p.bias != nullptr ? load_bias(p.bias, p.bias_f16, at) : 0.f);
+          // (gated: 32 gates, then their ups)
+          const int c = 2 * (kForm == kGated ? i >> 1 : i) + side, f = j0 + 32 * c + lane;
+          const bool there = 32 * c < features && f < limit;
+          const int64_t at = (int64_t)ti.e * p.n + f + (kForm == kGated && (i & 1) ? half : 0);
+          ptx::sts32f(scale0 + 128 * i + 4 * lane, there ? p.w_scale[at] : 0.f);
+          ptx::sts32f(bias0 + 128 * i + 4 * lane, there && p.bias != nullptr ? load_bias(p.bias, p.bias_f16, at) : 0.f);
         }
-        if (live) xs = p.x_scale[row];
+        if (lane < rows) xs = p.x_scale[first + lane];
         __syncwarp();
       }
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(&ctrl->acc_full[a], (acc_it >> 1) & 1, abort_flag))) {
@@ -294,41 +352,29 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
           f[i + 3] = (float)(int)v[i + 3] * xs * ws.w + b.w;
         }
       };
-      if (kForm == kGated) {
+      if (rows > 0) {
 #pragma unroll 1
-        for (int c0 = 0; c0 < 64; c0 += 32) {
-          const int col = side * 64 + c0;
-          uint32_t g[32], u[32];
+        for (int c = side; 32 * c < features && j0 + 32 * c < limit; c += 2) {
+          const int col = 32 * c, l = kForm == kGated ? 32 * (c & ~1) : 16 * (c & ~1);
+          uint32_t g[32], u[kForm == kGated ? 32 : 1];
           __syncwarp();
           ptx::tmem_ld_32x32(acc + col, g);
-          ptx::tmem_ld_32x32(acc + 128 + col, u);
-          ptx::tmem_wait_ld(g, u);
-          if (live) {
-            float gate[32], up[32];
-            scaled(gate, g, c0);
-            scaled(up, u, 64 + c0);
+          if (kForm == kGated) ptx::tmem_ld_32x32(acc + features + col, reinterpret_cast<uint32_t(&)[32]>(u));
+          if (kForm == kGated) ptx::tmem_wait_ld(g, u);
+          else ptx::tmem_wait_ld(g);
+          float f[32];
+          scaled(f, g, l);
+          if (kForm == kGated) {
+            float up[32];
+            scaled(up, reinterpret_cast<uint32_t(&)[32]>(u), l + 32);
             if (p.pre != nullptr) {
-              store_32(p.pre, B200MOE_F32, row * p.n, j0 + col, limit, gate, p.pre_wide);
-              store_32(p.pre + half, B200MOE_F32, row * p.n, j0 + col, limit, up, p.pre_wide);
+              store_32(p.pre, B200MOE_F32, first * p.n, p.n, rows, j0 + col, limit, f, p.pre_wide, narrow);
+              store_32(p.pre + half, B200MOE_F32, first * p.n, p.n, rows, j0 + col, limit, up, p.pre_wide, narrow);
             }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) gate[i] = gated_product(gate[i], up[i], p.clamp);
-            store_32(p.d, p.d_dtype, row * p.d_stride, j0 + col, limit, gate, p.d_wide);
+            for (int i = 0; i < 32; ++i) f[i] = gated_product(f[i], up[i], p.clamp);
           }
-        }
-      } else {
-#pragma unroll 1
-        for (int c0 = 0; c0 < 128; c0 += 32) {
-          const int col = side * 128 + c0;
-          uint32_t v[32];
-          __syncwarp();
-          ptx::tmem_ld_32x32(acc + col, v);
-          ptx::tmem_wait_ld(v);
-          if (live) {
-            float f[32];
-            scaled(f, v, c0);
-            store_32(p.d, p.d_dtype, row * p.d_stride, j0 + col, limit, f, p.d_wide);
-          }
+          store_32(p.d, p.d_dtype, first * p.d_stride, p.d_stride, rows, j0 + col, limit, f, p.d_wide, narrow);
         }
       }
       __syncwarp();
@@ -390,24 +436,49 @@ CUtensorMapDataType map_type(DenseType t) {
   return t == kDenseI8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                        : t == kDenseBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
-// An operand of `rows` rows of k (mn: stored by column, k rows of `rows`), `stride` elements from one stored row to the next.
-int operand_map(CUtensorMap* map, DenseType t, const void* base, int64_t rows, int64_t k, int64_t stride, bool mn, int experts) {
+// An operand of `rows` rows of k (mn: stored by column, k rows of `rows`), `stride` elements from one stored row to the next;
+// a load brings 128 bytes of `box` stored rows.
+int operand_map(CUtensorMap* map, DenseType t, const void* base, int64_t rows, int64_t k, int64_t stride, bool mn, int experts, int box_rows) {
   const int size = t == kDenseI8 ? 1 : 2;
   const int64_t inner = mn ? rows : k, outer = mn ? k : rows;
   const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)std::max(experts, 1)};
   const cuuint64_t strides[2] = {(cuuint64_t)(stride * size), (cuuint64_t)(stride * size * outer)};
-  const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)(mn ? 64 : 128), 1};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
   return encode_map(map, map_type(t), experts > 0 ? 3 : 2, base, dims, strides, box);
+}
+// Weight rows of a tile: what leaves the least for the pair that has most to do.  A K block of a tile costs 2 cycles a weight row in the
+// tensor cores, 64 bytes a weight row and the rows of X on the way into a CTA (some 56 bytes a cycle), and, where no other tile of rows
+// reads the same weights, 64 bytes a weight row from HBM (23 bytes a cycle and SM); a tile costs some 600 cycles besides.
+int tile_width(const TcDense& p, int64_t features, bool gated, int64_t row_tiles, int rows, int pairs) {
+  const int step = gated ? 64 : 32;
+  int best = 0;
+  double least = 0;
+  for (int width = kTile; width >= 64; width -= step) {
+    const int64_t tiles = row_tiles * ((features + (gated ? width / 2 : width) - 1) / (gated ? width / 2 : width));
+    const double load = (128.0 * std::min(rows, 128) + 64.0 * width) / 56, hbm = row_tiles == 1 ? 64.0 * width / 23 : 0;
+    const double cost = (double)((tiles + pairs - 1) / pairs) * (p.num_kb * std::max({2.0 * width, load, hbm}) + 600);
+    if (best == 0 || cost < least) { best = width; least = cost; }
+  }
+  return best;
 }
 int store_width(const void* p, int64_t row_bytes, int64_t cols_bytes) {
   for (int w : {32, 16})
     if (((uintptr_t)p % w) == 0 && row_bytes % w == 0 && cols_bytes % w == 0) return w;
   return 0;
 }
-uint32_t idesc_of(DenseType t, bool x_mn, bool w_mn) {
-  if (t == kDenseI8) return ptx::make_idesc_i8(256, kTile);
+uint32_t idesc_of(DenseType t, bool x_mn, bool w_mn, int width) {
+  if (t == kDenseI8) return ptx::make_idesc_i8(256, width);
   const uint32_t fmt = t == kDenseBf16 ? 1u : 0u;
-  return ptx::make_idesc(fmt, fmt, x_mn ? 1u : 0u, w_mn ? 1u : 0u, 256, kTile);
+  return ptx::make_idesc(fmt, fmt, x_mn ? 1u : 0u, w_mn ? 1u : 0u, 256, width);
+}
+// What follows from a tile's width.
+void set_width(TcDense& p, DenseType t, bool x_mn, bool w_mn, int width, int features, bool gated) {
+  p.width = width;
+  p.n_tiles = (features + (gated ? width / 2 : width) - 1) / (gated ? width / 2 : width);
+  p.w_bytes = w_mn ? (width > 128 ? kOperand : kOperand / 2) : width * 64;
+  p.stage_bytes = kOperand + p.w_bytes;
+  p.stages = std::min(kMaxStages, kRing / p.stage_bytes);
+  p.idesc = idesc_of(t, x_mn, w_mn, width);
 }
 
 }  // namespace
@@ -420,15 +491,24 @@ int dense_tc(const DenseJob& j, cudaStream_t st) {
   const int per_kb = j.type == kDenseI8 ? 128 : 64, n_out = j.gated ? j.n / 2 : j.n;
   p.num_kb = (j.k + per_kb - 1) / per_kb;
   p.m_tiles = (int)((j.m + kTile - 1) / kTile);
-  p.n_tiles = j.gated ? (n_out + 127) / 128 : (n_out + kTile - 1) / kTile;
-  p.idesc = idesc_of(j.type, false, false);
+  const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m, each = (rows + j.experts - 1) / j.experts;
+  const int64_t sets = j.rows_per_expert != nullptr ? std::min<int64_t>(j.experts, rows) : 1;
+  int width = 0;
+  {
+    // (as if every set had the mean number of rows; sets that share a tile of rows with no other read their weights once)
+    const int64_t tiles_each = (each + kTile - 1) / kTile;
+    const int pairs = std::max(1, (j.max_ctas > 0 ? std::min(j.max_ctas, sm_count()) : sm_count()) / 2);
+    width = tile_width(p, n_out * sets, j.gated, tiles_each, (int)std::min<int64_t>(each, kTile), pairs);
+  }
+  set_width(p, j.type, false, false, width, n_out, j.gated);
+  p.x_box = each <= 96 ? 32 : 128;
   p.d_dtype = j.d_dtype; p.bias_f16 = j.bias_f16; p.clamp = j.clamp;
   const int out_size = dtype_bytes(j.d_dtype);
   p.d_wide = store_width(j.d, j.d_stride * out_size, (int64_t)n_out * out_size);
   if (j.pre != nullptr) p.pre_wide = store_width(j.pre, (int64_t)j.n * 4, (int64_t)n_out * 4);
   CUtensorMap tx, tw;
-  if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, false, 0)) return rc;
-  if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, false, j.experts)) return rc;
+  if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, false, 0, p.x_box)) return rc;
+  if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, false, j.experts, width / 2)) return rc;
   const int64_t tiles = (p.m_tiles + (j.rows_per_expert != nullptr ? (int64_t)j.experts : 0)) * p.n_tiles;
   if (j.type == kDenseI8) {
     const int rc = j.gated ? launch<true, kGated, false, false>(tx, tw, p, tiles, j.max_ctas, j.early, st)
@@ -444,13 +524,14 @@ int dense_plain(const PlainJob& j, cudaStream_t st) {
   p.d = j.d; p.status = j.status; p.m = j.m; p.d_stride = j.d_stride; p.n = j.n; p.experts = 1;
   p.num_kb = (int)((j.k + 63) / 64);
   p.m_tiles = (int)((j.m + kTile - 1) / kTile);
-  p.n_tiles = (j.n + kTile - 1) / kTile;
-  p.idesc = idesc_of(j.type, j.x_by_column, true);
+  const int width = tile_width(p, j.n, false, p.m_tiles, (int)std::min<int64_t>(j.m, kTile), std::max(1, sm_count() / 2));
+  set_width(p, j.type, j.x_by_column, true, width, j.n, false);
+  p.x_box = 128;
   p.d_dtype = j.type == kDenseF16 ? B200MOE_F16 : B200MOE_BF16;
   p.d_wide = store_width(j.d, j.d_stride * 2, (int64_t)j.n * 2);
   CUtensorMap tx, tw;
-  if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, j.x_by_column, 0)) return rc;
-  if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, true, 1)) return rc;
+  if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, j.x_by_column, 0, j.x_by_column ? 64 : 128)) return rc;
+  if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, true, 1, 64)) return rc;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
   return j.x_by_column ? launch<false, kPlain, true, true>(tx, tw, p, tiles, 0, j.early, st)
                        : launch<false, kPlain, false, true>(tx, tw, p, tiles, 0, j.early, st);

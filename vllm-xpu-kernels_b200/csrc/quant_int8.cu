@@ -6,11 +6,10 @@
 // in torch operations gives).  A row that holds a NaN or an infinity gets a scale that is not finite and codes that are zero
 // where it holds it: every output of the product that it goes into is a NaN.
 #include "common.cuh"
+#include "quant_int8.cuh"
 
 namespace b200moe {
 namespace {
-
-constexpr float kLeastAmax = 1e-10f;
 
 struct QuantInt8Params {
   const void* in;
@@ -21,18 +20,7 @@ struct QuantInt8Params {
   int hidden, num_segments;
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ uint32_t code_of(float v, float scale) {
-  // (a NaN, from a scale that is not finite, becomes 0; the limits are for quotients of subnormal scales)
-  const float r = rintf(__fdiv_rn(v, scale));
-  return r == r ? (uint32_t)(int)fminf(fmaxf(r, -127.f), 127.f) & 0xffu : 0u;
-}
 __device__ __forceinline__ float gated_value(float g, float u) { return g / (1.0f + expf(-g)) * u; }
-__device__ __forceinline__ float scale_of(float amax) { return __fdiv_rn(max_nan(amax, kLeastAmax), 127.f); }
 
 __device__ __forceinline__ int64_t rows_in_use(const QuantInt8Params& p) {
   if (p.rows_per_segment == nullptr) return p.rows;
@@ -99,21 +87,19 @@ quant_int8_rows_kernel(const QuantInt8Params p, int threads) {
       }
     }
   }
-  const float scale = scale_of(row_max(amax, threads, part));
+  const Int8Scale s(row_max(amax, threads, part));
   if (!live) return;
-  if (t == 0) p.scales[row] = scale;
+  if (t == 0) p.scales[row] = s.scale;
   int8_t* q = p.q + row * p.q_stride;
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
     const int c = t + i * threads;
     if (c < nvec) {
-      const T* x = reinterpret_cast<const T*>(&a[i]);
-      uint32_t w[N / 4];
+      float y[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const uint32_t code = code_of(kGated ? v[kGated ? i * N + k : 0] : to_f32<T>(x[k]), scale);
-        w[k / 4] = (k % 4 ? w[k / 4] : 0u) | code << (8 * (k % 4));
-      }
+      for (int k = 0; k < N; ++k) y[k] = kGated ? v[kGated ? i * N + k : 0] : to_f32<T>(reinterpret_cast<const T*>(&a[i])[k]);
+      uint32_t w[N / 4];
+      s.codes(y, w);
       if (N == 8) *reinterpret_cast<uint2*>(q + (int64_t)c * N) = make_uint2(w[0], w[N / 4 - 1]);
       else *reinterpret_cast<uint32_t*>(q + (int64_t)c * N) = w[0];
     }
@@ -136,9 +122,14 @@ quant_int8_any_kernel(const QuantInt8Params p) {
   };
   float amax = 0.f;
   for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) amax = max_nan(amax, fabsf(value(c)));
-  const float scale = scale_of(row_max(amax, blockDim.x, part));
-  if (threadIdx.x == 0) p.scales[row] = scale;
-  for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) p.q[row * p.q_stride + c] = (int8_t)code_of(value(c), scale);
+  const Int8Scale s(row_max(amax, blockDim.x, part));
+  if (threadIdx.x == 0) p.scales[row] = s.scale;
+  for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) {
+    const float y[4] = {value(c), 0.f, 0.f, 0.f};
+    uint32_t w[1];
+    s.codes(y, w);
+    p.q[row * p.q_stride + c] = (int8_t)w[0];
+  }
 }
 
 template <typename T, bool kGated>

@@ -63,7 +63,7 @@ def _near(got, want, tol, what):
 
 
 SIZES = [(1, 8, 1), (1, 64, 16), (2, 72, 33), (8, 512, 100), (9, 264, 7), (16, 1024, 256), (17, 128, 8), (33, 200, 130), (128, 512, 129),
-         (255, 136, 300), (257, 264, 128), (600, 1032, 520)]
+         (255, 136, 300), (257, 264, 128), (600, 1032, 520), (40, 4096, 130), (300, 2056, 77), (40, 256, 2100), (3000, 64, 40), (270, 512, 1500)]
 
 
 @pytest.mark.parametrize("dtype", [B16, F16])

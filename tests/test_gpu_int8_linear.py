@@ -86,7 +86,8 @@ def _check(out, q, qs, w, ws, bias):
 @pytest.mark.parametrize("out_dtype,bias", [(B16, False), (F16, True), (F32, True)])
 @pytest.mark.parametrize("rows,n,k", [(1, 1, 16), (1, 33, 48), (2, 31, 1040), (8, 100, 128), (9, 64, 2048), (16, 130, 4096),
                                       (17, 1, 16), (17, 255, 144), (40, 257, 128), (129, 300, 272), (256, 256, 512), (257, 513, 1040),
-                                      (700, 1000, 2048)])
+                                      (700, 1000, 2048), (40, 256, 4096), (130, 40, 6160), (300, 521, 7168), (64, 300, 2064),
+                                      (513, 250, 16384), (20, 2000, 4096)])
 def test_product_of_codes(native, rows, n, k, out_dtype, bias):
     gen = torch.Generator().manual_seed(rows + n + k)
     q, qs = ref.weights(rows, k, gen)

@@ -32,7 +32,7 @@ constexpr int kThreads = 96 + 32 * kEpi;
 constexpr int kTile = 256;                        // rows of X of a pair's tile, and the most rows of W
 constexpr int kOperand = 128 * 128;               // bytes of an operand in a stage: 128 rows of 128 bytes
 constexpr int kRing = 6 * 2 * kOperand;           // bytes of all stages
-constexpr int kMaxStages = 9;                     // (of tiles of 64 weight rows)
+constexpr int kMaxStages = 12;
 
 enum Form { kPlain, kScaled, kGated };
 
@@ -49,7 +49,9 @@ struct TcDense {
   int num_kb;
   int m_tiles, n_tiles;
   int width;                // weight rows of a tile: a multiple of 32, gated of 64
-  int stages, stage_bytes, w_bytes;   // w_bytes: of a CTA's weight rows in a stage
+  int half_rows;            // rows of X that a CTA has of a tile: 32, 64 or 128 (in tensor memory they are the first of 128)
+  int stages, blocks;       // of the ring; K blocks of a stage: 1 or 2
+  int block_bytes, x_bytes, w_bytes;   // of a K block, its X and its W
   int x_box;                // rows that a load of X brings
   uint32_t idesc;
   b200moe_dtype d_dtype;
@@ -73,6 +75,8 @@ struct Ctrl {
 constexpr size_t kSmem = 1024 + (size_t)kRing + sizeof(Ctrl);
 static_assert(kSmem <= kMaxSmem, "shared memory");
 
+__device__ __forceinline__ int tile_rows(const TcDense& p) { return 2 * p.half_rows; }
+
 // Tiles of one set of weights: eight tiles of rows side by side, so that pairs that run at the same time share both operands in L2.
 __device__ __forceinline__ void locate_dense(const TcDense& p, int t, TileInfo& ti) {
   const int group = 8 * p.n_tiles, g = t / group, in = t - g * group, first = 8 * g;
@@ -80,89 +84,166 @@ __device__ __forceinline__ void locate_dense(const TcDense& p, int t, TileInfo& 
   ti.e = 0;
   ti.n_tile = in / rows;
   ti.m_tile = first + in - ti.n_tile * rows;
-  ti.row0 = ti.m_tile * kTile;
-  ti.valid = (int)(p.m - ti.row0 < kTile ? p.m - ti.row0 : kTile);
+  ti.row0 = ti.m_tile * tile_rows(p);
+  ti.valid = (int)min((int64_t)tile_rows(p), p.m - ti.row0);
 }
 
-// A warp's 32 rows x 32 columns, a row a lane, of which the first `rows` rows and the columns below `limit` exist: in pieces of 32 or
+// A warp's 32 rows x 16 columns, a row a lane, of which the first `rows` rows and the columns below `limit` exist: in pieces of 32 or
 // 16 bytes where they are aligned, else through shared memory, so that lanes that store together are neighbours in a row.
 // (Odd row lengths, value by value from the row's own lane: 1001 x 2011 x 2032 48 us.)
-__device__ __forceinline__ void store_32(void* d, b200moe_dtype t, int64_t row_at, int64_t stride, int rows, int col, int limit,
-                                         const float (&v)[32], int wide, uint32_t narrow) {
+__device__ __forceinline__ void store_16(void* d, b200moe_dtype t, int64_t row_at, int64_t stride, int rows, int col, int limit,
+                                         const float (&v)[16], int wide, uint32_t narrow) {
   const int lane = threadIdx.x & 31;
-  if (t == B200MOE_F32) {
+  const bool f32 = t == B200MOE_F32;
+  uint8_t* const to = reinterpret_cast<uint8_t*>(d) + (row_at + col) * (f32 ? 4 : 2);
+  const int64_t pitch = stride * (f32 ? 4 : 2);
+  // 32 bytes of every row, of which `left` bytes exist
+  auto piece = [&](uint8_t* at0, const uint32_t (&w)[8], int left) {
     if (wide != 0) {
-      float* to = reinterpret_cast<float*>(d) + row_at + lane * stride + col;
-      if (lane >= rows) return;
-#pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        if (wide == 32) {
-          if (col + i < limit)
-            ptx::stg256(to + i, {__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]),
-                                 __float_as_uint(v[i + 4]), __float_as_uint(v[i + 5]), __float_as_uint(v[i + 6]), __float_as_uint(v[i + 7])});
-        } else {
-#pragma unroll
-          for (int k = i; k < i + 8; k += 4)
-            if (col + k < limit) *reinterpret_cast<float4*>(to + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-        }
+      if (lane >= rows || left <= 0) return;
+      uint8_t* const at = at0 + lane * pitch;
+      if (wide == 32) {
+        ptx::stg256(at, w);
+      } else {
+        *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (left > 16) *reinterpret_cast<uint4*>(at + 16) = make_uint4(w[4], w[5], w[6], w[7]);
       }
       return;
     }
-    float* to = reinterpret_cast<float*>(d) + row_at + col;
-#pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      ptx::sts128(narrow + lane * 32, make_uint4(__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3])));
-      ptx::sts128(narrow + lane * 32 + 16, make_uint4(__float_as_uint(v[i + 4]), __float_as_uint(v[i + 5]), __float_as_uint(v[i + 6]), __float_as_uint(v[i + 7])));
-      __syncwarp();
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const int r = 4 * n + (lane >> 3), c = i + (lane & 7);
-        if (r < rows && col + c < limit) to[r * stride + c] = ptx::lds32f(narrow + r * 32 + (lane & 7) * 4);
+    __syncwarp();
+    ptx::sts128(narrow + lane * 32, make_uint4(w[0], w[1], w[2], w[3]));
+    ptx::sts128(narrow + lane * 32 + 16, make_uint4(w[4], w[5], w[6], w[7]));
+    __syncwarp();
+    if (f32) {
+#pragma unroll 2
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3), c = (lane & 7) * 4;
+        if (r < rows && c < left) *reinterpret_cast<uint32_t*>(at0 + r * pitch + c) = ptx::lds32(narrow + r * 32 + c);
       }
-      __syncwarp();
-    }
-    return;
-  }
-  const int f16 = t == B200MOE_F16;
-  uint32_t w[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = (uint32_t)bits16(v[2 * i], f16) | (uint32_t)bits16(v[2 * i + 1], f16) << 16;
-  if (wide != 0) {
-    uint16_t* to = reinterpret_cast<uint16_t*>(d) + row_at + lane * stride + col;
-    if (lane >= rows) return;
-#pragma unroll
-    for (int i = 0; i < 16; i += 8) {
-      if (wide == 32) {
-        if (col + 2 * i < limit) ptx::stg256(to + 2 * i, {w[i], w[i + 1], w[i + 2], w[i + 3], w[i + 4], w[i + 5], w[i + 6], w[i + 7]});
-      } else {
-#pragma unroll
-        for (int k = i; k < i + 8; k += 4)
-          if (col + 2 * k < limit) *reinterpret_cast<uint4*>(to + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+    } else {
+#pragma unroll 2
+      for (int i = 0; i < 16; ++i) {
+        const int r = 2 * i + (lane >> 4), c = (lane & 15) * 2;
+        if (r < rows && c < left) *reinterpret_cast<uint16_t*>(at0 + r * pitch + c) = ptx::lds16(narrow + r * 32 + c);
       }
     }
-    return;
-  }
-  uint16_t* to = reinterpret_cast<uint16_t*>(d) + row_at + col;
+  };
+  uint32_t w[8];
+  if (f32) {
 #pragma unroll
-  for (int i = 0; i < 16; i += 8) {
-    ptx::sts128(narrow + lane * 32, make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
-    ptx::sts128(narrow + lane * 32 + 16, make_uint4(w[i + 4], w[i + 5], w[i + 6], w[i + 7]));
-    __syncwarp();
+    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[i]);
+    piece(to, w, 4 * (limit - col));
 #pragma unroll
-    for (int n = 0; n < 16; ++n) {
-      const int r = 2 * n + (lane >> 4), c = 2 * i + (lane & 15);
-      if (r < rows && col + c < limit) to[r * stride + c] = ptx::lds16(narrow + r * 32 + (lane & 15) * 2);
-    }
-    __syncwarp();
+    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 + i]);
+    piece(to + 32, w, 4 * (limit - col) - 32);
+  } else {
+    const int f16 = t == B200MOE_F16;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = (uint32_t)bits16(v[2 * i], f16) | (uint32_t)bits16(v[2 * i + 1], f16) << 16;
+    piece(to, w, 2 * (limit - col));
   }
 }
+
+struct EpilogueTile {
+  int64_t first;      // the warp's first row
+  int rows;           // ... and how many it has
+  int features, j0, limit;
+  float xs;           // scale of the lane's row
+  float scale[4], bias[4];   // of weight rows, on their way to shared memory
+};
+// What an epilogue warp does with sums: rows (quarter of the CTA's 128, a lane each) of every second 16 columns.  (Sixteen at a time:
+// a call of few tiles runs this code once, and most of what it takes is the way of the instructions.)
+template <bool kI8, int kForm>
+struct Epilogue {
+  const TcDense& p;
+  const int side, quarter, cta;
+  const uint32_t lane_sel, scale0, bias0, narrow;
+  __device__ __forceinline__ Epilogue(const TcDense& job, Ctrl& ctrl, int cta_, int e)
+      : p(job), side(e >> 2), quarter((threadIdx.x >> 5) & 3), cta(cta_), lane_sel((uint32_t)(quarter * 32) << 16),
+        scale0(ptx::smem_u32(ctrl.scale[e])), bias0(ptx::smem_u32(ctrl.bias[e])), narrow(ptx::smem_u32(ctrl.narrow[e])) {}
+  // The warp's part of a tile, and the scales and biases that it will need: asked for a tile ahead (the way from HBM takes as long as
+  // a tile of a few K blocks: 1 row each of 128 experts of 2048 x 768 ..).
+  __device__ __forceinline__ EpilogueTile fetch(const TileInfo& ti) const {
+    const int lane = threadIdx.x & 31, half = p.n >> 1;
+    EpilogueTile t;
+    const int in_cta = quarter * 32, row0 = cta * p.half_rows + in_cta;
+    t.first = (int64_t)ti.row0 + row0;
+    t.rows = in_cta < p.half_rows ? (int)min((int64_t)min(ti.valid - row0, 32), p.m - t.first) : 0;
+    t.features = kForm == kGated ? p.width >> 1 : p.width;
+    t.j0 = ti.n_tile * t.features;
+    t.limit = kForm == kGated ? half : p.n;
+    t.xs = 1.f;
+    if (kI8 && t.rows > 0) {
+      // columns 16 c + .., c = side, side + 2, .., one after the other; gated 16 gates, then their ups
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int l = 32 * i + lane, c = 2 * (kForm == kGated ? i : l >> 4) + side, f = t.j0 + 16 * c + (lane & 15);
+        const bool there = 16 * c < t.features && f < t.limit;
+        const int64_t at = (int64_t)ti.e * p.n + f + (kForm == kGated && (lane & 16) ? half : 0);
+        t.scale[i] = there ? p.w_scale[at] : 0.f;
+        t.bias[i] = there && p.bias != nullptr ? load_bias(p.bias, p.bias_f16, at) : 0.f;
+      }
+      if (lane < t.rows) t.xs = p.x_scale[t.first + lane];
+    }
+    return t;
+  }
+  // ... to shared memory (every warp its own copy, so that no barrier couples the warps)
+  __device__ __forceinline__ void put(const EpilogueTile& t) const {
+    if (!kI8 || t.rows <= 0) return;
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ptx::sts32f(scale0 + 128 * i + 4 * lane, t.scale[i]);
+      ptx::sts32f(bias0 + 128 * i + 4 * lane, t.bias[i]);
+    }
+    __syncwarp();
+  }
+  // sums as the product's values; `l`: the first one's place among the warp's scales
+  __device__ __forceinline__ void scaled(float (&f)[16], const uint32_t (&v)[16], float xs, int l) const {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      if (!kI8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[i + k] = __uint_as_float(v[i + k]);
+        continue;
+      }
+      const float4 ws = ptx::lds128f(scale0 + 4 * (l + i)), b = ptx::lds128f(bias0 + 4 * (l + i));
+      f[i] = (float)(int)v[i] * xs * ws.x + b.x;
+      f[i + 1] = (float)(int)v[i + 1] * xs * ws.y + b.y;
+      f[i + 2] = (float)(int)v[i + 2] * xs * ws.z + b.z;
+      f[i + 3] = (float)(int)v[i + 3] * xs * ws.w + b.w;
+    }
+  }
+  // Columns 16 c.. of the tile (u: of ups, gated).
+  __device__ __forceinline__ void store(const EpilogueTile& t, int c, const uint32_t (&g)[16], const uint32_t (&u)[16]) const {
+    const int col = t.j0 + 16 * c, l = (kForm == kGated ? 16 : 8) * (c & ~1);
+    float f[16];
+    scaled(f, g, t.xs, l);
+    if (kForm == kGated) {
+      float up[16];
+      scaled(up, u, t.xs, l + 16);
+      if (p.pre != nullptr) {
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = h == 0 ? f[i] : up[i];
+          store_16(p.pre + h * (p.n >> 1), B200MOE_F32, t.first * p.n, p.n, t.rows, col, t.limit, v, p.pre_wide, narrow);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[i] = gated_product(f[i], up[i], p.clamp);
+    }
+    store_16(p.d, p.d_dtype, t.first * p.d_stride, p.d_stride, t.rows, col, t.limit, f, p.d_wide, narrow);
+  }
+};
 
 // kXMn, kWMn: the operand is stored by column (its rows' index is the dense one): 16-bit types, two boxes of 64 rows x 64 k.
 template <bool kI8, int kForm, bool kXMn, bool kWMn>
 __global__ void __launch_bounds__(kThreads, 1)
 dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const TcDense p) {
   constexpr int kPerKb = kI8 ? 128 : 64;
-  constexpr bool kScales = kI8 || kForm == kScaled;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + kRing);
@@ -224,8 +305,7 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       bool ok = true;
       const uint32_t full0 = ptx::smem_u32(&ctrl->full[0]), empty0 = ptx::smem_u32(&ctrl->empty[0]);
       const uint32_t bar0 = ptx::map_to_cta(full0, 0);   // the even CTA's barriers count the bytes of both CTAs
-      const uint32_t st0 = ptx::smem_u32(smem);
-      uint32_t st = st0;
+      const uint32_t st = ptx::smem_u32(smem);
       auto first_row = [&](const TileInfo& ti) {   // of W, of this CTA
         return kForm == kGated ? (cta == 0 ? 0 : half) + ti.n_tile * (p.width >> 1) : ti.n_tile * p.width + (int)cta * (p.width >> 1);
       };
@@ -233,36 +313,40 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         TileInfo ti;
         locate(t, ti);
         // rows past the end are filled with zeros
-        const int row = ti.row0 + (int)cta * 128;
+        const int row = ti.row0 + (int)cta * p.half_rows;
         const int n0 = first_row(ti);
         // loads of X in either CTA: as many as the tile's rows take
         auto boxes = [&](int c) {
-          const int rows = min(max(ti.valid - 128 * c, 0), 128);
+          const int rows = min(max(ti.valid - p.half_rows * c, 0), p.half_rows);
           return kXMn ? 2 : (rows + p.x_box - 1) / p.x_box;
         };
         const int mine = boxes((int)cta);
         const uint32_t box_bytes = kXMn ? kOperand / 2 : p.x_box * 128;
         const uint32_t tx = 2 * p.w_bytes + (boxes(0) + boxes(1)) * box_bytes;
-        for (int kb = 0; kb < p.num_kb; ++kb) {
+        for (int kb = 0; kb < p.num_kb;) {
           if (!ptx::paced::mbar_wait_s(empty0 + 8 * s, ph, abort_flag)) { ok = false; break; }
-          if (is_w && cta == 0) ptx::mbar_expect_tx_s(full0 + 8 * s, tx);
+          const int end = min(kb + p.blocks, p.num_kb);
+          if (is_w && cta == 0) ptx::mbar_expect_tx_s(full0 + 8 * s, tx * (end - kb));
           const uint32_t bar = bar0 + 8 * s;
-          const int k0 = kb * kPerKb;
-          if (!is_w) {
-            if (kXMn) {
-              ptx::tma_load_2d_pair(st, &tmap_x, bar, row, k0);
-              ptx::tma_load_2d_pair(st + kOperand / 2, &tmap_x, bar, row + 64, k0);
+          uint32_t to = st + s * p.blocks * p.block_bytes;
+          for (; kb < end; ++kb, to += p.block_bytes) {
+            const int k0 = kb * kPerKb;
+            const uint32_t w_to = to + p.x_bytes;
+            if (!is_w) {
+              if (kXMn) {
+                ptx::tma_load_2d_pair(to, &tmap_x, bar, row, k0);
+                ptx::tma_load_2d_pair(to + kOperand / 2, &tmap_x, bar, row + 64, k0);
+              } else {
+                for (int b = 0; b < mine; ++b) ptx::tma_load_2d_pair(to + b * box_bytes, &tmap_x, bar, k0, row + b * p.x_box);
+              }
+            } else if (kWMn) {
+              ptx::tma_load_3d_pair(w_to, &tmap_w, bar, n0, k0, ti.e);
+              if (p.w_bytes > kOperand / 2) ptx::tma_load_3d_pair(w_to + kOperand / 2, &tmap_w, bar, n0 + 64, k0, ti.e);
             } else {
-              for (int b = 0; b < mine; ++b) ptx::tma_load_2d_pair(st + b * box_bytes, &tmap_x, bar, k0, row + b * p.x_box);
+              ptx::tma_load_3d_pair(w_to, &tmap_w, bar, k0, n0, ti.e);
             }
-          } else if (kWMn) {
-            ptx::tma_load_3d_pair(st + kOperand, &tmap_w, bar, n0, k0, ti.e);
-            if (p.w_bytes > kOperand / 2) ptx::tma_load_3d_pair(st + kOperand + kOperand / 2, &tmap_w, bar, n0 + 64, k0, ti.e);
-          } else {
-            ptx::tma_load_3d_pair(st + kOperand, &tmap_w, bar, k0, n0, ti.e);
           }
-          st += p.stage_bytes;
-          if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; st = st0; }
+          if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
         }
       }
     }
@@ -277,22 +361,23 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       // 16-byte units between the K steps of an operand: 32 bytes of its rows, or 16 of the k that are its rows
       constexpr int kXStep = kXMn ? 2048 / 16 : 2, kWStep = kWMn ? 2048 / 16 : 2;
       const uint64_t xdesc0 = ptx::make_smem_desc(ptx::smem_u32(smem), kXMn ? 8192u : 16u, 1024);
-      const uint64_t wdesc0 = ptx::make_smem_desc(ptx::smem_u32(smem) + kOperand, kWMn ? 8192u : 16u, 1024);
-      uint64_t xdesc = xdesc0, wdesc = wdesc0;
-      const uint64_t stage16 = p.stage_bytes >> 4;
+      const uint64_t wdesc0 = ptx::make_smem_desc(ptx::smem_u32(smem) + p.x_bytes, kWMn ? 8192u : 16u, 1024);
+      const uint64_t block16 = p.block_bytes >> 4, stage16 = p.blocks * block16;
+      uint64_t at = 0;     // of the stage, from the first one's descriptors
       for (int t = walker; t < total && ok; t += walkers) {
         const uint32_t a = acc_it & 1;
         if (!ptx::mbar_wait_s(acc_empty0 + 8 * a, ((acc_it >> 1) & 1) ^ 1, abort_flag)) break;
         ptx::tc_fence_after();
-        for (int kb = 0; kb < p.num_kb; ++kb) {
+        for (int kb = 0; kb < p.num_kb;) {
           if (!ptx::mbar_wait_s(full0 + 8 * s, ph, abort_flag)) { ok = false; break; }
           ptx::tc_fence_after();
-          if (kI8) ptx::umma_i8_pair_block<kXStep, kWStep>(tmem_base + a * kTile, xdesc, wdesc, p.idesc, kb > 0 ? 1u : 0u);
-          else ptx::umma_f16_pair_block<kXStep, kWStep>(tmem_base + a * kTile, xdesc, wdesc, p.idesc, kb > 0 ? 1u : 0u);
+          const int end = min(kb + p.blocks, p.num_kb);
+          for (uint64_t d = at; kb < end; ++kb, d += block16) {
+            ptx::umma_pair_block<kI8, kXStep, kWStep>(tmem_base + a * kTile, xdesc0 + d, wdesc0 + d, p.idesc, kb > 0 ? 1u : 0u);
+          }
           ptx::umma_commit_pair(empty0 + 8 * s);
-          xdesc += stage16;
-          wdesc += stage16;
-          if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; xdesc = xdesc0; wdesc = wdesc0; }
+          at += stage16;
+          if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; at = 0; }
         }
         if (ok) { ptx::umma_commit_pair(acc_full0 + 8 * a); ++acc_it; }
       }
@@ -300,97 +385,68 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
     __syncwarp();
   } else {
     // ------------------------------ epilogue ----------------------------------
-    const int quarter = warp & 3, side = (warp - 2) >> 2;
-    const uint32_t lane_sel = (uint32_t)(quarter * 32) << 16;
+    const Epilogue<kI8, kForm> ep(p, *ctrl, (int)cta, warp - 2);
     const uint32_t acc_empty0 = ptx::map_to_cta(ptx::smem_u32(&ctrl->acc_empty[0]), 0);
-    const uint32_t scale0 = ptx::smem_u32(ctrl->scale[warp - 2]), bias0 = ptx::smem_u32(ctrl->bias[warp - 2]);
-    const uint32_t narrow = ptx::smem_u32(ctrl->narrow[warp - 2]);
     uint32_t acc_it = 0;
-    for (int t = walker; t < total; t += walkers) {
+    auto fetch = [&](int t) {
       TileInfo ti;
       locate(t, ti);
+      return ep.fetch(ti);
+    };
+    EpilogueTile next = walker < total ? fetch(walker) : EpilogueTile{};
+    for (int t = walker; t < total; t += walkers) {
       const uint32_t a = acc_it & 1;
-      const int row0 = (int)cta * 128 + quarter * 32;      // this warp's first row in the tile
-      const int64_t first = (int64_t)ti.row0 + row0;
-      const int rows = (int)min((int64_t)min(ti.valid - row0, 32), p.m - first);
-      const int features = kForm == kGated ? p.width >> 1 : p.width, j0 = ti.n_tile * features;
-      const int limit = kForm == kGated ? half : p.n;
-      float xs = 1.f;
-      if (kScales) {
-        // the weight rows' scales and biases: every warp its own copy, so that no barrier couples the warps
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // (gated: 32 gates, then their ups)
-          const int c = 2 * (kForm == kGated ? i >> 1 : i) + side, f = j0 + 32 * c + lane;
-          const bool there = 32 * c < features && f < limit;
-          const int64_t at = (int64_t)ti.e * p.n + f + (kForm == kGated && (i & 1) ? half : 0);
-          ptx::sts32f(scale0 + 128 * i + 4 * lane, there ? p.w_scale[at] : 0.f);
-          ptx::sts32f(bias0 + 128 * i + 4 * lane, there && p.bias != nullptr ? load_bias(p.bias, p.bias_f16, at) : 0.f);
-        }
-        if (lane < rows) xs = p.x_scale[first + lane];
-        __syncwarp();
-      }
+      const EpilogueTile et = next;
+      ep.put(et);
+      if (t + walkers < total) next = fetch(t + walkers);
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(&ctrl->acc_full[a], (acc_it >> 1) & 1, abort_flag))) {
         *abort_flag = 1;
         break;
       }
       ptx::tc_fence_after();
-      const uint32_t acc = tmem_base + a * kTile + lane_sel;
-      // sums as the product's values; `l`: the first one's place among the warp's scales
-      auto scaled = [&](float (&f)[32], const uint32_t (&v)[32], int l) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          if (!kScales) {
-            for (int k = 0; k < 4; ++k) f[i + k] = __uint_as_float(v[i + k]);
-            continue;
-          }
-          const float4 ws = ptx::lds128f(scale0 + 4 * (l + i)), b = ptx::lds128f(bias0 + 4 * (l + i));
-          f[i] = (float)(int)v[i] * xs * ws.x + b.x;
-          f[i + 1] = (float)(int)v[i + 1] * xs * ws.y + b.y;
-          f[i + 2] = (float)(int)v[i + 2] * xs * ws.z + b.z;
-          f[i + 3] = (float)(int)v[i + 3] * xs * ws.w + b.w;
-        }
-      };
-      if (rows > 0) {
-#pragma unroll 1
-        for (int c = side; 32 * c < features && j0 + 32 * c < limit; c += 2) {
-          const int col = 32 * c, l = kForm == kGated ? 32 * (c & ~1) : 16 * (c & ~1);
-          uint32_t g[32], u[kForm == kGated ? 32 : 1];
+      const uint32_t acc = tmem_base + a * kTile + ep.lane_sel;
+      if (et.rows > 0) {
+        constexpr int kParts = kForm == kGated ? 2 : 1;
+        const int units = min(et.features, et.limit - et.j0);     // columns that exist
+        uint32_t v[2][kParts][16];
+        auto load = [&](int c, int b) {
           __syncwarp();
-          ptx::tmem_ld_32x32(acc + col, g);
-          if (kForm == kGated) ptx::tmem_ld_32x32(acc + features + col, reinterpret_cast<uint32_t(&)[32]>(u));
-          if (kForm == kGated) ptx::tmem_wait_ld(g, u);
-          else ptx::tmem_wait_ld(g);
-          float f[32];
-          scaled(f, g, l);
-          if (kForm == kGated) {
-            float up[32];
-            scaled(up, reinterpret_cast<uint32_t(&)[32]>(u), l + 32);
-            if (p.pre != nullptr) {
-              store_32(p.pre, B200MOE_F32, first * p.n, p.n, rows, j0 + col, limit, f, p.pre_wide, narrow);
-              store_32(p.pre + half, B200MOE_F32, first * p.n, p.n, rows, j0 + col, limit, up, p.pre_wide, narrow);
-            }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = gated_product(f[i], up[i], p.clamp);
-          }
-          store_32(p.d, p.d_dtype, first * p.d_stride, p.d_stride, rows, j0 + col, limit, f, p.d_wide, narrow);
+          for (int part = 0; part < kParts; ++part) ptx::tmem_ld_32x16(acc + part * et.features + 16 * c, v[b][part]);
+        };
+        auto store = [&](int c, int b) { ep.store(et, c, v[b][0], v[b][kParts - 1]); };
+        // the next columns are on their way while these are stored
+        auto wait = [&](int b) {
+          if (kParts == 2) ptx::tmem_wait_ld(v[b][0], v[b][kParts - 1]);
+          else ptx::tmem_wait_ld(v[b][0]);
+        };
+        if (16 * ep.side < units) load(ep.side, 0);
+#pragma unroll 1
+        for (int c = ep.side; 16 * c < units; c += 4) {
+          wait(0);
+          if (16 * (c + 2) < units) load(c + 2, 1);
+          store(c, 0);
+          if (16 * (c + 2) >= units) break;
+          wait(1);
+          if (16 * (c + 4) < units) load(c + 4, 0);
+          store(c + 2, 1);
         }
       }
       __syncwarp();
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(acc_empty0 + a * 8);
+      // (nobody waits for the last two: no arrival is on its way to a CTA that may have left)
+      if (lane == 0 && t + 2 * walkers < total) ptx::mbar_arrive_cluster(acc_empty0 + a * 8);
       ++acc_it;
     }
   }
-
   // Teardown: neither CTA frees tensor memory or leaves while the other may still use its shared memory, its barriers or MMAs
-  // in flight (every thread of both CTAs gets here after bounded waits).
+  // in flight (every thread of both CTAs gets here after bounded waits).  Nothing that one CTA wrote is read by another any more: a
+  // barrier that also waits until all rows that were stored have reached L2 took 2 to 4 us longer.
   pdl_trigger();
   ptx::tc_fence_before();
   __syncthreads();
-  ptx::cluster_sync();
+  ptx::cluster_sync_relaxed();
   if (warp == 1) {
     ptx::tc_fence_after();
     if (*abort_flag != 0) __nanosleep(20000);
@@ -400,37 +456,49 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
 }
 
 template <bool kI8, int kForm, bool kXMn, bool kWMn>
-int launch(const CUtensorMap& tx, const CUtensorMap& tw, const TcDense& p, int64_t tiles, int max_ctas, bool early, cudaStream_t st) {
-  auto kern = dense_tc_kernel<kI8, kForm, kXMn, kWMn>;
-  static SmemConfig configured;
-  if (int rc = configured.ensure(kern)) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = kSmem; cfg.stream = st;
-  cfg.attrs = attr; cfg.numAttrs = 1;
-  static std::atomic<int> resident[kMaxDevices];
-  const int dev = current_device();
-  int pairs = resident[dev].load(std::memory_order_relaxed);
-  if (pairs == 0) {
-    cfg.gridDim = dim3(2 * (sm_count() / 2));
-    if (cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg) != cudaSuccess || pairs < 1) {
+struct Kernel {
+  static constexpr auto kern = dense_tc_kernel<kI8, kForm, kXMn, kWMn>;
+  // How many pairs the device runs at once; 0 if none (a partition with too few SMs per GPC, say).
+  static int pairs() {
+    static std::atomic<int> cached[kMaxDevices];
+    const int dev = current_device();
+    int n = cached[dev].load(std::memory_order_relaxed);
+    if (n != 0) return n < 0 ? 0 : n;
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg = config(attr, 1, std::max(1, sm_count() / 2), 0);
+    if (configured() != B200MOE_OK || cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
       (void)cudaGetLastError();
-      pairs = -1;   // this device (a partition with too few SMs per GPC, say) runs no such cluster
+      n = -1;
     }
-    resident[dev].store(pairs, std::memory_order_relaxed);
+    cached[dev].store(n, std::memory_order_relaxed);
+    return n < 0 ? 0 : n;
   }
-  if (pairs < 0) return fail(B200MOE_E_UNSUPPORTED, "dense products: this device runs no clusters of two CTAs");
-  if (max_ctas > 0) pairs = std::min(pairs, std::max(1, max_ctas / 2));
-  pairs = (int)std::max<int64_t>(1, std::min<int64_t>(pairs, tiles));
-  cfg.gridDim = dim3(2 * pairs);
-  cfg.numAttrs = early ? 2 : 1;
-  B200_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, tx, tw, p));
-  return B200MOE_OK;
-}
+  static int launch(const CUtensorMap& tx, const CUtensorMap& tw, const TcDense& p, int64_t pairs, bool early, cudaStream_t st) {
+    if (int rc = configured()) return rc;
+    cudaLaunchAttribute attr[2];
+    const cudaLaunchConfig_t cfg = config(attr, early ? 2 : 1, pairs, st);
+    B200_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, tx, tw, p));
+    return B200MOE_OK;
+  }
+
+ private:
+  static int configured() {
+    static SmemConfig done;
+    return done.ensure(kern);
+  }
+  static cudaLaunchConfig_t config(cudaLaunchAttribute* attr, int attrs, int64_t pairs, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    if (attrs > 1) {
+      attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[1].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = kSmem; cfg.stream = st;
+    cfg.attrs = attr; cfg.numAttrs = attrs;
+    return cfg;
+  }
+};
 
 CUtensorMapDataType map_type(DenseType t) {
   return t == kDenseI8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
@@ -446,20 +514,26 @@ int operand_map(CUtensorMap* map, DenseType t, const void* base, int64_t rows, i
   const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
   return encode_map(map, map_type(t), experts > 0 ? 3 : 2, base, dims, strides, box);
 }
-// Weight rows of a tile: what leaves the least for the pair that has most to do.  A K block of a tile costs 2 cycles a weight row in the
-// tensor cores, 64 bytes a weight row and the rows of X on the way into a CTA (some 56 bytes a cycle), and, where no other tile of rows
-// reads the same weights, 64 bytes a weight row from HBM (23 bytes a cycle and SM); a tile costs some 600 cycles besides.
-int tile_width(const TcDense& p, int64_t features, bool gated, int64_t row_tiles, int rows, int pairs) {
+// K blocks of a stage: as many as leave four stages.  A wait, and what goes with it (the producers' arrivals, the issuer's commit to both
+// CTAs), takes either single thread some 360 cycles, a load or a block's products 50 to 100.  64 x 7168 x 2048 gated, tiles of 64
+// weight rows, 1 / 2 / 3 / 4 / 6 blocks of 8 KB a stage 33.9 / 24.6 / 21.5 / 20.0 / 18.7 us; 256 rows (20 KB) 34.1 / 25.3 / 25.2 / 29.7 / 45.7.
+int stage_blocks(int block_bytes) { return std::max(1, std::min(6, kRing / (4 * block_bytes))); }
+
+// Weight rows of a tile: what takes the fewest cycles by this estimate.  A K block of a tile takes 170 cycles and its share of the waits, 2.45 a
+// weight row in the tensor cores, and a cycle for each 60 of its bytes; a tile costs some 2000 besides; and the weights pass HBM at 3440
+// bytes a cycle at the most.  2000 x 4096 x 4096 from codes with 64 / 128 / 192 / 256 weight rows 46 / 31 / 29 / 26 us, 1001 x 2016 x 2032
+// 11.8 / 9.3 / 10.9 / 12.1, 64 x 4096 x 4096 8.5 / 10.0 / 12.5 / 15.3; 15 rows each of 8 experts of 4096 x 14336, a layer, 440 / 300 / 284 / 266.
+void choose_tile(TcDense& p, int64_t sets, int64_t row_tiles, int features, bool gated, bool w_mn, int64_t pairs, int64_t w_bytes) {
   const int step = gated ? 64 : 32;
-  int best = 0;
   double least = 0;
+  p.width = 0;
   for (int width = kTile; width >= 64; width -= step) {
-    const int64_t tiles = row_tiles * ((features + (gated ? width / 2 : width) - 1) / (gated ? width / 2 : width));
-    const double load = (128.0 * std::min(rows, 128) + 64.0 * width) / 56, hbm = row_tiles == 1 ? 64.0 * width / 23 : 0;
-    const double cost = (double)((tiles + pairs - 1) / pairs) * (p.num_kb * std::max({2.0 * width, load, hbm}) + 600);
-    if (best == 0 || cost < least) { best = width; least = cost; }
+    const int out = gated ? width / 2 : width, bytes = p.half_rows * 128 + (w_mn ? (width + 127) / 128 * 8192 : width * 64);
+    const int64_t tiles = sets * row_tiles * ((features + out - 1) / out), rounds = (tiles + pairs - 1) / pairs;
+    const double block = std::max({300.0 / stage_blocks(bytes) + 170, 2.45 * width, bytes / 60.0});
+    const double cost = std::max(rounds * (p.num_kb * block + 2000), w_bytes / 3440.0);
+    if (p.width == 0 || cost < least) { p.width = width; least = cost; }
   }
-  return best;
 }
 int store_width(const void* p, int64_t row_bytes, int64_t cols_bytes) {
   for (int w : {32, 16})
@@ -472,12 +546,14 @@ uint32_t idesc_of(DenseType t, bool x_mn, bool w_mn, int width) {
   return ptx::make_idesc(fmt, fmt, x_mn ? 1u : 0u, w_mn ? 1u : 0u, 256, width);
 }
 // What follows from a tile's width.
-void set_width(TcDense& p, DenseType t, bool x_mn, bool w_mn, int width, int features, bool gated) {
-  p.width = width;
+void set_width(TcDense& p, DenseType t, bool x_mn, bool w_mn, int features, bool gated) {
+  const int width = p.width;
   p.n_tiles = (features + (gated ? width / 2 : width) - 1) / (gated ? width / 2 : width);
+  p.x_bytes = p.half_rows * 128;
   p.w_bytes = w_mn ? (width > 128 ? kOperand : kOperand / 2) : width * 64;
-  p.stage_bytes = kOperand + p.w_bytes;
-  p.stages = std::min(kMaxStages, kRing / p.stage_bytes);
+  p.block_bytes = p.x_bytes + p.w_bytes;
+  p.blocks = stage_blocks(p.block_bytes);
+  p.stages = std::min(kMaxStages, kRing / (p.blocks * p.block_bytes));
   p.idesc = idesc_of(t, x_mn, w_mn, width);
 }
 
@@ -490,51 +566,57 @@ int dense_tc(const DenseJob& j, cudaStream_t st) {
   p.m = j.m; p.d_stride = j.d_stride; p.n = j.n; p.experts = j.experts;
   const int per_kb = j.type == kDenseI8 ? 128 : 64, n_out = j.gated ? j.n / 2 : j.n;
   p.num_kb = (j.k + per_kb - 1) / per_kb;
-  p.m_tiles = (int)((j.m + kTile - 1) / kTile);
-  const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m, each = (rows + j.experts - 1) / j.experts;
-  const int64_t sets = j.rows_per_expert != nullptr ? std::min<int64_t>(j.experts, rows) : 1;
-  int width = 0;
-  {
-    // (as if every set had the mean number of rows; sets that share a tile of rows with no other read their weights once)
-    const int64_t tiles_each = (each + kTile - 1) / kTile;
-    const int pairs = std::max(1, (j.max_ctas > 0 ? std::min(j.max_ctas, sm_count()) : sm_count()) / 2);
-    width = tile_width(p, n_out * sets, j.gated, tiles_each, (int)std::min<int64_t>(each, kTile), pairs);
-  }
-  set_width(p, j.type, false, false, width, n_out, j.gated);
-  p.x_box = each <= 96 ? 32 : 128;
+  // Rows of a tile (one set of weights): 256, fewer for fewer.  (The tensor cores always take 128 a CTA: those behind a CTA's own make
+  // sums of whatever follows in shared memory, which nobody reads.)
+  p.half_rows = j.rows_per_expert != nullptr || j.m > 128 ? 128 : j.m > 64 ? 64 : 32;
+  p.m_tiles = (int)((j.m + 2 * p.half_rows - 1) / (2 * p.half_rows));
   p.d_dtype = j.d_dtype; p.bias_f16 = j.bias_f16; p.clamp = j.clamp;
   const int out_size = dtype_bytes(j.d_dtype);
   p.d_wide = store_width(j.d, j.d_stride * out_size, (int64_t)n_out * out_size);
   if (j.pre != nullptr) p.pre_wide = store_width(j.pre, (int64_t)j.n * 4, (int64_t)n_out * 4);
-  CUtensorMap tx, tw;
-  if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, false, 0, p.x_box)) return rc;
-  if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, false, j.experts, width / 2)) return rc;
-  const int64_t tiles = (p.m_tiles + (j.rows_per_expert != nullptr ? (int64_t)j.experts : 0)) * p.n_tiles;
-  if (j.type == kDenseI8) {
-    const int rc = j.gated ? launch<true, kGated, false, false>(tx, tw, p, tiles, j.max_ctas, j.early, st)
-                           : launch<true, kScaled, false, false>(tx, tw, p, tiles, j.max_ctas, j.early, st);
-    return rc == B200MOE_E_UNSUPPORTED ? dense_rows(j, st) : rc;
-  }
-  const int rc = launch<false, kGated, false, false>(tx, tw, p, tiles, j.max_ctas, j.early, st);
-  return rc == B200MOE_E_UNSUPPORTED ? dense_rows(j, st) : rc;
+  // (tiles as if every set of weights had the mean number of rows)
+  const bool grouped = j.rows_per_expert != nullptr;
+  const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m, each = (rows + j.experts - 1) / j.experts;
+  const int64_t sets = grouped ? std::min<int64_t>(j.experts, rows) : 1;
+  p.x_box = grouped ? (each <= 96 ? 32 : 128) : p.half_rows;
+  auto run = [&](auto kernel) {
+    using K = decltype(kernel);
+    if (K::pairs() == 0) return dense_rows(j, st);   // no clusters on this device
+    const int64_t pairs = j.max_ctas > 0 ? std::min(K::pairs(), std::max(1, j.max_ctas / 2)) : K::pairs();
+    choose_tile(p, sets, grouped ? (each + kTile - 1) / kTile : p.m_tiles, n_out, j.gated, false, pairs,
+                sets * j.n * (int64_t)j.k * (j.type == kDenseI8 ? 1 : 2));
+    set_width(p, j.type, false, false, n_out, j.gated);
+    CUtensorMap tx, tw;
+    if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, false, 0, p.x_box)) return rc;
+    if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, false, j.experts, p.width / 2)) return rc;
+    const int64_t tiles = (p.m_tiles + (grouped ? (int64_t)j.experts : 0)) * p.n_tiles;
+    return K::launch(tx, tw, p, std::min(pairs, tiles), j.early, st);
+  };
+  if (j.type != kDenseI8) return run(Kernel<false, kGated, false, false>());
+  return j.gated ? run(Kernel<true, kGated, false, false>()) : run(Kernel<true, kScaled, false, false>());
 }
 
 int dense_plain(const PlainJob& j, cudaStream_t st) {
   TcDense p = {};
   p.d = j.d; p.status = j.status; p.m = j.m; p.d_stride = j.d_stride; p.n = j.n; p.experts = 1;
   p.num_kb = (int)((j.k + 63) / 64);
-  p.m_tiles = (int)((j.m + kTile - 1) / kTile);
-  const int width = tile_width(p, j.n, false, p.m_tiles, (int)std::min<int64_t>(j.m, kTile), std::max(1, sm_count() / 2));
-  set_width(p, j.type, j.x_by_column, true, width, j.n, false);
-  p.x_box = 128;
+  p.half_rows = j.x_by_column || j.m > 128 ? 128 : j.m > 64 ? 64 : 32;
+  p.m_tiles = (int)((j.m + 2 * p.half_rows - 1) / (2 * p.half_rows));
+  p.x_box = p.half_rows;
   p.d_dtype = j.type == kDenseF16 ? B200MOE_F16 : B200MOE_BF16;
   p.d_wide = store_width(j.d, j.d_stride * 2, (int64_t)j.n * 2);
-  CUtensorMap tx, tw;
-  if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, j.x_by_column, 0, j.x_by_column ? 64 : 128)) return rc;
-  if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, true, 1, 64)) return rc;
-  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-  return j.x_by_column ? launch<false, kPlain, true, true>(tx, tw, p, tiles, 0, j.early, st)
-                       : launch<false, kPlain, false, true>(tx, tw, p, tiles, 0, j.early, st);
+  auto run = [&](auto kernel) {
+    using K = decltype(kernel);
+    if (K::pairs() == 0) return fail(B200MOE_E_UNSUPPORTED, "dense products: this device runs no clusters of two CTAs");
+    choose_tile(p, 1, p.m_tiles, j.n, false, true, K::pairs(), 0);
+    set_width(p, j.type, j.x_by_column, true, j.n, false);
+    CUtensorMap tx, tw;
+    if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, j.x_by_column, 0, j.x_by_column ? 64 : p.x_box)) return rc;
+    if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, true, 1, 64)) return rc;
+    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+    return K::launch(tx, tw, p, std::min<int64_t>(K::pairs(), tiles), j.early, st);
+  };
+  return j.x_by_column ? run(Kernel<false, kPlain, true, true>()) : run(Kernel<false, kPlain, false, true>());
 }
 
 }  // namespace b200moe

@@ -289,6 +289,10 @@ __device__ __forceinline__ uint32_t cluster_count_x() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same without making memory visible: that all threads have come this far.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 // The shared::cluster address of `addr` (a shared address of this CTA) in CTA `rank`.
 __device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -673,13 +677,16 @@ __device__ __forceinline__ void umma_f16_pair_block(uint32_t tmem_d, uint64_t ad
         "n"(3 * kAStep), "n"(kBStep), "n"(2 * kBStep), "n"(3 * kBStep)
       : "memory");
 }
-// 8-bit integers (both signed, int32 sums): kind::i8, K = 32 bytes an instruction as for the other 8-bit types.
+// The same for 8-bit integers (kI8: both signed, int32 sums, K = 32 bytes an instruction as for the other 8-bit types) or 16-bit values.
 __host__ __device__ constexpr uint32_t make_idesc_i8(uint32_t M, uint32_t N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
-template <int kAStep, int kBStep>
-__device__ __forceinline__ void umma_i8_pair_block(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                                   uint32_t accumulate) {
+template <bool kI8, int kAStep, int kBStep>
+__device__ __forceinline__ void umma_pair_block(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  if (!kI8) {
+    umma_f16_pair_block<kAStep, kBStep>(tmem_d, adesc, bdesc, idesc, accumulate);
+    return;
+  }
   asm volatile(
       "{\n\t.reg .pred pa;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\tsetp.ne.b32 pa, %4, 0;\n\t"
       "add.u64 a1, %1, %5;\n\tadd.u64 a2, %1, %6;\n\tadd.u64 a3, %1, %7;\n\t"

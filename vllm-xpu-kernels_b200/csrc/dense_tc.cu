@@ -88,6 +88,31 @@ __device__ __forceinline__ void locate_dense(const TcDense& p, int t, TileInfo& 
   ti.valid = (int)min((int64_t)tile_rows(p), p.m - ti.row0);
 }
 
+// A tile of the walk over experts' rows.  (locate_tile of gemm_tc_common.cuh with a shorter search: a pair's next tile is some experts on, as
+// many as tiles fit an expert with one tile of rows, which most are.)
+__device__ __forceinline__ void locate_grouped(const TcDense& p, const TileWalk& w, int t, int& cursor, TileInfo& ti) {
+  if (t >= w.tile_start[cursor + 1]) {
+    int hi = min(cursor + (t - w.tile_start[cursor]) / p.n_tiles, w.n - 1);   // no expert has fewer than n_tiles tiles
+    if (w.tile_start[hi] > t) {
+      int lo = cursor + 1;
+      --hi;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (w.tile_start[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+    }
+    cursor = hi;
+  }
+  const int local = t - w.tile_start[cursor], row = w.row_start[cursor], rows = w.row_start[cursor + 1] - row;
+  const int m_tiles = (rows + kTile - 1) / kTile;
+  ti.e = w.expert[cursor];
+  ti.n_tile = m_tiles == 1 ? local : local / m_tiles;
+  ti.m_tile = local - ti.n_tile * m_tiles;
+  ti.row0 = row + ti.m_tile * kTile;
+  ti.valid = min(rows - ti.m_tile * kTile, kTile);
+}
+
 // A warp's 32 rows x 16 columns, a row a lane, of which the first `rows` rows and the columns below `limit` exist: in pieces of 32 or
 // 16 bytes where they are aligned, else through shared memory, so that lanes that store together are neighbours in a row.
 // (Odd row lengths, value by value from the row's own lane: 1001 x 2011 x 2032 48 us.)
@@ -137,9 +162,19 @@ __device__ __forceinline__ void store_16(void* d, b200moe_dtype t, int64_t row_a
     for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 + i]);
     piece(to + 32, w, 4 * (limit - col) - 32);
   } else {
-    const int f16 = t == B200MOE_F16;
+    if (t == B200MOE_F16) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = (uint32_t)bits16(v[2 * i], f16) | (uint32_t)bits16(v[2 * i + 1], f16) << 16;
+      for (int i = 0; i < 8; ++i) {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
     piece(to, w, 2 * (limit - col));
   }
 }
@@ -147,9 +182,10 @@ __device__ __forceinline__ void store_16(void* d, b200moe_dtype t, int64_t row_a
 struct EpilogueTile {
   int64_t first;      // the warp's first row
   int rows;           // ... and how many it has
-  int features, j0, limit;
+  int features, j0, limit;   // its columns of D are j0 .. limit - 1
   float xs;           // scale of the lane's row
-  float scale[4], bias[4];   // of weight rows, on their way to shared memory
+  float scale[4];     // of weight rows, on their way to shared memory
+  uint16_t bias[4];
 };
 // What an epilogue warp does with sums: rows (quarter of the CTA's 128, a lane each) of every second 16 columns.  (Sixteen at a time:
 // a call of few tiles runs this code once, and most of what it takes is the way of the instructions.)
@@ -171,19 +207,20 @@ struct Epilogue {
     t.rows = in_cta < p.half_rows ? (int)min((int64_t)min(ti.valid - row0, 32), p.m - t.first) : 0;
     t.features = kForm == kGated ? p.width >> 1 : p.width;
     t.j0 = ti.n_tile * t.features;
-    t.limit = kForm == kGated ? half : p.n;
+    t.limit = min(kForm == kGated ? half : p.n, t.j0 + t.features);
     t.xs = 1.f;
     if (kI8 && t.rows > 0) {
-      // columns 16 c + .., c = side, side + 2, .., one after the other; gated 16 gates, then their ups
+      // columns 16 c + .., c = side, side + 2, .., one after the other; gated 16 gates, then their ups.  (Nothing is done with what
+      // is loaded, not even for columns that do not exist, so that nothing waits for it here.)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int l = 32 * i + lane, c = 2 * (kForm == kGated ? i : l >> 4) + side, f = t.j0 + 16 * c + (lane & 15);
-        const bool there = 16 * c < t.features && f < t.limit;
+        const int l = 32 * i + lane, c = 2 * (kForm == kGated ? i : l >> 4) + side, f = min(t.j0 + 16 * c + (lane & 15), t.limit - 1);
         const int64_t at = (int64_t)ti.e * p.n + f + (kForm == kGated && (lane & 16) ? half : 0);
-        t.scale[i] = there ? p.w_scale[at] : 0.f;
-        t.bias[i] = there && p.bias != nullptr ? load_bias(p.bias, p.bias_f16, at) : 0.f;
+        t.scale[i] = p.w_scale[at];
+        t.bias[i] = 0;
+        if (p.bias != nullptr) t.bias[i] = reinterpret_cast<const uint16_t*>(p.bias)[at];
       }
-      if (lane < t.rows) t.xs = p.x_scale[t.first + lane];
+      t.xs = p.x_scale[min(t.first + lane, p.m - 1)];
     }
     return t;
   }
@@ -195,25 +232,38 @@ struct Epilogue {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       ptx::sts32f(scale0 + 128 * i + 4 * lane, t.scale[i]);
-      ptx::sts32f(bias0 + 128 * i + 4 * lane, t.bias[i]);
+      ptx::sts32f(bias0 + 128 * i + 4 * lane, load_bias(&t.bias[i], p.bias_f16, 0));
     }
     __syncwarp();
   }
   // sums as the product's values; `l`: the first one's place among the warp's scales
   __device__ __forceinline__ void scaled(float (&f)[16], const uint32_t (&v)[16], float xs, int l) const {
+    if (!kI8) {
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      if (!kI8) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) f[i + k] = __uint_as_float(v[i + k]);
-        continue;
-      }
-      const float4 ws = ptx::lds128f(scale0 + 4 * (l + i)), b = ptx::lds128f(bias0 + 4 * (l + i));
-      f[i] = (float)(int)v[i] * xs * ws.x + b.x;
-      f[i + 1] = (float)(int)v[i + 1] * xs * ws.y + b.y;
-      f[i + 2] = (float)(int)v[i + 2] * xs * ws.z + b.z;
-      f[i + 3] = (float)(int)v[i + 3] * xs * ws.w + b.w;
+      for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+      return;
     }
+    float4 ws[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ws[i] = ptx::lds128f(scale0 + 4 * (l + 4 * i));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = ptx::lds128f(bias0 + 4 * (l + 4 * i));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[4 * i] = (float)(int)v[4 * i] * xs * ws[i].x + b[i].x;
+      f[4 * i + 1] = (float)(int)v[4 * i + 1] * xs * ws[i].y + b[i].y;
+      f[4 * i + 2] = (float)(int)v[4 * i + 2] * xs * ws[i].z + b[i].z;
+      f[4 * i + 3] = (float)(int)v[4 * i + 3] * xs * ws[i].w + b[i].w;
+    }
+  }
+  // Columns 16 c.. and 16 (c + 2).. of the tile (not gated).
+  __device__ __forceinline__ void store_two(const EpilogueTile& t, int c, const uint32_t (&a)[16], const uint32_t (&b)[16]) const {
+    const int col = t.j0 + 16 * c, l = 8 * (c & ~1);
+    float f[16], g[16];
+    scaled(f, a, t.xs, l);
+    scaled(g, b, t.xs, l + 16);
+    store_16(p.d, p.d_dtype, t.first * p.d_stride, p.d_stride, t.rows, col, t.limit, f, p.d_wide, narrow);
+    store_16(p.d, p.d_dtype, t.first * p.d_stride, p.d_stride, t.rows, col + 32, t.limit, g, p.d_wide, narrow);
   }
   // Columns 16 c.. of the tile (u: of ups, gated).
   __device__ __forceinline__ void store(const EpilogueTile& t, int c, const uint32_t (&g)[16], const uint32_t (&u)[16]) const {
@@ -265,7 +315,7 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
     ptx::tmem_relinquish_pair();
   } else if (warp == 2 && lane == 0) {
     for (int s = 0; s < kMaxStages; ++s) {
-      ptx::mbar_init(&ctrl->full[s], 1);
+      ptx::mbar_init(&ctrl->full[s], 3);     // the even CTA's producer of W, which announces the bytes, and both producers of X
       ptx::mbar_init(&ctrl->empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -291,7 +341,7 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   const int half = p.n >> 1;
   int cursor = 0;
   auto locate = [&](int t, TileInfo& ti) {
-    if (grouped) locate_tile<kTile>(walk, t, cursor, ti);
+    if (grouped) locate_grouped(p, walk, t, cursor, ti);
     else locate_dense(p, t, ti);
   };
 
@@ -326,8 +376,11 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         for (int kb = 0; kb < p.num_kb;) {
           if (!ptx::paced::mbar_wait_s(empty0 + 8 * s, ph, abort_flag)) { ok = false; break; }
           const int end = min(kb + p.blocks, p.num_kb);
-          if (is_w && cta == 0) ptx::mbar_expect_tx_s(full0 + 8 * s, tx * (end - kb));
           const uint32_t bar = bar0 + 8 * s;
+          if (is_w && cta == 0) ptx::mbar_expect_tx_s(full0 + 8 * s, tx * (end - kb));
+          // (of a tile with few rows a CTA may have none to bring; it must not fall behind by a round of the stages, whose phases it
+          // tells apart by their parity alone)
+          if (!is_w) ptx::mbar_arrive_cluster(bar);
           uint32_t to = st + s * p.blocks * p.block_bytes;
           for (; kb < end; ++kb, to += p.block_bytes) {
             const int k0 = kb * kPerKb;
@@ -407,7 +460,7 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       const uint32_t acc = tmem_base + a * kTile + ep.lane_sel;
       if (et.rows > 0) {
         constexpr int kParts = kForm == kGated ? 2 : 1;
-        const int units = min(et.features, et.limit - et.j0);     // columns that exist
+        const int units = et.limit - et.j0;     // columns that exist
         uint32_t v[2][kParts][16];
         auto load = [&](int c, int b) {
           __syncwarp();
@@ -415,21 +468,30 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
           for (int part = 0; part < kParts; ++part) ptx::tmem_ld_32x16(acc + part * et.features + 16 * c, v[b][part]);
         };
         auto store = [&](int c, int b) { ep.store(et, c, v[b][0], v[b][kParts - 1]); };
-        // the next columns are on their way while these are stored
         auto wait = [&](int b) {
           if (kParts == 2) ptx::tmem_wait_ld(v[b][0], v[b][kParts - 1]);
           else ptx::tmem_wait_ld(v[b][0]);
         };
-        if (16 * ep.side < units) load(ep.side, 0);
+        if (kParts == 2) {             // the next columns are on their way while these are stored
+          if (16 * ep.side < units) load(ep.side, 0);
 #pragma unroll 1
-        for (int c = ep.side; 16 * c < units; c += 4) {
-          wait(0);
-          if (16 * (c + 2) < units) load(c + 2, 1);
-          store(c, 0);
-          if (16 * (c + 2) >= units) break;
-          wait(1);
-          if (16 * (c + 4) < units) load(c + 4, 0);
-          store(c + 2, 1);
+          for (int c = ep.side; 16 * c < units; c += 4) {
+            wait(0);
+            if (16 * (c + 2) < units) load(c + 2, 1);
+            store(c, 0);
+            if (16 * (c + 2) >= units) break;
+            wait(1);
+            if (16 * (c + 4) < units) load(c + 4, 0);
+            store(c + 2, 1);
+          }
+        } else {                       // twice as many at once
+#pragma unroll 1
+          for (int c = ep.side; 16 * c < units; c += 4) {
+            load(c, 0);
+            load(c + 2, 1);            // (a tile's columns are there, whether or not they exist in D)
+            ptx::tmem_wait_ld(v[0][0], v[1][0]);
+            ep.store_two(et, c, v[0][0], v[1][0]);
+          }
         }
       }
       __syncwarp();

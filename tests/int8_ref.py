@@ -5,11 +5,12 @@ LEAST = 1e-10
 
 
 def quant_rows(v):
-    """Codes and scales of rows by the definition, in fp32 with IEEE divisions (on the CPU)."""
+    """Codes and scales of rows by the definition: fp32 quotients (IEEE: on the CPU), the product unrounded (64 bits hold it)."""
     v = v.float().cpu()
     amax = v.abs().amax(dim=-1) if v.shape[-1] else v.new_zeros(v.shape[:-1])
-    scale = torch.maximum(amax, torch.tensor(LEAST)) / torch.tensor(127.0)
-    return torch.round(v / scale[..., None]).clamp(-127, 127).to(torch.int8), scale
+    amax = torch.maximum(amax, torch.tensor(LEAST))
+    inv = torch.tensor(127.0) / amax
+    return torch.round(v.double() * inv.double()[..., None]).to(torch.int8), amax / torch.tensor(127.0)
 
 
 def linear(q, qs, w, ws, bias=None):

@@ -299,6 +299,17 @@ int b200moe_remap_quant_fp8(const void* hidden, b200moe_dtype dtype,
                             int total_experts, int local_experts,
                             void* workspace, size_t workspace_bytes,
                             b200moe_stream stream);
+/* The same with int8 codes [T*K,H] and one fp32 scale a row [T*K] (b200moe_quant_int8_rows) instead of fp8;
+ * hidden_size a multiple of 8. */
+int b200moe_remap_quant_int8(const void* hidden, b200moe_dtype dtype,
+                             int8_t* remapped_q, float* remapped_scales,
+                             const int32_t* expert_map,
+                             int32_t* rows_per_expert, int32_t* row_map,
+                             const void* topk_ids, b200moe_dtype ids_dtype,
+                             int64_t num_rows, int hidden_size, int topk,
+                             int total_experts, int local_experts,
+                             void* workspace, size_t workspace_bytes,
+                             b200moe_stream stream);
 /* The same with MXFP8 planes (b200moe_quant_mxfp8) instead of fp8: codes
  * [planes][T*K,H], scale words [planes][ceil(H/128)][T*K]; with block_sums
  * fp32 sums [ceil(H/128)][T*K] follow the words (values, `planes` and order of the

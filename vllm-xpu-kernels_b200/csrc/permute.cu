@@ -20,6 +20,7 @@
 
 #include "common.cuh"
 #include "mx_quant.cuh"
+#include "quant_int8.cuh"
 #include "sort.cuh"
 
 namespace b200moe {
@@ -27,12 +28,12 @@ namespace {
 
 // ------------------------- row copies ------------------------------------------
 // One block per token: its row is read once and written to its K destinations (`dest` in shared
-// memory, negative = none), as it is, quantised to e4m3 per 1x128 group, or as MXFP8 planes.
+// memory, negative = none), as it is, quantised to e4m3 per 1x128 group, as MXFP8 planes, or as int8 codes.
 struct RowJob {
   const void* src;
   void* dst;
   const void* src_s;     // copy: the caller's scale rows, or null
-  void* dst_s;           // copy: their destination; fp8: fp32 [rows, H/128]; mx: words [planes][ceil(H/128)][rows]
+  void* dst_s;           // copy: their destination; fp8: fp32 [rows, H/128]; mx: words [planes][ceil(H/128)][rows]; int8: fp32 [rows]
   int row_bytes;         // copy
   int scale_row_bytes;   // copy
   int H;                 // quantised forms: values per row
@@ -138,15 +139,28 @@ __device__ __forceinline__ void quant_piece_mx(const RowJob& a, int j, bool in, 
   }
 }
 
-enum RowForm { kRowCopy = 0, kRowFp8 = 1, kRowMx = 2 };
-// Piece j (16 bytes of the source row; `v` is read only for j < nvec) to its destinations.
+enum RowForm { kRowCopy = 0, kRowFp8 = 1, kRowMx = 2, kRowInt8 = 3 };
+// Piece j (16 bytes of the source row; `v` is read only for j < nvec) to its destinations.  `s`: int8, the row's scale.
 template <typename T, int kForm>
-__device__ __forceinline__ void place_piece(const RowJob& a, int j, int nvec, const vec16& v, const int* dest) {
+__device__ __forceinline__ void place_piece(const RowJob& a, int j, int nvec, const vec16& v, const int* dest,
+                                            const Int8Scale& s = Int8Scale()) {
   if (kForm == kRowCopy) {
     if (j >= nvec) return;
     for (int k = 0; k < a.K; ++k) {
       const int r = dest[k];
       if (r >= 0) st16(reinterpret_cast<uint8_t*>(a.dst) + (int64_t)r * a.row_bytes + (int64_t)j * 16, v);
+    }
+  } else if constexpr (kForm == kRowInt8) {
+    if (j >= nvec) return;
+    float y[8];
+    unpack(v, y, T());
+    uint32_t w[2];
+    s.codes(y, w);
+    for (int k = 0; k < a.K; ++k) {
+      const int r = dest[k];
+      if (r < 0) continue;
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.dst) + (int64_t)r * a.H + (int64_t)j * 8) = make_uint2(w[0], w[1]);
+      if (j == 0) reinterpret_cast<float*>(a.dst_s)[r] = s.scale;
     }
   } else if (kForm == kRowFp8) {
     quant_piece_fp8<T>(a, j, j < nvec, v, dest);
@@ -155,7 +169,7 @@ __device__ __forceinline__ void place_piece(const RowJob& a, int j, int nvec, co
   }
 }
 template <typename T, int kForm>
-__device__ __forceinline__ void place_row(const RowJob& a, int64_t tok, const int* dest) {
+__device__ __forceinline__ void place_row(const RowJob& a, int64_t tok, const int* dest, const Int8Scale& s = Int8Scale()) {
   const int nvec = kForm == kRowCopy ? a.row_bytes >> 4 : a.H / 8;
   const int steps = kForm == kRowMx ? ((a.H + 127) / 128) * 16 : nvec;
   const uint8_t* src = reinterpret_cast<const uint8_t*>(a.src) + tok * (int64_t)nvec * 16;
@@ -164,7 +178,7 @@ __device__ __forceinline__ void place_row(const RowJob& a, int64_t tok, const in
     const int j = j0 + (threadIdx.x & 31);
     vec16 v;
     if (j < nvec) v = ld16(src + (int64_t)j * 16);
-    place_piece<T, kForm>(a, j, nvec, v, dest);
+    place_piece<T, kForm>(a, j, nvec, v, dest, s);
   }
   if (kForm == kRowCopy) copy_scales(a, tok, dest);
 }
@@ -177,6 +191,30 @@ remap_rows_kernel(const RowJob a, const int32_t* __restrict__ row_map) {
   __shared__ int dest[32];
   const int64_t tok = blockIdx.x;
   if (threadIdx.x < a.K) dest[threadIdx.x] = row_map[tok * a.K + threadIdx.x];
+  if constexpr (kForm == kRowInt8) {
+    // the row's largest magnitude; up to two pieces a thread stay between that and the codes
+    __shared__ float most[8];
+    const int nvec = a.H / 8;
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(a.src) + tok * (int64_t)nvec * 16;
+    vec16 held[2];
+    uint32_t m = 0;
+    for (int j = threadIdx.x, i = 0; j < nvec; j += 256, ++i) {
+      const vec16 v = ld16(src + (int64_t)j * 16);
+      if (i < 2) held[i & 1] = v;
+      m = largest(v, m, T());
+    }
+    const float amax = warp_largest(largest_of(m, T()));
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = amax;
+    __syncthreads();
+    const Int8Scale s(warp_largest(most[threadIdx.x & 7]));
+    if (nvec <= 512) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) place_piece<T, kForm>(a, threadIdx.x + 256 * i, nvec, held[i], dest, s);
+    } else {
+      place_row<T, kForm>(a, tok, dest, s);
+    }
+    return;
+  }
   __syncthreads();
   place_row<T, kForm>(a, tok, dest);
 }
@@ -204,6 +242,7 @@ remap_small_kernel(const Id* __restrict__ ids, const int32_t* __restrict__ map, 
   __shared__ int dest[kSmallK];
   __shared__ uint32_t part[kSmallThreads / 32][kSmallK / 2];
   __shared__ int hist[kMaxBuckets];
+  __shared__ float most[kForm == kRowInt8 ? kSmallThreads / 32 : 1];
   pdl_trigger();
   pdl_wait();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, K = a.K;
@@ -249,6 +288,15 @@ remap_small_kernel(const Id* __restrict__ ids, const int32_t* __restrict__ map, 
     cnt[k] = __reduce_add_sync(0xffffffffu, cnt[k]);
     if (lane == 0) part[warp][k] = cnt[k];
   }
+  if constexpr (kForm == kRowInt8) {   // the row's largest magnitude, before the same barrier
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kSmallPre; ++i)
+      if (t + kSmallThreads * i < nvec) m = largest(pre[i], m, T());
+    for (int j = t + kSmallThreads * kSmallPre; j < nvec; j += kSmallThreads) m = largest(ld16(src + (int64_t)j * 16), m, T());
+    const float amax = warp_largest(largest_of(m, T()));
+    if (lane == 0) most[warp] = amax;
+  }
   __syncthreads();
   if (t < K) {
     uint32_t sum = 0;
@@ -260,13 +308,15 @@ remap_small_kernel(const Id* __restrict__ ids, const int32_t* __restrict__ map, 
   }
   __syncthreads();
   const int steps = kForm == kRowMx ? ((a.H + 127) / 128) * 16 : nvec;
+  Int8Scale s;
+  if constexpr (kForm == kRowInt8) s = Int8Scale(warp_largest(most[lane & (kSmallThreads / 32 - 1)]));
   if (steps <= kSmallThreads * kSmallPre) {
 #pragma unroll
     for (int i = 0; i < kSmallPre; ++i)
-      if ((t & ~31) + kSmallThreads * i < steps) place_piece<T, kForm>(a, t + kSmallThreads * i, nvec, pre[i], dest);
+      if ((t & ~31) + kSmallThreads * i < steps) place_piece<T, kForm>(a, t + kSmallThreads * i, nvec, pre[i], dest, s);
     if (kForm == kRowCopy) copy_scales(a, tok, dest);
   } else {
-    place_row<T, kForm>(a, tok, dest);
+    place_row<T, kForm>(a, tok, dest, s);
   }
 }
 
@@ -693,6 +743,27 @@ extern "C" int b200moe_remap_quant_fp8(
   RowJob job = {};
   job.src = hidden; job.dst = remapped_q; job.dst_s = remapped_scales; job.H = hidden_size; job.K = topk;
   auto run = dtype == B200MOE_BF16 ? remap_rows<__nv_bfloat16, kRowFp8> : remap_rows<__half, kRowFp8>;
+  return run(p, job, rows_per_expert, row_map, num_rows, workspace, workspace_bytes, as_stream(stream));
+}
+
+extern "C" int b200moe_remap_quant_int8(
+    const void* hidden, b200moe_dtype dtype, int8_t* remapped_q, float* remapped_scales,
+    const int32_t* expert_map, int32_t* rows_per_expert, int32_t* row_map,
+    const void* topk_ids, b200moe_dtype ids_dtype, int64_t num_rows, int hidden_size,
+    int topk, int total_experts, int local_experts, void* workspace,
+    size_t workspace_bytes, b200moe_stream stream) {
+  B200_CHECK_ARG(dtype == B200MOE_BF16 || dtype == B200MOE_F16,
+                 "remap_quant_int8: activations must be bfloat16 or float16");
+  B200_CHECK_ARG(num_rows >= 0 && hidden_size > 0 && hidden_size % 8 == 0, "remap_quant_int8: hidden_size must be a multiple of 8");
+  SortParams p;
+  if (int rc = remap_params(p, expert_map, rows_per_expert, row_map, topk_ids, ids_dtype, num_rows, topk,
+                            total_experts, local_experts)) return rc;
+  B200_CHECK_ARG(num_rows == 0 || (hidden && remapped_q && remapped_scales), "remap_quant_int8: null pointer");
+  B200_CHECK_ARG(((uintptr_t)hidden & 15) == 0 && ((uintptr_t)remapped_q & 7) == 0,
+                 "remap_quant_int8: buffers must be 16-byte aligned");
+  RowJob job = {};
+  job.src = hidden; job.dst = remapped_q; job.dst_s = remapped_scales; job.H = hidden_size; job.K = topk;
+  auto run = dtype == B200MOE_BF16 ? remap_rows<__nv_bfloat16, kRowInt8> : remap_rows<__half, kRowInt8>;
   return run(p, job, rows_per_expert, row_map, num_rows, workspace, workspace_bytes, as_stream(stream));
 }
 

@@ -49,52 +49,6 @@ __device__ __forceinline__ float row_max(float amax, int threads, float* part) {
   return amax;
 }
 
-// The values of 16 bytes.  (16-bit types two at a time: a conversion of a bfloat16 by itself is an instruction of a slow unit.)
-__device__ __forceinline__ void unpack(const vec16& a, float (&v)[4], float) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(a.w[i]);
-}
-__device__ __forceinline__ void unpack(const vec16& a, float (&v)[8], __nv_bfloat16) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(a.w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(a.w[i] & 0xffff0000u);
-  }
-}
-__device__ __forceinline__ void unpack(const vec16& a, float (&v)[8], __half) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a.w[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-// The largest magnitude of 16 bytes and `most`, which begins as zero bits: two 16-bit values, or a float.
-__device__ __forceinline__ uint32_t largest(const vec16& a, uint32_t most, float) {
-  float m = __uint_as_float(most);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m = max_nan(m, fabsf(__uint_as_float(a.w[i])));
-  return __float_as_uint(m);
-}
-template <typename P>
-__device__ __forceinline__ uint32_t largest_pair(const vec16& a, uint32_t most) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t x = a.w[i] & 0x7fff7fffu;
-    const P m = __hmax2_nan(*reinterpret_cast<const P*>(&most), *reinterpret_cast<const P*>(&x));
-    most = *reinterpret_cast<const uint32_t*>(&m);
-  }
-  return most;
-}
-__device__ __forceinline__ uint32_t largest(const vec16& a, uint32_t most, __nv_bfloat16) { return largest_pair<__nv_bfloat162>(a, most); }
-__device__ __forceinline__ uint32_t largest(const vec16& a, uint32_t most, __half) { return largest_pair<__half2>(a, most); }
-__device__ __forceinline__ float largest_of(uint32_t most, float) { return __uint_as_float(most); }
-template <typename T>
-__device__ __forceinline__ float largest_of(uint32_t most, T) {
-  const T* m = reinterpret_cast<const T*>(&most);
-  return max_nan(to_f32<T>(m[0]), to_f32<T>(m[1]));
-}
-
 // Rows whose 16-byte pieces are aligned, P of them a thread (gated: of gates and of ups), which stay in registers between the maximum
 // and the codes: every byte is read once.  Blocks stay, and have the next row on its way while they are at work on one (not gated:
 // registers).  8192 rows of 7168 bfloat16 values 51.7 us with a block a row, .. so.

@@ -14,9 +14,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
+// The largest of a warp's values, in every lane.
+__device__ __forceinline__ float warp_largest(float m) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, off));
+  return m;
+}
+
 // A row that holds a NaN or an infinity gets a scale of NaN, so that every output of the product that it goes into is one.
 struct Int8Scale {
   float scale, inv;
+  Int8Scale() = default;
   __device__ __forceinline__ explicit Int8Scale(float amax) {
     amax = max_nan(amax, 1e-10f);
     scale = amax < INFINITY ? __fdiv_rn(amax, 127.f) : __uint_as_float(0x7fc00000u);
@@ -36,6 +44,52 @@ struct Int8Scale {
     }
   }
 };
+
+// The values of 16 bytes.  (16-bit types two at a time: a conversion of a bfloat16 by itself is an instruction of a slow unit.)
+__device__ __forceinline__ void unpack(const vec16& a, float (&v)[4], float) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(a.w[i]);
+}
+__device__ __forceinline__ void unpack(const vec16& a, float (&v)[8], __nv_bfloat16) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(a.w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(a.w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const vec16& a, float (&v)[8], __half) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a.w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+// The largest magnitude of 16 bytes and `most`, which begins as zero bits: two 16-bit values, or a float.
+__device__ __forceinline__ uint32_t largest(const vec16& a, uint32_t most, float) {
+  float m = __uint_as_float(most);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max_nan(m, fabsf(__uint_as_float(a.w[i])));
+  return __float_as_uint(m);
+}
+template <typename P>
+__device__ __forceinline__ uint32_t largest_pair(const vec16& a, uint32_t most) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = a.w[i] & 0x7fff7fffu;
+    const P m = __hmax2_nan(*reinterpret_cast<const P*>(&most), *reinterpret_cast<const P*>(&x));
+    most = *reinterpret_cast<const uint32_t*>(&m);
+  }
+  return most;
+}
+__device__ __forceinline__ uint32_t largest(const vec16& a, uint32_t most, __nv_bfloat16) { return largest_pair<__nv_bfloat162>(a, most); }
+__device__ __forceinline__ uint32_t largest(const vec16& a, uint32_t most, __half) { return largest_pair<__half2>(a, most); }
+__device__ __forceinline__ float largest_of(uint32_t most, float) { return __uint_as_float(most); }
+template <typename T>
+__device__ __forceinline__ float largest_of(uint32_t most, T) {
+  const T* m = reinterpret_cast<const T*>(&most);
+  return max_nan(to_f32<T>(m[0]), to_f32<T>(m[1]));
+}
 
 }  // namespace
 }  // namespace b200moe

@@ -501,12 +501,10 @@ PyObject* layer_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const size_t sort_bytes = b200moe_sort_workspace_bytes(M, (int)p.experts);
   const size_t sort_at = l.take(sort_bytes);
   const size_t a_at = l.end;
-  size_t as_at = a_at, token_at = a_at, token_s_at = a_at;
+  size_t as_at = a_at;
   if (weights.i8) {
     l.take(M * H);
     as_at = l.take(M * 4);
-    token_at = l.take(T * H);
-    token_s_at = l.take(T * 4);
   } else if (quant_fp8) {
     l.take(M * H);
     as_at = l.take(M * (H / 128) * 4);
@@ -527,12 +525,9 @@ PyObject* layer_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int32_t *rows = (int32_t*)(ws + rows_at), *row_map = (int32_t*)(ws + map_at);
   const int32_t* emap = map.has_value() ? map->data_ptr<int32_t>() : nullptr;
   if (weights.i8) {
-    // a token is quantised once, then copied to its experts' rows
-    check_status(b200moe_quant_int8_rows(x.data_ptr(), float_dtype(x, "hidden_states"), H, (int8_t*)(ws + token_at), H,
-                                         (float*)(ws + token_s_at), T, (int)H, 0, nullptr, 0, st));
-    check_status(b200moe_remap_hidden_states(ws + token_at, ws + token_s_at, ws + a_at, ws + as_at, emap, rows, row_map, ids.data_ptr(),
-                                             index_dtype(ids), T, (int)H, 1, 1, 4, (int)K, (int)p.total_experts, (int)p.experts,
-                                             ws + sort_at, sort_bytes, st));
+    check_status(b200moe_remap_quant_int8(x.data_ptr(), float_dtype(x, "hidden_states"), (int8_t*)(ws + a_at), (float*)(ws + as_at),
+                                          emap, rows, row_map, ids.data_ptr(), index_dtype(ids), T, (int)H, (int)K,
+                                          (int)p.total_experts, (int)p.experts, ws + sort_at, sort_bytes, st));
   } else if (quant_fp8)
     check_status(b200moe_remap_quant_fp8(x.data_ptr(), float_dtype(x, "b200_remap_quant_fp8"), ws + a_at,
                                          (float*)(ws + as_at), emap, rows, row_map, ids.data_ptr(), index_dtype(ids), T,

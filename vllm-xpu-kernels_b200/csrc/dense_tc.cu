@@ -105,12 +105,12 @@ __device__ __forceinline__ void locate_grouped(const TcDense& p, const TileWalk&
     cursor = hi;
   }
   const int local = t - w.tile_start[cursor], row = w.row_start[cursor], rows = w.row_start[cursor + 1] - row;
-  const int m_tiles = (rows + kTile - 1) / kTile;
+  const int height = tile_rows(p), m_tiles = rows <= height ? 1 : (rows + height - 1) / height;
   ti.e = w.expert[cursor];
   ti.n_tile = m_tiles == 1 ? local : local / m_tiles;
   ti.m_tile = local - ti.n_tile * m_tiles;
-  ti.row0 = row + ti.m_tile * kTile;
-  ti.valid = min(rows - ti.m_tile * kTile, kTile);
+  ti.row0 = row + ti.m_tile * height;
+  ti.valid = min(rows - ti.m_tile * height, height);
 }
 
 // A warp's 32 rows x 16 columns, a row a lane, of which the first `rows` rows and the columns below `limit` exist: in pieces of 32 or
@@ -305,7 +305,11 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
 
   if (warp == 0) {
     pdl_wait();
-    if (grouped) build_tile_walk<kTile>(p.rows_per_expert, p.experts, p.n_tiles, ctrl->walk);
+    if (grouped) {
+      if (p.half_rows == 32) build_tile_walk<64>(p.rows_per_expert, p.experts, p.n_tiles, ctrl->walk);
+      else if (p.half_rows == 64) build_tile_walk<128>(p.rows_per_expert, p.experts, p.n_tiles, ctrl->walk);
+      else build_tile_walk<kTile>(p.rows_per_expert, p.experts, p.n_tiles, ctrl->walk);
+    }
     if (lane == 0) {
       ptx::prefetch_tensormap(&tmap_x);
       ptx::prefetch_tensormap(&tmap_w);
@@ -628,10 +632,6 @@ int dense_tc(const DenseJob& j, cudaStream_t st) {
   p.m = j.m; p.d_stride = j.d_stride; p.n = j.n; p.experts = j.experts;
   const int per_kb = j.type == kDenseI8 ? 128 : 64, n_out = j.gated ? j.n / 2 : j.n;
   p.num_kb = (j.k + per_kb - 1) / per_kb;
-  // Rows of a tile (one set of weights): 256, fewer for fewer.  (The tensor cores always take 128 a CTA: those behind a CTA's own make
-  // sums of whatever follows in shared memory, which nobody reads.)
-  p.half_rows = j.rows_per_expert != nullptr || j.m > 128 ? 128 : j.m > 64 ? 64 : 32;
-  p.m_tiles = (int)((j.m + 2 * p.half_rows - 1) / (2 * p.half_rows));
   p.d_dtype = j.d_dtype; p.bias_f16 = j.bias_f16; p.clamp = j.clamp;
   const int out_size = dtype_bytes(j.d_dtype);
   p.d_wide = store_width(j.d, j.d_stride * out_size, (int64_t)n_out * out_size);
@@ -640,12 +640,17 @@ int dense_tc(const DenseJob& j, cudaStream_t st) {
   const bool grouped = j.rows_per_expert != nullptr;
   const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m, each = (rows + j.experts - 1) / j.experts;
   const int64_t sets = grouped ? std::min<int64_t>(j.experts, rows) : 1;
-  p.x_box = grouped ? (each <= 96 ? 32 : 128) : p.half_rows;
+  // Rows of a tile: 256, fewer for fewer, which leaves more room for weights on their way (routing is never even, so sets of rows get
+  // some headroom).  The tensor cores always take 128 rows a CTA: those behind a CTA's own make sums of whatever follows in
+  // shared memory, which nobody reads.
+  p.half_rows = each > (grouped ? 96 : 128) ? 128 : each > (grouped ? 40 : 64) ? 64 : 32;
+  p.m_tiles = (int)((j.m + 2 * p.half_rows - 1) / (2 * p.half_rows));
+  p.x_box = grouped ? 32 : p.half_rows;
   auto run = [&](auto kernel) {
     using K = decltype(kernel);
     if (K::pairs() == 0) return dense_rows(j, st);   // no clusters on this device
     const int64_t pairs = j.max_ctas > 0 ? std::min(K::pairs(), std::max(1, j.max_ctas / 2)) : K::pairs();
-    choose_tile(p, sets, grouped ? (each + kTile - 1) / kTile : p.m_tiles, n_out, j.gated, false, pairs,
+    choose_tile(p, sets, grouped ? (each + 2 * p.half_rows - 1) / (2 * p.half_rows) : p.m_tiles, n_out, j.gated, false, pairs,
                 sets * j.n * (int64_t)j.k * (j.type == kDenseI8 ? 1 : 2));
     set_width(p, j.type, false, false, n_out, j.gated);
     CUtensorMap tx, tw;

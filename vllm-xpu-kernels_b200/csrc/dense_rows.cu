@@ -328,7 +328,7 @@ int launch(RowsParams& p, cudaStream_t st) {
   const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m;
   const int64_t tiles = j.rows_per_expert != nullptr ? (rows / BT + std::min<int64_t>(rows, j.experts)) * p.f_tiles
                                                      : (int64_t)p.t_tiles * p.f_tiles;
-  const int64_t blocks = (j.max_ctas > 0 ? std::min(j.max_ctas, sm_count()) : sm_count()) * 2;
+  const int64_t blocks = j.max_ctas > 0 ? std::min(j.max_ctas, 2 * sm_count()) : 2 * sm_count();
   // Warps of a team: rounds of tiles times the units of a warp, and as much as kTileCost units for what a tile costs besides.
   constexpr int kTileCost = 4;
   int64_t best = -1;

@@ -51,8 +51,8 @@ struct TcDense {
   int width;                // weight rows of a tile: a multiple of 32, gated of 64
   int half_rows;            // rows of X that a CTA has of a tile: 32, 64 or 128 (in tensor memory they are the first of 128)
   int stages, blocks;       // of the ring; K blocks of a stage: 1 or 2
-  int block_bytes, x_bytes, w_bytes;   // of a K block, its X and its W
-  int x_box;                // rows that a load of X brings
+  int x_bytes, w_bytes;     // of a K block
+  int stage_bytes;          // X of its blocks, then their W
   uint32_t idesc;
   b200moe_dtype d_dtype;
   int bias_f16;
@@ -289,8 +289,9 @@ struct Epilogue {
   }
 };
 
+// kWide: a load brings all K blocks of a stage (rows of whole blocks).
 // kXMn, kWMn: the operand is stored by column (its rows' index is the dense one): 16-bit types, two boxes of 64 rows x 64 k.
-template <bool kI8, int kForm, bool kXMn, bool kWMn>
+template <bool kI8, int kForm, bool kXMn, bool kWMn, bool kWide>
 __global__ void __launch_bounds__(kThreads, 1)
 dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const TcDense p) {
   constexpr int kPerKb = kI8 ? 128 : 64;
@@ -349,58 +350,79 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
     else locate_dense(p, t, ti);
   };
 
-  if (warp == 0 || warp == 2 + kEpi) {
-    // ------------------------------ TMA producers -----------------------------
-    // W by the one, X by the other: a load costs its thread some 100 cycles, a K block of a tile with few rows hardly more
-    // in the tensor cores.
-    const bool is_w = warp == 0;
+  if (warp == 0) {
+    // ------------------------------ TMA producer of W -------------------------
     if (ptx::elect_one()) {
       uint32_t s = 0, ph = 1;
       bool ok = true;
       const uint32_t full0 = ptx::smem_u32(&ctrl->full[0]), empty0 = ptx::smem_u32(&ctrl->empty[0]);
       const uint32_t bar0 = ptx::map_to_cta(full0, 0);   // the even CTA's barriers count the bytes of both CTAs
-      const uint32_t st = ptx::smem_u32(smem);
-      auto first_row = [&](const TileInfo& ti) {   // of W, of this CTA
-        return kForm == kGated ? (cta == 0 ? 0 : half) + ti.n_tile * (p.width >> 1) : ti.n_tile * p.width + (int)cta * (p.width >> 1);
-      };
+      const uint32_t st = ptx::smem_u32(smem) + p.blocks * p.x_bytes;
       for (int t = walker; t < total && ok; t += walkers) {
         TileInfo ti;
         locate(t, ti);
-        // rows past the end are filled with zeros
-        const int row = ti.row0 + (int)cta * p.half_rows;
-        const int n0 = first_row(ti);
-        // loads of X in either CTA: as many as the tile's rows take
-        auto boxes = [&](int c) {
-          const int rows = min(max(ti.valid - p.half_rows * c, 0), p.half_rows);
-          return kXMn ? 2 : (rows + p.x_box - 1) / p.x_box;
-        };
-        const int mine = boxes((int)cta);
-        const uint32_t box_bytes = kXMn ? kOperand / 2 : p.x_box * 128;
-        const uint32_t tx = 2 * p.w_bytes + (boxes(0) + boxes(1)) * box_bytes;
+        // (rows past the end are filled with zeros)
+        const int n0 = kForm == kGated ? (cta == 0 ? 0 : half) + ti.n_tile * (p.width >> 1) : ti.n_tile * p.width + (int)cta * (p.width >> 1);
+        const uint32_t tx = 2 * p.w_bytes + ((ti.valid > 0) + (ti.valid > p.half_rows)) * p.x_bytes;
         for (int kb = 0; kb < p.num_kb;) {
           if (!ptx::paced::mbar_wait_s(empty0 + 8 * s, ph, abort_flag)) { ok = false; break; }
-          const int end = min(kb + p.blocks, p.num_kb);
           const uint32_t bar = bar0 + 8 * s;
-          if (is_w && cta == 0) ptx::mbar_expect_tx_s(full0 + 8 * s, tx * (end - kb));
-          // (of a tile with few rows a CTA may have none to bring; it must not fall behind by a round of the stages, whose phases it
-          // tells apart by their parity alone)
-          if (!is_w) ptx::mbar_arrive_cluster(bar);
-          uint32_t to = st + s * p.blocks * p.block_bytes;
-          for (; kb < end; ++kb, to += p.block_bytes) {
-            const int k0 = kb * kPerKb;
-            const uint32_t w_to = to + p.x_bytes;
-            if (!is_w) {
-              if (kXMn) {
-                ptx::tma_load_2d_pair(to, &tmap_x, bar, row, k0);
-                ptx::tma_load_2d_pair(to + kOperand / 2, &tmap_x, bar, row + 64, k0);
+          uint32_t to = st + s * p.stage_bytes;
+          if (kWide) {   // (blocks past the end are zeros)
+            if (cta == 0) ptx::mbar_expect_tx_s(full0 + 8 * s, tx * p.blocks);
+            ptx::tma_load_4d_pair(to, &tmap_w, bar, 0, n0, kb, ti.e);
+            kb += p.blocks;
+          } else {
+            const int end = min(kb + p.blocks, p.num_kb);
+            if (cta == 0) ptx::mbar_expect_tx_s(full0 + 8 * s, tx * (end - kb));
+            for (; kb < end; ++kb, to += p.w_bytes) {
+              const int k0 = kb * kPerKb;
+              if (kWMn) {
+                ptx::tma_load_3d_pair(to, &tmap_w, bar, n0, k0, ti.e);
+                if (p.w_bytes > kOperand / 2) ptx::tma_load_3d_pair(to + kOperand / 2, &tmap_w, bar, n0 + 64, k0, ti.e);
               } else {
-                for (int b = 0; b < mine; ++b) ptx::tma_load_2d_pair(to + b * box_bytes, &tmap_x, bar, k0, row + b * p.x_box);
+                ptx::tma_load_3d_pair(to, &tmap_w, bar, k0, n0, ti.e);
               }
-            } else if (kWMn) {
-              ptx::tma_load_3d_pair(w_to, &tmap_w, bar, n0, k0, ti.e);
-              if (p.w_bytes > kOperand / 2) ptx::tma_load_3d_pair(w_to + kOperand / 2, &tmap_w, bar, n0 + 64, k0, ti.e);
-            } else {
-              ptx::tma_load_3d_pair(w_to, &tmap_w, bar, k0, n0, ti.e);
+            }
+          }
+          if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2 + kEpi) {
+    // ------------------------------ TMA producer of X -------------------------
+    // (A thread of its own: a load costs some 100 cycles, a K block of a narrow tile hardly more in the tensor cores.)
+    if (ptx::elect_one()) {
+      uint32_t s = 0, ph = 1;
+      bool ok = true;
+      const uint32_t empty0 = ptx::smem_u32(&ctrl->empty[0]), bar0 = ptx::map_to_cta(ptx::smem_u32(&ctrl->full[0]), 0);
+      const uint32_t st = ptx::smem_u32(smem);
+      for (int t = walker; t < total && ok; t += walkers) {
+        TileInfo ti;
+        locate(t, ti);
+        const int row = ti.row0 + (int)cta * p.half_rows;
+        const bool mine = ti.valid > (int)cta * p.half_rows;    // (of a tile with few rows a CTA may have none)
+        for (int kb = 0; kb < p.num_kb;) {
+          if (!ptx::paced::mbar_wait_s(empty0 + 8 * s, ph, abort_flag)) { ok = false; break; }
+          const uint32_t bar = bar0 + 8 * s;
+          // An arrival besides the bytes, which a CTA may have none of: a producer must not fall behind by a round of the
+          // stages, whose phases it tells apart by their parity alone.
+          ptx::mbar_arrive_cluster(bar);
+          uint32_t to = st + s * p.stage_bytes;
+          if (kWide) {
+            if (mine) ptx::tma_load_3d_pair(to, &tmap_x, bar, 0, row, kb);
+            kb += p.blocks;
+          } else {
+            const int end = min(kb + p.blocks, p.num_kb);
+            for (; kb < end; ++kb, to += p.x_bytes) {
+              if (!mine) continue;
+              if (kXMn) {
+                ptx::tma_load_2d_pair(to, &tmap_x, bar, row, kb * kPerKb);
+                ptx::tma_load_2d_pair(to + kOperand / 2, &tmap_x, bar, row + 64, kb * kPerKb);
+              } else {
+                ptx::tma_load_2d_pair(to, &tmap_x, bar, kb * kPerKb, row);
+              }
             }
           }
           if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; }
@@ -418,8 +440,8 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       // 16-byte units between the K steps of an operand: 32 bytes of its rows, or 16 of the k that are its rows
       constexpr int kXStep = kXMn ? 2048 / 16 : 2, kWStep = kWMn ? 2048 / 16 : 2;
       const uint64_t xdesc0 = ptx::make_smem_desc(ptx::smem_u32(smem), kXMn ? 8192u : 16u, 1024);
-      const uint64_t wdesc0 = ptx::make_smem_desc(ptx::smem_u32(smem) + p.x_bytes, kWMn ? 8192u : 16u, 1024);
-      const uint64_t block16 = p.block_bytes >> 4, stage16 = p.blocks * block16;
+      const uint64_t wdesc0 = ptx::make_smem_desc(ptx::smem_u32(smem) + p.blocks * p.x_bytes, kWMn ? 8192u : 16u, 1024);
+      const uint64_t x16 = p.x_bytes >> 4, w16 = p.w_bytes >> 4, stage16 = p.stage_bytes >> 4;
       uint64_t at = 0;     // of the stage, from the first one's descriptors
       for (int t = walker; t < total && ok; t += walkers) {
         const uint32_t a = acc_it & 1;
@@ -429,9 +451,8 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
           if (!ptx::mbar_wait_s(full0 + 8 * s, ph, abort_flag)) { ok = false; break; }
           ptx::tc_fence_after();
           const int end = min(kb + p.blocks, p.num_kb);
-          for (uint64_t d = at; kb < end; ++kb, d += block16) {
-            ptx::umma_pair_block<kI8, kXStep, kWStep>(tmem_base + a * kTile, xdesc0 + d, wdesc0 + d, p.idesc, kb > 0 ? 1u : 0u);
-          }
+          for (uint64_t x = xdesc0 + at, w = wdesc0 + at; kb < end; ++kb, x += x16, w += w16)
+            ptx::umma_pair_block<kI8, kXStep, kWStep>(tmem_base + a * kTile, x, w, p.idesc, kb > 0 ? 1u : 0u);
           ptx::umma_commit_pair(empty0 + 8 * s);
           at += stage16;
           if (++s == (uint32_t)p.stages) { s = 0; ph ^= 1; at = 0; }
@@ -521,9 +542,10 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   if (tid == 0 && *abort_flag != 0) report_timeout(p.status);
 }
 
-template <bool kI8, int kForm, bool kXMn, bool kWMn>
+template <bool kI8, int kForm, bool kXMn, bool kWMn, bool kWide>
 struct Kernel {
-  static constexpr auto kern = dense_tc_kernel<kI8, kForm, kXMn, kWMn>;
+  static constexpr bool wide = kWide;
+  static constexpr auto kern = dense_tc_kernel<kI8, kForm, kXMn, kWMn, kWide>;
   // How many pairs the device runs at once; 0 if none (a partition with too few SMs per GPC, say).
   static int pairs() {
     static std::atomic<int> cached[kMaxDevices];
@@ -571,7 +593,7 @@ CUtensorMapDataType map_type(DenseType t) {
                        : t == kDenseBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
 // An operand of `rows` rows of k (mn: stored by column, k rows of `rows`), `stride` elements from one stored row to the next;
-// a load brings 128 bytes of `box` stored rows.
+// a load brings 128 bytes of `box_rows` stored rows.
 int operand_map(CUtensorMap* map, DenseType t, const void* base, int64_t rows, int64_t k, int64_t stride, bool mn, int experts, int box_rows) {
   const int size = t == kDenseI8 ? 1 : 2;
   const int64_t inner = mn ? rows : k, outer = mn ? k : rows;
@@ -580,10 +602,20 @@ int operand_map(CUtensorMap* map, DenseType t, const void* base, int64_t rows, i
   const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
   return encode_map(map, map_type(t), experts > 0 ? 3 : 2, base, dims, strides, box);
 }
-// K blocks of a stage: as many as leave four stages.  A wait, and what goes with it (the producers' arrivals, the issuer's commit to both
-// CTAs), takes either single thread some 360 cycles, a load or a block's products 50 to 100.  64 x 7168 x 2048 gated, tiles of 64
-// weight rows, 1 / 2 / 3 / 4 / 6 blocks of 8 KB a stage 33.9 / 24.6 / 21.5 / 20.0 / 18.7 us; 256 rows (20 KB) 34.1 / 25.3 / 25.2 / 29.7 / 45.7.
-int stage_blocks(int block_bytes) { return std::max(1, std::min(6, kRing / (4 * block_bytes))); }
+// The same with the 128-byte blocks of a row as a dimension of their own, of which a load brings `blocks`: [128 bytes, rows, k / 128
+// bytes] and, with experts, [.., experts].  Rows are whole blocks.
+int wide_map(CUtensorMap* map, DenseType t, const void* base, int64_t rows, int64_t k, int64_t stride, int experts, int box_rows, int blocks) {
+  const int size = t == kDenseI8 ? 1 : 2, inner = 128 / size;
+  const cuuint64_t dims[4] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)(k / inner), (cuuint64_t)std::max(experts, 1)};
+  const cuuint64_t strides[3] = {(cuuint64_t)(stride * size), 128, (cuuint64_t)(stride * size * rows)};
+  const cuuint32_t box[4] = {(cuuint32_t)inner, (cuuint32_t)box_rows, (cuuint32_t)blocks, 1};
+  return encode_map(map, map_type(t), experts > 0 ? 4 : 3, base, dims, strides, box);
+}
+// K blocks of a stage.  A wait, and what goes with it (the producers' arrivals, the issuer's commit to both CTAs), takes either single thread
+// some 360 cycles, a block's products 50 to 100, where the tensor cores have 512 cycles of work with 256 weight rows and 128 with 64.
+// 64 x 7168 x 2048 gated, tiles of 64 weight rows, 1 / 2 / 3 / 4 / 6 blocks a stage 33.9 / 18.7 / 16.2 / 16.2 / 16.3 us, of 128 - / 20.9 / 21.2 /
+// 21.4 / 25.7; 256 rows, tiles of 64 weight rows 34.1 / 24.0 / 24.4 / 28.9 / 42.3.
+int stage_blocks(int width, int block_bytes) { return width == kTile ? 1 : block_bytes <= 8192 ? 3 : 2; }
 
 // Weight rows of a tile: what takes the fewest cycles by this estimate.  A K block of a tile takes 170 cycles and its share of the waits, 2.45 a
 // weight row in the tensor cores, and a cycle for each 60 of its bytes; a tile costs some 2000 besides; and the weights pass HBM at 3440
@@ -596,9 +628,10 @@ void choose_tile(TcDense& p, int64_t sets, int64_t row_tiles, int features, bool
   for (int width = kTile; width >= 64; width -= step) {
     const int out = gated ? width / 2 : width, bytes = p.half_rows * 128 + (w_mn ? (width + 127) / 128 * 8192 : width * 64);
     const int64_t tiles = sets * row_tiles * ((features + out - 1) / out), rounds = (tiles + pairs - 1) / pairs;
-    const double block = std::max({300.0 / stage_blocks(bytes) + 170, 2.45 * width, bytes / 60.0});
+    const double block = std::max({300.0 / stage_blocks(width, bytes) + 170, 2.45 * width, bytes / 60.0});
     const double cost = std::max(rounds * (p.num_kb * block + 2000), w_bytes / 3440.0);
-    if (p.width == 0 || cost < least) { p.width = width; least = cost; }
+    // (a narrower tile that promises little more gave nothing: 64 rows each of 8 experts of 4096 x 28672 175 us with 224, 170 with 256)
+    if (p.width == 0 || cost < 0.94 * least) { p.width = width; least = cost; }
   }
 }
 int store_width(const void* p, int64_t row_bytes, int64_t cols_bytes) {
@@ -617,9 +650,9 @@ void set_width(TcDense& p, DenseType t, bool x_mn, bool w_mn, int features, bool
   p.n_tiles = (features + (gated ? width / 2 : width) - 1) / (gated ? width / 2 : width);
   p.x_bytes = p.half_rows * 128;
   p.w_bytes = w_mn ? (width > 128 ? kOperand : kOperand / 2) : width * 64;
-  p.block_bytes = p.x_bytes + p.w_bytes;
-  p.blocks = stage_blocks(p.block_bytes);
-  p.stages = std::min(kMaxStages, kRing / (p.blocks * p.block_bytes));
+  p.blocks = std::min(p.num_kb, stage_blocks(width, p.x_bytes + p.w_bytes));
+  p.stage_bytes = p.blocks * (p.x_bytes + p.w_bytes);
+  p.stages = std::min(kMaxStages, kRing / p.stage_bytes);
   p.idesc = idesc_of(t, x_mn, w_mn, width);
 }
 
@@ -645,7 +678,6 @@ int dense_tc(const DenseJob& j, cudaStream_t st) {
   // shared memory, which nobody reads.
   p.half_rows = each > (grouped ? 96 : 128) ? 128 : each > (grouped ? 40 : 64) ? 64 : 32;
   p.m_tiles = (int)((j.m + 2 * p.half_rows - 1) / (2 * p.half_rows));
-  p.x_box = grouped ? 32 : p.half_rows;
   auto run = [&](auto kernel) {
     using K = decltype(kernel);
     if (K::pairs() == 0) return dense_rows(j, st);   // no clusters on this device
@@ -654,13 +686,20 @@ int dense_tc(const DenseJob& j, cudaStream_t st) {
                 sets * j.n * (int64_t)j.k * (j.type == kDenseI8 ? 1 : 2));
     set_width(p, j.type, false, false, n_out, j.gated);
     CUtensorMap tx, tw;
-    if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, false, 0, p.x_box)) return rc;
-    if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, false, j.experts, p.width / 2)) return rc;
+    if (K::wide) {
+      if (int rc = wide_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, 0, p.half_rows, p.blocks)) return rc;
+      if (int rc = wide_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, j.experts, p.width / 2, p.blocks)) return rc;
+    } else {
+      if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, false, 0, p.half_rows)) return rc;
+      if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, false, j.experts, p.width / 2)) return rc;
+    }
     const int64_t tiles = (p.m_tiles + (grouped ? (int64_t)j.experts : 0)) * p.n_tiles;
     return K::launch(tx, tw, p, std::min(pairs, tiles), j.early, st);
   };
-  if (j.type != kDenseI8) return run(Kernel<false, kGated, false, false>());
-  return j.gated ? run(Kernel<true, kGated, false, false>()) : run(Kernel<true, kScaled, false, false>());
+  const bool wide = j.k % per_kb == 0;
+  if (j.type != kDenseI8) return wide ? run(Kernel<false, kGated, false, false, true>()) : run(Kernel<false, kGated, false, false, false>());
+  if (j.gated) return wide ? run(Kernel<true, kGated, false, false, true>()) : run(Kernel<true, kGated, false, false, false>());
+  return wide ? run(Kernel<true, kScaled, false, false, true>()) : run(Kernel<true, kScaled, false, false, false>());
 }
 
 int dense_plain(const PlainJob& j, cudaStream_t st) {
@@ -669,7 +708,6 @@ int dense_plain(const PlainJob& j, cudaStream_t st) {
   p.num_kb = (int)((j.k + 63) / 64);
   p.half_rows = j.x_by_column || j.m > 128 ? 128 : j.m > 64 ? 64 : 32;
   p.m_tiles = (int)((j.m + 2 * p.half_rows - 1) / (2 * p.half_rows));
-  p.x_box = p.half_rows;
   p.d_dtype = j.type == kDenseF16 ? B200MOE_F16 : B200MOE_BF16;
   p.d_wide = store_width(j.d, j.d_stride * 2, (int64_t)j.n * 2);
   auto run = [&](auto kernel) {
@@ -678,12 +716,12 @@ int dense_plain(const PlainJob& j, cudaStream_t st) {
     choose_tile(p, 1, p.m_tiles, j.n, false, true, K::pairs(), 0);
     set_width(p, j.type, j.x_by_column, true, j.n, false);
     CUtensorMap tx, tw;
-    if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, j.x_by_column, 0, j.x_by_column ? 64 : p.x_box)) return rc;
+    if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, j.x_by_column, 0, j.x_by_column ? 64 : p.half_rows)) return rc;
     if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, true, 1, 64)) return rc;
     const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
     return K::launch(tx, tw, p, std::min<int64_t>(K::pairs(), tiles), j.early, st);
   };
-  return j.x_by_column ? run(Kernel<false, kPlain, true, true>()) : run(Kernel<false, kPlain, false, true>());
+  return j.x_by_column ? run(Kernel<false, kPlain, true, true, false>()) : run(Kernel<false, kPlain, false, true, false>());
 }
 
 }  // namespace b200moe

@@ -122,7 +122,7 @@ extern "C" int b200moe_int8_linear(const b200moe_int8_linear_args* a, b200moe_st
   j.x = a->x; j.w = a->w; j.x_scale = a->x_scale; j.w_scale = a->w_scale; j.bias = a->bias; j.d = a->d; j.status = a->status;
   j.m = a->rows; j.x_stride = a->x_stride; j.w_stride = a->k; j.d_stride = a->d_stride; j.n = a->n; j.k = a->k; j.experts = 1;
   j.type = kDenseI8; j.d_dtype = a->d_dtype; j.bias_f16 = a->bias_dtype == B200MOE_F16; j.early = a->rows <= kEarlyLaunchRows;
-  return dense(j, as_stream(stream));
+  return j.x_dtype != B200MOE_I8 ? dense_rows(j, as_stream(stream)) : dense(j, as_stream(stream));
 }
 
 extern "C" int b200moe_gated_linear(const b200moe_gated_linear_args* a, b200moe_stream stream) {

@@ -37,18 +37,24 @@ struct DenseJob {
 
 int dense_rows(const DenseJob& j, cudaStream_t st);      // dense_rows.cu
 // Whether dense_rows takes rows of 16 or 32 bits and int8 weights, every block making the codes for itself: up to so many values
-// that takes less time than a kernel of its own.
+// that takes less time than a kernel of its own (1 x 4096 x 4096 5.7 us, 7.2 with two kernels; 4 x 4096 x 4096 6.6 and 7.7; 1 x 4096 x
+// 14336 13.2 and 13.7; 8 x 4096 x 4096 9.8 and 7.5).
 constexpr int kQuantValues = 16384;
 bool dense_rows_quantises(int64_t rows, int k);
 int dense_tc(const DenseJob& j, cudaStream_t st);        // dense_tc.cu
 
-// Rows (an expert) up to which the kernel for a few rows takes a call.  By expert, layer calls, that kernel / the one for many, us:
-// 8 experts of 4096 x 14336, 4 rows 246 / 257, 15 rows 365 / 265; 128 of 2048 x 768, 1 row 86.8 / 88.6, 8 rows 172 / 147; 8 of
-// 2048 x 1408, 4 rows 28.4 / 36.3, 16 rows 39.8 / 36.8.
-constexpr int kDenseFewRows = 16, kGroupedFewRows = 5;
+// Rows (of an expert, on average) up to which the kernel for a few rows takes a call; that kernel / the one for many, us.  By expert, layer
+// calls: 128 experts of 2048 x 768, 8 rows 129 / 139, 12 rows 139 / 141, 16 rows 170 / 142; 8 of 4096 x 14336, 8 rows 265 / 279, 12 rows
+// 288 / 278; 8 of 2048 x 1408, 8 rows 27 / 34, 20 rows 37 / 34.  One set of weights: 16 x 4096 x 4096 5.9 / 7.9, 16 x 7168 x 2048
+// gated 14.4 / 16.0, 20 rows 8.0 / 7.9 and 20.4 / 16.0.  Above 8 rows the tokens take as much of L2's time as the weights, which tells
+// where the weights are many: 12 x 14336 x 2048 9.3 / 11.1, 12 x 8192 x 8192 16.3 / 16.0, 12 x 28672 x 4096 31.9 / 25.5.
+constexpr int kDenseFewRows = 16, kGroupedFewRows = 10;
+constexpr int64_t kFewRowsBytes = 64 << 20;      // of weights, one set and more than 8 rows
 inline int dense(const DenseJob& j, cudaStream_t st) {
-  const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m;
-  return (rows + j.experts - 1) / j.experts <= (j.rows_per_expert != nullptr ? kGroupedFewRows : kDenseFewRows) ? dense_rows(j, st) : dense_tc(j, st);
+  const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m, mean = (rows + j.experts - 1) / j.experts;
+  const bool few = j.rows_per_expert != nullptr ? mean <= kGroupedFewRows
+                                                : mean <= 8 || (mean <= kDenseFewRows && (int64_t)j.n * j.k * (j.type == kDenseI8 ? 1 : 2) <= kFewRowsBytes);
+  return few ? dense_rows(j, st) : dense_tc(j, st);
 }
 
 namespace {

@@ -13,8 +13,9 @@
 // cp.async fills several units ahead, across tiles, and which only this lane reads again, so that nothing but its own wait stands
 // between the two.
 //
-// Up to eight tokens of one set of weights lie in shared memory as a whole (a panel): with every block asking L2 for the same lines
-// of one token at the same time, unit after unit, a token of 7168 x 2048 took longer than sixteen (18.6 and 13.9 us).
+// All blocks ask L2 for the same lines of the tokens at the same time, unit after unit.  Where that is few lines it is what takes longest: one
+// token of 7168 x 2048 (gated, bfloat16) 18.6 us when lanes without a token of their own read the last one, sixteen tokens 13.9.  So
+// lanes without a token bring nothing, and tiles of eight go through L1: 10.8 us, 5.1 TB/s.
 #include "dense.cuh"
 
 namespace b200moe {
@@ -22,7 +23,6 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kUnit = 128;      // bytes of a row that a warp takes at a time
-constexpr int kPanelBytes = 32768;   // of a panel: two blocks stay on an SM
 
 struct RowsParams {
   DenseJob j;
@@ -33,7 +33,6 @@ struct RowsParams {
   int t_tiles;                  // one set of weights: tiles of tokens
   int team;                     // warps of a tile: 1, 2, 4 or 8
   int panel_pitch;              // bytes from row to row of a panel
-  bool near;                    // tokens go through L1
 };
 
 template <int kType>
@@ -61,7 +60,8 @@ __device__ __forceinline__ void mma(uint32_t (&d)[4], uint32_t a0, uint32_t a1, 
 __device__ __forceinline__ void copy16(uint32_t to, const uint8_t* from, bool there) {   // (zeros where there is nothing)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
-// ... of a token, which the SM's other tiles read as well
+// ... of a token, which the SM's other tiles read as well.  Tiles of eight have it, 8 x 2880 x 2880 3.4 us, 3.6 without, 4 x 2048 x 1408 gated 4.0
+// and 4.3; tiles of sixteen have too many lines for L1, 16 x 4096 x 4096 6.5 us, 5.7 without.
 __device__ __forceinline__ void copy16_token(uint32_t to, const uint8_t* from, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
@@ -114,41 +114,27 @@ __device__ __forceinline__ void quantise_rows(const RowsParams& p, uint8_t* code
   __syncthreads();
 }
 
-// Up to eight rows as they are, zeros up to a whole unit.
-__device__ __forceinline__ void copy_rows(const RowsParams& p, uint8_t* panel) {
-  const uint8_t* x = reinterpret_cast<const uint8_t*>(p.j.x);
-  const int pieces = p.units * (kUnit / 16), total = (int)p.j.m * pieces;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < total; i += 32 * kWarps) {
-    const int row = i / pieces, c = (i - row * pieces) * 16;
-    const vec16 v = c < p.k_bytes ? ld16(x + row * p.x_pitch + c) : vec16{{0, 0, 0, 0}};
-    *reinterpret_cast<vec16*>(panel + row * p.panel_pitch + c) = v;
-  }
-  __syncthreads();
-}
-
 template <int NT>
 struct alignas(128) Fixed {
-  uint32_t sums[2][kWarps][NT][4][32];
+  // (Once, with a second barrier: sums of two tiles left room for one block an SM, 5 rows each of 128 experts of 2048 x 1536 gated 97 us, 75 so.)
+  uint32_t sums[kWarps][NT][4][32];
   float x_scales[8], part[kWarps];      // of rows that are quantised on the way
 };
 
-// Where tokens come from: beside the weights through the lanes' slots, or from a panel of the rows or of their codes.
-enum Tokens { kRing, kPanel, kCodes };
-
-// NT: tiles of 8 tokens.  kAhead: units in flight.
-template <int kType, bool kGated, int NT, int kAhead, int kTokens>
+// NT: tiles of 8 tokens.  kAhead: units in flight.  kCodes: tokens come from a panel of the codes that the block makes of them, not
+// beside the weights through the lanes' slots.
+template <int kType, bool kGated, int NT, int kAhead, bool kCodes>
 __global__ void __launch_bounds__(32 * kWarps, 2)
 dense_rows_kernel(const __grid_constant__ RowsParams p) {
   constexpr int BT = 8 * NT;
-  constexpr int kSlots = 4 + (kTokens == kRing ? 2 * NT : 0);      // 16-byte pieces of a unit that a lane has
+  constexpr int kSlots = 4 + (kCodes ? 0 : 2 * NT);      // 16-byte pieces of a unit that a lane has
   extern __shared__ __align__(128) uint8_t dyn[];
   Fixed<NT>& fixed = *reinterpret_cast<Fixed<NT>*>(dyn);
   auto& sums = fixed.sums;
   const DenseJob& j = p.j;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int team = warp / p.team, in_team = warp - team * p.team, teams = kWarps / p.team;   // (p.team divides kWarps)
-  const bool grouped = kTokens == kRing && j.rows_per_expert != nullptr;
+  const bool grouped = !kCodes && j.rows_per_expert != nullptr;
   uint8_t* const behind = dyn + sizeof(Fixed<NT>) + kWarps * kAhead * kSlots * 512;      // the panel, or the tile walk
   const uint32_t ring = ptx::smem_u32(dyn) + sizeof(Fixed<NT>) + warp * kAhead * kSlots * 512 + lane * 16;
   const uint32_t panel = ptx::smem_u32(behind) + min(g, (int)min(j.m, (int64_t)8) - 1) * p.panel_pitch + 16 * q;
@@ -184,17 +170,20 @@ dense_rows_kernel(const __grid_constant__ RowsParams p) {
     if (next_tile >= total) return;
     TileInfo ti;
     locate(next_tile, next_cursor, ti);
-    // (rows past the end read the last one, and are not stored)
+    // Weight rows past the end are the last one, and not stored.  Tokens that a tile lacks are not brought: what lies in their slots
+    // makes sums that nobody reads.  (9 x 4096 x 4096 5.2 us, 9.2 with copies of the last token in their place.)
     const int f = ti.n_tile * (kGated ? 8 : 16) + g;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = kGated ? min(f, limit - 1) + i * half : min(f + i * half, limit - 1);
       wr[i] = w + ((int64_t)ti.e * j.n + row) * p.w_pitch + 16 * q;
     }
-    if (kTokens == kRing) {
+    if (!kCodes) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-        xr[i] = x + min((int64_t)ti.row0 + min(g + 8 * i, ti.valid - 1), j.m - 1) * p.x_pitch + 16 * q;
+      for (int i = 0; i < NT; ++i) {
+        const int64_t row = (int64_t)ti.row0 + g + 8 * i;
+        xr[i] = g + 8 * i < ti.valid && row < j.m ? x + row * p.x_pitch + 16 * q : nullptr;
+      }
     }
   };
   auto copy = [&](uint32_t slot) {
@@ -204,10 +193,11 @@ dense_rows_kernel(const __grid_constant__ RowsParams p) {
       const bool there = k + 16 * q < p.k_bytes;
 #pragma unroll
       for (int i = 0; i < 2; ++i) copy16(slot + (2 * s + i) * 512, wr[i] + k, there);
-      if (kTokens == kRing) {
+      if (!kCodes) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          if (p.near) copy16_token(slot + (4 + NT * s + i) * 512, xr[i] + k, there);
+          if (xr[i] == nullptr) continue;
+          if (NT == 1) copy16_token(slot + (4 + NT * s + i) * 512, xr[i] + k, there);
           else copy16(slot + (4 + NT * s + i) * 512, xr[i] + k, there);
         }
       }
@@ -239,14 +229,17 @@ dense_rows_kernel(const __grid_constant__ RowsParams p) {
     if (mine && next_tile < total) copy(ring + a * kSlots * 512);
     commit();
   }
-  if (kTokens == kCodes) quantise_rows(p, behind, fixed.x_scales, fixed.part);
-  if (kTokens == kPanel) copy_rows(p, behind);
+  if (kCodes) quantise_rows(p, behind, fixed.x_scales, fixed.part);
 
   // the outputs of this thread: one feature of the 8 (and of which 8), every some tokens
   const int tt = in_team * 32 + lane, f = tt & 7, h = kGated ? 0 : (tt >> 3) & 1;
   const int t0 = tt >> (kGated ? 3 : 4), t_step = 2 * p.team * (kGated ? 2 : 1);
-  int slot = 0, cursor = 0, parity = 0;
-  for (int tile = first_tile; tile < total; tile += step, parity ^= 1) {
+  auto team_sync = [&]() {
+    if (p.team == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * p.team) : "memory");
+  };
+  int slot = 0, cursor = 0;
+  for (int tile = first_tile; tile < total; tile += step) {
     TileInfo ti;
     locate(tile, cursor, ti);
     // scales and biases are on their way while the weights are
@@ -260,6 +253,8 @@ dense_rows_kernel(const __grid_constant__ RowsParams p) {
         if (j.bias != nullptr) bias[i] = load_bias(j.bias, j.bias_f16, at + i * half);
       }
     }
+    float x_scale = 1.f;       // of the token that the lane's number says
+    if (kType == kDenseI8 && !kCodes && lane < ti.valid && ti.row0 + (int64_t)lane < j.m) x_scale = j.x_scale[ti.row0 + (int64_t)lane];
     uint32_t acc[NT][4] = {};
     for (int unit = in_team; unit < p.units; unit += p.team) {
       const uint32_t from = ring + slot * kSlots * 512;
@@ -269,7 +264,7 @@ dense_rows_kernel(const __grid_constant__ RowsParams p) {
         const uint4 a = ptx::lds128(from + 2 * s * 512), b = ptx::lds128(from + (2 * s + 1) * 512);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          const uint4 t = kTokens == kRing ? ptx::lds128(from + (4 + NT * s + i) * 512) : ptx::lds128(panel + unit * kUnit + 64 * s);
+          const uint4 t = kCodes ? ptx::lds128(panel + unit * kUnit + 64 * s) : ptx::lds128(from + (4 + NT * s + i) * 512);
           mma<kType>(acc[i], a.x, b.x, a.y, b.y, t.x, t.y);
           mma<kType>(acc[i], a.z, b.z, a.w, b.w, t.z, t.w);
         }
@@ -279,27 +274,25 @@ dense_rows_kernel(const __grid_constant__ RowsParams p) {
       commit();
       if (++slot == kAhead) slot = 0;
     }
+    team_sync();               // the sums of the tile before have been read
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sums[parity][warp][i][r][lane] = acc[i][r];
-    // (one barrier a tile: the sums of the tile before are in the other half)
-    if (p.team == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * p.team) : "memory");
-    if (feat >= limit) continue;
-    for (int t = t0; t < ti.valid; t += t_step) {
+      for (int r = 0; r < 4; ++r) sums[warp][i][r][lane] = acc[i][r];
+    team_sync();
+    for (int t = t0; t - t0 < ti.valid; t += t_step) {      // (every lane as often)
       const int64_t row = (int64_t)ti.row0 + t;
-      if (row >= j.m) break;
-      const float xs = kType != kDenseI8 ? 1.f : kTokens == kCodes ? fixed.x_scales[t] : j.x_scale[row];
+      const float xs = kType != kDenseI8 ? 1.f : kCodes ? fixed.x_scales[t & 7] : __shfl_sync(0xffffffffu, x_scale, t & (BT - 1));
+      if (feat >= limit || t >= ti.valid || row >= j.m) continue;
       auto value = [&](int i) {
         const int r = 2 * (h + i) + (t & 1), l = f * 4 + ((t & 7) >> 1);
         if (kType == kDenseI8) {
           int sum = 0;
-          for (int n = 0; n < p.team; ++n) sum += (int)sums[parity][team * p.team + n][t >> 3][r][l];
+          for (int n = 0; n < p.team; ++n) sum += (int)sums[team * p.team + n][t >> 3][r][l];
           return (float)sum * xs * ws[i] + bias[i];
         }
         float v = 0.f;
-        for (int n = 0; n < p.team; ++n) v += __uint_as_float(sums[parity][team * p.team + n][t >> 3][r][l]);
+        for (int n = 0; n < p.team; ++n) v += __uint_as_float(sums[team * p.team + n][t >> 3][r][l]);
         return v + bias[i];
       };
       float v = value(0);
@@ -316,15 +309,15 @@ dense_rows_kernel(const __grid_constant__ RowsParams p) {
   }
 }
 
-template <int kType, bool kGated, int NT, int kAhead, int kTokens>
+template <int kType, bool kGated, int NT, int kAhead, bool kCodes>
 int launch(RowsParams& p, cudaStream_t st) {
   constexpr int BT = 8 * NT;
   const DenseJob& j = p.j;
-  auto kern = dense_rows_kernel<kType, kGated, NT, kAhead, kTokens>;
+  auto kern = dense_rows_kernel<kType, kGated, NT, kAhead, kCodes>;
   static SmemConfig configured;
   if (int rc = configured.ensure(kern)) return rc;
-  const size_t smem = sizeof(Fixed<NT>) + (size_t)kWarps * kAhead * (4 + (kTokens == kRing ? 2 * NT : 0)) * 512 +
-                      (kTokens != kRing ? (size_t)j.m * p.panel_pitch : j.rows_per_expert != nullptr ? tile_walk_bytes(j.experts) : 0);
+  const size_t smem = sizeof(Fixed<NT>) + (size_t)kWarps * kAhead * (4 + (kCodes ? 0 : 2 * NT)) * 512 +
+                      (kCodes ? (size_t)j.m * p.panel_pitch : j.rows_per_expert != nullptr ? tile_walk_bytes(j.experts) : 0);
   const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m;
   const int64_t tiles = j.rows_per_expert != nullptr ? (rows / BT + std::min<int64_t>(rows, j.experts)) * p.f_tiles
                                                      : (int64_t)p.t_tiles * p.f_tiles;
@@ -337,7 +330,10 @@ int launch(RowsParams& p, cudaStream_t st) {
     const int64_t cost = rounds * ((p.units + team - 1) / team + kTileCost);
     if (best < 0 || cost < best) { best = cost; p.team = team; }
   }
-  const int64_t grid = std::max<int64_t>(1, std::min(blocks, (tiles * p.team + kWarps - 1) / kWarps));
+  // Teams that have a tile are spread over all blocks (14336 weight rows of 4096, 8 tokens 11.6 us, 12.2 packed; 16 tokens 17.8 and 21.4), unless
+  // packed they leave a block on each SM at the most and are tiles of eight, whose tokens they then share in L1 (6144 of 2048, 8 tokens 4.3 and 3.9).
+  const int64_t packed = (tiles * p.team + kWarps - 1) / kWarps;
+  const int64_t grid = std::max<int64_t>(1, NT == 1 && packed <= sm_count() ? packed : std::min(blocks, tiles));
   B200_LAUNCHED("dense_rows_kernel", launch_pdl(j.early, kern, dim3((unsigned)grid), dim3(32 * kWarps), smem, st, p));
   return B200MOE_OK;
 }
@@ -345,17 +341,10 @@ template <int kType, bool kGated>
 int launch_tokens(RowsParams& p, cudaStream_t st) {
   const DenseJob& j = p.j;
   const bool one_set = j.rows_per_expert == nullptr;
-  if (one_set && j.m <= 8 && j.m * p.panel_pitch <= kPanelBytes) {
-    p.t_tiles = 1;
-    return launch<kType, kGated, 1, 4, kPanel>(p, st);
-  }
   const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m;
-  const bool eight = (rows + j.experts - 1) / j.experts <= (one_set ? 8 : 4);
+  const bool eight = (rows + j.experts - 1) / j.experts <= (one_set ? 8 : 6);
   p.t_tiles = (int)((j.m + (eight ? 7 : 15)) / (eight ? 8 : 16));
-  // Tokens that L1 holds are asked of L2 once an SM: one token of two experts of 4096 x 28672 102.7 us without, 45.3 with L1, 15 tokens
-  // each of eight 288 and 216; 16 x 4096 x 7168 (115 KB of tokens) 11.9 and 13.2.
-  p.near = std::min<int64_t>((rows + j.experts - 1) / j.experts, 16) * p.k_bytes <= 65536;
-  return eight ? launch<kType, kGated, 1, 4, kRing>(p, st) : launch<kType, kGated, 2, 3, kRing>(p, st);
+  return eight ? launch<kType, kGated, 1, 4, false>(p, st) : launch<kType, kGated, 2, 3, false>(p, st);
 }
 
 }  // namespace
@@ -374,7 +363,7 @@ int dense_rows(const DenseJob& j, cudaStream_t st) {
   p.f_tiles = j.gated ? (j.n / 2 + 7) / 8 : (j.n + 15) / 16;
   if (j.type == kDenseI8 && j.x_dtype != B200MOE_I8) {
     p.t_tiles = 1;
-    return launch<kDenseI8, false, 1, 4, kCodes>(p, st);
+    return launch<kDenseI8, false, 1, 4, true>(p, st);
   }
   if (j.type == kDenseI8) return j.gated ? launch_tokens<kDenseI8, true>(p, st) : launch_tokens<kDenseI8, false>(p, st);
   if (!j.gated) return fail(B200MOE_E_UNSUPPORTED, "dense_rows: 16-bit products are gated");

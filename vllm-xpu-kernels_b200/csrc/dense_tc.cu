@@ -197,8 +197,8 @@ struct Epilogue {
   __device__ __forceinline__ Epilogue(const TcDense& job, Ctrl& ctrl, int cta_, int e)
       : p(job), side(e >> 2), quarter((threadIdx.x >> 5) & 3), cta(cta_), lane_sel((uint32_t)(quarter * 32) << 16),
         scale0(ptx::smem_u32(ctrl.scale[e])), bias0(ptx::smem_u32(ctrl.bias[e])), narrow(ptx::smem_u32(ctrl.narrow[e])) {}
-  // The warp's part of a tile, and the scales and biases that it will need: asked for a tile ahead (the way from HBM takes as long as
-  // a tile of a few K blocks: 1 row each of 128 experts of 2048 x 768 ..).
+  // The warp's part of a tile, and the scales and biases that it will need: asked for a tile ahead (their way from HBM takes as long as
+  // a tile of a few K blocks).
   __device__ __forceinline__ EpilogueTile fetch(const TileInfo& ti) const {
     const int lane = threadIdx.x & 31, half = p.n >> 1;
     EpilogueTile t;

@@ -50,8 +50,8 @@ __device__ __forceinline__ float row_max(float amax, int threads, float* part) {
 }
 
 // Rows whose 16-byte pieces are aligned, P of them a thread (gated: of gates and of ups), which stay in registers between the maximum
-// and the codes: every byte is read once.  Blocks stay, and have the next row on its way while they are at work on one (not gated:
-// registers).  8192 rows of 7168 bfloat16 values 51.7 us with a block a row, .. so.
+// and the codes: every byte is read once.  Blocks stay: 8192 rows of 7168 bfloat16 values 30.1 us, 5.9 TB/s (31.3 with a block a row), gated
+// 72.3 (77.3); 4096 rows of 14336 float32 values 45.3, 6.5 TB/s (44.9), gated 99.9 (108.1).
 template <typename T, bool kGated, int P>
 __global__ void __launch_bounds__(512, kGated || P == 8 ? 1 : 2)
 quant_int8_rows_kernel(const QuantInt8Params p, int threads) {

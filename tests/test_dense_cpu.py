@@ -139,6 +139,17 @@ def test_quantiser_refused_before_any_launch(lib):
         assert message in lib.b200moe_last_error()
 
 
+@pytest.mark.parametrize("change,message", [
+    (dict(dtype=0), b"bfloat16 or float16"), (dict(hidden=44), b"multiple of 8"), (dict(hidden=0), b"multiple of 8"), (dict(x=264), b"16-byte aligned"),
+    (dict(q=260), b"16-byte aligned"),
+])
+def test_permuting_quantiser_refused_before_any_launch(lib, change, message):
+    v = {**dict(x=256, dtype=2, q=256, hidden=64), **change}
+    assert lib.b200moe_remap_quant_int8(P(v["x"]), v["dtype"], P(v["q"]), P(256), None, P(256), P(256), P(256), 5, L(4), v["hidden"], 2, 8, 8,
+                                        None, Z(0), None) == -1
+    assert message in lib.b200moe_last_error()
+
+
 def test_schemas_and_no_cpu_path(native):
     def schema(op):
         args = op.default._schema.arguments

@@ -53,7 +53,8 @@ def _silu(g, u, eg, eu):
     return h, 1.1 * u.abs() * eg + ref.silu(g).abs() * eu + h.abs() * (2.0 ** -20 + g.abs() * 2.0 ** -23)
 
 
-def _check(out, x, weights, ids, w13, s13, b13, w2, s2, b2, act=_silu, clamp=None, emap=None):
+def _check(out, x, weights, ids, w13, s13, b13, w2, s2, b2, act=_silu, clamp=None, emap=None, parts=0.0):
+    """`parts`: half a step of parts of a token's sum that are rounded before they are added up."""
     dtype = out.dtype
     step = torch.finfo(dtype).eps / 2
     want, tol = torch.zeros_like(out, dtype=torch.float64), torch.full_like(out, torch.finfo(dtype).smallest_normal * step, dtype=torch.float64)
@@ -66,7 +67,7 @@ def _check(out, x, weights, ids, w13, s13, b13, w2, s2, b2, act=_silu, clamp=Non
         y, off = _exact_rows(x[t], w13[e], s13[e], b(b13), w2[e], s2[e], b(b2), act, clamp)
         w = weights[t, k].double()[:, None]
         want.index_add_(0, t, w * y)
-        tol.index_add_(0, t, w.abs() * (off + (y.abs() + off) * (step + 10 * U)))     # rows are rounded, then added up in fp32
+        tol.index_add_(0, t, w.abs() * (off + (y.abs() + off) * (step + 10 * U + parts * (1 + step))))     # rows are rounded, then added up in fp32
     tol = tol + (want.abs() + tol) * step * (1 + 2.0 ** -10)
     err = (out.double() - want).abs()
     assert torch.all(err <= tol), float((err / tol).max())
@@ -263,3 +264,116 @@ def test_a_block_with_a_shared_expert(native, T):
         return _silu(g, u, eg + g.abs() * 2.0 ** -8 * 1.01, eu + u.abs() * 2.0 ** -8 * 1.01)
     one = torch.ones(T, 1, device=DEV)
     _check(shared, normed, one, torch.zeros(T, 1, dtype=torch.int32, device=DEV), v13[None], t13[None], None, v2[None], t2[None], None, act=rounded)
+
+
+# T, E, K, H, I: rows of more pieces than a block of the permutation keeps, more slots than its small form takes, more than eight experts a token
+@pytest.mark.parametrize("T,E,K,H,I", [(5, 2, 1, 8448, 16), (3, 4, 2, 33024, 16), (40, 2, 2, 20016, 16), (1100, 8, 4, 128, 32), (1100, 4, 2, 8448, 16),
+                                       (30, 16, 10, 64, 32), (300, 32, 16, 48, 16), (1, 256, 8, 64, 16)])
+def test_permutations(native, T, E, K, H, I):
+    gen = torch.Generator().manual_seed(T + H)
+    w13, s13, w2, s2 = _weights(E, H, I, gen)
+    x = torch.randn(T, H, generator=gen).to(B16).to(DEV)
+    weights, ids = _routing(T, E, K, gen)
+    out = torch.full((T, H), float("nan"), dtype=B16, device=DEV)
+    native.XpuFusedMoe(w13, s13, None, w2, s2, None, K, "silu", E).apply(out, x, weights, ids)
+    _check(out, x, weights, ids, w13, s13, None, w2, s2, None)
+
+
+def test_nothing_to_do(native):
+    """No tokens; experts that get none; a token none of whose experts are here; a row of zeros."""
+    gen = torch.Generator().manual_seed(3)
+    E, K, H, I = 4, 2, 64, 32
+    w13, s13, w2, s2 = _weights(E, H, I, gen)
+    layer = native.XpuFusedMoe(w13, s13, None, w2, s2, None, K, "silu", E)
+    empty = torch.empty(0, H, dtype=B16, device=DEV)
+    layer.apply(empty, empty.clone(), torch.empty(0, K, device=DEV), torch.empty(0, K, dtype=torch.int32, device=DEV))
+    x = torch.randn(6, H, generator=gen).to(B16).to(DEV)
+    x[2] = 0
+    weights, ids = torch.rand(6, K, generator=gen).to(DEV), torch.tensor([[1, 1], [1, 3], [1, 3], [-1, -1], [3, -1], [1, 3]], dtype=torch.int32, device=DEV)
+    out = torch.full((6, H), float("nan"), dtype=B16, device=DEV)
+    layer.apply(out, x, weights, ids)
+    # (an id that is not an expert's drops its slot)
+    _check(out, x, weights, ids, w13, s13, None, w2, s2, None)
+    assert not out[2].any() and not out[3].any()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_row_that_is_not_finite_stays_visible_and_alone(native, bad):
+    gen = torch.Generator().manual_seed(4)
+    E, K, H, I, T = 4, 2, 64, 32, 40
+    w13, s13, w2, s2 = _weights(E, H, I, gen)
+    x = torch.randn(T, H, generator=gen).to(B16).to(DEV)
+    weights, ids = _routing(T, E, K, gen)
+    layer = native.XpuFusedMoe(w13, s13, None, w2, s2, None, K, "silu", E)
+    want, got = (torch.empty(T, H, dtype=B16, device=DEV) for _ in range(2))
+    layer.apply(want, x, weights, ids)
+    x[7, 5] = bad
+    layer.apply(got, x, weights, ids)
+    assert torch.isnan(got[7]).all()
+    others = torch.arange(T, device=DEV) != 7
+    assert torch.equal(got[others], want[others])
+
+
+@pytest.mark.parametrize("T", [3, 90])
+def test_two_graphs_replayed_in_turn(native, T):
+    """Two layers of one shape captured after each other, on one stream's workspace, with a dense product in the second graph."""
+    gen = torch.Generator().manual_seed(T)
+    E, K, H, I = 8, 2, 128, 64
+    graphs, outs, inputs, eager = [], [], [], []
+    for _ in range(2):
+        w13, s13, w2, s2 = _weights(E, H, I, gen)
+        layer = native.XpuFusedMoe(w13, s13, None, w2, s2, None, K, "silu", E)
+        v, t = ref.weights(48, H, gen)
+        x = torch.randn(T, H, generator=gen).to(B16).to(DEV)
+        weights, ids = _routing(T, E, K, gen)
+        out, dense = torch.empty(T, H, dtype=B16, device=DEV), torch.empty(T, 48, dtype=B16, device=DEV)
+
+        def run(out=out, dense=dense, x=x, layer=layer, v=v, t=t, weights=weights, ids=ids):
+            layer.apply(out, x, weights, ids)
+            torch.ops._xpu_C.b200_int8_linear(dense, x, None, v, t)
+        run()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        graphs.append(graph), outs.append((out, dense)), inputs.append(x), eager.append(run)
+    for step in range(3):
+        for x in inputs:
+            x.copy_(torch.randn(T, H, generator=gen).to(B16))
+        wants = []
+        for run, pair in zip(eager, outs):
+            run()
+            wants.append([o.clone() for o in pair])
+            for o in pair:
+                o.fill_(float("nan"))
+        for i in (step % 2, 1 - step % 2):
+            graphs[i].replay()
+        for pair, want in zip(outs, wants):
+            assert all(torch.equal(o, w) for o, w in zip(pair, want))
+
+
+@pytest.mark.parametrize("ep,tokens", [(2, (5, 9)), (4, (33, 0, 64, 7))])
+def test_expert_parallel_over_peer_memory(native, ep, tokens):
+    """All ranks in this process, one phase after the other; every rank's part of a token's sum travels as a 16-bit row."""
+    from vllm_xpu_kernels.ep_moe import EpPeerFusedMoe, LocalPeerWorld
+    gen = torch.Generator().manual_seed(ep)
+    E, K, H, I = 8, 4, 128, 64
+    w13, s13, w2, s2 = _weights(E, H, I, gen)
+    n, world = E // ep, LocalPeerWorld(ep, DEV)
+    layers = []
+    for r in range(ep):
+        mine = slice(r * n, (r + 1) * n)
+        layers.append(EpPeerFusedMoe(w13[mine].contiguous(), s13[mine].contiguous(), None, w2[mine].contiguous(), s2[mine].contiguous(), None,
+                                     K, "silu", n, world.member(r), max(tokens), H))
+    for _ in range(2):      # the second call runs over the first one's leftovers
+        given = []
+        for r in range(ep):
+            weights, ids = _routing(max(tokens[r], 1), E, K, gen)
+            given.append((torch.randn(tokens[r], H, generator=gen).to(B16).to(DEV), weights[:tokens[r]], ids[:tokens[r]]))
+            layers[r].dispatch(*given[r])
+        for r in range(ep):
+            layers[r].experts_and_combine()
+        for r in range(ep):
+            out = torch.full((tokens[r], H), float("nan"), dtype=B16, device=DEV)
+            layers[r].finish(out)
+            if tokens[r]:
+                _check(out, *given[r], w13, s13, None, w2, s2, None, parts=2.0 ** -8)

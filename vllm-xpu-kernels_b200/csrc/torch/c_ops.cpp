@@ -238,16 +238,6 @@ void silu_and_mul_quant(at::Tensor& out, at::Tensor& input, at::Tensor& scale) {
                                           scale.data_ptr<float>(), rows, (int)d, current_stream()));
 }
 
-// Memory as `n` pieces of `length` bytes, `stride` bytes apart.
-struct Pieces {
-  const char* at;
-  int64_t n, stride, length;
-  const char* end() const { return at + (n - 1) * stride + length; }
-};
-Pieces pieces_of_rows(const at::Tensor& t, int64_t row_stride) {
-  const int64_t hidden = t.size(-1), rows = hidden ? t.numel() / hidden : 0, size = t.element_size();
-  return {(const char*)t.data_ptr(), row_stride == 0 ? std::min<int64_t>(rows, 1) : rows, row_stride * size, hidden * size};
-}
 // ... of scales [rows, groups], by row or by group, whichever is dense, else all that they span.
 Pieces pieces_of_scales(const at::Tensor& t) {
   const int64_t rows = t.size(0), groups = t.size(1), size = t.element_size();
@@ -257,17 +247,6 @@ Pieces pieces_of_scales(const at::Tensor& t) {
   if (rows == 1 || t.stride(0) == 1) return {at, groups, t.stride(1) * size, rows * size};
   return {at, 1, 0, ((rows - 1) * t.stride(0) + (groups - 1) * t.stride(1) + 1) * size};
 }
-// Whether a and b share bytes.  (Pieces of different strides whose spans overlap are taken to.)
-bool overlap(const Pieces& a, const Pieces& b) {
-  if (a.n == 0 || b.n == 0 || a.length == 0 || b.length == 0 || a.at >= b.end() || b.at >= a.end()) return false;
-  if (a.n > 1 && b.n > 1 && a.stride != b.stride) return true;
-  // columns of one buffer: where b's pieces are, modulo the stride
-  const int64_t stride = a.n > 1 ? a.stride : b.stride;
-  if ((a.n == 1 && b.n == 1) || stride <= 0) return true;
-  const int64_t d = ((b.at - a.at) % stride + stride) % stride;
-  return d < a.length || d + b.length > stride;
-}
-
 // residual += input, norm, weight; the result in the input's dtype (out) and as e4m3 rows with scales (out_q, scales).
 void b200_add_rms_norm(const at::Tensor& input, const std::optional<at::Tensor>& residual,
                        const std::optional<at::Tensor>& weight, double epsilon, const std::optional<at::Tensor>& out,

@@ -1,6 +1,5 @@
 // The dense layers beside the routed experts: torch.ops._xpu_C.b200_int8_linear, b200_gated_linear,
 // b200_gated_linear_backward and, with gradients, b200_gated_product over the C ABI.  No counterpart in the reference, which multiplies dense layers by library calls.
-#include <ATen/MemoryOverlap.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 #include "layer.h"
@@ -12,14 +11,16 @@ namespace {
 void same_device(const at::Tensor& t, const at::Tensor& input, const char* op, const char* name) {
   TORCH_CHECK(t.device() == input.device(), op, ": ", name, " must be on the input's device");
 }
+// A tensor that is written shares no byte with itself or with one of the others (rows may lie between another's).
+Pieces pieces_of(const at::Tensor& t, const char* op, const char* name) { return pieces_of_rows(t, row_stride(t, op, name)); }
 void writable(const at::Tensor& t, const char* op, const char* name, std::initializer_list<const at::Tensor*> others) {
-  TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, op, ": ", name, " must not be expanded");
+  if (t.numel() == 0) return;
+  const Pieces mine = pieces_of(t, op, name);
+  TORCH_CHECK(mine.n * mine.length == (int64_t)t.numel() * (int64_t)t.element_size() && (mine.n <= 1 || mine.stride >= mine.length), op,
+              ": the rows of ", name, " must not overlap");
   for (const at::Tensor* o : others)
-    if (o != nullptr && o->defined()) {
-      const auto s = at::get_overlap_status(t, *o);
-      TORCH_CHECK(s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial, op, ": ", name,
-                  " must not share memory with another tensor of the call");
-    }
+    if (o != nullptr && o->numel() > 0)
+      TORCH_CHECK(!overlap(mine, pieces_of(*o, op, "another tensor")), op, ": ", name, " must not share memory with another tensor of the call");
 }
 bool same_leading(const at::Tensor& a, const at::Tensor& b) {
   return a.dim() == b.dim() && a.sizes().slice(0, a.dim() - 1) == b.sizes().slice(0, b.dim() - 1);

@@ -279,16 +279,17 @@ struct Experts {
 
   // Int8 layers: rows between the GEMMs are quantised from the activation's fp32 values where gemm1's epilogue applies it
   // (16-bit ones would move every twentieth code), else from 16 bits as the activation kernels take and give them.
-  void quantise_int8(uint8_t* ws, const void* from, b200moe_dtype type, int64_t stride, int gated) const {
+  // (Of buffers that are sized for a worst case, the rows in use.)
+  void quantise_int8(uint8_t* ws, const void* from, b200moe_dtype type, int64_t stride, int gated, const int32_t* rows) const {
     check_status(b200moe_quant_int8_rows(from, type, stride, (int8_t*)(ws + act_q), inter2(), (float*)(ws + act_s), M, (int)inter2(),
-                                         gated, nullptr, 0, stream));
+                                         gated, o.rows_hint > 0 ? rows : nullptr, segments, stream));
   }
   void run(uint8_t* ws, const void* a, const void* a_scale, const int32_t* rows, void* d) const {
     const int64_t I = p.inter, I2 = inter2();
     if (weights.i8 && o.form == kEpilogue) {
       gemm(true, a, B200MOE_I8, a_scale, ws + act, B200MOE_F32, nullptr, rows, B200MOE_EPI_SILU_MUL);
       mark(o, gil, "gemm1");
-      quantise_int8(ws, ws + act, B200MOE_F32, I, 0);
+      quantise_int8(ws, ws + act, B200MOE_F32, I, 0, rows);
       mark(o, gil, "activation");
       gemm(false, ws + act_q, B200MOE_I8, ws + act_s, d, out, nullptr, rows, B200MOE_EPI_NONE);
       mark(o, gil, "gemm2");
@@ -324,7 +325,7 @@ struct Experts {
         (pairs ? t.slice(1, 1, 2 * I, 2) : t.narrow(1, I, I)).clamp_(-p.clamp, p.clamp);
       }
       if (weights.i8 && p.act == kSilu) {
-        quantise_int8(ws, ws + g1, out, 2 * I, 1);
+        quantise_int8(ws, ws + g1, out, 2 * I, 1, rows);
       } else if (p.block_fp8 && p.act == kSilu && I % 128 == 0) {
         // SiLU, multiply and the 1x128 e4m3 quantisation of gemm2's input in one pass over the rows
         // that the experts' segments use (the buffers may be sized for a worst case)
@@ -349,7 +350,7 @@ struct Experts {
     }
     mark(o, gil, "activation");
     if (weights.i8) {
-      if (p.act != kSilu) quantise_int8(ws, ws + act, out, I2, 0);
+      if (p.act != kSilu) quantise_int8(ws, ws + act, out, I2, 0, rows);
       gemm(false, ws + act_q, B200MOE_I8, ws + act_s, d, out, nullptr, rows, B200MOE_EPI_NONE);
     } else if (p.block_fp8) {
       if (!fp8_ready)
@@ -477,6 +478,7 @@ PyObject* layer_run(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const b200moe_stream st = (b200moe_stream)stream.stream();
   const Weights weights = describe(p, H, od, x.device());
   raise_if_timed_out(device_status_word(x.get_device()));   // an earlier call on this device gave up a wait
+  if (gather && T == 0) Py_RETURN_NONE;
   if (o.rows_hint == 0 && map.has_value() && p.total_experts > p.experts)
     o.rows_hint = std::max<int64_t>(1, M * p.experts / p.total_experts);   // the other ranks' share is masked
   TORCH_CHECK_NOT_IMPLEMENTED(!weights.i8 || (!a1q.has_value() && o.form != kFp8),

@@ -10,6 +10,7 @@
 #include <torch/library.h>
 #include <torch/types.h>
 
+#include <algorithm>
 #include <optional>
 
 #include "../../../include/b200moe.h"
@@ -80,6 +81,27 @@ inline int64_t row_stride(const at::Tensor& t, const char* op, const char* name)
     next *= t.size(d);
   }
   return stride;
+}
+
+// Memory as `n` pieces of `length` bytes, `stride` bytes apart.
+struct Pieces {
+  const char* at;
+  int64_t n, stride, length;
+  const char* end() const { return at + (n - 1) * stride + length; }
+};
+inline Pieces pieces_of_rows(const at::Tensor& t, int64_t row_stride) {
+  const int64_t hidden = t.size(-1), rows = hidden ? t.numel() / hidden : 0, size = t.element_size();
+  return {(const char*)t.data_ptr(), row_stride == 0 ? std::min<int64_t>(rows, 1) : rows, row_stride * size, hidden * size};
+}
+// Whether a and b share bytes.  (Pieces of different strides whose spans overlap are taken to.)
+inline bool overlap(const Pieces& a, const Pieces& b) {
+  if (a.n == 0 || b.n == 0 || a.length == 0 || b.length == 0 || a.at >= b.end() || b.at >= a.end()) return false;
+  if (a.n > 1 && b.n > 1 && a.stride != b.stride) return true;
+  // columns of one buffer: where b's pieces are, modulo the stride
+  const int64_t stride = a.n > 1 ? a.stride : b.stride;
+  if ((a.n == 1 && b.n == 1) || stride <= 0) return true;
+  const int64_t d = ((b.at - a.at) % stride + stride) % stride;
+  return d < a.length || d + b.length > stride;
 }
 
 // Scratch for the multi-block sort path; empty when the single-block path runs.

@@ -56,7 +56,7 @@ struct TcDense {
   uint32_t idesc;
   b200moe_dtype d_dtype;
   int bias_f16;
-  int d_wide, pre_wide;     // bytes of a store: 32, 16, or 0 for value by value
+  bool d_wide, pre_wide;    // stores in pieces of 16 bytes, else value by value
   float clamp;
 };
 
@@ -68,8 +68,8 @@ struct Ctrl {
   uint32_t tmem_base;
   int abort_flag;
   alignas(16) float scale[kEpi][128];    // per epilogue warp: of the weight rows that it has columns of
-  alignas(16) float bias[kEpi][128];
-  alignas(16) uint8_t narrow[kEpi][32 * 32];   // 32 bytes of each of a warp's rows, for stores that are not aligned
+  alignas(16) uint16_t bias[kEpi][128];
+  alignas(16) uint8_t stage[kEpi][32 * 64];    // ... 64 bytes of each of its rows on their way out
   alignas(16) uint8_t walk[tile_walk_bytes(kMaxExperts)];
 };
 constexpr size_t kSmem = 1024 + (size_t)kRing + sizeof(Ctrl);
@@ -113,90 +113,93 @@ __device__ __forceinline__ void locate_grouped(const TcDense& p, const TileWalk&
   ti.valid = min(rows - ti.m_tile * height, height);
 }
 
-// A warp's 32 rows x 16 columns, a row a lane, of which the first `rows` rows and the columns below `limit` exist: in pieces of 32 or
-// 16 bytes where they are aligned, else through shared memory, so that lanes that store together are neighbours in a row.
-// (Odd row lengths, value by value from the row's own lane: 1001 x 2011 x 2032 48 us.)
-__device__ __forceinline__ void store_16(void* d, b200moe_dtype t, int64_t row_at, int64_t stride, int rows, int col, int limit,
-                                         const float (&v)[16], int wide, uint32_t narrow) {
+// B bytes of each of a warp's 32 rows, a row a lane, of which the first `rows` rows and `bytes` bytes exist, to `at` and every `pitch`
+// bytes on.  Through shared memory, so that lanes that store together are neighbours in a row: in 16-byte pieces where they are aligned
+// (wide), else value by value.  (A lane's own row in 32-byte pieces took a warp 1000 cycles for 32 columns, which is what bounded tiles of
+// few K blocks: 128 rows each of 128 experts of 768 x 2048 59.4 us, 53.5 so.)
+template <int B>
+__device__ __forceinline__ void store_rows(uint8_t* at, int64_t pitch, int rows, int bytes, const uint32_t (&w)[B / 4], bool wide, int size,
+                                           uint32_t stage) {
+  constexpr int kPer = B / 16;
   const int lane = threadIdx.x & 31;
-  const bool f32 = t == B200MOE_F32;
-  uint8_t* const to = reinterpret_cast<uint8_t*>(d) + (row_at + col) * (f32 ? 4 : 2);
-  const int64_t pitch = stride * (f32 ? 4 : 2);
-  // 32 bytes of every row, of which `left` bytes exist
-  auto piece = [&](uint8_t* at0, const uint32_t (&w)[8], int left) {
-    if (wide != 0) {
-      if (lane >= rows || left <= 0) return;
-      uint8_t* const at = at0 + lane * pitch;
-      if (wide == 32) {
-        ptx::stg256(at, w);
-      } else {
-        *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
-        if (left > 16) *reinterpret_cast<uint4*>(at + 16) = make_uint4(w[4], w[5], w[6], w[7]);
-      }
-      return;
-    }
-    __syncwarp();
-    ptx::sts128(narrow + lane * 32, make_uint4(w[0], w[1], w[2], w[3]));
-    ptx::sts128(narrow + lane * 32 + 16, make_uint4(w[4], w[5], w[6], w[7]));
-    __syncwarp();
-    if (f32) {
-#pragma unroll 2
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3), c = (lane & 7) * 4;
-        if (r < rows && c < left) *reinterpret_cast<uint32_t*>(at0 + r * pitch + c) = ptx::lds32(narrow + r * 32 + c);
-      }
-    } else {
-#pragma unroll 2
-      for (int i = 0; i < 16; ++i) {
-        const int r = 2 * i + (lane >> 4), c = (lane & 15) * 2;
-        if (r < rows && c < left) *reinterpret_cast<uint16_t*>(at0 + r * pitch + c) = ptx::lds16(narrow + r * 32 + c);
-      }
-    }
-  };
-  uint32_t w[8];
-  if (f32) {
+  auto place = [&](int row, int byte) { return stage + row * 64 + (byte ^ ((row & 6) << 3)); };    // (no two lanes of a phase in one bank)
+  __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[i]);
-    piece(to, w, 4 * (limit - col));
+  for (int i = 0; i < kPer; ++i) ptx::sts128(place(lane, 16 * i), make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+  __syncwarp();
+  if (wide) {
+    const int c = lane % kPer * 16, r0 = lane / kPer;
+    uint8_t* to = at + r0 * pitch + c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 + i]);
-    piece(to + 32, w, 4 * (limit - col) - 32);
+    for (int i = 0; i < kPer; ++i) {
+      const int r = r0 + i * (32 / kPer);
+      const uint4 v = ptx::lds128(place(r, c));
+      if (r < rows && c < bytes) *reinterpret_cast<uint4*>(to + (int64_t)i * (32 / kPer) * pitch) = v;
+    }
+  } else if (size == 4) {
+    constexpr int kRows = 128 / B;     // at a time
+    const int c = lane % (B / 4) * 4;
+#pragma unroll 2
+    for (int r = lane / (B / 4); r < 32; r += kRows)
+      if (r < rows && c < bytes) *reinterpret_cast<uint32_t*>(at + r * pitch + c) = ptx::lds32(place(r, c));
   } else {
-    if (t == B200MOE_F16) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-    }
-    piece(to, w, 2 * (limit - col));
+    constexpr int kRows = 64 / B;
+    const int c = lane % (B / 2) * 2;
+#pragma unroll 2
+    for (int r = lane / (B / 2); r < 32; r += kRows)
+      if (r < rows && c < bytes) *reinterpret_cast<uint16_t*>(at + r * pitch + c) = ptx::lds16(place(r, c));
   }
+}
+// The same for kN values of each row.
+template <int kN>
+__device__ __forceinline__ void store_values(uint8_t* at, int64_t pitch, b200moe_dtype t, int rows, int left, const float (&v)[kN], bool wide,
+                                             uint32_t stage) {
+  if (t == B200MOE_F32) {
+#pragma unroll
+    for (int h = 0; h < kN / 16; ++h) {
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[16 * h + i]);
+      store_rows<64>(at + 64 * h, pitch, rows, 4 * left - 64 * h, w, wide, 4, stage);
+    }
+    return;
+  }
+  uint32_t w[kN / 2];
+  if (t == B200MOE_F16) {
+#pragma unroll
+    for (int i = 0; i < kN / 2; ++i) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kN / 2; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  store_rows<2 * kN>(at, pitch, rows, 2 * left, w, wide, 2, stage);
 }
 
 struct EpilogueTile {
   int64_t first;      // the warp's first row
   int rows;           // ... and how many it has
   int features, j0, limit;   // its columns of D are j0 .. limit - 1
+  uint8_t* at;        // the first row of D, column j0
   float xs;           // scale of the lane's row
   float scale[4];     // of weight rows, on their way to shared memory
   uint16_t bias[4];
 };
-// What an epilogue warp does with sums: rows (quarter of the CTA's 128, a lane each) of every second 16 columns.  (Sixteen at a time:
-// a call of few tiles runs this code once, and most of what it takes is the way of the instructions.)
+// What an epilogue warp does with sums: rows (quarter of the CTA's 128, a lane each) of every second 32 columns, gated 16 gates and 16 ups.
+// (So few at a time: a call of few tiles runs this code once, and most of what it takes is the way of the instructions.)
 template <bool kI8, int kForm>
 struct Epilogue {
   const TcDense& p;
-  const int side, quarter, cta;
-  const uint32_t lane_sel, scale0, bias0, narrow;
+  const int side, quarter, cta, size_shift;
+  const uint32_t lane_sel, scale0, bias0, stage;
   __device__ __forceinline__ Epilogue(const TcDense& job, Ctrl& ctrl, int cta_, int e)
-      : p(job), side(e >> 2), quarter((threadIdx.x >> 5) & 3), cta(cta_), lane_sel((uint32_t)(quarter * 32) << 16),
-        scale0(ptx::smem_u32(ctrl.scale[e])), bias0(ptx::smem_u32(ctrl.bias[e])), narrow(ptx::smem_u32(ctrl.narrow[e])) {}
+      : p(job), side(e >> 2), quarter((threadIdx.x >> 5) & 3), cta(cta_), size_shift(job.d_dtype == B200MOE_F32 ? 2 : 1), lane_sel((uint32_t)(quarter * 32) << 16),
+        scale0(ptx::smem_u32(ctrl.scale[e])), bias0(ptx::smem_u32(ctrl.bias[e])), stage(ptx::smem_u32(ctrl.stage[e])) {}
   // The warp's part of a tile, and the scales and biases that it will need: asked for a tile ahead (their way from HBM takes as long as
   // a tile of a few K blocks).
   __device__ __forceinline__ EpilogueTile fetch(const TileInfo& ti) const {
@@ -208,13 +211,14 @@ struct Epilogue {
     t.features = kForm == kGated ? p.width >> 1 : p.width;
     t.j0 = ti.n_tile * t.features;
     t.limit = min(kForm == kGated ? half : p.n, t.j0 + t.features);
+    t.at = reinterpret_cast<uint8_t*>(p.d) + ((t.first * p.d_stride + t.j0) << size_shift);
     t.xs = 1.f;
     if (kI8 && t.rows > 0) {
-      // columns 16 c + .., c = side, side + 2, .., one after the other; gated 16 gates, then their ups.  (Nothing is done with what
-      // is loaded, not even for columns that do not exist, so that nothing waits for it here.)
+      // every second 32 columns, one after the other; gated 16 gates, then their ups.  (Nothing is done with what is loaded, not even for
+      // columns that do not exist, so that nothing waits for it here.)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int l = 32 * i + lane, c = 2 * (kForm == kGated ? i : l >> 4) + side, f = min(t.j0 + 16 * c + (lane & 15), t.limit - 1);
+        const int c = 2 * i + side, f = min(t.j0 + (kForm == kGated ? 16 * c + (lane & 15) : 32 * c + lane), t.limit - 1);
         const int64_t at = (int64_t)ti.e * p.n + f + (kForm == kGated && (lane & 16) ? half : 0);
         t.scale[i] = p.w_scale[at];
         t.bias[i] = 0;
@@ -232,60 +236,62 @@ struct Epilogue {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       ptx::sts32f(scale0 + 128 * i + 4 * lane, t.scale[i]);
-      ptx::sts32f(bias0 + 128 * i + 4 * lane, load_bias(&t.bias[i], p.bias_f16, 0));
+      if (p.bias != nullptr) ptx::sts16(bias0 + 64 * i + 2 * lane, t.bias[i]);
     }
     __syncwarp();
   }
   // sums as the product's values; `l`: the first one's place among the warp's scales
-  __device__ __forceinline__ void scaled(float (&f)[16], const uint32_t (&v)[16], float xs, int l) const {
+  template <int kN>
+  __device__ __forceinline__ void scaled(float* f, const uint32_t (&v)[kN], float xs, int l) const {
     if (!kI8) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+      for (int i = 0; i < kN; ++i) f[i] = __uint_as_float(v[i]);
       return;
     }
-    float4 ws[4], b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ws[i] = ptx::lds128f(scale0 + 4 * (l + 4 * i));
+    for (int i = 0; i < kN / 4; ++i) {
+      const float4 ws = ptx::lds128f(scale0 + 4 * (l + 4 * i));
+      f[4 * i] = (float)(int)v[4 * i] * xs * ws.x;
+      f[4 * i + 1] = (float)(int)v[4 * i + 1] * xs * ws.y;
+      f[4 * i + 2] = (float)(int)v[4 * i + 2] * xs * ws.z;
+      f[4 * i + 3] = (float)(int)v[4 * i + 3] * xs * ws.w;
+    }
+    if (p.bias == nullptr) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = ptx::lds128f(bias0 + 4 * (l + 4 * i));
+    for (int i = 0; i < kN / 8; ++i) {
+      const uint4 b = ptx::lds128(bias0 + 2 * (l + 8 * i));
+      const uint16_t* const each = reinterpret_cast<const uint16_t*>(&b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[4 * i] = (float)(int)v[4 * i] * xs * ws[i].x + b[i].x;
-      f[4 * i + 1] = (float)(int)v[4 * i + 1] * xs * ws[i].y + b[i].y;
-      f[4 * i + 2] = (float)(int)v[4 * i + 2] * xs * ws[i].z + b[i].z;
-      f[4 * i + 3] = (float)(int)v[4 * i + 3] * xs * ws[i].w + b[i].w;
+      for (int k = 0; k < 8; ++k) f[8 * i + k] += load_bias(each, p.bias_f16, k);
     }
   }
-  // Columns 16 c.. and 16 (c + 2).. of the tile (not gated).
+  // Columns 32 c.. of the tile (not gated).
   __device__ __forceinline__ void store_two(const EpilogueTile& t, int c, const uint32_t (&a)[16], const uint32_t (&b)[16]) const {
-    const int col = t.j0 + 16 * c, l = 8 * (c & ~1);
-    float f[16], g[16];
+    const int l = 32 * (c >> 1);
+    float f[32];
     scaled(f, a, t.xs, l);
-    scaled(g, b, t.xs, l + 16);
-    store_16(p.d, p.d_dtype, t.first * p.d_stride, p.d_stride, t.rows, col, t.limit, f, p.d_wide, narrow);
-    store_16(p.d, p.d_dtype, t.first * p.d_stride, p.d_stride, t.rows, col + 32, t.limit, g, p.d_wide, narrow);
+    scaled(f + 16, b, t.xs, l + 16);
+    store_values(t.at + ((32 * c) << size_shift), p.d_stride << size_shift, p.d_dtype, t.rows, t.limit - t.j0 - 32 * c, f, p.d_wide, stage);
   }
   // Columns 16 c.. of the tile (u: of ups, gated).
   __device__ __forceinline__ void store(const EpilogueTile& t, int c, const uint32_t (&g)[16], const uint32_t (&u)[16]) const {
-    const int col = t.j0 + 16 * c, l = (kForm == kGated ? 16 : 8) * (c & ~1);
-    float f[16];
+    const int left = t.limit - t.j0 - 16 * c, l = 32 * (c >> 1);
+    float f[16], up[16];
     scaled(f, g, t.xs, l);
-    if (kForm == kGated) {
-      float up[16];
-      scaled(up, u, t.xs, l + 16);
-      if (p.pre != nullptr) {
+    scaled(up, u, t.xs, l + 16);
+    if (p.pre != nullptr) {
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          float v[16];
+      for (int h = 0; h < 2; ++h) {
+        float v[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = h == 0 ? f[i] : up[i];
-          store_16(p.pre + h * (p.n >> 1), B200MOE_F32, t.first * p.n, p.n, t.rows, col, t.limit, v, p.pre_wide, narrow);
-        }
+        for (int i = 0; i < 16; ++i) v[i] = h == 0 ? f[i] : up[i];
+        store_values(reinterpret_cast<uint8_t*>(p.pre + t.first * p.n + h * (p.n >> 1) + t.j0 + 16 * c), (int64_t)p.n * 4, B200MOE_F32, t.rows,
+                     left, v, p.pre_wide, stage);
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) f[i] = gated_product(f[i], up[i], p.clamp);
     }
-    store_16(p.d, p.d_dtype, t.first * p.d_stride, p.d_stride, t.rows, col, t.limit, f, p.d_wide, narrow);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = gated_product(f[i], up[i], p.clamp);
+    store_values(t.at + ((16 * c) << size_shift), p.d_stride << size_shift, p.d_dtype, t.rows, left, f, p.d_wide, stage);
   }
 };
 
@@ -509,11 +515,11 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
             if (16 * (c + 4) < units) load(c + 4, 0);
             store(c + 2, 1);
           }
-        } else {                       // twice as many at once
+        } else {                       // twice as many at once (a tile's columns are there, whether or not they exist in D)
 #pragma unroll 1
-          for (int c = ep.side; 16 * c < units; c += 4) {
-            load(c, 0);
-            load(c + 2, 1);            // (a tile's columns are there, whether or not they exist in D)
+          for (int c = ep.side; 32 * c < units; c += 2) {
+            load(2 * c, 0);
+            load(2 * c + 1, 1);
             ptx::tmem_wait_ld(v[0][0], v[1][0]);
             ep.store_two(et, c, v[0][0], v[1][0]);
           }
@@ -634,11 +640,7 @@ void choose_tile(TcDense& p, int64_t sets, int64_t row_tiles, int features, bool
     if (p.width == 0 || cost < 0.94 * least) { p.width = width; least = cost; }
   }
 }
-int store_width(const void* p, int64_t row_bytes, int64_t cols_bytes) {
-  for (int w : {32, 16})
-    if (((uintptr_t)p % w) == 0 && row_bytes % w == 0 && cols_bytes % w == 0) return w;
-  return 0;
-}
+bool stores_wide(const void* p, int64_t row_bytes, int64_t cols_bytes) { return ((uintptr_t)p | row_bytes | cols_bytes) % 16 == 0; }
 uint32_t idesc_of(DenseType t, bool x_mn, bool w_mn, int width) {
   if (t == kDenseI8) return ptx::make_idesc_i8(256, width);
   const uint32_t fmt = t == kDenseBf16 ? 1u : 0u;
@@ -667,8 +669,8 @@ int dense_tc(const DenseJob& j, cudaStream_t st) {
   p.num_kb = (j.k + per_kb - 1) / per_kb;
   p.d_dtype = j.d_dtype; p.bias_f16 = j.bias_f16; p.clamp = j.clamp;
   const int out_size = dtype_bytes(j.d_dtype);
-  p.d_wide = store_width(j.d, j.d_stride * out_size, (int64_t)n_out * out_size);
-  if (j.pre != nullptr) p.pre_wide = store_width(j.pre, (int64_t)j.n * 4, (int64_t)n_out * 4);
+  p.d_wide = stores_wide(j.d, j.d_stride * out_size, (int64_t)n_out * out_size);
+  if (j.pre != nullptr) p.pre_wide = stores_wide(j.pre, (int64_t)j.n * 4, (int64_t)n_out * 4);
   // (tiles as if every set of weights had the mean number of rows)
   const bool grouped = j.rows_per_expert != nullptr;
   const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m, each = (rows + j.experts - 1) / j.experts;
@@ -709,7 +711,7 @@ int dense_plain(const PlainJob& j, cudaStream_t st) {
   p.half_rows = j.x_by_column || j.m > 128 ? 128 : j.m > 64 ? 64 : 32;
   p.m_tiles = (int)((j.m + 2 * p.half_rows - 1) / (2 * p.half_rows));
   p.d_dtype = j.type == kDenseF16 ? B200MOE_F16 : B200MOE_BF16;
-  p.d_wide = store_width(j.d, j.d_stride * 2, (int64_t)j.n * 2);
+  p.d_wide = stores_wide(j.d, j.d_stride * 2, (int64_t)j.n * 2);
   auto run = [&](auto kernel) {
     using K = decltype(kernel);
     if (K::pairs() == 0) return fail(B200MOE_E_UNSUPPORTED, "dense products: this device runs no clusters of two CTAs");

@@ -191,7 +191,9 @@ int launch(const QuantInt8Params& p, cudaStream_t st) {
                                                       dim3(threads), 0, st, p));
     return B200MOE_OK;
   }
-  return nvec <= 2048 ? launch_rows<T, kGated, 4>(p, nvec, st) : launch_rows<T, kGated, 8>(p, nvec, st);
+  // (Many short rows: a warp each, and no barrier.  16384 rows of 768 float32 values 11.6 us, 13.0 with two warps a row, 8192 of 2048 bfloat16
+  // values 10.0 and 11.2; 300 of 768 2.1 and 1.7; gated 16384 of 768 23 and 16.)
+  return nvec > 2048 || (!kGated && nvec <= 256 && p.rows > 1024) ? launch_rows<T, kGated, 8>(p, nvec, st) : launch_rows<T, kGated, 4>(p, nvec, st);
 }
 
 }  // namespace

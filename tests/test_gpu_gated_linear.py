@@ -231,6 +231,68 @@ def test_autograd_under_capture(gl):
     assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+def test_leaves_of_a_graph_outside_the_capture_are_refused(gl):
+    x, w, d = _inputs(20, 64, 24, B16)
+    w.requires_grad_(True)
+    alive = gl.gated_linear(x, w)
+    with pytest.raises(RuntimeError, match="outside this stream capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            gl.gated_linear(x, w)
+    want, = torch.autograd.grad(alive, w, d)
+    del alive
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        loss = gl.gated_linear(x, w) + gl.gated_linear(x, w)      # (a leaf used twice inside is none of that)
+        loss.backward(d)
+    g.replay()
+    torch.testing.assert_close(w.grad, 2 * want, rtol=0, atol=0)   # (equal parts: their sum is exact)
+
+
+def test_two_graphs_replayed_in_turn(gl):
+    """Steps of two sizes captured one after the other: each keeps its own workspace."""
+    steps, replays = [], []
+    for rows, inter in ((40, 72), (150, 130)):
+        x, w, d = _inputs(rows, 128, inter, B16)
+        pre = torch.empty(rows, 2 * inter, device=DEV)
+        out, dx, dw = torch.empty(rows, inter, dtype=B16, device=DEV), torch.empty_like(x), torch.empty_like(w)
+
+        def step(x=x, w=w, d=d, pre=pre, out=out, dx=dx, dw=dw):
+            torch.ops._xpu_C.b200_gated_linear(out, x, w, pre)
+            torch.ops._xpu_C.b200_gated_linear_backward(d, pre, x, w, dx, dw)
+        step()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step()
+        steps.append((step, x, (out, dx, dw)))
+        replays.append(g)
+    gen = torch.Generator().manual_seed(1)
+    for turn in range(3):
+        wants = []
+        for step, x, results in steps:
+            x.copy_(torch.randn(x.shape, generator=gen).to(B16))
+            step()
+            wants.append([r.clone() for r in results])
+            for r in results:
+                r.fill_(float("nan"))
+        for i in (turn % 2, 1 - turn % 2):
+            replays[i].replay()
+        for (_, _, results), want in zip(steps, wants):
+            assert all(torch.equal(r, v) for r, v in zip(results, want))
+
+
+def test_a_row_that_is_not_finite_stays_alone(gl):
+    for rows in (6, 200):
+        x, w, d = _inputs(rows, 64, 24, B16)
+        want = gl.gated_linear(x, w)
+        x[3, 7] = float("nan")
+        x[4, 9] = float("inf")
+        got = gl.gated_linear(x, w)
+        assert torch.isnan(got[3]).all()
+        assert not torch.isfinite(got[4]).all()
+        others = [r for r in range(rows) if r not in (3, 4)]
+        assert torch.equal(got[others], want[others])
+
+
 def test_refusals(gl):
     x, w, d = _inputs(6, 64, 24, B16)
     out, pre = torch.empty(6, 24, dtype=B16, device=DEV), torch.empty(6, 48, device=DEV)

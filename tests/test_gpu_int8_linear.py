@@ -140,6 +140,24 @@ def test_linear_of_strided_rows_leaves_the_rest_alone(native, rows):
         assert torch.all(room[:, :left] == 7) and torch.all(room[:, left + n:] == 7) and torch.all(room[rows] == 7)
 
 
+@pytest.mark.parametrize("rows", [3, 70])
+def test_columns_of_one_buffer(native, rows):
+    """Input and output as columns of the same rows; those that share a byte are refused."""
+    gen = torch.Generator().manual_seed(rows)
+    n, k = 40, 64
+    w, ws = ref.weights(n, k, gen)
+    room = torch.zeros(rows, k + n + 8, dtype=B16, device=DEV)
+    room[:, :k] = _rows((rows, k), B16, gen).to(DEV)
+    x = room[:, :k].clone()
+    torch.ops._xpu_C.b200_int8_linear(room[:, k:k + n], room[:, :k], None, w, ws)
+    want = torch.empty(rows, n, dtype=B16, device=DEV)
+    torch.ops._xpu_C.b200_int8_linear(want, x, None, w, ws)
+    assert torch.equal(room[:, k:k + n], want) and torch.equal(room[:, :k], x)
+    for bad in (room[:, k - 1:k - 1 + n], room[:, 8:8 + n]):
+        with pytest.raises(RuntimeError, match="share memory"):
+            torch.ops._xpu_C.b200_int8_linear(bad, room[:, :k], None, w, ws)
+
+
 def test_linear_of_more_dimensions_and_of_none(native):
     gen = torch.Generator().manual_seed(2)
     w, ws = ref.weights(40, 64, gen)

@@ -1,6 +1,8 @@
 // The dense layers beside the routed experts: torch.ops._xpu_C.b200_int8_linear, b200_gated_linear,
 // b200_gated_linear_backward and, with gradients, b200_gated_product over the C ABI.  No counterpart in the reference, which multiplies dense layers by library calls.
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include "layer.h"
 
@@ -240,9 +242,24 @@ class GatedProduct : public torch::autograd::Function<GatedProduct> {
     return {dx.has_value() ? *dx : at::Tensor(), dw.has_value() ? *dw : at::Tensor()};
   }
 };
+// A leaf's gradient is waited for on the stream that its first live graph was made on.  Where that is another one than a capturing one, the
+// captured backward pass cannot wait for it, and the error ends the process: refused here, while it is one call's.
+void check_capture(const at::Tensor& t, const char* name) {
+  if (!t.requires_grad() || !t.is_leaf()) return;
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (accumulator == nullptr) return;
+  const auto stream = accumulator->stream();
+  TORCH_CHECK(!stream.has_value() || *stream == at::cuda::getCurrentCUDAStream(t.get_device()).unwrap(), "b200_gated_product: ", name,
+              " is part of a graph that lives outside this stream capture; let go of what was computed from it first");
+}
 at::Tensor b200_gated_product_autograd(const at::Tensor& input, const at::Tensor& weight) {
-  if (at::GradMode::is_enabled() && (input.requires_grad() || weight.requires_grad()) && input.is_cuda())
+  if (at::GradMode::is_enabled() && (input.requires_grad() || weight.requires_grad()) && input.is_cuda()) {
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) {
+      check_capture(input, "input");
+      check_capture(weight, "weight");
+    }
     return GatedProduct::apply(input, weight);
+  }
   at::AutoDispatchBelowADInplaceOrView below;
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("_xpu_C::b200_gated_product", "")
                              .typed<at::Tensor(const at::Tensor&, const at::Tensor&)>();

@@ -17,7 +17,7 @@ def gated_linear(input, weight):
 
     With gradients enabled and asked for, the two products are kept in fp32 (8 bytes for each value of the result) and the gradients of
     either operand are computed from them; they are not differentiable again.  Weights that are not contiguous, and
-    rows that are not evenly spaced on 16-byte boundaries, are copied first.  Under stream capture, as for any autograd function, the
-    leaves must have no live graph from outside the capture."""
+    rows that are not evenly spaced on 16-byte boundaries, are copied first.  Under stream capture a
+    leaf that a live graph from outside the capture uses is refused: let go of what was computed from it first."""
     _require_native()
     return torch.ops._xpu_C.b200_gated_product(input, weight)

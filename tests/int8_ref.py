@@ -5,12 +5,19 @@ LEAST = 1e-10
 
 
 def quant_rows(v):
-    """Codes and scales of rows by the definition: fp32 quotients (IEEE: on the CPU), the product unrounded (64 bits hold it)."""
+    """Codes and scales of rows by the definition.  16-bit rows: 127 v / a, ties to even (127 v is exact in 64 bits, so a tie's quotient is);
+    32-bit rows: v times the least fp32 number that is no less than 127 / a, unrounded (64 bits hold the product)."""
+    wide = v.dtype == torch.float32
     v = v.float().cpu()
     amax = v.abs().amax(dim=-1) if v.shape[-1] else v.new_zeros(v.shape[:-1])
     amax = torch.maximum(amax, torch.tensor(LEAST))
-    inv = torch.tensor(127.0) / amax
-    return torch.round(v.double() * inv.double()[..., None]).to(torch.int8), amax / torch.tensor(127.0)
+    if wide:
+        inv = torch.tensor(127.0) / amax
+        inv = torch.where(inv.double() * amax.double() < 127.0, torch.nextafter(inv, torch.full_like(inv, float("inf"))), inv)
+        q = v.double() * inv.double()[..., None]
+    else:
+        q = 127.0 * v.double() / amax.double()[..., None]
+    return torch.round(q).to(torch.int8), amax / torch.tensor(127.0)
 
 
 def linear(q, qs, w, ws, bias=None):

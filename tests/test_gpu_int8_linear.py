@@ -32,6 +32,23 @@ def test_codes_and_scales_are_the_formulas(native, dtype, rows, hidden):
     assert torch.equal(q.cpu(), want_q)
 
 
+@pytest.mark.parametrize("dtype,bits", [(B16, 8), (F16, 11)])
+def test_every_mantissa_and_tie_of_16_bits(native, dtype, bits):
+    """Rows whose largest value has each mantissa, with every value that the type has in the three powers of two below it: ties among them."""
+    m = torch.arange(2 ** (bits - 1), 2 ** bits, dtype=torch.float64)
+    below = torch.cat([m * 2.0 ** -s for s in range(4)])
+    rows = torch.where(below[None] <= m[:, None], below[None], 0.0 * below[None])
+    x = torch.cat((m[:, None], rows, -rows, torch.zeros(len(m), 7, dtype=torch.float64)), dim=1) / 2 ** bits
+    x = x.to(dtype)
+    want_q, want_s = ref.quant_rows(x)
+    tie = 254 * x.double().abs() / x[:, :1].double()
+    assert int(((tie == torch.floor(tie)) & (tie % 2 == 1)).sum()) > len(m)            # (there are ties)
+    for part in (x[:, :-7].contiguous(), x[:, :-6].contiguous()):                      # (an odd length too)
+        q, s = torch.empty(part.shape, dtype=torch.int8, device=DEV), torch.empty(len(m), device=DEV)
+        torch.ops._C.b200_quant_int8_rows(part.to(DEV), q, s)
+        assert torch.equal(q.cpu(), want_q[:, :part.shape[1]]) and torch.equal(s.cpu(), want_s)
+
+
 @pytest.mark.parametrize("dtype", [B16, F16, F32])
 @pytest.mark.parametrize("rows,hidden", [(1, 8), (2, 33), (5, 768), (300, 1408), (2, 14336), (1, 33000)])
 def test_gated_codes(native, dtype, rows, hidden):

@@ -98,19 +98,21 @@ __device__ __forceinline__ void quantise_rows(const RowsParams& p, uint8_t* code
   if (lane == 0) part[warp] = amax;
   __syncthreads();
   for (int i = 0; i < each; ++i) amax = max_nan(amax, part[warp / each * each + i]);
-  const Int8Scale s(amax);
-  if (row < m) {
+  auto write = [&](const auto& s) {
+    if (row >= m) return;
     if (t == 0) scales[row] = s.scale;
 #pragma unroll 4
     for (int c = t; c < pieces; c += threads) {
       float v[8];
       values(c, v);
       uint32_t w[2];
-      s.codes<2>(v, w);
+      s.template codes<2>(v, w);
       if (per == 8) *reinterpret_cast<uint2*>(codes + row * p.panel_pitch + c * 8) = make_uint2(w[0], w[1]);
       else *reinterpret_cast<uint32_t*>(codes + row * p.panel_pitch + c * 4) = w[0];
     }
-  }
+  };
+  if (j.x_dtype == B200MOE_F16) write(Int8Scale<__half>(amax));
+  else write(Int8Scale<float>(amax));
   __syncthreads();
 }
 
@@ -333,7 +335,7 @@ int launch(RowsParams& p, cudaStream_t st) {
   // Teams that have a tile are spread over all blocks (14336 weight rows of 4096, 8 tokens 11.6 us, 12.2 packed; 16 tokens 17.8 and 21.4), unless
   // packed they leave a block on each SM at the most and are tiles of eight, whose tokens they then share in L1 (6144 of 2048, 8 tokens 4.3 and 3.9).
   const int64_t packed = (tiles * p.team + kWarps - 1) / kWarps;
-  const int64_t grid = std::max<int64_t>(1, NT == 1 && packed <= sm_count() ? packed : std::min(blocks, tiles));
+  const int64_t grid = std::max<int64_t>(1, std::min(blocks, NT == 1 && packed <= sm_count() ? packed : tiles));
   B200_LAUNCHED("dense_rows_kernel", launch_pdl(j.early, kern, dim3((unsigned)grid), dim3(32 * kWarps), smem, st, p));
   return B200MOE_OK;
 }

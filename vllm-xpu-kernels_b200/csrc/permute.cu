@@ -143,7 +143,7 @@ enum RowForm { kRowCopy = 0, kRowFp8 = 1, kRowMx = 2, kRowInt8 = 3 };
 // Piece j (16 bytes of the source row; `v` is read only for j < nvec) to its destinations.  `s`: int8, the row's scale.
 template <typename T, int kForm>
 __device__ __forceinline__ void place_piece(const RowJob& a, int j, int nvec, const vec16& v, const int* dest,
-                                            const Int8Scale& s = Int8Scale()) {
+                                            const Int8Scale<T>& s = Int8Scale<T>()) {
   if (kForm == kRowCopy) {
     if (j >= nvec) return;
     for (int k = 0; k < a.K; ++k) {
@@ -169,7 +169,7 @@ __device__ __forceinline__ void place_piece(const RowJob& a, int j, int nvec, co
   }
 }
 template <typename T, int kForm>
-__device__ __forceinline__ void place_row(const RowJob& a, int64_t tok, const int* dest, const Int8Scale& s = Int8Scale()) {
+__device__ __forceinline__ void place_row(const RowJob& a, int64_t tok, const int* dest, const Int8Scale<T>& s = Int8Scale<T>()) {
   const int nvec = kForm == kRowCopy ? a.row_bytes >> 4 : a.H / 8;
   const int steps = kForm == kRowMx ? ((a.H + 127) / 128) * 16 : nvec;
   const uint8_t* src = reinterpret_cast<const uint8_t*>(a.src) + tok * (int64_t)nvec * 16;
@@ -206,7 +206,7 @@ remap_rows_kernel(const RowJob a, const int32_t* __restrict__ row_map) {
     const float amax = warp_largest(largest_of(m, T()));
     if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = amax;
     __syncthreads();
-    const Int8Scale s(warp_largest(most[threadIdx.x & 7]));
+    const Int8Scale<T> s(warp_largest(most[threadIdx.x & 7]));
     if (nvec <= 512) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) place_piece<T, kForm>(a, threadIdx.x + 256 * i, nvec, held[i], dest, s);
@@ -308,8 +308,8 @@ remap_small_kernel(const Id* __restrict__ ids, const int32_t* __restrict__ map, 
   }
   __syncthreads();
   const int steps = kForm == kRowMx ? ((a.H + 127) / 128) * 16 : nvec;
-  Int8Scale s;
-  if constexpr (kForm == kRowInt8) s = Int8Scale(warp_largest(most[lane & (kSmallThreads / 32 - 1)]));
+  Int8Scale<T> s;
+  if constexpr (kForm == kRowInt8) s = Int8Scale<T>(warp_largest(most[lane & (kSmallThreads / 32 - 1)]));
   if (steps <= kSmallThreads * kSmallPre) {
 #pragma unroll
     for (int i = 0; i < kSmallPre; ++i)

@@ -1,10 +1,8 @@
 // Rows as 8-bit integers with one scale each, as the int8 GEMM takes its activations:
 //
-//   v = x, or silu(gate) * up of a row [gate | up];  a = max(amax|v|, 1e-10);  scale = a / 127;  q = rint(v * (127 / a))
+//   v = x, or silu(gate) * up of a row [gate | up];  a = max(amax|v|, 1e-10);  scale = a / 127;  q = 127 v / a, ties to even
 //
-// in fp32, the quotients IEEE ones, the product unrounded: within 127 * 2^-24 of a step of the nearest whole number to v / scale.  (With
-// rint(v / scale) of an IEEE quotient, made of a product wherever that is far enough from a tie, 8192 rows of 7168 bfloat16 values took
-// 48 to 55 us.)  A row with a NaN or an infinity has a scale of NaN.
+// (quant_int8.cuh on their rounding).  A row with a NaN or an infinity has a scale of NaN.
 #include <algorithm>
 
 #include "common.cuh"
@@ -109,7 +107,7 @@ quant_int8_rows_kernel(const QuantInt8Params p, int threads) {
     }
     if (!kGated) amax = largest_of(most, T());
     // (the maxima of the row before are in the other half)
-    const Int8Scale s(row_max(amax, threads, part[parity]));
+    const Int8Scale<std::conditional_t<kGated, float, T>> s(row_max(amax, threads, part[parity]));
     if (live) {
       if (t == 0) p.scales[row] = s.scale;
       int8_t* q = p.q + row * p.q_stride;
@@ -151,7 +149,7 @@ quant_int8_any_kernel(const QuantInt8Params p) {
   };
   float amax = 0.f;
   for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) amax = max_nan(amax, fabsf(value(c)));
-  const Int8Scale s(row_max(amax, blockDim.x, part));
+  const Int8Scale<std::conditional_t<kGated, float, T>> s(row_max(amax, blockDim.x, part));
   if (threadIdx.x == 0) p.scales[row] = s.scale;
   for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) {
     const float y[4] = {value(c), 0.f, 0.f, 0.f};

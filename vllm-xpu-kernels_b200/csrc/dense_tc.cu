@@ -50,7 +50,8 @@ struct TcDense {
   int m_tiles, n_tiles;
   int width;                // weight rows of a tile: a multiple of 32, gated of 64
   int half_rows;            // rows of X that a CTA has of a tile: 32, 64 or 128 (in tensor memory they are the first of 128)
-  int stages, blocks;       // of the ring; K blocks of a stage: 1 or 2
+  bool halved;              // tiles of at most 128 rows: instructions of M = 128, whose sums' second half of columns is on other lanes
+  int stages, blocks;       // of the ring; K blocks of a stage
   int x_bytes, w_bytes;     // of a K block
   int stage_bytes;          // X of its blocks, then their W
   uint32_t idesc;
@@ -184,7 +185,7 @@ __device__ __forceinline__ void store_values(uint8_t* at, int64_t pitch, b200moe
 struct EpilogueTile {
   int64_t first;      // the warp's first row
   int rows;           // ... and how many it has
-  int features, j0, limit;   // its columns of D are j0 .. limit - 1
+  int features, j0, limit;   // its columns of D are j0 .. limit - 1, at most `features`
   uint8_t* at;        // the first row of D, column j0
   float xs;           // scale of the lane's row
   float scale[4];     // of weight rows, on their way to shared memory
@@ -205,12 +206,14 @@ struct Epilogue {
   __device__ __forceinline__ EpilogueTile fetch(const TileInfo& ti) const {
     const int lane = threadIdx.x & 31, half = p.n >> 1;
     EpilogueTile t;
-    const int in_cta = quarter * 32, row0 = cta * p.half_rows + in_cta;
+    // (halved: the quarters are rows 0 and 32, then the same rows of the second half of the columns)
+    const int in_cta = (p.halved ? quarter & 1 : quarter) * 32, row0 = cta * p.half_rows + in_cta, part = p.halved ? quarter >> 1 : 0;
     t.first = (int64_t)ti.row0 + row0;
     t.rows = in_cta < p.half_rows ? (int)min((int64_t)min(ti.valid - row0, 32), p.m - t.first) : 0;
-    t.features = kForm == kGated ? p.width >> 1 : p.width;
-    t.j0 = ti.n_tile * t.features;
-    t.limit = min(kForm == kGated ? half : p.n, t.j0 + t.features);
+    const int tile = kForm == kGated ? p.width >> 1 : p.width, all = kForm == kGated ? half : p.n;
+    t.features = p.halved ? tile >> 1 : tile;
+    t.j0 = ti.n_tile * tile + part * t.features;
+    t.limit = min(all, t.j0 + t.features);
     t.at = reinterpret_cast<uint8_t*>(p.d) + ((t.first * p.d_stride + t.j0) << size_shift);
     t.xs = 1.f;
     if (kI8 && t.rows > 0) {
@@ -218,7 +221,7 @@ struct Epilogue {
       // columns that do not exist, so that nothing waits for it here.)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int c = 2 * i + side, f = min(t.j0 + (kForm == kGated ? 16 * c + (lane & 15) : 32 * c + lane), t.limit - 1);
+        const int c = 2 * i + side, f = min(t.j0 + (kForm == kGated ? 16 * c + (lane & 15) : 32 * c + lane), all - 1);
         const int64_t at = (int64_t)ti.e * p.n + f + (kForm == kGated && (lane & 16) ? half : 0);
         t.scale[i] = p.w_scale[at];
         t.bias[i] = 0;
@@ -349,7 +352,6 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
     walk = tile_walk_at(ctrl->walk, p.experts);
     total = walk.total;
   }
-  const int half = p.n >> 1;
   int cursor = 0;
   auto locate = [&](int t, TileInfo& ti) {
     if (grouped) locate_grouped(p, walk, t, cursor, ti);
@@ -368,7 +370,10 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         TileInfo ti;
         locate(t, ti);
         // (rows past the end are filled with zeros)
-        const int n0 = kForm == kGated ? (cta == 0 ? 0 : half) + ti.n_tile * (p.width >> 1) : ti.n_tile * p.width + (int)cta * (p.width >> 1);
+        // (gated: the even CTA's are gates, the odd one's ups; halved: either has gates and their ups)
+        const int n0 = kForm != kGated ? ti.n_tile * p.width + (int)cta * (p.width >> 1)
+                       : ti.n_tile * (p.width >> 1) + (p.halved ? (int)cta * (p.width >> 2) : 0);
+        const int up = kForm == kGated && !p.halved ? (int)cta : 0;
         const uint32_t tx = 2 * p.w_bytes + ((ti.valid > 0) + (ti.valid > p.half_rows)) * p.x_bytes;
         for (int kb = 0; kb < p.num_kb;) {
           if (!ptx::paced::mbar_wait_s(empty0 + 8 * s, ph, abort_flag)) { ok = false; break; }
@@ -376,7 +381,8 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
           uint32_t to = st + s * p.stage_bytes;
           if (kWide) {   // (blocks past the end are zeros)
             if (cta == 0) ptx::mbar_expect_tx_s(full0 + 8 * s, tx * p.blocks);
-            ptx::tma_load_4d_pair(to, &tmap_w, bar, 0, n0, kb, ti.e);
+            if (kForm == kGated) ptx::tma_load_5d_pair(to, &tmap_w, bar, 0, n0, up, kb, ti.e);
+            else ptx::tma_load_4d_pair(to, &tmap_w, bar, 0, n0, kb, ti.e);
             kb += p.blocks;
           } else {
             const int end = min(kb + p.blocks, p.num_kb);
@@ -386,6 +392,8 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
               if (kWMn) {
                 ptx::tma_load_3d_pair(to, &tmap_w, bar, n0, k0, ti.e);
                 if (p.w_bytes > kOperand / 2) ptx::tma_load_3d_pair(to + kOperand / 2, &tmap_w, bar, n0 + 64, k0, ti.e);
+              } else if (kForm == kGated) {
+                ptx::tma_load_4d_pair(to, &tmap_w, bar, k0, n0, up, ti.e);
               } else {
                 ptx::tma_load_3d_pair(to, &tmap_w, bar, k0, n0, ti.e);
               }
@@ -598,24 +606,41 @@ CUtensorMapDataType map_type(DenseType t) {
   return t == kDenseI8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                        : t == kDenseBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
-// An operand of `rows` rows of k (mn: stored by column, k rows of `rows`), `stride` elements from one stored row to the next;
-// a load brings 128 bytes of `box_rows` stored rows.
-int operand_map(CUtensorMap* map, DenseType t, const void* base, int64_t rows, int64_t k, int64_t stride, bool mn, int experts, int box_rows) {
+// An operand of `rows` rows of k, `stride` elements from one to the next (mn: stored by column, k rows of `rows`); a load brings 128 bytes
+// of `box_rows` stored rows.  sets: of one after the other, or 0.
+int operand_map(CUtensorMap* map, DenseType t, const void* base, int64_t rows, int64_t k, int64_t stride, bool mn, int sets, int box_rows) {
   const int size = t == kDenseI8 ? 1 : 2;
   const int64_t inner = mn ? rows : k, outer = mn ? k : rows;
-  const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)std::max(experts, 1)};
+  const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)std::max(sets, 1)};
   const cuuint64_t strides[2] = {(cuuint64_t)(stride * size), (cuuint64_t)(stride * size * outer)};
   const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
-  return encode_map(map, map_type(t), experts > 0 ? 3 : 2, base, dims, strides, box);
+  return encode_map(map, map_type(t), sets > 0 ? 3 : 2, base, dims, strides, box);
 }
-// The same with the 128-byte blocks of a row as a dimension of their own, of which a load brings `blocks`: [128 bytes, rows, k / 128
-// bytes] and, with experts, [.., experts].  Rows are whole blocks.
-int wide_map(CUtensorMap* map, DenseType t, const void* base, int64_t rows, int64_t k, int64_t stride, int experts, int box_rows, int blocks) {
+// The dimensions of an operand that is stored by row, one by one.
+struct Dims {
+  cuuint64_t dims[5], strides[5];     // (strides[i]: of dimension i, in bytes)
+  cuuint32_t box[5];
+  int n = 0;
+  void add(int64_t size, int64_t stride, int64_t loaded) {
+    dims[n] = (cuuint64_t)size;
+    strides[n] = (cuuint64_t)stride;
+    box[n++] = (cuuint32_t)loaded;
+  }
+  int encode(CUtensorMap* map, DenseType t, const void* base) const { return encode_map(map, map_type(t), n, base, dims, strides + 1, box); }
+};
+// blocks > 0: rows are whole blocks of 128 bytes, of which a load brings as many.  parts: the rows' equal parts (gates and ups), of which it
+// brings `box_parts`, `box_rows` rows of each.
+int row_map(CUtensorMap* map, DenseType t, const void* base, int64_t rows, int64_t k, int64_t stride, int sets, int parts, int box_rows, int box_parts,
+            int blocks) {
   const int size = t == kDenseI8 ? 1 : 2, inner = 128 / size;
-  const cuuint64_t dims[4] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)(k / inner), (cuuint64_t)std::max(experts, 1)};
-  const cuuint64_t strides[3] = {(cuuint64_t)(stride * size), 128, (cuuint64_t)(stride * size * rows)};
-  const cuuint32_t box[4] = {(cuuint32_t)inner, (cuuint32_t)box_rows, (cuuint32_t)blocks, 1};
-  return encode_map(map, map_type(t), experts > 0 ? 4 : 3, base, dims, strides, box);
+  const int64_t pitch = stride * size;
+  Dims d;
+  d.add(blocks > 0 ? inner : k, size, inner);
+  d.add(rows / parts, pitch, box_rows);
+  if (parts > 1) d.add(parts, rows / parts * pitch, box_parts);
+  if (blocks > 0) d.add(k / inner, 128, blocks);
+  if (sets > 0) d.add(sets, rows * pitch, 1);
+  return d.encode(map, t, base);
 }
 // K blocks of a stage.  A wait, and what goes with it (the producers' arrivals, the issuer's commit to both CTAs), takes either single thread
 // some 360 cycles, a block's products 50 to 100, where the tensor cores have 512 cycles of work with 256 weight rows and 128 with 64.
@@ -634,17 +659,17 @@ void choose_tile(TcDense& p, int64_t sets, int64_t row_tiles, int features, bool
   for (int width = kTile; width >= 64; width -= step) {
     const int out = gated ? width / 2 : width, bytes = p.half_rows * 128 + (w_mn ? (width + 127) / 128 * 8192 : width * 64);
     const int64_t tiles = sets * row_tiles * ((features + out - 1) / out), rounds = (tiles + pairs - 1) / pairs;
-    const double block = std::max({300.0 / stage_blocks(width, bytes) + 170, 2.45 * width, bytes / 60.0});
+    const double block = std::max({300.0 / stage_blocks(width, bytes) + 170, (p.halved ? 1.25 : 2.45) * width, bytes / 60.0});
     const double cost = std::max(rounds * (p.num_kb * block + 2000), w_bytes / 3440.0);
     // (a narrower tile that promises little more gave nothing: 64 rows each of 8 experts of 4096 x 28672 175 us with 224, 170 with 256)
     if (p.width == 0 || cost < 0.94 * least) { p.width = width; least = cost; }
   }
 }
 bool stores_wide(const void* p, int64_t row_bytes, int64_t cols_bytes) { return ((uintptr_t)p | row_bytes | cols_bytes) % 16 == 0; }
-uint32_t idesc_of(DenseType t, bool x_mn, bool w_mn, int width) {
-  if (t == kDenseI8) return ptx::make_idesc_i8(256, width);
+uint32_t idesc_of(DenseType t, bool x_mn, bool w_mn, int rows, int width) {
+  if (t == kDenseI8) return ptx::make_idesc_i8(rows, width);
   const uint32_t fmt = t == kDenseBf16 ? 1u : 0u;
-  return ptx::make_idesc(fmt, fmt, x_mn ? 1u : 0u, w_mn ? 1u : 0u, 256, width);
+  return ptx::make_idesc(fmt, fmt, x_mn ? 1u : 0u, w_mn ? 1u : 0u, rows, width);
 }
 // What follows from a tile's width.
 void set_width(TcDense& p, DenseType t, bool x_mn, bool w_mn, int features, bool gated) {
@@ -655,7 +680,7 @@ void set_width(TcDense& p, DenseType t, bool x_mn, bool w_mn, int features, bool
   p.blocks = std::min(p.num_kb, stage_blocks(width, p.x_bytes + p.w_bytes));
   p.stage_bytes = p.blocks * (p.x_bytes + p.w_bytes);
   p.stages = std::min(kMaxStages, kRing / p.stage_bytes);
-  p.idesc = idesc_of(t, x_mn, w_mn, width);
+  p.idesc = idesc_of(t, x_mn, w_mn, p.halved ? 128 : 256, width);
 }
 
 }  // namespace
@@ -679,6 +704,7 @@ int dense_tc(const DenseJob& j, cudaStream_t st) {
   // some headroom).  The tensor cores always take 128 rows a CTA: those behind a CTA's own make sums of whatever follows in
   // shared memory, which nobody reads.
   p.half_rows = each > (grouped ? 96 : 128) ? 128 : each > (grouped ? 40 : 64) ? 64 : 32;
+  p.halved = p.half_rows <= 64;
   p.m_tiles = (int)((j.m + 2 * p.half_rows - 1) / (2 * p.half_rows));
   auto run = [&](auto kernel) {
     using K = decltype(kernel);
@@ -688,13 +714,10 @@ int dense_tc(const DenseJob& j, cudaStream_t st) {
                 sets * j.n * (int64_t)j.k * (j.type == kDenseI8 ? 1 : 2));
     set_width(p, j.type, false, false, n_out, j.gated);
     CUtensorMap tx, tw;
-    if (K::wide) {
-      if (int rc = wide_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, 0, p.half_rows, p.blocks)) return rc;
-      if (int rc = wide_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, j.experts, p.width / 2, p.blocks)) return rc;
-    } else {
-      if (int rc = operand_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, false, 0, p.half_rows)) return rc;
-      if (int rc = operand_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, false, j.experts, p.width / 2)) return rc;
-    }
+    const int blocks = K::wide ? p.blocks : 0;
+    if (int rc = row_map(&tx, j.type, j.x, j.m, j.k, j.x_stride, 0, 1, p.half_rows, 1, blocks)) return rc;
+    if (int rc = j.gated ? row_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, j.experts, 2, p.halved ? p.width / 4 : p.width / 2, p.halved ? 2 : 1, blocks)
+                         : row_map(&tw, j.type, j.w, j.n, j.k, j.w_stride, j.experts, 1, p.width / 2, 1, blocks)) return rc;
     const int64_t tiles = (p.m_tiles + (grouped ? (int64_t)j.experts : 0)) * p.n_tiles;
     return K::launch(tx, tw, p, std::min(pairs, tiles), j.early, st);
   };
@@ -709,6 +732,7 @@ int dense_plain(const PlainJob& j, cudaStream_t st) {
   p.d = j.d; p.status = j.status; p.m = j.m; p.d_stride = j.d_stride; p.n = j.n; p.experts = 1;
   p.num_kb = (int)((j.k + 63) / 64);
   p.half_rows = j.x_by_column || j.m > 128 ? 128 : j.m > 64 ? 64 : 32;
+  p.halved = p.half_rows <= 64;
   p.m_tiles = (int)((j.m + 2 * p.half_rows - 1) / (2 * p.half_rows));
   p.d_dtype = j.type == kDenseF16 ? B200MOE_F16 : B200MOE_BF16;
   p.d_wide = stores_wide(j.d, j.d_stride * 2, (int64_t)j.n * 2);

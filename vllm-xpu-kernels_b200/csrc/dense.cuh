@@ -43,17 +43,20 @@ constexpr int kQuantValues = 16384;
 bool dense_rows_quantises(int64_t rows, int k);
 int dense_tc(const DenseJob& j, cudaStream_t st);        // dense_tc.cu
 
-// Rows (of an expert, on average) up to which the kernel for a few rows takes a call; that kernel / the one for many, us.  By expert, layer
-// calls: 128 experts of 2048 x 768, 8 rows 129 / 139, 12 rows 139 / 141, 16 rows 170 / 142; 8 of 4096 x 14336, 8 rows 265 / 279, 12 rows
-// 288 / 278; 8 of 2048 x 1408, 8 rows 27 / 34, 20 rows 37 / 34.  One set of weights: 16 x 4096 x 4096 5.9 / 7.9, 16 x 7168 x 2048
-// gated 14.4 / 16.0, 20 rows 8.0 / 7.9 and 20.4 / 16.0.  Above 8 rows the tokens take as much of L2's time as the weights, which tells
-// where the weights are many: 12 x 14336 x 2048 9.3 / 11.1, 12 x 8192 x 8192 16.3 / 16.0, 12 x 28672 x 4096 31.9 / 25.5.
+// Which kernel takes a call; that for a few rows / that for many, us.  By expert: with two rows of an expert, on average, or fewer the first one; with
+// up to ten where the weights of all are few, so that what a call costs besides counts.  Layer calls: 128 experts of 2048 x 768, 1 row 85 / 81,
+// 4 rows 119 / 115, 10 rows 135 / 119; 8 of 4096 x 14336, 1 row 182 / 188, 3 rows 235 / 230, 10 rows 278 / 238; 8 of 2048 x 1408 (46 and 23 MB),
+// 4 rows 25 / 32, 10 rows 27 / 30, 16 rows 32 / 29.
+// One set: up to eight rows, and up to sixteen where the SMs have few tiles of weight rows each: then the tokens take as much of L2's
+// time as the weights.  16 x 4096 x 4096 5.9 / 7.5, 16 x 4096 x 14336 14.3 / 14.0, 12 x 7168 x 2048 gated 13.4 / 13.6, 16 x 8192 x 4096 10.2 / 9.9,
+// 9 x 14336 x 4096 15.8 / 13.6.
 constexpr int kDenseFewRows = 16, kGroupedFewRows = 10;
-constexpr int64_t kFewRowsBytes = 64 << 20;      // of weights, one set and more than 8 rows
+constexpr int64_t kFewBytes = 64 << 20;
 inline int dense(const DenseJob& j, cudaStream_t st) {
   const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m, mean = (rows + j.experts - 1) / j.experts;
-  const bool few = j.rows_per_expert != nullptr ? mean <= kGroupedFewRows
-                                                : mean <= 8 || (mean <= kDenseFewRows && (int64_t)j.n * j.k * (j.type == kDenseI8 ? 1 : 2) <= kFewRowsBytes);
+  const bool few = j.rows_per_expert != nullptr
+                       ? mean <= 2 || (mean <= kGroupedFewRows && std::min<int64_t>(j.experts, rows) * j.n * j.k <= kFewBytes)
+                       : mean <= 8 || (mean <= kDenseFewRows && j.n <= 64 * sm_count());
   return few ? dense_rows(j, st) : dense_tc(j, st);
 }
 

@@ -11,9 +11,10 @@
 // overlaps the products of the next.  Rows of X lie on the lanes: a thread of the epilogue owns one row, its
 // scale is one register, and gate and up of a gated tile (128 gates and their 128 ups are the tile's 256 weight rows) meet in one thread.
 //
-// How wide a tile is follows from what the pairs have to do (tile_width below): 256 weight rows share the rows of X best, fewer leave
-// fewer pairs idle in the last round.  Of a tile with few rows only those are brought in (what lies behind them in shared
-// memory makes sums of rows that nobody stores).
+// How wide a tile is follows from what the pairs have to do (choose_tile below): 256 weight rows share the rows of X best, fewer leave
+// fewer pairs idle in the last round.  Calls of up to 128 rows (an expert, on average) have tiles of 128 or 64 rows and instructions of
+// 128 (`halved`): a CTA's 64 rows lie on the first 64 lanes with the first half of the tile's columns, on the others with the second, so the
+// even CTA's weight rows, which are that first half, are then gates and their ups, and so are the odd one's.
 //
 //   warps 0 and 10: TMA producers of W and X;  warp 1: MMA issuer (even CTA), tensor memory;  warps 2-9: epilogue, every second 32
 //   columns each four
@@ -146,7 +147,7 @@ __device__ __forceinline__ void store_rows(uint8_t* at, int64_t pitch, int rows,
   } else {
     constexpr int kRows = 64 / B;
     const int c = lane % (B / 2) * 2;
-#pragma unroll 2
+#pragma unroll 8
     for (int r = lane / (B / 2); r < 32; r += kRows)
       if (r < rows && c < bytes) *reinterpret_cast<uint16_t*>(at + r * pitch + c) = ptx::lds16(place(r, c));
   }
@@ -643,15 +644,18 @@ int row_map(CUtensorMap* map, DenseType t, const void* base, int64_t rows, int64
   return d.encode(map, t, base);
 }
 // K blocks of a stage.  A wait, and what goes with it (the producers' arrivals, the issuer's commit to both CTAs), takes either single thread
-// some 360 cycles, a block's products 50 to 100, where the tensor cores have 512 cycles of work with 256 weight rows and 128 with 64.
-// 64 x 7168 x 2048 gated, tiles of 64 weight rows, 1 / 2 / 3 / 4 / 6 blocks a stage 33.9 / 18.7 / 16.2 / 16.2 / 16.3 us, of 128 - / 20.9 / 21.2 /
-// 21.4 / 25.7; 256 rows, tiles of 64 weight rows 34.1 / 24.0 / 24.4 / 28.9 / 42.3.
-int stage_blocks(int width, int block_bytes) { return width == kTile ? 1 : block_bytes <= 8192 ? 3 : 2; }
+// some 300 cycles, a block's instructions 100, where the tensor cores have 512 cycles of work with 256 weight rows and 256 rows of X, and
+// 64 with 64 and 128.  1 / 2 / 3 / 4 / 6 / 8 blocks a stage, us: 64 x 7168 x 2048 gated, tiles of 64 weight rows 27.0 / 18.5 / 15.8 / 14.0 / 14.1 / 14.7,
+// of 128 27.1 / 18.5 / 17.0 / 17.0, of 256 27.8 / 25.6 / 26.4 / 31.8 (few stages are left); 256 rows, tiles of 64 34.1 / 24.0 / 24.4 / 28.9 / 42.3.
+int stage_blocks(const TcDense& p, int width, int block_bytes) {
+  if (p.halved) return block_bytes <= 12288 ? 4 : 2;
+  return width == kTile ? 1 : block_bytes <= 8192 ? 3 : 2;
+}
 
-// Weight rows of a tile: what takes the fewest cycles by this estimate.  A K block of a tile takes 170 cycles and its share of the waits, 2.45 a
-// weight row in the tensor cores, and a cycle for each 60 of its bytes; a tile costs some 2000 besides; and the weights pass HBM at 3440
-// bytes a cycle at the most.  2000 x 4096 x 4096 from codes with 64 / 128 / 192 / 256 weight rows 46 / 31 / 29 / 26 us, 1001 x 2016 x 2032
-// 11.8 / 9.3 / 10.9 / 12.1, 64 x 4096 x 4096 8.5 / 10.0 / 12.5 / 15.3; 15 rows each of 8 experts of 4096 x 14336, a layer, 440 / 300 / 284 / 266.
+// Weight rows of a tile: what takes the fewest cycles by this estimate.  A K block of a tile takes the issuer's time, the tensor cores' for
+// its weight rows, or a cycle for each 60 of its bytes; a tile costs some 1400 to 2000 besides; and the weights pass HBM at 3440 bytes a
+// cycle at the most.  With 64 / 128 / 192 / 256 weight rows, us: 2000 x 4096 x 4096 46 / 31 / 29 / 26, 1001 x 2016 x 2032 11.8 / 9.3 / 10.9 / 12.1,
+// 64 x 4096 x 4096 7.1 / 7.8 / 8.7 / 10.4, 64 x 14336 x 4096 15.1 / 13.8 / 16.6 / 14.0, 16 rows each of 128 experts of 768 x 2048 64 / 41 / 37 / 36.
 void choose_tile(TcDense& p, int64_t sets, int64_t row_tiles, int features, bool gated, bool w_mn, int64_t pairs, int64_t w_bytes) {
   const int step = gated ? 64 : 32;
   double least = 0;
@@ -659,10 +663,12 @@ void choose_tile(TcDense& p, int64_t sets, int64_t row_tiles, int features, bool
   for (int width = kTile; width >= 64; width -= step) {
     const int out = gated ? width / 2 : width, bytes = p.half_rows * 128 + (w_mn ? (width + 127) / 128 * 8192 : width * 64);
     const int64_t tiles = sets * row_tiles * ((features + out - 1) / out), rounds = (tiles + pairs - 1) / pairs;
-    const double block = std::max({300.0 / stage_blocks(width, bytes) + 170, (p.halved ? 1.25 : 2.45) * width, bytes / 60.0});
-    const double cost = std::max(rounds * (p.num_kb * block + 2000), w_bytes / 3440.0);
-    // (a narrower tile that promises little more gave nothing: 64 rows each of 8 experts of 4096 x 28672 175 us with 224, 170 with 256)
-    if (p.width == 0 || cost < 0.94 * least) { p.width = width; least = cost; }
+    const int g = stage_blocks(p, width, bytes);
+    const double block = p.halved ? std::max({280.0 / g + 100, 1.25 * width, bytes / 60.0}) : std::max({300.0 / g + 170, 2.45 * width, bytes / 60.0});
+    const double cost = std::max(rounds * (p.num_kb * block + (p.halved ? 1400 : 2000)), w_bytes / 3440.0);
+    // (of several rounds, a narrower tile that promises little more gave nothing: 64 rows each of 8 experts of 4096 x 28672 175 us with 224,
+    // 170 with 256)
+    if (p.width == 0 || cost < (rounds > 1 ? 0.94 : 1.0) * least) { p.width = width; least = cost; }
   }
 }
 bool stores_wide(const void* p, int64_t row_bytes, int64_t cols_bytes) { return ((uintptr_t)p | row_bytes | cols_bytes) % 16 == 0; }
@@ -677,7 +683,7 @@ void set_width(TcDense& p, DenseType t, bool x_mn, bool w_mn, int features, bool
   p.n_tiles = (features + (gated ? width / 2 : width) - 1) / (gated ? width / 2 : width);
   p.x_bytes = p.half_rows * 128;
   p.w_bytes = w_mn ? (width > 128 ? kOperand : kOperand / 2) : width * 64;
-  p.blocks = std::min(p.num_kb, stage_blocks(width, p.x_bytes + p.w_bytes));
+  p.blocks = std::min(p.num_kb, stage_blocks(p, width, p.x_bytes + p.w_bytes));
   p.stage_bytes = p.blocks * (p.x_bytes + p.w_bytes);
   p.stages = std::min(kMaxStages, kRing / p.stage_bytes);
   p.idesc = idesc_of(t, x_mn, w_mn, p.halved ? 128 : 256, width);
@@ -700,10 +706,11 @@ int dense_tc(const DenseJob& j, cudaStream_t st) {
   const bool grouped = j.rows_per_expert != nullptr;
   const int64_t rows = j.rows_hint > 0 && j.rows_hint < j.m ? j.rows_hint : j.m, each = (rows + j.experts - 1) / j.experts;
   const int64_t sets = grouped ? std::min<int64_t>(j.experts, rows) : 1;
-  // Rows of a tile: 256, fewer for fewer, which leaves more room for weights on their way (routing is never even, so sets of rows get
-  // some headroom).  The tensor cores always take 128 rows a CTA: those behind a CTA's own make sums of whatever follows in
-  // shared memory, which nobody reads.
-  p.half_rows = each > (grouped ? 96 : 128) ? 128 : each > (grouped ? 40 : 64) ? 64 : 32;
+  // Rows of a tile: 256, 128 or 64 (routing is never even, so sets of rows get some headroom for 64).  Of 128 and fewer the tensor cores take
+  // half the time, and an epilogue warp has half the columns: 128 rows each of 8 experts of 4096 x 28672 162 us, 186 with tiles of 256; of
+  // 256 rows on average 294 and 284 (128 experts of 2048 x 768, a layer).  64 bring half as many rows of X as 128, of which there may be fewer still:
+  // what follows them in shared memory makes sums that nobody reads.
+  p.half_rows = each > 128 ? 128 : each > (grouped ? 40 : 64) ? 64 : 32;
   p.halved = p.half_rows <= 64;
   p.m_tiles = (int)((j.m + 2 * p.half_rows - 1) / (2 * p.half_rows));
   auto run = [&](auto kernel) {

@@ -207,7 +207,7 @@ int grouped_gemm_i8(const b200moe_gemm_args* a, cudaStream_t st) {
   j.max_ctas = a->max_ctas; j.type = kDenseI8; j.x_dtype = B200MOE_I8; j.gated = gated; j.d_dtype = a->d_dtype;
   j.bias_f16 = (f32 ? a->mid_dtype : a->d_dtype) == B200MOE_F16;
   j.clamp = gated ? a->clamp_limit : 0.f;
-  j.early = a->m <= kEarlyLaunchRows;
+  j.early = a->m <= kEarlyStayingRows;
   return dense(j, st);
 }
 

@@ -173,7 +173,7 @@ int launch_rows(const QuantInt8Params& p, int nvec, cudaStream_t st) {
     cached.store(std::max(n, 1), std::memory_order_relaxed);
   }
   const int64_t blocks = std::min<int64_t>((p.rows + per_block - 1) / per_block, (int64_t)std::max(n, 1) * sm_count());
-  B200_LAUNCHED("quant_int8_rows_kernel", launch_pdl(p.rows <= kEarlyLaunchRows, kern, dim3((unsigned)blocks), dim3(block), 0, st, p, threads));
+  B200_LAUNCHED("quant_int8_rows_kernel", launch_pdl(p.rows <= kEarlyStayingRows, kern, dim3((unsigned)blocks), dim3(block), 0, st, p, threads));
   return B200MOE_OK;
 }
 

@@ -377,3 +377,51 @@ def test_expert_parallel_over_peer_memory(native, ep, tokens):
             layers[r].finish(out)
             if tokens[r]:
                 _check(out, *given[r], w13, s13, None, w2, s2, None, parts=2.0 ** -8)
+
+
+def test_first_calls_under_capture():
+    """A process whose first call of every operator is captured, and replayed on other inputs."""
+    import subprocess
+    import sys
+
+    from conftest import PKG_DIR
+    code = f"""
+import sys
+sys.path.insert(0, {str(PKG_DIR)!r})
+import torch
+import vllm_xpu_kernels.fused_moe_interface as fmi
+from vllm_xpu_kernels.gated_linear import gated_linear
+gen = torch.Generator().manual_seed(1)
+B16, DEV = torch.bfloat16, "cuda"
+def codes(*shape):
+    return torch.randint(-127, 128, shape, generator=gen, dtype=torch.int8).to(DEV), (torch.rand(shape[:-1], generator=gen) * 1e-3).to(DEV)
+E, K, H, I = 8, 2, 128, 64
+layer = fmi.XpuFusedMoe(*codes(E, 2 * I, H), None, *codes(E, H, I), None, K, "silu", E)
+w, ws = codes(48, H)
+g = torch.randn(2 * I, H, generator=gen).to(B16).to(DEV).requires_grad_(True)
+runs = []
+for T in (3, 40, 300):
+    x = torch.randn(T, H, generator=gen).to(B16).to(DEV)
+    top = torch.rand(T, E, generator=gen).topk(K, dim=-1)
+    weights, ids = torch.softmax(top.values, -1).to(DEV), top.indices.int().to(DEV)
+    d = torch.randn(T, I, generator=gen).to(B16).to(DEV)
+    out, dense = torch.empty(T, H, dtype=B16, device=DEV), torch.empty(T, 48, dtype=B16, device=DEV)
+    def run(T=T, x=x, weights=weights, ids=ids, d=d, out=out, dense=dense):
+        layer.apply(out, x, weights, ids)
+        torch.ops._xpu_C.b200_int8_linear(dense, x, None, w, ws)
+        y = gated_linear(x, g)
+        return out, dense, y.detach(), torch.autograd.grad(y, g, d)[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    runs.append((run, x, graph, got))
+for run, x, graph, got in runs:
+    for _ in range(2):
+        x.copy_(torch.randn(x.shape, generator=gen))
+        graph.replay()
+        got2 = [t.clone() for t in got]
+        assert all(torch.equal(a, b) for a, b in zip(got2, run()))
+print("the same")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "the same" in done.stdout, done.stderr[-2000:]

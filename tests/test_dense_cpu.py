@@ -128,6 +128,11 @@ def test_grouped_int8_refused_before_any_launch(lib, change, message):
     assert message in lib.b200moe_last_error()
 
 
+def test_grouped_int8_without_rows_is_no_launch(lib):
+    a = dict(a_dtype=10, w=256, w_format=9, w_scale=256, d_dtype=2, rows_per_expert=256, m=0, n=16, k=64, num_experts=4)
+    assert lib.b200moe_grouped_gemm(ct.byref(_filled(GemmArgs, **a)), None) == 0
+
+
 def test_quantiser_refused_before_any_launch(lib):
     call = lambda rows=4, hidden=64, dtype=2, x=256, q=256, s=256, segments=None, n=0: lib.b200moe_quant_int8_rows(  # noqa: E731
         P(x), dtype, L(hidden), P(q), L(hidden), P(s), L(rows), hidden, 0, P(segments), n, None)

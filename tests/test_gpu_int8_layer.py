@@ -67,7 +67,9 @@ def _check(out, x, weights, ids, w13, s13, b13, w2, s2, b2, act=_silu, clamp=Non
         y, off = _exact_rows(x[t], w13[e], s13[e], b(b13), w2[e], s2[e], b(b2), act, clamp)
         w = weights[t, k].double()[:, None]
         want.index_add_(0, t, w * y)
-        tol.index_add_(0, t, w.abs() * (off + (y.abs() + off) * (step + 10 * U + parts * (1 + step))))     # rows are rounded, then added up in fp32
+        # rows are rounded, half a step of their size or of the type's subnormal numbers (a row's -1.208e-5 of float16, weight 0.47, may be off by
+        # 2^-25 of them: 1.4e-8, and their sum by as much as that and 2^-25), then added up in fp32
+        tol.index_add_(0, t, w.abs() * (off + (y.abs() + off) * (step + 10 * U + parts * (1 + step)) + torch.finfo(dtype).smallest_normal * step))
     tol = tol + (want.abs() + tol) * step * (1 + 2.0 ** -10)
     err = (out.double() - want).abs()
     assert torch.all(err <= tol), float((err / tol).max())

@@ -181,7 +181,8 @@ namespace b200moe {
 // b200moe_grouped_gemm with int8 weights.
 int grouped_gemm_i8(const b200moe_gemm_args* a, cudaStream_t st) {
   const bool gated = a->epilogue == B200MOE_EPI_SILU_MUL, f32 = a->d_dtype == B200MOE_F32;
-  B200_CHECK_ARG(a->a_dtype == B200MOE_I8 && a->a_scale != nullptr && a->w_scale != nullptr,
+  // (no rows: nor are there scales of them)
+  B200_CHECK_ARG(a->a_dtype == B200MOE_I8 && (a->a_scale != nullptr || a->m == 0) && a->w_scale != nullptr,
                  "grouped_gemm: int8 weights need int8 rows and the scales of both");
   B200_CHECK_ARG(a->k % 16 == 0 && a->k <= B200MOE_INT8_MAX_K,
                  "grouped_gemm: int8 weights need K divisible by 16 and at most %d", B200MOE_INT8_MAX_K);

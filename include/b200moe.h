@@ -441,7 +441,7 @@ int b200moe_grouped_gemm(const b200moe_gemm_args* args, b200moe_stream stream);
 
 /* Rows as 8-bit integers with one scale each: v = in, or with `gated` silu(gate) * up of rows
  * [gate(hidden) | up(hidden)]; a = max(amax|v|, 1e-10), scale = a / 127 in fp32, q the whole number nearest to 127 v / a,
- * ties to even (F32 and gated: to 127 * 2^-23 of a step).  A row with a NaN or an infinity has a scale of NaN.  in [rows, hidden (gated: 2 hidden)] F32, F16 or BF16,
+ * ties to even (F32, gated, and rows below 1e-10: to 127 * 2^-23 of a step).  A row with a NaN or an infinity has a scale of NaN.  in [rows, hidden (gated: 2 hidden)] F32, F16 or BF16,
  * in_stride / q_stride elements from row to row; scales [rows].  rows_per_segment (int32 [num_segments], device) or NULL:
  * only the first sum(rows_per_segment) rows are read and written.  No counterpart op in the reference. */
 int b200moe_quant_int8_rows(const void* in, b200moe_dtype dtype, int64_t in_stride, int8_t* q, int64_t q_stride,

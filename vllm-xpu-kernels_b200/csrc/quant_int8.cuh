@@ -1,7 +1,7 @@
 // A row's scale and codes, from a = max(amax|v|, 1e-10): scale = a / 127, rounded to fp32; q = 127 v / a as the nearest whole number, ties
 // to even.
 //
-// Rows of 16-bit values get that q exactly.  Half of the row's largest value is a tie, 63.5, and common: some three of 2048 bfloat16
+// Rows of 16-bit values (the largest of them no less than 1e-10) get that q exactly.  Half of the row's largest value is a tie, 63.5, and common: some three of 2048 bfloat16
 // values, and two roundings of a quotient leave it to chance which way they go, which the codes of a layer's second GEMM, whose rows are quantised
 // again, multiply (0.9 % of the result where 16 bits cost 0.17 %).  So the product with 127 / a is not rounded, and 127 / a is rounded up:
 //   * a tie k + 1/2 of 254 v = (2 k + 1) a needs a 127 among its factors.  Is 2 k + 1 = 127, the tie goes up to 64, which is even, as it does

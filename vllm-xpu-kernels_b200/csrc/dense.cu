@@ -84,8 +84,12 @@ int check_gated(const b200moe_gated_linear_args* a) {
 
 using namespace b200moe;
 
+// Codes of rows that are quantised on the way: longer ones begin on 128 bytes, so that 128 bytes of a row are one line of L2, not parts of two
+// (4000 x 4096 x 4080 71.7 -> 59.5 us, 64 rows 11.0 -> 9.9; 30 x 3000 x 1504 7.2 -> 7.3).
+static int64_t codes_pitch(int k) { return k <= 128 ? k : ((int64_t)k + 127) / 128 * 128; }
+
 extern "C" size_t b200moe_int8_linear_workspace_bytes(int64_t rows, int k) {
-  return rows <= 0 || k <= 0 ? 0 : (size_t)rows * k + (size_t)rows * 4;
+  return rows <= 0 || k <= 0 ? 0 : (size_t)rows * codes_pitch(k) + (size_t)rows * 4;
 }
 
 extern "C" int b200moe_int8_linear(const b200moe_int8_linear_args* a, b200moe_stream stream) {
@@ -113,10 +117,11 @@ extern "C" int b200moe_int8_linear(const b200moe_int8_linear_args* a, b200moe_st
     if (a->workspace == nullptr || a->workspace_bytes < b200moe_int8_linear_workspace_bytes(a->rows, a->k) || !aligned16(a->workspace))
       return fail(B200MOE_E_WORKSPACE, "int8_linear: workspace missing, too small or not 16-byte aligned");
     int8_t* const q = (int8_t*)a->workspace;
-    float* const s = (float*)(q + a->rows * a->k);
-    if (int rc = b200moe_quant_int8_rows(a->x, a->x_dtype, a->x_stride, q, a->k, s, a->rows, a->k, 0, nullptr, 0, stream)) return rc;
+    const int64_t pitch = codes_pitch(a->k);
+    float* const s = (float*)(q + a->rows * pitch);
+    if (int rc = b200moe_quant_int8_rows(a->x, a->x_dtype, a->x_stride, q, pitch, s, a->rows, a->k, 0, nullptr, 0, stream)) return rc;
     b200moe_int8_linear_args b = *a;
-    b.x = q; b.x_scale = s; b.x_dtype = B200MOE_I8; b.x_stride = a->k;
+    b.x = q; b.x_scale = s; b.x_dtype = B200MOE_I8; b.x_stride = pitch;
     return b200moe_int8_linear(&b, stream);
   }
   j.x = a->x; j.w = a->w; j.x_scale = a->x_scale; j.w_scale = a->w_scale; j.bias = a->bias; j.d = a->d; j.status = a->status;

@@ -52,7 +52,12 @@ gated_grad_kernel(const T* grad, const float* pre, T* both, int64_t rows, int in
   }
 }
 
-int64_t both_stride(int inter) { return ((int64_t)2 * inter + 7) / 8 * 8; }   // (rows of 16-byte pieces, for TMA)
+// Rows of 16-byte pieces, for TMA; longer ones begin on 128 bytes, so that 128 bytes of a row are one line of L2 (both gradients of 4096 x
+// 7168 x 2044 415 -> 375 us, of 1001 x 2048 x 1404 40.4 -> 36.7).
+int64_t both_stride(int inter) {
+  const int64_t n = 2 * (int64_t)inter, to = n <= 64 ? 8 : 64;
+  return (n + to - 1) / to * to;
+}
 
 template <typename T>
 int gated_grad(const b200moe_gated_linear_args* a, T* both, cudaStream_t st) {

@@ -161,6 +161,13 @@ at::Tensor grouped_gemm_impl(at::Tensor& ptr_A, const std::optional<at::Tensor>&
                              bool mid_f16 = false) {
   check_cuda(ptr_A, "ptr_A");
   const auto A_dtype = ptr_A.scalar_type();
+  // (a kernel that is given another device's pointer faults)
+  auto same_device = [&](const std::optional<at::Tensor>& t, const char* name) {
+    TORCH_CHECK(!t.has_value() || t->device() == ptr_A.device(), name, " must be on the device of ptr_A");
+  };
+  same_device(ptr_B, "ptr_B"); same_device(ptr_B_scale, "ptr_scales"); same_device(ptr_bias, "ptr_bias"); same_device(ptr_D, "ptr_D");
+  same_device(rows_per_expert, "rows_per_expert"); same_device(ptr_D_scale, "ptr_D_scale");
+  if (A_dtype != at::kBFloat16 && A_dtype != at::kHalf) same_device(ptr_A_scale, "ptr_A_scale");   // (else it is not read)
   TORCH_CHECK(ptr_A.dim() == 2, "ptr_A must be 2D [Total_M, K]");
   TORCH_CHECK(ptr_D.dim() == 2, "ptr_D must be 2D [Total_M, N]");
   if (ptr_bias.has_value()) TORCH_CHECK(ptr_bias->dim() == 2, "ptr_bias must be 2D [num_experts, N]");

@@ -490,7 +490,7 @@ typedef struct {
   void* workspace;        /* backward: ..._workspace_bytes, 16-byte aligned           */
   size_t workspace_bytes;
   int64_t rows, x_stride, out_stride, grad_stride, grad_x_stride;
-  int inter, hidden;      /* hidden: a multiple of 8                                  */
+  int inter, hidden;      /* hidden: a multiple of 8; either at most 2^29            */
   b200moe_dtype dtype;    /* F16 or BF16, of all matrices but pre                     */
   int32_t* status;        /* as in b200moe_gemm_args, or NULL                         */
 } b200moe_gated_linear_args;

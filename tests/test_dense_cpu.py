@@ -190,3 +190,22 @@ def test_int8_layers_are_told_apart(native):
             native.XpuFusedMoe(w13, s13, None, w2, s2, None, 1, bad.pop("activation", "silu"), E, **bad)
     with pytest.raises(ValueError, match="both"):
         native.XpuFusedMoe(w13, s13, None, w2, None, None, 1, "silu", E)
+
+
+@pytest.mark.parametrize("hidden", [(1 << 29) + 8, 1 << 30, (1 << 31) - 8])
+def test_gated_rows_whose_bytes_32_bits_do_not_hold_are_refused(lib, hidden):
+    """Rows are counted in bytes: of 2^30 values and more nothing was multiplied, and zeros came out."""
+    a = {**GATED, "hidden": hidden, "x_stride": hidden, "grad_x_stride": hidden}
+    assert lib.b200moe_gated_linear(ct.byref(_filled(GatedLinearArgs, **a)), None) == -1
+    assert b"too large" in lib.b200moe_last_error()
+    assert lib.b200moe_gated_linear_backward(ct.byref(_filled(GatedLinearArgs, **a, grad=256, pre=256, grad_x=256)), None) == -1
+    assert b"too large" in lib.b200moe_last_error()
+
+
+def test_weight_rows_that_32_bits_do_not_hold_with_a_tile_more_are_refused(lib):
+    n = (1 << 31) - 8
+    assert lib.b200moe_int8_linear(ct.byref(_filled(Int8LinearArgs, **{**LINEAR, "n": n, "d_stride": n})), None) == -1
+    assert b"too large" in lib.b200moe_last_error()
+    a = dict(a=256, a_dtype=10, a_scale=256, w=256, w_format=9, w_scale=256, d=256, d_dtype=2, rows_per_expert=256, m=4, n=n, k=64, num_experts=1)
+    assert lib.b200moe_grouped_gemm(ct.byref(_filled(GemmArgs, **a)), None) == -1
+    assert b"too many rows or features" in lib.b200moe_last_error()

@@ -72,11 +72,14 @@ int gated_grad(const b200moe_gated_linear_args* a, T* both, cudaStream_t st) {
   return B200MOE_OK;
 }
 
+constexpr int kMaxValues = 1 << 29;      // of a gated product's rows and half of its weight rows
+constexpr int kMaxFeatures = 0x7fffffff - 512;   // of an int8 product: weight rows, with those that its last tile would have, fit 32 bits
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int check_gated(const b200moe_gated_linear_args* a) {
   B200_CHECK_ARG(a != nullptr, "gated_linear: null argument struct");
-  B200_CHECK_ARG(a->rows >= 0 && a->rows <= 0x7fffffff && a->inter >= 0 && a->inter <= (1 << 29) && a->hidden >= 0,
+  // (the kernels count a row's bytes and the weights' rows in 32 bits)
+  B200_CHECK_ARG(a->rows >= 0 && a->rows <= 0x7fffffff && a->inter >= 0 && a->inter <= kMaxValues && a->hidden >= 0 && a->hidden <= kMaxValues,
                  "gated_linear: negative or too large size");
   B200_CHECK_ARG(a->dtype == B200MOE_BF16 || a->dtype == B200MOE_F16, "gated_linear: only float16 and bfloat16 are supported");
   B200_CHECK_ARG(a->hidden % 8 == 0 && a->x_stride % 8 == 0, "gated_linear: rows must be multiples of 16 bytes apart and long");
@@ -99,7 +102,8 @@ extern "C" size_t b200moe_int8_linear_workspace_bytes(int64_t rows, int k) {
 
 extern "C" int b200moe_int8_linear(const b200moe_int8_linear_args* a, b200moe_stream stream) {
   B200_CHECK_ARG(a != nullptr, "int8_linear: null argument struct");
-  B200_CHECK_ARG(a->rows >= 0 && a->rows <= 0x7fffffff && a->n >= 0 && a->k >= 0, "int8_linear: negative or too large size");
+  B200_CHECK_ARG(a->rows >= 0 && a->rows <= 0x7fffffff && a->n >= 0 && a->n <= kMaxFeatures && a->k >= 0,
+                 "int8_linear: negative or too large size");
   B200_CHECK_ARG(a->k <= B200MOE_INT8_MAX_K, "int8_linear: K must be at most %d, so that sums fit 32 bits", B200MOE_INT8_MAX_K);
   B200_CHECK_ARG(a->k > 0 && a->k % 16 == 0, "int8_linear: rows must be multiples of 16 values long");
   B200_CHECK_ARG(a->x_dtype == B200MOE_I8 || a->x_dtype == B200MOE_F32 || a->x_dtype == B200MOE_F16 || a->x_dtype == B200MOE_BF16,
@@ -204,7 +208,7 @@ int grouped_gemm_i8(const b200moe_gemm_args* a, cudaStream_t st) {
   B200_CHECK_ARG(a->w_experts == 0 || a->w_experts == a->num_experts,
                  "grouped_gemm: row segments that share weight sets need 16-bit or block-scaled fp8 weights");
   B200_CHECK_ARG(a->num_experts <= kMaxExperts, "grouped_gemm: more than %d experts", kMaxExperts);
-  B200_CHECK_ARG(a->m <= 0x7fffffff, "grouped_gemm: too many rows");
+  B200_CHECK_ARG(a->m <= 0x7fffffff && a->n <= kMaxFeatures, "grouped_gemm: too many rows or features");
   if (a->m == 0 || a->n == 0) return B200MOE_OK;
   B200_CHECK_ARG(a->a && a->w && a->d && a->rows_per_expert, "grouped_gemm: null pointer");
   B200_CHECK_ARG(aligned16(a->a) && aligned16(a->w), "grouped GEMM: A, W and D must be 16-byte aligned");

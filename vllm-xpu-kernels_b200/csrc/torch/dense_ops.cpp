@@ -112,7 +112,8 @@ b200moe_gated_linear_args gated_args(const at::Tensor& input, const at::Tensor& 
   same_device(weight, input, op, "weight");
   b200moe_gated_linear_args a = {};
   const int64_t rows = rows_of(input);
-  TORCH_CHECK(rows <= 0x7fffffff && weight.size(0) <= 0x3fffffff && weight.size(1) <= 0x7fffffff, op, ": too large");
+  TORCH_CHECK(rows <= 0x7fffffff && weight.size(0) <= 1 << 30 && weight.size(1) <= 1 << 29, op,
+              ": too large (rows of at most 2^29 values, 2^30 of them in weight)");
   a.x = input.data_ptr(); a.w = weight.data_ptr();
   a.rows = rows; a.inter = (int)(weight.size(0) / 2); a.hidden = (int)weight.size(1);
   a.x_stride = row_stride(input, op, "input");

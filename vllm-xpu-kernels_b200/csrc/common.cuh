@@ -164,6 +164,22 @@ __device__ __forceinline__ float e8m0_to_f32(uint32_t b) {
   return __uint_as_float(b << 23);
 }
 
+// ---- activations -------------------------------------------------------------
+// Minimum and maximum that keep a NaN.  (fminf and fmaxf give the other operand: behind a limit a row that is not finite looks like one that is.)
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float clamp_nan(float v, float limit) { return max_nan(min_nan(v, limit), -limit); }
+// 1 / (1 + e^-g) by the hardware's exponential and quotient: some 2^-20 of the value, and 2^-23 |g| for the exponential's argument.
+__device__ __forceinline__ float fast_sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
+
 // ---- 16-byte vector load/store ---------------------------------------------
 struct alignas(16) vec16 { uint32_t w[4]; };
 

@@ -37,7 +37,7 @@ gated_grad_kernel(const T* grad, const float* pre, T* both, int64_t rows, int in
     T dg[N], du[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const float s = __fdividef(1.0f, 1.0f + __expf(-g[k])), x = to_f32<T>(d[k]);
+      const float s = fast_sigmoid(g[k]), x = to_f32<T>(d[k]);
       dg[k] = from_f32<T>(x * u[k] * s * (1.0f + g[k] * (1.0f - s)));
       du[k] = from_f32<T>(x * g[k] * s);
     }

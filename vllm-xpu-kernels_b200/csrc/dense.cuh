@@ -61,10 +61,10 @@ inline int dense(const DenseJob& j, cudaStream_t st) {
 }
 
 namespace {
-// silu(gate) * up.  The hardware's exponential and quotient: some 2^-21 of the value.
+// silu(gate) * up.  A limit keeps a NaN: all that marks an int8 row that is not finite is its scale, and so its products.
 __device__ __forceinline__ float gated_product(float g, float u, float clamp) {
-  if (clamp > 0.f) { g = fminf(g, clamp); u = fminf(fmaxf(u, -clamp), clamp); }
-  return g * __fdividef(1.0f, 1.0f + __expf(-g)) * u;
+  if (clamp > 0.f) { g = min_nan(g, clamp); u = clamp_nan(u, clamp); }
+  return g * fast_sigmoid(g) * u;
 }
 __device__ __forceinline__ void store_as(void* d, b200moe_dtype t, int64_t at, float v) {
   if (t == B200MOE_F32) reinterpret_cast<float*>(d)[at] = v;

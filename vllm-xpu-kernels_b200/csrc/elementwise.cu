@@ -56,7 +56,7 @@ silu_and_mul_kernel(T* __restrict__ out, const T* __restrict__ in, int d, bool v
 // Other gated activations of the layer (csrc/activation.cpp:45-75, 299-312 of the
 // reference).  kKind 1: gelu (erf), 2: gelu (tanh form): out = T(act(x)) *_T y as
 // in silu_and_mul; 3: swiglustep: out = T(min(silu(g), limit) * clamp(u, +-limit))
-// in fp32; 4: relu2_no_mul: out = T(max(x, 0)^2), no second half.
+// in fp32; 4: relu2_no_mul: out = T(max(x, 0)^2), no second half.  A NaN stays one.
 template <typename T, int kKind>
 __device__ __forceinline__ T gated_act(T gv, T uv, float limit) {
   const float f = to_f32<T>(gv);
@@ -68,11 +68,9 @@ __device__ __forceinline__ T gated_act(T gv, T uv, float limit) {
     const T a = from_f32<T>(0.5f * f * (1.0f + tanhf(inner)));
     return from_f32<T>(to_f32<T>(a) * to_f32<T>(uv));
   } else if (kKind == 3) {
-    const float sg = fminf(silu_f32(f), limit);
-    const float u = fminf(fmaxf(to_f32<T>(uv), -limit), limit);
-    return from_f32<T>(sg * u);
+    return from_f32<T>(min_nan(silu_f32(f), limit) * clamp_nan(to_f32<T>(uv), limit));
   } else {
-    const float r = fmaxf(f, 0.0f);
+    const float r = max_nan(f, 0.0f);
     return from_f32<T>(r * r);
   }
 }
@@ -108,8 +106,8 @@ gated_act_kernel(T* __restrict__ out, const T* __restrict__ in, int d, float lim
 }
 
 __device__ __forceinline__ float swigluoai_f32(float g, float u, float alpha, float limit) {
-  g = fminf(g, limit);
-  u = fminf(fmaxf(u, -limit), limit);
+  g = min_nan(g, limit);
+  u = clamp_nan(u, limit);
   const float sig = 1.0f / (1.0f + expf(-g * alpha));
   return (u + 1.0f) * g * sig;
 }

@@ -76,19 +76,6 @@ __device__ __forceinline__ int local_expert(const FewParams& p, int slot) {
   return e >= 0 && e < p.experts ? e : -1;
 }
 
-// Minimum and maximum that keep a NaN.
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float d;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float clamp_nan(float v, float limit) { return max_nan(min_nan(v, limit), -limit); }
-
 // The gated activation in fp32, unrounded.
 __device__ __forceinline__ float gated(int act, float alpha, float limit, float clamp, float g, float u) {
   if (clamp > 0.f) {

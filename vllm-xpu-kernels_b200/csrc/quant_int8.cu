@@ -20,8 +20,7 @@ struct QuantInt8Params {
   int hidden, num_segments;
 };
 
-// silu(gate) * up.  The hardware's exponential and quotient: some 2^-20 of the value, and 2^-23 |gate| for the exponential's argument.
-__device__ __forceinline__ float gated_value(float g, float u) { return g * __fdividef(1.0f, 1.0f + __expf(-g)) * u; }
+__device__ __forceinline__ float gated_value(float g, float u) { return g * fast_sigmoid(g) * u; }   // silu(gate) * up
 
 __device__ __forceinline__ int64_t rows_in_use(const QuantInt8Params& p) {
   if (p.rows_per_segment == nullptr) return p.rows;

@@ -26,13 +26,6 @@ constexpr int64_t kEarlyStayingRows = 32768;
 
 namespace {
 
-// Maximum that keeps a NaN.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
 // The largest of a warp's values, in every lane.
 __device__ __forceinline__ float warp_largest(float m) {
 #pragma unroll

@@ -32,13 +32,6 @@ struct RmsParams {
   uint32_t least;      // bits of the least sum of squares that eps does not cover (see row_factor)
 };
 
-// Maximum that keeps a NaN.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
 // Smallest power of two that is at least x (x > 0, normal); NaN and infinity stay.
 __device__ __forceinline__ float up_to_pow2(float x) {
   const uint32_t b = __float_as_uint(x);

@@ -209,3 +209,16 @@ def test_weight_rows_that_32_bits_do_not_hold_with_a_tile_more_are_refused(lib):
     a = dict(a=256, a_dtype=10, a_scale=256, w=256, w_format=9, w_scale=256, d=256, d_dtype=2, rows_per_expert=256, m=4, n=n, k=64, num_experts=1)
     assert lib.b200moe_grouped_gemm(ct.byref(_filled(GemmArgs, **a)), None) == -1
     assert b"too many rows or features" in lib.b200moe_last_error()
+
+
+@pytest.mark.parametrize("operand", [0, 1])
+def test_forward_mode_derivatives_of_the_gated_product_are_refused(native, operand):
+    """(On any device: below autograd the tangent would be lost, and the derivative come out as zero.)"""
+    from vllm_xpu_kernels.gated_linear import gated_linear
+    operands = [torch.ones(2, 16, dtype=torch.bfloat16), torch.ones(8, 16, dtype=torch.bfloat16)]
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: gated_linear(*operands[:operand], t, *operands[operand + 1:]), (operands[operand],), (operands[operand],))
+    with torch.autograd.forward_ad.dual_level():
+        operands[operand] = torch.autograd.forward_ad.make_dual(operands[operand], torch.ones_like(operands[operand]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            gated_linear(*operands)

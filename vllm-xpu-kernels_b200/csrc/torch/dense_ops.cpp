@@ -224,6 +224,9 @@ at::Tensor b200_gated_product(const at::Tensor& input, const at::Tensor& weight)
   return gated_product(readable(input, true), weight.contiguous(), nullptr);
 }
 
+// Whether forward-mode differentiation (make_dual, torch.func.jvp) is on its way through `t`.
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
+
 class GatedProduct : public torch::autograd::Function<GatedProduct> {
  public:
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& input, const at::Tensor& weight) {
@@ -237,6 +240,7 @@ class GatedProduct : public torch::autograd::Function<GatedProduct> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(grads[0]), "b200_gated_product: its gradients have no forward-mode derivative");
     TORCH_CHECK(!at::GradMode::is_enabled() || !grads[0].requires_grad(), "b200_gated_product is not differentiable twice");
     const at::Tensor &x = saved[0], &w = saved[1], grad = readable(grads[0], false);
     at::AutoDispatchBelowADInplaceOrView below;
@@ -258,6 +262,8 @@ void check_capture(const at::Tensor& t, const char* name) {
               " is part of a graph that lives outside this stream capture; let go of what was computed from it first");
 }
 at::Tensor b200_gated_product_autograd(const at::Tensor& input, const at::Tensor& weight) {
+  // (below autograd a tangent would be dropped, and the derivative be zero)
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(input) && !has_tangent(weight), "b200_gated_product has no forward-mode derivative");
   if (at::GradMode::is_enabled() && (input.requires_grad() || weight.requires_grad()) && input.is_cuda()) {
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) {
       check_capture(input, "input");

@@ -45,3 +45,50 @@ def test_a_gradient_with_a_tangent_is_refused(gated_linear):
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(y, x, torch.autograd.forward_ad.make_dual(d, torch.ones_like(d)))
+
+
+# ---- second order -------------------------------------------------------------------
+
+def _odd(x):
+    """The same rows, one value off a boundary of 16 bytes: the product reads a copy."""
+    room = torch.zeros(x.shape[0], x.shape[1] + 9, dtype=x.dtype, device=x.device)
+    return torch.cat((room[:, :1], x, room[:, 1:9]), dim=1)[:, 1:1 + x.shape[1]]
+
+
+@pytest.mark.parametrize("consumer", ["linear", "nonlinear"])
+@pytest.mark.parametrize("wanted", ["x", "w"])
+@pytest.mark.parametrize("copied", [False, True])
+def test_second_order_terms_are_refused(gated_linear, consumer, wanted, copied):
+    x, w, _ = _inputs()
+    if wanted == "x":
+        w.requires_grad_(False)      # (the gradient of x is one of x alone)
+    y = gated_linear(_odd(x) if copied else x, w)
+    loss = y.sum() if consumer == "linear" else y.float().pow(2).sum()
+    first, = torch.autograd.grad(loss, x if wanted == "x" else w, create_graph=True)
+    assert first.requires_grad
+    total = loss + first.float().pow(2).sum()          # (a penalty beside a loss that has a graph of its own)
+    with pytest.raises(RuntimeError, match="not differentiable twice"):
+        torch.autograd.grad(total, x, retain_graph=True)
+    if wanted == "w":
+        with pytest.raises(RuntimeError, match="not differentiable twice"):
+            torch.autograd.grad(total, w, retain_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable twice"):
+        total.backward()
+
+
+def test_the_incoming_gradient_is_not_differentiated_either(gated_linear):
+    x, w, d = _inputs()
+    d.requires_grad_(True)
+    dx, = torch.autograd.grad(gated_linear(x, w), x, d, create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable twice"):
+        torch.autograd.grad(dx.sum(), d)
+
+
+def test_a_graph_that_nobody_differentiates_changes_nothing(gated_linear):
+    x, w, d = _inputs()
+    want = torch.autograd.grad(gated_linear(x, w), (x, w), d)
+    got = torch.autograd.grad(gated_linear(x, w), (x, w), d, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    gated_linear(x, w).backward(d, create_graph=True)
+    assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
+    x.grad = w.grad = None

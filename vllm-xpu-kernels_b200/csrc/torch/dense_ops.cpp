@@ -2,6 +2,8 @@
 // b200_gated_linear_backward and, with gradients, b200_gated_product over the C ABI.  No counterpart in the reference, which multiplies dense layers by library calls.
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include "layer.h"
@@ -241,14 +243,27 @@ class GatedProduct : public torch::autograd::Function<GatedProduct> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(grads[0]), "b200_gated_product: its gradients have no forward-mode derivative");
-    TORCH_CHECK(!at::GradMode::is_enabled() || !grads[0].requires_grad(), "b200_gated_product is not differentiable twice");
     const at::Tensor &x = saved[0], &w = saved[1], grad = readable(grads[0], false);
     at::AutoDispatchBelowADInplaceOrView below;
     std::optional<at::Tensor> dx, dw;
     if (ctx->saved_data["x"].toBool()) dx = at::empty(x.sizes(), x.options());
     if (ctx->saved_data["w"].toBool()) dw = at::empty(w.sizes(), w.options());
     b200_gated_linear_backward(grad, saved[2], x, w, dx, dw);
+    if (at::GradMode::is_enabled()) refuse_twice(grads[0], {dx.has_value() ? &*dx : nullptr, dw.has_value() ? &*dw : nullptr});
     return {dx.has_value() ? *dx : at::Tensor(), dw.has_value() ? *dw : at::Tensor()};
+  }
+
+ private:
+  // Gradients that are part of a graph (create_graph) depend on both operands and on the incoming gradient, whether or not that one has a graph
+  // itself.  Their own derivative raises on the way to any of the three: without a node there it would be left out of a sum of
+  // losses in silence.
+  static void refuse_twice(const at::Tensor& grad, std::initializer_list<at::Tensor*> gradients) {
+    const auto self = torch::autograd::get_current_node();
+    torch::autograd::edge_list to = self->next_edges();
+    if (grad.requires_grad()) to.push_back(torch::autograd::impl::gradient_edge(grad));
+    const auto node = std::make_shared<torch::autograd::Error>("b200_gated_product is not differentiable twice", std::move(to));
+    for (at::Tensor* t : gradients)
+      if (t != nullptr) torch::autograd::set_history(*t, node);
   }
 };
 // A leaf's gradient is waited for on the stream that its first live graph was made on.  Where that is another one than a capturing one, the

@@ -92,3 +92,23 @@ def test_a_graph_that_nobody_differentiates_changes_nothing(gated_linear):
     gated_linear(x, w).backward(d, create_graph=True)
     assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
     x.grad = w.grad = None
+
+
+# ---- which gradients ----------------------------------------------------------------
+
+def test_only_the_gradients_that_are_asked_for(gated_linear):
+    """... are computed: a call takes no memory for the other one."""
+    for rows, hidden, inter, operand in ((8, 2048, 1024, 0), (4096, 2048, 8, 1)):
+        x, w, d = _inputs(rows, hidden, inter)
+        both = torch.autograd.grad(gated_linear(x, w), (x, w), d)
+        y = gated_linear(x, w)
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got, = torch.autograd.grad(y, (x, w)[operand], d)
+        grown = torch.cuda.max_memory_allocated() - before
+        other = (w, x)[operand]
+        assert torch.equal(got, both[operand])
+        assert grown < other.numel() * other.element_size(), grown
+        y = gated_linear(x, w)
+        y.backward(d, inputs=[(x, w)[operand]])
+        assert torch.equal((x, w)[operand].grad, both[operand]) and other.grad is None

@@ -236,8 +236,6 @@ class GatedProduct : public torch::autograd::Function<GatedProduct> {
     const at::Tensor x = readable(input, true), w = weight.contiguous();
     at::Tensor pre, out = gated_product(x, w, &pre);
     ctx->save_for_backward({x.is_same(input) ? input : x, w.is_same(weight) ? weight : w, pre});
-    ctx->saved_data["x"] = input.requires_grad();
-    ctx->saved_data["w"] = weight.requires_grad();
     return out;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
@@ -246,8 +244,9 @@ class GatedProduct : public torch::autograd::Function<GatedProduct> {
     const at::Tensor &x = saved[0], &w = saved[1], grad = readable(grads[0], false);
     at::AutoDispatchBelowADInplaceOrView below;
     std::optional<at::Tensor> dx, dw;
-    if (ctx->saved_data["x"].toBool()) dx = at::empty(x.sizes(), x.options());
-    if (ctx->saved_data["w"].toBool()) dw = at::empty(w.sizes(), w.options());
+    // (those that this pass wants: either is a product of its own, half of the work)
+    if (ctx->needs_input_grad(0)) dx = at::empty(x.sizes(), x.options());
+    if (ctx->needs_input_grad(1)) dw = at::empty(w.sizes(), w.options());
     b200_gated_linear_backward(grad, saved[2], x, w, dx, dw);
     if (at::GradMode::is_enabled()) refuse_twice(grads[0], {dx.has_value() ? &*dx : nullptr, dw.has_value() ? &*dw : nullptr});
     return {dx.has_value() ? *dx : at::Tensor(), dw.has_value() ? *dw : at::Tensor()};

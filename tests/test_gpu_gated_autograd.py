@@ -1,5 +1,7 @@
 """GPU: what autograd may ask of the gated product beyond a first gradient: derivatives that it does not have are refused, not dropped, and
 gradients that nobody wants are not computed."""
+import gc
+
 import pytest
 import torch
 
@@ -112,3 +114,42 @@ def test_only_the_gradients_that_are_asked_for(gated_linear):
         y = gated_linear(x, w)
         y.backward(d, inputs=[(x, w)[operand]])
         assert torch.equal((x, w)[operand].grad, both[operand]) and other.grad is None
+
+
+# ---- capture ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("view", [lambda w: w.view(2, 24, 64).view(48, 64), lambda w: w * 1, lambda w: w.t().t()[:40]])
+def test_operands_made_of_a_leaf_that_lives_outside_the_capture_are_refused(gated_linear, view):
+    x, w, d = _inputs()
+    x.requires_grad_(False)
+    alive = gated_linear(x, w)
+    for operands in ((lambda: (x, view(w))), (lambda: (view(w), torch.ones(16, 64, dtype=B16, device=DEV)))):
+        with pytest.raises(RuntimeError, match="outside this stream capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                gated_linear(*operands())
+    del alive
+    gc.collect()          # (an exception's frames hold on to what they had)
+    want, = torch.autograd.grad(gated_linear(x, view(w)), w, d[:, :view(w).shape[0] // 2])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got, = torch.autograd.grad(gated_linear(x, view(w)), w, d[:, :view(w).shape[0] // 2])
+    g.replay()
+    assert torch.equal(got, want)
+
+
+def test_a_leaf_of_another_stream_of_the_same_capture_is_taken(gated_linear):
+    x, w, d = _inputs()
+    want = torch.autograd.grad(gated_linear(x, w), (x, w), d)
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            view = w * 1                          # (w's accumulator belongs to the side stream)
+            keep = w.view(-1)
+        main.wait_stream(side)
+        y = gated_linear(x, view)
+        got = torch.autograd.grad(y, (x, w), d)
+        main.wait_stream(side)
+    g.replay()
+    assert keep.requires_grad and all(torch.equal(a, b) for a, b in zip(got, want))

@@ -1,10 +1,13 @@
 // The dense layers beside the routed experts: torch.ops._xpu_C.b200_int8_linear, b200_gated_linear,
 // b200_gated_linear_backward and, with gradients, b200_gated_product over the C ABI.  No counterpart in the reference, which multiplies dense layers by library calls.
-#include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/variable.h>
+
+#include <unordered_set>
 
 #include "layer.h"
 
@@ -265,23 +268,45 @@ class GatedProduct : public torch::autograd::Function<GatedProduct> {
       if (t != nullptr) torch::autograd::set_history(*t, node);
   }
 };
+bool is_capturing(const c10::Stream& stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  // (the legacy stream cannot be asked while another one captures, so it does not)
+  if (cudaStreamIsCapturing(c10::cuda::CUDAStream(stream).stream(), &status) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  return status != cudaStreamCaptureStatusNone;
+}
 // A leaf's gradient is waited for on the stream that its first live graph was made on.  Where that is another one than a capturing one, the
-// captured backward pass cannot wait for it, and the error ends the process: refused here, while it is one call's.
-void check_capture(const at::Tensor& t, const char* name) {
-  if (!t.requires_grad() || !t.is_leaf()) return;
-  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (accumulator == nullptr) return;
-  const auto stream = accumulator->stream();
-  TORCH_CHECK(!stream.has_value() || *stream == at::cuda::getCurrentCUDAStream(t.get_device()).unwrap(), "b200_gated_product: ", name,
-              " is part of a graph that lives outside this stream capture; let go of what was computed from it first");
+// captured backward pass cannot wait for it, and the error ends the process: refused here, while it is one call's.  That goes for leaves that `t` is
+// made of (a view or a copy of a parameter, the layers before) as for `t` itself.
+void check_capture(const at::Tensor& t, const char* name, const c10::Stream& capturing) {
+  if (!t.requires_grad()) return;
+  std::vector<std::shared_ptr<torch::autograd::Node>> to_do;
+  std::unordered_set<torch::autograd::Node*> seen;
+  auto add = [&](std::shared_ptr<torch::autograd::Node> node) {
+    if (node != nullptr && seen.insert(node.get()).second) to_do.push_back(std::move(node));
+  };
+  add(t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn());
+  while (!to_do.empty()) {
+    const auto node = std::move(to_do.back());
+    to_do.pop_back();
+    const auto edges = node->next_edges();
+    for (const auto& edge : edges) add(edge.function);
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get()) == nullptr) continue;
+    const auto stream = node->stream();
+    TORCH_CHECK(!stream.has_value() || stream->device() != capturing.device() || *stream == capturing || is_capturing(*stream), "b200_gated_product: ", name,
+                " is part of a graph that lives outside this stream capture; let go of what was computed from it first");
+  }
 }
 at::Tensor b200_gated_product_autograd(const at::Tensor& input, const at::Tensor& weight) {
   // (below autograd a tangent would be dropped, and the derivative be zero)
   TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(input) && !has_tangent(weight), "b200_gated_product has no forward-mode derivative");
   if (at::GradMode::is_enabled() && (input.requires_grad() || weight.requires_grad()) && input.is_cuda()) {
-    if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) {
-      check_capture(input, "input");
-      check_capture(weight, "weight");
+    const c10::Stream stream = at::cuda::getCurrentCUDAStream(input.get_device()).unwrap();
+    if (is_capturing(stream)) {
+      check_capture(input, "input", stream);
+      check_capture(weight, "weight", stream);
     }
     return GatedProduct::apply(input, weight);
   }

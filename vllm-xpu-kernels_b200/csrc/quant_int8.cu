@@ -180,10 +180,10 @@ template <typename T, bool kGated>
 int launch(const QuantInt8Params& p, cudaStream_t st) {
   constexpr int N = 16 / sizeof(T);
   const int nvec = p.hidden / N;
-  const bool whole = p.hidden % N == 0 && p.in_stride % N == 0 && p.q_stride % N == 0 && ((uintptr_t)p.in & 15) == 0 &&
+  const bool whole = nvec > 0 && p.hidden % N == 0 && p.in_stride % N == 0 && p.q_stride % N == 0 && ((uintptr_t)p.in & 15) == 0 &&
                      ((uintptr_t)p.q & (N - 1)) == 0 && nvec <= 4096;
   if (!whole) {
-    const int threads = p.hidden >= 1024 ? 1024 : (p.hidden + 31) / 32 * 32;
+    const int threads = p.hidden >= 1024 ? 1024 : std::max(32, (p.hidden + 31) / 32 * 32);
     B200_LAUNCHED("quant_int8_any_kernel", launch_pdl(p.rows <= kEarlyLaunchRows, quant_int8_any_kernel<T, kGated>, dim3((unsigned)p.rows),
                                                       dim3(threads), 0, st, p));
     return B200MOE_OK;
@@ -203,8 +203,8 @@ extern "C" int b200moe_quant_int8_rows(const void* in, b200moe_dtype dtype, int6
                                        int num_segments, b200moe_stream stream) {
   B200_CHECK_ARG(rows >= 0 && rows <= 0x7fffffff && hidden >= 0, "quant_int8_rows: negative or too large size");
   B200_CHECK_ARG(rows_per_segment == nullptr || num_segments >= 0, "quant_int8_rows: negative number of segments");
-  if (rows == 0 || hidden == 0) return B200MOE_OK;
-  B200_CHECK_ARG(in && q && scales, "quant_int8_rows: null pointer");
+  if (rows == 0) return B200MOE_OK;
+  B200_CHECK_ARG(((in && q) || hidden == 0) && scales, "quant_int8_rows: null pointer");   // (rows without values have a scale too)
   const QuantInt8Params p = {in, q, scales, rows_per_segment, rows, in_stride, q_stride, hidden, num_segments};
   int rc = B200MOE_OK;
   B200_DISPATCH_FLOAT(dtype, "quant_int8_rows",

@@ -356,7 +356,7 @@ void quant_int8_rows(const at::Tensor& input, const at::Tensor& out, const at::T
   const Pieces s = {(const char*)scales.data_ptr(), scales.numel() ? 1 : 0, 0, scales.numel() * 4};
   const Pieces q = pieces_of_rows(out, q_stride), in = pieces_of_rows(input, in_stride);
   TORCH_CHECK(!overlap(q, in) && !overlap(s, in) && !overlap(s, q), op, ": tensors must not overlap");
-  if (rows == 0 || hidden == 0) return;
+  if (rows == 0) return;
   const c10::cuda::CUDAGuard guard(input.device());
   check_status(b200moe_quant_int8_rows(input.data_ptr(), dtype, in_stride, (int8_t*)out.data_ptr(), q_stride, scales.data_ptr<float>(),
                                        rows, (int)hidden, gated, nullptr, 0, current_stream()));

@@ -261,6 +261,7 @@ class GatedProduct : public torch::autograd::Function<GatedProduct> {
   // losses in silence.
   static void refuse_twice(const at::Tensor& grad, std::initializer_list<at::Tensor*> gradients) {
     const auto self = torch::autograd::get_current_node();
+    TORCH_CHECK(self != nullptr, "b200_gated_product is not differentiable twice");   // (called by no engine: no edges to lead on)
     torch::autograd::edge_list to = self->next_edges();
     if (grad.requires_grad()) to.push_back(torch::autograd::impl::gradient_edge(grad));
     const auto node = std::make_shared<torch::autograd::Error>("b200_gated_product is not differentiable twice", std::move(to));

@@ -394,7 +394,8 @@ typedef struct {
   b200moe_epilogue epilogue;
   float act_alpha, act_limit; /* SwigluOAI parameters                             */
   float clamp_limit;      /* >0: gate=min(gate,L), up=clamp(up,-L,L) before the
-                             gated epilogue (only with a gated epilogue)          */
+                             gated epilogue (only with a gated epilogue); with int8
+                             weights a NaN stays one                              */
   int32_t* status;        /* int the device can write (device memory or mapped host
                              memory): set to 1 if a bounded wait gave up; may be
                              NULL                                                 */
@@ -461,6 +462,7 @@ typedef struct {
   void* d;                /* [rows, n] d_dtype, d_stride from row to row             */
   int64_t rows, x_stride, d_stride;
   int n, k;               /* k: a multiple of 16, at most B200MOE_INT8_MAX_K         */
+                          /* n: at most 2^31 - 513                                   */
   b200moe_dtype x_dtype;  /* I8, F32, F16 or BF16                                    */
   b200moe_dtype d_dtype;  /* F32, F16 or BF16                                        */
   b200moe_dtype bias_dtype; /* F16 or BF16                                           */
@@ -475,7 +477,8 @@ int b200moe_int8_linear(const b200moe_int8_linear_args* args, b200moe_stream str
  *   [g | u] = x w^T,  out = silu(g) * u                                w [2 inter, hidden], gate rows first
  *   dg = grad u s (1 + g (1 - s)),  du = grad g s,  s = sigmoid(g)
  *   grad_x = [dg | du] w,  grad_w = [dg | du]^T x
- * Sums are fp32; g and u stay fp32 until the activation, and in `pre`; dg and du are rounded to dtype.  The forward pass
+ * Sums are fp32; g and u stay fp32 until the activation, and in `pre`; dg and du are rounded to dtype (F16: beyond 65504 they
+ * are infinite, and what they go into is not finite).  The forward pass
  * reads x, w and writes out and, unless it is NULL, pre; the backward pass reads grad, pre, x, w and writes those of grad_x
  * and grad_w that are not NULL.  All matrices but w, pre and grad_w may have rows that are further apart than they are
  * long (strides in elements).  Zero-initialise the struct. */

@@ -153,3 +153,26 @@ def test_a_leaf_of_another_stream_of_the_same_capture_is_taken(gated_linear):
         main.wait_stream(side)
     g.replay()
     assert keep.requires_grad and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- range --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [6, 300])
+def test_float16_gradients_that_overflow_between_the_kernels_show(gated_linear, rows):
+    """dg and du are float16: the row and the weight row of one beyond 65504 have gradients that are not finite, and no others.  Every weight row is
+    a unit vector, so that g and u are values of x."""
+    gen = torch.Generator().manual_seed(rows)
+    x, d = torch.randn(rows, 64, generator=gen), torch.randn(rows, 24, generator=gen)
+    x[1, 3], x[1, 24 + 3], d[1, 3] = 8.0, 100.0, 1000.0         # dg = 1000 * 100 * 1.002..., du = 1000 * 8 * 0.9996...
+    x[4, 5], x[4, 24 + 5], d[4, 5] = 100.0, 0.0, 1000.0         # dg = 0, du = 1000 * 100
+    x, d, w = x.half().to(DEV).requires_grad_(True), d.half().to(DEV), torch.eye(64)[:48].half().to(DEV).requires_grad_(True)
+    dx, dw = torch.autograd.grad(gated_linear(x, w), (x, w), d)
+    broken_rows, broken_features = torch.zeros(rows, dtype=torch.bool, device=DEV), torch.zeros(48, dtype=torch.bool, device=DEV)
+    broken_rows[1] = broken_rows[4] = broken_features[3] = broken_features[24 + 5] = True
+    g, u = (x.detach().double() @ w.detach().double().t()).chunk(2, -1)
+    both = torch.cat((d.double() * u * torch.sigmoid(g) * (1 + g * (1 - torch.sigmoid(g))), d.double() * g * torch.sigmoid(g)), -1)
+    # (dw[24 + 3, 24 + 3] is 8000 * 100 and more: that one value is beyond float16 itself, without any help)
+    for got, exact, broken in ((dx, both @ w.detach().double(), broken_rows), (dw, both.t() @ x.detach().double(), broken_features)):
+        assert not torch.isfinite(got[broken]).any()
+        assert torch.isfinite(got[~broken][exact[~broken].abs() < 65000]).all()
+        assert (exact[~broken].abs() >= 65000).sum() <= 1

@@ -7,7 +7,9 @@ namespace {
 
 // Gradients of the two products from the gradient of silu(g) * u, in the operands' type for the products that follow:
 //   dg = d u s (1 + g (1 - s)),  du = d g s,  s = 1 / (1 + e^-g);  both = [dg | du] a row
-// g and u come in 32 bits, as the forward pass had them; rounding dg and du to 16 bits is what the tensor cores ask for.
+// g and u come in 32 bits, as the forward pass had them; rounding dg and du to 16 bits is what the tensor cores ask for.  It takes the
+// gradients' error from 1.7e-3 to 2.4e-3 in bfloat16 and from 2.1e-4 to 2.9e-4 in float16 (the first is the results' own 16 bits); in float16 a dg or du beyond
+// 65504 is an infinity, and the rows and columns of the gradients that it goes into are not finite.
 // A stream of 14 bytes for each value of d; N values a thread.
 template <typename T, int N>
 __global__ void __launch_bounds__(256)

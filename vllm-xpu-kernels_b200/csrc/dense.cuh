@@ -46,7 +46,8 @@ int dense_tc(const DenseJob& j, cudaStream_t st);        // dense_tc.cu
 // Which kernel takes a call; that for a few rows / that for many, us.  By expert: with two rows of an expert, on average, or fewer the first one; with
 // up to ten where the weights of all are few, so that what a call costs besides counts.  Layer calls: 128 experts of 2048 x 768, 1 row 85 / 81,
 // 4 rows 119 / 115, 10 rows 135 / 119; 8 of 4096 x 14336, 1 row 182 / 188, 3 rows 235 / 230, 10 rows 278 / 238; 8 of 2048 x 1408 (46 and 23 MB),
-// 4 rows 25 / 32, 10 rows 27 / 30, 16 rows 32 / 29.
+// 4 rows 25 / 32, 10 rows 27 / 30, 16 rows 32 / 29.  (One row an expert on average goes either way: what the first loses with many small experts, 4 us of 81,
+// is less than it wins with a few large ones, 6 of 188, and the rule does not tell them apart.)
 // One set: up to eight rows, and up to sixteen where the SMs have few tiles of weight rows each: then the tokens take as much of L2's
 // time as the weights.  16 x 4096 x 4096 5.9 / 7.5, 16 x 4096 x 14336 14.3 / 14.0, 12 x 7168 x 2048 gated 13.4 / 13.6, 16 x 8192 x 4096 10.2 / 9.9,
 // 9 x 14336 x 4096 15.8 / 13.6.

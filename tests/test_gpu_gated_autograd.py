@@ -155,6 +155,23 @@ def test_a_leaf_of_another_stream_of_the_same_capture_is_taken(gated_linear):
     assert keep.requires_grad and all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("made", [lambda w: w, lambda w: w * 1])
+def test_a_leaf_of_a_graph_on_another_stream_outside_the_capture_is_taken(gated_linear, made):
+    """(That stream joins the capture.  Modules whose hooks keep the leaves' nodes for good are set up so.)"""
+    x, w, d = _inputs()
+    want = torch.autograd.grad(gated_linear(x, w), (x, w), d)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = gated_linear(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = torch.autograd.grad(gated_linear(x, made(w)), (x, w), d)
+    g.replay()
+    assert alive.requires_grad and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---- range --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows", [6, 300])

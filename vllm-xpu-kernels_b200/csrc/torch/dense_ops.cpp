@@ -269,19 +269,19 @@ class GatedProduct : public torch::autograd::Function<GatedProduct> {
       if (t != nullptr) torch::autograd::set_history(*t, node);
   }
 };
-bool is_capturing(const c10::Stream& stream) {
+bool is_capturing(cudaStream_t stream) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-  // (the legacy stream cannot be asked while another one captures, so it does not)
-  if (cudaStreamIsCapturing(c10::cuda::CUDAStream(stream).stream(), &status) != cudaSuccess) {
+  // (the default stream cannot be asked while another one captures, and does not itself)
+  if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) {
     (void)cudaGetLastError();
     return false;
   }
   return status != cudaStreamCaptureStatusNone;
 }
-// A leaf's gradient is waited for on the stream that its first live graph was made on.  Where that is another one than a capturing one, the
-// captured backward pass cannot wait for it, and the error ends the process: refused here, while it is one call's.  That goes for leaves that `t` is
-// made of (a view or a copy of a parameter, the layers before) as for `t` itself.
-void check_capture(const at::Tensor& t, const char* name, const c10::Stream& capturing) {
+// A leaf's gradient is waited for on the stream that its first live graph was made on.  Another stream than the capturing one joins the capture by
+// that; the default stream cannot, and the error ends the process in the captured backward pass: refused here, while it is one call's.  That goes
+// for leaves that `t` is made of (a view or a copy of a parameter, the layers before) as for `t` itself.
+void check_capture(const at::Tensor& t, const char* name) {
   if (!t.requires_grad()) return;
   std::vector<std::shared_ptr<torch::autograd::Node>> to_do;
   std::unordered_set<torch::autograd::Node*> seen;
@@ -296,18 +296,17 @@ void check_capture(const at::Tensor& t, const char* name, const c10::Stream& cap
     for (const auto& edge : edges) add(edge.function);
     if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get()) == nullptr) continue;
     const auto stream = node->stream();
-    TORCH_CHECK(!stream.has_value() || stream->device() != capturing.device() || *stream == capturing || is_capturing(*stream), "b200_gated_product: ", name,
-                " is part of a graph that lives outside this stream capture; let go of what was computed from it first");
+    TORCH_CHECK(!stream.has_value() || c10::cuda::CUDAStream(*stream).stream() != nullptr, "b200_gated_product: ", name,
+                " is part of a graph that lives outside this stream capture, on the default stream; let go of what was computed from it first");
   }
 }
 at::Tensor b200_gated_product_autograd(const at::Tensor& input, const at::Tensor& weight) {
   // (below autograd a tangent would be dropped, and the derivative be zero)
   TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(input) && !has_tangent(weight), "b200_gated_product has no forward-mode derivative");
   if (at::GradMode::is_enabled() && (input.requires_grad() || weight.requires_grad()) && input.is_cuda()) {
-    const c10::Stream stream = at::cuda::getCurrentCUDAStream(input.get_device()).unwrap();
-    if (is_capturing(stream)) {
-      check_capture(input, "input", stream);
-      check_capture(weight, "weight", stream);
+    if (is_capturing(at::cuda::getCurrentCUDAStream(input.get_device()))) {
+      check_capture(input, "input");
+      check_capture(weight, "weight");
     }
     return GatedProduct::apply(input, weight);
   }

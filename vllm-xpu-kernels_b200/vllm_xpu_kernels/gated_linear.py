@@ -20,7 +20,7 @@ def gated_linear(input, weight):
     are asked for, forward-mode ones (``make_dual``, ``torch.func.jvp``) at the call.  Between the kernels the gradients of the two products
     are of the operands' type: in float16 what is beyond 65504 becomes an infinity, which the results show, and what is below 2^-25 zero.
     Weights that are not contiguous, and rows that are not evenly spaced on 16-byte boundaries, are copied first.  Under stream
-    capture an operand that is, or is made of, a leaf that a live graph from outside the capture uses is refused: let go of
-    what was computed from it first."""
+    capture an operand that is, or is made of, a leaf that a live graph from outside the capture uses on the default stream
+    is refused: let go of what was computed from it first."""
     _require_native()
     return torch.ops._xpu_C.b200_gated_product(input, weight)
